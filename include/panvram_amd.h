@@ -359,6 +359,66 @@ int32_t pv_streams_concurrent(void* a, void* b, int32_t* concurrent, char* err, 
 int32_t pv_fasta_layout_hip(const uint8_t* bases, uint64_t b0, uint64_t nb, const int64_t* rec, int32_t nrec, const uint8_t* hdrs,
                             uint64_t f0, uint64_t nf, uint8_t* out, void* stream, char* err, size_t errcap);
 
+/* ---- Operators of a recurrent language model over windows (panvram_amd/ops). No reference counterpart. ----
+ * All pointers are device memory unless said otherwise; tensors' last dimension has neighbouring elements, other strides are
+ * given in elements. Launches go to `stream` (hipStream_t), nothing is waited for or allocated, and a call may be captured
+ * into a graph. `work` is scratch of at least the bytes that the operator's _work_bytes gives for the same sizes, 16-byte
+ * aligned, and need not be cleared. PV_EARG for arguments outside what is described. */
+
+/* element types of a tensor, and 8-bit formats */
+enum pv_dtype { PV_F32 = 0, PV_BF16 = 1, PV_F16 = 2 };
+enum pv_format8 { PV_E4M3 = 0, PV_INT8 = 1 };
+
+/* h[b, t, d] = (1 - z) h[b, t-1, d] + z value[b, t, d], z = sigmoid(gate[b, t, d]), T >= 1. gate, value: [B, T, D] of `dtype`
+ * with strides (gate_b, gate_t), (value_b, value_t). state: f32[B, D] before step 0, or NULL: zero. reset: u8[B, T], or NULL;
+ * where not 0, h[b, t-1] is dropped. out: [B, T, D] of `dtype`; last: f32[B, D] = h[b, T-1]. carry: NULL, or
+ * f32[B, pv_gated_scan_chunks(T), D] that the backward pass takes. */
+int64_t pv_gated_scan_chunks(int64_t T);
+uint64_t pv_gated_scan_work_bytes(int64_t B, int64_t T, int64_t D);
+int32_t pv_gated_scan_hip(const void* gate, const void* value, const float* state, const uint8_t* reset, int64_t B, int64_t T, int64_t D, int64_t gate_b,
+                          int64_t gate_t, int64_t value_b, int64_t value_t, int32_t dtype, void* out, float* last, float* carry, void* work,
+                          uint64_t work_bytes, void* stream, char* err, size_t errcap);
+/* Its gradients from d_out ([B, T, D] of `dtype`, strides (d_out_b, d_out_t)) and d_last (f32[B, D], or NULL: zero): d_gate,
+ * d_value ([B, T, D] of `dtype`) and d_state (f32[B, D], or NULL). carry: as the forward call left it. */
+int32_t pv_gated_scan_backward_hip(const void* gate, const void* value, const float* carry, const uint8_t* reset, int64_t B, int64_t T, int64_t D,
+                                   int64_t gate_b, int64_t gate_t, int64_t value_b, int64_t value_t, const void* d_out, int64_t d_out_b, int64_t d_out_t,
+                                   const float* d_last, int32_t dtype, void* d_gate, void* d_value, float* d_state, void* work, uint64_t work_bytes,
+                                   void* stream, char* err, size_t errcap);
+
+/* s = x + residual, rounded to `dtype` (stream_out [N, D]; residual NULL: s = x, stream_out is not written);
+ * y[n, :] = s r weight, r = 1 / sqrt(mean(s^2) + eps). x, residual: [N, D] of `dtype` with the given row strides; weight:
+ * f32[D]; y: [N, D] of `dtype`; rstd: NULL, or f32[N] = r. */
+int32_t pv_add_rms_norm_hip(const void* x, const void* residual, const float* weight, int64_t N, int64_t D, int64_t x_row, int64_t residual_row, float eps,
+                            int32_t dtype, void* y, void* stream_out, float* rstd, void* stream, char* err, size_t errcap);
+/* The same with y in 8 bits: scale[n] = max |y[n, :]| / (448 or 127), q = y / scale to the nearest value (ties to even); a
+ * row of zeros has scale 0, a row with a NaN or an infinity scale NaN. format: PV_E4M3 or PV_INT8. */
+int32_t pv_add_rms_norm_8bit_hip(const void* x, const void* residual, const float* weight, int64_t N, int64_t D, int64_t x_row, int64_t residual_row, float eps,
+                                 int32_t dtype, int32_t format, void* q, float* scale, void* stream_out, void* stream, char* err, size_t errcap);
+/* The gradients from d_y and d_stream (NULL: zero), both [N, D] of `dtype`, with s ([N, D], row stride s_row) and rstd of the
+ * forward call: d (of x and of residual alike, [N, D] of `dtype`) and d_weight (f32[D]). */
+uint64_t pv_add_rms_norm_work_bytes(int64_t N, int64_t D);
+int32_t pv_add_rms_norm_backward_hip(const void* s, const float* rstd, const float* weight, int64_t N, int64_t D, int64_t s_row, const void* d_y,
+                                     const void* d_stream, int32_t dtype, void* d, float* d_weight, void* work, uint64_t work_bytes, void* stream, char* err,
+                                     size_t errcap);
+
+/* Cross-entropy of the next token under softmax(hidden weight^T). hidden: [B, T, D] of `dtype`, strides (hidden_b, hidden_t);
+ * weight: [V, D] of weight_dtype (`dtype` or PV_F32), V <= 16; tokens: [B, T], row stride tokens_b, u8 or i64 (token_bytes 1 or
+ * 8). Place (b, t) counts if tokens[b, t+1] is in [0, V) and not `ignore` (t = T-1 never does). each: NULL, or f32[B, T], the
+ * places' losses (0 where they do not count); loss: NULL, or f32[1], their mean over the places that count (0 for none).
+ * d_hidden ([B, T, D] of `dtype`) and d_weight ([V, D] of weight_dtype), both or neither: the gradients of scale * mean (scale:
+ * f32[1], NULL: 1), or with factor (f32[B, T]) of sum factor * each. */
+uint64_t pv_next_base_loss_work_bytes(int64_t B, int64_t T, int64_t D, int32_t V, int32_t gradients);
+int32_t pv_next_base_loss_hip(const void* hidden, const void* weight, const void* tokens, int64_t B, int64_t T, int64_t D, int32_t V, int64_t hidden_b,
+                              int64_t hidden_t, int64_t tokens_b, int64_t ignore, int32_t dtype, int32_t weight_dtype, int32_t token_bytes, const float* scale,
+                              const float* factor, float* each, float* loss, void* d_hidden, void* d_weight, void* work, uint64_t work_bytes, void* stream,
+                              char* err, size_t errcap);
+
+/* norm (f32[1]) = sqrt(sum over `count` tensors of their squares). grads, sizes (elements), dtypes, out: host arrays. out: NULL,
+ * or for each tensor where grads[i] * min(1, max_norm / (norm + 1e-6)) goes (grads[i] itself, or memory apart from all). */
+uint64_t pv_gradient_norm_work_bytes(const int64_t* sizes, int32_t count);
+int32_t pv_gradient_norm_hip(const void* const* grads, void* const* out, const int64_t* sizes, const int32_t* dtypes, int32_t count, float max_norm, float* norm,
+                             void* work, uint64_t work_bytes, void* stream, char* err, size_t errcap);
+
 #ifdef __cplusplus
 }
 #endif

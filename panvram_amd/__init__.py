@@ -9,13 +9,16 @@ call returns a tensor on that device:
     gen = torch.Generator(device="cuda").manual_seed(0)
     batch = cohort.sample(1024, 8192, generator=gen)          # 1024 random windows of 8192 bases, uint8
     piece = cohort.fetch("hap001", "chr1", 10_000, 5_000)     # bases [10000, 15000) of one contig
+
+`ops` has what a sequence model trained on such windows needs beside torch: a gated recurrence over long sequences, the
+residual stream's norm, the loss over the bases, and the clipping of gradients.
 """
 import torch  # noqa: F401  (the HIP runtime that libpanvram_amd.so binds to, loaded as torch loads it)
 
-from . import _native
+from . import _native, ops
 from .cohort import DATASETS, Cohort
 
 FormatError = _native.FormatError
 with_cuda = True            # the package is GPU-only: the HIP library is required (ImportError at first use otherwise)
 __version__ = "0.1.0"
-__all__ = ["Cohort", "DATASETS", "FormatError", "with_cuda"]
+__all__ = ["Cohort", "DATASETS", "FormatError", "ops", "with_cuda"]

@@ -19,9 +19,12 @@ PV_OK, PV_EFORMAT, PV_EARG, PV_EHIP, PV_ENOMEM = 0, 1, 2, 3, 4
  ARR_GRP_OFF, ARR_GRP_ST, ARR_RUN0G, ARR_BLEN, ARR_BCODE, ARR_EXC_B, ARR_EXC_ST, ARR_COUNT) = range(26)
 FORM_PACKED_REF, FORM_COMPACT_BLOCKS = 1, 2
 WAIT_EVENT, WAIT_COUNTER = 0, 1
+F32, BF16, F16 = 0, 1, 2
+E4M3, INT8 = 0, 1
 
 vp, i32, i64, u32, u64, cp, sz = (ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_uint32, ctypes.c_uint64,
                                   ctypes.c_char_p, ctypes.c_size_t)
+f32 = ctypes.c_float
 
 
 class FormatError(ValueError):
@@ -98,6 +101,18 @@ SIGNATURES = {
     "pv_windows_hip_noalloc": (i32, [ctypes.POINTER(DevCohort), vp, vp, i64, i64, vp, i32, i32, vp, vp, vp, cp, sz]),
     "pv_selftest_bytes": (i32, []),
     "pv_fetch_hip": (i32, [ctypes.POINTER(DevCohort), i64, i64, i64, i32, i32, vp, vp, vp, u64, vp, cp, sz]),
+    "pv_gated_scan_chunks": (i64, [i64]),
+    "pv_gated_scan_work_bytes": (u64, [i64, i64, i64]),
+    "pv_gated_scan_hip": (i32, [vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, i32, vp, vp, vp, vp, u64, vp, cp, sz]),
+    "pv_gated_scan_backward_hip": (i32, [vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, vp, i64, i64, vp, i32, vp, vp, vp, vp, u64, vp, cp, sz]),
+    "pv_add_rms_norm_hip": (i32, [vp, vp, vp, i64, i64, i64, i64, f32, i32, vp, vp, vp, vp, cp, sz]),
+    "pv_add_rms_norm_8bit_hip": (i32, [vp, vp, vp, i64, i64, i64, i64, f32, i32, i32, vp, vp, vp, vp, cp, sz]),
+    "pv_add_rms_norm_work_bytes": (u64, [i64, i64]),
+    "pv_add_rms_norm_backward_hip": (i32, [vp, vp, vp, i64, i64, i64, vp, vp, i32, vp, vp, vp, u64, vp, cp, sz]),
+    "pv_next_base_loss_work_bytes": (u64, [i64, i64, i64, i32, i32]),
+    "pv_next_base_loss_hip": (i32, [vp, vp, vp, i64, i64, i64, i32, i64, i64, i64, i64, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, u64, vp, cp, sz]),
+    "pv_gradient_norm_work_bytes": (u64, [vp, i32]),
+    "pv_gradient_norm_hip": (i32, [vp, vp, vp, vp, i32, f32, vp, vp, u64, vp, cp, sz]),
 }
 
 _lib = None

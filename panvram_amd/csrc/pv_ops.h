@@ -1,0 +1,60 @@
+// What the operators' kernels (pv_scan.hip, pv_norm.hip, pv_loss.hip, pv_clip.hip) share: element types, wide loads and
+// stores, wave sums, and the checks of a C entry.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <stdio.h>
+#include "../../include/panvram_amd.h"
+
+namespace pvo {
+
+constexpr int WAVE = 64;
+
+// What the kernels hold one element as: PV_F32, PV_BF16, PV_F16. Conversions from float round to nearest even.
+using bf16 = __bf16;
+using f16 = _Float16;
+
+template <int BYTES> struct raw_of;
+template <> struct raw_of<1> { using type = uint8_t; };
+template <> struct raw_of<2> { using type = uint16_t; };
+template <> struct raw_of<4> { using type = uint32_t; };
+template <> struct raw_of<8> { using type = uint2; };
+template <> struct raw_of<16> { using type = uint4; };
+
+// N elements moved by one load or store of N * sizeof(T) bytes, which the address has to be a multiple of
+template <typename T, int N> struct pack {
+    using raw = typename raw_of<int(sizeof(T)) * N>::type;
+    union { raw bits; T v[N]; };
+    __device__ static pack load(const T* p) { pack r; r.bits = *reinterpret_cast<const raw*>(p); return r; }
+    __device__ void store(T* p) const { *reinterpret_cast<raw*>(p) = bits; }
+};
+
+inline bool aligned(const void* p, uint64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+__device__ inline float wave_sum(float x) {
+#pragma unroll
+    for (int d = WAVE / 2; d; d >>= 1) x += __shfl_xor(x, d, WAVE);
+    return x;
+}
+
+inline int32_t fail(int32_t code, char* err, size_t cap, const char* m) {
+    if (err && cap) snprintf(err, cap, "%s", m);
+    return code;
+}
+
+// The last launch's error as a status code
+inline int32_t launched(char* err, size_t cap) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? PV_OK : fail(PV_EHIP, err, cap, hipGetErrorString(e));
+}
+
+inline int element_bytes(int32_t dtype) { return dtype == PV_F32 ? 4 : dtype == PV_BF16 || dtype == PV_F16 ? 2 : 0; }
+
+// f.template operator()<T>() of the element type `dtype` names (checked before)
+template <typename F> int32_t with_type(int32_t dtype, F&& f) {
+    if (dtype == PV_F32) return f(float{});
+    if (dtype == PV_BF16) return f(bf16{});
+    return f(f16{});
+}
+
+}  // namespace pvo
