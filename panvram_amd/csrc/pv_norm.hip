@@ -4,114 +4,322 @@
 //   r = 1 / sqrt(mean(s^2) + eps),  y = s r weight
 //   8 bits: scale = max |y| / the largest value of the format, per row; q = round(y / scale)
 //   backward, with u = s r and g = d_y weight:  d = d_stream + r (g - u mean(g u));  d_weight = sum over rows of d_y u
-// One wave per row; sums in 32 bits. Every byte is read and written once but for the row that a second pass takes from the
-// caches.
+//
+// A row's elements stay in registers between its sums and its outputs: every byte is read once and written once. A row is held
+// by one wave, or by a workgroup, as LANES x PACKS loads of 16 bytes a lane (`Plan`); rows that have no such form (over 8,192
+// elements and not 16-byte aligned, or larger than a workgroup's registers) are read again for each pass, from the caches.
+// Sums in 32 bits.
 #include "pv_ops.h"
 
 using namespace pvo;
 
 namespace {
 
-constexpr int ROWS = 4;                    // waves, and rows at a time, of a workgroup
-constexpr int BLOCK = ROWS * WAVE;
-constexpr int PARTS = 256;                 // workgroups of the backward pass at most: rows of partial weight gradients
+constexpr int PARTS = 512;                 // workgroups of the backward pass at most: rows of partial weight gradients
 
-__device__ inline float wave_max_nan(float x) {       // the largest, or NaN if there is one
-#pragma unroll
-    for (int d = WAVE / 2; d; d >>= 1) {
-        const float o = __shfl_xor(x, d, WAVE);
-        x = o != o || o > x ? o : x;
-    }
-    return x;
-}
+// The larger of two values that are not negative, a NaN being the largest: their bits are in that order
+__device__ inline float larger_or_nan(float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); }
 
+// An 8-bit format: its largest value, and P values of it from floats that are at most that but for a rounding
 struct Fp8 {
     using type = uint8_t;
-    static constexpr float MOST = 448.0f;
-    // (|v| is at most 448 but for the quotient's rounding, and what is nearer to 448 than to 480 rounds to it; NaN stays NaN)
-    static __device__ type make(float v) { return uint8_t(__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false)); }
+    static constexpr float MOST = 448.0f;          // (what is nearer to 448 than to 480 rounds to it; NaN stays NaN)
+    template <int P> static __device__ void make(const float* v, pack<type, P>& o) {
+        if constexpr (P >= 4) {
+            uint32_t w[P / 4];
+#pragma unroll
+            for (int j = 0; j < P; j += 4) {
+                int x = __builtin_amdgcn_cvt_pk_fp8_f32(v[j], v[j + 1], 0, false);
+                w[j / 4] = __builtin_amdgcn_cvt_pk_fp8_f32(v[j + 2], v[j + 3], x, true);
+            }
+            __builtin_memcpy(&o, w, P);
+        } else {
+#pragma unroll
+            for (int j = 0; j < P; j++) o.v[j] = type(__builtin_amdgcn_cvt_pk_fp8_f32(v[j], v[j], 0, false));
+        }
+    }
 };
 struct Int8 {
     using type = int8_t;
     static constexpr float MOST = 127.0f;
-    static __device__ type make(float v) { return v != v ? 0 : int8_t(fminf(fmaxf(rintf(v), -127.0f), 127.0f)); }
+    template <int P> static __device__ void make(const float* v, pack<type, P>& o) {
+#pragma unroll
+        for (int j = 0; j < P; j++) o.v[j] = v[j] != v[j] ? 0 : type(fminf(fmaxf(rintf(v[j]), -MOST), MOST));
+    }
 };
 
-template <typename E, typename Q>
-__global__ __launch_bounds__(BLOCK) void norm_kernel(const E* x, const E* residual, const float* weight, int64_t N, int64_t D, int64_t xs, int64_t rs,
-                                                     float eps, E* y, E* stream, float* rstd, typename Q::type* q, float* scale) {
-    const int lane = threadIdx.x % WAVE;
-    const int64_t n = int64_t(blockIdx.x) * ROWS + threadIdx.x / WAVE;
-    if (n >= N) return;
+// One row: D elements as packs of P, pack k * LANES + lane in register k of a lane; PACKS 0: not held, any number of packs
+template <int LANES_, int PACKS_, int P_, int ROWS_> struct Plan {
+    static constexpr int LANES = LANES_, PACKS = PACKS_, P = P_, ROWS = ROWS_;      // ROWS: rows at a time of a workgroup
+    static constexpr int BLOCK = LANES * ROWS, WAVES = LANES / WAVE;
+};
+
+// A sum, or a largest value, over the lanes of a row
+template <typename L, typename F> __device__ inline float over_row(float x, float* lds, F&& join) {
+#pragma unroll
+    for (int d = WAVE / 2; d; d >>= 1) x = join(x, __shfl_xor(x, d, WAVE));
+    if constexpr (L::WAVES > 1) {
+        const int row = threadIdx.x / L::LANES, wave = threadIdx.x / WAVE;
+        __syncthreads();                                       // the last use of lds is over
+        if (threadIdx.x % WAVE == 0) lds[wave] = x;
+        __syncthreads();
+        x = lds[row * L::WAVES];
+#pragma unroll
+        for (int w = 1; w < L::WAVES; w++) x = join(x, lds[row * L::WAVES + w]);
+    }
+    return x;
+}
+template <typename L> __device__ inline float row_sum(float x, float* lds) {
+    return over_row<L>(x, lds, [](float a, float b) { return a + b; });
+}
+
+template <typename E, typename Q, typename L>
+__global__ __launch_bounds__(L::BLOCK) void norm_kernel(const E* __restrict__ x, const E* __restrict__ residual, const float* __restrict__ weight, int64_t N,
+                                                        int64_t D, int64_t xs, int64_t rs, float eps, E* __restrict__ y, E* __restrict__ stream,
+                                                        float* __restrict__ rstd, typename Q::type* __restrict__ q, float* __restrict__ scale) {
+    __shared__ float lds[L::BLOCK / WAVE];
+    constexpr int P = L::P, HELD = L::PACKS ? L::PACKS : 1;
+    using pk = pack<E, P>;
+    const int lane = threadIdx.x % L::LANES;
+    int64_t n = int64_t(blockIdx.x) * L::ROWS + threadIdx.x / L::LANES;
+    const bool on = n < N;
+    if (!on) n = N - 1;                    // (a workgroup's last rows: computed for the barriers' sake, not stored)
     const E* row = x + n * xs;
-    float sum = 0.0f;
-    for (int64_t i = lane; i < D; i += WAVE) {
-        float s = float(row[i]);
-        if (residual) {
-            const E t = E(s + float(residual[n * rs + i]));
-            stream[n * D + i] = t;
-            s = float(t);
+    const E* add = residual ? residual + n * rs : nullptr;
+    const int64_t packs = D / P;
+    pk held[HELD];
+    auto each = [&](auto&& f) {            // f(pack's values, first element's index) over the lane's packs
+        if constexpr (L::PACKS) {
+#pragma unroll
+            for (int k = 0; k < HELD; k++) if (const int64_t i = k * L::LANES + lane; i < packs) f(held[k], i * P);
+        } else {
+            const E* from = residual ? stream + n * D : row;
+            for (int64_t i = lane; i < packs; i += L::LANES) { pk h = pk::load(from + i * P); f(h, i * P); }
         }
-        sum = fmaf(s, s, sum);
+    };
+    auto get = [&](int64_t i) {            // a pack of the stream, stored where there is an addition
+        pk h = pk::load(row + i * P);
+        if (add) {
+            const pk a = pk::load(add + i * P);
+#pragma unroll
+            for (int j = 0; j < P; j++) h.v[j] = E(float(h.v[j]) + float(a.v[j]));
+            if (on || !L::PACKS) h.store(stream + n * D + i * P);
+        }
+        return h;
+    };
+    float sum = 0.0f;
+    auto square = [&](const pk& h, float m) {
+#pragma unroll
+        for (int j = 0; j < P; j++) { const float s = m * float(h.v[j]); sum = fmaf(s, s, sum); }
+    };
+    if constexpr (L::PACKS) {
+        pk more[HELD];                     // all loads before the first sum
+#pragma unroll
+        for (int k = 0; k < HELD; k++) if (const int64_t i = k * L::LANES + lane; i < packs) {
+            held[k] = pk::load(row + i * P);
+            if (add) more[k] = pk::load(add + i * P);
+        }
+#pragma unroll
+        for (int k = 0; k < HELD; k++) if (const int64_t i = k * L::LANES + lane; i < packs) {
+            if (add) {
+#pragma unroll
+                for (int j = 0; j < P; j++) held[k].v[j] = E(float(held[k].v[j]) + float(more[k].v[j]));
+                if (on) held[k].store(stream + n * D + i * P);
+            }
+            square(held[k], 1.0f);
+        }
+    } else {
+        for (int64_t i = lane; i < packs; i += L::LANES) square(get(i), 1.0f);
     }
-    const E* from = residual ? stream + n * D : row;
-    sum = wave_sum(sum);
-    float r = rsqrtf(sum / float(D) + eps);
-    if (sum == INFINITY) {                 // squares over 2^128: once more of 2^-64 s
+    sum = row_sum<L>(sum, lds);
+    // squares that leave 32 bits, or vanish in them where eps does too: once more of m s
+    float m = 1.0f;
+    if (sum == INFINITY || (sum < 0x1p-96f && eps < 0x1p-60f)) {
+        m = sum < 1.0f ? 0x1p48f : 0x1p-64f;
         sum = 0.0f;
-        for (int64_t i = lane; i < D; i += WAVE) { const float s = 0x1p-64f * float(from[i]); sum = fmaf(s, s, sum); }
-        r = 0x1p-64f * rsqrtf(wave_sum(sum) / float(D) + 0x1p-128f * eps);
+        each([&](const pk& h, int64_t) { square(h, m); });
+        sum = row_sum<L>(sum, lds);
     }
-    if (rstd && lane == 0) rstd[n] = r;
+    const float r = rsqrtf(sum / float(D) + m * m * eps);
+    if (rstd && on && lane == 0) rstd[n] = m * r;
     if (y) {
-        for (int64_t i = lane; i < D; i += WAVE) y[n * D + i] = E(float(from[i]) * r * weight[i]);
+        each([&](const pk& h, int64_t i) {
+            pk o;
+#pragma unroll
+            for (int j = 0; j < P; j++) o.v[j] = E(m * float(h.v[j]) * r * weight[i + j]);
+            if (on) o.store(y + n * D + i);
+        });
         return;
     }
+    // r is in every y of the row: q = s weight (448 / max |s weight|), without the roundings of y and of its scale
     float most = 0.0f;
-    for (int64_t i = lane; i < D; i += WAVE) {
-        const float a = fabsf(float(from[i]) * r * weight[i]);
-        most = a != a || a > most ? a : most;
-    }
-    const float sc = wave_max_nan(most) / Q::MOST;
-    if (lane == 0) scale[n] = sc;
-    for (int64_t i = lane; i < D; i += WAVE) q[n * D + i] = Q::make(sc == 0.0f ? 0.0f : float(from[i]) * r * weight[i] / sc);
+    each([&](const pk& h, int64_t i) {
+#pragma unroll
+        for (int j = 0; j < P; j++) most = larger_or_nan(most, fabsf(m * float(h.v[j]) * weight[i + j]));
+    });
+    most = over_row<L>(most, lds, larger_or_nan);
+    if (r == 0.0f) most = NAN;             // an infinity in the row
+    if (!on) return;
+    if (lane == 0) scale[n] = most / Q::MOST * r;
+    if (most < 0x1p-100f) { m *= 0x1p64f; most *= 0x1p64f; }
+    const float up = most == 0.0f ? 0.0f : Q::MOST / most;
+    each([&](const pk& h, int64_t i) {
+        float v[P];
+#pragma unroll
+        for (int j = 0; j < P; j++) v[j] = m * float(h.v[j]) * weight[i + j] * up;
+        pack<typename Q::type, P> o;
+        Q::template make<P>(v, o);
+        o.store(q + n * D + i);
+    });
 }
 
-template <typename E>
-__global__ __launch_bounds__(BLOCK) void norm_back_kernel(const E* s, const float* rstd, const float* weight, int64_t N, int64_t D, int64_t ss, const E* d_y,
-                                                          const E* d_stream, E* d, float* parts) {
-    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
-    float* part = parts + (int64_t(blockIdx.x) * ROWS + wave) * D;
-    for (int64_t i = lane; i < D; i += WAVE) part[i] = 0.0f;
-    for (int64_t n = int64_t(blockIdx.x) * ROWS + wave; n < N; n += int64_t(gridDim.x) * ROWS) {
+template <typename E, typename L>
+__global__ __launch_bounds__(L::BLOCK) void norm_back_kernel(const E* __restrict__ s, const float* __restrict__ rstd, const float* __restrict__ weight, int64_t N,
+                                                             int64_t D, int64_t ss, const E* __restrict__ d_y, const E* __restrict__ d_stream, E* __restrict__ d,
+                                                             float* __restrict__ parts) {
+    constexpr int P = L::P, HELD = L::PACKS ? L::PACKS : 1;
+    using pk = pack<E, P>;
+    __shared__ float lds[L::BLOCK / WAVE];
+    const int lane = threadIdx.x % L::LANES, at = threadIdx.x / L::LANES;
+    const int64_t packs = D / P;
+    float* part = parts + int64_t(blockIdx.x) * D;
+    float w[HELD][P], dw[HELD][P];
+    if constexpr (L::PACKS) {
+#pragma unroll
+        for (int k = 0; k < HELD; k++) {
+            const int64_t i = k * L::LANES + lane;
+#pragma unroll
+            for (int j = 0; j < P; j++) { w[k][j] = i < packs ? weight[i * P + j] : 0.0f; dw[k][j] = 0.0f; }
+        }
+    } else {
+        for (int64_t i = lane; i < D; i += L::LANES) part[i] = 0.0f;
+        __syncthreads();
+    }
+    for (int64_t first = int64_t(blockIdx.x) * L::ROWS; first < N; first += int64_t(gridDim.x) * L::ROWS) {
+        const bool on = first + at < N;
+        const int64_t n = on ? first + at : N - 1;
         const float r = rstd[n];
         float sum = 0.0f;
-        for (int64_t i = lane; i < D; i += WAVE) {
-            const float u = float(s[n * ss + i]) * r, dy = float(d_y[n * D + i]);
-            sum = fmaf(dy * weight[i], u, sum);
-            part[i] = fmaf(dy, u, part[i]);
+        pk u[HELD], dy[HELD], ds[HELD];
+        if constexpr (L::PACKS) {
+#pragma unroll
+            for (int k = 0; k < HELD; k++) if (const int64_t i = k * L::LANES + lane; i < packs) {
+                u[k] = pk::load(s + n * ss + i * P);
+                dy[k] = pk::load(d_y + n * D + i * P);
+                if (d_stream) ds[k] = pk::load(d_stream + n * D + i * P);
+            }
+#pragma unroll
+            for (int k = 0; k < HELD; k++) if (const int64_t i = k * L::LANES + lane; i < packs) {
+#pragma unroll
+                for (int j = 0; j < P; j++) {
+                    const float a = float(u[k].v[j]) * r, b = float(dy[k].v[j]);
+                    sum = fmaf(b * w[k][j], a, sum);
+                    if (on) dw[k][j] = fmaf(b, a, dw[k][j]);
+                }
+            }
+        } else {
+            for (int64_t i = lane; i < D; i += L::LANES) {
+                const float a = float(s[n * ss + i]) * r, b = float(d_y[n * D + i]);
+                sum = fmaf(b * weight[i], a, sum);
+                if (on) part[i] = fmaf(b, a, part[i]);
+            }
         }
-        const float m = wave_sum(sum) / float(D);
-        for (int64_t i = lane; i < D; i += WAVE) {
-            const float u = float(s[n * ss + i]) * r, g = float(d_y[n * D + i]) * weight[i];
-            d[n * D + i] = E((d_stream ? float(d_stream[n * D + i]) : 0.0f) + r * (g - u * m));
+        const float mean = row_sum<L>(sum, lds) / float(D);
+        if (!on) continue;                 // (the last pass of the loop)
+        if constexpr (L::PACKS) {
+#pragma unroll
+            for (int k = 0; k < HELD; k++) if (const int64_t i = k * L::LANES + lane; i < packs) {
+                pk o;
+#pragma unroll
+                for (int j = 0; j < P; j++) {
+                    const float a = float(u[k].v[j]) * r, g = float(dy[k].v[j]) * w[k][j];
+                    o.v[j] = E((d_stream ? float(ds[k].v[j]) : 0.0f) + r * (g - a * mean));
+                }
+                o.store(d + n * D + i * P);
+            }
+        } else {
+            for (int64_t i = lane; i < D; i += L::LANES) {
+                const float a = float(s[n * ss + i]) * r, g = float(d_y[n * D + i]) * weight[i];
+                d[n * D + i] = E((d_stream ? float(d_stream[n * D + i]) : 0.0f) + r * (g - a * mean));
+            }
+        }
+    }
+    if constexpr (L::PACKS) {
+        if constexpr (L::ROWS > 1) {       // the rows that the workgroup has at a time, summed in row 0's lanes
+            __shared__ float sums[L::ROWS - 1][HELD * P][L::LANES];
+            if (at) {
+#pragma unroll
+                for (int k = 0; k < HELD; k++)
+#pragma unroll
+                    for (int j = 0; j < P; j++) sums[at - 1][k * P + j][lane] = dw[k][j];
+            }
+            __syncthreads();
+            if (at) return;
+#pragma unroll
+            for (int k = 0; k < HELD; k++)
+#pragma unroll
+                for (int j = 0; j < P; j++)
+#pragma unroll
+                    for (int o = 0; o < L::ROWS - 1; o++) dw[k][j] += sums[o][k * P + j][lane];
+        }
+#pragma unroll
+        for (int k = 0; k < HELD; k++) if (const int64_t i = k * L::LANES + lane; i < packs) {
+#pragma unroll
+            for (int j = 0; j < P; j++) part[i * P + j] = dw[k][j];
         }
     }
 }
 
-__global__ __launch_bounds__(BLOCK) void norm_weight_kernel(const float* parts, int64_t rows, int64_t D, float* d_weight) {
-    const int64_t i = int64_t(blockIdx.x) * BLOCK + threadIdx.x;
-    if (i >= D) return;
+// d_weight[i] = sum of the partial rows: 64 columns a workgroup, its 16 waves a run of rows each
+constexpr int END_WAVES = 16;
+__global__ __launch_bounds__(END_WAVES* WAVE) void norm_weight_kernel(const float* __restrict__ parts, int64_t rows, int64_t D, float* __restrict__ d_weight) {
+    __shared__ float lds[END_WAVES][WAVE];
+    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+    const int64_t i = int64_t(blockIdx.x) * WAVE + lane;
     float sum = 0.0f;
-    for (int64_t k = 0; k < rows; k++) sum += parts[k * D + i];
+    if (i < D) {
+#pragma unroll 8
+        for (int64_t k = wave; k < rows; k += END_WAVES) sum += parts[k * D + i];
+    }
+    lds[wave][lane] = sum;
+    __syncthreads();
+    if (wave || i >= D) return;
+#pragma unroll
+    for (int w = 1; w < END_WAVES; w++) sum += lds[w][lane];
     d_weight[i] = sum;
 }
 
-int64_t parts_of(int64_t N) { const int64_t g = (N + ROWS - 1) / ROWS; return g < PARTS ? g : PARTS; }
+// f(Plan) for rows of D elements of type E; wide: every row and tensor starts at a multiple of 16 bytes. The backward pass
+// holds three tensors, the weights and their gradients' sums, so its lanes take half as many elements.
+template <typename E, bool BACK, typename F> int32_t with_plan(int64_t D, bool wide, F&& f) {
+    if (wide) {
+        constexpr int P = 16 / sizeof(E);
+        const int64_t packs = D / P;
+        if (packs <= 64) return f(Plan<64, 1, P, 4>{});
+        if (packs <= 128) return f(Plan<64, 2, P, 4>{});
+        if constexpr (BACK) {
+            if (packs <= 256) return f(Plan<256, 1, P, 1>{});
+            if (packs <= 512) return f(Plan<256, 2, P, 1>{});
+            if (packs <= 2048) return f(Plan<1024, 2, P, 1>{});
+        } else {
+            if (packs <= 256) return f(Plan<64, 4, P, 4>{});
+            if (packs <= 512) return f(Plan<256, 2, P, 1>{});
+            if (packs <= 1024) return f(Plan<256, 4, P, 1>{});
+            if (packs <= 4096) return f(Plan<1024, 4, P, 1>{});
+        }
+    } else {
+        if (D <= 256) return f(Plan<64, 4, 1, 4>{});
+        if (D <= 2048) return f(Plan<256, 8, 1, 1>{});
+        if (D <= 8192) return f(Plan<1024, 8, 1, 1>{});
+    }
+    return f(Plan<256, 0, 1, 1>{});
+}
+
+int64_t groups_of(int64_t N, int rows) { const int64_t g = (N + rows - 1) / rows; return g < PARTS ? g : PARTS; }
 
 int32_t check(int64_t N, int64_t D, int32_t dtype, char* err, size_t cap) {
     if (!element_bytes(dtype)) return fail(PV_EARG, err, cap, "dtype: one of PV_F32, PV_BF16, PV_F16");
-    if (N < 0 || D < 1 || N > int64_t(ROWS) * INT32_MAX) return fail(PV_EARG, err, cap, "shape: 0 <= N < 2^33, D >= 1");
+    if (N < 0 || D < 1 || N > INT32_MAX) return fail(PV_EARG, err, cap, "shape: 0 <= N < 2^31, D >= 1");
     return PV_OK;
 }
 
@@ -123,10 +331,16 @@ int32_t forward(const void* x, const void* residual, const float* weight, int64_
     if (!x || !weight || (residual && !stream_out) || (!y && (!q || !scale))) return fail(PV_EARG, err, errcap, "null argument");
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
-        norm_kernel<E, Q><<<dim3((N + ROWS - 1) / ROWS), BLOCK, 0, hipStream_t(stream)>>>(
-            static_cast<const E*>(x), static_cast<const E*>(residual), weight, N, D, xs, rs, eps, static_cast<E*>(y), static_cast<E*>(stream_out), rstd,
-            static_cast<typename Q::type*>(q), scale);
-        return launched(err, errcap);
+        constexpr int packed = 16 / sizeof(E);
+        const bool wide = D % packed == 0 && (N == 1 || (xs % packed == 0 && (!residual || rs % packed == 0))) && aligned(x, 16) && aligned(residual, 16) &&
+                          aligned(y, 16) && aligned(stream_out, 16) && aligned(q, packed);
+        return with_plan<E, false>(D, wide, [&](auto plan) {
+            using L = decltype(plan);
+            norm_kernel<E, Q, L><<<dim3((N + L::ROWS - 1) / L::ROWS), L::BLOCK, 0, hipStream_t(stream)>>>(
+                static_cast<const E*>(x), static_cast<const E*>(residual), weight, N, D, xs, rs, eps, static_cast<E*>(y), static_cast<E*>(stream_out), rstd,
+                static_cast<typename Q::type*>(q), scale);
+            return launched(err, errcap);
+        });
     });
 }
 
@@ -149,7 +363,7 @@ int32_t pv_add_rms_norm_8bit_hip(const void* x, const void* residual, const floa
     return fail(PV_EARG, err, errcap, "format: PV_E4M3 or PV_INT8");
 }
 
-uint64_t pv_add_rms_norm_work_bytes(int64_t N, int64_t D) { return N > 0 && D > 0 ? uint64_t(parts_of(N)) * ROWS * uint64_t(D) * 4 : 0; }
+uint64_t pv_add_rms_norm_work_bytes(int64_t N, int64_t D) { return N > 0 && D > 0 ? uint64_t(groups_of(N, 1)) * uint64_t(D) * 4 : 0; }
 
 int32_t pv_add_rms_norm_backward_hip(const void* s, const float* rstd, const float* weight, int64_t N, int64_t D, int64_t s_row, const void* d_y,
                                      const void* d_stream, int32_t dtype, void* d, float* d_weight, void* work, uint64_t work_bytes, void* stream, char* err,
@@ -161,11 +375,16 @@ int32_t pv_add_rms_norm_backward_hip(const void* s, const float* rstd, const flo
     float* parts = static_cast<float*>(work);
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
-        const int64_t g = parts_of(N);
-        if (N) norm_back_kernel<E><<<dim3(g), BLOCK, 0, st>>>(static_cast<const E*>(s), rstd, weight, N, D, s_row, static_cast<const E*>(d_y),
-                                                              static_cast<const E*>(d_stream), static_cast<E*>(d), parts);
-        norm_weight_kernel<<<dim3((D + BLOCK - 1) / BLOCK), BLOCK, 0, st>>>(parts, g * ROWS, D, d_weight);
-        return launched(err, errcap);
+        constexpr int packed = 16 / sizeof(E);
+        const bool wide = D % packed == 0 && (N <= 1 || s_row % packed == 0) && aligned(s, 16) && aligned(d_y, 16) && aligned(d_stream, 16) && aligned(d, 16);
+        return with_plan<E, true>(D, wide, [&](auto plan) {
+            using L = decltype(plan);
+            const int64_t g = groups_of(N, L::ROWS);
+            if (N) norm_back_kernel<E, L><<<dim3(g), L::BLOCK, 0, st>>>(static_cast<const E*>(s), rstd, weight, N, D, s_row, static_cast<const E*>(d_y),
+                                                                        static_cast<const E*>(d_stream), static_cast<E*>(d), parts);
+            norm_weight_kernel<<<dim3((D + WAVE - 1) / WAVE), END_WAVES * WAVE, 0, st>>>(parts, g, D, d_weight);
+            return launched(err, errcap);
+        });
     });
 }
 
