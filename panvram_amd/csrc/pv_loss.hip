@@ -6,6 +6,16 @@
 //   d_logits = (softmax - onehot) * w, w = scale / count or the place's own factor;
 //   d_hidden = d_logits weight (0 where a place does not count);  d_weight = sum over places of d_logits^T hidden
 // What stands in hidden at places that do not count (NaN too) reaches nothing.
+//
+// The alphabet fills one 16-wide matrix tile. A tile of 16 places goes through it three times: logits = weight hidden^T
+// (contracted over D), d_hidden = weight^T d_logits (over the ids), d_weight = hidden^T d_logits (over the places). A wave has
+// a slab of columns and keeps there, in registers, the weights in both operands' layouts, the tile's hidden values and the sums
+// of d_weight: `fused_kernel` reads hidden once for all three, with one exchange of partial logits between the waves of a
+// workgroup a tile. Rows of more slabs than a workgroup has waves go through `place_kernel` (logits, d_logits stored) and
+// `grad_kernel` (the other two by columns), which reads hidden again.
+// The operand that a product needs transposed is made by a product with the identity, which is exact.
+//   Bf  hidden and weight in bfloat16: bfloat16 products, sums in 32 bits; d_logits as the sum of two bfloat16, 16 bits of it
+//   F3  all others: values in 32 bits, 32-bit products
 #include "pv_ops.h"
 
 using namespace pvo;
@@ -13,159 +23,493 @@ using namespace pvo;
 namespace {
 
 constexpr int VMAX = 16;                   // ids at most
-constexpr int ROWS = 4;                    // waves, and places at a time, of a workgroup
-constexpr int BLOCK = ROWS * WAVE;
+constexpr int TILE = 16;                   // places of a tile
 constexpr int COUNTS = 256;                // workgroups that count places
-constexpr int SPLITS = 64;                 // runs of places in which weight gradients are summed
+constexpr int BLOCK = 256;
+constexpr int MOST_WAVES = 16;             // of a workgroup
+constexpr int END_WAVES = 16;
+
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using bf16x4 = __attribute__((ext_vector_type(4))) __bf16;
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using s16x4 = __attribute__((ext_vector_type(4))) short;
 
 struct Shape {
-    int64_t B, T, D, hb, ht, tb;           // strides in elements: hidden (batch, time), tokens (batch); channels, tokens are neighbours
-    int64_t ignore;
-    int32_t V;
+    int64_t B, T, D, N, hb, ht, tb;        // N = B T; strides in elements: hidden (batch, time), tokens (batch)
+    int64_t ignore, Dp;                    // Dp: D filled up to whole slabs
+    int32_t V, token_bytes;
+    bool flat;                             // hidden's places are ht apart throughout
 };
 
-// the id that place n predicts, or -1 where it does not count
-template <typename I> __device__ inline int target(const Shape& S, const I* tokens, int64_t n) {
-    const int64_t b = n / S.T, t = n % S.T;
+// What the matrix instructions hold in a lane: l = 16 g + c. First operand: row c, elements k of its group g; second: column
+// c, the same k; result: column c, rows 4 g + r. k is 8 g + j for 16x16x32, 4 g + j for 16x16x16, g for 16x16x4.
+__device__ inline int lane_c() { return threadIdx.x % 16; }
+__device__ inline int lane_g() { return threadIdx.x % WAVE / 16; }
+
+// N elements at p[i], i < left only, others 0
+template <bool WIDE, typename E, int N> __device__ inline pack<E, N> get(const E* p, int64_t left) {
+    if constexpr (WIDE) {
+        if (left > 0) return pack<E, N>::load(p);
+        pack<E, N> z;
+#pragma unroll
+        for (int j = 0; j < N; j++) z.v[j] = E(0.0f);
+        return z;
+    } else {
+        pack<E, N> r;
+#pragma unroll
+        for (int j = 0; j < N; j++) r.v[j] = j < left ? p[j] : E(0.0f);
+        return r;
+    }
+}
+template <bool WIDE, typename E, int N> __device__ inline void put(const pack<E, N>& v, E* p, int64_t left) {
+    if constexpr (WIDE) {
+        if (left > 0) v.store(p);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j++) if (j < left) p[j] = v.v[j];
+    }
+}
+
+// A slab of 128 columns in bfloat16
+template <typename E_, bool WIDE> struct Bf {
+    using E = E_;
+    using K = __bf16;                      // what the weights are laid out as
+    static constexpr int COLS = 128, STEPS = 4, TILES = 8;
+    struct Rows { bf16x8 h[STEPS]; };      // column 32 q + 8 g + j of place c
+    struct Sums { f32x4 dw[TILES]; };      // id c, columns 16 k + 4 g + r
+    bf16x8 w[STEPS];                       // id c, columns as Rows
+    s16x4 wt[TILES];                       // column 32 q + 8 (c / 4) + 4 t + c % 4 at 2 q + t, ids 4 g + j
+
+    __device__ void weights(const K* wr, int64_t Dp, int64_t c0) {
+#pragma unroll
+        for (int q = 0; q < STEPS; q++) w[q] = *reinterpret_cast<const bf16x8*>(wr + lane_c() * Dp + c0 + 32 * q + 8 * lane_g());
+    }
+    __device__ void weights_back(const K* wc, int64_t c0) {
+        const int c = lane_c();
+#pragma unroll
+        for (int k = 0; k < TILES; k++)
+            wt[k] = *reinterpret_cast<const s16x4*>(wc + (c0 + 32 * (k / 2) + 8 * (c / 4) + 4 * (k % 2) + c % 4) * VMAX + 4 * lane_g());
+    }
+    static __device__ Rows rows(const E* row, int64_t c0, int64_t D, bool on) {
+        Rows R;
+#pragma unroll
+        for (int q = 0; q < STEPS; q++) {
+            const int64_t i = c0 + 32 * q + 8 * lane_g();
+            const auto p = get<WIDE, E, 8>(row + i, on ? D - i : 0);
+            __builtin_memcpy(&R.h[q], &p, 16);
+        }
+        return R;
+    }
+    static __device__ void clear(Rows& R) {
+#pragma unroll
+        for (int q = 0; q < STEPS; q++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) R.h[q][j] = __bf16(0.0f);
+    }
+    __device__ f32x4 logits(const Rows& R, f32x4 l) const {
+#pragma unroll
+        for (int q = 0; q < STEPS; q++) l = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[q], R.h[q], l, 0, 0, 0);
+        return l;
+    }
+    static __device__ s16x4 bits(f32x4 x) {
+        const bf16x4 b = __builtin_convertvector(x, bf16x4);
+        return __builtin_bit_cast(s16x4, b);
+    }
+    static __device__ f32x4 product(s16x4 a, s16x4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0); }
+    // dl: d_logits of place c, ids 4 g + j
+    __device__ void back(const Rows& R, f32x4 dl, E* d_row, int64_t c0, int64_t D, bool store, Sums& S) const {
+        const int c = lane_c(), g = lane_g();
+        const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+        const s16x4 hi = bits(dl);
+        const s16x4 lo = bits(dl - __builtin_convertvector(__builtin_bit_cast(bf16x4, hi), f32x4));
+        s16x4 one;                         // the identity, 16 x 16
+        bf16x8 half[2];                    // columns 0..15 and 16..31 of the identity, 32 x 32
+#pragma unroll
+        for (int j = 0; j < 4; j++) one[j] = c == 4 * g + j ? 0x3f80 : 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) { half[0][j] = __bf16(c == 8 * g + j ? 1.0f : 0.0f); half[1][j] = __bf16(c + 16 == 8 * g + j ? 1.0f : 0.0f); }
+        const s16x4 thi = bits(product(hi, one, none)), tlo = bits(product(lo, one, none));      // id c, places 4 g + j
+#pragma unroll
+        for (int q = 0; q < STEPS; q++) {
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const s16x4 ht = bits(__builtin_amdgcn_mfma_f32_16x16x32_bf16(R.h[q], half[s], none, 0, 0, 0));      // column 32 q + 16 s + c, places 4 g + j
+                S.dw[2 * q + s] = product(ht, tlo, product(ht, thi, S.dw[2 * q + s]));
+            }
+            pack<E, 8> o;
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const f32x4 x = product(wt[2 * q + t], lo, product(wt[2 * q + t], hi, none));
+#pragma unroll
+                for (int r = 0; r < 4; r++) o.v[4 * t + r] = E(x[r]);
+            }
+            const int64_t i = c0 + 32 * q + 8 * g;
+            put<WIDE, E, 8>(o, d_row + i, store ? D - i : 0);
+        }
+    }
+};
+
+// A slab of 64 columns in 32 bits
+template <typename E_, bool WIDE> struct F3 {
+    using E = E_;
+    using K = float;
+    static constexpr int COLS = 64, STEPS = 4, TILES = 4;
+    struct Rows { pack<E, 4> h[STEPS]; };  // column 16 s + 4 g + j of place c
+    struct Sums { f32x4 dw[TILES]; };      // id c, columns 16 s + 4 g + r
+    f32x4 w[STEPS], wt[TILES];             // id c, columns as Rows; column 16 s + c, ids 4 g + j
+
+    __device__ void weights(const K* wr, int64_t Dp, int64_t c0) {
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) w[s] = *reinterpret_cast<const f32x4*>(wr + lane_c() * Dp + c0 + 16 * s + 4 * lane_g());
+    }
+    __device__ void weights_back(const K* wc, int64_t c0) {
+#pragma unroll
+        for (int s = 0; s < TILES; s++) wt[s] = *reinterpret_cast<const f32x4*>(wc + (c0 + 16 * s + lane_c()) * VMAX + 4 * lane_g());
+    }
+    static __device__ Rows rows(const E* row, int64_t c0, int64_t D, bool on) {
+        Rows R;
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            const int64_t i = c0 + 16 * s + 4 * lane_g();
+            R.h[s] = get<WIDE, E, 4>(row + i, on ? D - i : 0);
+        }
+        return R;
+    }
+    static __device__ void clear(Rows& R) {
+#pragma unroll
+        for (int s = 0; s < STEPS; s++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) R.h[s].v[j] = E(0.0f);
+    }
+    static __device__ f32x4 product(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+    __device__ f32x4 logits(const Rows& R, f32x4 l) const {
+#pragma unroll
+        for (int s = 0; s < STEPS; s++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) l = product(w[s][j], float(R.h[s].v[j]), l);
+        return l;
+    }
+    __device__ void back(const Rows& R, f32x4 dl, E* d_row, int64_t c0, int64_t D, bool store, Sums& S) const {
+        const int c = lane_c(), g = lane_g();
+        const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+        float one[4];                      // rows j, 4 + j, 8 + j, 12 + j of the identity
+#pragma unroll
+        for (int j = 0; j < 4; j++) one[j] = c == 4 * g + j ? 1.0f : 0.0f;
+        f32x4 t = none;                    // id c, places 4 g + j
+#pragma unroll
+        for (int j = 0; j < 4; j++) t = product(dl[j], one[j], t);
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            f32x4 ht = none, x = none;     // ht: column 16 s + c, places 4 g + j
+#pragma unroll
+            for (int j = 0; j < 4; j++) ht = product(float(R.h[s].v[j]), one[j], ht);
+#pragma unroll
+            for (int j = 0; j < 4; j++) { S.dw[s] = product(ht[j], t[j], S.dw[s]); x = product(wt[s][j], dl[j], x); }
+            pack<E, 4> o;
+#pragma unroll
+            for (int r = 0; r < 4; r++) o.v[r] = E(x[r]);
+            const int64_t i = c0 + 16 * s + 4 * g;
+            put<WIDE, E, 4>(o, d_row + i, store ? D - i : 0);
+        }
+    }
+};
+
+// Place n: where its row is, and the id that it predicts (-1: it does not count)
+__device__ inline void split(const Shape& S, int64_t n, int64_t& b, int64_t& t) {
+    if (S.N <= UINT32_MAX) { const uint32_t m = uint32_t(n), d = uint32_t(S.T); b = m / d; t = m % d; }
+    else { b = n / S.T; t = n % S.T; }
+}
+template <typename E> __device__ inline const E* place(const Shape& S, const E* hidden, int64_t b, int64_t t, int64_t n) {
+    return hidden + (S.flat ? n * S.ht : b * S.hb + t * S.ht);
+}
+__device__ inline int target(const Shape& S, const void* tokens, int64_t b, int64_t t) {
     if (t + 1 >= S.T) return -1;
-    const int64_t v = int64_t(tokens[b * S.tb + t + 1]);
+    const int64_t i = b * S.tb + t + 1;
+    const int64_t v = S.token_bytes == 1 ? int64_t(static_cast<const uint8_t*>(tokens)[i]) : static_cast<const int64_t*>(tokens)[i];
     return v >= 0 && v < S.V && v != S.ignore ? int(v) : -1;
 }
 
-template <typename X> __device__ inline X block_sum(X x, X* lds) {
+template <typename X> __device__ inline X wave_total(X x) {
 #pragma unroll
     for (int d = WAVE / 2; d; d >>= 1) x += __shfl_xor(x, d, WAVE);
-    if (threadIdx.x % WAVE == 0) lds[threadIdx.x / WAVE] = x;
-    __syncthreads();
-    X sum = 0;
-    for (int w = 0; w < int(blockDim.x) / WAVE; w++) sum += lds[w];
-    __syncthreads();
-    return sum;
+    return x;
 }
-
-template <typename I> __global__ __launch_bounds__(BLOCK) void loss_count_kernel(Shape S, const I* tokens, int64_t* counts) {
-    __shared__ int64_t lds[ROWS];
+// scale / count, from the counting workgroups' numbers
+__device__ inline float mean_factor(const int64_t* counts, const float* scale) {
     int64_t k = 0;
-    for (int64_t n = int64_t(blockIdx.x) * BLOCK + threadIdx.x; n < S.B * S.T; n += int64_t(gridDim.x) * BLOCK) k += target(S, tokens, n) >= 0;
-    k = block_sum(k, lds);
-    if (threadIdx.x == 0) counts[blockIdx.x] = k;
+    for (int j = threadIdx.x % WAVE; j < COUNTS; j += WAVE) k += counts[j];
+    k = wave_total(k);
+    return (scale ? *scale : 1.0f) / float(k > 0 ? k : 1);
 }
 
-template <typename E, typename W, typename I>
-__global__ __launch_bounds__(BLOCK) void loss_place_kernel(Shape S, const E* hidden, const W* weight, const I* tokens, const int64_t* counts, const float* scale,
-                                                           const float* factor, float* each, E* d_hidden, float* d_logits, double* sums) {
-    __shared__ int64_t ilds[ROWS];
-    __shared__ double dlds[ROWS];
-    float base = 1.0f;
-    if (counts) {
-        const int64_t k = block_sum(counts[threadIdx.x], ilds);
-        base = (scale ? *scale : 1.0f) / float(k > 0 ? k : 1);
+// A place's loss from its logits (place c, ids 4 g + r), and in their place the gradients of the logits times `w`
+__device__ inline float softmax(f32x4& l, int at, int V, float w) {
+    const int first = 4 * lane_g();
+    float top = -INFINITY, total = 0.0f, own = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        if (first + r == at) own = l[r];
+        if (first + r < V) top = fmaxf(top, l[r]);
     }
-    const int lane = threadIdx.x % WAVE;
-    double sum = 0.0;
-    for (int64_t n = int64_t(blockIdx.x) * ROWS + threadIdx.x / WAVE; n < S.B * S.T; n += int64_t(gridDim.x) * ROWS) {
-        const int at = target(S, tokens, n);
-        const E* h = hidden + n / S.T * S.hb + n % S.T * S.ht;
-        float p[VMAX] = {};
-        if (at >= 0) {
-            for (int64_t i = lane; i < S.D; i += WAVE) {
-                const float x = float(h[i]);
+    top = fmaxf(top, __shfl_xor(top, 16, WAVE));
+    top = fmaxf(top, __shfl_xor(top, 32, WAVE));
 #pragma unroll
-                for (int v = 0; v < VMAX; v++) if (v < S.V) p[v] = fmaf(x, float(weight[v * S.D + i]), p[v]);
-            }
-            float top = -INFINITY, total = 0.0f, own = 0.0f;
+    for (int r = 0; r < 4; r++) { l[r] = first + r < V ? expf(l[r] - top) : 0.0f; total += l[r]; }
+    total += __shfl_xor(total, 16, WAVE);
+    total += __shfl_xor(total, 32, WAVE);
+    own += __shfl_xor(own, 16, WAVE);
+    own += __shfl_xor(own, 32, WAVE);
+    const float up = 1.0f / total;
 #pragma unroll
-            for (int v = 0; v < VMAX; v++) if (v < S.V) {
-                p[v] = wave_sum(p[v]);
-                top = fmaxf(top, p[v]);
-                if (v == at) own = p[v];
-            }
-#pragma unroll
-            for (int v = 0; v < VMAX; v++) if (v < S.V) { p[v] = expf(p[v] - top); total += p[v]; }
-            const float l = logf(total) + top - own;
-            if (lane == 0) { if (each) each[n] = l; sum += double(l); }
-            if (d_hidden) {
-                const float w = factor ? factor[n] : base;
-#pragma unroll
-                for (int v = 0; v < VMAX; v++) if (v < S.V) p[v] = (p[v] / total - float(v == at)) * w;
-            }
-        } else if (each && lane == 0) each[n] = 0.0f;
-        if (!d_hidden) continue;
-        if (lane == 0) for (int v = 0; v < VMAX; v++) d_logits[n * VMAX + v] = v < S.V ? p[v] : 0.0f;
-        for (int64_t i = lane; i < S.D; i += WAVE) {
-            float x = 0.0f;
-#pragma unroll
-            for (int v = 0; v < VMAX; v++) if (v < S.V) x = fmaf(p[v], float(weight[v * S.D + i]), x);
-            d_hidden[n * S.D + i] = at >= 0 ? E(x) : E(0.0f);
+    for (int r = 0; r < 4; r++) l[r] = at >= 0 ? (l[r] * up - (first + r == at ? 1.0f : 0.0f)) * w : 0.0f;
+    return at >= 0 ? logf(total) + top - own : 0.0f;
+}
+
+// Workgroups below `counting`: how many places count. The others: the weights, filled up with zeros to 16 ids and whole slabs,
+// by ids (wr) and by columns (wc).
+template <typename W, typename K>
+__global__ __launch_bounds__(BLOCK) void begin_kernel(Shape S, const void* tokens, int counting, int64_t* counts, const W* weight, K* wr, K* wc) {
+    if (int(blockIdx.x) < counting) {
+        __shared__ int64_t lds[BLOCK / WAVE];
+        int64_t k = 0;
+        for (int64_t n = int64_t(blockIdx.x) * BLOCK + threadIdx.x; n < S.N; n += int64_t(COUNTS) * BLOCK) {
+            int64_t b, t;
+            split(S, n, b, t);
+            k += target(S, tokens, b, t) >= 0;
         }
+        k = wave_total(k);
+        if (threadIdx.x % WAVE == 0) lds[threadIdx.x / WAVE] = k;
+        __syncthreads();
+        if (threadIdx.x) return;
+        for (int w = 1; w < BLOCK / WAVE; w++) k += lds[w];
+        counts[blockIdx.x] = k;
+        return;
     }
-    sum = block_sum(sum, dlds);
-    if (threadIdx.x == 0) sums[blockIdx.x] = sum;
+    const int64_t e = int64_t(blockIdx.x - counting) * BLOCK + threadIdx.x, v = e / S.Dp, i = e % S.Dp;
+    if (v >= VMAX) return;
+    const K x = v < S.V && i < S.D ? K(float(weight[v * S.D + i])) : K(0.0f);
+    wr[e] = x;
+    if (wc) wc[i * VMAX + v] = x;
 }
 
-// parts[s, v, i]: the sum of one run of places
-template <typename E, typename I>
-__global__ __launch_bounds__(WAVE) void loss_weight_kernel(Shape S, const E* hidden, const I* tokens, const float* d_logits, float* parts) {
-    const int64_t i = int64_t(blockIdx.x) * WAVE + threadIdx.x, N = S.B * S.T, run = (N + SPLITS - 1) / SPLITS;
-    const int64_t from = blockIdx.y * run, to = from + run < N ? from + run : N;
-    float p[VMAX] = {};
-    for (int64_t n = from; n < to; n++) {
-        if (target(S, tokens, n) < 0 || i >= S.D) continue;
-        const float x = float(hidden[n / S.T * S.hb + n % S.T * S.ht + i]);
+// Logits, losses and all gradients in one pass over hidden; a wave for each slab of the row
+template <typename M>
+__global__ __launch_bounds__(MOST_WAVES* WAVE)
+void fused_kernel(Shape S, const typename M::E* __restrict__ hidden, const void* __restrict__ tokens, const typename M::K* __restrict__ wr,
+                  const typename M::K* __restrict__ wc, const int64_t* counts, const float* scale, const float* __restrict__ factor, float* __restrict__ each,
+                  typename M::E* __restrict__ d_hidden, double* sums, float* __restrict__ parts) {
+    extern __shared__ f32x4 lds[];         // partial logits, for this tile and the one before: [2][waves][lanes]
+    const int wave = threadIdx.x / WAVE, waves = blockDim.x / WAVE, lane = threadIdx.x % WAVE, c = lane_c();
+    const int64_t c0 = int64_t(wave) * M::COLS;
+    M m;
+    m.weights(wr, S.Dp, c0);
+    m.weights_back(wc, c0);
+    typename M::Sums sum = {};
+    const float base = counts ? mean_factor(counts, scale) : 0.0f;
+    double loss = 0.0;
+    struct Next { typename M::Rows rows; int at; float w; } next;
+    auto fetch = [&](int64_t tile) {
+        const int64_t n = tile * TILE + c;
+        const bool on = n < S.N;
+        int64_t b, t;
+        split(S, on ? n : 0, b, t);
+        next.rows = M::rows(place(S, hidden, b, t, on ? n : 0), c0, S.D, on);
+        next.at = on ? target(S, tokens, b, t) : -1;
+        next.w = factor && on ? factor[n] : base;
+    };
+    const int64_t tiles = (S.N + TILE - 1) / TILE;
+    int turn = 0;
+    if (blockIdx.x < tiles) fetch(blockIdx.x);
+    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
+        Next now = next;
+        if (tile + gridDim.x < tiles) fetch(tile + gridDim.x);
+        if (now.at < 0) M::clear(now.rows);
+        f32x4 l = m.logits(now.rows, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+        if (waves > 1) {
+            f32x4* mine = lds + turn * waves * WAVE;
+            mine[wave * WAVE + lane] = l;
+            __syncthreads();               // (the other half is free again: every wave has passed the tile before)
+            l = mine[lane];
+            for (int k = 1; k < waves; k++) l += mine[k * WAVE + lane];
+        }
+        const float x = softmax(l, now.at, S.V, now.w);
+        const int64_t n = tile * TILE + c;
+        if (wave == 0 && lane < TILE && n < S.N) {
+            loss += double(x);
+            if (each) each[n] = x;
+        }
+        m.back(now.rows, l, d_hidden + n * S.D, c0, S.D, n < S.N, sum);
+    }
+    if (wave == 0) {
+        loss = wave_total(loss);
+        if (lane == 0) sums[blockIdx.x] = loss;
+    }
+    if (c < S.V) {
 #pragma unroll
-        for (int v = 0; v < VMAX; v++) p[v] = fmaf(d_logits[n * VMAX + v], x, p[v]);
+        for (int k = 0; k < M::TILES; k++) *reinterpret_cast<f32x4*>(parts + (int64_t(blockIdx.x) * S.V + c) * S.Dp + c0 + 16 * k + 4 * lane_g()) = sum.dw[k];
     }
-    if (i >= S.D) return;
-    for (int v = 0; v < S.V; v++) parts[(blockIdx.y * int64_t(S.V) + v) * S.D + i] = p[v];
 }
 
+// Logits and losses of a tile by one wave, over all columns; with d_logits, their gradients ([N, 16])
+template <typename M>
+__global__ __launch_bounds__(BLOCK) void place_kernel(Shape S, const typename M::E* __restrict__ hidden, const void* __restrict__ tokens,
+                                                      const typename M::K* __restrict__ wr, const int64_t* counts, const float* scale,
+                                                      const float* __restrict__ factor, float* __restrict__ each, f32x4* __restrict__ d_logits, double* sums) {
+    __shared__ double lds[BLOCK / WAVE];
+    const int lane = threadIdx.x % WAVE, c = lane_c();
+    const float base = d_logits && counts ? mean_factor(counts, scale) : 0.0f;
+    double loss = 0.0;
+    const int64_t tiles = (S.N + TILE - 1) / TILE;
+    for (int64_t tile = int64_t(blockIdx.x) * (BLOCK / WAVE) + threadIdx.x / WAVE; tile < tiles; tile += int64_t(gridDim.x) * (BLOCK / WAVE)) {
+        const int64_t n = tile * TILE + c;
+        const bool on = n < S.N;
+        int64_t b, t;
+        split(S, on ? n : 0, b, t);
+        const typename M::E* row = place(S, hidden, b, t, on ? n : 0);
+        const int at = on ? target(S, tokens, b, t) : -1;
+        f32x4 l = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int64_t c0 = 0; c0 < S.D; c0 += M::COLS) {
+            M m;
+            m.weights(wr, S.Dp, c0);
+            l = m.logits(M::rows(row, c0, S.D, on), l);
+        }
+        const float x = softmax(l, at, S.V, factor && on ? factor[n] : base);
+        if (lane < TILE && on) {
+            loss += double(x);
+            if (each) each[n] = x;
+        }
+        if (d_logits && on) d_logits[n * 4 + lane_g()] = l;
+    }
+    loss = wave_total(loss);
+    if (lane == 0) lds[threadIdx.x / WAVE] = loss;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int w = 1; w < BLOCK / WAVE; w++) loss += lds[w];
+    sums[blockIdx.x] = loss;
+}
+
+// d_hidden and d_weight from d_logits, a wave for each slab
+template <typename M>
+__global__ __launch_bounds__(BLOCK) void grad_kernel(Shape S, const typename M::E* __restrict__ hidden, const void* __restrict__ tokens,
+                                                     const typename M::K* __restrict__ wc, const f32x4* __restrict__ d_logits,
+                                                     typename M::E* __restrict__ d_hidden, float* __restrict__ parts) {
+    const int c = lane_c();
+    const int64_t c0 = (int64_t(blockIdx.x) * (BLOCK / WAVE) + threadIdx.x / WAVE) * M::COLS;
+    if (c0 >= S.Dp) return;
+    M m;
+    m.weights_back(wc, c0);
+    typename M::Sums sum = {};
+    const int64_t tiles = (S.N + TILE - 1) / TILE;
+    for (int64_t tile = blockIdx.y; tile < tiles; tile += gridDim.y) {
+        const int64_t n = tile * TILE + c;
+        const bool on = n < S.N;
+        int64_t b, t;
+        split(S, on ? n : 0, b, t);
+        typename M::Rows rows = M::rows(place(S, hidden, b, t, on ? n : 0), c0, S.D, on);
+        const f32x4 dl = on ? d_logits[n * 4 + lane_g()] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (!on || target(S, tokens, b, t) < 0) M::clear(rows);
+        m.back(rows, dl, d_hidden + n * S.D, c0, S.D, on, sum);
+    }
+    if (c < S.V) {
+#pragma unroll
+        for (int k = 0; k < M::TILES; k++) *reinterpret_cast<f32x4*>(parts + (int64_t(blockIdx.y) * S.V + c) * S.Dp + c0 + 16 * k + 4 * lane_g()) = sum.dw[k];
+    }
+}
+
+// The mean loss (the last workgroup), and d_weight from the workgroups' parts: 64 columns a workgroup, a run of parts a wave
 template <typename W>
-__global__ __launch_bounds__(BLOCK) void loss_end_kernel(Shape S, const int64_t* counts, const double* sums, int nsums, float* loss, const float* parts, W* d_weight) {
-    if (blockIdx.x == 0 && loss) {
-        __shared__ int64_t ilds[ROWS];
-        __shared__ double dlds[ROWS];
-        const int64_t k = block_sum(counts[threadIdx.x], ilds);
+__global__ __launch_bounds__(END_WAVES* WAVE) void end_kernel(Shape S, const int64_t* counts, const double* sums, int nsums, float* loss, const float* __restrict__ parts,
+                                                              int nparts, W* __restrict__ d_weight) {
+    __shared__ double lds[END_WAVES][WAVE];
+    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+    if (loss && blockIdx.x == gridDim.x - 1) {
+        if (wave) return;
+        int64_t k = 0;
+        for (int j = lane; j < COUNTS; j += WAVE) k += counts[j];
+        k = wave_total(k);
         double s = 0.0;
-        for (int j = threadIdx.x; j < nsums; j += BLOCK) s += sums[j];
-        s = block_sum(s, dlds);
-        if (threadIdx.x == 0) *loss = float(s / double(k > 0 ? k : 1));
+        for (int j = lane; j < nsums; j += WAVE) s += sums[j];
+        s = wave_total(s);
+        if (lane == 0) *loss = float(s / double(k > 0 ? k : 1));
+        return;
     }
-    const int64_t i = int64_t(blockIdx.x) * BLOCK + threadIdx.x;
-    if (!d_weight || i >= S.V * S.D) return;
+    const int64_t e = int64_t(blockIdx.x) * WAVE + lane, size = S.V * S.Dp;
     float x = 0.0f;
-    for (int j = 0; j < SPLITS; j++) x += parts[j * int64_t(S.V) * S.D + i];
-    d_weight[i] = W(x);
+    if (e < size) {
+#pragma unroll 8
+        for (int p = wave; p < nparts; p += END_WAVES) x += parts[p * size + e];
+    }
+    float* part = reinterpret_cast<float*>(lds);
+    part[wave * WAVE + lane] = x;
+    __syncthreads();
+    if (wave || e >= size) return;
+#pragma unroll
+    for (int w = 1; w < END_WAVES; w++) x += part[w * WAVE + lane];
+    const int64_t v = e / S.Dp, i = e % S.Dp;
+    if (i < S.D) d_weight[v * S.D + i] = W(x);
 }
 
-constexpr int GRID = 2048;                 // workgroups of loss_place_kernel at most
+// How a call is cut up: columns of a slab, waves of a fused workgroup (0: the row has more slabs than that), workgroups
+struct Cut { int64_t Dp; int waves, groups; };
+Cut cut_of(int64_t N, int64_t D, bool narrow) {
+    const int64_t cols = narrow ? 128 : 64, slabs = (D + cols - 1) / cols, tiles = (N + TILE - 1) / TILE;
+    Cut k;
+    k.Dp = slabs * cols;
+    k.waves = slabs <= MOST_WAVES ? int(slabs) : 0;
+    const int64_t most = k.waves ? 256 * (MOST_WAVES / k.waves) : 256;      // 16 waves a CU
+    k.groups = int(tiles < most ? tiles : most);
+    return k;
+}
+constexpr int PLACE_GROUPS = 2048;
 
-struct Work { int64_t* counts; double* sums; float* d_logits; float* parts; };
-Work layout(void* work, int64_t N) {
+struct Work { int64_t* counts; double* sums; char *wr, *wc; float *d_logits, *parts; uint64_t bytes; };
+Work layout(void* work, int64_t N, int64_t D, int32_t V, bool narrow, bool gradients) {
+    const Cut k = cut_of(N, D, narrow);
+    const uint64_t e = narrow ? 2 : 4;
+    char* at = static_cast<char*>(work);
+    auto take = [&](uint64_t bytes) { char* p = at; at += (bytes + 15) & ~15ull; return p; };
     Work w;
-    w.counts = static_cast<int64_t*>(work);
-    w.sums = reinterpret_cast<double*>(w.counts + COUNTS);
-    w.d_logits = reinterpret_cast<float*>(w.sums + GRID);
-    w.parts = w.d_logits + N * VMAX;
+    w.counts = reinterpret_cast<int64_t*>(take(COUNTS * 8));
+    w.sums = reinterpret_cast<double*>(take((k.groups > PLACE_GROUPS ? k.groups : PLACE_GROUPS) * 8));
+    w.wr = take(VMAX * k.Dp * e);
+    w.wc = gradients ? take(VMAX * k.Dp * e) : nullptr;
+    w.d_logits = reinterpret_cast<float*>(gradients && !k.waves ? take(uint64_t(N) * VMAX * 4) : nullptr);
+    w.parts = reinterpret_cast<float*>(gradients ? take(uint64_t(k.groups) * V * k.Dp * 4) : nullptr);
+    w.bytes = uint64_t(at - static_cast<char*>(work));
     return w;
 }
 
-template <typename E, typename W, typename I>
-int32_t run(const Shape& S, const void* hidden, const void* weight, const void* tokens, const float* scale, const float* factor, float* each, float* loss,
-            void* d_hidden, void* d_weight, void* work, hipStream_t st, char* err, size_t errcap) {
-    const int64_t N = S.B * S.T;
-    const Work w = layout(work, N);
-    const int64_t need = (N + ROWS - 1) / ROWS;
-    const int grid = int(need < GRID ? need : GRID);
-    const I* tok = static_cast<const I*>(tokens);
-    const bool mean = loss || !factor;
-    static_assert(COUNTS == BLOCK, "one count a lane");
-    if (mean) loss_count_kernel<I><<<COUNTS, BLOCK, 0, st>>>(S, tok, w.counts);
-    loss_place_kernel<E, W, I><<<grid, BLOCK, 0, st>>>(S, static_cast<const E*>(hidden), static_cast<const W*>(weight), tok, mean ? w.counts : nullptr, scale,
-                                                       factor, each, static_cast<E*>(d_hidden), w.d_logits, w.sums);
-    if (d_weight)
-        loss_weight_kernel<E, I><<<dim3((S.D + WAVE - 1) / WAVE, SPLITS), WAVE, 0, st>>>(S, static_cast<const E*>(hidden), tok, w.d_logits, w.parts);
-    if (loss || d_weight)
-        loss_end_kernel<W><<<dim3(d_weight ? (S.V * S.D + BLOCK - 1) / BLOCK : 1), BLOCK, 0, st>>>(S, w.counts, w.sums, grid, loss, w.parts, static_cast<W*>(d_weight));
+template <typename M, typename W>
+int32_t run(Shape S, const void* hidden_, const void* weight, const void* tokens, const float* scale, const float* factor, float* each, float* loss, void* d_hidden_,
+            void* d_weight, void* work, hipStream_t st, char* err, size_t errcap) {
+    using E = typename M::E;
+    using K = typename M::K;
+    const bool narrow = sizeof(K) == 2, grads = d_hidden_;
+    const Work w = layout(work, S.N, S.D, S.V, narrow, grads);
+    const Cut k = cut_of(S.N, S.D, narrow);
+    S.Dp = k.Dp;
+    const E* hidden = static_cast<const E*>(hidden_);
+    E* d_hidden = static_cast<E*>(d_hidden_);
+    K *wr = reinterpret_cast<K*>(w.wr), *wc = reinterpret_cast<K*>(w.wc);
+    const bool mean = loss || (grads && !factor);
+    const int counting = mean ? COUNTS : 0;
+    begin_kernel<W, K><<<counting + (VMAX * k.Dp + BLOCK - 1) / BLOCK, BLOCK, 0, st>>>(S, tokens, counting, w.counts, static_cast<const W*>(weight), wr, wc);
+    const int64_t* counts = mean ? w.counts : nullptr;
+    int nsums = k.groups;
+    if (grads && k.waves) {
+        fused_kernel<M><<<k.groups, k.waves * WAVE, 2 * k.waves * WAVE * sizeof(f32x4), st>>>(S, hidden, tokens, wr, wc, counts, scale, factor, each, d_hidden, w.sums,
+                                                                                             w.parts);
+    } else {
+        const int64_t need = (S.N + TILE * (BLOCK / WAVE) - 1) / (TILE * (BLOCK / WAVE));
+        nsums = int(need < PLACE_GROUPS ? need : PLACE_GROUPS);
+        place_kernel<M><<<nsums, BLOCK, 0, st>>>(S, hidden, tokens, wr, counts, scale, factor, each, reinterpret_cast<f32x4*>(w.d_logits), w.sums);
+        if (grads)
+            grad_kernel<M><<<dim3((k.Dp + M::COLS * (BLOCK / WAVE) - 1) / (M::COLS * (BLOCK / WAVE)), k.groups), BLOCK, 0, st>>>(
+                S, hidden, tokens, wc, reinterpret_cast<const f32x4*>(w.d_logits), d_hidden, w.parts);
+    }
+    if (loss || grads)
+        end_kernel<W><<<(grads ? (S.V * k.Dp + WAVE - 1) / WAVE : 0) + (loss ? 1 : 0), END_WAVES * WAVE, 0, st>>>(S, w.counts, w.sums, nsums, loss, w.parts, k.groups,
+                                                                                                              static_cast<W*>(d_weight));
     return launched(err, errcap);
 }
 
@@ -174,9 +518,9 @@ int32_t run(const Shape& S, const void* hidden, const void* weight, const void* 
 extern "C" {
 
 uint64_t pv_next_base_loss_work_bytes(int64_t B, int64_t T, int64_t D, int32_t V, int32_t gradients) {
-    if (B <= 0 || T <= 0 || D <= 0 || V <= 0) return 0;
-    const uint64_t head = (COUNTS + GRID) * 8;
-    return gradients ? head + uint64_t(B) * T * VMAX * 4 + uint64_t(SPLITS) * V * D * 4 : head;
+    if (B <= 0 || T <= 0 || D <= 0 || V <= 0 || B > (int64_t(1) << 40) / T) return 0;
+    const uint64_t a = layout(nullptr, B * T, D, V, true, gradients).bytes, b = layout(nullptr, B * T, D, V, false, gradients).bytes;
+    return a > b ? a : b;
 }
 
 int32_t pv_next_base_loss_hip(const void* hidden, const void* weight, const void* tokens, int64_t B, int64_t T, int64_t D, int32_t V, int64_t hidden_b,
@@ -190,14 +534,21 @@ int32_t pv_next_base_loss_hip(const void* hidden, const void* weight, const void
     if (V < 1 || V > VMAX) return fail(PV_EARG, err, errcap, "V: 1 to 16 ids");
     if (!hidden || !weight || !tokens || !d_hidden != !d_weight) return fail(PV_EARG, err, errcap, "null argument");
     if (!work || work_bytes < pv_next_base_loss_work_bytes(B, T, D, V, d_hidden != nullptr)) return fail(PV_EARG, err, errcap, "work: too small");
-    const Shape S{B, T, D, hidden_b, hidden_t, tokens_b, ignore, V};
+    Shape S{B, T, D, B * T, hidden_b, hidden_t, tokens_b, ignore, 0, V, token_bytes, B == 1 || hidden_b == T * hidden_t};
+    const bool narrow = dtype == PV_BF16 && weight_dtype == PV_BF16;
+    const int64_t per = narrow ? 8 : 4, bytes = per * element_bytes(dtype);
+    const bool wide = D % per == 0 && (T == 1 || hidden_t % per == 0) && (B == 1 || hidden_b % per == 0) && aligned(hidden, bytes) && aligned(d_hidden, bytes);
+    const hipStream_t st = hipStream_t(stream);
+    if (narrow) {
+        if (wide) return run<Bf<bf16, true>, bf16>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, st, err, errcap);
+        return run<Bf<bf16, false>, bf16>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, st, err, errcap);
+    }
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
         auto go = [&](auto w) {
             using W = decltype(w);
-            if (token_bytes == 1)
-                return run<E, W, uint8_t>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, hipStream_t(stream), err, errcap);
-            return run<E, W, int64_t>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, hipStream_t(stream), err, errcap);
+            if (wide) return run<F3<E, true>, W>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, st, err, errcap);
+            return run<F3<E, false>, W>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, st, err, errcap);
         };
         return weight_dtype == PV_F32 ? go(float{}) : go(E{});
     });
