@@ -10,16 +10,21 @@ using namespace pvo;
 
 namespace {
 
-constexpr int GROUP = 120;                 // tensors of one launch: 28 bytes each of the 4 KiB that a launch's arguments may take
+constexpr int GROUP = 120;                 // tensors of one launch: 29 bytes each of the 4 KiB that a launch's arguments may take
 constexpr int BLOCK = 256;
-constexpr int64_t PIECE = 16384;           // elements of a workgroup
+// Bytes of a workgroup. Scaling: four loads of 16 bytes a lane (1 GiB read and written in 334 us; 370 with 64 KiB, 394 with 256).
+// The sum of squares: the same, or more, so that there are no more than MOST partial sums for one workgroup to add up (1 GiB
+// read in 154-166 us with any from 16 to 256 KiB).
+constexpr int64_t LINE = BLOCK * 16, PIECE = 4 * LINE, MOST = 4096;
 
 struct Group {
     const void* from[GROUP];
     void* to[GROUP];
     int64_t n[GROUP];
     uint32_t first[GROUP];                 // workgroup that begins a tensor
+    uint8_t dtype[GROUP];
     int32_t count;
+    int64_t piece;                         // bytes of a workgroup
 };
 static_assert(sizeof(Group) <= 3600, "a launch's arguments");
 
@@ -33,56 +38,123 @@ __device__ inline int tensor_of(const Group& G, uint32_t b) {
     return lo;
 }
 
-__device__ inline double block_sum(double x) {
-    __shared__ double lds[BLOCK / WAVE];
+template <int WAVES> __device__ inline double block_sum(double x) {
+    __shared__ double lds[WAVES];
 #pragma unroll
     for (int d = WAVE / 2; d; d >>= 1) x += __shfl_xor(x, d, WAVE);
     if (threadIdx.x % WAVE == 0) lds[threadIdx.x / WAVE] = x;
     __syncthreads();
     double sum = 0.0;
-    for (int w = 0; w < BLOCK / WAVE; w++) sum += lds[w];
+    for (int w = 0; w < WAVES; w++) sum += lds[w];
     return sum;
 }
 
-template <typename E> __global__ __launch_bounds__(BLOCK) void square_kernel(Group G, double* parts) {
-    const int k = tensor_of(G, blockIdx.x);
-    const E* g = static_cast<const E*>(G.from[k]);
-    const int64_t i0 = int64_t(blockIdx.x - G.first[k]) * PIECE, i1 = i0 + PIECE < G.n[k] ? i0 + PIECE : G.n[k];
-    double sum = 0.0;
-    for (int64_t i = i0 + threadIdx.x; i < i1; i += BLOCK) { const double x = double(float(g[i])); sum = fma(x, x, sum); }
-    sum = block_sum(sum);
-    if (threadIdx.x == 0) parts[blockIdx.x] = sum;
+// A workgroup's part of a tensor of type E: packs of 16 bytes from the first address that is a multiple of 16, and single
+// elements before (workgroup 0) and behind them (the last). f(i) and wide(i): element i, and the pack that begins there.
+template <typename E, typename F, typename G> __device__ inline void over_part(const E* p, int64_t n, int64_t part, int64_t piece, F&& f, G&& wide) {
+    constexpr int P = 16 / sizeof(E);
+    int64_t head = (-reinterpret_cast<uintptr_t>(p) & 15) / sizeof(E);
+    if (head > n) head = n;
+    const int64_t packs = (n - head) / P, per = piece / 16, i0 = part * per, i1 = i0 + per < packs ? i0 + per : packs;
+    int64_t i = i0 + threadIdx.x;
+    for (; i + 3 * BLOCK < i1; i += 4 * BLOCK) wide(std::integral_constant<int, 4>{}, head + i * P);
+    for (; i < i1; i += BLOCK) wide(std::integral_constant<int, 1>{}, head + i * P);
+    if (part == 0 && threadIdx.x < head) f(int64_t(threadIdx.x));
+    const int64_t tail = head + packs * P;
+    if (i0 + per >= packs && i0 <= packs && tail + threadIdx.x < n && (i0 < packs || part == 0)) f(tail + threadIdx.x);
 }
 
-__global__ __launch_bounds__(BLOCK) void norm_end_kernel(const double* parts, int64_t n, float* norm) {
+__global__ __launch_bounds__(BLOCK) void square_kernel(Group G, double* parts) {
+    const int k = tensor_of(G, blockIdx.x);
+    double sum[4] = {};
+    auto go = [&](auto e) {
+        using E = decltype(e);
+        const E* g = static_cast<const E*>(G.from[k]);
+        constexpr int P = 16 / sizeof(E);
+        over_part(g, G.n[k], blockIdx.x - G.first[k], G.piece,
+                  [&](int64_t i) { const double x = double(float(g[i])); sum[0] = fma(x, x, sum[0]); },
+                  [&](auto many, int64_t i) {
+                      constexpr int M = decltype(many)::value;
+                      pack<E, P> v[M];
+#pragma unroll
+                      for (int m = 0; m < M; m++) v[m] = pack<E, P>::load_once(g + i + int64_t(m) * BLOCK * P);
+#pragma unroll
+                      for (int m = 0; m < M; m++)
+#pragma unroll
+                          for (int j = 0; j < P; j++) { const double x = double(float(v[m].v[j])); sum[j % 4] = fma(x, x, sum[j % 4]); }
+                  });
+    };
+    if (G.dtype[k] == PV_F32) go(float{}); else if (G.dtype[k] == PV_BF16) go(bf16{}); else go(f16{});
+    const double all = block_sum<BLOCK / WAVE>((sum[0] + sum[1]) + (sum[2] + sum[3]));
+    if (threadIdx.x == 0) parts[blockIdx.x] = all;
+}
+
+constexpr int END = 1024;
+__global__ __launch_bounds__(END) void norm_end_kernel(const double* parts, int64_t n, float* norm) {
     double sum = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += BLOCK) sum += parts[i];
-    sum = block_sum(sum);
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < n; i += END) sum += parts[i];
+    sum = block_sum<END / WAVE>(sum);
     if (threadIdx.x == 0) *norm = float(sqrt(sum));
 }
 
-template <typename E> __global__ __launch_bounds__(BLOCK) void scale_kernel(Group G, const float* norm, float max_norm) {
+// Last workgroups first: what square_kernel read last may still be in the caches
+__global__ __launch_bounds__(BLOCK) void scale_kernel(Group G, const float* norm, float max_norm) {
     const float c = max_norm / (*norm + 1e-6f);
     const float factor = c > 1.0f ? 1.0f : c;          // (NaN stays)
-    const int k = tensor_of(G, blockIdx.x);
-    const E* g = static_cast<const E*>(G.from[k]);
-    E* o = static_cast<E*>(G.to[k]);
-    if (factor == 1.0f && g == o) return;
-    const int64_t i0 = int64_t(blockIdx.x - G.first[k]) * PIECE, i1 = i0 + PIECE < G.n[k] ? i0 + PIECE : G.n[k];
-    for (int64_t i = i0 + threadIdx.x; i < i1; i += BLOCK) o[i] = E(float(g[i]) * factor);
+    const uint32_t b = gridDim.x - 1 - blockIdx.x;
+    const int k = tensor_of(G, b);
+    if (factor == 1.0f && G.from[k] == G.to[k]) return;
+    auto go = [&](auto e) {
+        using E = decltype(e);
+        const E* g = static_cast<const E*>(G.from[k]);
+        E* o = static_cast<E*>(G.to[k]);
+        constexpr int P = 16 / sizeof(E);
+        auto one = [&](int64_t i) { o[i] = E(float(g[i]) * factor); };
+        auto packs = [&](auto many, int64_t i, auto&& store) {
+            constexpr int M = decltype(many)::value;
+            pack<E, P> v[M];
+#pragma unroll
+            for (int m = 0; m < M; m++) v[m] = pack<E, P>::load_once(g + i + int64_t(m) * BLOCK * P);
+#pragma unroll
+            for (int m = 0; m < M; m++) {
+#pragma unroll
+                for (int j = 0; j < P; j++) v[m].v[j] = E(float(v[m].v[j]) * factor);
+                store(v[m], o + i + int64_t(m) * BLOCK * P);
+            }
+        };
+        const bool alike = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(o)) & 15) == 0;      // both start a pack at the same elements
+        if (alike)
+            over_part(g, G.n[k], b - G.first[k], G.piece, one, [&](auto many, int64_t i) { packs(many, i, [](const pack<E, P>& v, E* to) { v.store_once(to); }); });
+        else
+            over_part(g, G.n[k], b - G.first[k], G.piece, one, [&](auto many, int64_t i) {
+                packs(many, i, [](const pack<E, P>& v, E* to) {
+#pragma unroll
+                    for (int j = 0; j < P; j++) to[j] = v.v[j];
+                });
+            });
+    };
+    if (G.dtype[k] == PV_F32) go(float{}); else if (G.dtype[k] == PV_BF16) go(bf16{}); else go(f16{});
 }
 
-uint64_t blocks_of(int64_t n) { return uint64_t((n + PIECE - 1) / PIECE); }
+int64_t piece_of(const int64_t* sizes, const int32_t* dtypes, int32_t count) {
+    int64_t bytes = 0;
+    for (int32_t i = 0; i < count; i++) if (sizes[i] > 0) bytes += sizes[i] * element_bytes(dtypes[i]);
+    const int64_t piece = (bytes / MOST + LINE - 1) / LINE * LINE;
+    return piece > PIECE ? piece : PIECE;
+}
+int64_t blocks_of(int64_t n, int32_t dtype, int64_t piece) { return (n * element_bytes(dtype) + piece - 1) / piece; }
 
-// Groups of up to GROUP tensors of one type, in order; f(group, workgroups, workgroups of the type's earlier groups)
-template <typename F> void groups(const void* const* from, void* const* to, const int64_t* n, const int32_t* dtypes, int32_t count, int32_t dtype, F&& f) {
+// f(group, its workgroups) for groups of up to GROUP tensors; `back`: the last first
+template <typename F> void groups(const void* const* from, void* const* to, const int64_t* n, const int32_t* dtypes, int32_t count, int64_t piece, bool back, F&& f) {
     Group G;
     G.count = 0;
-    uint64_t blocks = 0;
-    for (int32_t i = 0; i < count; i++) {
-        if (dtypes[i] != dtype || !n[i]) continue;
-        const uint64_t b = blocks_of(n[i]);
-        if (G.count == GROUP || (G.count && blocks + b > INT32_MAX)) {
+    G.piece = piece;
+    int64_t blocks = 0;
+    for (int32_t k = 0; k < count; k++) {
+        const int32_t i = back ? count - 1 - k : k;
+        if (!n[i]) continue;
+        if (G.count == GROUP) {
             f(G, uint32_t(blocks));
             G.count = 0;
             blocks = 0;
@@ -90,8 +162,9 @@ template <typename F> void groups(const void* const* from, void* const* to, cons
         G.from[G.count] = from[i];
         G.to[G.count] = to ? to[i] : nullptr;
         G.n[G.count] = n[i];
+        G.dtype[G.count] = uint8_t(dtypes[i]);
         G.first[G.count++] = uint32_t(blocks);
-        blocks += b;
+        blocks += blocks_of(n[i], dtypes[i], piece);
     }
     if (G.count) f(G, uint32_t(blocks));
 }
@@ -100,41 +173,37 @@ template <typename F> void groups(const void* const* from, void* const* to, cons
 
 extern "C" {
 
-uint64_t pv_gradient_norm_work_bytes(const int64_t* sizes, int32_t count) {
+uint64_t pv_gradient_norm_work_bytes(const int64_t* sizes, const int32_t* dtypes, int32_t count) {
+    if (!sizes || !dtypes) return 0;
+    const int64_t piece = piece_of(sizes, dtypes, count);
     uint64_t b = 0;
-    for (int32_t i = 0; sizes && i < count; i++) if (sizes[i] > 0) b += blocks_of(sizes[i]);
+    for (int32_t i = 0; i < count; i++) if (sizes[i] > 0) b += uint64_t(blocks_of(sizes[i], dtypes[i], piece));
     return b * 8;
 }
 
 int32_t pv_gradient_norm_hip(const void* const* grads, void* const* out, const int64_t* sizes, const int32_t* dtypes, int32_t count, float max_norm, float* norm,
                              void* work, uint64_t work_bytes, void* stream, char* err, size_t errcap) {
     if (count < 0 || !norm || (count && (!grads || !sizes || !dtypes))) return fail(PV_EARG, err, errcap, "null argument");
+    int64_t all = 0;
     for (int32_t i = 0; i < count; i++) {
         if (!element_bytes(dtypes[i])) return fail(PV_EARG, err, errcap, "dtype: one of PV_F32, PV_BF16, PV_F16");
-        if (sizes[i] < 0 || blocks_of(sizes[i]) > INT32_MAX) return fail(PV_EARG, err, errcap, "size: 0 to 2^45 elements");
+        if (sizes[i] < 0 || sizes[i] > (int64_t(1) << 40) || (all += sizes[i]) > (int64_t(1) << 40)) return fail(PV_EARG, err, errcap, "size: 0 to 2^40 elements in all");
         if (sizes[i] && (!grads[i] || (out && !out[i]))) return fail(PV_EARG, err, errcap, "null argument");
+        if (sizes[i] && (!aligned(grads[i], element_bytes(dtypes[i])) || (out && !aligned(out[i], element_bytes(dtypes[i]))))) return fail(PV_EARG, err, errcap, "address: not a multiple of the element's size");
     }
-    const uint64_t need = pv_gradient_norm_work_bytes(sizes, count);
+    const uint64_t need = pv_gradient_norm_work_bytes(sizes, dtypes, count);
     if (need && (!work || work_bytes < need)) return fail(PV_EARG, err, errcap, "work: too small");
     const hipStream_t st = hipStream_t(stream);
     double* parts = static_cast<double*>(work);
-    uint64_t done = 0;
-    for (int32_t dtype : {PV_F32, PV_BF16, PV_F16})
-        with_type(dtype, [&](auto e) {
-            groups(grads, nullptr, sizes, dtypes, count, dtype, [&](const Group& G, uint32_t blocks) {
-                square_kernel<decltype(e)><<<blocks, BLOCK, 0, st>>>(G, parts + done);
-                done += blocks;
-            });
-            return 0;
-        });
-    norm_end_kernel<<<1, BLOCK, 0, st>>>(parts, int64_t(done), norm);
+    const int64_t piece = piece_of(sizes, dtypes, count);
+    int64_t done = 0;
+    groups(grads, nullptr, sizes, dtypes, count, piece, false, [&](const Group& G, uint32_t blocks) {
+        square_kernel<<<blocks, BLOCK, 0, st>>>(G, parts + done);
+        done += blocks;
+    });
+    norm_end_kernel<<<1, END, 0, st>>>(parts, done, norm);
     if (out)
-        for (int32_t dtype : {PV_F32, PV_BF16, PV_F16})
-            with_type(dtype, [&](auto e) {
-                groups(grads, out, sizes, dtypes, count, dtype,
-                       [&](const Group& G, uint32_t blocks) { scale_kernel<decltype(e)><<<blocks, BLOCK, 0, st>>>(G, norm, max_norm); });
-                return 0;
-            });
+        groups(grads, out, sizes, dtypes, count, PIECE, true, [&](const Group& G, uint32_t blocks) { scale_kernel<<<blocks, BLOCK, 0, st>>>(G, norm, max_norm); });
     return launched(err, errcap);
 }
 

@@ -18,8 +18,8 @@ template <int BYTES> struct raw_of;
 template <> struct raw_of<1> { using type = uint8_t; };
 template <> struct raw_of<2> { using type = uint16_t; };
 template <> struct raw_of<4> { using type = uint32_t; };
-template <> struct raw_of<8> { using type = uint2; };
-template <> struct raw_of<16> { using type = uint4; };
+template <> struct raw_of<8> { using type = __attribute__((ext_vector_type(2))) uint32_t; };
+template <> struct raw_of<16> { using type = __attribute__((ext_vector_type(4))) uint32_t; };
 
 // N elements moved by one load or store of N * sizeof(T) bytes, which the address has to be a multiple of
 template <typename T, int N> struct pack {
@@ -27,6 +27,9 @@ template <typename T, int N> struct pack {
     union { raw bits; T v[N]; };
     __device__ static pack load(const T* p) { pack r; r.bits = *reinterpret_cast<const raw*>(p); return r; }
     __device__ void store(T* p) const { *reinterpret_cast<raw*>(p) = bits; }
+    // the same past the caches, for what is not used again soon
+    __device__ static pack load_once(const T* p) { pack r; r.bits = __builtin_nontemporal_load(reinterpret_cast<const raw*>(p)); return r; }
+    __device__ void store_once(T* p) const { __builtin_nontemporal_store(bits, reinterpret_cast<raw*>(p)); }
 };
 
 inline bool aligned(const void* p, uint64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }

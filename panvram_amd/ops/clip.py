@@ -1,6 +1,6 @@
 """The norm over many gradient tensors, and clipping to it (panvram_amd/csrc/pv_clip.hip)."""
-import ctypes
-import math
+from array import array
+from operator import attrgetter, eq
 
 import torch
 
@@ -20,18 +20,33 @@ def _dense(t):
     return True
 
 
-def _run(name, grads, max_norm, out):
-    index = on_gpu(name, *grads)
-    for g in grads:
-        need(g.dtype in DTYPES, f"{name}: gradients are float32, bfloat16 or float16, got {g.dtype}")
+_ptr, _numel, _whole, _gpu = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device
+_dtype, _shape = attrgetter("dtype"), attrgetter("shape")
+
+
+def _checked(name, grads):
+    """The GPU that all of `grads` are on; their types are ones that the kernels take. (Many tensors: one pass of a C-level
+    map for each thing that is asked, not a loop.)"""
+    if not all(issubclass(c, torch.Tensor) for c in set(map(type, grads))):
+        raise TypeError(f"{name}: tensors expected")
+    where = set(map(_gpu, grads))
+    if len(where) != 1 or -1 in where:
+        on_gpu(name, *grads)
+    need(set(map(_dtype, grads)) <= DTYPES.keys(), f"{name}: gradients are float32, bfloat16 or float16")
+    return where.pop()
+
+
+def _run(index, grads, max_norm, out):
+    """grads, out: each one run of memory, each pair's elements in the same order."""
     n = len(grads)
-    sizes = (ctypes.c_int64 * n)(*[g.numel() for g in grads])
-    types = (ctypes.c_int32 * n)(*[DTYPES[g.dtype] for g in grads])
-    src = (ctypes.c_void_p * n)(*[g.data_ptr() for g in grads])
-    dst = (ctypes.c_void_p * n)(*[o.data_ptr() for o in out]) if out is not None else None
+    sizes = array("q", map(_numel, grads))
+    types = array("i", map(DTYPES.__getitem__, map(_dtype, grads)))
+    src = array("Q", map(_ptr, grads))
+    dst = array("Q", map(_ptr, out)) if out is not None else None
+    at = [a.buffer_info()[0] if a is not None else None for a in (src, dst, sizes, types)]
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    work = torch.empty(N.lib().pv_gradient_norm_work_bytes(sizes, n), dtype=torch.uint8, device=norm.device)
-    call("pv_gradient_norm_hip", index, src, dst, sizes, types, n, max_norm, norm.data_ptr(), work.data_ptr(), work.numel())
+    work = torch.empty(N.lib().pv_gradient_norm_work_bytes(at[2], at[3], n), dtype=torch.uint8, device=norm.device)
+    call("pv_gradient_norm_hip", index, *at, n, max_norm, norm.data_ptr(), work.data_ptr(), work.numel())
     return norm
 
 
@@ -39,8 +54,13 @@ def _run(name, grads, max_norm, out):
 def gradient_norm(grads):
     """sqrt of the sum of all squares of all tensors in `grads` (on one GPU), as a float32 tensor of no dimensions. A NaN
     or an infinity anywhere shows in it; squares are summed in 64 bits."""
-    grads = [g if _dense(g) else g.contiguous() for g in grads]
-    return _run("gradient_norm", grads, 0.0, None) if grads else torch.zeros(())
+    grads = list(grads)
+    if not grads:
+        return torch.zeros(())
+    index = _checked("gradient_norm", grads)
+    if not all(map(_whole, grads)):
+        grads = [g if _dense(g) else g.contiguous() for g in grads]
+    return _run(index, grads, 0.0, None)
 
 
 @torch.no_grad()
@@ -51,27 +71,29 @@ def clip_gradients(grads, max_norm, out=None):
     read back: the factor is made and used on the GPU. If the norm is not finite, neither are the scaled gradients."""
     grads = list(grads)
     max_norm = float(max_norm)
-    need(max_norm >= 0 and not math.isnan(max_norm), f"clip_gradients: max_norm is not negative, got {max_norm}")
-    back = []
-    if out is None:
-        work = [g if _dense(g) else g.contiguous() for g in grads]
-        back = [(g, w) for g, w in zip(grads, work) if g is not w]
-        grads, out = work, work
-    else:
-        out = list(out)
-        need(len(out) == len(grads), f"clip_gradients: {len(grads)} gradients and {len(out)} tensors in out")
-        if grads:
-            on_gpu("clip_gradients", *grads, *out)
-        for i, (g, o) in enumerate(zip(grads, out)):
-            need(o.dtype == g.dtype and o.shape == g.shape, f"clip_gradients: out[{i}] is {o.dtype} {list(o.shape)}, its gradient {g.dtype} {list(g.shape)}")
-            if g.stride() != o.stride() or not _dense(g):
-                grads[i] = g = g.contiguous()
-                if not o.is_contiguous():
-                    out[i] = torch.empty_like(g)
-                    back.append((o, out[i]))
+    need(max_norm >= 0, f"clip_gradients: max_norm is not negative, got {max_norm}")
+    out = None if out is None else list(out)
+    need(out is None or len(out) == len(grads), f"clip_gradients: {len(grads)} gradients and {len(out or ())} tensors in out")
     if not grads:
         return torch.zeros(())
-    norm = _run("clip_gradients", grads, max_norm, out)
-    for to, made in back:
-        to.copy_(made)
+    index = _checked("clip_gradients", grads)
+    if out is not None:
+        need(_checked("clip_gradients", out) == index, "clip_gradients: grads and out on one GPU")
+        if not all(map(eq, map(_shape, grads), map(_shape, out))) or not all(map(eq, map(_dtype, grads), map(_dtype, out))):
+            i = next(i for i, (g, o) in enumerate(zip(grads, out)) if g.shape != o.shape or g.dtype != o.dtype)
+            raise ValueError(f"clip_gradients: out[{i}] is {out[i].dtype} {list(out[i].shape)}, its gradient {grads[i].dtype} {list(grads[i].shape)}")
+    back = []           # (tensor, what its values are made in) where memory is not one run, or in another order
+    if not all(map(_whole, grads)) or (out is not None and not all(map(_whole, out))):
+        to = grads if out is None else out
+        grads, out = list(grads), list(to)
+        for i, (g, o) in enumerate(zip(grads, to)):
+            if g.stride() != o.stride() or not _dense(g):
+                grads[i] = g.contiguous()
+                if o.is_contiguous():
+                    continue
+                out[i] = torch.empty_like(grads[i])
+                back.append((o, out[i]))
+    norm = _run(index, grads, max_norm, grads if out is None else out)
+    for o, made in back:
+        o.copy_(made)
     return norm
