@@ -27,31 +27,23 @@ struct Shape {
     int64_t chunks, tiles;                     // chunks of T, tiles of D
 };
 
-// z = sigmoid(g) and 1 - z, each to a few units in its last place: from exp(-|g|), so that neither is a difference
-__device__ inline void sigmoid2(float g, float& z, float& keep) {
+// z = sigmoid(g) and k = 1 - z of a step in one register: the smaller of the two, its sign bit set where that is z. It is made from
+// exp(-|g|), to a few units in its last place; the other is 1 minus it, at least a half and so as exact. -0: z = 0, k = 1.
+__device__ inline float gate_of(float g) {
     const float e = __expf(-fabsf(g));
-    const float r = __builtin_amdgcn_rcpf(1.0f + e);
-    const float s = e * r;
-    z = g >= 0.0f ? r : s;
-    keep = g >= 0.0f ? s : r;
+    return copysignf(e * __builtin_amdgcn_rcpf(1.0f + e), g);
+}
+__device__ inline void both(float q, float& z, float& k) {
+    const float a = fabsf(q), b = 1.0f - a;
+    const bool low = int32_t(__float_as_uint(q)) < 0;
+    z = low ? a : b;
+    k = low ? b : a;
 }
 
-template <int VEC> struct Map { float A[VEC], H[VEC]; };
-template <int VEC> __device__ inline Map<VEC> identity() {
-    Map<VEC> m;
-#pragma unroll
-    for (int v = 0; v < VEC; v++) { m.A[v] = 1.0f; m.H[v] = 0.0f; }
-    return m;
-}
-__device__ inline float apply(float A, float H, float before) { return A == CUT ? H : fmaf(A, before, H); }
-template <int VEC> __device__ inline Map<VEC> then(const Map<VEC>& first, const Map<VEC>& second) {
-    Map<VEC> m;
-#pragma unroll
-    for (int v = 0; v < VEC; v++) {
-        m.H[v] = apply(second.A[v], second.H[v], first.H[v]);
-        m.A[v] = first.A[v] == CUT || second.A[v] == CUT ? CUT : first.A[v] * second.A[v];
-    }
-    return m;
+struct Map { float A, H; };
+__device__ inline float apply(Map m, float before) { return m.A == CUT ? m.H : fmaf(m.A, before, m.H); }
+__device__ inline Map then(Map first, Map second) {
+    return {first.A == CUT || second.A == CUT ? CUT : first.A * second.A, apply(second, first.H)};
 }
 
 // ---- Maps of chunks, in the order of the walk (position 0 first), passed between workgroups.
@@ -81,45 +73,35 @@ __device__ inline uint64_t word_of(float A, float H) {
     const uint32_t a = A != A ? 0x7fc00000u : __float_as_uint(A), h = H != H ? 0x7fc00000u : __float_as_uint(H);
     return uint64_t(h) << 32 | a;
 }
-template <int VEC> __device__ inline void publish(uint64_t* at, const Map<VEC>& m, bool on) {
-    if (!on) return;
-#pragma unroll
-    for (int v = 0; v < VEC; v++) __hip_atomic_store(at + v, word_of(m.A[v], m.H[v]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ inline void publish(uint64_t* at, Map m, bool on) {
+    if (on) __hip_atomic_store(at, word_of(m.A, m.H), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// The map of all chunks before position p, for one wave's channels (from d on, where `on`); own: the chunk's map
-template <int VEC> __device__ inline Map<VEC> before_chunk(const Records& R, const Shape& S, int64_t b, int64_t p, int64_t d, bool on, Map<VEC> own) {
-    Map<VEC> all = identity<VEC>();
+// The map of all chunks before position p, for the lane's channel d (where `on`); own: the chunk's map
+__device__ inline Map before_chunk(const Records& R, const Shape& S, int64_t b, int64_t p, int64_t d, bool on, Map own) {
+    Map all = {1.0f, 0.0f};
     int64_t n = S.chunks;
     bool whole = true;                     // own is the map of a whole group of this level
     for (int l = 0; l < LEVELS && n > 0; l++, n /= FAN) {
         const int64_t at = p & ~int64_t(FAN - 1);      // the group's first
         const int many = int(p - at);
         uint64_t* rec = R.level[l] + b * n * S.D + d;
-        if (whole) publish<VEC>(rec + p * S.D, own, on);
-        uint64_t w[FAN - 1][VEC];
+        if (whole) publish(rec + p * S.D, own, on);
+        uint64_t w[FAN - 1];
 #pragma unroll
-        for (int i = 0; i < FAN - 1; i++)
-#pragma unroll
-            for (int v = 0; v < VEC; v++) {
-                w[i][v] = 0;
-                if (i < many && on) w[i][v] = __hip_atomic_load(rec + (at + i) * S.D + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-        Map<VEC> level = identity<VEC>();
+        for (int i = 0; i < FAN - 1; i++) {
+            w[i] = 0;
+            if (i < many && on) w[i] = __hip_atomic_load(rec + (at + i) * S.D, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        Map level = {1.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < FAN - 1; i++) {
             if (i >= many) break;
-            Map<VEC> m;
-#pragma unroll
-            for (int v = 0; v < VEC; v++) {
-                for (int k = 0; __any(w[i][v] == EMPTY) && k < POLLS; k++) {
-                    __builtin_amdgcn_s_sleep(1);
-                    if (on) w[i][v] = __hip_atomic_load(rec + (at + i) * S.D + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                }
-                m.A[v] = __uint_as_float(uint32_t(w[i][v]));
-                m.H[v] = __uint_as_float(uint32_t(w[i][v] >> 32));
+            for (int k = 0; __any(w[i] == EMPTY) && k < POLLS; k++) {
+                __builtin_amdgcn_s_sleep(1);
+                if (on) w[i] = __hip_atomic_load(rec + (at + i) * S.D, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
-            level = then(level, m);
+            level = then(level, {__uint_as_float(uint32_t(w[i])), __uint_as_float(uint32_t(w[i] >> 32))});
         }
         all = then(level, all);
         whole = whole && many == FAN - 1;
@@ -132,7 +114,6 @@ template <int VEC> __device__ inline Map<VEC> before_chunk(const Records& R, con
 // ---- What a workgroup works on: channels d.. of sequence b, position p of the walk
 template <int VEC, int WAVES, bool ONE> struct Place {
     int64_t b, p, d0, d;                   // d: the lane's first channel, d0: the wave's
-    uint32_t at;                           // d - d0
     int wave, lane;
     bool on;
     __device__ Place(const Shape& S, const Records& R) {
@@ -146,12 +127,12 @@ template <int VEC, int WAVES, bool ONE> struct Place {
             turn = __builtin_amdgcn_readfirstlane(given);
         }
         const uint32_t rows = uint32_t(S.B * S.tiles);
-        p = turn / rows;
-        const uint32_t rest = turn % rows;
-        b = rest / uint32_t(S.tiles);
-        d0 = int64_t(rest % uint32_t(S.tiles)) * (WAVE * VEC);
-        at = uint32_t(lane * VEC);
-        d = d0 + at;
+        const uint32_t q = __builtin_amdgcn_readfirstlane(turn / rows), rest = turn - q * rows;
+        const uint32_t c = __builtin_amdgcn_readfirstlane(rest / uint32_t(S.tiles));
+        p = q;
+        b = c;
+        d0 = int64_t(rest - c * uint32_t(S.tiles)) * (WAVE * VEC);
+        d = d0 + lane * VEC;
         on = d < S.D;
     }
 };
@@ -168,197 +149,264 @@ __device__ inline Span span_of(const Shape& S, const uint8_t* reset, int64_t b, 
     return s;
 }
 // (from is the same for the wave, at: the lane's channel in it)
-template <typename E, int VEC> __device__ inline void load_steps(pack<E, VEC>* to, const E* from, int64_t stride, const Span& s, uint32_t at, bool on) {
-    from += s.t0 * stride;
-#pragma unroll
-    for (int i = 0; i < STEPS; i++) {
-        if (on && i < s.steps) to[i] = pack<E, VEC>::load(from + i * stride + at);
-        else
-#pragma unroll
-            for (int v = 0; v < VEC; v++) to[i].v[v] = E(0.0f);
+// A wave's steps of a tensor as a buffer of its rows: step i is at i * stride bytes, and what lies behind the span (or at NO_LANE)
+// is not read and not written, so that neither the end of T nor that of D needs a branch.
+constexpr uint32_t NO_LANE = 1u << 31;
+constexpr int64_t MOST_STRIDE = 1 << 26;   // bytes: a span's offsets stay below 2^30
+struct Rows {
+    __amdgpu_buffer_rsrc_t buffer;
+    int stride;
+    template <typename E> __device__ Rows(const E* from, int64_t step, const Span& s, int64_t channels) {
+        stride = int(step * int64_t(sizeof(E)));
+        const int bytes = s.steps ? (s.steps - 1) * stride + int(channels * int64_t(sizeof(E))) : 0;
+        buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(from + s.t0 * step), 0, bytes, 0x00027000);
     }
+    template <typename P> __device__ P load(int i, uint32_t at) const {
+        P r;
+        if constexpr (sizeof(P) == 4) r.bits = __builtin_amdgcn_raw_buffer_load_b32(buffer, at, i * stride, 0);
+        else r.bits = __builtin_amdgcn_raw_buffer_load_b16(buffer, at, i * stride, 0);
+        return r;
+    }
+    template <typename P> __device__ void store(const P& v, int i, uint32_t at) const {
+        if constexpr (sizeof(P) == 4) __builtin_amdgcn_raw_buffer_store_b32(v.bits, buffer, at, i * stride, 0);
+        else __builtin_amdgcn_raw_buffer_store_b16(v.bits, buffer, at, i * stride, 0);
+    }
+};
+template <typename P> __device__ inline void load_steps(P* to, const Rows& rows, uint32_t at) {
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) to[i] = rows.load<P>(i, at);
 }
-
-template <typename E, int VEC, int WAVES, bool ONE>
-__global__ __launch_bounds__(WAVES* WAVE) void scan_kernel(Shape S, Records R, const E* __restrict__ gate, const E* __restrict__ value,
-                                                           const float* __restrict__ state, const uint8_t* __restrict__ reset, E* __restrict__ out,
-                                                           float* __restrict__ last, float* __restrict__ carry) {
-    __shared__ Map<VEC> maps[WAVES][WAVE];
-    __shared__ float starts[VEC][WAVE];
-    const Place<VEC, WAVES, ONE> P(S, R);
-    const Span s = span_of(S, reset, P.b, (P.p * WAVES + P.wave) * STEPS, P.lane);
-    pack<E, VEC> g[STEPS], x[STEPS];
-    load_steps<E, VEC>(g, gate + P.b * S.gb + P.d0, S.gt, s, P.at, P.on);
-    load_steps<E, VEC>(x, value + P.b * S.vb + P.d0, S.vt, s, P.at, P.on);
-    float K[STEPS][VEC], X[STEPS][VEC];
-    Map<VEC> m = identity<VEC>();
+// Behind the end: gates that leave the state as it is (z = 0), zeros in the other tensors. (A buffer's zeros are no such thing
+// for the gates, and are not there where all steps are one and the same row, stride 0.)
+template <typename E, int VEC> __device__ inline void end_steps(pack<E, VEC>* x, const Span& s, float rest) {
+    if (s.steps == STEPS) return;
 #pragma unroll
     for (int i = 0; i < STEPS; i++)
 #pragma unroll
-        for (int v = 0; v < VEC; v++) {
-            float z;
-            sigmoid2(float(g[i].v[v]), z, K[i][v]);
-            X[i][v] = z * float(x[i].v[v]);
-            if (i >= s.steps) { K[i][v] = 1.0f; X[i][v] = 0.0f; }
-            m.A[v] *= K[i][v];
-            m.H[v] = s.cuts >> i & 1 ? X[i][v] : fmaf(K[i][v], m.H[v], X[i][v]);
-        }
-    if (s.cuts)
+        for (int v = 0; v < VEC; v++) if (i >= s.steps) x[i].v[v] = E(rest);
+}
+// The compiler is to make what follows from these registers again where it needs it: kept from one walk over the steps to the
+// next, z, 1 - z and the products would take two to four times the registers
+template <int VEC> __device__ inline void anew(float (*q)[VEC]) {
 #pragma unroll
-        for (int v = 0; v < VEC; v++) m.A[v] = CUT;
-    if constexpr (WAVES > 1) {
-        maps[P.wave][P.lane] = m;
-        __syncthreads();
-    }
-    float h[VEC];
-    if (ONE || P.wave == 0) {
+    for (int i = 0; i < STEPS; i++)
 #pragma unroll
-        for (int v = 0; v < VEC; v++) h[v] = state && P.on ? state[P.b * S.D + P.d + v] : 0.0f;
-    }
-    if (P.wave == 0) {
-        if constexpr (!ONE) {
-            Map<VEC> own = m;
-#pragma unroll
-            for (int w = 1; w < WAVES; w++) own = then(own, maps[w][P.lane]);
-            const Map<VEC> b = before_chunk<VEC>(R, S, P.b, P.p, P.d, P.on, own);
-#pragma unroll
-            for (int v = 0; v < VEC; v++) starts[v][P.lane] = h[v] = apply(b.A[v], b.H[v], h[v]);
-        }
-        if (carry && P.on)
-#pragma unroll
-            for (int v = 0; v < VEC; v++) carry[(P.b * S.chunks + P.p) * S.D + P.d + v] = h[v];
-    }
-    if constexpr (!ONE) {
-        __syncthreads();
-#pragma unroll
-        for (int v = 0; v < VEC; v++) h[v] = starts[v][P.lane];
-    }
-    for (int w = 0; w < P.wave; w++)
-#pragma unroll
-        for (int v = 0; v < VEC; v++) h[v] = apply(maps[w][P.lane].A[v], maps[w][P.lane].H[v], h[v]);
-    E* to = out + (P.b * S.T + s.t0) * S.D + P.d0;
+        for (int v = 0; v < VEC; v++) asm volatile("" : "+v"(q[i][v]));
+}
+template <typename E, int VEC> __device__ inline void anew(pack<E, VEC>* x) {
 #pragma unroll
     for (int i = 0; i < STEPS; i++) {
+        uint32_t w = x[i].bits;
+        asm volatile("" : "+v"(w));
+        x[i].bits = typename pack<E, VEC>::raw(w);
+    }
+}
+// f(i, whether step i has a reset) over the steps in order or backwards
+template <bool RESET, bool BACK, typename F> __device__ inline void over_steps(const Span& s, F&& f) {
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) { const int k = BACK ? STEPS - 1 - i : i; f(k, RESET && (s.cuts >> k & 1)); }
+}
+
+// The waves' maps of a chunk, by channel
+template <int VEC, int WAVES> struct Maps {
+    pack<float, VEC> A[WAVES][WAVE], H[WAVES][WAVE];
+    __device__ void put(int wave, int lane, const Map* m) {
+#pragma unroll
+        for (int v = 0; v < VEC; v++) { A[wave][lane].v[v] = m[v].A; H[wave][lane].v[v] = m[v].H; }
+    }
+    __device__ Map get(int wave, int channel) const { return {A[wave][0].v[channel], H[wave][0].v[channel]}; }
+};
+
+template <typename E, int VEC, int WAVES, bool ONE, bool RESET>
+__global__ __launch_bounds__(WAVES* WAVE) void scan_kernel(Shape S, Records R, const E* __restrict__ gate, const E* __restrict__ value,
+                                                           const float* __restrict__ state, const uint8_t* __restrict__ reset, E* __restrict__ out,
+                                                           float* __restrict__ last, float* __restrict__ carry) {
+    __shared__ Maps<VEC, WAVES> maps;
+    __shared__ pack<float, VEC> starts[WAVE];
+    const Place<VEC, WAVES, ONE> P(S, R);
+    const Span s = span_of(S, reset, P.b, (P.p * WAVES + P.wave) * STEPS, P.lane);
+    const uint32_t at = P.on ? P.lane * VEC * sizeof(E) : NO_LANE;
+    const int64_t width = S.D - P.d0 < WAVE * VEC ? S.D - P.d0 : WAVE * VEC;
+    pack<E, VEC> g[STEPS], x[STEPS];
+    load_steps(g, Rows(gate + P.b * S.gb + P.d0, S.gt, s, width), at);
+    load_steps(x, Rows(value + P.b * S.vb + P.d0, S.vt, s, width), at);
+    end_steps<E, VEC>(g, s, -INFINITY);
+    end_steps<E, VEC>(x, s, 0.0f);
+    float Z[STEPS][VEC], h[VEC];
+    if constexpr (WAVES > 1) {
+        Map m[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; v++) m[v] = {1.0f, 0.0f};
+        over_steps<RESET, false>(s, [&](int i, bool cut) {
+#pragma unroll
+            for (int v = 0; v < VEC; v++) {
+                Z[i][v] = gate_of(float(g[i].v[v]));
+                float z, k;
+                both(Z[i][v], z, k);
+                const float in = z * float(x[i].v[v]);
+                m[v].A *= k;
+                m[v].H = cut ? in : fmaf(k, m[v].H, in);
+            }
+        });
+        if (RESET && s.cuts)
+#pragma unroll
+            for (int v = 0; v < VEC; v++) m[v].A = CUT;
+        maps.put(P.wave, P.lane, m);
+        __syncthreads();
+        anew<VEC>(Z);
+        anew<E, VEC>(x);
+    } else {
+        over_steps<RESET, false>(s, [&](int i, bool) {
+#pragma unroll
+            for (int v = 0; v < VEC; v++) Z[i][v] = gate_of(float(g[i].v[v]));
+        });
+    }
+    if constexpr (ONE) {
+#pragma unroll
+        for (int v = 0; v < VEC; v++) h[v] = state && P.on ? state[P.b * S.D + P.d + v] : 0.0f;
+        if (carry && P.on && P.wave == 0)
+#pragma unroll
+            for (int v = 0; v < VEC; v++) carry[P.b * S.D + P.d + v] = h[v];
+    } else {
+        if (P.wave < VEC) {                // 64 of the workgroup's channels each
+            const int c = P.wave * WAVE + P.lane;
+            const int64_t d = P.d0 + c;
+            const bool on = d < S.D;
+            const float first = state && on ? state[P.b * S.D + d] : 0.0f;
+            Map own = maps.get(0, c);
+#pragma unroll
+            for (int w = 1; w < WAVES; w++) own = then(own, maps.get(w, c));
+            const float start = apply(before_chunk(R, S, P.b, P.p, d, on, own), first);
+            starts[0].v[c] = start;
+            if (carry && on) carry[(P.b * S.chunks + P.p) * S.D + d] = start;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < VEC; v++) h[v] = starts[P.lane].v[v];
+    }
+    if constexpr (WAVES > 1)
+        for (int w = 0; w < P.wave; w++)
+#pragma unroll
+            for (int v = 0; v < VEC; v++) h[v] = apply(maps.get(w, P.lane * VEC + v), h[v]);
+    const Rows to(out + P.b * S.T * S.D + P.d0, S.D, s, width);
+    over_steps<RESET, false>(s, [&](int i, bool cut) {
         pack<E, VEC> o;
 #pragma unroll
         for (int v = 0; v < VEC; v++) {
-            h[v] = s.cuts >> i & 1 ? X[i][v] : fmaf(K[i][v], h[v], X[i][v]);
+            float z, k;
+            both(Z[i][v], z, k);
+            const float in = z * float(x[i].v[v]);
+            h[v] = cut ? in : fmaf(k, h[v], in);
             o.v[v] = E(h[v]);
         }
-        if (P.on && i < s.steps) o.store(to + i * S.D + P.at);
-    }
+        to.store(o, i, at);
+    });
     if (P.on && s.steps && s.t0 + s.steps == S.T)
 #pragma unroll
         for (int v = 0; v < VEC; v++) last[P.b * S.D + P.d + v] = h[v];
 }
 
-template <typename E, int VEC, int WAVES, bool ONE>
+template <typename E, int VEC, int WAVES, bool ONE, bool RESET>
 __global__ __launch_bounds__(WAVES* WAVE) void scan_back_kernel(Shape S, Records R, const E* __restrict__ gate, const E* __restrict__ value,
                                                                 const uint8_t* __restrict__ reset, const float* __restrict__ carry,
                                                                 const E* __restrict__ d_out, const float* __restrict__ d_last, E* __restrict__ d_gate,
                                                                 E* __restrict__ d_value, float* __restrict__ d_state) {
-    __shared__ Map<VEC> maps[WAVES][WAVE];             // forwards: (A, H); backwards: (A, flows)
-    __shared__ float flows[WAVES][VEC][WAVE], ends[VEC][WAVE];
+    __shared__ Maps<VEC, WAVES> maps;                  // forwards: (A, H)
+    __shared__ pack<float, VEC> flows[WAVES][WAVE];    // backwards: (A, flows)
+    __shared__ pack<float, VEC> ends[WAVE];
     const Place<VEC, WAVES, ONE> P(S, R);
     const int64_t c = S.chunks - 1 - P.p;              // the walk begins at the last chunk
     const Span s = span_of(S, reset, P.b, (c * WAVES + P.wave) * STEPS, P.lane);
+    const uint32_t at = P.on ? P.lane * VEC * sizeof(E) : NO_LANE;
+    const int64_t width = S.D - P.d0 < WAVE * VEC ? S.D - P.d0 : WAVE * VEC;
     pack<E, VEC> g[STEPS], x[STEPS], y[STEPS];
-    load_steps<E, VEC>(g, gate + P.b * S.gb + P.d0, S.gt, s, P.at, P.on);
-    load_steps<E, VEC>(x, value + P.b * S.vb + P.d0, S.vt, s, P.at, P.on);
-    load_steps<E, VEC>(y, d_out + P.b * S.db + P.d0, S.dt, s, P.at, P.on);
-    // z and 1 - z of a step in one register: the smaller of the two, its sign bit set where that is z. The other is 1 minus it,
-    // at least a half and so as exact.
-    float Z[STEPS][VEC];
-    auto both = [&](float q, float& z, float& k) {
-        const float a = fabsf(q), b = 1.0f - a;
-        const bool low = int32_t(__float_as_uint(q)) < 0;
-        z = low ? a : b;
-        k = low ? b : a;
-    };
-    Map<VEC> m = identity<VEC>();
+    load_steps(g, Rows(gate + P.b * S.gb + P.d0, S.gt, s, width), at);
+    load_steps(x, Rows(value + P.b * S.vb + P.d0, S.vt, s, width), at);
+    load_steps(y, Rows(d_out + P.b * S.db + P.d0, S.dt, s, width), at);
+    end_steps<E, VEC>(g, s, -INFINITY);
+    end_steps<E, VEC>(x, s, 0.0f);
+    end_steps<E, VEC>(y, s, 0.0f);
+    float Z[STEPS][VEC], C[VEC], h[VEC];
+    over_steps<RESET, false>(s, [&](int i, bool) {
 #pragma unroll
-    for (int i = 0; i < STEPS; i++)
-#pragma unroll
-        for (int v = 0; v < VEC; v++) {
-            const float a = float(g[i].v[v]), e = __expf(-fabsf(a));
-            const float q = i < s.steps ? copysignf(e * __builtin_amdgcn_rcpf(1.0f + e), a) : -0.0f;
-            Z[i][v] = q;
-            float z, k;
-            both(q, z, k);
-            const float in = z * float(x[i].v[v]);
-            m.A[v] *= k;
-            m.H[v] = s.cuts >> i & 1 ? in : fmaf(k, m.H[v], in);
-        }
-    float C[VEC] = {};
-#pragma unroll
-    for (int i = STEPS - 1; i >= 0; i--)
-#pragma unroll
-        for (int v = 0; v < VEC; v++) {
-            float z, k;
-            both(Z[i][v], z, k);
-            C[v] = s.cuts >> i & 1 ? 0.0f : k * (float(y[i].v[v]) + C[v]);
-        }
-    if (s.cuts)
-#pragma unroll
-        for (int v = 0; v < VEC; v++) m.A[v] = CUT;
-    if constexpr (WAVES > 1) {
-        maps[P.wave][P.lane] = m;
-#pragma unroll
-        for (int v = 0; v < VEC; v++) flows[P.wave][v][P.lane] = C[v];
-        __syncthreads();
-    }
-    float end[VEC];
-    if (ONE || P.wave == 0) {
-#pragma unroll
-        for (int v = 0; v < VEC; v++) end[v] = d_last && P.on ? d_last[P.b * S.D + P.d + v] : 0.0f;
-    }
-    if constexpr (!ONE) {
-        if (P.wave == 0) {
-            Map<VEC> own = identity<VEC>();
-#pragma unroll
-            for (int w = WAVES - 1; w >= 0; w--) {
-                Map<VEC> k = maps[w][P.lane];
-#pragma unroll
-                for (int v = 0; v < VEC; v++) k.H[v] = flows[w][v][P.lane];
-                own = then(own, k);
-            }
-            const Map<VEC> b = before_chunk<VEC>(R, S, P.b, P.p, P.d, P.on, own);
-#pragma unroll
-            for (int v = 0; v < VEC; v++) ends[v][P.lane] = apply(b.A[v], b.H[v], end[v]);
-        }
-    }
-    // value minus the state before each step
-    float h[VEC], U[STEPS][VEC];
+        for (int v = 0; v < VEC; v++) Z[i][v] = gate_of(float(g[i].v[v]));
+    });
 #pragma unroll
     for (int v = 0; v < VEC; v++) h[v] = P.on ? carry[(P.b * S.chunks + c) * S.D + P.d + v] : 0.0f;
-    for (int w = 0; w < P.wave; w++)
+    if constexpr (WAVES > 1) {
+        Map m[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; v++) h[v] = apply(maps[w][P.lane].A[v], maps[w][P.lane].H[v], h[v]);
+        for (int v = 0; v < VEC; v++) { m[v] = {1.0f, 0.0f}; C[v] = 0.0f; }
+        over_steps<RESET, false>(s, [&](int i, bool cut) {
 #pragma unroll
-    for (int i = 0; i < STEPS; i++)
+            for (int v = 0; v < VEC; v++) {
+                float z, k;
+                both(Z[i][v], z, k);
+                const float in = z * float(x[i].v[v]);
+                m[v].A *= k;
+                m[v].H = cut ? in : fmaf(k, m[v].H, in);
+            }
+        });
+        anew<VEC>(Z);
+        over_steps<RESET, true>(s, [&](int i, bool cut) {
+#pragma unroll
+            for (int v = 0; v < VEC; v++) {
+                float z, k;
+                both(Z[i][v], z, k);
+                C[v] = cut ? 0.0f : k * (float(y[i].v[v]) + C[v]);
+            }
+        });
+        if (RESET && s.cuts)
+#pragma unroll
+            for (int v = 0; v < VEC; v++) m[v].A = CUT;
+        maps.put(P.wave, P.lane, m);
+#pragma unroll
+        for (int v = 0; v < VEC; v++) flows[P.wave][P.lane].v[v] = C[v];
+        __syncthreads();
+        for (int w = 0; w < P.wave; w++)
+#pragma unroll
+            for (int v = 0; v < VEC; v++) h[v] = apply(maps.get(w, P.lane * VEC + v), h[v]);
+        anew<VEC>(Z);
+        anew<E, VEC>(x);
+        anew<E, VEC>(y);
+    }
+    if constexpr (ONE) {
+#pragma unroll
+        for (int v = 0; v < VEC; v++) C[v] = d_last && P.on ? d_last[P.b * S.D + P.d + v] : 0.0f;
+    } else if (P.wave < VEC) {
+        const int k = P.wave * WAVE + P.lane;
+        const int64_t d = P.d0 + k;
+        const bool on = d < S.D;
+        const float first = d_last && on ? d_last[P.b * S.D + d] : 0.0f;
+        Map own = {1.0f, 0.0f};
+#pragma unroll
+        for (int w = WAVES - 1; w >= 0; w--) own = then(own, {maps.get(w, k).A, flows[w][0].v[k]});
+        ends[0].v[k] = apply(before_chunk(R, S, P.b, P.p, d, on, own), first);
+    }
+    float U[STEPS][VEC];                   // value minus the state before each step
+    over_steps<RESET, false>(s, [&](int i, bool cut) {
 #pragma unroll
         for (int v = 0; v < VEC; v++) {
             float z, k;
             both(Z[i][v], z, k);
-            if (s.cuts >> i & 1) h[v] = 0.0f;
+            if (cut) h[v] = 0.0f;
             const float a = float(x[i].v[v]);
             U[i][v] = a - h[v];
             h[v] = fmaf(k, h[v], z * a);
         }
+    });
     if constexpr (!ONE) {
         __syncthreads();
 #pragma unroll
-        for (int v = 0; v < VEC; v++) end[v] = ends[v][P.lane];
+        for (int v = 0; v < VEC; v++) C[v] = ends[P.lane].v[v];
     }
+    if constexpr (WAVES > 1)
+        for (int w = WAVES - 1; w > P.wave; w--)
 #pragma unroll
-    for (int v = 0; v < VEC; v++) C[v] = end[v];
-    for (int w = WAVES - 1; w > P.wave; w--)
-#pragma unroll
-        for (int v = 0; v < VEC; v++) C[v] = apply(maps[w][P.lane].A[v], flows[w][v][P.lane], C[v]);
-    E* const to_gate = d_gate + (P.b * S.T + s.t0) * S.D + P.d0;
-    E* const to_value = d_value + (P.b * S.T + s.t0) * S.D + P.d0;
-#pragma unroll
-    for (int i = STEPS - 1; i >= 0; i--) {
+            for (int v = 0; v < VEC; v++) C[v] = apply({maps.get(w, P.lane * VEC + v).A, flows[w][P.lane].v[v]}, C[v]);
+    anew<VEC>(Z);
+    const Rows to_gate(d_gate + P.b * S.T * S.D + P.d0, S.D, s, width), to_value(d_value + P.b * S.T * S.D + P.d0, S.D, s, width);
+    over_steps<RESET, true>(s, [&](int i, bool cut) {
         pack<E, VEC> og, ov;
 #pragma unroll
         for (int v = 0; v < VEC; v++) {
@@ -367,13 +415,11 @@ __global__ __launch_bounds__(WAVES* WAVE) void scan_back_kernel(Shape S, Records
             const float G = float(y[i].v[v]) + C[v], in = z * G;
             ov.v[v] = E(in);
             og.v[v] = E(in * k * U[i][v]);
-            C[v] = s.cuts >> i & 1 ? 0.0f : k * G;
+            C[v] = cut ? 0.0f : k * G;
         }
-        if (P.on && i < s.steps) {
-            ov.store(to_value + i * S.D + P.at);
-            og.store(to_gate + i * S.D + P.at);
-        }
-    }
+        to_value.store(ov, i, at);
+        to_gate.store(og, i, at);
+    });
     if (d_state && P.on && c == 0 && P.wave == 0)
 #pragma unroll
         for (int v = 0; v < VEC; v++) d_state[P.b * S.D + P.d + v] = C[v];
@@ -391,19 +437,20 @@ int64_t words_of(int64_t B, int64_t chunks, int64_t D) {
 }
 
 // What both entries ask of their arguments
-int32_t check(int64_t B, int64_t T, int64_t D, int32_t dtype, const void* work, uint64_t work_bytes, char* err, size_t cap) {
+template <typename... I> int32_t check(int64_t B, int64_t T, int64_t D, int32_t dtype, const void* work, uint64_t work_bytes, char* err, size_t cap, I... steps) {
     if (!element_bytes(dtype)) return fail(PV_EARG, err, cap, "dtype: one of PV_F32, PV_BF16, PV_F16");
     if (B < 0 || T < 1 || D < 0) return fail(PV_EARG, err, cap, "shape: B >= 0, T >= 1, D >= 0");
     const int64_t most = int64_t(1) << 40;
     if (B > INT32_MAX || T > INT32_MAX || D > INT32_MAX || (B && D && (B * D > most || T > most / (B * D)))) return fail(PV_EARG, err, cap, "shape: B T D of 2^40 at most");
     if (B && D && B * chunks_of(T) * ((D + WAVE - 1) / WAVE) > INT32_MAX) return fail(PV_EARG, err, cap, "shape: too many chunks");
+    for (int64_t st : {steps...}) if (T > 1 && (st < 0 || st * element_bytes(dtype) > MOST_STRIDE)) return fail(PV_EARG, err, cap, "stride: a step's is 0 to 2^26 bytes");
     const uint64_t need = pv_gated_scan_work_bytes(B, T, D);
     if (need && (!work || work_bytes < need || !aligned(work, 16))) return fail(PV_EARG, err, cap, "work: too small, or not 16-byte aligned");
     return PV_OK;
 }
 
-// f(vector of channels, waves, one chunk only) with the records cleared
-template <typename F> int32_t launch(Shape& S, bool pairs, void* work, hipStream_t st, F&& f) {
+// f(channels of a lane, waves, one chunk only, resets) with the records cleared
+template <typename F> int32_t launch(Shape& S, bool pairs, bool resets, void* work, hipStream_t st, F&& f) {
     const int vec = pairs ? 2 : 1;
     S.chunks = chunks_of(S.T);
     S.tiles = (S.D + WAVE * vec - 1) / (WAVE * vec);
@@ -419,12 +466,13 @@ template <typename F> int32_t launch(Shape& S, bool pairs, void* work, hipStream
     }
     const uint32_t groups = uint32_t(S.B * S.tiles * S.chunks);
     using std::integral_constant;
-    auto with = [&](auto vec) {
-        if (S.T <= STEPS) return f(vec, integral_constant<int, 1>{}, integral_constant<bool, true>{}, R, groups);
-        if (S.chunks == 1) return f(vec, integral_constant<int, CHUNK_WAVES>{}, integral_constant<bool, true>{}, R, groups);
-        return f(vec, integral_constant<int, CHUNK_WAVES>{}, integral_constant<bool, false>{}, R, groups);
+    auto with = [&](auto vec, auto resets) {
+        if (S.T <= STEPS) return f(vec, integral_constant<int, 1>{}, std::true_type{}, resets, R, groups);
+        if (S.chunks == 1) return f(vec, integral_constant<int, CHUNK_WAVES>{}, std::true_type{}, resets, R, groups);
+        return f(vec, integral_constant<int, CHUNK_WAVES>{}, std::false_type{}, resets, R, groups);
     };
-    return pairs ? with(integral_constant<int, 2>{}) : with(integral_constant<int, 1>{});
+    if (pairs) return resets ? with(integral_constant<int, 2>{}, std::true_type{}) : with(integral_constant<int, 2>{}, std::false_type{});
+    return resets ? with(integral_constant<int, 1>{}, std::true_type{}) : with(integral_constant<int, 1>{}, std::false_type{});
 }
 
 // Whether a [B, T, D] tensor's rows can be read two channels at a time
@@ -444,7 +492,7 @@ uint64_t pv_gated_scan_work_bytes(int64_t B, int64_t T, int64_t D) {
 int32_t pv_gated_scan_hip(const void* gate, const void* value, const float* state, const uint8_t* reset, int64_t B, int64_t T, int64_t D, int64_t gate_b,
                           int64_t gate_t, int64_t value_b, int64_t value_t, int32_t dtype, void* out, float* last, float* carry, void* work,
                           uint64_t work_bytes, void* stream, char* err, size_t errcap) {
-    if (int32_t e = check(B, T, D, dtype, work, work_bytes, err, errcap)) return e;
+    if (int32_t e = check(B, T, D, dtype, work, work_bytes, err, errcap, gate_t, value_t, D)) return e;
     if (!B || !D) return PV_OK;
     if (!gate || !value || !out || !last) return fail(PV_EARG, err, errcap, "null argument");
     Shape S{B, T, D, gate_b, gate_t, value_b, value_t, 0, 0, 0, 0};
@@ -452,11 +500,11 @@ int32_t pv_gated_scan_hip(const void* gate, const void* value, const float* stat
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
         const bool pairs = sizeof(E) == 2 && D % 2 == 0 && pairs_of<E>(gate, B, T, gate_b, gate_t) && pairs_of<E>(value, B, T, value_b, value_t) && aligned(out, 4);
-        return launch(S, pairs, work, st, [&](auto vec, auto waves, auto one, const Records& R, uint32_t groups) {
+        return launch(S, pairs, reset, work, st, [&](auto vec, auto waves, auto one, auto resets, const Records& R, uint32_t groups) {
             constexpr int V = decltype(vec)::value, W = decltype(waves)::value;
-            constexpr bool ONE = decltype(one)::value;
+            constexpr bool ONE = decltype(one)::value, RESET = decltype(resets)::value;
             if constexpr (V == 1 || sizeof(E) == 2)
-                scan_kernel<E, V, W, ONE><<<groups, W * WAVE, 0, st>>>(S, R, static_cast<const E*>(gate), static_cast<const E*>(value), state, reset,
+                scan_kernel<E, V, W, ONE, RESET><<<groups, W * WAVE, 0, st>>>(S, R, static_cast<const E*>(gate), static_cast<const E*>(value), state, reset,
                                                                        static_cast<E*>(out), last, carry);
             return launched(err, errcap);
         });
@@ -467,7 +515,7 @@ int32_t pv_gated_scan_backward_hip(const void* gate, const void* value, const fl
                                    int64_t gate_b, int64_t gate_t, int64_t value_b, int64_t value_t, const void* d_out, int64_t d_out_b, int64_t d_out_t,
                                    const float* d_last, int32_t dtype, void* d_gate, void* d_value, float* d_state, void* work, uint64_t work_bytes,
                                    void* stream, char* err, size_t errcap) {
-    if (int32_t e = check(B, T, D, dtype, work, work_bytes, err, errcap)) return e;
+    if (int32_t e = check(B, T, D, dtype, work, work_bytes, err, errcap, gate_t, value_t, d_out_t, D)) return e;
     if (!B || !D) return PV_OK;
     if (!gate || !value || !carry || !d_out || !d_gate || !d_value) return fail(PV_EARG, err, errcap, "null argument");
     Shape S{B, T, D, gate_b, gate_t, value_b, value_t, d_out_b, d_out_t, 0, 0};
@@ -476,11 +524,11 @@ int32_t pv_gated_scan_backward_hip(const void* gate, const void* value, const fl
         using E = decltype(e);
         const bool pairs = sizeof(E) == 2 && D % 2 == 0 && pairs_of<E>(gate, B, T, gate_b, gate_t) && pairs_of<E>(value, B, T, value_b, value_t) &&
                            pairs_of<E>(d_out, B, T, d_out_b, d_out_t) && aligned(d_gate, 4) && aligned(d_value, 4);
-        return launch(S, pairs, work, st, [&](auto vec, auto waves, auto one, const Records& R, uint32_t groups) {
+        return launch(S, pairs, reset, work, st, [&](auto vec, auto waves, auto one, auto resets, const Records& R, uint32_t groups) {
             constexpr int V = decltype(vec)::value, W = decltype(waves)::value;
-            constexpr bool ONE = decltype(one)::value;
+            constexpr bool ONE = decltype(one)::value, RESET = decltype(resets)::value;
             if constexpr (V == 1 || sizeof(E) == 2)
-                scan_back_kernel<E, V, W, ONE><<<groups, W * WAVE, 0, st>>>(S, R, static_cast<const E*>(gate), static_cast<const E*>(value), reset, carry,
+                scan_back_kernel<E, V, W, ONE, RESET><<<groups, W * WAVE, 0, st>>>(S, R, static_cast<const E*>(gate), static_cast<const E*>(value), reset, carry,
                                                                             static_cast<const E*>(d_out), d_last, static_cast<E*>(d_gate),
                                                                             static_cast<E*>(d_value), d_state);
             return launched(err, errcap);

@@ -6,6 +6,12 @@ from .. import _native as N
 from ._call import DTYPES, call, need, on_gpu, ptr, rows
 
 
+def _steps(t):
+    """`t` with neighbouring channels, and steps at most 64 MiB apart (the kernels' offsets within a chunk): itself, or a copy."""
+    t = rows(t)
+    return t if t.stride(1) * t.element_size() <= 1 << 26 else t.contiguous()
+
+
 def _forward(gate, value, state, reset, keep_carry):
     B, T, D = gate.shape
     dev = gate.device
@@ -33,7 +39,7 @@ class _GatedScan(torch.autograd.Function):
         gate, value, carry, reset = ctx.saved_tensors
         B, T, D = gate.shape
         dev = gate.device
-        d_out, d_last = rows(d_out), d_last.contiguous()
+        d_out, d_last = _steps(d_out), d_last.contiguous()
         d_gate = torch.empty(B, T, D, dtype=gate.dtype, device=dev)
         d_value = torch.empty(B, T, D, dtype=gate.dtype, device=dev)
         d_state = torch.empty(B, D, dtype=torch.float32, device=dev) if ctx.has_state else None
@@ -64,7 +70,7 @@ def gated_scan(gate, value, state=None, reset=None):
         reset = reset.contiguous()
     if T == 0:
         return gate * value, state.clone() if state is not None else torch.zeros(B, D, dtype=torch.float32, device=gate.device)
-    gate, value = rows(gate), rows(value)
+    gate, value = _steps(gate), _steps(value)
     if torch.is_grad_enabled() and (gate.requires_grad or value.requires_grad or (state is not None and state.requires_grad)):
         return _GatedScan.apply(gate, value, state, reset)
     return _forward(gate, value, state, reset, False)[:2]

@@ -173,6 +173,14 @@ def test_empty():
         assert gate.grad is None or gate.grad.shape == gate.shape
 
 
+def test_steps_far_apart():
+    """Steps 128 MiB apart in memory."""
+    room = torch.zeros(3, 1 << 26, dtype=torch.bfloat16, device="cuda")
+    gate, value, state, _, _, _ = make(1, 3, 64, torch.bfloat16, seed=30)
+    room[:, :64] = gate[0]
+    check(room[None, :, :64], value, state, None)
+
+
 def test_other_stream_and_capture():
     """On a stream of its own, and captured into a graph that is replayed on new inputs between eager work."""
     from panvram_amd import ops

@@ -26,6 +26,7 @@ def test_scan_entry():
     assert "shape" in scan(B=-1)
     assert "shape" in scan(T=0)
     assert "work" in scan(T=5000, work_bytes=8)
+    assert "stride" in refused("pv_gated_scan_hip", FAKE, FAKE, None, None, 1, 8, 4, 32, 1 << 25, 32, 4, N.F32, FAKE, FAKE, None, FAKE, 1 << 20)
     assert "null" in scan(gate=None)
     assert "null" in scan(out=None)
     m = refused("pv_gated_scan_backward_hip", FAKE, FAKE, None, None, 1, 8, 4, 32, 4, 32, 4, FAKE, 32, 4, None, N.F32, FAKE, FAKE, None, FAKE, 1 << 20)
