@@ -413,11 +413,14 @@ int32_t pv_next_base_loss_hip(const void* hidden, const void* weight, const void
                               const float* factor, float* each, float* loss, void* d_hidden, void* d_weight, void* work, uint64_t work_bytes, void* stream,
                               char* err, size_t errcap);
 
-/* norm (f32[1]) = sqrt(sum over `count` tensors of their squares). grads, sizes (elements), dtypes, out: host arrays. out: NULL,
- * or for each tensor where grads[i] * min(1, max_norm / (norm + 1e-6)) goes (grads[i] itself, or memory apart from all). */
+/* norm (f32[1]) = sqrt(sum over `count` tensors of their squares). grads, sizes (elements), dtypes: host arrays. */
 uint64_t pv_gradient_norm_work_bytes(const int64_t* sizes, const int32_t* dtypes, int32_t count);
-int32_t pv_gradient_norm_hip(const void* const* grads, void* const* out, const int64_t* sizes, const int32_t* dtypes, int32_t count, float max_norm, float* norm,
-                             void* work, uint64_t work_bytes, void* stream, char* err, size_t errcap);
+int32_t pv_gradient_norm_hip(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int32_t count, float* norm, void* work, uint64_t work_bytes,
+                             void* stream, char* err, size_t errcap);
+/* out[i] = grads[i] * min(1, max_norm / (norm + 1e-6)), norm as pv_gradient_norm_hip left it. out: host array; out[i] is
+ * grads[i] itself, or memory apart from all of grads. */
+int32_t pv_scale_gradients_hip(const void* const* grads, void* const* out, const int64_t* sizes, const int32_t* dtypes, int32_t count, float max_norm,
+                               const float* norm, void* stream, char* err, size_t errcap);
 
 #ifdef __cplusplus
 }

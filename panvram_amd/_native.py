@@ -112,7 +112,8 @@ SIGNATURES = {
     "pv_next_base_loss_work_bytes": (u64, [i64, i64, i64, i32, i32]),
     "pv_next_base_loss_hip": (i32, [vp, vp, vp, i64, i64, i64, i32, i64, i64, i64, i64, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, u64, vp, cp, sz]),
     "pv_gradient_norm_work_bytes": (u64, [vp, vp, i32]),
-    "pv_gradient_norm_hip": (i32, [vp, vp, vp, vp, i32, f32, vp, vp, u64, vp, cp, sz]),
+    "pv_gradient_norm_hip": (i32, [vp, vp, vp, i32, vp, vp, u64, vp, cp, sz]),
+    "pv_scale_gradients_hip": (i32, [vp, vp, vp, vp, i32, f32, vp, vp, cp, sz]),
 }
 
 _lib = None

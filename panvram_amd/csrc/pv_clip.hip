@@ -169,6 +169,20 @@ template <typename F> void groups(const void* const* from, void* const* to, cons
     if (G.count) f(G, uint32_t(blocks));
 }
 
+// What both entries ask of their arguments
+int32_t check(const void* const* grads, void* const* out, const int64_t* sizes, const int32_t* dtypes, int32_t count, char* err, size_t cap) {
+    if (count < 0 || (count && (!grads || !sizes || !dtypes))) return fail(PV_EARG, err, cap, "null argument");
+    int64_t all = 0;
+    for (int32_t i = 0; i < count; i++) {
+        const int bytes = element_bytes(dtypes[i]);
+        if (!bytes) return fail(PV_EARG, err, cap, "dtype: one of PV_F32, PV_BF16, PV_F16");
+        if (sizes[i] < 0 || sizes[i] > (int64_t(1) << 40) || (all += sizes[i]) > (int64_t(1) << 40)) return fail(PV_EARG, err, cap, "size: 0 to 2^40 elements in all");
+        if (sizes[i] && (!grads[i] || (out && !out[i]))) return fail(PV_EARG, err, cap, "null argument");
+        if (sizes[i] && (!aligned(grads[i], bytes) || (out && !aligned(out[i], bytes)))) return fail(PV_EARG, err, cap, "address: not a multiple of the element's size");
+    }
+    return PV_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -181,29 +195,29 @@ uint64_t pv_gradient_norm_work_bytes(const int64_t* sizes, const int32_t* dtypes
     return b * 8;
 }
 
-int32_t pv_gradient_norm_hip(const void* const* grads, void* const* out, const int64_t* sizes, const int32_t* dtypes, int32_t count, float max_norm, float* norm,
-                             void* work, uint64_t work_bytes, void* stream, char* err, size_t errcap) {
-    if (count < 0 || !norm || (count && (!grads || !sizes || !dtypes))) return fail(PV_EARG, err, errcap, "null argument");
-    int64_t all = 0;
-    for (int32_t i = 0; i < count; i++) {
-        if (!element_bytes(dtypes[i])) return fail(PV_EARG, err, errcap, "dtype: one of PV_F32, PV_BF16, PV_F16");
-        if (sizes[i] < 0 || sizes[i] > (int64_t(1) << 40) || (all += sizes[i]) > (int64_t(1) << 40)) return fail(PV_EARG, err, errcap, "size: 0 to 2^40 elements in all");
-        if (sizes[i] && (!grads[i] || (out && !out[i]))) return fail(PV_EARG, err, errcap, "null argument");
-        if (sizes[i] && (!aligned(grads[i], element_bytes(dtypes[i])) || (out && !aligned(out[i], element_bytes(dtypes[i]))))) return fail(PV_EARG, err, errcap, "address: not a multiple of the element's size");
-    }
+int32_t pv_gradient_norm_hip(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int32_t count, float* norm, void* work, uint64_t work_bytes,
+                             void* stream, char* err, size_t errcap) {
+    if (!norm) return fail(PV_EARG, err, errcap, "null argument");
+    if (int32_t e = check(grads, nullptr, sizes, dtypes, count, err, errcap)) return e;
     const uint64_t need = pv_gradient_norm_work_bytes(sizes, dtypes, count);
     if (need && (!work || work_bytes < need)) return fail(PV_EARG, err, errcap, "work: too small");
     const hipStream_t st = hipStream_t(stream);
     double* parts = static_cast<double*>(work);
-    const int64_t piece = piece_of(sizes, dtypes, count);
     int64_t done = 0;
-    groups(grads, nullptr, sizes, dtypes, count, piece, false, [&](const Group& G, uint32_t blocks) {
+    groups(grads, nullptr, sizes, dtypes, count, piece_of(sizes, dtypes, count), false, [&](const Group& G, uint32_t blocks) {
         square_kernel<<<blocks, BLOCK, 0, st>>>(G, parts + done);
         done += blocks;
     });
     norm_end_kernel<<<1, END, 0, st>>>(parts, done, norm);
-    if (out)
-        groups(grads, out, sizes, dtypes, count, PIECE, true, [&](const Group& G, uint32_t blocks) { scale_kernel<<<blocks, BLOCK, 0, st>>>(G, norm, max_norm); });
+    return launched(err, errcap);
+}
+
+int32_t pv_scale_gradients_hip(const void* const* grads, void* const* out, const int64_t* sizes, const int32_t* dtypes, int32_t count, float max_norm,
+                               const float* norm, void* stream, char* err, size_t errcap) {
+    if (!norm || (count && !out)) return fail(PV_EARG, err, errcap, "null argument");
+    if (int32_t e = check(grads, out, sizes, dtypes, count, err, errcap)) return e;
+    groups(grads, out, sizes, dtypes, count, PIECE, true,
+           [&](const Group& G, uint32_t blocks) { scale_kernel<<<blocks, BLOCK, 0, hipStream_t(stream)>>>(G, norm, max_norm); });
     return launched(err, errcap);
 }
 

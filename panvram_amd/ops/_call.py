@@ -1,40 +1,48 @@
-"""What the operators' Python side shares: checks of tensors, and calls of the library on the current stream."""
+"""What the operators' Python side shares: checks of tensors, and calls of the library on the current stream. A call of a
+few rows costs its host time, so what is asked of the arguments is asked once and messages are made only where they are
+raised."""
+import threading
+
 import torch
 
 from .. import _native as N
+from .._streams import raw as _raw
 
 DTYPES = {torch.float32: N.F32, torch.bfloat16: N.BF16, torch.float16: N.F16}
 
 
-def need(ok, message):
-    if not ok:
-        raise ValueError(message)
+def on_gpu(name, first, *others):
+    """The index of the GPU that all tensors (None: left out) are on; an error naming what is not there."""
+    index = first.get_device() if isinstance(first, torch.Tensor) else -1
+    for t in others:
+        if t is not None and (index < 0 or not isinstance(t, torch.Tensor) or t.get_device() != index):
+            index = -1
+    if index >= 0:
+        return index
+    where = []
+    for t in (first, *others):
+        if t is not None:
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{name}: tensors expected, got {type(t).__name__}")
+            if not t.is_cuda:
+                raise RuntimeError(f"{name} runs on the GPU only; got a tensor on {t.device}")
+            where.append(str(t.device))
+    raise ValueError(f"{name}: tensors on {' and '.join(sorted(set(where)))}")
 
 
-def on_gpu(name, *tensors):
-    """The index of the GPU that all tensors (None: left out) are on."""
-    index = None
-    for t in tensors:
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name}: tensors expected, got {type(t).__name__}")
-        if not t.is_cuda:
-            raise RuntimeError(f"{name} runs on the GPU only; got a tensor on {t.device}")
-        i = t.get_device()
-        if index is not None and i != index:
-            raise ValueError(f"{name}: tensors on cuda:{index} and cuda:{i}")
-        index = i
-    return index
+_local = threading.local()
 
 
 def call(fn, index, *args):
-    """fn(*args, stream, err, errcap) of the library on GPU `index`'s current stream; errors raise."""
+    """fn(*args, stream, err, errcap), a function of the library, on GPU `index`'s current stream; errors raise."""
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
             return call(fn, index, *args)
-    err = N.errbuf()
-    code = getattr(N.lib(), fn)(*args, torch.cuda.current_stream(index).cuda_stream, err, len(err))
+    try:
+        err = _local.err
+    except AttributeError:
+        err = _local.err = N.errbuf()
+    code = fn(*args, _raw.get(index), err, 4096)
     if code:
         N.raise_for(code, err)
 

@@ -1,11 +1,11 @@
 """The norm over many gradient tensors, and clipping to it (panvram_amd/csrc/pv_clip.hip)."""
 from array import array
-from operator import attrgetter, eq
+from operator import attrgetter
 
 import torch
 
 from .. import _native as N
-from ._call import DTYPES, call, need, on_gpu
+from ._call import DTYPES, call, on_gpu
 
 
 def _dense(t):
@@ -21,33 +21,52 @@ def _dense(t):
 
 
 _ptr, _numel, _whole, _gpu = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device
-_dtype, _shape = attrgetter("dtype"), attrgetter("shape")
+_dtype = attrgetter("dtype")
 
 
-def _checked(name, grads):
-    """The GPU that all of `grads` are on; their types are ones that the kernels take. (Many tensors: one pass of a C-level
-    map for each thing that is asked, not a loop.)"""
-    if not all(issubclass(c, torch.Tensor) for c in set(map(type, grads))):
-        raise TypeError(f"{name}: tensors expected")
-    where = set(map(_gpu, grads))
-    if len(where) != 1 or -1 in where:
-        on_gpu(name, *grads)
-    need(set(map(_dtype, grads)) <= DTYPES.keys(), f"{name}: gradients are float32, bfloat16 or float16")
-    return where.pop()
+class _List:
+    """Many tensors as the library takes them: addresses, sizes, types. (One pass of a C-level map for each thing that is
+    asked, not a loop: 150 tensors cost 40 us.)"""
+
+    def __init__(self, name, tensors):
+        self.tensors, self.name = tensors, name
+        if not all(issubclass(c, torch.Tensor) for c in set(map(type, tensors))):
+            raise TypeError(f"{name}: tensors expected")
+        where = set(map(_gpu, tensors))
+        if len(where) != 1 or -1 in where:
+            on_gpu(name, *tensors)
+        self.index = where.pop()
+        self.dtypes = list(map(_dtype, tensors))
+        kinds = set(self.dtypes)
+        if not kinds <= DTYPES.keys():
+            raise ValueError(f"{name}: gradients are float32, bfloat16 or float16, got {[k for k in kinds if k not in DTYPES]}")
+        self.types = array("i", [DTYPES[kinds.pop()]]) * len(tensors) if len(kinds) == 1 else array("i", map(DTYPES.__getitem__, self.dtypes))
+        self.sizes = array("q", map(_numel, tensors))
+        self.whole = all(map(_whole, tensors))
+        self.made = []                     # copies, kept until the call is made
+
+    def replace(self, i, t):
+        if not self.made:
+            self.tensors = list(self.tensors)
+        self.made.append(t)
+        self.tensors[i] = t
+
+    def pointers(self):
+        return array("Q", map(_ptr, self.tensors))
 
 
-def _run(index, grads, max_norm, out):
-    """grads, out: each one run of memory, each pair's elements in the same order."""
-    n = len(grads)
-    sizes = array("q", map(_numel, grads))
-    types = array("i", map(DTYPES.__getitem__, map(_dtype, grads)))
-    src = array("Q", map(_ptr, grads))
-    dst = array("Q", map(_ptr, out)) if out is not None else None
-    at = [a.buffer_info()[0] if a is not None else None for a in (src, dst, sizes, types)]
-    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    work = torch.empty(N.lib().pv_gradient_norm_work_bytes(at[2], at[3], n), dtype=torch.uint8, device=norm.device)
-    call("pv_gradient_norm_hip", index, *at, n, max_norm, norm.data_ptr(), work.data_ptr(), work.numel())
-    return norm
+def _at(a):
+    return a.buffer_info()[0]
+
+
+def _norm(g):
+    """The norm, and what its kernels were given"""
+    norm = torch.empty((), dtype=torch.float32, device=g.tensors[0].device)
+    L, n, src = N.lib(), len(g.tensors), g.pointers()
+    size = L.pv_gradient_norm_work_bytes(_at(g.sizes), _at(g.types), n)
+    work = torch.empty(size, dtype=torch.uint8, device=norm.device)
+    call(L.pv_gradient_norm_hip, g.index, _at(src), _at(g.sizes), _at(g.types), n, norm.data_ptr(), work.data_ptr(), size)
+    return norm, src
 
 
 @torch.no_grad()
@@ -57,43 +76,54 @@ def gradient_norm(grads):
     grads = list(grads)
     if not grads:
         return torch.zeros(())
-    index = _checked("gradient_norm", grads)
-    if not all(map(_whole, grads)):
-        grads = [g if _dense(g) else g.contiguous() for g in grads]
-    return _run(index, grads, 0.0, None)
+    g = _List("gradient_norm", grads)
+    if not g.whole:
+        for i, t in enumerate(grads):
+            if not _dense(t):
+                g.replace(i, t.contiguous())
+    return _norm(g)[0]
 
 
 @torch.no_grad()
 def clip_gradients(grads, max_norm, out=None):
     """Scales the tensors in `grads` (float32, bfloat16, float16, mixed as they come, on one GPU) by
-    min(1, max_norm / (norm + 1e-6)), in place or into the tensors of `out` (alike, for instance views of one flat buffer;
-    each one grads' own tensor or apart from all of them), and returns the norm before, as gradient_norm does. Nothing is
-    read back: the factor is made and used on the GPU. If the norm is not finite, neither are the scaled gradients."""
+    min(1, max_norm / (norm + 1e-6)), in place or into the tensors of `out`, and returns the norm before, as gradient_norm
+    does. out: for each gradient a tensor of its type and size, for instance views of one flat buffer; the gradient itself,
+    or memory apart from all of them. Nothing is read back: the factor is made and used on the GPU. If the norm is not
+    finite, neither are the scaled gradients."""
     grads = list(grads)
     max_norm = float(max_norm)
-    need(max_norm >= 0, f"clip_gradients: max_norm is not negative, got {max_norm}")
+    if not max_norm >= 0:
+        raise ValueError(f"clip_gradients: max_norm is not negative, got {max_norm}")
     out = None if out is None else list(out)
-    need(out is None or len(out) == len(grads), f"clip_gradients: {len(grads)} gradients and {len(out or ())} tensors in out")
+    if out is not None and len(out) != len(grads):
+        raise ValueError(f"clip_gradients: {len(grads)} gradients and {len(out)} tensors in out")
     if not grads:
         return torch.zeros(())
-    index = _checked("clip_gradients", grads)
-    if out is not None:
-        need(_checked("clip_gradients", out) == index, "clip_gradients: grads and out on one GPU")
-        if not all(map(eq, map(_shape, grads), map(_shape, out))) or not all(map(eq, map(_dtype, grads), map(_dtype, out))):
-            i = next(i for i, (g, o) in enumerate(zip(grads, out)) if g.shape != o.shape or g.dtype != o.dtype)
-            raise ValueError(f"clip_gradients: out[{i}] is {out[i].dtype} {list(out[i].shape)}, its gradient {grads[i].dtype} {list(grads[i].shape)}")
+    g = _List("clip_gradients", grads)
+    o = g if out is None else _List("clip_gradients", out)
+    if o is not g and (o.index != g.index or o.dtypes != g.dtypes or o.sizes != g.sizes):
+        for i, (a, b) in enumerate(zip(grads, out)):
+            if a.dtype != b.dtype or a.numel() != b.numel() or a.device != b.device:
+                raise ValueError(f"clip_gradients: out[{i}] is {b.dtype} {list(b.shape)} on {b.device}, its gradient {a.dtype} {list(a.shape)} on {a.device}")
     back = []           # (tensor, what its values are made in) where memory is not one run, or in another order
-    if not all(map(_whole, grads)) or (out is not None and not all(map(_whole, out))):
+    if not (g.whole and o.whole):
         to = grads if out is None else out
-        grads, out = list(grads), list(to)
-        for i, (g, o) in enumerate(zip(grads, to)):
-            if g.stride() != o.stride() or not _dense(g):
-                grads[i] = g.contiguous()
-                if o.is_contiguous():
-                    continue
-                out[i] = torch.empty_like(grads[i])
-                back.append((o, out[i]))
-    norm = _run(index, grads, max_norm, grads if out is None else out)
-    for o, made in back:
-        o.copy_(made)
+        if o is g:
+            o = _List("clip_gradients", grads)
+        for i, (a, b) in enumerate(zip(grads, to)):
+            if (a.is_contiguous() and b.is_contiguous()) or (a.stride() == b.stride() and a.shape == b.shape and _dense(a)):
+                continue
+            if a.shape != b.shape:
+                raise ValueError(f"clip_gradients: out[{i}] is {list(b.shape)}, its gradient {list(a.shape)}, and one of them is not contiguous")
+            if not a.is_contiguous():
+                g.replace(i, a.contiguous())
+            if not b.is_contiguous():
+                o.replace(i, torch.empty_like(a, memory_format=torch.contiguous_format))
+                back.append((b, o.made[-1]))
+    norm, src = _norm(g)
+    dst = src if o is g else o.pointers()
+    call(N.lib().pv_scale_gradients_hip, g.index, _at(src), _at(dst), _at(g.sizes), _at(g.types), len(grads), max_norm, norm.data_ptr())
+    for b, made in back:
+        b.copy_(made)
     return norm

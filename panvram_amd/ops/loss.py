@@ -3,21 +3,24 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _native as N
-from ._call import DTYPES, call, need, on_gpu, ptr, rows
+from ._call import DTYPES, call, on_gpu, ptr, rows
 
 
 def _run(hidden, weight, tokens, ignore, want_each, want_loss, grads, scale=None, factor=None):
     B, T, D = hidden.shape
     V = weight.shape[0]
     dev = hidden.device
-    each = torch.empty(B, T, dtype=torch.float32, device=dev) if want_each else None
+    each = torch.empty((B, T), dtype=torch.float32, device=dev) if want_each else None
     loss = torch.empty((), dtype=torch.float32, device=dev) if want_loss else None
-    d_hidden = torch.empty(B, T, D, dtype=hidden.dtype, device=dev) if grads else None
-    d_weight = torch.empty(V, D, dtype=weight.dtype, device=dev) if grads else None
-    work = torch.empty(N.lib().pv_next_base_loss_work_bytes(B, T, D, V, grads), dtype=torch.uint8, device=dev)
-    call("pv_next_base_loss_hip", hidden.get_device(), hidden.data_ptr(), weight.data_ptr(), tokens.data_ptr(), B, T, D, V, hidden.stride(0), hidden.stride(1),
-         tokens.stride(0), ignore, DTYPES[hidden.dtype], DTYPES[weight.dtype], tokens.element_size(), ptr(scale), ptr(factor), ptr(each), ptr(loss), ptr(d_hidden),
-         ptr(d_weight), work.data_ptr(), work.numel())
+    d_hidden = torch.empty((B, T, D), dtype=hidden.dtype, device=dev) if grads else None
+    d_weight = torch.empty((V, D), dtype=weight.dtype, device=dev) if grads else None
+    L = N.lib()
+    size = L.pv_next_base_loss_work_bytes(B, T, D, V, grads)
+    work = torch.empty(size, dtype=torch.uint8, device=dev)
+    hb, ht, _ = hidden.stride()
+    call(L.pv_next_base_loss_hip, hidden.get_device(), hidden.data_ptr(), weight.data_ptr(), tokens.data_ptr(), B, T, D, V, hb, ht, tokens.stride(0), ignore,
+         DTYPES[hidden.dtype], DTYPES[weight.dtype], tokens.element_size(), ptr(scale), ptr(factor), ptr(each), ptr(loss), ptr(d_hidden), ptr(d_weight),
+         work.data_ptr(), size)
     return each, loss, d_hidden, d_weight
 
 
@@ -40,12 +43,15 @@ class _NextBaseLoss(torch.autograd.Function):
 
 def _checked(name, hidden, weight, tokens, ignore):
     on_gpu(name, hidden, weight, tokens)
-    need(hidden.dim() == 3 and hidden.dtype in DTYPES, f"{name}: hidden is [B, T, D] in float32, bfloat16 or float16, got {hidden.dtype} {list(hidden.shape)}")
+    if hidden.dim() != 3 or hidden.dtype not in DTYPES or hidden.numel() == 0:
+        raise ValueError(f"{name}: hidden is [B, T, D] in float32, bfloat16 or float16 and not empty, got {hidden.dtype} {list(hidden.shape)}")
     B, T, D = hidden.shape
-    need(B >= 1 and T >= 1 and D >= 1, f"{name}: hidden is empty: {list(hidden.shape)}")
-    need(weight.dim() == 2 and weight.shape[1] == D and 1 <= weight.shape[0] <= 16, f"{name}: weight is [V, {D}] with 1 to 16 ids, got {list(weight.shape)}")
-    need(weight.dtype in (hidden.dtype, torch.float32), f"{name}: weight is in hidden's type or float32, got {weight.dtype}")
-    need(tokens.shape == (B, T) and tokens.dtype in (torch.uint8, torch.int64), f"{name}: tokens are uint8 or int64 {[B, T]}, got {tokens.dtype} {list(tokens.shape)}")
+    if weight.dim() != 2 or weight.shape[1] != D or not 1 <= weight.shape[0] <= 16:
+        raise ValueError(f"{name}: weight is [V, {D}] with 1 to 16 ids, got {list(weight.shape)}")
+    if weight.dtype != hidden.dtype and weight.dtype != torch.float32:
+        raise ValueError(f"{name}: weight is in hidden's type or float32, got {weight.dtype}")
+    if tokens.shape != (B, T) or tokens.dtype not in (torch.uint8, torch.int64):
+        raise ValueError(f"{name}: tokens are uint8 or int64 {[B, T]}, got {tokens.dtype} {list(tokens.shape)}")
     return rows(hidden), weight.contiguous(), rows(tokens), -1 if ignore is None else int(ignore)
 
 
@@ -58,7 +64,8 @@ def next_base_loss(hidden, weight, tokens, ignore=4, reduction="mean"):
     a row. reduction: "mean" over the places that count (0 where there are none), or "none": float32 [B, T] with 0 at places
     that do not count. Gradients flow to hidden and weight; what stands in hidden where nothing counts reaches neither."""
     hidden, weight, tokens, ignore = _checked("next_base_loss", hidden, weight, tokens, ignore)
-    need(reduction in ("mean", "none"), f'next_base_loss: reduction is "mean" or "none", got {reduction!r}')
+    if reduction not in ("mean", "none"):
+        raise ValueError(f'next_base_loss: reduction is "mean" or "none", got {reduction!r}')
     mean = reduction == "mean"
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         return _NextBaseLoss.apply(hidden, weight, tokens, ignore, mean)
@@ -74,6 +81,7 @@ def next_base_loss_grad(hidden, weight, tokens, ignore=4, scale=None):
     hidden, weight, tokens, ignore = _checked("next_base_loss_grad", hidden, weight, tokens, ignore)
     if scale is not None:
         on_gpu("next_base_loss_grad", hidden, scale)
-        need(scale.dtype == torch.float32 and scale.numel() == 1, f"next_base_loss_grad: scale is one float32, got {scale.dtype} {list(scale.shape)}")
+        if scale.dtype != torch.float32 or scale.numel() != 1:
+            raise ValueError(f"next_base_loss_grad: scale is one float32, got {scale.dtype} {list(scale.shape)}")
     _, loss, d_hidden, d_weight = _run(hidden, weight, tokens, ignore, False, True, True, scale=scale)
     return loss, d_hidden, d_weight

@@ -89,14 +89,21 @@ def test_loss_entry():
     assert "work" in loss(work=None) and "work" in loss(work_bytes=8)
 
 
-def test_norm_of_gradients_entry():
-    def clip(grad=FAKE, size=100, dtype=N.F32, out=FAKE, norm=FAKE, work=FAKE, work_bytes=1 << 20):
-        vp, i64, i32 = ctypes.c_void_p * 1, ctypes.c_int64 * 1, ctypes.c_int32 * 1
-        return refused("pv_gradient_norm_hip", vp(grad), vp(out), i64(size), i32(dtype), 1, 1.0, norm, work, work_bytes)
-    assert "dtype" in clip(dtype=5)
-    assert "size" in clip(size=-1)
-    assert "null" in clip(grad=None) and "null" in clip(out=None) and "null" in clip(norm=None)
-    assert "work" in clip(work=None) and "work" in clip(work_bytes=4)
+def test_gradients_entries():
+    vp, i64, i32 = ctypes.c_void_p * 1, ctypes.c_int64 * 1, ctypes.c_int32 * 1
+
+    def norm(grad=FAKE, size=100, dtype=N.F32, norm=FAKE, work=FAKE, work_bytes=1 << 20):
+        return refused("pv_gradient_norm_hip", vp(grad), i64(size), i32(dtype), 1, norm, work, work_bytes)
+
+    def scale(grad=FAKE, out=FAKE, size=100, dtype=N.F32, norm=FAKE):
+        return refused("pv_scale_gradients_hip", vp(grad), vp(out), i64(size), i32(dtype), 1, 1.0, norm)
+    for fn in (norm, scale):
+        assert "dtype" in fn(dtype=5)
+        assert "size" in fn(size=-1) and "size" in fn(size=1 << 41)
+        assert "null" in fn(grad=None) and "null" in fn(norm=None)
+        assert "address" in fn(grad=FAKE + 2)
+    assert "null" in scale(out=None)
+    assert "work" in norm(work=None) and "work" in norm(work_bytes=4)
 
 
 @pytest.mark.gpu
@@ -128,7 +135,7 @@ def test_loss_arguments():
 def test_clip_arguments():
     g = torch.zeros(5, device="cuda")
     for bad in (dict(grads=[g], max_norm=-1.0), dict(grads=[g], max_norm=float("nan")), dict(grads=[g.double()], max_norm=1.0), dict(grads=[g], max_norm=1.0, out=[]),
-                dict(grads=[g], max_norm=1.0, out=[g[:3]]), dict(grads=[g], max_norm=1.0, out=[g.bfloat16()])):
+                dict(grads=[g], max_norm=1.0, out=[g[:3]]), dict(grads=[g], max_norm=1.0, out=[g.bfloat16()]), dict(grads=[g[::2]], max_norm=1.0, out=[torch.zeros(3, 1, device="cuda")])):
         with pytest.raises(ValueError):
             ops.clip_gradients(**bad)
     with pytest.raises(RuntimeError, match="GPU only"):
