@@ -372,8 +372,8 @@ enum pv_format8 { PV_E4M3 = 0, PV_INT8 = 1 };
 /* h[b, t, d] = (1 - z) h[b, t-1, d] + z value[b, t, d], z = sigmoid(gate[b, t, d]), T >= 1. gate, value: [B, T, D] of `dtype`
  * with strides (gate_b, gate_t), (value_b, value_t), a step's at most 2^26 bytes. state: f32[B, D] before step 0, or NULL: zero. reset: u8[B, T], or NULL;
  * where not 0, h[b, t-1] is dropped. out: [B, T, D] of `dtype`; last: f32[B, D] = h[b, T-1]. carry: NULL, or
- * f32[B, pv_gated_scan_chunks(T), D] that the backward pass takes. */
-int64_t pv_gated_scan_chunks(int64_t T);
+ * f32[B, pv_gated_scan_spans(T), D] that the backward pass takes. */
+int64_t pv_gated_scan_spans(int64_t T);
 uint64_t pv_gated_scan_work_bytes(int64_t B, int64_t T, int64_t D);
 int32_t pv_gated_scan_hip(const void* gate, const void* value, const float* state, const uint8_t* reset, int64_t B, int64_t T, int64_t D, int64_t gate_b,
                           int64_t gate_t, int64_t value_b, int64_t value_t, int32_t dtype, void* out, float* last, float* carry, void* work,

@@ -101,7 +101,7 @@ SIGNATURES = {
     "pv_windows_hip_noalloc": (i32, [ctypes.POINTER(DevCohort), vp, vp, i64, i64, vp, i32, i32, vp, vp, vp, cp, sz]),
     "pv_selftest_bytes": (i32, []),
     "pv_fetch_hip": (i32, [ctypes.POINTER(DevCohort), i64, i64, i64, i32, i32, vp, vp, vp, u64, vp, cp, sz]),
-    "pv_gated_scan_chunks": (i64, [i64]),
+    "pv_gated_scan_spans": (i64, [i64]),
     "pv_gated_scan_work_bytes": (u64, [i64, i64, i64]),
     "pv_gated_scan_hip": (i32, [vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, i32, vp, vp, vp, vp, u64, vp, cp, sz]),
     "pv_gated_scan_backward_hip": (i32, [vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, vp, i64, i64, vp, i32, vp, vp, vp, vp, u64, vp, cp, sz]),

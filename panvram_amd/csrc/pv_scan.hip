@@ -3,11 +3,11 @@
 // A run of steps is the map h -> A h + H of the state before it: A the product of its (1 - z), H the run started at zero.
 // Maps of neighbouring runs join, so all of T is worked on at once and every byte is read once and written once:
 //   - a wave holds STEPS steps of 64 x VEC channels in registers, a workgroup of WAVES waves a chunk of WAVES x STEPS steps;
-//   - the workgroup makes its chunk's map, publishes it (`before_chunk`), joins the maps of the chunks before, and walks its
+//   - the workgroup makes its chunk's map, publishes it (`Before`), joins the maps of the chunks before, and walks its
 //     steps from there.
 // The gradient is the same recurrence backwards: C[t] = (1 - z[t]) (d_out[t] + C[t+1]), C what flows into h[t-1]; the states
-// before each step are made again from the chunk's start, which the forward pass leaves in `carry` (one f32 per chunk and
-// channel, so that h is never read). A step's arithmetic is the same for every cut of T, and so is the order in which maps are
+// before each step are made again from the start of the wave's STEPS steps, which the forward pass leaves in `carry` (one f32 for
+// STEPS steps of a channel, so that h is never read). A step's arithmetic is the same for every cut of T, and so is the order in which maps are
 // joined: results do not depend on which workgroup was faster.
 //
 // A reset at t drops h[t-1], whatever it holds (a NaN too): the step is chosen, not multiplied by zero, and the map of a run
@@ -24,7 +24,7 @@ constexpr float CUT = -1.0f;
 
 struct Shape {
     int64_t B, T, D, gb, gt, vb, vt, db, dt;   // strides in elements: gate, value, d_out (batch, time); channels are neighbours
-    int64_t chunks, tiles;                     // chunks of T, tiles of D
+    int64_t spans, chunks, tiles;              // spans of STEPS and chunks of T, tiles of D
 };
 
 // z = sigmoid(g) and k = 1 - z of a step in one register: the smaller of the two, its sign bit set where that is z. It is made from
@@ -54,8 +54,7 @@ __device__ inline Map then(Map first, Map second) {
 // A map is one 8-byte word (A, H) per channel, written by one store; EMPTY until then. Its NaNs are stored as 0x7fc00000, so
 // that no map is EMPTY. A word is read and written past the L2 caches (agent scope); no other data depends on the order.
 // Every wait ends: a workgroup takes its position from a counter, so all earlier positions belong to workgroups that run
-// already, a position publishes level 0 without waiting, and each level waits for earlier positions only. (Should a word not
-// come in some seconds all the same, it counts as NaN.)
+// already, a position publishes level 0 without waiting, and each other level after waiting for earlier positions only. (Should a word not come in some seconds all the same, it counts as NaN.)
 constexpr int FAN = 8, LEVELS = 8;         // 8^8 chunks
 constexpr uint64_t EMPTY = ~0ull;
 constexpr int POLLS = 1 << 22;
@@ -77,36 +76,25 @@ __device__ inline void publish(uint64_t* at, Map m, bool on) {
     if (on) __hip_atomic_store(at, word_of(m.A, m.H), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// The map of all chunks before position p, for the lane's channel d (where `on`); own: the chunk's map
-__device__ inline Map before_chunk(const Records& R, const Shape& S, int64_t b, int64_t p, int64_t d, bool on, Map own) {
+// The maps of a group's first members on level l, up to position p of that level, joined in order; for the lane's channel d (on)
+__device__ inline Map before_at(const Records& R, const Shape& S, int64_t b, int l, int64_t n, int64_t p, int64_t d, bool on) {
+    const int many = int(p & (FAN - 1));
+    const uint64_t* rec = R.level[l] + (b * n + (p - many)) * S.D + d;
+    uint64_t w[FAN - 1];
+#pragma unroll
+    for (int i = 0; i < FAN - 1; i++) {
+        w[i] = 0;
+        if (i < many && on) w[i] = __hip_atomic_load(rec + i * S.D, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
     Map all = {1.0f, 0.0f};
-    int64_t n = S.chunks;
-    bool whole = true;                     // own is the map of a whole group of this level
-    for (int l = 0; l < LEVELS && n > 0; l++, n /= FAN) {
-        const int64_t at = p & ~int64_t(FAN - 1);      // the group's first
-        const int many = int(p - at);
-        uint64_t* rec = R.level[l] + b * n * S.D + d;
-        if (whole) publish(rec + p * S.D, own, on);
-        uint64_t w[FAN - 1];
 #pragma unroll
-        for (int i = 0; i < FAN - 1; i++) {
-            w[i] = 0;
-            if (i < many && on) w[i] = __hip_atomic_load(rec + (at + i) * S.D, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int i = 0; i < FAN - 1; i++) {
+        if (i >= many) break;
+        for (int k = 0; __any(w[i] == EMPTY) && k < POLLS; k++) {
+            __builtin_amdgcn_s_sleep(1);
+            if (on) w[i] = __hip_atomic_load(rec + i * S.D, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        Map level = {1.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < FAN - 1; i++) {
-            if (i >= many) break;
-            for (int k = 0; __any(w[i] == EMPTY) && k < POLLS; k++) {
-                __builtin_amdgcn_s_sleep(1);
-                if (on) w[i] = __hip_atomic_load(rec + (at + i) * S.D, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-            level = then(level, {__uint_as_float(uint32_t(w[i])), __uint_as_float(uint32_t(w[i] >> 32))});
-        }
-        all = then(level, all);
-        whole = whole && many == FAN - 1;
-        if (whole) own = then(level, own);
-        p /= FAN;
+        all = then(all, {__uint_as_float(uint32_t(w[i])), __uint_as_float(uint32_t(w[i] >> 32))});
     }
     return all;
 }
@@ -207,6 +195,43 @@ template <bool RESET, bool BACK, typename F> __device__ inline void over_steps(c
     for (int i = 0; i < STEPS; i++) { const int k = BACK ? STEPS - 1 - i : i; f(k, RESET && (s.cuts >> k & 1)); }
 }
 
+// The maps of the chunks before a workgroup's, level by level and by channel. VEC waves, of 64 channels each, have a level: all
+// levels are waited for at once.
+template <int VEC, int WAVES> struct Before {
+    int levels;                            // of the chunks
+    pack<float, VEC> A[LEVELS][WAVE], H[LEVELS][WAVE];
+
+    // own: the chunk's map, wanted of the first VEC waves. Those have level 0, and where they are the last of a group they make the
+    // group's map of its members' and their own at once, and so on up: no map waits for one of a higher level.
+    __device__ void wait(const Records& R, const Shape& S, int64_t b, int64_t p, int64_t d0, int wave, int lane, Map own) {
+        constexpr int TEAMS = WAVES / VEC;
+        const int c = wave % VEC * WAVE + lane, team = wave / VEC;
+        const int64_t d = d0 + c;
+        const bool on = d < S.D;
+        if (team == 0) publish(R.level[0] + (b * S.chunks + p) * S.D + d, own, on);
+        int64_t n = S.chunks;
+        int l = 0;
+        for (bool whole = team == 0; l < LEVELS && n > 0; l++, n /= FAN, p /= FAN) {
+            if (!whole && l % TEAMS != team) continue;
+            const Map m = before_at(R, S, b, l, n, p, d, on);
+            if (l % TEAMS == team) {
+                A[l][0].v[c] = m.A;
+                H[l][0].v[c] = m.H;
+            }
+            whole = whole && p % FAN == FAN - 1 && l + 1 < LEVELS;
+            if (whole) {
+                own = then(m, own);
+                publish(R.level[l + 1] + (b * (n / FAN) + p / FAN) * S.D + d, own, on);
+            }
+        }
+        levels = l;
+    }
+    __device__ float from(float first, int lane, int v) const {
+        for (int l = levels - 1; l >= 0; l--) first = apply({A[l][lane].v[v], H[l][lane].v[v]}, first);
+        return first;
+    }
+};
+
 // The waves' maps of a chunk, by channel
 template <int VEC, int WAVES> struct Maps {
     pack<float, VEC> A[WAVES][WAVE], H[WAVES][WAVE];
@@ -222,7 +247,7 @@ __global__ __launch_bounds__(WAVES* WAVE) void scan_kernel(Shape S, Records R, c
                                                            const float* __restrict__ state, const uint8_t* __restrict__ reset, E* __restrict__ out,
                                                            float* __restrict__ last, float* __restrict__ carry) {
     __shared__ Maps<VEC, WAVES> maps;
-    __shared__ pack<float, VEC> starts[WAVE];
+    __shared__ Before<VEC, WAVES> before;
     const Place<VEC, WAVES, ONE> P(S, R);
     const Span s = span_of(S, reset, P.b, (P.p * WAVES + P.wave) * STEPS, P.lane);
     const uint32_t at = P.on ? P.lane * VEC * sizeof(E) : NO_LANE;
@@ -261,33 +286,25 @@ __global__ __launch_bounds__(WAVES* WAVE) void scan_kernel(Shape S, Records R, c
             for (int v = 0; v < VEC; v++) Z[i][v] = gate_of(float(g[i].v[v]));
         });
     }
-    if constexpr (ONE) {
 #pragma unroll
-        for (int v = 0; v < VEC; v++) h[v] = state && P.on ? state[P.b * S.D + P.d + v] : 0.0f;
-        if (carry && P.on && P.wave == 0)
+    for (int v = 0; v < VEC; v++) h[v] = state && P.on ? state[P.b * S.D + P.d + v] : 0.0f;
+    if constexpr (!ONE) {
+        Map own = {1.0f, 0.0f};
+        if (P.wave < VEC)
 #pragma unroll
-            for (int v = 0; v < VEC; v++) carry[P.b * S.D + P.d + v] = h[v];
-    } else {
-        if (P.wave < VEC) {                // 64 of the workgroup's channels each
-            const int c = P.wave * WAVE + P.lane;
-            const int64_t d = P.d0 + c;
-            const bool on = d < S.D;
-            const float first = state && on ? state[P.b * S.D + d] : 0.0f;
-            Map own = maps.get(0, c);
-#pragma unroll
-            for (int w = 1; w < WAVES; w++) own = then(own, maps.get(w, c));
-            const float start = apply(before_chunk(R, S, P.b, P.p, d, on, own), first);
-            starts[0].v[c] = start;
-            if (carry && on) carry[(P.b * S.chunks + P.p) * S.D + d] = start;
-        }
+            for (int w = 0; w < WAVES; w++) own = then(own, maps.get(w, P.wave * WAVE + P.lane));
+        before.wait(R, S, P.b, P.p, P.d0, P.wave, P.lane, own);
         __syncthreads();
 #pragma unroll
-        for (int v = 0; v < VEC; v++) h[v] = starts[P.lane].v[v];
+        for (int v = 0; v < VEC; v++) h[v] = before.from(h[v], P.lane, v);
     }
     if constexpr (WAVES > 1)
         for (int w = 0; w < P.wave; w++)
 #pragma unroll
             for (int v = 0; v < VEC; v++) h[v] = apply(maps.get(w, P.lane * VEC + v), h[v]);
+    if (carry && P.on && s.steps)
+#pragma unroll
+        for (int v = 0; v < VEC; v++) carry[(P.b * S.spans + s.t0 / STEPS) * S.D + P.d + v] = h[v];
     const Rows to(out + P.b * S.T * S.D + P.d0, S.D, s, width);
     over_steps<RESET, false>(s, [&](int i, bool cut) {
         pack<E, VEC> o;
@@ -311,9 +328,8 @@ __global__ __launch_bounds__(WAVES* WAVE) void scan_back_kernel(Shape S, Records
                                                                 const uint8_t* __restrict__ reset, const float* __restrict__ carry,
                                                                 const E* __restrict__ d_out, const float* __restrict__ d_last, E* __restrict__ d_gate,
                                                                 E* __restrict__ d_value, float* __restrict__ d_state) {
-    __shared__ Maps<VEC, WAVES> maps;                  // forwards: (A, H)
-    __shared__ pack<float, VEC> flows[WAVES][WAVE];    // backwards: (A, flows)
-    __shared__ pack<float, VEC> ends[WAVE];
+    __shared__ Maps<VEC, WAVES> maps;
+    __shared__ Before<VEC, WAVES> before;
     const Place<VEC, WAVES, ONE> P(S, R);
     const int64_t c = S.chunks - 1 - P.p;              // the walk begins at the last chunk
     const Span s = span_of(S, reset, P.b, (c * WAVES + P.wave) * STEPS, P.lane);
@@ -332,56 +348,36 @@ __global__ __launch_bounds__(WAVES* WAVE) void scan_back_kernel(Shape S, Records
         for (int v = 0; v < VEC; v++) Z[i][v] = gate_of(float(g[i].v[v]));
     });
 #pragma unroll
-    for (int v = 0; v < VEC; v++) h[v] = P.on ? carry[(P.b * S.chunks + c) * S.D + P.d + v] : 0.0f;
+    for (int v = 0; v < VEC; v++) h[v] = P.on && s.steps ? carry[(P.b * S.spans + s.t0 / STEPS) * S.D + P.d + v] : 0.0f;
     if constexpr (WAVES > 1) {
         Map m[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; v++) { m[v] = {1.0f, 0.0f}; C[v] = 0.0f; }
-        over_steps<RESET, false>(s, [&](int i, bool cut) {
-#pragma unroll
-            for (int v = 0; v < VEC; v++) {
-                float z, k;
-                both(Z[i][v], z, k);
-                const float in = z * float(x[i].v[v]);
-                m[v].A *= k;
-                m[v].H = cut ? in : fmaf(k, m[v].H, in);
-            }
-        });
-        anew<VEC>(Z);
+        for (int v = 0; v < VEC; v++) m[v] = {1.0f, 0.0f};
         over_steps<RESET, true>(s, [&](int i, bool cut) {
 #pragma unroll
             for (int v = 0; v < VEC; v++) {
                 float z, k;
                 both(Z[i][v], z, k);
-                C[v] = cut ? 0.0f : k * (float(y[i].v[v]) + C[v]);
+                m[v].A *= k;
+                m[v].H = cut ? 0.0f : k * (float(y[i].v[v]) + m[v].H);
             }
         });
         if (RESET && s.cuts)
 #pragma unroll
             for (int v = 0; v < VEC; v++) m[v].A = CUT;
         maps.put(P.wave, P.lane, m);
-#pragma unroll
-        for (int v = 0; v < VEC; v++) flows[P.wave][P.lane].v[v] = C[v];
         __syncthreads();
-        for (int w = 0; w < P.wave; w++)
-#pragma unroll
-            for (int v = 0; v < VEC; v++) h[v] = apply(maps.get(w, P.lane * VEC + v), h[v]);
         anew<VEC>(Z);
-        anew<E, VEC>(x);
         anew<E, VEC>(y);
     }
-    if constexpr (ONE) {
 #pragma unroll
-        for (int v = 0; v < VEC; v++) C[v] = d_last && P.on ? d_last[P.b * S.D + P.d + v] : 0.0f;
-    } else if (P.wave < VEC) {
-        const int k = P.wave * WAVE + P.lane;
-        const int64_t d = P.d0 + k;
-        const bool on = d < S.D;
-        const float first = d_last && on ? d_last[P.b * S.D + d] : 0.0f;
+    for (int v = 0; v < VEC; v++) C[v] = d_last && P.on ? d_last[P.b * S.D + P.d + v] : 0.0f;
+    if constexpr (!ONE) {
         Map own = {1.0f, 0.0f};
+        if (P.wave < VEC)
 #pragma unroll
-        for (int w = WAVES - 1; w >= 0; w--) own = then(own, {maps.get(w, k).A, flows[w][0].v[k]});
-        ends[0].v[k] = apply(before_chunk(R, S, P.b, P.p, d, on, own), first);
+            for (int w = WAVES - 1; w >= 0; w--) own = then(own, maps.get(w, P.wave * WAVE + P.lane));
+        before.wait(R, S, P.b, P.p, P.d0, P.wave, P.lane, own);
     }
     float U[STEPS][VEC];                   // value minus the state before each step
     over_steps<RESET, false>(s, [&](int i, bool cut) {
@@ -398,12 +394,12 @@ __global__ __launch_bounds__(WAVES* WAVE) void scan_back_kernel(Shape S, Records
     if constexpr (!ONE) {
         __syncthreads();
 #pragma unroll
-        for (int v = 0; v < VEC; v++) C[v] = ends[P.lane].v[v];
+        for (int v = 0; v < VEC; v++) C[v] = before.from(C[v], P.lane, v);
     }
     if constexpr (WAVES > 1)
         for (int w = WAVES - 1; w > P.wave; w--)
 #pragma unroll
-            for (int v = 0; v < VEC; v++) C[v] = apply({maps.get(w, P.lane * VEC + v).A, flows[w][P.lane].v[v]}, C[v]);
+            for (int v = 0; v < VEC; v++) C[v] = apply(maps.get(w, P.lane * VEC + v), C[v]);
     anew<VEC>(Z);
     const Rows to_gate(d_gate + P.b * S.T * S.D + P.d0, S.D, s, width), to_value(d_value + P.b * S.T * S.D + P.d0, S.D, s, width);
     over_steps<RESET, true>(s, [&](int i, bool cut) {
@@ -425,6 +421,7 @@ __global__ __launch_bounds__(WAVES* WAVE) void scan_back_kernel(Shape S, Records
         for (int v = 0; v < VEC; v++) d_state[P.b * S.D + P.d + v] = C[v];
 }
 
+int64_t spans_of(int64_t T) { return (T + STEPS - 1) / STEPS; }
 int64_t chunk_steps(int64_t T) { return T <= STEPS ? STEPS : STEPS * CHUNK_WAVES; }
 int64_t chunks_of(int64_t T) { return (T + chunk_steps(T) - 1) / chunk_steps(T); }
 
@@ -452,6 +449,7 @@ template <typename... I> int32_t check(int64_t B, int64_t T, int64_t D, int32_t 
 // f(channels of a lane, waves, one chunk only, resets) with the records cleared
 template <typename F> int32_t launch(Shape& S, bool pairs, bool resets, void* work, hipStream_t st, F&& f) {
     const int vec = pairs ? 2 : 1;
+    S.spans = spans_of(S.T);
     S.chunks = chunks_of(S.T);
     S.tiles = (S.D + WAVE * vec - 1) / (WAVE * vec);
     Records R = {};
@@ -484,7 +482,7 @@ template <typename E> bool pairs_of(const void* p, int64_t B, int64_t T, int64_t
 
 extern "C" {
 
-int64_t pv_gated_scan_chunks(int64_t T) { return T > 0 ? chunks_of(T) : 0; }
+int64_t pv_gated_scan_spans(int64_t T) { return T > 0 ? spans_of(T) : 0; }
 uint64_t pv_gated_scan_work_bytes(int64_t B, int64_t T, int64_t D) {
     return B > 0 && T > 0 && D > 0 ? uint64_t(words_of(B, chunks_of(T), D)) * 8 : 0;
 }
@@ -495,7 +493,7 @@ int32_t pv_gated_scan_hip(const void* gate, const void* value, const float* stat
     if (int32_t e = check(B, T, D, dtype, work, work_bytes, err, errcap, gate_t, value_t, D)) return e;
     if (!B || !D) return PV_OK;
     if (!gate || !value || !out || !last) return fail(PV_EARG, err, errcap, "null argument");
-    Shape S{B, T, D, gate_b, gate_t, value_b, value_t, 0, 0, 0, 0};
+    Shape S{B, T, D, gate_b, gate_t, value_b, value_t, 0, 0, 0, 0, 0};
     const hipStream_t st = hipStream_t(stream);
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
@@ -518,7 +516,7 @@ int32_t pv_gated_scan_backward_hip(const void* gate, const void* value, const fl
     if (int32_t e = check(B, T, D, dtype, work, work_bytes, err, errcap, gate_t, value_t, d_out_t, D)) return e;
     if (!B || !D) return PV_OK;
     if (!gate || !value || !carry || !d_out || !d_gate || !d_value) return fail(PV_EARG, err, errcap, "null argument");
-    Shape S{B, T, D, gate_b, gate_t, value_b, value_t, d_out_b, d_out_t, 0, 0};
+    Shape S{B, T, D, gate_b, gate_t, value_b, value_t, d_out_b, d_out_t, 0, 0, 0};
     const hipStream_t st = hipStream_t(stream);
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);

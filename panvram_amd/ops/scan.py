@@ -29,7 +29,7 @@ def _forward(index, gate, value, state, reset, keep_carry):
     out = torch.empty((B, T, D), dtype=dtype, device=dev)
     last = torch.empty((B, D), dtype=torch.float32, device=dev)
     L = N.lib()
-    carry = torch.empty((B, L.pv_gated_scan_chunks(T), D), dtype=torch.float32, device=dev) if keep_carry else None
+    carry = torch.empty((B, L.pv_gated_scan_spans(T), D), dtype=torch.float32, device=dev) if keep_carry else None
     work, size = _work(L, B, T, D, dev)
     call(L.pv_gated_scan_hip, index, gate.data_ptr(), value.data_ptr(), ptr(state), ptr(reset), B, T, D, gb, gt, vb, vt, DTYPES[dtype], out.data_ptr(),
          last.data_ptr(), ptr(carry), ptr(work), size)
