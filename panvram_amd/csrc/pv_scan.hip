@@ -149,29 +149,47 @@ struct Rows {
         const int bytes = s.steps ? (s.steps - 1) * stride + int(channels * int64_t(sizeof(E))) : 0;
         buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(from + s.t0 * step), 0, bytes, 0x00027000);
     }
-    template <typename P> __device__ P load(int i, uint32_t at) const {
-        P r;
-        if constexpr (sizeof(P) == 4) r.bits = __builtin_amdgcn_raw_buffer_load_b32(buffer, at, i * stride, 0);
-        else r.bits = __builtin_amdgcn_raw_buffer_load_b16(buffer, at, i * stride, 0);
-        return r;
+    template <int BYTES> __device__ uint32_t load(int i, uint32_t at) const {
+        if constexpr (BYTES == 4) return __builtin_amdgcn_raw_buffer_load_b32(buffer, at, i * stride, 0);
+        else return __builtin_amdgcn_raw_buffer_load_b16(buffer, at, i * stride, 0);
     }
-    template <typename P> __device__ void store(const P& v, int i, uint32_t at) const {
-        if constexpr (sizeof(P) == 4) __builtin_amdgcn_raw_buffer_store_b32(v.bits, buffer, at, i * stride, 0);
-        else __builtin_amdgcn_raw_buffer_store_b16(v.bits, buffer, at, i * stride, 0);
+    template <int BYTES> __device__ void store(uint32_t bits, int i, uint32_t at) const {
+        if constexpr (BYTES == 4) __builtin_amdgcn_raw_buffer_store_b32(bits, buffer, at, i * stride, 0);
+        else __builtin_amdgcn_raw_buffer_store_b16(uint16_t(bits), buffer, at, i * stride, 0);
     }
 };
-template <typename P> __device__ inline void load_steps(P* to, const Rows& rows, uint32_t at) {
+
+// A step's VEC values in one register, as they lie in memory. (As elements the compiler would give each a register.)
+template <typename E, int VEC> struct Word {
+    static constexpr int BYTES = VEC * int(sizeof(E));
+    static_assert(BYTES <= 4, "one register");
+    uint32_t bits;
+    __device__ float get(int v) const {
+        if constexpr (sizeof(E) == 4) return __uint_as_float(bits);
+        else if constexpr (std::is_same_v<E, bf16>) return __uint_as_float(v ? bits & 0xffff0000u : bits << 16);
+        else return float(__builtin_bit_cast(f16, uint16_t(bits >> 16 * v)));
+    }
+    static __device__ Word of(const float* x) {
+        if constexpr (sizeof(E) == 4) return {__float_as_uint(x[0])};
+        else if constexpr (VEC == 1) return {__builtin_bit_cast(uint16_t, E(x[0]))};
+        else {
+            using F2 = __attribute__((ext_vector_type(2))) float;
+            using E2 = __attribute__((ext_vector_type(2))) E;
+            return {__builtin_bit_cast(uint32_t, __builtin_convertvector((F2{x[0], x[1]}), E2))};
+        }
+    }
+};
+template <typename E, int VEC> __device__ inline void load_steps(Word<E, VEC>* to, const Rows& rows, uint32_t at) {
 #pragma unroll
-    for (int i = 0; i < STEPS; i++) to[i] = rows.load<P>(i, at);
+    for (int i = 0; i < STEPS; i++) to[i].bits = rows.load<Word<E, VEC>::BYTES>(i, at);
 }
 // Behind the end: gates that leave the state as it is (z = 0), zeros in the other tensors. (A buffer's zeros are no such thing
 // for the gates, and are not there where all steps are one and the same row, stride 0.)
-template <typename E, int VEC> __device__ inline void end_steps(pack<E, VEC>* x, const Span& s, float rest) {
+template <typename E, int VEC> __device__ inline void end_steps(Word<E, VEC>* x, const Span& s, float rest) {
     if (s.steps == STEPS) return;
+    const float both[2] = {rest, rest};
 #pragma unroll
-    for (int i = 0; i < STEPS; i++)
-#pragma unroll
-        for (int v = 0; v < VEC; v++) if (i >= s.steps) x[i].v[v] = E(rest);
+    for (int i = 0; i < STEPS; i++) if (i >= s.steps) x[i] = Word<E, VEC>::of(both);
 }
 // The compiler is to make what follows from these registers again where it needs it: kept from one walk over the steps to the
 // next, z, 1 - z and the products would take two to four times the registers
@@ -181,13 +199,9 @@ template <int VEC> __device__ inline void anew(float (*q)[VEC]) {
 #pragma unroll
         for (int v = 0; v < VEC; v++) asm volatile("" : "+v"(q[i][v]));
 }
-template <typename E, int VEC> __device__ inline void anew(pack<E, VEC>* x) {
+template <typename E, int VEC> __device__ inline void anew(Word<E, VEC>* x) {
 #pragma unroll
-    for (int i = 0; i < STEPS; i++) {
-        uint32_t w = x[i].bits;
-        asm volatile("" : "+v"(w));
-        x[i].bits = typename pack<E, VEC>::raw(w);
-    }
+    for (int i = 0; i < STEPS; i++) asm volatile("" : "+v"(x[i].bits));
 }
 // f(i, whether step i has a reset) over the steps in order or backwards
 template <bool RESET, bool BACK, typename F> __device__ inline void over_steps(const Span& s, F&& f) {
@@ -243,7 +257,7 @@ template <int VEC, int WAVES> struct Maps {
 };
 
 template <typename E, int VEC, int WAVES, bool ONE, bool RESET>
-__global__ __launch_bounds__(WAVES* WAVE) void scan_kernel(Shape S, Records R, const E* __restrict__ gate, const E* __restrict__ value,
+__global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC == 2 && WAVES > 1 ? 6 : 1))) void scan_kernel(Shape S, Records R, const E* __restrict__ gate, const E* __restrict__ value,
                                                            const float* __restrict__ state, const uint8_t* __restrict__ reset, E* __restrict__ out,
                                                            float* __restrict__ last, float* __restrict__ carry) {
     __shared__ Maps<VEC, WAVES> maps;
@@ -252,7 +266,7 @@ __global__ __launch_bounds__(WAVES* WAVE) void scan_kernel(Shape S, Records R, c
     const Span s = span_of(S, reset, P.b, (P.p * WAVES + P.wave) * STEPS, P.lane);
     const uint32_t at = P.on ? P.lane * VEC * sizeof(E) : NO_LANE;
     const int64_t width = S.D - P.d0 < WAVE * VEC ? S.D - P.d0 : WAVE * VEC;
-    pack<E, VEC> g[STEPS], x[STEPS];
+    Word<E, VEC> g[STEPS], x[STEPS];
     load_steps(g, Rows(gate + P.b * S.gb + P.d0, S.gt, s, width), at);
     load_steps(x, Rows(value + P.b * S.vb + P.d0, S.vt, s, width), at);
     end_steps<E, VEC>(g, s, -INFINITY);
@@ -265,10 +279,10 @@ __global__ __launch_bounds__(WAVES* WAVE) void scan_kernel(Shape S, Records R, c
         over_steps<RESET, false>(s, [&](int i, bool cut) {
 #pragma unroll
             for (int v = 0; v < VEC; v++) {
-                Z[i][v] = gate_of(float(g[i].v[v]));
+                Z[i][v] = gate_of(g[i].get(v));
                 float z, k;
                 both(Z[i][v], z, k);
-                const float in = z * float(x[i].v[v]);
+                const float in = z * x[i].get(v);
                 m[v].A *= k;
                 m[v].H = cut ? in : fmaf(k, m[v].H, in);
             }
@@ -283,7 +297,7 @@ __global__ __launch_bounds__(WAVES* WAVE) void scan_kernel(Shape S, Records R, c
     } else {
         over_steps<RESET, false>(s, [&](int i, bool) {
 #pragma unroll
-            for (int v = 0; v < VEC; v++) Z[i][v] = gate_of(float(g[i].v[v]));
+            for (int v = 0; v < VEC; v++) Z[i][v] = gate_of(g[i].get(v));
         });
     }
 #pragma unroll
@@ -307,16 +321,16 @@ __global__ __launch_bounds__(WAVES* WAVE) void scan_kernel(Shape S, Records R, c
         for (int v = 0; v < VEC; v++) carry[(P.b * S.spans + s.t0 / STEPS) * S.D + P.d + v] = h[v];
     const Rows to(out + P.b * S.T * S.D + P.d0, S.D, s, width);
     over_steps<RESET, false>(s, [&](int i, bool cut) {
-        pack<E, VEC> o;
+        float o[VEC];
 #pragma unroll
         for (int v = 0; v < VEC; v++) {
             float z, k;
             both(Z[i][v], z, k);
-            const float in = z * float(x[i].v[v]);
+            const float in = z * x[i].get(v);
             h[v] = cut ? in : fmaf(k, h[v], in);
-            o.v[v] = E(h[v]);
+            o[v] = h[v];
         }
-        to.store(o, i, at);
+        to.store<Word<E, VEC>::BYTES>(Word<E, VEC>::of(o).bits, i, at);
     });
     if (P.on && s.steps && s.t0 + s.steps == S.T)
 #pragma unroll
@@ -324,7 +338,7 @@ __global__ __launch_bounds__(WAVES* WAVE) void scan_kernel(Shape S, Records R, c
 }
 
 template <typename E, int VEC, int WAVES, bool ONE, bool RESET>
-__global__ __launch_bounds__(WAVES* WAVE) void scan_back_kernel(Shape S, Records R, const E* __restrict__ gate, const E* __restrict__ value,
+__global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC == 2 && WAVES > 1 ? 4 : 1))) void scan_back_kernel(Shape S, Records R, const E* __restrict__ gate, const E* __restrict__ value,
                                                                 const uint8_t* __restrict__ reset, const float* __restrict__ carry,
                                                                 const E* __restrict__ d_out, const float* __restrict__ d_last, E* __restrict__ d_gate,
                                                                 E* __restrict__ d_value, float* __restrict__ d_state) {
@@ -335,7 +349,7 @@ __global__ __launch_bounds__(WAVES* WAVE) void scan_back_kernel(Shape S, Records
     const Span s = span_of(S, reset, P.b, (c * WAVES + P.wave) * STEPS, P.lane);
     const uint32_t at = P.on ? P.lane * VEC * sizeof(E) : NO_LANE;
     const int64_t width = S.D - P.d0 < WAVE * VEC ? S.D - P.d0 : WAVE * VEC;
-    pack<E, VEC> g[STEPS], x[STEPS], y[STEPS];
+    Word<E, VEC> g[STEPS], x[STEPS], y[STEPS];
     load_steps(g, Rows(gate + P.b * S.gb + P.d0, S.gt, s, width), at);
     load_steps(x, Rows(value + P.b * S.vb + P.d0, S.vt, s, width), at);
     load_steps(y, Rows(d_out + P.b * S.db + P.d0, S.dt, s, width), at);
@@ -345,7 +359,7 @@ __global__ __launch_bounds__(WAVES* WAVE) void scan_back_kernel(Shape S, Records
     float Z[STEPS][VEC], C[VEC], h[VEC];
     over_steps<RESET, false>(s, [&](int i, bool) {
 #pragma unroll
-        for (int v = 0; v < VEC; v++) Z[i][v] = gate_of(float(g[i].v[v]));
+        for (int v = 0; v < VEC; v++) Z[i][v] = gate_of(g[i].get(v));
     });
 #pragma unroll
     for (int v = 0; v < VEC; v++) h[v] = P.on && s.steps ? carry[(P.b * S.spans + s.t0 / STEPS) * S.D + P.d + v] : 0.0f;
@@ -359,7 +373,7 @@ __global__ __launch_bounds__(WAVES* WAVE) void scan_back_kernel(Shape S, Records
                 float z, k;
                 both(Z[i][v], z, k);
                 m[v].A *= k;
-                m[v].H = cut ? 0.0f : k * (float(y[i].v[v]) + m[v].H);
+                m[v].H = cut ? 0.0f : k * (y[i].get(v) + m[v].H);
             }
         });
         if (RESET && s.cuts)
@@ -386,7 +400,7 @@ __global__ __launch_bounds__(WAVES* WAVE) void scan_back_kernel(Shape S, Records
             float z, k;
             both(Z[i][v], z, k);
             if (cut) h[v] = 0.0f;
-            const float a = float(x[i].v[v]);
+            const float a = x[i].get(v);
             U[i][v] = a - h[v];
             h[v] = fmaf(k, h[v], z * a);
         }
@@ -403,18 +417,18 @@ __global__ __launch_bounds__(WAVES* WAVE) void scan_back_kernel(Shape S, Records
     anew<VEC>(Z);
     const Rows to_gate(d_gate + P.b * S.T * S.D + P.d0, S.D, s, width), to_value(d_value + P.b * S.T * S.D + P.d0, S.D, s, width);
     over_steps<RESET, true>(s, [&](int i, bool cut) {
-        pack<E, VEC> og, ov;
+        float og[VEC], ov[VEC];
 #pragma unroll
         for (int v = 0; v < VEC; v++) {
             float z, k;
             both(Z[i][v], z, k);
-            const float G = float(y[i].v[v]) + C[v], in = z * G;
-            ov.v[v] = E(in);
-            og.v[v] = E(in * k * U[i][v]);
+            const float G = y[i].get(v) + C[v], in = z * G;
+            ov[v] = in;
+            og[v] = in * k * U[i][v];
             C[v] = cut ? 0.0f : k * G;
         }
-        to_value.store(ov, i, at);
-        to_gate.store(og, i, at);
+        to_value.store<Word<E, VEC>::BYTES>(Word<E, VEC>::of(ov).bits, i, at);
+        to_gate.store<Word<E, VEC>::BYTES>(Word<E, VEC>::of(og).bits, i, at);
     });
     if (d_state && P.on && c == 0 && P.wave == 0)
 #pragma unroll
