@@ -63,7 +63,7 @@ template <bool WIDE, typename E, int N> __device__ inline pack<E, N> get(const E
 }
 template <bool WIDE, typename E, int N> __device__ inline void put(const pack<E, N>& v, E* p, int64_t left) {
     if constexpr (WIDE) {
-        if (left > 0) v.store(p);
+        if (left > 0) v.store_once(p);
     } else {
 #pragma unroll
         for (int j = 0; j < N; j++) if (j < left) p[j] = v.v[j];
@@ -285,28 +285,23 @@ __global__ __launch_bounds__(BLOCK) void begin_kernel(Shape S, const void* token
         counts[blockIdx.x] = k;
         return;
     }
-    const int64_t e = int64_t(blockIdx.x - counting) * BLOCK + threadIdx.x, v = e / S.Dp, i = e % S.Dp;
-    if (v >= VMAX) return;
+    const int v = (blockIdx.x - counting) % VMAX;
+    const int64_t i = int64_t((blockIdx.x - counting) / VMAX) * BLOCK + threadIdx.x;
+    if (i >= S.Dp) return;
     const K x = v < S.V && i < S.D ? K(float(weight[v * S.D + i])) : K(0.0f);
-    wr[e] = x;
+    wr[v * S.Dp + i] = x;
     if (wc) wc[i * VMAX + v] = x;
 }
 
-// Logits, losses and all gradients in one pass over hidden; a wave for each slab of the row
-template <typename M>
+// Logits, losses and, with GRADS, all gradients in one pass over hidden; a wave for each slab of the row
+template <typename M, bool GRADS>
 __global__ __launch_bounds__(MOST_WAVES* WAVE)
 void fused_kernel(Shape S, const typename M::E* __restrict__ hidden, const void* __restrict__ tokens, const typename M::K* __restrict__ wr,
                   const typename M::K* __restrict__ wc, const int64_t* counts, const float* scale, const float* __restrict__ factor, float* __restrict__ each,
                   typename M::E* __restrict__ d_hidden, double* sums, float* __restrict__ parts) {
     extern __shared__ f32x4 lds[];         // partial logits, for this tile and the one before: [2][waves][lanes]
-    const int wave = threadIdx.x / WAVE, waves = blockDim.x / WAVE, lane = threadIdx.x % WAVE, c = lane_c();
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), waves = blockDim.x / WAVE, lane = threadIdx.x % WAVE, c = lane_c();
     const int64_t c0 = int64_t(wave) * M::COLS;
-    M m;
-    m.weights(wr, S.Dp, c0);
-    m.weights_back(wc, c0);
-    typename M::Sums sum = {};
-    const float base = counts ? mean_factor(counts, scale) : 0.0f;
-    double loss = 0.0;
     struct Next { typename M::Rows rows; int at; float w; } next;
     auto fetch = [&](int64_t tile) {
         const int64_t n = tile * TILE + c;
@@ -315,36 +310,43 @@ void fused_kernel(Shape S, const typename M::E* __restrict__ hidden, const void*
         split(S, on ? n : 0, b, t);
         next.rows = M::rows(place(S, hidden, b, t, on ? n : 0), c0, S.D, on);
         next.at = on ? target(S, tokens, b, t) : -1;
-        next.w = factor && on ? factor[n] : base;
+        if (GRADS) next.w = factor && on ? factor[n] : 0.0f;
     };
     const int64_t tiles = (S.N + TILE - 1) / TILE;
-    int turn = 0;
     if (blockIdx.x < tiles) fetch(blockIdx.x);
+    M m;
+    m.weights(wr, S.Dp, c0);
+    if (GRADS) m.weights_back(wc, c0);
+    typename M::Sums sum = {};
+    const float base = GRADS && counts ? mean_factor(counts, scale) : 0.0f;
+    double loss = 0.0;
+    int turn = 0;
     for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
         Next now = next;
         if (tile + gridDim.x < tiles) fetch(tile + gridDim.x);
-        if (now.at < 0) M::clear(now.rows);
+        if (GRADS && now.at < 0) M::clear(now.rows);
         f32x4 l = m.logits(now.rows, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
         if (waves > 1) {
             f32x4* mine = lds + turn * waves * WAVE;
             mine[wave * WAVE + lane] = l;
             __syncthreads();               // (the other half is free again: every wave has passed the tile before)
+            if (!GRADS && wave) continue;
             l = mine[lane];
             for (int k = 1; k < waves; k++) l += mine[k * WAVE + lane];
         }
-        const float x = softmax(l, now.at, S.V, now.w);
+        const float x = softmax(l, now.at, S.V, factor ? now.w : base);
         const int64_t n = tile * TILE + c;
         if (wave == 0 && lane < TILE && n < S.N) {
             loss += double(x);
             if (each) each[n] = x;
         }
-        m.back(now.rows, l, d_hidden + n * S.D, c0, S.D, n < S.N, sum);
+        if (GRADS) m.back(now.rows, l, d_hidden + n * S.D, c0, S.D, n < S.N, sum);
     }
     if (wave == 0) {
         loss = wave_total(loss);
         if (lane == 0) sums[blockIdx.x] = loss;
     }
-    if (c < S.V) {
+    if (GRADS && c < S.V) {
 #pragma unroll
         for (int k = 0; k < M::TILES; k++) *reinterpret_cast<f32x4*>(parts + (int64_t(blockIdx.x) * S.V + c) * S.Dp + c0 + 16 * k + 4 * lane_g()) = sum.dw[k];
     }
@@ -449,22 +451,23 @@ __global__ __launch_bounds__(END_WAVES* WAVE) void end_kernel(Shape S, const int
     if (i < S.D) d_weight[v * S.D + i] = W(x);
 }
 
-// How a call is cut up: columns of a slab, waves of a fused workgroup (0: the row has more slabs than that), workgroups
+// How a call is cut up: D in whole slabs, waves of a fused workgroup (0: the row has more slabs than that), workgroups
 struct Cut { int64_t Dp; int waves, groups; };
-Cut cut_of(int64_t N, int64_t D, bool narrow) {
+Cut cut_of(int64_t N, int64_t D, bool narrow, bool gradients) {
     const int64_t cols = narrow ? 128 : 64, slabs = (D + cols - 1) / cols, tiles = (N + TILE - 1) / TILE;
     Cut k;
     k.Dp = slabs * cols;
     k.waves = slabs <= MOST_WAVES ? int(slabs) : 0;
-    const int64_t most = k.waves ? 256 * (MOST_WAVES / k.waves) : 256;      // 16 waves a CU
-    k.groups = int(tiles < most ? tiles : most);
+    const int64_t most = k.waves ? 256 * ((gradients ? 16 : 24) / k.waves) : 256;      // of 256 CUs, 16 or 24 waves a CU
+    const int64_t rounds = (tiles + most - 1) / most;                          // all workgroups have as many tiles, one less here and there
+    k.groups = int((tiles + rounds - 1) / rounds);
     return k;
 }
 constexpr int PLACE_GROUPS = 2048;
 
 struct Work { int64_t* counts; double* sums; char *wr, *wc; float *d_logits, *parts; uint64_t bytes; };
 Work layout(void* work, int64_t N, int64_t D, int32_t V, bool narrow, bool gradients) {
-    const Cut k = cut_of(N, D, narrow);
+    const Cut k = cut_of(N, D, narrow, gradients);
     const uint64_t e = narrow ? 2 : 4;
     char* at = static_cast<char*>(work);
     auto take = [&](uint64_t bytes) { char* p = at; at += (bytes + 15) & ~15ull; return p; };
@@ -486,19 +489,21 @@ int32_t run(Shape S, const void* hidden_, const void* weight, const void* tokens
     using K = typename M::K;
     const bool narrow = sizeof(K) == 2, grads = d_hidden_;
     const Work w = layout(work, S.N, S.D, S.V, narrow, grads);
-    const Cut k = cut_of(S.N, S.D, narrow);
+    const Cut k = cut_of(S.N, S.D, narrow, grads);
     S.Dp = k.Dp;
     const E* hidden = static_cast<const E*>(hidden_);
     E* d_hidden = static_cast<E*>(d_hidden_);
     K *wr = reinterpret_cast<K*>(w.wr), *wc = reinterpret_cast<K*>(w.wc);
     const bool mean = loss || (grads && !factor);
     const int counting = mean ? COUNTS : 0;
-    begin_kernel<W, K><<<counting + (VMAX * k.Dp + BLOCK - 1) / BLOCK, BLOCK, 0, st>>>(S, tokens, counting, w.counts, static_cast<const W*>(weight), wr, wc);
+    begin_kernel<W, K><<<counting + VMAX * ((k.Dp + BLOCK - 1) / BLOCK), BLOCK, 0, st>>>(S, tokens, counting, w.counts, static_cast<const W*>(weight), wr, wc);
     const int64_t* counts = mean ? w.counts : nullptr;
     int nsums = k.groups;
+    const size_t exchange = 2 * k.waves * WAVE * sizeof(f32x4);
     if (grads && k.waves) {
-        fused_kernel<M><<<k.groups, k.waves * WAVE, 2 * k.waves * WAVE * sizeof(f32x4), st>>>(S, hidden, tokens, wr, wc, counts, scale, factor, each, d_hidden, w.sums,
-                                                                                             w.parts);
+        fused_kernel<M, true><<<k.groups, k.waves * WAVE, exchange, st>>>(S, hidden, tokens, wr, wc, counts, scale, factor, each, d_hidden, w.sums, w.parts);
+    } else if (k.waves) {
+        fused_kernel<M, false><<<k.groups, k.waves * WAVE, exchange, st>>>(S, hidden, tokens, wr, nullptr, nullptr, nullptr, nullptr, each, nullptr, w.sums, nullptr);
     } else {
         const int64_t need = (S.N + TILE * (BLOCK / WAVE) - 1) / (TILE * (BLOCK / WAVE));
         nsums = int(need < PLACE_GROUPS ? need : PLACE_GROUPS);
