@@ -70,34 +70,45 @@ template <bool WIDE, typename E, int N> __device__ inline void put(const pack<E,
     }
 }
 
+// f(true) for a slab that lies within the row and is read 16 bytes at a time, else f(false): asked once, not at each load
+template <bool WIDE, typename F> __device__ inline void over_slab(bool within, F&& f) {
+    if (WIDE && within) f(std::true_type{}); else f(std::false_type{});
+}
+
 // A slab of 128 columns in bfloat16
 template <typename E_, bool WIDE> struct Bf {
     using E = E_;
     using K = __bf16;                      // what the weights are laid out as
     static constexpr int COLS = 128, STEPS = 4, TILES = 8;
     struct Rows { bf16x8 h[STEPS]; };      // column 32 q + 8 g + j of place c
-    struct Sums { f32x4 dw[TILES]; };      // id c, columns 16 k + 4 g + r
+    struct Sums { f32x4 dw[TILES]; };      // id c, columns 32 q + 8 g + 4 t + r at 2 q + t
     bf16x8 w[STEPS];                       // id c, columns as Rows
-    s16x4 wt[TILES];                       // column 32 q + 8 (c / 4) + 4 t + c % 4 at 2 q + t, ids 4 g + j
+    using Back = s16x4;
+    const Back* wt;                        // [TILES][lanes], in LDS: column 32 q + 8 (c / 4) + 4 t + c % 4 at 2 q + t, ids 4 g + j
 
     __device__ void weights(const K* wr, int64_t Dp, int64_t c0) {
 #pragma unroll
         for (int q = 0; q < STEPS; q++) w[q] = *reinterpret_cast<const bf16x8*>(wr + lane_c() * Dp + c0 + 32 * q + 8 * lane_g());
     }
-    __device__ void weights_back(const K* wc, int64_t c0) {
+    // (to: the wave's own room, so no other wave waits for it)
+    __device__ void weights_back(const K* wc, int64_t c0, Back* to) {
         const int c = lane_c();
+        to += threadIdx.x % WAVE;
 #pragma unroll
         for (int k = 0; k < TILES; k++)
-            wt[k] = *reinterpret_cast<const s16x4*>(wc + (c0 + 32 * (k / 2) + 8 * (c / 4) + 4 * (k % 2) + c % 4) * VMAX + 4 * lane_g());
+            to[k * WAVE] = *reinterpret_cast<const Back*>(wc + (c0 + 32 * (k / 2) + 8 * (c / 4) + 4 * (k % 2) + c % 4) * VMAX + 4 * lane_g());
+        wt = to;
     }
-    static __device__ Rows rows(const E* row, int64_t c0, int64_t D, bool on) {
+    static __device__ Rows rows(const E* row, int64_t c0, int64_t D) {
         Rows R;
+        row += c0 + 8 * lane_g();
+        over_slab<WIDE>(c0 + COLS <= D, [&](auto whole) {
 #pragma unroll
-        for (int q = 0; q < STEPS; q++) {
-            const int64_t i = c0 + 32 * q + 8 * lane_g();
-            const auto p = get<WIDE, E, 8>(row + i, on ? D - i : 0);
-            __builtin_memcpy(&R.h[q], &p, 16);
-        }
+            for (int q = 0; q < STEPS; q++) {
+                const auto p = whole ? pack<E, 8>::load(row + 32 * q) : get<WIDE, E, 8>(row + 32 * q, D - c0 - 32 * q - 8 * lane_g());
+                __builtin_memcpy(&R.h[q], &p, 16);
+            }
+        });
         return R;
     }
     static __device__ void clear(Rows& R) {
@@ -123,30 +134,33 @@ template <typename E_, bool WIDE> struct Bf {
         const s16x4 hi = bits(dl);
         const s16x4 lo = bits(dl - __builtin_convertvector(__builtin_bit_cast(bf16x4, hi), f32x4));
         s16x4 one;                         // the identity, 16 x 16
-        bf16x8 half[2];                    // columns 0..15 and 16..31 of the identity, 32 x 32
 #pragma unroll
         for (int j = 0; j < 4; j++) one[j] = c == 4 * g + j ? 0x3f80 : 0;
-#pragma unroll
-        for (int j = 0; j < 8; j++) { half[0][j] = __bf16(c == 8 * g + j ? 1.0f : 0.0f); half[1][j] = __bf16(c + 16 == 8 * g + j ? 1.0f : 0.0f); }
         const s16x4 thi = bits(product(hi, one, none)), tlo = bits(product(lo, one, none));      // id c, places 4 g + j
+        const bool whole = WIDE && c0 + COLS <= D;
+        d_row += c0 + 8 * g;
 #pragma unroll
         for (int q = 0; q < STEPS; q++) {
-#pragma unroll
-            for (int s = 0; s < 2; s++) {
-                const s16x4 ht = bits(__builtin_amdgcn_mfma_f32_16x16x32_bf16(R.h[q], half[s], none, 0, 0, 0));      // column 32 q + 16 s + c, places 4 g + j
-                S.dw[2 * q + s] = product(ht, tlo, product(ht, thi, S.dw[2 * q + s]));
-            }
-            pack<E, 8> o;
+            bf16x4 o[2];
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                const f32x4 x = product(wt[2 * q + t], lo, product(wt[2 * q + t], hi, none));
+                bf16x4 h;                  // column 32 q + 8 g + 4 t + j of place c; turned: column 32 q + 8 (c / 4) + 4 t + c % 4, places 4 g + j
 #pragma unroll
-                for (int r = 0; r < 4; r++) o.v[4 * t + r] = E(x[r]);
+                for (int j = 0; j < 4; j++) h[j] = R.h[q][4 * t + j];
+                const s16x4 ht = bits(product(__builtin_bit_cast(s16x4, h), one, none));
+                S.dw[2 * q + t] = product(ht, tlo, product(ht, thi, S.dw[2 * q + t]));
+                o[t] = __builtin_convertvector(product(wt[(2 * q + t) * WAVE], lo, product(wt[(2 * q + t) * WAVE], hi, none)), bf16x4);
             }
-            const int64_t i = c0 + 32 * q + 8 * g;
-            put<WIDE, E, 8>(o, d_row + i, store ? D - i : 0);
+            if (store) {
+                pack<E, 8> p;
+                __builtin_memcpy(&p, o, 16);
+                if (whole) p.store_once(d_row + 32 * q);
+                else put<WIDE, E, 8>(p, d_row + 32 * q, D - c0 - 32 * q - 8 * g);
+            }
         }
     }
+    // where the columns of result k's rows 4 g + r begin
+    static __device__ int column(int k) { return 32 * (k / 2) + 8 * lane_g() + 4 * (k % 2); }
 };
 
 // A slab of 64 columns in 32 bits
@@ -156,23 +170,27 @@ template <typename E_, bool WIDE> struct F3 {
     static constexpr int COLS = 64, STEPS = 4, TILES = 4;
     struct Rows { pack<E, 4> h[STEPS]; };  // column 16 s + 4 g + j of place c
     struct Sums { f32x4 dw[TILES]; };      // id c, columns 16 s + 4 g + r
-    f32x4 w[STEPS], wt[TILES];             // id c, columns as Rows; column 16 s + c, ids 4 g + j
+    f32x4 w[STEPS];                        // id c, columns as Rows
+    using Back = f32x4;
+    const Back* wt;                        // [TILES][lanes], in LDS: column 16 s + c, ids 4 g + j
 
     __device__ void weights(const K* wr, int64_t Dp, int64_t c0) {
 #pragma unroll
         for (int s = 0; s < STEPS; s++) w[s] = *reinterpret_cast<const f32x4*>(wr + lane_c() * Dp + c0 + 16 * s + 4 * lane_g());
     }
-    __device__ void weights_back(const K* wc, int64_t c0) {
+    __device__ void weights_back(const K* wc, int64_t c0, Back* to) {
+        to += threadIdx.x % WAVE;
 #pragma unroll
-        for (int s = 0; s < TILES; s++) wt[s] = *reinterpret_cast<const f32x4*>(wc + (c0 + 16 * s + lane_c()) * VMAX + 4 * lane_g());
+        for (int s = 0; s < TILES; s++) to[s * WAVE] = *reinterpret_cast<const Back*>(wc + (c0 + 16 * s + lane_c()) * VMAX + 4 * lane_g());
+        wt = to;
     }
-    static __device__ Rows rows(const E* row, int64_t c0, int64_t D, bool on) {
+    static __device__ Rows rows(const E* row, int64_t c0, int64_t D) {
         Rows R;
+        row += c0 + 4 * lane_g();
+        over_slab<WIDE>(c0 + COLS <= D, [&](auto whole) {
 #pragma unroll
-        for (int s = 0; s < STEPS; s++) {
-            const int64_t i = c0 + 16 * s + 4 * lane_g();
-            R.h[s] = get<WIDE, E, 4>(row + i, on ? D - i : 0);
-        }
+            for (int s = 0; s < STEPS; s++) R.h[s] = whole ? pack<E, 4>::load(row + 16 * s) : get<WIDE, E, 4>(row + 16 * s, D - c0 - 16 * s - 4 * lane_g());
+        });
         return R;
     }
     static __device__ void clear(Rows& R) {
@@ -198,20 +216,26 @@ template <typename E_, bool WIDE> struct F3 {
         f32x4 t = none;                    // id c, places 4 g + j
 #pragma unroll
         for (int j = 0; j < 4; j++) t = product(dl[j], one[j], t);
+        const bool whole = WIDE && c0 + COLS <= D;
+        d_row += c0 + 4 * g;
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
             f32x4 ht = none, x = none;     // ht: column 16 s + c, places 4 g + j
+            const f32x4 ws = wt[s * WAVE];
 #pragma unroll
             for (int j = 0; j < 4; j++) ht = product(float(R.h[s].v[j]), one[j], ht);
 #pragma unroll
-            for (int j = 0; j < 4; j++) { S.dw[s] = product(ht[j], t[j], S.dw[s]); x = product(wt[s][j], dl[j], x); }
-            pack<E, 4> o;
+            for (int j = 0; j < 4; j++) { S.dw[s] = product(ht[j], t[j], S.dw[s]); x = product(ws[j], dl[j], x); }
+            if (store) {
+                pack<E, 4> o;
 #pragma unroll
-            for (int r = 0; r < 4; r++) o.v[r] = E(x[r]);
-            const int64_t i = c0 + 16 * s + 4 * g;
-            put<WIDE, E, 4>(o, d_row + i, store ? D - i : 0);
+                for (int r = 0; r < 4; r++) o.v[r] = E(x[r]);
+                if (whole) o.store_once(d_row + 16 * s);
+                else put<WIDE, E, 4>(o, d_row + 16 * s, D - c0 - 16 * s - 4 * g);
+            }
         }
     }
+    static __device__ int column(int k) { return 16 * k + 4 * lane_g(); }
 };
 
 // Place n: where its row is, and the id that it predicts (-1: it does not count)
@@ -242,27 +266,38 @@ __device__ inline float mean_factor(const int64_t* counts, const float* scale) {
     return (scale ? *scale : 1.0f) / float(k > 0 ? k : 1);
 }
 
-// A place's loss from its logits (place c, ids 4 g + r), and in their place the gradients of the logits times `w`
-__device__ inline float softmax(f32x4& l, int at, int V, float w) {
+// x joined with the values of the lanes of the same c (l ^ 16, l ^ 32, l ^ 48)
+template <typename F> __device__ inline float over_groups(float x, F&& join) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = join(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return join(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
+// Logits (place c, ids 4 g + r) made the gradients of the place's loss times `w` (0 where it does not count); the loss itself
+// where it is wanted (wave-uniform)
+__device__ inline float softmax(f32x4& l, int at, int V, float w, bool loss) {
     const int first = 4 * lane_g();
-    float top = -INFINITY, total = 0.0f, own = 0.0f;
+    const auto sum = [](float a, float b) { return a + b; };
+    float top = -INFINITY, total = 0.0f, x = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-        if (first + r == at) own = l[r];
-        if (first + r < V) top = fmaxf(top, l[r]);
+    for (int r = 0; r < 4; r++) if (first + r < V) top = fmaxf(top, l[r]);
+    top = over_groups(top, [](float a, float b) { return fmaxf(a, b); });
+    f32x4 e;
+#pragma unroll
+    for (int r = 0; r < 4; r++) { e[r] = first + r < V ? __expf(l[r] - top) : 0.0f; total += e[r]; }
+    total = over_groups(total, sum);
+    if (loss) {
+        float own = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 4; r++) own += first + r == at ? l[r] : 0.0f;
+        own = over_groups(own, sum);
+        x = at >= 0 ? logf(total) + (top - own) : 0.0f;
     }
-    top = fmaxf(top, __shfl_xor(top, 16, WAVE));
-    top = fmaxf(top, __shfl_xor(top, 32, WAVE));
+    const float up = __builtin_amdgcn_rcpf(total);
 #pragma unroll
-    for (int r = 0; r < 4; r++) { l[r] = first + r < V ? expf(l[r] - top) : 0.0f; total += l[r]; }
-    total += __shfl_xor(total, 16, WAVE);
-    total += __shfl_xor(total, 32, WAVE);
-    own += __shfl_xor(own, 16, WAVE);
-    own += __shfl_xor(own, 32, WAVE);
-    const float up = 1.0f / total;
-#pragma unroll
-    for (int r = 0; r < 4; r++) l[r] = at >= 0 ? (l[r] * up - (first + r == at ? 1.0f : 0.0f)) * w : 0.0f;
-    return at >= 0 ? logf(total) + top - own : 0.0f;
+    for (int r = 0; r < 4; r++) l[r] = at >= 0 ? (e[r] * up - (first + r == at ? 1.0f : 0.0f)) * w : 0.0f;
+    return x;
 }
 
 // Workgroups below `counting`: how many places count. The others: the weights, filled up with zeros to 16 ids and whole slabs,
@@ -299,7 +334,7 @@ __global__ __launch_bounds__(MOST_WAVES* WAVE)
 void fused_kernel(Shape S, const typename M::E* __restrict__ hidden, const void* __restrict__ tokens, const typename M::K* __restrict__ wr,
                   const typename M::K* __restrict__ wc, const int64_t* counts, const float* scale, const float* __restrict__ factor, float* __restrict__ each,
                   typename M::E* __restrict__ d_hidden, double* sums, float* __restrict__ parts) {
-    extern __shared__ f32x4 lds[];         // partial logits, for this tile and the one before: [2][waves][lanes]
+    extern __shared__ f32x4 lds[];         // partial logits, for this tile and the one before: [2][waves][lanes]; then the waves' wt
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), waves = blockDim.x / WAVE, lane = threadIdx.x % WAVE, c = lane_c();
     const int64_t c0 = int64_t(wave) * M::COLS;
     struct Next { typename M::Rows rows; int at; float w; } next;
@@ -308,7 +343,7 @@ void fused_kernel(Shape S, const typename M::E* __restrict__ hidden, const void*
         const bool on = n < S.N;
         int64_t b, t;
         split(S, on ? n : 0, b, t);
-        next.rows = M::rows(place(S, hidden, b, t, on ? n : 0), c0, S.D, on);
+        next.rows = M::rows(place(S, hidden, b, t, on ? n : 0), c0, S.D);
         next.at = on ? target(S, tokens, b, t) : -1;
         if (GRADS) next.w = factor && on ? factor[n] : 0.0f;
     };
@@ -316,7 +351,7 @@ void fused_kernel(Shape S, const typename M::E* __restrict__ hidden, const void*
     if (blockIdx.x < tiles) fetch(blockIdx.x);
     M m;
     m.weights(wr, S.Dp, c0);
-    if (GRADS) m.weights_back(wc, c0);
+    if (GRADS) m.weights_back(wc, c0, reinterpret_cast<typename M::Back*>(lds + 2 * waves * WAVE) + wave * M::TILES * WAVE);
     typename M::Sums sum = {};
     const float base = GRADS && counts ? mean_factor(counts, scale) : 0.0f;
     double loss = 0.0;
@@ -334,7 +369,7 @@ void fused_kernel(Shape S, const typename M::E* __restrict__ hidden, const void*
             l = mine[lane];
             for (int k = 1; k < waves; k++) l += mine[k * WAVE + lane];
         }
-        const float x = softmax(l, now.at, S.V, factor ? now.w : base);
+        const float x = softmax(l, now.at, S.V, factor ? now.w : base, wave == 0);
         const int64_t n = tile * TILE + c;
         if (wave == 0 && lane < TILE && n < S.N) {
             loss += double(x);
@@ -348,7 +383,7 @@ void fused_kernel(Shape S, const typename M::E* __restrict__ hidden, const void*
     }
     if (GRADS && c < S.V) {
 #pragma unroll
-        for (int k = 0; k < M::TILES; k++) *reinterpret_cast<f32x4*>(parts + (int64_t(blockIdx.x) * S.V + c) * S.Dp + c0 + 16 * k + 4 * lane_g()) = sum.dw[k];
+        for (int k = 0; k < M::TILES; k++) *reinterpret_cast<f32x4*>(parts + (int64_t(blockIdx.x) * S.V + c) * S.Dp + c0 + M::column(k)) = sum.dw[k];
     }
 }
 
@@ -373,9 +408,9 @@ __global__ __launch_bounds__(BLOCK) void place_kernel(Shape S, const typename M:
         for (int64_t c0 = 0; c0 < S.D; c0 += M::COLS) {
             M m;
             m.weights(wr, S.Dp, c0);
-            l = m.logits(M::rows(row, c0, S.D, on), l);
+            l = m.logits(M::rows(row, c0, S.D), l);
         }
-        const float x = softmax(l, at, S.V, factor && on ? factor[n] : base);
+        const float x = softmax(l, at, S.V, factor && on ? factor[n] : base, true);
         if (lane < TILE && on) {
             loss += double(x);
             if (each) each[n] = x;
@@ -399,7 +434,8 @@ __global__ __launch_bounds__(BLOCK) void grad_kernel(Shape S, const typename M::
     const int64_t c0 = (int64_t(blockIdx.x) * (BLOCK / WAVE) + threadIdx.x / WAVE) * M::COLS;
     if (c0 >= S.Dp) return;
     M m;
-    m.weights_back(wc, c0);
+    __shared__ typename M::Back room[BLOCK / WAVE][M::TILES * WAVE];
+    m.weights_back(wc, c0, room[threadIdx.x / WAVE]);
     typename M::Sums sum = {};
     const int64_t tiles = (S.N + TILE - 1) / TILE;
     for (int64_t tile = blockIdx.y; tile < tiles; tile += gridDim.y) {
@@ -407,14 +443,14 @@ __global__ __launch_bounds__(BLOCK) void grad_kernel(Shape S, const typename M::
         const bool on = n < S.N;
         int64_t b, t;
         split(S, on ? n : 0, b, t);
-        typename M::Rows rows = M::rows(place(S, hidden, b, t, on ? n : 0), c0, S.D, on);
+        typename M::Rows rows = M::rows(place(S, hidden, b, t, on ? n : 0), c0, S.D);
         const f32x4 dl = on ? d_logits[n * 4 + lane_g()] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         if (!on || target(S, tokens, b, t) < 0) M::clear(rows);
         m.back(rows, dl, d_hidden + n * S.D, c0, S.D, on, sum);
     }
     if (c < S.V) {
 #pragma unroll
-        for (int k = 0; k < M::TILES; k++) *reinterpret_cast<f32x4*>(parts + (int64_t(blockIdx.y) * S.V + c) * S.Dp + c0 + 16 * k + 4 * lane_g()) = sum.dw[k];
+        for (int k = 0; k < M::TILES; k++) *reinterpret_cast<f32x4*>(parts + (int64_t(blockIdx.y) * S.V + c) * S.Dp + c0 + M::column(k)) = sum.dw[k];
     }
 }
 
@@ -501,7 +537,7 @@ int32_t run(Shape S, const void* hidden_, const void* weight, const void* tokens
     int nsums = k.groups;
     const size_t exchange = 2 * k.waves * WAVE * sizeof(f32x4);
     if (grads && k.waves) {
-        fused_kernel<M, true><<<k.groups, k.waves * WAVE, exchange, st>>>(S, hidden, tokens, wr, wc, counts, scale, factor, each, d_hidden, w.sums, w.parts);
+        fused_kernel<M, true><<<k.groups, k.waves * WAVE, exchange + k.waves * M::TILES * WAVE * sizeof(typename M::Back), st>>>(S, hidden, tokens, wr, wc, counts, scale, factor, each, d_hidden, w.sums, w.parts);
     } else if (k.waves) {
         fused_kernel<M, false><<<k.groups, k.waves * WAVE, exchange, st>>>(S, hidden, tokens, wr, nullptr, nullptr, nullptr, nullptr, each, nullptr, w.sums, nullptr);
     } else {
