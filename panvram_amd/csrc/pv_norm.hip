@@ -15,7 +15,7 @@ using namespace pvo;
 
 namespace {
 
-constexpr int PARTS = 512;                 // workgroups of the backward pass at most: rows of partial weight gradients
+constexpr int PARTS = 1024;                 // workgroups of the backward pass at most: rows of partial weight gradients
 
 // The larger of two values that are not negative, a NaN being the largest: their bits are in that order
 __device__ inline float larger_or_nan(float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); }
@@ -116,8 +116,8 @@ __global__ __launch_bounds__(L::BLOCK) void norm_kernel(const E* __restrict__ x,
         pk more[HELD];                     // all loads before the first sum
 #pragma unroll
         for (int k = 0; k < HELD; k++) if (const int64_t i = k * L::LANES + lane; i < packs) {
-            held[k] = pk::load(row + i * P);
-            if (add) more[k] = pk::load(add + i * P);
+            held[k] = pk::load_once(row + i * P);
+            if (add) more[k] = pk::load_once(add + i * P);
         }
 #pragma unroll
         for (int k = 0; k < HELD; k++) if (const int64_t i = k * L::LANES + lane; i < packs) {
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(L::BLOCK) void norm_kernel(const E* __restrict__ x,
             pk o;
 #pragma unroll
             for (int j = 0; j < P; j++) o.v[j] = E(m * float(h.v[j]) * r * weight[i + j]);
-            if (on) o.store(y + n * D + i);
+            if (on) o.store_once(y + n * D + i);
         });
         return;
     }
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(L::BLOCK) void norm_kernel(const E* __restrict__ x,
         for (int j = 0; j < P; j++) v[j] = m * float(h.v[j]) * weight[i + j] * up;
         pack<typename Q::type, P> o;
         Q::template make<P>(v, o);
-        o.store(q + n * D + i);
+        o.store_once(q + n * D + i);
     });
 }
 
@@ -204,9 +204,9 @@ __global__ __launch_bounds__(L::BLOCK) void norm_back_kernel(const E* __restrict
         if constexpr (L::PACKS) {
 #pragma unroll
             for (int k = 0; k < HELD; k++) if (const int64_t i = k * L::LANES + lane; i < packs) {
-                u[k] = pk::load(s + n * ss + i * P);
-                dy[k] = pk::load(d_y + n * D + i * P);
-                if (d_stream) ds[k] = pk::load(d_stream + n * D + i * P);
+                u[k] = pk::load_once(s + n * ss + i * P);
+                dy[k] = pk::load_once(d_y + n * D + i * P);
+                if (d_stream) ds[k] = pk::load_once(d_stream + n * D + i * P);
             }
 #pragma unroll
             for (int k = 0; k < HELD; k++) if (const int64_t i = k * L::LANES + lane; i < packs) {
@@ -235,7 +235,7 @@ __global__ __launch_bounds__(L::BLOCK) void norm_back_kernel(const E* __restrict
                     const float a = float(u[k].v[j]) * r, g = float(dy[k].v[j]) * w[k][j];
                     o.v[j] = E((d_stream ? float(ds[k].v[j]) : 0.0f) + r * (g - a * mean));
                 }
-                o.store(d + n * D + i * P);
+                o.store_once(d + n * D + i * P);
             }
         } else {
             for (int64_t i = lane; i < D; i += L::LANES) {

@@ -6,8 +6,8 @@
 //   - the workgroup makes its chunk's map, publishes it (`Before`), joins the maps of the chunks before, and walks its
 //     steps from there.
 // The gradient is the same recurrence backwards: C[t] = (1 - z[t]) (d_out[t] + C[t+1]), C what flows into h[t-1]; the states
-// before each step are made again from the start of the wave's STEPS steps, which the forward pass leaves in `carry` (one f32 for
-// STEPS steps of a channel, so that h is never read). A step's arithmetic is the same for every cut of T, and so is the order in which maps are
+// before each step are made again from the start of the wave's steps, which the forward pass leaves in `carry` (one f32 for
+// SPAN steps of a channel, so that h is never read). A step's arithmetic is the same for every cut of T, and so is the order in which maps are
 // joined: results do not depend on which workgroup was faster.
 //
 // A reset at t drops h[t-1], whatever it holds (a NaN too): the step is chosen, not multiplied by zero, and the map of a run
@@ -18,13 +18,17 @@ using namespace pvo;
 
 namespace {
 
-constexpr int STEPS = 16;                  // of a wave: 16 loads of each tensor in flight
-constexpr int CHUNK_WAVES = 8;             // of a workgroup, where T has more than STEPS steps
+// Steps of a wave, whose loads are all in flight at once, and waves of a workgroup where T has more steps than a wave. Forwards 32
+// (1 x 2^20 x 512 bfloat16 in 640 us; 745 with 16, whose maps are twice as many), 4 for sequences that short (a single step is
+// all launch); backwards, with one tensor more to hold, 16.
+constexpr int STEPS_FORWARD = 32, STEPS_BACK = 16, STEPS_SHORT = 4, CHUNK_WAVES = 8;
+constexpr int SPAN = 16;                   // steps from one state that is kept for the backward pass to the next
+static_assert(SPAN == STEPS_BACK && STEPS_FORWARD % SPAN == 0, "a wave of the backward pass starts at a state that is kept");
 constexpr float CUT = -1.0f;
 
 struct Shape {
     int64_t B, T, D, gb, gt, vb, vt, db, dt;   // strides in elements: gate, value, d_out (batch, time); channels are neighbours
-    int64_t spans, chunks, tiles;              // spans of STEPS and chunks of T, tiles of D
+    int64_t spans, chunks, tiles;              // spans of SPAN and chunks of T, tiles of D
 };
 
 // z = sigmoid(g) and k = 1 - z of a step in one register: the smaller of the two, its sign bit set where that is z. It is made from
@@ -127,7 +131,7 @@ template <int VEC, int WAVES, bool ONE> struct Place {
 
 // A wave's steps [t0, t0 + steps), and a bit for each that has a reset
 struct Span { int64_t t0; int steps; uint32_t cuts; };
-__device__ inline Span span_of(const Shape& S, const uint8_t* reset, int64_t b, int64_t t0, int lane) {
+template <int STEPS> __device__ inline Span span_of(const Shape& S, const uint8_t* reset, int64_t b, int64_t t0, int lane) {
     Span s;
     s.t0 = t0;
     const int64_t left = S.T - t0;
@@ -140,7 +144,8 @@ __device__ inline Span span_of(const Shape& S, const uint8_t* reset, int64_t b, 
 // A wave's steps of a tensor as a buffer of its rows: step i is at i * stride bytes, and what lies behind the span (or at NO_LANE)
 // is not read and not written, so that neither the end of T nor that of D needs a branch.
 constexpr uint32_t NO_LANE = 1u << 31;
-constexpr int64_t MOST_STRIDE = 1 << 26;   // bytes: a span's offsets stay below 2^30
+constexpr int ONCE = 2;                    // the accesses' hint: not used again soon
+constexpr int64_t MOST_STRIDE = 1 << 26;   // bytes: the offsets of a wave's steps stay below 2^31
 struct Rows {
     __amdgpu_buffer_rsrc_t buffer;
     int stride;
@@ -150,12 +155,12 @@ struct Rows {
         buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(from + s.t0 * step), 0, bytes, 0x00027000);
     }
     template <int BYTES> __device__ uint32_t load(int i, uint32_t at) const {
-        if constexpr (BYTES == 4) return __builtin_amdgcn_raw_buffer_load_b32(buffer, at, i * stride, 0);
-        else return __builtin_amdgcn_raw_buffer_load_b16(buffer, at, i * stride, 0);
+        if constexpr (BYTES == 4) return __builtin_amdgcn_raw_buffer_load_b32(buffer, at, i * stride, ONCE);
+        else return __builtin_amdgcn_raw_buffer_load_b16(buffer, at, i * stride, ONCE);
     }
     template <int BYTES> __device__ void store(uint32_t bits, int i, uint32_t at) const {
-        if constexpr (BYTES == 4) __builtin_amdgcn_raw_buffer_store_b32(bits, buffer, at, i * stride, 0);
-        else __builtin_amdgcn_raw_buffer_store_b16(uint16_t(bits), buffer, at, i * stride, 0);
+        if constexpr (BYTES == 4) __builtin_amdgcn_raw_buffer_store_b32(bits, buffer, at, i * stride, ONCE);
+        else __builtin_amdgcn_raw_buffer_store_b16(uint16_t(bits), buffer, at, i * stride, ONCE);
     }
 };
 
@@ -179,13 +184,13 @@ template <typename E, int VEC> struct Word {
         }
     }
 };
-template <typename E, int VEC> __device__ inline void load_steps(Word<E, VEC>* to, const Rows& rows, uint32_t at) {
+template <int STEPS, typename E, int VEC> __device__ inline void load_steps(Word<E, VEC> (&to)[STEPS], const Rows& rows, uint32_t at) {
 #pragma unroll
     for (int i = 0; i < STEPS; i++) to[i].bits = rows.load<Word<E, VEC>::BYTES>(i, at);
 }
 // Behind the end: gates that leave the state as it is (z = 0), zeros in the other tensors. (A buffer's zeros are no such thing
 // for the gates, and are not there where all steps are one and the same row, stride 0.)
-template <typename E, int VEC> __device__ inline void end_steps(Word<E, VEC>* x, const Span& s, float rest) {
+template <int STEPS, typename E, int VEC> __device__ inline void end_steps(Word<E, VEC> (&x)[STEPS], const Span& s, float rest) {
     if (s.steps == STEPS) return;
     const float both[2] = {rest, rest};
 #pragma unroll
@@ -193,18 +198,18 @@ template <typename E, int VEC> __device__ inline void end_steps(Word<E, VEC>* x,
 }
 // The compiler is to make what follows from these registers again where it needs it: kept from one walk over the steps to the
 // next, z, 1 - z and the products would take two to four times the registers
-template <int VEC> __device__ inline void anew(float (*q)[VEC]) {
+template <int STEPS, int VEC> __device__ inline void anew(float (&q)[STEPS][VEC]) {
 #pragma unroll
     for (int i = 0; i < STEPS; i++)
 #pragma unroll
         for (int v = 0; v < VEC; v++) asm volatile("" : "+v"(q[i][v]));
 }
-template <typename E, int VEC> __device__ inline void anew(Word<E, VEC>* x) {
+template <int STEPS, typename E, int VEC> __device__ inline void anew(Word<E, VEC> (&x)[STEPS]) {
 #pragma unroll
     for (int i = 0; i < STEPS; i++) asm volatile("" : "+v"(x[i].bits));
 }
 // f(i, whether step i has a reset) over the steps in order or backwards
-template <bool RESET, bool BACK, typename F> __device__ inline void over_steps(const Span& s, F&& f) {
+template <int STEPS, bool RESET, bool BACK, typename F> __device__ inline void over_steps(const Span& s, F&& f) {
 #pragma unroll
     for (int i = 0; i < STEPS; i++) { const int k = BACK ? STEPS - 1 - i : i; f(k, RESET && (s.cuts >> k & 1)); }
 }
@@ -256,27 +261,27 @@ template <int VEC, int WAVES> struct Maps {
     __device__ Map get(int wave, int channel) const { return {A[wave][0].v[channel], H[wave][0].v[channel]}; }
 };
 
-template <typename E, int VEC, int WAVES, bool ONE, bool RESET>
-__global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC == 2 && WAVES > 1 ? 6 : 1))) void scan_kernel(Shape S, Records R, const E* __restrict__ gate, const E* __restrict__ value,
+template <typename E, int VEC, int STEPS, int WAVES, bool ONE, bool RESET>
+__global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC == 2 && WAVES > 1 ? 4 : 1))) void scan_kernel(Shape S, Records R, const E* __restrict__ gate, const E* __restrict__ value,
                                                            const float* __restrict__ state, const uint8_t* __restrict__ reset, E* __restrict__ out,
                                                            float* __restrict__ last, float* __restrict__ carry) {
     __shared__ Maps<VEC, WAVES> maps;
     __shared__ Before<VEC, WAVES> before;
     const Place<VEC, WAVES, ONE> P(S, R);
-    const Span s = span_of(S, reset, P.b, (P.p * WAVES + P.wave) * STEPS, P.lane);
+    const Span s = span_of<STEPS>(S, reset, P.b, (P.p * WAVES + P.wave) * STEPS, P.lane);
     const uint32_t at = P.on ? P.lane * VEC * sizeof(E) : NO_LANE;
     const int64_t width = S.D - P.d0 < WAVE * VEC ? S.D - P.d0 : WAVE * VEC;
     Word<E, VEC> g[STEPS], x[STEPS];
     load_steps(g, Rows(gate + P.b * S.gb + P.d0, S.gt, s, width), at);
     load_steps(x, Rows(value + P.b * S.vb + P.d0, S.vt, s, width), at);
-    end_steps<E, VEC>(g, s, -INFINITY);
-    end_steps<E, VEC>(x, s, 0.0f);
+    end_steps(g, s, -INFINITY);
+    end_steps(x, s, 0.0f);
     float Z[STEPS][VEC], h[VEC];
     if constexpr (WAVES > 1) {
         Map m[VEC];
 #pragma unroll
         for (int v = 0; v < VEC; v++) m[v] = {1.0f, 0.0f};
-        over_steps<RESET, false>(s, [&](int i, bool cut) {
+        over_steps<STEPS, RESET, false>(s, [&](int i, bool cut) {
 #pragma unroll
             for (int v = 0; v < VEC; v++) {
                 Z[i][v] = gate_of(g[i].get(v));
@@ -292,10 +297,10 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
             for (int v = 0; v < VEC; v++) m[v].A = CUT;
         maps.put(P.wave, P.lane, m);
         __syncthreads();
-        anew<VEC>(Z);
-        anew<E, VEC>(x);
+        anew(Z);
+        anew(x);
     } else {
-        over_steps<RESET, false>(s, [&](int i, bool) {
+        over_steps<STEPS, RESET, false>(s, [&](int i, bool) {
 #pragma unroll
             for (int v = 0; v < VEC; v++) Z[i][v] = gate_of(g[i].get(v));
         });
@@ -316,11 +321,11 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
         for (int w = 0; w < P.wave; w++)
 #pragma unroll
             for (int v = 0; v < VEC; v++) h[v] = apply(maps.get(w, P.lane * VEC + v), h[v]);
-    if (carry && P.on && s.steps)
-#pragma unroll
-        for (int v = 0; v < VEC; v++) carry[(P.b * S.spans + s.t0 / STEPS) * S.D + P.d + v] = h[v];
     const Rows to(out + P.b * S.T * S.D + P.d0, S.D, s, width);
-    over_steps<RESET, false>(s, [&](int i, bool cut) {
+    over_steps<STEPS, RESET, false>(s, [&](int i, bool cut) {
+        if (i % SPAN == 0 && carry && P.on && i < s.steps)
+#pragma unroll
+            for (int v = 0; v < VEC; v++) carry[(P.b * S.spans + (s.t0 + i) / SPAN) * S.D + P.d + v] = h[v];
         float o[VEC];
 #pragma unroll
         for (int v = 0; v < VEC; v++) {
@@ -337,7 +342,7 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
         for (int v = 0; v < VEC; v++) last[P.b * S.D + P.d + v] = h[v];
 }
 
-template <typename E, int VEC, int WAVES, bool ONE, bool RESET>
+template <typename E, int VEC, int STEPS, int WAVES, bool ONE, bool RESET>
 __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC == 2 && WAVES > 1 ? 4 : 1))) void scan_back_kernel(Shape S, Records R, const E* __restrict__ gate, const E* __restrict__ value,
                                                                 const uint8_t* __restrict__ reset, const float* __restrict__ carry,
                                                                 const E* __restrict__ d_out, const float* __restrict__ d_last, E* __restrict__ d_gate,
@@ -346,28 +351,28 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
     __shared__ Before<VEC, WAVES> before;
     const Place<VEC, WAVES, ONE> P(S, R);
     const int64_t c = S.chunks - 1 - P.p;              // the walk begins at the last chunk
-    const Span s = span_of(S, reset, P.b, (c * WAVES + P.wave) * STEPS, P.lane);
+    const Span s = span_of<STEPS>(S, reset, P.b, (c * WAVES + P.wave) * STEPS, P.lane);
     const uint32_t at = P.on ? P.lane * VEC * sizeof(E) : NO_LANE;
     const int64_t width = S.D - P.d0 < WAVE * VEC ? S.D - P.d0 : WAVE * VEC;
     Word<E, VEC> g[STEPS], x[STEPS], y[STEPS];
     load_steps(g, Rows(gate + P.b * S.gb + P.d0, S.gt, s, width), at);
     load_steps(x, Rows(value + P.b * S.vb + P.d0, S.vt, s, width), at);
     load_steps(y, Rows(d_out + P.b * S.db + P.d0, S.dt, s, width), at);
-    end_steps<E, VEC>(g, s, -INFINITY);
-    end_steps<E, VEC>(x, s, 0.0f);
-    end_steps<E, VEC>(y, s, 0.0f);
+    end_steps(g, s, -INFINITY);
+    end_steps(x, s, 0.0f);
+    end_steps(y, s, 0.0f);
     float Z[STEPS][VEC], C[VEC], h[VEC];
-    over_steps<RESET, false>(s, [&](int i, bool) {
+    over_steps<STEPS, RESET, false>(s, [&](int i, bool) {
 #pragma unroll
         for (int v = 0; v < VEC; v++) Z[i][v] = gate_of(g[i].get(v));
     });
 #pragma unroll
-    for (int v = 0; v < VEC; v++) h[v] = P.on && s.steps ? carry[(P.b * S.spans + s.t0 / STEPS) * S.D + P.d + v] : 0.0f;
+    for (int v = 0; v < VEC; v++) h[v] = P.on && s.steps ? carry[(P.b * S.spans + s.t0 / SPAN) * S.D + P.d + v] : 0.0f;
     if constexpr (WAVES > 1) {
         Map m[VEC];
 #pragma unroll
         for (int v = 0; v < VEC; v++) m[v] = {1.0f, 0.0f};
-        over_steps<RESET, true>(s, [&](int i, bool cut) {
+        over_steps<STEPS, RESET, true>(s, [&](int i, bool cut) {
 #pragma unroll
             for (int v = 0; v < VEC; v++) {
                 float z, k;
@@ -381,8 +386,8 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
             for (int v = 0; v < VEC; v++) m[v].A = CUT;
         maps.put(P.wave, P.lane, m);
         __syncthreads();
-        anew<VEC>(Z);
-        anew<E, VEC>(y);
+        anew(Z);
+        anew(y);
     }
 #pragma unroll
     for (int v = 0; v < VEC; v++) C[v] = d_last && P.on ? d_last[P.b * S.D + P.d + v] : 0.0f;
@@ -394,7 +399,7 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
         before.wait(R, S, P.b, P.p, P.d0, P.wave, P.lane, own);
     }
     float U[STEPS][VEC];                   // value minus the state before each step
-    over_steps<RESET, false>(s, [&](int i, bool cut) {
+    over_steps<STEPS, RESET, false>(s, [&](int i, bool cut) {
 #pragma unroll
         for (int v = 0; v < VEC; v++) {
             float z, k;
@@ -414,9 +419,9 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
         for (int w = WAVES - 1; w > P.wave; w--)
 #pragma unroll
             for (int v = 0; v < VEC; v++) C[v] = apply(maps.get(w, P.lane * VEC + v), C[v]);
-    anew<VEC>(Z);
+    anew(Z);
     const Rows to_gate(d_gate + P.b * S.T * S.D + P.d0, S.D, s, width), to_value(d_value + P.b * S.T * S.D + P.d0, S.D, s, width);
-    over_steps<RESET, true>(s, [&](int i, bool cut) {
+    over_steps<STEPS, RESET, true>(s, [&](int i, bool cut) {
         float og[VEC], ov[VEC];
 #pragma unroll
         for (int v = 0; v < VEC; v++) {
@@ -435,9 +440,11 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
         for (int v = 0; v < VEC; v++) d_state[P.b * S.D + P.d + v] = C[v];
 }
 
-int64_t spans_of(int64_t T) { return (T + STEPS - 1) / STEPS; }
-int64_t chunk_steps(int64_t T) { return T <= STEPS ? STEPS : STEPS * CHUNK_WAVES; }
-int64_t chunks_of(int64_t T) { return (T + chunk_steps(T) - 1) / chunk_steps(T); }
+int64_t spans_of(int64_t T) { return (T + SPAN - 1) / SPAN; }
+int64_t chunks_of(int64_t T, int steps) {
+    const int64_t chunk = T <= steps ? steps : steps * CHUNK_WAVES;
+    return (T + chunk - 1) / chunk;
+}
 
 // 8-byte words of a call's records: two for the counter, then the levels
 int64_t words_of(int64_t B, int64_t chunks, int64_t D) {
@@ -453,18 +460,18 @@ template <typename... I> int32_t check(int64_t B, int64_t T, int64_t D, int32_t 
     if (B < 0 || T < 1 || D < 0) return fail(PV_EARG, err, cap, "shape: B >= 0, T >= 1, D >= 0");
     const int64_t most = int64_t(1) << 40;
     if (B > INT32_MAX || T > INT32_MAX || D > INT32_MAX || (B && D && (B * D > most || T > most / (B * D)))) return fail(PV_EARG, err, cap, "shape: B T D of 2^40 at most");
-    if (B && D && B * chunks_of(T) * ((D + WAVE - 1) / WAVE) > INT32_MAX) return fail(PV_EARG, err, cap, "shape: too many chunks");
+    if (B && D && B * chunks_of(T, STEPS_BACK) * ((D + WAVE - 1) / WAVE) > INT32_MAX) return fail(PV_EARG, err, cap, "shape: too many chunks");
     for (int64_t st : {steps...}) if (T > 1 && (st < 0 || st * element_bytes(dtype) > MOST_STRIDE)) return fail(PV_EARG, err, cap, "stride: a step's is 0 to 2^26 bytes");
     const uint64_t need = pv_gated_scan_work_bytes(B, T, D);
     if (need && (!work || work_bytes < need || !aligned(work, 16))) return fail(PV_EARG, err, cap, "work: too small, or not 16-byte aligned");
     return PV_OK;
 }
 
-// f(channels of a lane, waves, one chunk only, resets) with the records cleared
-template <typename F> int32_t launch(Shape& S, bool pairs, bool resets, void* work, hipStream_t st, F&& f) {
+// f(channels of a lane, steps of a wave, waves, one chunk only, resets) with the records cleared
+template <int STEPS, typename F> int32_t launch(Shape& S, bool pairs, bool resets, void* work, hipStream_t st, F&& f) {
     const int vec = pairs ? 2 : 1;
     S.spans = spans_of(S.T);
-    S.chunks = chunks_of(S.T);
+    S.chunks = chunks_of(S.T, STEPS);
     S.tiles = (S.D + WAVE * vec - 1) / (WAVE * vec);
     Records R = {};
     if (const int64_t words = words_of(S.B, S.chunks, S.D)) {
@@ -479,9 +486,13 @@ template <typename F> int32_t launch(Shape& S, bool pairs, bool resets, void* wo
     const uint32_t groups = uint32_t(S.B * S.tiles * S.chunks);
     using std::integral_constant;
     auto with = [&](auto vec, auto resets) {
-        if (S.T <= STEPS) return f(vec, integral_constant<int, 1>{}, std::true_type{}, resets, R, groups);
-        if (S.chunks == 1) return f(vec, integral_constant<int, CHUNK_WAVES>{}, std::true_type{}, resets, R, groups);
-        return f(vec, integral_constant<int, CHUNK_WAVES>{}, std::false_type{}, resets, R, groups);
+        const integral_constant<int, STEPS> steps;
+        const integral_constant<int, CHUNK_WAVES> waves;
+        if constexpr (STEPS > STEPS_BACK)
+            if (S.T <= STEPS_SHORT) return f(vec, integral_constant<int, STEPS_SHORT>{}, integral_constant<int, 1>{}, std::true_type{}, resets, R, groups);
+        if (S.T <= STEPS) return f(vec, steps, integral_constant<int, 1>{}, std::true_type{}, resets, R, groups);
+        if (S.chunks == 1) return f(vec, steps, waves, std::true_type{}, resets, R, groups);
+        return f(vec, steps, waves, std::false_type{}, resets, R, groups);
     };
     if (pairs) return resets ? with(integral_constant<int, 2>{}, std::true_type{}) : with(integral_constant<int, 2>{}, std::false_type{});
     return resets ? with(integral_constant<int, 1>{}, std::true_type{}) : with(integral_constant<int, 1>{}, std::false_type{});
@@ -498,7 +509,7 @@ extern "C" {
 
 int64_t pv_gated_scan_spans(int64_t T) { return T > 0 ? spans_of(T) : 0; }
 uint64_t pv_gated_scan_work_bytes(int64_t B, int64_t T, int64_t D) {
-    return B > 0 && T > 0 && D > 0 ? uint64_t(words_of(B, chunks_of(T), D)) * 8 : 0;
+    return B > 0 && T > 0 && D > 0 ? uint64_t(words_of(B, chunks_of(T, STEPS_BACK), D)) * 8 : 0;
 }
 
 int32_t pv_gated_scan_hip(const void* gate, const void* value, const float* state, const uint8_t* reset, int64_t B, int64_t T, int64_t D, int64_t gate_b,
@@ -512,11 +523,11 @@ int32_t pv_gated_scan_hip(const void* gate, const void* value, const float* stat
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
         const bool pairs = sizeof(E) == 2 && D % 2 == 0 && pairs_of<E>(gate, B, T, gate_b, gate_t) && pairs_of<E>(value, B, T, value_b, value_t) && aligned(out, 4);
-        return launch(S, pairs, reset, work, st, [&](auto vec, auto waves, auto one, auto resets, const Records& R, uint32_t groups) {
-            constexpr int V = decltype(vec)::value, W = decltype(waves)::value;
+        return launch<STEPS_FORWARD>(S, pairs, reset, work, st, [&](auto vec, auto steps, auto waves, auto one, auto resets, const Records& R, uint32_t groups) {
+            constexpr int V = decltype(vec)::value, N = decltype(steps)::value, W = decltype(waves)::value;
             constexpr bool ONE = decltype(one)::value, RESET = decltype(resets)::value;
             if constexpr (V == 1 || sizeof(E) == 2)
-                scan_kernel<E, V, W, ONE, RESET><<<groups, W * WAVE, 0, st>>>(S, R, static_cast<const E*>(gate), static_cast<const E*>(value), state, reset,
+                scan_kernel<E, V, N, W, ONE, RESET><<<groups, W * WAVE, 0, st>>>(S, R, static_cast<const E*>(gate), static_cast<const E*>(value), state, reset,
                                                                        static_cast<E*>(out), last, carry);
             return launched(err, errcap);
         });
@@ -536,11 +547,11 @@ int32_t pv_gated_scan_backward_hip(const void* gate, const void* value, const fl
         using E = decltype(e);
         const bool pairs = sizeof(E) == 2 && D % 2 == 0 && pairs_of<E>(gate, B, T, gate_b, gate_t) && pairs_of<E>(value, B, T, value_b, value_t) &&
                            pairs_of<E>(d_out, B, T, d_out_b, d_out_t) && aligned(d_gate, 4) && aligned(d_value, 4);
-        return launch(S, pairs, reset, work, st, [&](auto vec, auto waves, auto one, auto resets, const Records& R, uint32_t groups) {
-            constexpr int V = decltype(vec)::value, W = decltype(waves)::value;
+        return launch<STEPS_BACK>(S, pairs, reset, work, st, [&](auto vec, auto steps, auto waves, auto one, auto resets, const Records& R, uint32_t groups) {
+            constexpr int V = decltype(vec)::value, N = decltype(steps)::value, W = decltype(waves)::value;
             constexpr bool ONE = decltype(one)::value, RESET = decltype(resets)::value;
             if constexpr (V == 1 || sizeof(E) == 2)
-                scan_back_kernel<E, V, W, ONE, RESET><<<groups, W * WAVE, 0, st>>>(S, R, static_cast<const E*>(gate), static_cast<const E*>(value), reset, carry,
+                scan_back_kernel<E, V, N, W, ONE, RESET><<<groups, W * WAVE, 0, st>>>(S, R, static_cast<const E*>(gate), static_cast<const E*>(value), reset, carry,
                                                                             static_cast<const E*>(d_out), d_last, static_cast<E*>(d_gate),
                                                                             static_cast<E*>(d_value), d_state);
             return launched(err, errcap);
