@@ -144,9 +144,10 @@ template <int STEPS> __device__ inline Span span_of(const Shape& S, const uint8_
 // A wave's steps of a tensor as a buffer of its rows: step i is at i * stride bytes, and what lies behind the span (or at NO_LANE)
 // is not read and not written, so that neither the end of T nor that of D needs a branch.
 constexpr uint32_t NO_LANE = 1u << 31;
-constexpr int ONCE = 2;                    // the accesses' hint: not used again soon
+// ONCE: accesses with the hint that the data is not used again soon (`once_of` says when)
 constexpr int64_t MOST_STRIDE = 1 << 26;   // bytes: the offsets of a wave's steps stay below 2^31
-struct Rows {
+template <bool ONCE> struct Rows {
+    static constexpr int HINT = ONCE ? 2 : 0;
     __amdgpu_buffer_rsrc_t buffer;
     int stride;
     template <typename E> __device__ Rows(const E* from, int64_t step, const Span& s, int64_t channels) {
@@ -155,12 +156,12 @@ struct Rows {
         buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<E*>(from + s.t0 * step), 0, bytes, 0x00027000);
     }
     template <int BYTES> __device__ uint32_t load(int i, uint32_t at) const {
-        if constexpr (BYTES == 4) return __builtin_amdgcn_raw_buffer_load_b32(buffer, at, i * stride, ONCE);
-        else return __builtin_amdgcn_raw_buffer_load_b16(buffer, at, i * stride, ONCE);
+        if constexpr (BYTES == 4) return __builtin_amdgcn_raw_buffer_load_b32(buffer, at, i * stride, HINT);
+        else return __builtin_amdgcn_raw_buffer_load_b16(buffer, at, i * stride, HINT);
     }
     template <int BYTES> __device__ void store(uint32_t bits, int i, uint32_t at) const {
-        if constexpr (BYTES == 4) __builtin_amdgcn_raw_buffer_store_b32(bits, buffer, at, i * stride, ONCE);
-        else __builtin_amdgcn_raw_buffer_store_b16(uint16_t(bits), buffer, at, i * stride, ONCE);
+        if constexpr (BYTES == 4) __builtin_amdgcn_raw_buffer_store_b32(bits, buffer, at, i * stride, HINT);
+        else __builtin_amdgcn_raw_buffer_store_b16(uint16_t(bits), buffer, at, i * stride, HINT);
     }
 };
 
@@ -184,9 +185,9 @@ template <typename E, int VEC> struct Word {
         }
     }
 };
-template <int STEPS, typename E, int VEC> __device__ inline void load_steps(Word<E, VEC> (&to)[STEPS], const Rows& rows, uint32_t at) {
+template <int STEPS, typename E, int VEC, bool ONCE> __device__ inline void load_steps(Word<E, VEC> (&to)[STEPS], const Rows<ONCE>& rows, uint32_t at) {
 #pragma unroll
-    for (int i = 0; i < STEPS; i++) to[i].bits = rows.load<Word<E, VEC>::BYTES>(i, at);
+    for (int i = 0; i < STEPS; i++) to[i].bits = rows.template load<Word<E, VEC>::BYTES>(i, at);
 }
 // Behind the end: gates that leave the state as it is (z = 0), zeros in the other tensors. (A buffer's zeros are no such thing
 // for the gates, and are not there where all steps are one and the same row, stride 0.)
@@ -261,7 +262,7 @@ template <int VEC, int WAVES> struct Maps {
     __device__ Map get(int wave, int channel) const { return {A[wave][0].v[channel], H[wave][0].v[channel]}; }
 };
 
-template <typename E, int VEC, int STEPS, int WAVES, bool ONE, bool RESET>
+template <typename E, int VEC, int STEPS, int WAVES, bool ONE, bool RESET, bool ONCE>
 __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC == 2 && WAVES > 1 ? 4 : 1))) void scan_kernel(Shape S, Records R, const E* __restrict__ gate, const E* __restrict__ value,
                                                            const float* __restrict__ state, const uint8_t* __restrict__ reset, E* __restrict__ out,
                                                            float* __restrict__ last, float* __restrict__ carry) {
@@ -272,8 +273,8 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
     const uint32_t at = P.on ? P.lane * VEC * sizeof(E) : NO_LANE;
     const int64_t width = S.D - P.d0 < WAVE * VEC ? S.D - P.d0 : WAVE * VEC;
     Word<E, VEC> g[STEPS], x[STEPS];
-    load_steps(g, Rows(gate + P.b * S.gb + P.d0, S.gt, s, width), at);
-    load_steps(x, Rows(value + P.b * S.vb + P.d0, S.vt, s, width), at);
+    load_steps(g, Rows<ONCE>(gate + P.b * S.gb + P.d0, S.gt, s, width), at);
+    load_steps(x, Rows<ONCE>(value + P.b * S.vb + P.d0, S.vt, s, width), at);
     end_steps(g, s, -INFINITY);
     end_steps(x, s, 0.0f);
     float Z[STEPS][VEC], h[VEC];
@@ -321,7 +322,7 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
         for (int w = 0; w < P.wave; w++)
 #pragma unroll
             for (int v = 0; v < VEC; v++) h[v] = apply(maps.get(w, P.lane * VEC + v), h[v]);
-    const Rows to(out + P.b * S.T * S.D + P.d0, S.D, s, width);
+    const Rows<ONCE> to(out + P.b * S.T * S.D + P.d0, S.D, s, width);
     over_steps<STEPS, RESET, false>(s, [&](int i, bool cut) {
         if (i % SPAN == 0 && carry && P.on && i < s.steps)
 #pragma unroll
@@ -335,14 +336,14 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
             h[v] = cut ? in : fmaf(k, h[v], in);
             o[v] = h[v];
         }
-        to.store<Word<E, VEC>::BYTES>(Word<E, VEC>::of(o).bits, i, at);
+        to.template store<Word<E, VEC>::BYTES>(Word<E, VEC>::of(o).bits, i, at);
     });
     if (P.on && s.steps && s.t0 + s.steps == S.T)
 #pragma unroll
         for (int v = 0; v < VEC; v++) last[P.b * S.D + P.d + v] = h[v];
 }
 
-template <typename E, int VEC, int STEPS, int WAVES, bool ONE, bool RESET>
+template <typename E, int VEC, int STEPS, int WAVES, bool ONE, bool RESET, bool ONCE>
 __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC == 2 && WAVES > 1 ? 4 : 1))) void scan_back_kernel(Shape S, Records R, const E* __restrict__ gate, const E* __restrict__ value,
                                                                 const uint8_t* __restrict__ reset, const float* __restrict__ carry,
                                                                 const E* __restrict__ d_out, const float* __restrict__ d_last, E* __restrict__ d_gate,
@@ -355,9 +356,9 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
     const uint32_t at = P.on ? P.lane * VEC * sizeof(E) : NO_LANE;
     const int64_t width = S.D - P.d0 < WAVE * VEC ? S.D - P.d0 : WAVE * VEC;
     Word<E, VEC> g[STEPS], x[STEPS], y[STEPS];
-    load_steps(g, Rows(gate + P.b * S.gb + P.d0, S.gt, s, width), at);
-    load_steps(x, Rows(value + P.b * S.vb + P.d0, S.vt, s, width), at);
-    load_steps(y, Rows(d_out + P.b * S.db + P.d0, S.dt, s, width), at);
+    load_steps(g, Rows<ONCE>(gate + P.b * S.gb + P.d0, S.gt, s, width), at);
+    load_steps(x, Rows<ONCE>(value + P.b * S.vb + P.d0, S.vt, s, width), at);
+    load_steps(y, Rows<ONCE>(d_out + P.b * S.db + P.d0, S.dt, s, width), at);
     end_steps(g, s, -INFINITY);
     end_steps(x, s, 0.0f);
     end_steps(y, s, 0.0f);
@@ -420,7 +421,7 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
 #pragma unroll
             for (int v = 0; v < VEC; v++) C[v] = apply(maps.get(w, P.lane * VEC + v), C[v]);
     anew(Z);
-    const Rows to_gate(d_gate + P.b * S.T * S.D + P.d0, S.D, s, width), to_value(d_value + P.b * S.T * S.D + P.d0, S.D, s, width);
+    const Rows<ONCE> to_gate(d_gate + P.b * S.T * S.D + P.d0, S.D, s, width), to_value(d_value + P.b * S.T * S.D + P.d0, S.D, s, width);
     over_steps<STEPS, RESET, true>(s, [&](int i, bool cut) {
         float og[VEC], ov[VEC];
 #pragma unroll
@@ -432,8 +433,8 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
             og[v] = in * k * U[i][v];
             C[v] = cut ? 0.0f : k * G;
         }
-        to_value.store<Word<E, VEC>::BYTES>(Word<E, VEC>::of(ov).bits, i, at);
-        to_gate.store<Word<E, VEC>::BYTES>(Word<E, VEC>::of(og).bits, i, at);
+        to_value.template store<Word<E, VEC>::BYTES>(Word<E, VEC>::of(ov).bits, i, at);
+        to_gate.template store<Word<E, VEC>::BYTES>(Word<E, VEC>::of(og).bits, i, at);
     });
     if (d_state && P.on && c == 0 && P.wave == 0)
 #pragma unroll
@@ -467,8 +468,14 @@ template <typename... I> int32_t check(int64_t B, int64_t T, int64_t D, int32_t 
     return PV_OK;
 }
 
-// f(channels of a lane, steps of a wave, waves, one chunk only, resets) with the records cleared
-template <int STEPS, typename F> int32_t launch(Shape& S, bool pairs, bool resets, void* work, hipStream_t st, F&& f) {
+// Whether a call's accesses get the hint ONCE: tensors that the caches (256 MB) do not hold from one kernel to the next, with rows
+// of whole 128-byte lines (of a line shared by two workgroups each would read it all). 8 x 8,192 x 1,024 (134 MB a tensor in
+// bfloat16) 99 us forwards and 142 backwards with it, 105 and 156 without; 5 x 2,049 x 512 float32 (21 MB) 28 and 36 with it, 24
+// and 33 without; 5 x 2,049 x 500, rows off the lines, 29 and 44, and 25 and 35.
+bool once_of(int64_t B, int64_t T, int64_t D, int bytes) { return D * bytes % 128 == 0 && B * T * D * bytes >= (int64_t(64) << 20); }
+
+// f(channels of a lane, steps of a wave, waves, one chunk only, resets, once) with the records cleared
+template <int STEPS, typename F> int32_t launch(Shape& S, bool pairs, bool resets, bool once, void* work, hipStream_t st, F&& f) {
     const int vec = pairs ? 2 : 1;
     S.spans = spans_of(S.T);
     S.chunks = chunks_of(S.T, STEPS);
@@ -489,10 +496,11 @@ template <int STEPS, typename F> int32_t launch(Shape& S, bool pairs, bool reset
         const integral_constant<int, STEPS> steps;
         const integral_constant<int, CHUNK_WAVES> waves;
         if constexpr (STEPS > STEPS_BACK)
-            if (S.T <= STEPS_SHORT) return f(vec, integral_constant<int, STEPS_SHORT>{}, integral_constant<int, 1>{}, std::true_type{}, resets, R, groups);
-        if (S.T <= STEPS) return f(vec, steps, integral_constant<int, 1>{}, std::true_type{}, resets, R, groups);
-        if (S.chunks == 1) return f(vec, steps, waves, std::true_type{}, resets, R, groups);
-        return f(vec, steps, waves, std::false_type{}, resets, R, groups);
+            if (S.T <= STEPS_SHORT) return f(vec, integral_constant<int, STEPS_SHORT>{}, integral_constant<int, 1>{}, std::true_type{}, resets, std::false_type{}, R, groups);
+        if (S.T <= STEPS) return f(vec, steps, integral_constant<int, 1>{}, std::true_type{}, resets, std::false_type{}, R, groups);
+        if (S.chunks == 1) return f(vec, steps, waves, std::true_type{}, resets, std::false_type{}, R, groups);
+        if (once) return f(vec, steps, waves, std::false_type{}, resets, std::true_type{}, R, groups);
+        return f(vec, steps, waves, std::false_type{}, resets, std::false_type{}, R, groups);
     };
     if (pairs) return resets ? with(integral_constant<int, 2>{}, std::true_type{}) : with(integral_constant<int, 2>{}, std::false_type{});
     return resets ? with(integral_constant<int, 1>{}, std::true_type{}) : with(integral_constant<int, 1>{}, std::false_type{});
@@ -523,11 +531,11 @@ int32_t pv_gated_scan_hip(const void* gate, const void* value, const float* stat
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
         const bool pairs = sizeof(E) == 2 && D % 2 == 0 && pairs_of<E>(gate, B, T, gate_b, gate_t) && pairs_of<E>(value, B, T, value_b, value_t) && aligned(out, 4);
-        return launch<STEPS_FORWARD>(S, pairs, reset, work, st, [&](auto vec, auto steps, auto waves, auto one, auto resets, const Records& R, uint32_t groups) {
+        return launch<STEPS_FORWARD>(S, pairs, reset, once_of(B, T, D, sizeof(E)), work, st, [&](auto vec, auto steps, auto waves, auto one, auto resets, auto once, const Records& R, uint32_t groups) {
             constexpr int V = decltype(vec)::value, N = decltype(steps)::value, W = decltype(waves)::value;
-            constexpr bool ONE = decltype(one)::value, RESET = decltype(resets)::value;
+            constexpr bool ONE = decltype(one)::value, RESET = decltype(resets)::value, ONCE = decltype(once)::value && V * sizeof(E) == 4;
             if constexpr (V == 1 || sizeof(E) == 2)
-                scan_kernel<E, V, N, W, ONE, RESET><<<groups, W * WAVE, 0, st>>>(S, R, static_cast<const E*>(gate), static_cast<const E*>(value), state, reset,
+                scan_kernel<E, V, N, W, ONE, RESET, ONCE><<<groups, W * WAVE, 0, st>>>(S, R, static_cast<const E*>(gate), static_cast<const E*>(value), state, reset,
                                                                        static_cast<E*>(out), last, carry);
             return launched(err, errcap);
         });
@@ -547,11 +555,11 @@ int32_t pv_gated_scan_backward_hip(const void* gate, const void* value, const fl
         using E = decltype(e);
         const bool pairs = sizeof(E) == 2 && D % 2 == 0 && pairs_of<E>(gate, B, T, gate_b, gate_t) && pairs_of<E>(value, B, T, value_b, value_t) &&
                            pairs_of<E>(d_out, B, T, d_out_b, d_out_t) && aligned(d_gate, 4) && aligned(d_value, 4);
-        return launch<STEPS_BACK>(S, pairs, reset, work, st, [&](auto vec, auto steps, auto waves, auto one, auto resets, const Records& R, uint32_t groups) {
+        return launch<STEPS_BACK>(S, pairs, reset, once_of(B, T, D, sizeof(E)), work, st, [&](auto vec, auto steps, auto waves, auto one, auto resets, auto once, const Records& R, uint32_t groups) {
             constexpr int V = decltype(vec)::value, N = decltype(steps)::value, W = decltype(waves)::value;
-            constexpr bool ONE = decltype(one)::value, RESET = decltype(resets)::value;
+            constexpr bool ONE = decltype(one)::value, RESET = decltype(resets)::value, ONCE = decltype(once)::value && V * sizeof(E) == 4;
             if constexpr (V == 1 || sizeof(E) == 2)
-                scan_back_kernel<E, V, N, W, ONE, RESET><<<groups, W * WAVE, 0, st>>>(S, R, static_cast<const E*>(gate), static_cast<const E*>(value), reset, carry,
+                scan_back_kernel<E, V, N, W, ONE, RESET, ONCE><<<groups, W * WAVE, 0, st>>>(S, R, static_cast<const E*>(gate), static_cast<const E*>(value), reset, carry,
                                                                             static_cast<const E*>(d_out), d_last, static_cast<E*>(d_gate),
                                                                             static_cast<E*>(d_value), d_state);
             return launched(err, errcap);
