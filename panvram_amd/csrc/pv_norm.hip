@@ -6,9 +6,8 @@
 //   backward, with u = s r and g = d_y weight:  d = d_stream + r (g - u mean(g u));  d_weight = sum over rows of d_y u
 //
 // A row's elements stay in registers between its sums and its outputs: every byte is read once and written once. A row is held
-// by one wave, or by a workgroup, as LANES x PACKS loads of 16 bytes a lane (`Plan`); rows that have no such form (over 8,192
-// elements and not 16-byte aligned, or larger than a workgroup's registers) are read again for each pass, from the caches.
-// Sums in 32 bits.
+// by LANES lanes, of a wave or of a workgroup, as PACKS packs of 16 bytes a lane (`Plan`); longer rows are read again for each
+// pass, from the caches. Rows may begin at any element; a row's last pack may be a part of one. Sums in 32 bits.
 #include "pv_ops.h"
 
 using namespace pvo;
@@ -48,16 +47,17 @@ struct Int8 {
     }
 };
 
-// One row: D elements as packs of P, pack k * LANES + lane in register k of a lane; PACKS 0: not held, any number of packs
-template <int LANES_, int PACKS_, int P_, int ROWS_> struct Plan {
-    static constexpr int LANES = LANES_, PACKS = PACKS_, P = P_, ROWS = ROWS_;      // ROWS: rows at a time of a workgroup
-    static constexpr int BLOCK = LANES * ROWS, WAVES = LANES / WAVE;
+// One row: D elements as packs of P, pack k * LANES + lane in register k of a lane; PACKS 0: not held, any number of packs.
+// ROWS: rows at a time of a workgroup
+template <int LANES_, int PACKS_, int ROWS_> struct Plan {
+    static constexpr int LANES = LANES_, PACKS = PACKS_, ROWS = ROWS_;
+    static constexpr int BLOCK = LANES * ROWS, WAVES = LANES > WAVE ? LANES / WAVE : 1;
 };
 
 // A sum, or a largest value, over the lanes of a row
 template <typename L, typename F> __device__ inline float over_row(float x, float* lds, F&& join) {
 #pragma unroll
-    for (int d = WAVE / 2; d; d >>= 1) x = join(x, __shfl_xor(x, d, WAVE));
+    for (int d = (L::LANES < WAVE ? L::LANES : WAVE) / 2; d; d >>= 1) x = join(x, __shfl_xor(x, d, WAVE));
     if constexpr (L::WAVES > 1) {
         const int row = threadIdx.x / L::LANES, wave = threadIdx.x / WAVE;
         __syncthreads();                                       // the last use of lds is over
@@ -73,12 +73,23 @@ template <typename L> __device__ inline float row_sum(float x, float* lds) {
     return over_row<L>(x, lds, [](float a, float b) { return a + b; });
 }
 
+// A pack of a row at element i of D: whole, or a part of one at the row's end
+template <int P, bool ONCE, typename T> __device__ inline pack<T, P> take(const T* row, int64_t i, int64_t D) {
+    if (i + P <= D) return ONCE ? pack<T, P>::load_once(row + i) : pack<T, P>::load(row + i);
+    return pack<T, P>::load_part(row + i, D - i);
+}
+template <bool ONCE, typename T, int P> __device__ inline void leave(const pack<T, P>& v, T* row, int64_t i, int64_t D) {
+    if (i + P > D) v.store_part(row + i, D - i);
+    else if (ONCE) v.store_once(row + i);
+    else v.store(row + i);
+}
+
 template <typename E, typename Q, typename L>
 __global__ __launch_bounds__(L::BLOCK) void norm_kernel(const E* __restrict__ x, const E* __restrict__ residual, const float* __restrict__ weight, int64_t N,
                                                         int64_t D, int64_t xs, int64_t rs, float eps, E* __restrict__ y, E* __restrict__ stream,
                                                         float* __restrict__ rstd, typename Q::type* __restrict__ q, float* __restrict__ scale) {
     __shared__ float lds[L::BLOCK / WAVE];
-    constexpr int P = L::P, HELD = L::PACKS ? L::PACKS : 1;
+    constexpr int P = 16 / sizeof(E), HELD = L::PACKS ? L::PACKS : 1;
     using pk = pack<E, P>;
     const int lane = threadIdx.x % L::LANES;
     int64_t n = int64_t(blockIdx.x) * L::ROWS + threadIdx.x / L::LANES;
@@ -86,26 +97,23 @@ __global__ __launch_bounds__(L::BLOCK) void norm_kernel(const E* __restrict__ x,
     if (!on) n = N - 1;                    // (a workgroup's last rows: computed for the barriers' sake, not stored)
     const E* row = x + n * xs;
     const E* add = residual ? residual + n * rs : nullptr;
-    const int64_t packs = D / P;
+    E* const to = stream + n * D;
+    const int64_t packs = (D + P - 1) / P;
     pk held[HELD];
-    auto each = [&](auto&& f) {            // f(pack's values, first element's index) over the lane's packs
+    auto each = [&](auto&& f) {            // f(pack, first element's index) over the lane's packs
         if constexpr (L::PACKS) {
 #pragma unroll
             for (int k = 0; k < HELD; k++) if (const int64_t i = k * L::LANES + lane; i < packs) f(held[k], i * P);
         } else {
-            const E* from = residual ? stream + n * D : row;
-            for (int64_t i = lane; i < packs; i += L::LANES) { pk h = pk::load(from + i * P); f(h, i * P); }
+            const E* from = residual ? to : row;
+            for (int64_t i = lane; i < packs; i += L::LANES) f(take<P, false>(from, i * P, D), i * P);
         }
     };
-    auto get = [&](int64_t i) {            // a pack of the stream, stored where there is an addition
-        pk h = pk::load(row + i * P);
-        if (add) {
-            const pk a = pk::load(add + i * P);
+    auto join = [&](pk& h, const pk& a, int64_t i) {       // the stream's pack, stored where there is an addition
+        if (!add) return;
 #pragma unroll
-            for (int j = 0; j < P; j++) h.v[j] = E(float(h.v[j]) + float(a.v[j]));
-            if (on || !L::PACKS) h.store(stream + n * D + i * P);
-        }
-        return h;
+        for (int j = 0; j < P; j++) h.v[j] = E(float(h.v[j]) + float(a.v[j]));
+        if (on) leave<false>(h, to, i, D);
     };
     float sum = 0.0f;
     auto square = [&](const pk& h, float m) {
@@ -116,23 +124,25 @@ __global__ __launch_bounds__(L::BLOCK) void norm_kernel(const E* __restrict__ x,
         pk more[HELD];                     // all loads before the first sum
 #pragma unroll
         for (int k = 0; k < HELD; k++) if (const int64_t i = k * L::LANES + lane; i < packs) {
-            held[k] = pk::load_once(row + i * P);
-            if (add) more[k] = pk::load_once(add + i * P);
+            held[k] = take<P, true>(row, i * P, D);
+            if (add) more[k] = take<P, true>(add, i * P, D);
         }
 #pragma unroll
         for (int k = 0; k < HELD; k++) if (const int64_t i = k * L::LANES + lane; i < packs) {
-            if (add) {
-#pragma unroll
-                for (int j = 0; j < P; j++) held[k].v[j] = E(float(held[k].v[j]) + float(more[k].v[j]));
-                if (on) held[k].store(stream + n * D + i * P);
-            }
+            join(held[k], more[k], i * P);
             square(held[k], 1.0f);
         }
     } else {
-        for (int64_t i = lane; i < packs; i += L::LANES) square(get(i), 1.0f);
+        for (int64_t i = lane; i < packs; i += L::LANES) {
+            pk h = take<P, false>(row, i * P, D), a = h;
+            if (add) a = take<P, false>(add, i * P, D);
+            join(h, a, i * P);
+            square(h, 1.0f);
+        }
     }
     sum = row_sum<L>(sum, lds);
-    // squares that leave 32 bits, or vanish in them where eps does too: once more of m s
+    // squares that leave 32 bits, or vanish in them where eps does too: once more of m s. (Every lane of a workgroup goes the same
+    // way where the sum has a barrier in it: such a workgroup has one row.)
     float m = 1.0f;
     if (sum == INFINITY || (sum < 0x1p-96f && eps < 0x1p-60f)) {
         m = sum < 1.0f ? 0x1p48f : 0x1p-64f;
@@ -144,18 +154,20 @@ __global__ __launch_bounds__(L::BLOCK) void norm_kernel(const E* __restrict__ x,
     if (rstd && on && lane == 0) rstd[n] = m * r;
     if (y) {
         each([&](const pk& h, int64_t i) {
+            const auto w = take<P, false>(weight, i, D);
             pk o;
 #pragma unroll
-            for (int j = 0; j < P; j++) o.v[j] = E(m * float(h.v[j]) * r * weight[i + j]);
-            if (on) o.store_once(y + n * D + i);
+            for (int j = 0; j < P; j++) o.v[j] = E(m * float(h.v[j]) * r * w.v[j]);
+            if (on) leave<true>(o, y + n * D, i, D);
         });
         return;
     }
     // r is in every y of the row: q = s weight (448 / max |s weight|), without the roundings of y and of its scale
     float most = 0.0f;
     each([&](const pk& h, int64_t i) {
+        const auto w = take<P, false>(weight, i, D);
 #pragma unroll
-        for (int j = 0; j < P; j++) most = larger_or_nan(most, fabsf(m * float(h.v[j]) * weight[i + j]));
+        for (int j = 0; j < P; j++) most = larger_or_nan(most, fabsf(m * float(h.v[j]) * w.v[j]));
     });
     most = over_row<L>(most, lds, larger_or_nan);
     if (r == 0.0f) most = NAN;             // an infinity in the row
@@ -164,12 +176,13 @@ __global__ __launch_bounds__(L::BLOCK) void norm_kernel(const E* __restrict__ x,
     if (most < 0x1p-100f) { m *= 0x1p64f; most *= 0x1p64f; }
     const float up = most == 0.0f ? 0.0f : Q::MOST / most;
     each([&](const pk& h, int64_t i) {
+        const auto w = take<P, false>(weight, i, D);
         float v[P];
 #pragma unroll
-        for (int j = 0; j < P; j++) v[j] = m * float(h.v[j]) * weight[i + j] * up;
+        for (int j = 0; j < P; j++) v[j] = m * float(h.v[j]) * w.v[j] * up;
         pack<typename Q::type, P> o;
         Q::template make<P>(v, o);
-        o.store_once(q + n * D + i);
+        leave<true>(o, q + n * D, i, D);
     });
 }
 
@@ -177,19 +190,21 @@ template <typename E, typename L>
 __global__ __launch_bounds__(L::BLOCK) void norm_back_kernel(const E* __restrict__ s, const float* __restrict__ rstd, const float* __restrict__ weight, int64_t N,
                                                              int64_t D, int64_t ss, const E* __restrict__ d_y, const E* __restrict__ d_stream, E* __restrict__ d,
                                                              float* __restrict__ parts) {
-    constexpr int P = L::P, HELD = L::PACKS ? L::PACKS : 1;
+    constexpr int P = 16 / sizeof(E), HELD = L::PACKS ? L::PACKS : 1;
     using pk = pack<E, P>;
     __shared__ float lds[L::BLOCK / WAVE];
     const int lane = threadIdx.x % L::LANES, at = threadIdx.x / L::LANES;
-    const int64_t packs = D / P;
+    const int64_t packs = (D + P - 1) / P;
     float* part = parts + int64_t(blockIdx.x) * D;
-    float w[HELD][P], dw[HELD][P];
+    pack<float, P> w[HELD];
+    float dw[HELD][P];
     if constexpr (L::PACKS) {
 #pragma unroll
         for (int k = 0; k < HELD; k++) {
             const int64_t i = k * L::LANES + lane;
+            w[k] = i < packs ? take<P, false>(weight, i * P, D) : pack<float, P>::load_part(weight, 0);
 #pragma unroll
-            for (int j = 0; j < P; j++) { w[k][j] = i < packs ? weight[i * P + j] : 0.0f; dw[k][j] = 0.0f; }
+            for (int j = 0; j < P; j++) dw[k][j] = 0.0f;
         }
     } else {
         for (int64_t i = lane; i < D; i += L::LANES) part[i] = 0.0f;
@@ -204,16 +219,16 @@ __global__ __launch_bounds__(L::BLOCK) void norm_back_kernel(const E* __restrict
         if constexpr (L::PACKS) {
 #pragma unroll
             for (int k = 0; k < HELD; k++) if (const int64_t i = k * L::LANES + lane; i < packs) {
-                u[k] = pk::load_once(s + n * ss + i * P);
-                dy[k] = pk::load_once(d_y + n * D + i * P);
-                if (d_stream) ds[k] = pk::load_once(d_stream + n * D + i * P);
+                u[k] = take<P, true>(s + n * ss, i * P, D);
+                dy[k] = take<P, true>(d_y + n * D, i * P, D);
+                if (d_stream) ds[k] = take<P, true>(d_stream + n * D, i * P, D);
             }
 #pragma unroll
             for (int k = 0; k < HELD; k++) if (const int64_t i = k * L::LANES + lane; i < packs) {
 #pragma unroll
                 for (int j = 0; j < P; j++) {
                     const float a = float(u[k].v[j]) * r, b = float(dy[k].v[j]);
-                    sum = fmaf(b * w[k][j], a, sum);
+                    sum = fmaf(b * w[k].v[j], a, sum);
                     if (on) dw[k][j] = fmaf(b, a, dw[k][j]);
                 }
             }
@@ -232,10 +247,10 @@ __global__ __launch_bounds__(L::BLOCK) void norm_back_kernel(const E* __restrict
                 pk o;
 #pragma unroll
                 for (int j = 0; j < P; j++) {
-                    const float a = float(u[k].v[j]) * r, g = float(dy[k].v[j]) * w[k][j];
+                    const float a = float(u[k].v[j]) * r, g = float(dy[k].v[j]) * w[k].v[j];
                     o.v[j] = E((d_stream ? float(ds[k].v[j]) : 0.0f) + r * (g - a * mean));
                 }
-                o.store_once(d + n * D + i * P);
+                leave<true>(o, d + n * D, i * P, D);
             }
         } else {
             for (int64_t i = lane; i < D; i += L::LANES) {
@@ -245,27 +260,33 @@ __global__ __launch_bounds__(L::BLOCK) void norm_back_kernel(const E* __restrict
         }
     }
     if constexpr (L::PACKS) {
-        if constexpr (L::ROWS > 1) {       // the rows that the workgroup has at a time, summed in row 0's lanes
-            __shared__ float sums[L::ROWS - 1][HELD * P][L::LANES];
-            if (at) {
+        if constexpr (L::ROWS > 1) {       // the rows that the workgroup has at a time: summed by halves, in a fixed order
+            __shared__ float sums[L::ROWS / 2][HELD * P][L::LANES];
 #pragma unroll
-                for (int k = 0; k < HELD; k++)
+            for (int half = L::ROWS / 2; half; half /= 2) {
+                if (at >= half && at < 2 * half) {
 #pragma unroll
-                    for (int j = 0; j < P; j++) sums[at - 1][k * P + j][lane] = dw[k][j];
+                    for (int k = 0; k < HELD; k++)
+#pragma unroll
+                        for (int j = 0; j < P; j++) sums[at - half][k * P + j][lane] = dw[k][j];
+                }
+                __syncthreads();
+                if (at < half) {
+#pragma unroll
+                    for (int k = 0; k < HELD; k++)
+#pragma unroll
+                        for (int j = 0; j < P; j++) dw[k][j] += sums[at][k * P + j][lane];
+                }
+                __syncthreads();
             }
-            __syncthreads();
             if (at) return;
-#pragma unroll
-            for (int k = 0; k < HELD; k++)
-#pragma unroll
-                for (int j = 0; j < P; j++)
-#pragma unroll
-                    for (int o = 0; o < L::ROWS - 1; o++) dw[k][j] += sums[o][k * P + j][lane];
         }
 #pragma unroll
         for (int k = 0; k < HELD; k++) if (const int64_t i = k * L::LANES + lane; i < packs) {
+            pack<float, P> o;
 #pragma unroll
-            for (int j = 0; j < P; j++) part[i * P + j] = dw[k][j];
+            for (int j = 0; j < P; j++) o.v[j] = dw[k][j];
+            leave<false>(o, part, i * P, D);
         }
     }
 }
@@ -289,30 +310,27 @@ __global__ __launch_bounds__(END_WAVES* WAVE) void norm_weight_kernel(const floa
     d_weight[i] = sum;
 }
 
-// f(Plan) for rows of D elements of type E; wide: every row and tensor starts at a multiple of 16 bytes. The backward pass
-// holds three tensors, the weights and their gradients' sums, so its lanes take half as many elements.
-template <typename E, bool BACK, typename F> int32_t with_plan(int64_t D, bool wide, F&& f) {
-    if (wide) {
-        constexpr int P = 16 / sizeof(E);
-        const int64_t packs = D / P;
-        if (packs <= 64) return f(Plan<64, 1, P, 4>{});
-        if (packs <= 128) return f(Plan<64, 2, P, 4>{});
-        if constexpr (BACK) {
-            if (packs <= 256) return f(Plan<256, 1, P, 1>{});
-            if (packs <= 512) return f(Plan<256, 2, P, 1>{});
-            if (packs <= 2048) return f(Plan<1024, 2, P, 1>{});
-        } else {
-            if (packs <= 256) return f(Plan<64, 4, P, 4>{});
-            if (packs <= 512) return f(Plan<256, 2, P, 1>{});
-            if (packs <= 1024) return f(Plan<256, 4, P, 1>{});
-            if (packs <= 4096) return f(Plan<1024, 4, P, 1>{});
-        }
+// f(Plan) for rows of D elements of type E: as few lanes as hold the row in one pack each, up to a wave, then more packs, then more
+// waves. The backward pass holds three tensors, the weights and their gradients' sums, so its lanes take half as many elements.
+template <typename E, bool BACK, typename F> int32_t with_plan(int64_t D, F&& f) {
+    constexpr int P = 16 / sizeof(E);
+    const int64_t packs = (D + P - 1) / P;
+    if (packs <= 8) return f(Plan<8, 1, 32>{});
+    if (packs <= 16) return f(Plan<16, 1, 16>{});
+    if (packs <= 32) return f(Plan<32, 1, 8>{});
+    if (packs <= 64) return f(Plan<64, 1, 4>{});
+    if (packs <= 128) return f(Plan<64, 2, 4>{});
+    if constexpr (BACK) {
+        if (packs <= 256) return f(Plan<256, 1, 1>{});
+        if (packs <= 512) return f(Plan<256, 2, 1>{});
+        if (packs <= 2048) return f(Plan<1024, 2, 1>{});
     } else {
-        if (D <= 256) return f(Plan<64, 4, 1, 4>{});
-        if (D <= 2048) return f(Plan<256, 8, 1, 1>{});
-        if (D <= 8192) return f(Plan<1024, 8, 1, 1>{});
+        if (packs <= 256) return f(Plan<64, 4, 4>{});
+        if (packs <= 512) return f(Plan<256, 2, 1>{});
+        if (packs <= 1024) return f(Plan<256, 4, 1>{});
+        if (packs <= 4096) return f(Plan<1024, 4, 1>{});
     }
-    return f(Plan<256, 0, 1, 1>{});
+    return f(Plan<256, 0, 1>{});
 }
 
 int64_t groups_of(int64_t N, int rows) { const int64_t g = (N + rows - 1) / rows; return g < PARTS ? g : PARTS; }
@@ -331,10 +349,7 @@ int32_t forward(const void* x, const void* residual, const float* weight, int64_
     if (!x || !weight || (residual && !stream_out) || (!y && (!q || !scale))) return fail(PV_EARG, err, errcap, "null argument");
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
-        constexpr int packed = 16 / sizeof(E);
-        const bool wide = D % packed == 0 && (N == 1 || (xs % packed == 0 && (!residual || rs % packed == 0))) && aligned(x, 16) && aligned(residual, 16) &&
-                          aligned(y, 16) && aligned(stream_out, 16) && aligned(q, packed);
-        return with_plan<E, false>(D, wide, [&](auto plan) {
+        return with_plan<E, false>(D, [&](auto plan) {
             using L = decltype(plan);
             norm_kernel<E, Q, L><<<dim3((N + L::ROWS - 1) / L::ROWS), L::BLOCK, 0, hipStream_t(stream)>>>(
                 static_cast<const E*>(x), static_cast<const E*>(residual), weight, N, D, xs, rs, eps, static_cast<E*>(y), static_cast<E*>(stream_out), rstd,
@@ -375,9 +390,7 @@ int32_t pv_add_rms_norm_backward_hip(const void* s, const float* rstd, const flo
     float* parts = static_cast<float*>(work);
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
-        constexpr int packed = 16 / sizeof(E);
-        const bool wide = D % packed == 0 && (N <= 1 || s_row % packed == 0) && aligned(s, 16) && aligned(d_y, 16) && aligned(d_stream, 16) && aligned(d, 16);
-        return with_plan<E, true>(D, wide, [&](auto plan) {
+        return with_plan<E, true>(D, [&](auto plan) {
             using L = decltype(plan);
             const int64_t g = groups_of(N, L::ROWS);
             if (N) norm_back_kernel<E, L><<<dim3(g), L::BLOCK, 0, st>>>(static_cast<const E*>(s), rstd, weight, N, D, s_row, static_cast<const E*>(d_y),

@@ -20,16 +20,30 @@ template <> struct raw_of<2> { using type = uint16_t; };
 template <> struct raw_of<4> { using type = uint32_t; };
 template <> struct raw_of<8> { using type = __attribute__((ext_vector_type(2))) uint32_t; };
 template <> struct raw_of<16> { using type = __attribute__((ext_vector_type(4))) uint32_t; };
+template <> struct raw_of<32> { using type = __attribute__((ext_vector_type(8))) uint32_t; };      // (two loads)
 
-// N elements moved by one load or store of N * sizeof(T) bytes, which the address has to be a multiple of
+// N elements moved by one load or store of N * sizeof(T) bytes, from any address that an element may have: the compiler knows that
+// gfx950 takes global accesses off their own size's alignment, and makes one of each
 template <typename T, int N> struct pack {
     using raw = typename raw_of<int(sizeof(T)) * N>::type;
+    struct __attribute__((packed, aligned(sizeof(T)))) at_element { raw bits; };
     union { raw bits; T v[N]; };
-    __device__ static pack load(const T* p) { pack r; r.bits = *reinterpret_cast<const raw*>(p); return r; }
-    __device__ void store(T* p) const { *reinterpret_cast<raw*>(p) = bits; }
+    __device__ static pack load(const T* p) { pack r; r.bits = reinterpret_cast<const at_element*>(p)->bits; return r; }
+    __device__ void store(T* p) const { reinterpret_cast<at_element*>(p)->bits = bits; }
     // the same past the caches, for what is not used again soon
-    __device__ static pack load_once(const T* p) { pack r; r.bits = __builtin_nontemporal_load(reinterpret_cast<const raw*>(p)); return r; }
-    __device__ void store_once(T* p) const { __builtin_nontemporal_store(bits, reinterpret_cast<raw*>(p)); }
+    __device__ static pack load_once(const T* p) { pack r; r.bits = __builtin_nontemporal_load(&reinterpret_cast<const at_element*>(p)->bits); return r; }
+    __device__ void store_once(T* p) const { __builtin_nontemporal_store(bits, &reinterpret_cast<at_element*>(p)->bits); }
+    // the same of the first `left` elements, where there are fewer than N: one by one, the others 0 and not written
+    __device__ static pack load_part(const T* p, int64_t left) {
+        pack r;
+#pragma unroll
+        for (int j = 0; j < N; j++) r.v[j] = j < left ? p[j] : T(0.0f);
+        return r;
+    }
+    __device__ void store_part(T* p, int64_t left) const {
+#pragma unroll
+        for (int j = 0; j < N; j++) if (j < left) p[j] = v[j];
+    }
 };
 
 inline bool aligned(const void* p, uint64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
