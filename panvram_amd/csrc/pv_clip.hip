@@ -111,7 +111,8 @@ __global__ __launch_bounds__(BLOCK) void scale_kernel(Group G, const float* norm
         E* o = static_cast<E*>(G.to[k]);
         constexpr int P = 16 / sizeof(E);
         auto one = [&](int64_t i) { o[i] = E(float(g[i]) * factor); };
-        auto packs = [&](auto many, int64_t i, auto&& store) {
+        // (o may be off the 16 bytes that g's packs start at)
+        over_part(g, G.n[k], b - G.first[k], G.piece, one, [&](auto many, int64_t i) {
             constexpr int M = decltype(many)::value;
             pack<E, P> v[M];
 #pragma unroll
@@ -120,19 +121,9 @@ __global__ __launch_bounds__(BLOCK) void scale_kernel(Group G, const float* norm
             for (int m = 0; m < M; m++) {
 #pragma unroll
                 for (int j = 0; j < P; j++) v[m].v[j] = E(float(v[m].v[j]) * factor);
-                store(v[m], o + i + int64_t(m) * BLOCK * P);
+                v[m].store_once(o + i + int64_t(m) * BLOCK * P);
             }
-        };
-        const bool alike = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(o)) & 15) == 0;      // both start a pack at the same elements
-        if (alike)
-            over_part(g, G.n[k], b - G.first[k], G.piece, one, [&](auto many, int64_t i) { packs(many, i, [](const pack<E, P>& v, E* to) { v.store_once(to); }); });
-        else
-            over_part(g, G.n[k], b - G.first[k], G.piece, one, [&](auto many, int64_t i) {
-                packs(many, i, [](const pack<E, P>& v, E* to) {
-#pragma unroll
-                    for (int j = 0; j < P; j++) to[j] = v.v[j];
-                });
-            });
+        });
     };
     if (G.dtype[k] == PV_F32) go(float{}); else if (G.dtype[k] == PV_BF16) go(bf16{}); else go(f16{});
 }

@@ -46,37 +46,20 @@ struct Shape {
 __device__ inline int lane_c() { return threadIdx.x % 16; }
 __device__ inline int lane_g() { return threadIdx.x % WAVE / 16; }
 
-// N elements at p[i], i < left only, others 0
-template <bool WIDE, typename E, int N> __device__ inline pack<E, N> get(const E* p, int64_t left) {
-    if constexpr (WIDE) {
-        if (left > 0) return pack<E, N>::load(p);
-        pack<E, N> z;
-#pragma unroll
-        for (int j = 0; j < N; j++) z.v[j] = E(0.0f);
-        return z;
-    } else {
-        pack<E, N> r;
-#pragma unroll
-        for (int j = 0; j < N; j++) r.v[j] = j < left ? p[j] : E(0.0f);
-        return r;
-    }
+// A pack of which `left` elements are in the row: all, some, or none
+template <typename E, int N> __device__ inline pack<E, N> get(const E* p, int64_t left) {
+    return left >= N ? pack<E, N>::load(p) : pack<E, N>::load_part(p, left);
 }
-template <bool WIDE, typename E, int N> __device__ inline void put(const pack<E, N>& v, E* p, int64_t left) {
-    if constexpr (WIDE) {
-        if (left > 0) v.store_once(p);
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; j++) if (j < left) p[j] = v.v[j];
-    }
+template <typename E, int N> __device__ inline void put(const pack<E, N>& v, E* p, int64_t left) {
+    if (left >= N) v.store(p); else v.store_part(p, left);
 }
-
-// f(true) for a slab that lies within the row and is read 16 bytes at a time, else f(false): asked once, not at each load
-template <bool WIDE, typename F> __device__ inline void over_slab(bool within, F&& f) {
-    if (WIDE && within) f(std::true_type{}); else f(std::false_type{});
+// f(true) for a slab that lies within the row, else f(false): asked once, not at each load
+template <typename F> __device__ inline void over_slab(bool within, F&& f) {
+    if (within) f(std::true_type{}); else f(std::false_type{});
 }
 
 // A slab of 128 columns in bfloat16
-template <typename E_, bool WIDE> struct Bf {
+template <typename E_> struct Bf {
     using E = E_;
     using K = __bf16;                      // what the weights are laid out as
     static constexpr int COLS = 128, STEPS = 4, TILES = 8;
@@ -102,10 +85,10 @@ template <typename E_, bool WIDE> struct Bf {
     static __device__ Rows rows(const E* row, int64_t c0, int64_t D) {
         Rows R;
         row += c0 + 8 * lane_g();
-        over_slab<WIDE>(c0 + COLS <= D, [&](auto whole) {
+        over_slab(c0 + COLS <= D, [&](auto whole) {
 #pragma unroll
             for (int q = 0; q < STEPS; q++) {
-                const auto p = whole ? pack<E, 8>::load(row + 32 * q) : get<WIDE, E, 8>(row + 32 * q, D - c0 - 32 * q - 8 * lane_g());
+                const auto p = whole ? pack<E, 8>::load(row + 32 * q) : get<E, 8>(row + 32 * q, D - c0 - 32 * q - 8 * lane_g());
                 __builtin_memcpy(&R.h[q], &p, 16);
             }
         });
@@ -137,7 +120,7 @@ template <typename E_, bool WIDE> struct Bf {
 #pragma unroll
         for (int j = 0; j < 4; j++) one[j] = c == 4 * g + j ? 0x3f80 : 0;
         const s16x4 thi = bits(product(hi, one, none)), tlo = bits(product(lo, one, none));      // id c, places 4 g + j
-        const bool whole = WIDE && c0 + COLS <= D;
+        const bool whole = c0 + COLS <= D;
         d_row += c0 + 8 * g;
 #pragma unroll
         for (int q = 0; q < STEPS; q++) {
@@ -154,8 +137,8 @@ template <typename E_, bool WIDE> struct Bf {
             if (store) {
                 pack<E, 8> p;
                 __builtin_memcpy(&p, o, 16);
-                if (whole) p.store_once(d_row + 32 * q);
-                else put<WIDE, E, 8>(p, d_row + 32 * q, D - c0 - 32 * q - 8 * g);
+                if (whole) p.store_once(d_row + 32 * q);       // (8 x 8,192 x 512 in 44 us, 50 by way of the caches; F3's is as fast or faster by way of them)
+                else put<E, 8>(p, d_row + 32 * q, D - c0 - 32 * q - 8 * g);
             }
         }
     }
@@ -164,7 +147,7 @@ template <typename E_, bool WIDE> struct Bf {
 };
 
 // A slab of 64 columns in 32 bits
-template <typename E_, bool WIDE> struct F3 {
+template <typename E_> struct F3 {
     using E = E_;
     using K = float;
     static constexpr int COLS = 64, STEPS = 4, TILES = 4;
@@ -187,9 +170,9 @@ template <typename E_, bool WIDE> struct F3 {
     static __device__ Rows rows(const E* row, int64_t c0, int64_t D) {
         Rows R;
         row += c0 + 4 * lane_g();
-        over_slab<WIDE>(c0 + COLS <= D, [&](auto whole) {
+        over_slab(c0 + COLS <= D, [&](auto whole) {
 #pragma unroll
-            for (int s = 0; s < STEPS; s++) R.h[s] = whole ? pack<E, 4>::load(row + 16 * s) : get<WIDE, E, 4>(row + 16 * s, D - c0 - 16 * s - 4 * lane_g());
+            for (int s = 0; s < STEPS; s++) R.h[s] = whole ? pack<E, 4>::load(row + 16 * s) : get<E, 4>(row + 16 * s, D - c0 - 16 * s - 4 * lane_g());
         });
         return R;
     }
@@ -216,7 +199,7 @@ template <typename E_, bool WIDE> struct F3 {
         f32x4 t = none;                    // id c, places 4 g + j
 #pragma unroll
         for (int j = 0; j < 4; j++) t = product(dl[j], one[j], t);
-        const bool whole = WIDE && c0 + COLS <= D;
+        const bool whole = c0 + COLS <= D;
         d_row += c0 + 4 * g;
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
@@ -230,8 +213,8 @@ template <typename E_, bool WIDE> struct F3 {
                 pack<E, 4> o;
 #pragma unroll
                 for (int r = 0; r < 4; r++) o.v[r] = E(x[r]);
-                if (whole) o.store_once(d_row + 16 * s);
-                else put<WIDE, E, 4>(o, d_row + 16 * s, D - c0 - 16 * s - 4 * g);
+                if (whole) o.store(d_row + 16 * s);
+                else put<E, 4>(o, d_row + 16 * s, D - c0 - 16 * s - 4 * g);
             }
         }
     }
@@ -577,21 +560,12 @@ int32_t pv_next_base_loss_hip(const void* hidden, const void* weight, const void
     if (!work || work_bytes < pv_next_base_loss_work_bytes(B, T, D, V, d_hidden != nullptr)) return fail(PV_EARG, err, errcap, "work: too small");
     Shape S{B, T, D, B * T, hidden_b, hidden_t, tokens_b, ignore, 0, V, token_bytes, B == 1 || hidden_b == T * hidden_t};
     const bool narrow = dtype == PV_BF16 && weight_dtype == PV_BF16;
-    const int64_t per = narrow ? 8 : 4, bytes = per * element_bytes(dtype);
-    const bool wide = D % per == 0 && (T == 1 || hidden_t % per == 0) && (B == 1 || hidden_b % per == 0) && aligned(hidden, bytes) && aligned(d_hidden, bytes);
     const hipStream_t st = hipStream_t(stream);
-    if (narrow) {
-        if (wide) return run<Bf<bf16, true>, bf16>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, st, err, errcap);
-        return run<Bf<bf16, false>, bf16>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, st, err, errcap);
-    }
+    if (narrow) return run<Bf<bf16>, bf16>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, st, err, errcap);
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
-        auto go = [&](auto w) {
-            using W = decltype(w);
-            if (wide) return run<F3<E, true>, W>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, st, err, errcap);
-            return run<F3<E, false>, W>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, st, err, errcap);
-        };
-        return weight_dtype == PV_F32 ? go(float{}) : go(E{});
+        if (weight_dtype == PV_F32) return run<F3<E>, float>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, st, err, errcap);
+        return run<F3<E>, E>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, st, err, errcap);
     });
 }
 
