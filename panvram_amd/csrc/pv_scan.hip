@@ -50,6 +50,15 @@ __device__ inline Map then(Map first, Map second) {
     return {first.A == CUT || second.A == CUT ? CUT : first.A * second.A, apply(second, first.H)};
 }
 
+// A wave has 64 x VEC channels from d0 on, slot VEC * lane + v. The last lane of an odd D takes channel D - 2 once more beside the
+// last one: it computes and writes what its neighbour does.
+template <int VEC> __device__ inline int64_t channel_of(int64_t D, int64_t d0, int slot) {
+    int64_t d = d0 + slot / VEC * VEC;
+    if (VEC > 1 && d + VEC > D) d = D - VEC;
+    return d + slot % VEC;
+}
+template <int VEC> __device__ inline bool is_channel(int64_t D, int64_t d0, int slot) { return d0 + slot / VEC * VEC < D; }
+
 // ---- Maps of chunks, in the order of the walk (position 0 first), passed between workgroups.
 // Level 0 has a map for each chunk, level l + 1 one for each FAN whole neighbours of level l. The workgroup at position p needs
 // the maps of its predecessors within its group of FAN, of their group's predecessors within its, and so on: the base-FAN
@@ -124,8 +133,9 @@ template <int VEC, int WAVES, bool ONE> struct Place {
         p = q;
         b = c;
         d0 = int64_t(rest - c * uint32_t(S.tiles)) * (WAVE * VEC);
-        d = d0 + lane * VEC;
-        on = d < S.D;
+        if (S.D - d0 < VEC) d0 = S.D - VEC;    // (one channel left over: with its neighbour)
+        d = channel_of<VEC>(S.D, d0, lane * VEC);
+        on = is_channel<VEC>(S.D, d0, lane * VEC);
     }
 };
 
@@ -142,7 +152,8 @@ template <int STEPS> __device__ inline Span span_of(const Shape& S, const uint8_
 }
 // (from is the same for the wave, at: the lane's channel in it)
 // A wave's steps of a tensor as a buffer of its rows: step i is at i * stride bytes, and what lies behind the span (or at NO_LANE)
-// is not read and not written, so that neither the end of T nor that of D needs a branch.
+// is not read and not written, so that neither the end of T nor that of D needs a branch. Rows may begin at any element: gfx950
+// takes a 4-byte access at 2 bytes' alignment.
 constexpr uint32_t NO_LANE = 1u << 31;
 // ONCE: accesses with the hint that the data is not used again soon (`once_of` says when)
 constexpr int64_t MOST_STRIDE = 1 << 26;   // bytes: the offsets of a wave's steps stay below 2^31
@@ -226,8 +237,8 @@ template <int VEC, int WAVES> struct Before {
     __device__ void wait(const Records& R, const Shape& S, int64_t b, int64_t p, int64_t d0, int wave, int lane, Map own) {
         constexpr int TEAMS = WAVES / VEC;
         const int c = wave % VEC * WAVE + lane, team = wave / VEC;
-        const int64_t d = d0 + c;
-        const bool on = d < S.D;
+        const int64_t d = channel_of<VEC>(S.D, d0, c);
+        const bool on = is_channel<VEC>(S.D, d0, c);
         if (team == 0) publish(R.level[0] + (b * S.chunks + p) * S.D + d, own, on);
         int64_t n = S.chunks;
         int l = 0;
@@ -270,7 +281,7 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
     __shared__ Before<VEC, WAVES> before;
     const Place<VEC, WAVES, ONE> P(S, R);
     const Span s = span_of<STEPS>(S, reset, P.b, (P.p * WAVES + P.wave) * STEPS, P.lane);
-    const uint32_t at = P.on ? P.lane * VEC * sizeof(E) : NO_LANE;
+    const uint32_t at = P.on ? uint32_t(P.d - P.d0) * sizeof(E) : NO_LANE;
     const int64_t width = S.D - P.d0 < WAVE * VEC ? S.D - P.d0 : WAVE * VEC;
     Word<E, VEC> g[STEPS], x[STEPS];
     load_steps(g, Rows<ONCE>(gate + P.b * S.gb + P.d0, S.gt, s, width), at);
@@ -353,7 +364,7 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
     const Place<VEC, WAVES, ONE> P(S, R);
     const int64_t c = S.chunks - 1 - P.p;              // the walk begins at the last chunk
     const Span s = span_of<STEPS>(S, reset, P.b, (c * WAVES + P.wave) * STEPS, P.lane);
-    const uint32_t at = P.on ? P.lane * VEC * sizeof(E) : NO_LANE;
+    const uint32_t at = P.on ? uint32_t(P.d - P.d0) * sizeof(E) : NO_LANE;
     const int64_t width = S.D - P.d0 < WAVE * VEC ? S.D - P.d0 : WAVE * VEC;
     Word<E, VEC> g[STEPS], x[STEPS], y[STEPS];
     load_steps(g, Rows<ONCE>(gate + P.b * S.gb + P.d0, S.gt, s, width), at);
@@ -506,11 +517,6 @@ template <int STEPS, typename F> int32_t launch(Shape& S, bool pairs, bool reset
     return resets ? with(integral_constant<int, 1>{}, std::true_type{}) : with(integral_constant<int, 1>{}, std::false_type{});
 }
 
-// Whether a [B, T, D] tensor's rows can be read two channels at a time
-template <typename E> bool pairs_of(const void* p, int64_t B, int64_t T, int64_t sb, int64_t st) {
-    return aligned(p, 2 * sizeof(E)) && (B == 1 || sb % 2 == 0) && (T == 1 || st % 2 == 0);
-}
-
 }  // namespace
 
 extern "C" {
@@ -530,7 +536,7 @@ int32_t pv_gated_scan_hip(const void* gate, const void* value, const float* stat
     const hipStream_t st = hipStream_t(stream);
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
-        const bool pairs = sizeof(E) == 2 && D % 2 == 0 && pairs_of<E>(gate, B, T, gate_b, gate_t) && pairs_of<E>(value, B, T, value_b, value_t) && aligned(out, 4);
+        const bool pairs = sizeof(E) == 2 && D > 1;
         return launch<STEPS_FORWARD>(S, pairs, reset, once_of(B, T, D, sizeof(E)), work, st, [&](auto vec, auto steps, auto waves, auto one, auto resets, auto once, const Records& R, uint32_t groups) {
             constexpr int V = decltype(vec)::value, N = decltype(steps)::value, W = decltype(waves)::value;
             constexpr bool ONE = decltype(one)::value, RESET = decltype(resets)::value, ONCE = decltype(once)::value && V * sizeof(E) == 4;
@@ -553,8 +559,7 @@ int32_t pv_gated_scan_backward_hip(const void* gate, const void* value, const fl
     const hipStream_t st = hipStream_t(stream);
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
-        const bool pairs = sizeof(E) == 2 && D % 2 == 0 && pairs_of<E>(gate, B, T, gate_b, gate_t) && pairs_of<E>(value, B, T, value_b, value_t) &&
-                           pairs_of<E>(d_out, B, T, d_out_b, d_out_t) && aligned(d_gate, 4) && aligned(d_value, 4);
+        const bool pairs = sizeof(E) == 2 && D > 1;
         return launch<STEPS_BACK>(S, pairs, reset, once_of(B, T, D, sizeof(E)), work, st, [&](auto vec, auto steps, auto waves, auto one, auto resets, auto once, const Records& R, uint32_t groups) {
             constexpr int V = decltype(vec)::value, N = decltype(steps)::value, W = decltype(waves)::value;
             constexpr bool ONE = decltype(one)::value, RESET = decltype(resets)::value, ONCE = decltype(once)::value && V * sizeof(E) == 4;
