@@ -16,9 +16,6 @@ namespace {
 
 constexpr int PARTS = 1024;                 // workgroups of the backward pass at most: rows of partial weight gradients
 
-// The larger of two values that are not negative, a NaN being the largest: their bits are in that order
-__device__ inline float larger_or_nan(float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); }
-
 // An 8-bit format: its largest value, and P values of it from floats that are at most that but for a rounding
 struct Fp8 {
     using type = uint8_t;
@@ -55,9 +52,9 @@ template <int LANES_, int PACKS_, int ROWS_> struct Plan {
 };
 
 // A sum, or a largest value, over the lanes of a row
-template <typename L, typename F> __device__ inline float over_row(float x, float* lds, F&& join) {
+template <typename L, typename T, typename F> __device__ inline T over_row(T x, T* lds, F&& join) {
 #pragma unroll
-    for (int d = (L::LANES < WAVE ? L::LANES : WAVE) / 2; d; d >>= 1) x = join(x, __shfl_xor(x, d, WAVE));
+    for (int d = (L::LANES < WAVE ? L::LANES : WAVE) / 2; d; d >>= 1) x = join(x, T(__shfl_xor(x, d, WAVE)));
     if constexpr (L::WAVES > 1) {
         const int row = threadIdx.x / L::LANES, wave = threadIdx.x / WAVE;
         __syncthreads();                                       // the last use of lds is over
@@ -162,24 +159,40 @@ __global__ __launch_bounds__(L::BLOCK) void norm_kernel(const E* __restrict__ x,
         });
         return;
     }
-    // r is in every y of the row: q = s weight (448 / max |s weight|), without the roundings of y and of its scale
-    float most = 0.0f;
+    // r is in every y of the row: q = s weight (448 / max |s weight|), and is made from products in two floats (x + the rest of x), so
+    // that it is the value nearest to the exact quotient, a tie of which a rounding before would decide by chance. The largest
+    // product is found by a key: its bits, which are in order as it is not negative (a NaN being the largest), then its rest's.
+    __shared__ unsigned long long keys[L::BLOCK / WAVE];
+    unsigned long long key = 0;
     each([&](const pk& h, int64_t i) {
         const auto w = take<P, false>(weight, i, D);
 #pragma unroll
-        for (int j = 0; j < P; j++) most = larger_or_nan(most, fabsf(m * float(h.v[j]) * w.v[j]));
+        for (int j = 0; j < P; j++) {
+            const float a = fabsf(m * float(h.v[j])), b = fabsf(w.v[j]), x = a * b;
+            const int32_t rest = __float_as_int(fmaf(a, b, -x));
+            const unsigned long long k = uint64_t(__float_as_uint(x)) << 32 | uint32_t(rest ^ (rest >> 31 | INT32_MIN));
+            key = k > key ? k : key;
+        }
     });
-    most = over_row<L>(most, lds, larger_or_nan);
+    key = over_row<L>(key, keys, [](unsigned long long a, unsigned long long b) { return a > b ? a : b; });
+    float most = __uint_as_float(uint32_t(key >> 32));
+    const int32_t bits = int32_t(uint32_t(key));
+    float rest = most < INFINITY ? __int_as_float(bits ^ (~bits >> 31 | INT32_MIN)) : 0.0f;
     if (r == 0.0f) most = NAN;             // an infinity in the row
     if (!on) return;
     if (lane == 0) scale[n] = most / Q::MOST * r;
-    if (most < 0x1p-100f) { m *= 0x1p64f; most *= 0x1p64f; }
+    if (most < 0x1p-100f) { m *= 0x1p64f; most *= 0x1p64f; rest *= 0x1p64f; }
     const float up = most == 0.0f ? 0.0f : Q::MOST / most;
+    const float up_rest = most == 0.0f ? 0.0f : fmaf(-up, rest, fmaf(-up, most, Q::MOST)) / most;
     each([&](const pk& h, int64_t i) {
         const auto w = take<P, false>(weight, i, D);
         float v[P];
 #pragma unroll
-        for (int j = 0; j < P; j++) v[j] = m * float(h.v[j]) * w.v[j] * up;
+        for (int j = 0; j < P; j++) {
+#pragma clang fp contract(off)     // (y + ... as one operation would count y's own rounding twice)
+            const float a = m * float(h.v[j]), x = a * w.v[j], y = x * up;
+            v[j] = y + fmaf(fmaf(a, w.v[j], -x), up, fmaf(x, up_rest, fmaf(x, up, -y)));
+        }
         pack<typename Q::type, P> o;
         Q::template make<P>(v, o);
         leave<true>(o, q + n * D, i, D);
