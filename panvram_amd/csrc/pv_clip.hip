@@ -7,15 +7,15 @@
 //
 // What bounds it: the bytes, read once for the norm and once more for the scaling where they are more than the caches hold.
 // Measured: 500 M bfloat16 elements in 300 tensors, squares 166 us (1.0 GB: 6.0 TB/s), scaling 328 us (2.0 GB: 6.1 TB/s; the last
-// tensors first, which the caches may still have). 2 M float32 elements in 150 tensors 22 us in five launches, where the host
-// needs 100 us for their addresses, sizes and types.
+// tensors first, which the caches may still have). 2 M float32 elements in 150 tensors 17 us in three launches, where the host
+// needs 90 us for their addresses, sizes and types.
 #include "pv_ops.h"
 
 using namespace pvo;
 
 namespace {
 
-constexpr int GROUP = 120;                 // tensors of one launch: 29 bytes each of the 4 KiB that a launch's arguments may take
+constexpr int GROUP = 160;                 // tensors of one launch: 25 bytes each of the 4 KiB that a launch's arguments may take
 constexpr int BLOCK = 256;
 // Bytes of a workgroup. Scaling: four loads of 16 bytes a lane (1 GiB read and written in 334 us; 370 with 64 KiB, 394 with 256).
 // The sum of squares: the same, or more, so that there are no more than MOST partial sums for one workgroup to add up (1 GiB
@@ -25,13 +25,16 @@ constexpr int64_t LINE = BLOCK * 16, PIECE = 4 * LINE, MOST = 4096;
 struct Group {
     const void* from[GROUP];
     void* to[GROUP];
-    int64_t n[GROUP];
     uint32_t first[GROUP];                 // workgroup that begins a tensor
-    uint8_t dtype[GROUP];
+    uint32_t low[GROUP];                   // its elements: low 32 bits, and 6 above them beside the type's 2
+    uint8_t high[GROUP];
     int32_t count;
     int64_t piece;                         // bytes of a workgroup
+    __host__ __device__ int64_t size(int k) const { return int64_t(high[k] >> 2) << 32 | low[k]; }
+    __host__ __device__ int32_t dtype(int k) const { return high[k] & 3; }
 };
-static_assert(sizeof(Group) <= 3600, "a launch's arguments");
+static_assert(sizeof(Group) <= 4064, "a launch's arguments");
+constexpr int64_t MOST_SIZE = int64_t(1) << 38;
 
 // The tensor that workgroup `b` works on: the last that begins at or before it
 __device__ inline int tensor_of(const Group& G, uint32_t b) {
@@ -76,7 +79,7 @@ __global__ __launch_bounds__(BLOCK) void square_kernel(Group G, double* parts) {
         using E = decltype(e);
         const E* g = static_cast<const E*>(G.from[k]);
         constexpr int P = 16 / sizeof(E);
-        over_part(g, G.n[k], blockIdx.x - G.first[k], G.piece,
+        over_part(g, G.size(k), blockIdx.x - G.first[k], G.piece,
                   [&](int64_t i) { const double x = double(float(g[i])); sum[0] = fma(x, x, sum[0]); },
                   [&](auto many, int64_t i) {
                       constexpr int M = decltype(many)::value;
@@ -89,7 +92,7 @@ __global__ __launch_bounds__(BLOCK) void square_kernel(Group G, double* parts) {
                           for (int j = 0; j < P; j++) { const double x = double(float(v[m].v[j])); sum[j % 4] = fma(x, x, sum[j % 4]); }
                   });
     };
-    if (G.dtype[k] == PV_F32) go(float{}); else if (G.dtype[k] == PV_BF16) go(bf16{}); else go(f16{});
+    if (G.dtype(k) == PV_F32) go(float{}); else if (G.dtype(k) == PV_BF16) go(bf16{}); else go(f16{});
     const double all = block_sum<BLOCK / WAVE>((sum[0] + sum[1]) + (sum[2] + sum[3]));
     if (threadIdx.x == 0) parts[blockIdx.x] = all;
 }
@@ -117,7 +120,7 @@ __global__ __launch_bounds__(BLOCK) void scale_kernel(Group G, const float* norm
         constexpr int P = 16 / sizeof(E);
         auto one = [&](int64_t i) { o[i] = E(float(g[i]) * factor); };
         // (o may be off the 16 bytes that g's packs start at)
-        over_part(g, G.n[k], b - G.first[k], G.piece, one, [&](auto many, int64_t i) {
+        over_part(g, G.size(k), b - G.first[k], G.piece, one, [&](auto many, int64_t i) {
             constexpr int M = decltype(many)::value;
             pack<E, P> v[M];
 #pragma unroll
@@ -130,7 +133,7 @@ __global__ __launch_bounds__(BLOCK) void scale_kernel(Group G, const float* norm
             }
         });
     };
-    if (G.dtype[k] == PV_F32) go(float{}); else if (G.dtype[k] == PV_BF16) go(bf16{}); else go(f16{});
+    if (G.dtype(k) == PV_F32) go(float{}); else if (G.dtype(k) == PV_BF16) go(bf16{}); else go(f16{});
 }
 
 int64_t piece_of(const int64_t* sizes, const int32_t* dtypes, int32_t count) {
@@ -157,8 +160,8 @@ template <typename F> void groups(const void* const* from, void* const* to, cons
         }
         G.from[G.count] = from[i];
         G.to[G.count] = to ? to[i] : nullptr;
-        G.n[G.count] = n[i];
-        G.dtype[G.count] = uint8_t(dtypes[i]);
+        G.low[G.count] = uint32_t(n[i]);
+        G.high[G.count] = uint8_t(n[i] >> 32 << 2 | dtypes[i]);
         G.first[G.count++] = uint32_t(blocks);
         blocks += blocks_of(n[i], dtypes[i], piece);
     }
@@ -172,7 +175,7 @@ int32_t check(const void* const* grads, void* const* out, const int64_t* sizes, 
     for (int32_t i = 0; i < count; i++) {
         const int bytes = element_bytes(dtypes[i]);
         if (!bytes) return fail(PV_EARG, err, cap, "dtype: one of PV_F32, PV_BF16, PV_F16");
-        if (sizes[i] < 0 || sizes[i] > (int64_t(1) << 40) || (all += sizes[i]) > (int64_t(1) << 40)) return fail(PV_EARG, err, cap, "size: 0 to 2^40 elements in all");
+        if (sizes[i] < 0 || sizes[i] >= MOST_SIZE || (all += sizes[i]) > (int64_t(1) << 40)) return fail(PV_EARG, err, cap, "size: 0 to 2^38 elements, 2^40 in all");
         if (sizes[i] && (!grads[i] || (out && !out[i]))) return fail(PV_EARG, err, cap, "null argument");
         if (sizes[i] && (!aligned(grads[i], bytes) || (out && !aligned(out[i], bytes)))) return fail(PV_EARG, err, cap, "address: not a multiple of the element's size");
     }
