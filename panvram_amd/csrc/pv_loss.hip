@@ -355,8 +355,14 @@ void fused_kernel(Shape S, const typename M::E* __restrict__ hidden, const void*
             mine[wave * WAVE + lane] = l;
             __syncthreads();               // (the other half is free again: every wave has passed the tile before)
             if (!GRADS && wave) continue;
-            l = mine[lane];
-            for (int k = 1; k < waves; k++) l += mine[k * WAVE + lane];
+            mine += lane;
+            l = mine[0];
+            int k = 1;
+            for (; !GRADS && k + 3 < waves; k += 4) {      // (four reads under way at a time; with gradients there are no registers for them)
+                const f32x4 a = mine[k * WAVE], b = mine[(k + 1) * WAVE], d = mine[(k + 2) * WAVE], e = mine[(k + 3) * WAVE];
+                l += (a + b) + (d + e);
+            }
+            for (; k < waves; k++) l += mine[k * WAVE];
         }
         const float x = softmax(l, now.at, S.V, factor ? now.w : base, wave == 0);
         const int64_t n = tile * TILE + c;
