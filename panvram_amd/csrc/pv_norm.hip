@@ -352,6 +352,11 @@ template <typename E, bool BACK, typename F> int32_t with_plan(int64_t D, F&& f)
     return f(Plan<256, 0, 1>{});
 }
 
+template <typename E> int rows_of(int64_t D) {
+    int rows = 0;
+    with_plan<E, true>(D, [&](auto plan) { rows = decltype(plan)::ROWS; return 0; });
+    return rows;
+}
 int64_t groups_of(int64_t N, int rows) { const int64_t g = (N + rows - 1) / rows; return g < PARTS ? g : PARTS; }
 
 int32_t check(int64_t N, int64_t D, int32_t dtype, char* err, size_t cap) {
@@ -397,24 +402,29 @@ int32_t pv_add_rms_norm_8bit_hip(const void* x, const void* residual, const floa
     return fail(PV_EARG, err, errcap, "format: PV_E4M3 or PV_INT8");
 }
 
-uint64_t pv_add_rms_norm_work_bytes(int64_t N, int64_t D) { return N > 0 && D > 0 ? uint64_t(groups_of(N, 1)) * uint64_t(D) * 4 : 0; }
+uint64_t pv_add_rms_norm_work_bytes(int64_t N, int64_t D) {
+    // (rows at a time of a workgroup are as many or fewer for 16-bit elements, whose packs are fewer: float's plan has the fewest)
+    const int64_t g = N > 0 && D > 0 ? groups_of(N, rows_of<float>(D)) : 0;
+    return g > 1 ? uint64_t(g) * uint64_t(D) * 4 : 0;
+}
 
 int32_t pv_add_rms_norm_backward_hip(const void* s, const float* rstd, const float* weight, int64_t N, int64_t D, int64_t s_row, const void* d_y,
                                      const void* d_stream, int32_t dtype, void* d, float* d_weight, void* work, uint64_t work_bytes, void* stream, char* err,
                                      size_t errcap) {
     if (int32_t e = check(N, D, dtype, err, errcap)) return e;
     if (!d_weight || (N && (!s || !rstd || !weight || !d_y || !d))) return fail(PV_EARG, err, errcap, "null argument");
-    if (work_bytes < pv_add_rms_norm_work_bytes(N, D) || (N && !work)) return fail(PV_EARG, err, errcap, "work: too small");
+    const uint64_t need = pv_add_rms_norm_work_bytes(N, D);
+    if (need && (!work || work_bytes < need)) return fail(PV_EARG, err, errcap, "work: too small");
     const hipStream_t st = hipStream_t(stream);
-    float* parts = static_cast<float*>(work);
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
         return with_plan<E, true>(D, [&](auto plan) {
             using L = decltype(plan);
             const int64_t g = groups_of(N, L::ROWS);
+            float* parts = g > 1 ? static_cast<float*>(work) : d_weight;       // (one workgroup's part is the sum)
             if (N) norm_back_kernel<E, L><<<dim3(g), L::BLOCK, 0, st>>>(static_cast<const E*>(s), rstd, weight, N, D, s_row, static_cast<const E*>(d_y),
                                                                         static_cast<const E*>(d_stream), static_cast<E*>(d), parts);
-            norm_weight_kernel<<<dim3((D + WAVE - 1) / WAVE), END_WAVES * WAVE, 0, st>>>(parts, g, D, d_weight);
+            if (g != 1) norm_weight_kernel<<<dim3((D + WAVE - 1) / WAVE), END_WAVES * WAVE, 0, st>>>(parts, g, D, d_weight);
             return launched(err, errcap);
         });
     });

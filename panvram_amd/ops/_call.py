@@ -4,6 +4,7 @@ raised."""
 import threading
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _native as N
 from .._streams import raw as _raw
@@ -45,6 +46,17 @@ def call(fn, index, *args):
     code = fn(*args, _raw.get(index), err, 4096)
     if code:
         N.raise_for(code, err)
+
+
+def once(backward):
+    """An autograd function's backward(ctx, *gradients) that cannot be differentiated again. Asked for a graph of the
+    gradients (create_graph=True), it is torch's once_differentiable, which raises if that graph is used; else it runs as
+    it is, without that wrapper's 10 us."""
+    careful = once_differentiable(backward)
+
+    def either(ctx, *gradients):
+        return careful(ctx, *gradients) if torch.is_grad_enabled() else backward(ctx, *gradients)
+    return either
 
 
 def ptr(t):

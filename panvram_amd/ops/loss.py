@@ -1,9 +1,8 @@
 """The head and loss over a small alphabet (panvram_amd/csrc/pv_loss.hip)."""
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _native as N
-from ._call import DTYPES, call, on_gpu, ptr, rows
+from ._call import DTYPES, call, on_gpu, once, ptr, rows
 
 
 def _run(hidden, weight, tokens, ignore, want_each, want_loss, grads, scale=None, factor=None):
@@ -33,7 +32,7 @@ class _NextBaseLoss(torch.autograd.Function):
         return loss if mean else each
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, d):
         hidden, weight, tokens = ctx.saved_tensors
         d = d.contiguous()

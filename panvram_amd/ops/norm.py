@@ -1,9 +1,8 @@
 """The residual stream's addition and root-mean-square norm (panvram_amd/csrc/pv_norm.hip)."""
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _native as N
-from ._call import DTYPES, call, on_gpu, ptr
+from ._call import DTYPES, call, on_gpu, once, ptr
 
 _FORMATS = {torch.float8_e4m3fn: N.E4M3, torch.int8: N.INT8}
 
@@ -43,7 +42,7 @@ class _AddRmsNorm(torch.autograd.Function):
         return y if stream is None else (y, stream)
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, d_y, d_stream=None):
         s, rstd, weight = ctx.saved_tensors
         if d_y is None:
@@ -55,10 +54,10 @@ class _AddRmsNorm(torch.autograd.Function):
         d_weight = torch.empty(D, dtype=torch.float32, device=dev)
         L = N.lib()
         size = L.pv_add_rms_norm_work_bytes(count, D)
-        work = torch.empty(size, dtype=torch.uint8, device=dev)
+        work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         flat, ss = _flat(s)
         call(L.pv_add_rms_norm_backward_hip, s.get_device(), flat.data_ptr(), rstd.data_ptr(), weight.data_ptr(), count, D, ss, d_y.data_ptr(), ptr(d_stream),
-             DTYPES[dtype], d.data_ptr(), d_weight.data_ptr(), work.data_ptr(), size)
+             DTYPES[dtype], d.data_ptr(), d_weight.data_ptr(), ptr(work), size)
         return d, None if ctx.alone else d, d_weight, None
 
 

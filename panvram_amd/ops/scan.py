@@ -1,9 +1,8 @@
 """The gated linear recurrence over sequences (panvram_amd/csrc/pv_scan.hip)."""
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _native as N
-from ._call import DTYPES, call, on_gpu, ptr, rows
+from ._call import DTYPES, call, on_gpu, once, ptr, rows
 
 
 def _steps(t):
@@ -47,7 +46,7 @@ class _GatedScan(torch.autograd.Function):
         return out, last
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, d_out, d_last):
         gate, value, carry, reset = ctx.saved_tensors
         B, T, D = gate.shape

@@ -166,6 +166,19 @@ def test_gradients_against_differences():
         assert abs(float((got * way).sum()) - want) <= 1e-5 * float((got * way).abs().sum()) + 1e-6
 
 
+def test_gradients_of_gradients_are_refused():
+    """A graph of the gradients may be asked for (create_graph=True), but not differentiated."""
+    from panvram_amd import ops
+    x, _, weight, d_y, _ = make(4, 64, torch.float32, seed=6, residual=False)
+    a = x.clone().requires_grad_()
+    y, _ = ops.add_rms_norm(a, None, weight, eps=EPS)
+    (plain,) = torch.autograd.grad(y, (a,), d_y, retain_graph=True)
+    (d,) = torch.autograd.grad(y, (a,), d_y, create_graph=True)
+    assert torch.equal(plain, d)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(d.sum(), (a,))
+
+
 def test_empty():
     from panvram_amd import ops
     x = torch.zeros(0, 12, device="cuda", requires_grad=True)

@@ -70,7 +70,7 @@ def test_norm_entries():
     assert "null" in bits8(q=None) and "null" in bits8(scale=None)
 
     def back(work=FAKE, work_bytes=1 << 20, d=FAKE):
-        return refused("pv_add_rms_norm_backward_hip", FAKE, FAKE, FAKE, 4, 8, 8, FAKE, None, N.F32, d, FAKE, work, work_bytes)
+        return refused("pv_add_rms_norm_backward_hip", FAKE, FAKE, FAKE, 4000, 8, 8, FAKE, None, N.F32, d, FAKE, work, work_bytes)
     assert "work" in back(work=None) and "work" in back(work_bytes=16)
     assert "null" in back(d=None)
 
