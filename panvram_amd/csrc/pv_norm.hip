@@ -11,7 +11,7 @@
 //
 // What bounds it: the bytes. x, residual, y and all of the backward pass's tensors are passed by the caches, so that the stream,
 // which the next layer and the backward pass read, stays in them (65,536 x 1,024 bfloat16 forwards and backwards 197 us with
-// this, 240 without). Measured: those forwards 80-84 us (537 MB: 6.4-6.7 TB/s), backwards 83-86 us (537 MB: 6.2-6.4) and 4 us
+// this, 240 without; 3,487 x 4,127 float32, 58 MB a tensor, 49 and 70 us with it, 45 and 62 without). Measured: those forwards 80-84 us (537 MB: 6.4-6.7 TB/s), backwards 83-86 us (537 MB: 6.2-6.4) and 4 us
 // for the weight's parts; 32,768 x 4,096 to e4m3 167-175 us (939 MB: 5.4-5.6 TB/s); 65,536 x 513 67 and 84 us (4.0 and 3.2 TB/s;
 // rows off the lines); 16 x 1,024 3.6 us, a launch.
 #include "pv_ops.h"
@@ -330,7 +330,7 @@ __global__ __launch_bounds__(END_WAVES* WAVE) void norm_weight_kernel(const floa
 }
 
 // f(Plan) for rows of D elements of type E: as few lanes as hold the row in one pack each, up to a wave, then more packs, then more
-// waves. The backward pass holds three tensors, the weights and their gradients' sums, so its lanes take half as many elements.
+// waves: 16 elements a lane at most backwards, where three tensors, the weights and their gradients' sums are held, 32 forwards.
 template <typename E, bool BACK, typename F> int32_t with_plan(int64_t D, F&& f) {
     constexpr int P = 16 / sizeof(E);
     const int64_t packs = (D + P - 1) / P;
@@ -339,14 +339,16 @@ template <typename E, bool BACK, typename F> int32_t with_plan(int64_t D, F&& f)
     if (packs <= 32) return f(Plan<32, 1, 8>{});
     if (packs <= 64) return f(Plan<64, 1, 4>{});
     if (packs <= 128) return f(Plan<64, 2, 4>{});
-    if constexpr (BACK) {
+    if constexpr (BACK && sizeof(E) == 2) {
         if (packs <= 256) return f(Plan<256, 1, 1>{});
         if (packs <= 512) return f(Plan<256, 2, 1>{});
+        if (packs <= 1024) return f(Plan<512, 2, 1>{});
         if (packs <= 2048) return f(Plan<1024, 2, 1>{});
     } else {
         if (packs <= 256) return f(Plan<64, 4, 4>{});
         if (packs <= 512) return f(Plan<256, 2, 1>{});
         if (packs <= 1024) return f(Plan<256, 4, 1>{});
+        if (packs <= 2048) return f(Plan<512, 4, 1>{});
         if (packs <= 4096) return f(Plan<1024, 4, 1>{});
     }
     return f(Plan<256, 0, 1>{});
