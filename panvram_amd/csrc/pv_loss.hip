@@ -14,8 +14,9 @@
 // workgroup a tile. Rows of more slabs than a workgroup has waves go through `place_kernel` (logits, d_logits stored) and
 // `grad_kernel` (the other two by columns), which reads hidden again.
 // The operand that a product needs transposed is made by a product with the identity, which is exact.
-//   Bf  hidden and weight in bfloat16: bfloat16 products, sums in 32 bits; d_logits as the sum of two bfloat16, 16 bits of it
-//   F3  all others: values in 32 bits, 32-bit products
+//   H2  hidden and weight alike in bfloat16 or float16: products of such numbers, sums in 32 bits; d_logits as the sum of two of
+//       them, 16 bits of it or more
+//   F3  weight in float32: values in 32 bits, 32-bit products
 //
 // What bounds it: the bytes where only losses are asked for (16 x 32,768 x 512 bfloat16 97-102 us, 537 MB: 5.3-5.5 TB/s). With
 // gradients each tile is a chain of three products, an exchange and a softmax, every wave doing the softmax again for itself; 16
@@ -36,8 +37,6 @@ constexpr int MOST_WAVES = 16;             // of a workgroup
 constexpr int END_WAVES = 16;
 
 using f32x4 = __attribute__((ext_vector_type(4))) float;
-using bf16x4 = __attribute__((ext_vector_type(4))) __bf16;
-using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using s16x4 = __attribute__((ext_vector_type(4))) short;
 
 struct Shape {
@@ -64,20 +63,47 @@ template <typename F> __device__ inline void over_slab(bool within, F&& f) {
     if (within) f(std::true_type{}); else f(std::false_type{});
 }
 
-// A slab of 128 columns in bfloat16
-template <typename E_> struct Bf {
+// x joined with the values of the lanes of the same c (l ^ 16, l ^ 32, l ^ 48)
+template <typename F> __device__ inline float over_groups(float x, F&& join) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = join(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return join(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
+// The products of 16-bit operands, with sums in 32 bits
+template <typename E> struct Half {
+    using x4 = __attribute__((ext_vector_type(4))) E;
+    using x8 = __attribute__((ext_vector_type(8))) E;
+    static __device__ f32x4 product(x4 a, x4 b, f32x4 c) {             // 16 x 16 x 16
+        if constexpr (std::is_same_v<E, bf16>) return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ f32x4 product(x8 a, x8 b, f32x4 c) {             // 16 x 16 x 32
+        if constexpr (std::is_same_v<E, bf16>) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+// A slab of 128 columns in bfloat16 or float16. The gradients of the logits go into products as the sum of two such numbers. In
+// float16, whose exponents are few, powers of two bring them near its largest number first: a place's own for d_hidden, and for
+// d_weight one for all that the wave has summed up, which grows (with the sums rescaled) when a tile needs it.
+template <typename E_> struct H2 {
     using E = E_;
-    using K = __bf16;                      // what the weights are laid out as
+    using K = E_;                          // what the weights are laid out as
+    using x4 = typename Half<E>::x4;
+    using x8 = typename Half<E>::x8;
+    static constexpr bool SCALED = std::is_same_v<E, f16>;
     static constexpr int COLS = 128, STEPS = 4, TILES = 8;
-    struct Rows { bf16x8 h[STEPS]; };      // column 32 q + 8 g + j of place c
-    struct Sums { f32x4 dw[TILES]; };      // id c, columns 32 q + 8 g + 4 t + r at 2 q + t
-    bf16x8 w[STEPS];                       // id c, columns as Rows
-    using Back = s16x4;
+    struct Rows { x8 h[STEPS]; };          // column 32 q + 8 g + j of place c
+    struct Sums { f32x4 dw[TILES]; int e; };                  // id c, columns 32 q + 8 g + 4 t + r at 2 q + t (SCALED: over 2^(e - 15))
+    x8 w[STEPS];                           // id c, columns as Rows
+    using Back = x4;
     const Back* wt;                        // [TILES][lanes], in LDS: column 32 q + 8 (c / 4) + 4 t + c % 4 at 2 q + t, ids 4 g + j
 
     __device__ void weights(const K* wr, int64_t Dp, int64_t c0) {
 #pragma unroll
-        for (int q = 0; q < STEPS; q++) w[q] = *reinterpret_cast<const bf16x8*>(wr + lane_c() * Dp + c0 + 32 * q + 8 * lane_g());
+        for (int q = 0; q < STEPS; q++) w[q] = *reinterpret_cast<const x8*>(wr + lane_c() * Dp + c0 + 32 * q + 8 * lane_g());
     }
     // (to: the wave's own room, so no other wave waits for it)
     __device__ void weights_back(const K* wc, int64_t c0, Back* to) {
@@ -104,41 +130,73 @@ template <typename E_> struct Bf {
 #pragma unroll
         for (int q = 0; q < STEPS; q++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) R.h[q][j] = __bf16(0.0f);
+            for (int j = 0; j < 8; j++) R.h[q][j] = E(0.0f);
     }
     __device__ f32x4 logits(const Rows& R, f32x4 l) const {
 #pragma unroll
-        for (int q = 0; q < STEPS; q++) l = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[q], R.h[q], l, 0, 0, 0);
+        for (int q = 0; q < STEPS; q++) l = Half<E>::product(w[q], R.h[q], l);
         return l;
     }
-    static __device__ s16x4 bits(f32x4 x) {
-        const bf16x4 b = __builtin_convertvector(x, bf16x4);
-        return __builtin_bit_cast(s16x4, b);
+    static __device__ x4 rounded(f32x4 x) { return __builtin_convertvector(x, x4); }
+    static __device__ void parts(f32x4 dl, x4& hi, x4& lo) {
+        hi = rounded(dl);
+        lo = rounded(dl - __builtin_convertvector(hi, f32x4));
     }
-    static __device__ f32x4 product(s16x4 a, s16x4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0); }
+    static __device__ f32x4 times(f32x4 x, int e) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) x[r] = ldexpf(x[r], e);
+        return x;
+    }
     // dl: d_logits of place c, ids 4 g + j
     __device__ void back(const Rows& R, f32x4 dl, E* d_row, int64_t c0, int64_t D, bool store, Sums& S) const {
         const int c = lane_c(), g = lane_g();
         const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
-        const s16x4 hi = bits(dl);
-        const s16x4 lo = bits(dl - __builtin_convertvector(__builtin_bit_cast(bf16x4, hi), f32x4));
-        s16x4 one;                         // the identity, 16 x 16
+        x4 one;                            // the identity, 16 x 16
 #pragma unroll
-        for (int j = 0; j < 4; j++) one[j] = c == 4 * g + j ? 0x3f80 : 0;
-        const s16x4 thi = bits(product(hi, one, none)), tlo = bits(product(lo, one, none));      // id c, places 4 g + j
+        for (int j = 0; j < 4; j++) one[j] = E(c == 4 * g + j ? 1.0f : 0.0f);
+        int e = 0;
+        x4 hi, lo, thi, tlo;               // thi, tlo: id c, places 4 g + j
+        if constexpr (SCALED) {
+            float most = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) most = fabsf(dl[j]) < INFINITY ? fmaxf(most, fabsf(dl[j])) : most;
+            most = over_groups(most, [](float a, float b) { return fmaxf(a, b); });
+            e = int(__float_as_uint(fmaxf(most, 0x1p-100f)) >> 23) - 126;
+            int all = e;
+#pragma unroll
+            for (int d = 1; d < TILE; d *= 2) all = max(all, __shfl_xor(all, d, WAVE));
+            all = __builtin_amdgcn_readfirstlane(all);
+            if (all > S.e) {
+#pragma unroll
+                for (int k = 0; k < TILES; k++) S.dw[k] = times(S.dw[k], S.e - all);
+                S.e = all;
+            }
+            parts(times(dl, 15 - S.e), hi, lo);
+            thi = rounded(Half<E>::product(hi, one, none));
+            tlo = rounded(Half<E>::product(lo, one, none));
+            parts(times(dl, 15 - e), hi, lo);
+            e -= 15;
+        } else {
+            parts(dl, hi, lo);
+            thi = rounded(Half<E>::product(hi, one, none));
+            tlo = rounded(Half<E>::product(lo, one, none));
+        }
         const bool whole = c0 + COLS <= D;
         d_row += c0 + 8 * g;
 #pragma unroll
         for (int q = 0; q < STEPS; q++) {
-            bf16x4 o[2];
+            x4 o[2];
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                bf16x4 h;                  // column 32 q + 8 g + 4 t + j of place c; turned: column 32 q + 8 (c / 4) + 4 t + c % 4, places 4 g + j
+                x4 h;                      // column 32 q + 8 g + 4 t + j of place c; turned: column 32 q + 8 (c / 4) + 4 t + c % 4, places 4 g + j
 #pragma unroll
                 for (int j = 0; j < 4; j++) h[j] = R.h[q][4 * t + j];
-                const s16x4 ht = bits(product(__builtin_bit_cast(s16x4, h), one, none));
-                S.dw[2 * q + t] = product(ht, tlo, product(ht, thi, S.dw[2 * q + t]));
-                o[t] = __builtin_convertvector(product(wt[(2 * q + t) * WAVE], lo, product(wt[(2 * q + t) * WAVE], hi, none)), bf16x4);
+                const x4 ht = rounded(Half<E>::product(h, one, none)), back = wt[(2 * q + t) * WAVE];
+                f32x4& dw = S.dw[2 * q + t];
+                dw = Half<E>::product(ht, tlo, Half<E>::product(ht, thi, dw));
+                f32x4 x = Half<E>::product(back, lo, Half<E>::product(back, hi, none));
+                if constexpr (SCALED) x = times(x, e);
+                o[t] = rounded(x);
             }
             if (store) {
                 pack<E, 8> p;
@@ -148,6 +206,8 @@ template <typename E_> struct Bf {
             }
         }
     }
+    static __device__ void begin(Sums& S) { S = {}; S.e = -99; }
+    static __device__ f32x4 end(const Sums& S, int k) { return SCALED ? times(S.dw[k], S.e - 15) : S.dw[k]; }
     // where the columns of result k's rows 4 g + r begin
     static __device__ int column(int k) { return 32 * (k / 2) + 8 * lane_g() + 4 * (k % 2); }
 };
@@ -224,6 +284,8 @@ template <typename E_> struct F3 {
             }
         }
     }
+    static __device__ void begin(Sums& S) { S = {}; }
+    static __device__ f32x4 end(const Sums& S, int k) { return S.dw[k]; }
     static __device__ int column(int k) { return 16 * k + 4 * lane_g(); }
 };
 
@@ -255,13 +317,6 @@ __device__ inline float mean_factor(const int64_t* counts, const float* scale) {
     return (scale ? *scale : 1.0f) / float(k > 0 ? k : 1);
 }
 
-// x joined with the values of the lanes of the same c (l ^ 16, l ^ 32, l ^ 48)
-template <typename F> __device__ inline float over_groups(float x, F&& join) {
-    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = join(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return join(__uint_as_float(a[0]), __uint_as_float(a[1]));
-}
 
 // Logits (place c, ids 4 g + r) made the gradients of the place's loss times `w` (0 where it does not count); the loss itself
 // where it is wanted (wave-uniform)
@@ -341,7 +396,8 @@ void fused_kernel(Shape S, const typename M::E* __restrict__ hidden, const void*
     M m;
     m.weights(wr, S.Dp, c0);
     if (GRADS) m.weights_back(wc, c0, reinterpret_cast<typename M::Back*>(lds + 2 * waves * WAVE) + wave * M::TILES * WAVE);
-    typename M::Sums sum = {};
+    typename M::Sums sum;
+    M::begin(sum);
     const float base = GRADS && counts ? mean_factor(counts, scale) : 0.0f;
     double loss = 0.0;
     int turn = 0;
@@ -378,7 +434,7 @@ void fused_kernel(Shape S, const typename M::E* __restrict__ hidden, const void*
     }
     if (GRADS && c < S.V) {
 #pragma unroll
-        for (int k = 0; k < M::TILES; k++) *reinterpret_cast<f32x4*>(parts + (int64_t(blockIdx.x) * S.V + c) * S.Dp + c0 + M::column(k)) = sum.dw[k];
+        for (int k = 0; k < M::TILES; k++) *reinterpret_cast<f32x4*>(parts + (int64_t(blockIdx.x) * S.V + c) * S.Dp + c0 + M::column(k)) = M::end(sum, k);
     }
 }
 
@@ -431,7 +487,8 @@ __global__ __launch_bounds__(BLOCK) void grad_kernel(Shape S, const typename M::
     M m;
     __shared__ typename M::Back room[BLOCK / WAVE][M::TILES * WAVE];
     m.weights_back(wc, c0, room[threadIdx.x / WAVE]);
-    typename M::Sums sum = {};
+    typename M::Sums sum;
+    M::begin(sum);
     const int64_t tiles = (S.N + TILE - 1) / TILE;
     for (int64_t tile = blockIdx.y; tile < tiles; tile += gridDim.y) {
         const int64_t n = tile * TILE + c;
@@ -445,7 +502,7 @@ __global__ __launch_bounds__(BLOCK) void grad_kernel(Shape S, const typename M::
     }
     if (c < S.V) {
 #pragma unroll
-        for (int k = 0; k < M::TILES; k++) *reinterpret_cast<f32x4*>(parts + (int64_t(blockIdx.y) * S.V + c) * S.Dp + c0 + M::column(k)) = sum.dw[k];
+        for (int k = 0; k < M::TILES; k++) *reinterpret_cast<f32x4*>(parts + (int64_t(blockIdx.y) * S.V + c) * S.Dp + c0 + M::column(k)) = M::end(sum, k);
     }
 }
 
@@ -571,13 +628,13 @@ int32_t pv_next_base_loss_hip(const void* hidden, const void* weight, const void
     if (!hidden || !weight || !tokens || !d_hidden != !d_weight) return fail(PV_EARG, err, errcap, "null argument");
     if (!work || work_bytes < pv_next_base_loss_work_bytes(B, T, D, V, d_hidden != nullptr)) return fail(PV_EARG, err, errcap, "work: too small");
     Shape S{B, T, D, B * T, hidden_b, hidden_t, tokens_b, ignore, 0, V, token_bytes, B == 1 || hidden_b == T * hidden_t};
-    const bool narrow = dtype == PV_BF16 && weight_dtype == PV_BF16;
+    const bool narrow = dtype != PV_F32 && weight_dtype == dtype;
     const hipStream_t st = hipStream_t(stream);
-    if (narrow) return run<Bf<bf16>, bf16>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, st, err, errcap);
+    if (narrow && dtype == PV_BF16) return run<H2<bf16>, bf16>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, st, err, errcap);
+    if (narrow) return run<H2<f16>, f16>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, st, err, errcap);
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
-        if (weight_dtype == PV_F32) return run<F3<E>, float>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, st, err, errcap);
-        return run<F3<E>, E>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, st, err, errcap);
+        return run<F3<E>, float>(S, hidden, weight, tokens, scale, factor, each, loss, d_hidden, d_weight, work, st, err, errcap);
     });
 }
 

@@ -92,6 +92,23 @@ def test_strided(D, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,V", [(60, 5), (512, 16), (2100, 4)])
+def test_factors_of_all_sizes(D, V, dtype):
+    """Gradients of the places' losses from 2^-40 to 2^12, rising and falling: none is lost beside a larger one, and sums that
+    began small go on as large ones."""
+    from panvram_amd import ops
+    hidden, weight, tokens = make(2, 900, D, V, dtype, seed=D)
+    tokens %= V
+    rising = torch.exp2(torch.linspace(-40, 12, 1800)).view(2, 900)
+    h, w = hidden.requires_grad_(), weight.requires_grad_()
+    for factor in (rising, rising.flip(0, 1), torch.where(torch.arange(1800).view(2, 900) % 3 == 0, rising, 0)):
+        d = torch.autograd.grad(ops.next_base_loss(h, w, tokens, ignore=None, reduction="none"), (h, w), factor.cuda())
+        plain = P.loss(hidden.detach().cpu(), weight.detach().cpu(), tokens.cpu(), None, factor=factor)
+        for got, name in zip(d, ("d_hidden", "d_weight")):
+            P.inside(got, plain[name][0], plain[name][1] + P.rounded(plain[name][0], dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("D", [60, 512])
 def test_nothing_from_places_that_do_not_count(D, dtype):
     """NaN and infinities in hidden where no next token counts leave the loss and both gradients as they are."""
