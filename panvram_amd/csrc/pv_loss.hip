@@ -18,11 +18,12 @@
 //       them, 16 bits of it or more
 //   F3  weight in float32: values in 32 bits, 32-bit products
 //
-// What bounds it: the bytes where only losses are asked for (16 x 32,768 x 512 bfloat16 97-102 us, 537 MB: 5.3-5.5 TB/s). With
+// What bounds it: the bytes where only losses are asked for (16 x 32,768 x 512 bfloat16 95-98 us, 537 MB: 5.5-5.7 TB/s). With
 // gradients each tile is a chain of three products, an exchange and a softmax, every wave doing the softmax again for itself; 16
-// waves a CU overlap it with the loads and stores: 8 x 8,192 x 1,024 bfloat16 65-69 us (268 MB: 3.9-4.1 TB/s) and 11 us for the
+// waves a CU overlap it with the loads and stores: 8 x 8,192 x 1,024 bfloat16 65-67 us (268 MB: 4.0-4.1 TB/s) and 10 us for the
 // count before and the parts of d_weight after it. F3 is bound by its products' rate, an eighth of bfloat16's: the same in
-// float32 154 us (3.5 TB/s), in float16 132 us (2.0). 5 x 2,049 x 500 float32, two tiles a workgroup, 24 us and 7: latency.
+// float32 154 us (3.5 TB/s), float16 with weight in float32 132 us (2.0; all in float16 81 us with the launches beside it,
+// bfloat16 76). 5 x 2,049 x 500 float32, two tiles a workgroup, 24 us and 7: latency.
 #include "pv_ops.h"
 
 using namespace pvo;
