@@ -23,8 +23,10 @@
 // waves a CU overlap it with the loads and stores: 8 x 8,192 x 1,024 bfloat16 65-67 us (268 MB: 4.0-4.1 TB/s) and 10 us for the
 // count before and the parts of d_weight after it. F3 is bound by its products' rate, an eighth of bfloat16's: the same in
 // float32 154 us (3.5 TB/s), float16 with weight in float32 132 us (2.0; all in float16 81 us with the launches beside it,
-// bfloat16 76). 5 x 2,049 x 500 float32, two tiles a workgroup, 24 us and 7: latency.
+// bfloat16 76). 5 x 2,049 x 500 float32, one or two tiles a workgroup, 20 us and 8: latency.
 #include "pv_ops.h"
+
+#include <algorithm>
 
 using namespace pvo;
 
@@ -549,7 +551,12 @@ Cut cut_of(int64_t N, int64_t D, bool narrow, bool gradients) {
     k.waves = slabs <= MOST_WAVES ? int(slabs) : 0;
     const int64_t most = k.waves ? 256 * ((gradients ? 16 : 24) / k.waves) : 256;      // of 256 CUs, 16 or 24 waves a CU
     const int64_t rounds = (tiles + most - 1) / most;                          // all workgroups have as many tiles, one less here and there
-    k.groups = int((tiles + rounds - 1) / rounds);
+    int64_t groups = (tiles + rounds - 1) / rounds;
+    // With gradients and several workgroups a CU: as many on each CU (5 x 2,049 x 500 float32 as 321 workgroups 24.5 us, as 512
+    // 20.3; 33,600 x 512 57.7 and 53.5). With one a CU or without gradients more would cost: 25,000 x 1,000 float32 as 224
+    // 76.2 us, as 256 77.8; losses of 131,072 x 128 bfloat16 34 and 42.
+    if (gradients && most > 256) groups = std::min({(groups + 255) / 256 * 256, most, tiles});
+    k.groups = int(groups);
     return k;
 }
 constexpr int PLACE_GROUPS = 2048;
