@@ -14,8 +14,8 @@
 // workgroup a tile. Rows of more slabs than a workgroup has waves go through `place_kernel` (logits, d_logits stored) and
 // `grad_kernel` (the other two by columns), which reads hidden again.
 // The operand that a product needs transposed is made by a product with the identity, which is exact.
-//   H2  hidden and weight alike in bfloat16 or float16: products of such numbers, sums in 32 bits; d_logits as the sum of two of
-//       them, 16 bits of it or more
+//   H2  hidden and weight alike in bfloat16 or float16: products of such numbers, sums in 32 bits; d_logits as the sum of three of
+//       them, which is all of its 24 bits
 //   F3  weight in float32: values in 32 bits, 32-bit products
 //
 // What bounds it: the bytes where only losses are asked for (16 x 32,768 x 512 bfloat16 95-98 us, 537 MB: 5.5-5.7 TB/s). With
@@ -88,7 +88,7 @@ template <typename E> struct Half {
     }
 };
 
-// A slab of 128 columns in bfloat16 or float16. The gradients of the logits go into products as the sum of two such numbers. In
+// A slab of 128 columns in bfloat16 or float16. The gradients of the logits go into products as the sum of three such numbers. In
 // float16, whose exponents are few, powers of two bring them near its largest number first: a place's own for d_hidden, and for
 // d_weight one for all that the wave has summed up, which grows (with the sums rescaled) when a tile needs it.
 template <typename E_> struct H2 {
@@ -141,10 +141,32 @@ template <typename E_> struct H2 {
         return l;
     }
     static __device__ x4 rounded(f32x4 x) { return __builtin_convertvector(x, x4); }
-    static __device__ void parts(f32x4 dl, x4& hi, x4& lo) {
-        hi = rounded(dl);
-        lo = rounded(dl - __builtin_convertvector(hi, f32x4));
-    }
+    // A right operand as the sum of its parts, a product of 16 each, the smallest first. (The sum goes through products of one
+    // shape: a 16 x 16 x 16 product's sum taken up by a 16 x 16 x 32 one right behind it lost rows, the compiler leaving no wait.)
+    struct Parts {
+        x4 part[3];
+        static __device__ Parts of(f32x4 x) {
+            Parts p;
+#pragma unroll
+            for (int k = 0; k < 3; k++) {
+                p.part[k] = rounded(x);
+                x -= __builtin_convertvector(p.part[k], f32x4);
+            }
+            return p;
+        }
+        // by the identity: rows to columns
+        __device__ Parts turned(x4 one) const {
+            Parts p;
+#pragma unroll
+            for (int k = 0; k < 3; k++) p.part[k] = rounded(Half<E>::product(part[k], one, f32x4{0.0f, 0.0f, 0.0f, 0.0f}));
+            return p;
+        }
+        __device__ f32x4 product(x4 left, f32x4 c) const {
+#pragma unroll
+            for (int k = 2; k >= 0; k--) c = Half<E>::product(left, part[k], c);
+            return c;
+        }
+    };
     static __device__ f32x4 times(f32x4 x, int e) {
 #pragma unroll
         for (int r = 0; r < 4; r++) x[r] = ldexpf(x[r], e);
@@ -157,8 +179,7 @@ template <typename E_> struct H2 {
         x4 one;                            // the identity, 16 x 16
 #pragma unroll
         for (int j = 0; j < 4; j++) one[j] = E(c == 4 * g + j ? 1.0f : 0.0f);
-        int e = 0;
-        x4 hi, lo, thi, tlo;               // thi, tlo: id c, places 4 g + j
+        int e = 0;                         // d_hidden is made of 2^(15 - e) d_logits
         if constexpr (SCALED) {
             float most = 0.0f;
 #pragma unroll
@@ -174,39 +195,35 @@ template <typename E_> struct H2 {
                 for (int k = 0; k < TILES; k++) S.dw[k] = times(S.dw[k], S.e - all);
                 S.e = all;
             }
-            parts(times(dl, 15 - S.e), hi, lo);
-            thi = rounded(Half<E>::product(hi, one, none));
-            tlo = rounded(Half<E>::product(lo, one, none));
-            parts(times(dl, 15 - e), hi, lo);
-            e -= 15;
-        } else {
-            parts(dl, hi, lo);
-            thi = rounded(Half<E>::product(hi, one, none));
-            tlo = rounded(Half<E>::product(lo, one, none));
         }
+        const Parts p = Parts::of(SCALED ? times(dl, 15 - e) : dl);
         const bool whole = c0 + COLS <= D;
         d_row += c0 + 8 * g;
 #pragma unroll
         for (int q = 0; q < STEPS; q++) {
             x4 o[2];
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                x4 h;                      // column 32 q + 8 g + 4 t + j of place c; turned: column 32 q + 8 (c / 4) + 4 t + c % 4, places 4 g + j
-#pragma unroll
-                for (int j = 0; j < 4; j++) h[j] = R.h[q][4 * t + j];
-                const x4 ht = rounded(Half<E>::product(h, one, none)), back = wt[(2 * q + t) * WAVE];
-                f32x4& dw = S.dw[2 * q + t];
-                dw = Half<E>::product(ht, tlo, Half<E>::product(ht, thi, dw));
-                f32x4 x = Half<E>::product(back, lo, Half<E>::product(back, hi, none));
-                if constexpr (SCALED) x = times(x, e);
+            for (int t = 0; t < 2; t++) {  // (every lane's weights are operands, whether it stores or not)
+                f32x4 x = p.product(wt[(2 * q + t) * WAVE], none);
+                if constexpr (SCALED) x = times(x, e - 15);
                 o[t] = rounded(x);
             }
             if (store) {
-                pack<E, 8> p;
-                __builtin_memcpy(&p, o, 16);
-                if (whole) p.store(d_row + 32 * q);            // (past the caches, rows that are not whole lines take half as long again: 65,536 x 1,000 in 117 us instead of 78)
-                else put<E, 8>(p, d_row + 32 * q, D - c0 - 32 * q - 8 * g);
+                pack<E, 8> row;
+                __builtin_memcpy(&row, o, 16);
+                if (whole) row.store(d_row + 32 * q);          // (past the caches, rows that are not whole lines take half as long again: 65,536 x 1,000 in 117 us instead of 78)
+                else put<E, 8>(row, d_row + 32 * q, D - c0 - 32 * q - 8 * g);
             }
+        }
+        // Id c, places 4 g + j. (After d_hidden: with both operands' parts held at once registers were spilled, and 8 x 8,192 x 1,024
+        // took 80 us instead of 73 in bfloat16, 95 instead of 79 in float16.)
+        const Parts turned = (SCALED ? Parts::of(times(dl, 15 - S.e)) : p).turned(one);
+#pragma unroll
+        for (int k = 0; k < TILES; k++) {
+            x4 h;                          // column 32 q + 8 g + 4 t + j of place c; turned: column 32 q + 8 (c / 4) + 4 t + c % 4, places 4 g + j
+#pragma unroll
+            for (int j = 0; j < 4; j++) h[j] = R.h[k / 2][4 * (k % 2) + j];
+            S.dw[k] = turned.product(rounded(Half<E>::product(h, one, none)), S.dw[k]);
         }
     }
     static __device__ void begin(Sums& S) { S = {}; S.e = -99; }
