@@ -146,16 +146,17 @@ __global__ __launch_bounds__(L::BLOCK) void norm_kernel(const E* __restrict__ x,
         }
     }
     sum = row_sum<L>(sum, lds);
-    // squares that leave 32 bits, or vanish in them where eps does too: once more of m s. (Every lane of a workgroup goes the same
-    // way where the sum has a barrier in it: such a workgroup has one row.)
+    // squares that leave 32 bits, or vanish in them where eps does not cover them: once more of m s, m s being between 2^-53 and 2^48 in
+    // either case, whatever finite number s is. (Every lane of a workgroup goes the same way where the sum has a barrier in it: such
+    // a workgroup has one row.)
     float m = 1.0f;
-    if (sum == INFINITY || (sum < 0x1p-96f && eps < 0x1p-60f)) {
-        m = sum < 1.0f ? 0x1p48f : 0x1p-64f;
+    if (sum == INFINITY || (sum < 0x1p-96f && eps < 0x1p-66f)) {
+        m = sum < 1.0f ? 0x1p96f : 0x1p-96f;
         sum = 0.0f;
         each([&](const pk& h, int64_t) { square(h, m); });
         sum = row_sum<L>(sum, lds);
     }
-    const float r = rsqrtf(sum / float(D) + m * m * eps);
+    const float r = rsqrtf(sum / float(D) + m * (m * eps));
     if (rstd && on && lane == 0) rstd[n] = m * r;
     if (y) {
         each([&](const pk& h, int64_t i) {
@@ -189,7 +190,9 @@ __global__ __launch_bounds__(L::BLOCK) void norm_kernel(const E* __restrict__ x,
     if (r == 0.0f) most = NAN;             // an infinity in the row
     if (!on) return;
     if (lane == 0) scale[n] = most / Q::MOST * r;
-    if (most < 0x1p-100f) { m *= 0x1p64f; most *= 0x1p64f; rest *= 0x1p64f; }
+    const float n2 = most < 0x1p-100f ? 0x1p64f : 1.0f;    // (m n2 itself may be past 32 bits)
+    most *= n2;
+    rest *= n2;
     const float up = most == 0.0f ? 0.0f : Q::MOST / most;
     const float up_rest = most == 0.0f ? 0.0f : fmaf(-up, rest, fmaf(-up, most, Q::MOST)) / most;
     each([&](const pk& h, int64_t i) {
@@ -198,7 +201,7 @@ __global__ __launch_bounds__(L::BLOCK) void norm_kernel(const E* __restrict__ x,
 #pragma unroll
         for (int j = 0; j < P; j++) {
 #pragma clang fp contract(off)     // (y + ... as one operation would count y's own rounding twice)
-            const float a = m * float(h.v[j]), x = a * w.v[j], y = x * up;
+            const float a = m * float(h.v[j]) * n2, x = a * w.v[j], y = x * up;
             v[j] = y + fmaf(fmaf(a, w.v[j], -x), up, fmaf(x, up_rest, fmaf(x, up, -y)));
         }
         pack<typename Q::type, P> o;
