@@ -22,6 +22,7 @@ def _dense(t):
 
 _ptr, _numel, _whole, _gpu = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device
 _dtype = attrgetter("dtype")
+_written = torch.autograd.graph.increment_version        # autograd does not see the kernels' writes by itself
 
 
 class _List:
@@ -124,6 +125,7 @@ def clip_gradients(grads, max_norm, out=None):
     norm, src = _norm(g)
     dst = src if o is g else o.pointers()
     call(N.lib().pv_scale_gradients_hip, g.index, _at(src), _at(dst), _at(g.sizes), _at(g.types), len(grads), max_norm, norm.data_ptr())
+    _written(grads if out is None else out)
     for b, made in back:
         b.copy_(made)
     return norm
