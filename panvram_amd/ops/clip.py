@@ -60,14 +60,14 @@ def _at(a):
     return a.buffer_info()[0]
 
 
-def _norm(g):
-    """The norm, and what its kernels were given"""
+def _norm(g, src):
+    """The norm of g's tensors, which are at the addresses src"""
     norm = torch.empty((), dtype=torch.float32, device=g.tensors[0].device)
-    L, n, src = N.lib(), len(g.tensors), g.pointers()
+    L, n = N.lib(), len(g.tensors)
     size = L.pv_gradient_norm_work_bytes(_at(g.sizes), _at(g.types), n)
     work = torch.empty(size, dtype=torch.uint8, device=norm.device)
     call(L.pv_gradient_norm_hip, g.index, _at(src), _at(g.sizes), _at(g.types), n, norm.data_ptr(), work.data_ptr(), size)
-    return norm, src
+    return norm
 
 
 @torch.no_grad()
@@ -82,7 +82,7 @@ def gradient_norm(grads):
         for i, t in enumerate(grads):
             if not _dense(t):
                 g.replace(i, t.contiguous())
-    return _norm(g)[0]
+    return _norm(g, g.pointers())
 
 
 @torch.no_grad()
@@ -90,7 +90,7 @@ def clip_gradients(grads, max_norm, out=None):
     """Scales the tensors in `grads` (float32, bfloat16, float16, mixed as they come, on one GPU) by
     min(1, max_norm / (norm + 1e-6)), in place or into the tensors of `out`, and returns the norm before, as gradient_norm
     does. out: for each gradient a tensor of its type and size, for instance views of one flat buffer; the gradient itself,
-    or memory apart from all of them. Nothing is read back: the factor is made and used on the GPU. If the norm is not
+    or memory apart from all of them; no memory twice. Nothing is read back: the factor is made and used on the GPU. If the norm is not
     finite, neither are the scaled gradients."""
     grads = list(grads)
     max_norm = float(max_norm)
@@ -122,8 +122,13 @@ def clip_gradients(grads, max_norm, out=None):
             if not b.is_contiguous():
                 o.replace(i, torch.empty_like(a, memory_format=torch.contiguous_format))
                 back.append((b, o.made[-1]))
-    norm, src = _norm(g)
+    src = g.pointers()
     dst = src if o is g else o.pointers()
+    if len(set(dst)) < len(dst):
+        to = [p for p in dst if p]                  # (empty tensors have no address)
+        if len(set(to)) < len(to):
+            raise ValueError("clip_gradients: the same memory twice among the tensors to write")
+    norm = _norm(g, src)
     call(N.lib().pv_scale_gradients_hip, g.index, _at(src), _at(dst), _at(g.sizes), _at(g.types), len(grads), max_norm, norm.data_ptr())
     _written(grads if out is None else out)
     for b, made in back:

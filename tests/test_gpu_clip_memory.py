@@ -1,6 +1,8 @@
-"""What clipping does to the memory it writes: autograd knows of it. Run with -m gpu."""
+"""What clipping does to the memory it writes: autograd knows of it, and no gradient is scaled twice. Run with -m gpu."""
 import pytest
 import torch
+
+from tests import ops_plain as P
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +44,19 @@ def test_inference_tensors():
         g = [torch.full((100,), 2.0, device="cuda")]
         norm = ops.clip_gradients(g, 1.0)
         assert abs(float(norm) - 20) <= 1e-5 and float((g[0] - 0.1).abs().max()) <= 1e-6
+
+
+def test_the_same_memory_twice_is_refused():
+    """Two workgroups would scale the same elements, some once and some twice."""
+    from panvram_amd import ops
+    g, h = torch.randn(100, device="cuda"), torch.randn(100, device="cuda")
+    keep = g.clone()
+    with pytest.raises(ValueError, match="twice"):
+        ops.clip_gradients([g, h, g], 1.0)
+    with pytest.raises(ValueError, match="twice"):
+        ops.clip_gradients([g, h], 1.0, out=[g, g])
+    assert torch.equal(g, keep)
+    empty = torch.zeros(0, device="cuda")
+    norm = ops.clip_gradients([empty, g, empty, g[:0]], 1e-3)
+    assert abs(float(norm) / float(keep.norm()) - 1) <= 1e-6
+    assert abs(float(ops.gradient_norm([keep, keep])) / float(keep.double().norm() * 2 ** 0.5) - 1) <= 4 * P.U
