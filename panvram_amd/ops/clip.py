@@ -90,8 +90,9 @@ def clip_gradients(grads, max_norm, out=None):
     """Scales the tensors in `grads` (float32, bfloat16, float16, mixed as they come, on one GPU) by
     min(1, max_norm / (norm + 1e-6)), in place or into the tensors of `out`, and returns the norm before, as gradient_norm
     does. out: for each gradient a tensor of its type and size, for instance views of one flat buffer; the gradient itself,
-    or memory apart from all of them; no memory twice. Nothing is read back: the factor is made and used on the GPU. If the norm is not
-    finite, neither are the scaled gradients."""
+    or memory apart from all of them; no memory twice. Nothing is read back: the factor is made and used on the GPU. A norm
+    of NaN makes NaN of all elements. An infinite one, of an infinite element or of a sum whose root float32 does not hold,
+    makes a factor of 0: NaN of infinite elements, 0 of finite ones. A loop that is to skip such steps asks the norm."""
     grads = list(grads)
     max_norm = float(max_norm)
     if not max_norm >= 0:

@@ -1,4 +1,5 @@
-"""What clipping does to the memory it writes: autograd knows of it, and no gradient is scaled twice. Run with -m gpu."""
+"""What clipping does to the memory it writes: autograd knows of it, no gradient is scaled twice, and what an infinite or
+undefined norm leaves of each element. Run with -m gpu."""
 import pytest
 import torch
 
@@ -60,3 +61,25 @@ def test_the_same_memory_twice_is_refused():
     norm = ops.clip_gradients([empty, g, empty, g[:0]], 1e-3)
     assert abs(float(norm) / float(keep.norm()) - 1) <= 1e-6
     assert abs(float(ops.gradient_norm([keep, keep])) / float(keep.double().norm() * 2 ** 0.5) - 1) <= 4 * P.U
+
+
+def test_infinite_norms():
+    """factor = min(1, max_norm / (norm + 1e-6)) throughout: an infinite norm makes 0 of finite elements and NaN of infinite
+    ones, a norm of NaN makes NaN of all; a sum of squares whose root 32 bits do not hold is an infinite norm."""
+    from panvram_amd import ops
+    for apart in (False, True):
+        for bad in (float("nan"), float("inf"), -float("inf"), 3e38):
+            grads = [torch.randn(100, device="cuda"), torch.randn(5000, device="cuda")]
+            grads[1][4321] = bad
+            if bad == 3e38:
+                grads[0][7] = bad
+            out = [torch.zeros_like(g) for g in grads] if apart else None
+            norm = ops.clip_gradients(grads, 1.0, out=out)
+            got = torch.cat(out or grads)
+            if bad != bad:
+                assert torch.isnan(norm) and torch.isnan(got).all()
+            else:
+                assert float(norm) == float("inf")
+                at = torch.zeros(5100, dtype=torch.bool, device="cuda")
+                at[4421] = bad != 3e38
+                assert torch.equal(torch.isnan(got), at) and not got[~at].any()
