@@ -7,9 +7,10 @@
     next_base_loss_grad(hidden, weight, tokens)      the loss and its gradients in one pass
     gradient_norm(grads), clip_gradients(grads, m)   the norm over many tensors, and the tensors scaled to at most m
 
-The first four take part in autograd. Every call runs on the current stream of its tensors' device, waits for nothing,
-and may be captured into a graph; what it returns and the scratch memory it uses come from torch's allocator. Types:
-float32, bfloat16, float16; sums, norms and states are kept in 32 bits or more. The reference has no counterpart (its
+gated_scan, add_rms_norm and next_base_loss take part in autograd, backwards; forward-mode derivatives are refused. Every
+call runs on the current stream of its tensors' device, waits for nothing, and may be captured into a graph; what it
+returns and the scratch memory it uses come from torch's allocator. Types: float32, bfloat16, float16; sums, norms and
+states are kept in 32 bits or more. The reference has no counterpart (its
 examples/train_small.py trains a stock torch model on the same windows)."""
 from .clip import clip_gradients, gradient_norm
 from .loss import next_base_loss, next_base_loss_grad

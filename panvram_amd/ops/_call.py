@@ -4,6 +4,7 @@ raised."""
 import threading
 
 import torch
+from torch.autograd import forward_ad as _fw
 from torch.autograd.function import once_differentiable
 
 from .. import _native as N
@@ -12,8 +13,20 @@ from .._streams import raw as _raw
 DTYPES = {torch.float32: N.F32, torch.bfloat16: N.BF16, torch.float16: N.F16}
 
 
+def no_tangents(name, tensors):
+    """An error if one of `tensors` carries a forward-mode derivative: the kernels would drop it without a word. (Asked for
+    each tensor only while a level of dual numbers is open, of which torch keeps the number.)"""
+    if getattr(_fw, "_current_level", 0) < 0:
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and _fw.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} has no forward-mode derivative")
+
+
 def on_gpu(name, first, *others):
-    """The index of the GPU that all tensors (None: left out) are on; an error naming what is not there."""
+    """The index of the GPU that all tensors (None: left out) are on; an error naming what is not there, and for forward-mode
+    derivatives."""
+    no_tangents(name, (first, *others))
     index = first.get_device() if isinstance(first, torch.Tensor) else -1
     for t in others:
         if t is not None and (index < 0 or not isinstance(t, torch.Tensor) or t.get_device() != index):

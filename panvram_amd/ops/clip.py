@@ -5,7 +5,7 @@ from operator import attrgetter
 import torch
 
 from .. import _native as N
-from ._call import DTYPES, call, on_gpu
+from ._call import DTYPES, call, no_tangents, on_gpu
 
 
 def _dense(t):
@@ -33,6 +33,7 @@ class _List:
         self.tensors, self.name = tensors, name
         if not all(issubclass(c, torch.Tensor) for c in set(map(type, tensors))):
             raise TypeError(f"{name}: tensors expected")
+        no_tangents(name, tensors)
         where = set(map(_gpu, tensors))
         if len(where) != 1 or -1 in where:
             on_gpu(name, *tensors)
