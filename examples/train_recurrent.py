@@ -65,7 +65,8 @@ def train(cohort, model, steps, rows=16, window=2048, rate=2e-3, seed=0, tell=No
     for k in range(steps):
         tokens, reset = batch(cohort, rows, window, generator)
         hidden, _ = model(tokens, reset=reset)
-        loss = ops.next_base_loss(hidden, model.head, tokens)
+        # a row for each window, so that no window's last place predicts another one's first base
+        loss = ops.next_base_loss(hidden.view(2 * rows, window, -1), model.head, tokens.view(2 * rows, window))
         optimizer.zero_grad(set_to_none=True)
         loss.backward()
         norm = ops.clip_gradients([p.grad for p in model.parameters()], 1.0)

@@ -60,8 +60,9 @@ def next_base_loss(hidden, weight, tokens, ignore=4, reduction="mean"):
     hidden: [B, T, D], float32, bfloat16 or float16. weight: [V, D] with V up to 16, in hidden's type or float32. tokens:
     uint8 or int64 [B, T] as Cohort.sample returns them; hidden[:, t] predicts tokens[:, t + 1]. Places whose next token is
     `ignore` (4: every byte other than A, C, G, T; None: no such id) or no id of [0, V) do not count, nor does the last of
-    a row. reduction: "mean" over the places that count (0 where there are none), or "none": float32 [B, T] with 0 at places
-    that do not count. Gradients flow to hidden and weight; what stands in hidden where nothing counts reaches neither."""
+    a row: windows packed in a row go in as rows of their own (a view where they are of one length), or else the last place of
+    each predicts the next one's first token. reduction: "mean" over the places that count (0 where there are none), or
+    "none": float32 [B, T] with 0 at places that do not count. Gradients flow to hidden and weight; what stands in hidden where nothing counts reaches neither."""
     hidden, weight, tokens, ignore = _checked("next_base_loss", hidden, weight, tokens, ignore)
     if reduction not in ("mean", "none"):
         raise ValueError(f'next_base_loss: reduction is "mean" or "none", got {reduction!r}')
