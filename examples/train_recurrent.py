@@ -109,7 +109,7 @@ def main():
     train(cohort, model, a.steps, a.rows, a.window, tell=print)
     generator = torch.Generator(device=cohort.device).manual_seed(1)
     prompt = cohort.sample(4, a.window, generator=generator, tokens=True)
-    print(f"held-out windows: {float(score(model, prompt).mean()):.4f} bits a base")
+    print(f"other windows of the cohort it was trained on: {float(score(model, prompt).mean()):.4f} bits a base")
     for row in generate(model, prompt, 60, generator).tolist():
         print("".join(BASES[b] for b in row))
 
