@@ -370,7 +370,9 @@ enum pv_dtype { PV_F32 = 0, PV_BF16 = 1, PV_F16 = 2 };
 enum pv_format8 { PV_E4M3 = 0, PV_INT8 = 1 };
 
 /* h[b, t, d] = (1 - z) h[b, t-1, d] + z value[b, t, d], z = sigmoid(gate[b, t, d]), T >= 1. gate, value: [B, T, D] of `dtype`
- * with strides (gate_b, gate_t), (value_b, value_t), a step's at most 2^26 bytes. state: f32[B, D] before step 0, or NULL: zero. reset: u8[B, T], or NULL;
+ * with strides (gate_b, gate_t), (value_b, value_t), a step's at most 2^26 bytes. B T D is 2^40 at most; of B sequences' chunks
+ * (256 steps forwards, 128 backwards, of 128 channels in 16 bits, 64 in 32) there are fewer than 2^23, and where T is 32 or 16 steps
+ * at most fewer than 2^26. state: f32[B, D] before step 0, or NULL: zero. reset: u8[B, T], or NULL;
  * where not 0, h[b, t-1] is dropped. out: [B, T, D] of `dtype`; last: f32[B, D] = h[b, T-1]. carry: NULL, or
  * f32[B, pv_gated_scan_spans(T), D] that the backward pass takes. */
 int64_t pv_gated_scan_spans(int64_t T);

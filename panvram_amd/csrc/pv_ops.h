@@ -54,6 +54,9 @@ __device__ inline float wave_sum(float x) {
     return x;
 }
 
+// A launch's work items: HIP takes fewer than 2^32
+constexpr int64_t MOST_ITEMS = int64_t(1) << 32;
+
 inline int32_t fail(int32_t code, char* err, size_t cap, const char* m) {
     if (err && cap) snprintf(err, cap, "%s", m);
     return code;

@@ -472,13 +472,18 @@ int64_t words_of(int64_t B, int64_t chunks, int64_t D) {
     return n;
 }
 
+// Channels of a lane, and tiles of D by waves of that many
+int vec_of(int64_t D, int32_t dtype) { return element_bytes(dtype) == 2 && D > 1 ? 2 : 1; }
+int64_t tiles_of(int64_t D, int vec) { return (D + WAVE * vec - 1) / (WAVE * vec); }
+
 // What both entries ask of their arguments
-template <typename... I> int32_t check(int64_t B, int64_t T, int64_t D, int32_t dtype, const void* work, uint64_t work_bytes, char* err, size_t cap, I... steps) {
+template <int STEPS, typename... I> int32_t check(int64_t B, int64_t T, int64_t D, int32_t dtype, const void* work, uint64_t work_bytes, char* err, size_t cap, I... steps) {
     if (!element_bytes(dtype)) return fail(PV_EARG, err, cap, "dtype: one of PV_F32, PV_BF16, PV_F16");
     if (B < 0 || T < 1 || D < 0) return fail(PV_EARG, err, cap, "shape: B >= 0, T >= 1, D >= 0");
     const int64_t most = int64_t(1) << 40;
     if (B > INT32_MAX || T > INT32_MAX || D > INT32_MAX || (B && D && (B * D > most || T > most / (B * D)))) return fail(PV_EARG, err, cap, "shape: B T D of 2^40 at most");
-    if (B && D && B * chunks_of(T, STEPS_BACK) * ((D + WAVE - 1) / WAVE) > INT32_MAX) return fail(PV_EARG, err, cap, "shape: too many chunks");
+    const int64_t groups = B * chunks_of(T, STEPS) * tiles_of(D, vec_of(D, dtype)), items = (T <= STEPS ? 1 : CHUNK_WAVES) * WAVE;
+    if (groups >= MOST_ITEMS / items) return fail(PV_EARG, err, cap, "shape: too many chunks for a launch's work items");
     for (int64_t st : {steps...}) if (T > 1 && (st < 0 || st * element_bytes(dtype) > MOST_STRIDE)) return fail(PV_EARG, err, cap, "stride: a step's is 0 to 2^26 bytes");
     const uint64_t need = pv_gated_scan_work_bytes(B, T, D);
     if (need && (!work || work_bytes < need || !aligned(work, 16))) return fail(PV_EARG, err, cap, "work: too small, or not 16-byte aligned");
@@ -493,10 +498,9 @@ bool once_of(int64_t B, int64_t T, int64_t D, int bytes) { return D * bytes % 12
 
 // f(channels of a lane, steps of a wave, waves, one chunk only, resets, once) with the records cleared
 template <int STEPS, typename F> int32_t launch(Shape& S, bool pairs, bool resets, bool once, void* work, hipStream_t st, F&& f) {
-    const int vec = pairs ? 2 : 1;
     S.spans = spans_of(S.T);
     S.chunks = chunks_of(S.T, STEPS);
-    S.tiles = (S.D + WAVE * vec - 1) / (WAVE * vec);
+    S.tiles = tiles_of(S.D, pairs ? 2 : 1);
     Records R = {};
     if (const int64_t words = words_of(S.B, S.chunks, S.D)) {
         uint64_t* w = static_cast<uint64_t*>(work);
@@ -535,14 +539,14 @@ uint64_t pv_gated_scan_work_bytes(int64_t B, int64_t T, int64_t D) {
 int32_t pv_gated_scan_hip(const void* gate, const void* value, const float* state, const uint8_t* reset, int64_t B, int64_t T, int64_t D, int64_t gate_b,
                           int64_t gate_t, int64_t value_b, int64_t value_t, int32_t dtype, void* out, float* last, float* carry, void* work,
                           uint64_t work_bytes, void* stream, char* err, size_t errcap) {
-    if (int32_t e = check(B, T, D, dtype, work, work_bytes, err, errcap, gate_t, value_t, D)) return e;
+    if (int32_t e = check<STEPS_FORWARD>(B, T, D, dtype, work, work_bytes, err, errcap, gate_t, value_t, D)) return e;
     if (!B || !D) return PV_OK;
     if (!gate || !value || !out || !last) return fail(PV_EARG, err, errcap, "null argument");
     Shape S{B, T, D, gate_b, gate_t, value_b, value_t, 0, 0, 0, 0, 0};
     const hipStream_t st = hipStream_t(stream);
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
-        const bool pairs = sizeof(E) == 2 && D > 1;
+        const bool pairs = vec_of(D, dtype) == 2;
         return launch<STEPS_FORWARD>(S, pairs, reset, once_of(B, T, D, sizeof(E)), work, st, [&](auto vec, auto steps, auto waves, auto one, auto resets, auto once, const Records& R, uint32_t groups) {
             constexpr int V = decltype(vec)::value, N = decltype(steps)::value, W = decltype(waves)::value;
             constexpr bool ONE = decltype(one)::value, RESET = decltype(resets)::value, ONCE = decltype(once)::value && V * sizeof(E) == 4;
@@ -558,14 +562,14 @@ int32_t pv_gated_scan_backward_hip(const void* gate, const void* value, const fl
                                    int64_t gate_b, int64_t gate_t, int64_t value_b, int64_t value_t, const void* d_out, int64_t d_out_b, int64_t d_out_t,
                                    const float* d_last, int32_t dtype, void* d_gate, void* d_value, float* d_state, void* work, uint64_t work_bytes,
                                    void* stream, char* err, size_t errcap) {
-    if (int32_t e = check(B, T, D, dtype, work, work_bytes, err, errcap, gate_t, value_t, d_out_t, D)) return e;
+    if (int32_t e = check<STEPS_BACK>(B, T, D, dtype, work, work_bytes, err, errcap, gate_t, value_t, d_out_t, D)) return e;
     if (!B || !D) return PV_OK;
     if (!gate || !value || !carry || !d_out || !d_gate || !d_value) return fail(PV_EARG, err, errcap, "null argument");
     Shape S{B, T, D, gate_b, gate_t, value_b, value_t, d_out_b, d_out_t, 0, 0, 0};
     const hipStream_t st = hipStream_t(stream);
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
-        const bool pairs = sizeof(E) == 2 && D > 1;
+        const bool pairs = vec_of(D, dtype) == 2;
         return launch<STEPS_BACK>(S, pairs, reset, once_of(B, T, D, sizeof(E)), work, st, [&](auto vec, auto steps, auto waves, auto one, auto resets, auto once, const Records& R, uint32_t groups) {
             constexpr int V = decltype(vec)::value, N = decltype(steps)::value, W = decltype(waves)::value;
             constexpr bool ONE = decltype(one)::value, RESET = decltype(resets)::value, ONCE = decltype(once)::value && V * sizeof(E) == 4;
