@@ -315,12 +315,12 @@ __global__ __launch_bounds__(L::BLOCK) void norm_back_kernel(const E* __restrict
     }
 }
 
-// d_weight[i] = sum of the partial rows: 64 columns a workgroup, its 16 waves a run of rows each
+// d_weight[i] = sum of the partial rows, from column `first` on: 64 columns a workgroup, its 16 waves a run of rows each
 constexpr int END_WAVES = 16;
-__global__ __launch_bounds__(END_WAVES* WAVE) void norm_weight_kernel(const float* __restrict__ parts, int64_t rows, int64_t D, float* __restrict__ d_weight) {
+__global__ __launch_bounds__(END_WAVES* WAVE) void norm_weight_kernel(const float* __restrict__ parts, int64_t rows, int64_t D, int64_t first, float* __restrict__ d_weight) {
     __shared__ float lds[END_WAVES][WAVE];
     const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
-    const int64_t i = int64_t(blockIdx.x) * WAVE + lane;
+    const int64_t i = first + int64_t(blockIdx.x) * WAVE + lane;
     float sum = 0.0f;
     if (i < D) {
 #pragma unroll 8
@@ -384,9 +384,14 @@ int32_t forward(const void* x, const void* residual, const float* weight, int64_
         using E = decltype(e);
         return with_plan<E, false>(D, [&](auto plan) {
             using L = decltype(plan);
-            norm_kernel<E, Q, L><<<dim3((N + L::ROWS - 1) / L::ROWS), L::BLOCK, 0, hipStream_t(stream)>>>(
-                static_cast<const E*>(x), static_cast<const E*>(residual), weight, N, D, xs, rs, eps, static_cast<E*>(y), static_cast<E*>(stream_out), rstd,
-                static_cast<typename Q::type*>(q), scale);
+            constexpr int64_t MOST = (MOST_ITEMS - 1) / L::BLOCK * L::ROWS;    // rows of a launch
+            const auto from = [](auto* p, int64_t i) { return p ? p + i : nullptr; };
+            for (int64_t n = 0; n < N; n += MOST) {
+                const int64_t rows = std::min(N - n, MOST);
+                norm_kernel<E, Q, L><<<dim3((rows + L::ROWS - 1) / L::ROWS), L::BLOCK, 0, hipStream_t(stream)>>>(
+                    static_cast<const E*>(x) + n * xs, from(static_cast<const E*>(residual), n * rs), weight, rows, D, xs, rs, eps, from(static_cast<E*>(y), n * D),
+                    from(static_cast<E*>(stream_out), n * D), from(rstd, n), from(static_cast<typename Q::type*>(q), n * D), from(scale, n));
+            }
             return launched(err, errcap);
         });
     });
@@ -433,7 +438,9 @@ int32_t pv_add_rms_norm_backward_hip(const void* s, const float* rstd, const flo
             float* parts = g > 1 ? static_cast<float*>(work) : d_weight;       // (one workgroup's part is the sum)
             if (N) norm_back_kernel<E, L><<<dim3(g), L::BLOCK, 0, st>>>(static_cast<const E*>(s), rstd, weight, N, D, s_row, static_cast<const E*>(d_y),
                                                                         static_cast<const E*>(d_stream), static_cast<E*>(d), parts);
-            if (g != 1) norm_weight_kernel<<<dim3((D + WAVE - 1) / WAVE), END_WAVES * WAVE, 0, st>>>(parts, g, D, d_weight);
+            constexpr int64_t MOST = MOST_ITEMS / END_WAVES / 2;               // columns of a launch
+            for (int64_t i = 0; g != 1 && i < D; i += MOST)
+                norm_weight_kernel<<<dim3((std::min(D - i, MOST) + WAVE - 1) / WAVE), END_WAVES * WAVE, 0, st>>>(parts, g, D, i, d_weight);
             return launched(err, errcap);
         });
     });
