@@ -404,7 +404,7 @@ int32_t pv_add_rms_norm_backward_hip(const void* s, const float* rstd, const flo
                                      size_t errcap);
 
 /* Cross-entropy of the next token under softmax(hidden weight^T). hidden: [B, T, D] of `dtype`, strides (hidden_b, hidden_t);
- * weight: [V, D] of weight_dtype (`dtype` or PV_F32), V <= 16; tokens: [B, T], row stride tokens_b, u8 or i64 (token_bytes 1 or
+ * D <= 2^23. weight: [V, D] of weight_dtype (`dtype` or PV_F32), V <= 16; tokens: [B, T], row stride tokens_b, u8 or i64 (token_bytes 1 or
  * 8). Place (b, t) counts if tokens[b, t+1] is in [0, V) and not `ignore` (t = T-1 never does). each: NULL, or f32[B, T], the
  * places' losses (0 where they do not count); loss: NULL, or f32[1], their mean over the places that count (0 for none).
  * d_hidden ([B, T, D] of `dtype`) and d_weight ([V, D] of weight_dtype), both or neither: the gradients of scale * mean (scale:

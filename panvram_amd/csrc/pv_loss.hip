@@ -38,6 +38,9 @@ constexpr int COUNTS = 256;                // workgroups that count places
 constexpr int BLOCK = 256;
 constexpr int MOST_WAVES = 16;             // of a workgroup
 constexpr int END_WAVES = 16;
+// of a row: end_kernel has END_WAVES work items for each element of the head, and one workgroup more
+constexpr int64_t MOST_COLUMNS = 1 << 23;
+static_assert(MOST_COLUMNS * VMAX * END_WAVES + END_WAVES * 64 < MOST_ITEMS, "a launch's work items");
 
 using f32x4 = __attribute__((ext_vector_type(4))) float;
 using s16x4 = __attribute__((ext_vector_type(4))) short;
@@ -648,7 +651,7 @@ int32_t pv_next_base_loss_hip(const void* hidden, const void* weight, const void
     if (!element_bytes(dtype)) return fail(PV_EARG, err, errcap, "dtype: one of PV_F32, PV_BF16, PV_F16");
     if (weight_dtype != dtype && weight_dtype != PV_F32) return fail(PV_EARG, err, errcap, "weight_dtype: hidden's, or PV_F32");
     if (token_bytes != 1 && token_bytes != 8) return fail(PV_EARG, err, errcap, "token_bytes: 1 or 8");
-    if (B < 1 || T < 1 || D < 1 || B > (int64_t(1) << 40) / T) return fail(PV_EARG, err, errcap, "shape: B, T, D >= 1, B * T <= 2^40");
+    if (B < 1 || T < 1 || D < 1 || D > MOST_COLUMNS || B > (int64_t(1) << 40) / T) return fail(PV_EARG, err, errcap, "shape: B, T, D >= 1, D <= 2^23, B * T <= 2^40");
     if (V < 1 || V > VMAX) return fail(PV_EARG, err, errcap, "V: 1 to 16 ids");
     if (!hidden || !weight || !tokens || !d_hidden != !d_weight) return fail(PV_EARG, err, errcap, "null argument");
     if (!work || work_bytes < pv_next_base_loss_work_bytes(B, T, D, V, d_hidden != nullptr)) return fail(PV_EARG, err, errcap, "work: too small");

@@ -21,6 +21,12 @@ def test_scan_workgroups():
         assert "too many chunks" in fn(1 << 26, 1, 1)
 
 
+def test_loss_columns():
+    def loss(D):
+        return refused("pv_next_base_loss_hip", FAKE, FAKE, FAKE, 1, 2, D, 4, 2 * D, D, 2, 4, N.F32, N.F32, 1, None, None, None, FAKE, None, None, FAKE, 1 << 50)
+    assert "shape" in loss((1 << 23) + 1)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("count", [(1 << 29) + 7, (1 << 29)])
 def test_norm_of_many_rows(count):
