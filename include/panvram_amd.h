@@ -415,7 +415,8 @@ int32_t pv_next_base_loss_hip(const void* hidden, const void* weight, const void
                               const float* factor, float* each, float* loss, void* d_hidden, void* d_weight, void* work, uint64_t work_bytes, void* stream,
                               char* err, size_t errcap);
 
-/* norm (f32[1]) = sqrt(sum over `count` tensors of their squares). grads, sizes (elements), dtypes: host arrays. */
+/* norm (f32[1]) = sqrt(sum over `count` tensors of their squares). grads, sizes (elements; less than 2^38 bytes each), dtypes:
+ * host arrays. */
 uint64_t pv_gradient_norm_work_bytes(const int64_t* sizes, const int32_t* dtypes, int32_t count);
 int32_t pv_gradient_norm_hip(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int32_t count, float* norm, void* work, uint64_t work_bytes,
                              void* stream, char* err, size_t errcap);

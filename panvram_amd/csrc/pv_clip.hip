@@ -34,7 +34,8 @@ struct Group {
     __host__ __device__ int32_t dtype(int k) const { return high[k] & 3; }
 };
 static_assert(sizeof(Group) <= 4064, "a launch's arguments");
-constexpr int64_t MOST_SIZE = int64_t(1) << 38;
+// Workgroups of a launch, and bytes of a tensor, so that its pieces are one launch
+constexpr int64_t MOST_BLOCKS = MOST_ITEMS / BLOCK - 1, MOST_BYTES = MOST_BLOCKS * PIECE;
 
 // The tensor that workgroup `b` works on: the last that begins at or before it
 __device__ inline int tensor_of(const Group& G, uint32_t b) {
@@ -153,7 +154,8 @@ template <typename F> void groups(const void* const* from, void* const* to, cons
     for (int32_t k = 0; k < count; k++) {
         const int32_t i = back ? count - 1 - k : k;
         if (!n[i]) continue;
-        if (G.count == GROUP) {
+        const int64_t more = blocks_of(n[i], dtypes[i], piece);
+        if (G.count == GROUP || blocks + more > MOST_BLOCKS) {
             f(G, uint32_t(blocks));
             G.count = 0;
             blocks = 0;
@@ -163,7 +165,7 @@ template <typename F> void groups(const void* const* from, void* const* to, cons
         G.low[G.count] = uint32_t(n[i]);
         G.high[G.count] = uint8_t(n[i] >> 32 << 2 | dtypes[i]);
         G.first[G.count++] = uint32_t(blocks);
-        blocks += blocks_of(n[i], dtypes[i], piece);
+        blocks += more;
     }
     if (G.count) f(G, uint32_t(blocks));
 }
@@ -175,7 +177,8 @@ int32_t check(const void* const* grads, void* const* out, const int64_t* sizes, 
     for (int32_t i = 0; i < count; i++) {
         const int bytes = element_bytes(dtypes[i]);
         if (!bytes) return fail(PV_EARG, err, cap, "dtype: one of PV_F32, PV_BF16, PV_F16");
-        if (sizes[i] < 0 || sizes[i] >= MOST_SIZE || (all += sizes[i]) > (int64_t(1) << 40)) return fail(PV_EARG, err, cap, "size: 0 to 2^38 elements, 2^40 in all");
+        if (sizes[i] < 0 || sizes[i] > MOST_BYTES || sizes[i] * bytes > MOST_BYTES || (all += sizes[i]) > (int64_t(1) << 40))
+            return fail(PV_EARG, err, cap, "size: 0 elements to less than 2^38 bytes, 2^40 elements in all");
         if (sizes[i] && (!grads[i] || (out && !out[i]))) return fail(PV_EARG, err, cap, "null argument");
         if (sizes[i] && (!aligned(grads[i], bytes) || (out && !aligned(out[i], bytes)))) return fail(PV_EARG, err, cap, "address: not a multiple of the element's size");
     }

@@ -1,5 +1,7 @@
 """Sizes past what one launch takes (below 2^32 work items in a grid): refused by the C entries before any launch, or worked on
 in several."""
+import ctypes
+
 import pytest
 import torch
 
@@ -25,6 +27,13 @@ def test_loss_columns():
     def loss(D):
         return refused("pv_next_base_loss_hip", FAKE, FAKE, FAKE, 1, 2, D, 4, 2 * D, D, 2, 4, N.F32, N.F32, 1, None, None, None, FAKE, None, None, FAKE, 1 << 50)
     assert "shape" in loss((1 << 23) + 1)
+
+
+def test_clip_sizes():
+    vp, i64, i32 = ctypes.c_void_p * 1, ctypes.c_int64 * 1, ctypes.c_int32 * 1
+    for size, dtype in (((1 << 36), N.F32), ((1 << 37), N.BF16)):
+        assert "size" in refused("pv_gradient_norm_hip", vp(FAKE), i64(size), i32(dtype), 1, FAKE, FAKE, 1 << 40)
+        assert "size" in refused("pv_scale_gradients_hip", vp(FAKE), vp(FAKE), i64(size), i32(dtype), 1, 1.0, FAKE)
 
 
 @pytest.mark.gpu
