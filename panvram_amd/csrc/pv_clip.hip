@@ -202,7 +202,7 @@ int32_t pv_gradient_norm_hip(const void* const* grads, const int64_t* sizes, con
     if (!norm) return fail(PV_EARG, err, errcap, "null argument");
     if (int32_t e = check(grads, nullptr, sizes, dtypes, count, err, errcap)) return e;
     const uint64_t need = pv_gradient_norm_work_bytes(sizes, dtypes, count);
-    if (need && (!work || work_bytes < need)) return fail(PV_EARG, err, errcap, "work: too small");
+    if (need && (!work || work_bytes < need || !aligned(work, 16))) return fail(PV_EARG, err, errcap, "work: too small, or not 16-byte aligned");
     const hipStream_t st = hipStream_t(stream);
     double* parts = static_cast<double*>(work);
     int64_t done = 0;

@@ -654,7 +654,8 @@ int32_t pv_next_base_loss_hip(const void* hidden, const void* weight, const void
     if (B < 1 || T < 1 || D < 1 || D > MOST_COLUMNS || B > (int64_t(1) << 40) / T) return fail(PV_EARG, err, errcap, "shape: B, T, D >= 1, D <= 2^23, B * T <= 2^40");
     if (V < 1 || V > VMAX) return fail(PV_EARG, err, errcap, "V: 1 to 16 ids");
     if (!hidden || !weight || !tokens || !d_hidden != !d_weight) return fail(PV_EARG, err, errcap, "null argument");
-    if (!work || work_bytes < pv_next_base_loss_work_bytes(B, T, D, V, d_hidden != nullptr)) return fail(PV_EARG, err, errcap, "work: too small");
+    if (!work || work_bytes < pv_next_base_loss_work_bytes(B, T, D, V, d_hidden != nullptr) || !aligned(work, 16))
+        return fail(PV_EARG, err, errcap, "work: too small, or not 16-byte aligned");
     Shape S{B, T, D, B * T, hidden_b, hidden_t, tokens_b, ignore, 0, V, token_bytes, B == 1 || hidden_b == T * hidden_t};
     const bool narrow = dtype != PV_F32 && weight_dtype == dtype;
     const hipStream_t st = hipStream_t(stream);

@@ -428,7 +428,7 @@ int32_t pv_add_rms_norm_backward_hip(const void* s, const float* rstd, const flo
     if (int32_t e = check(N, D, dtype, err, errcap)) return e;
     if (!d_weight || (N && (!s || !rstd || !weight || !d_y || !d))) return fail(PV_EARG, err, errcap, "null argument");
     const uint64_t need = pv_add_rms_norm_work_bytes(N, D);
-    if (need && (!work || work_bytes < need)) return fail(PV_EARG, err, errcap, "work: too small");
+    if (need && (!work || work_bytes < need || !aligned(work, 16))) return fail(PV_EARG, err, errcap, "work: too small, or not 16-byte aligned");
     const hipStream_t st = hipStream_t(stream);
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
