@@ -34,6 +34,7 @@ constexpr float CUT = -1.0f;
 
 struct Shape {
     int64_t B, T, D, gb, gt, vb, vt, db, dt;   // strides in elements: gate, value, d_out (batch, time); channels are neighbours
+    int64_t ot;                                // of the outputs' steps: D
     int64_t spans, chunks, tiles;              // spans of SPAN and chunks of T, tiles of D
 };
 
@@ -339,7 +340,7 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
         for (int w = 0; w < P.wave; w++)
 #pragma unroll
             for (int v = 0; v < VEC; v++) h[v] = apply(maps.get(w, P.lane * VEC + v), h[v]);
-    const Rows<ONCE> to(out + P.b * S.T * S.D + P.d0, S.D, s, width);
+    const Rows<ONCE> to(out + P.b * S.T * S.D + P.d0, S.ot, s, width);
     over_steps<STEPS, RESET, false>(s, [&](int i, bool cut) {
         if (i % SPAN == 0 && carry && P.on && i < s.steps)
 #pragma unroll
@@ -438,7 +439,7 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(VEC
 #pragma unroll
             for (int v = 0; v < VEC; v++) C[v] = apply(maps.get(w, P.lane * VEC + v), C[v]);
     anew(Z);
-    const Rows<ONCE> to_gate(d_gate + P.b * S.T * S.D + P.d0, S.D, s, width), to_value(d_value + P.b * S.T * S.D + P.d0, S.D, s, width);
+    const Rows<ONCE> to_gate(d_gate + P.b * S.T * S.D + P.d0, S.ot, s, width), to_value(d_value + P.b * S.T * S.D + P.d0, S.ot, s, width);
     over_steps<STEPS, RESET, true>(s, [&](int i, bool cut) {
         float og[VEC], ov[VEC];
 #pragma unroll
@@ -498,6 +499,8 @@ bool once_of(int64_t B, int64_t T, int64_t D, int bytes) { return D * bytes % 12
 
 // f(channels of a lane, steps of a wave, waves, one chunk only, resets, once) with the records cleared
 template <int STEPS, typename F> int32_t launch(Shape& S, bool pairs, bool resets, bool once, void* work, hipStream_t st, F&& f) {
+    // A single step's row may be longer than 32 bits hold: the steps that are not there are put where each access is behind the row's end
+    if (S.T == 1) S.gt = S.vt = S.dt = S.ot = 2 * WAVE;
     S.spans = spans_of(S.T);
     S.chunks = chunks_of(S.T, STEPS);
     S.tiles = tiles_of(S.D, pairs ? 2 : 1);
@@ -542,7 +545,7 @@ int32_t pv_gated_scan_hip(const void* gate, const void* value, const float* stat
     if (int32_t e = check<STEPS_FORWARD>(B, T, D, dtype, work, work_bytes, err, errcap, gate_t, value_t, D)) return e;
     if (!B || !D) return PV_OK;
     if (!gate || !value || !out || !last) return fail(PV_EARG, err, errcap, "null argument");
-    Shape S{B, T, D, gate_b, gate_t, value_b, value_t, 0, 0, 0, 0, 0};
+    Shape S{B, T, D, gate_b, gate_t, value_b, value_t, 0, 0, D, 0, 0, 0};
     const hipStream_t st = hipStream_t(stream);
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
@@ -565,7 +568,7 @@ int32_t pv_gated_scan_backward_hip(const void* gate, const void* value, const fl
     if (int32_t e = check<STEPS_BACK>(B, T, D, dtype, work, work_bytes, err, errcap, gate_t, value_t, d_out_t, D)) return e;
     if (!B || !D) return PV_OK;
     if (!gate || !value || !carry || !d_out || !d_gate || !d_value) return fail(PV_EARG, err, errcap, "null argument");
-    Shape S{B, T, D, gate_b, gate_t, value_b, value_t, d_out_b, d_out_t, 0, 0, 0};
+    Shape S{B, T, D, gate_b, gate_t, value_b, value_t, d_out_b, d_out_t, D, 0, 0, 0};
     const hipStream_t st = hipStream_t(stream);
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
