@@ -253,8 +253,8 @@ template <int VEC, int WAVES> struct Before {
             if (!whole && l % TEAMS != team) continue;
             const Map m = before_at(R, S, b, l, n, p, d, on);
             if (l % TEAMS == team) {
-                A[l][0].v[c] = m.A;
-                H[l][0].v[c] = m.H;
+                A[l][c / VEC].v[c % VEC] = m.A;
+                H[l][c / VEC].v[c % VEC] = m.H;
             }
             whole = whole && p % FAN == FAN - 1 && l + 1 < LEVELS;
             if (whole) {
@@ -277,7 +277,7 @@ template <int VEC, int WAVES> struct Maps {
 #pragma unroll
         for (int v = 0; v < VEC; v++) { A[wave][lane].v[v] = m[v].A; H[wave][lane].v[v] = m[v].H; }
     }
-    __device__ Map get(int wave, int channel) const { return {A[wave][0].v[channel], H[wave][0].v[channel]}; }
+    __device__ Map get(int wave, int channel) const { return {A[wave][channel / VEC].v[channel % VEC], H[wave][channel / VEC].v[channel % VEC]}; }
 };
 
 template <typename E, int VEC, int STEPS, int WAVES, bool ONE, bool RESET, bool ONCE>
