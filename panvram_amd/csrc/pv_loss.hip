@@ -533,7 +533,7 @@ __global__ __launch_bounds__(BLOCK) void grad_kernel(Shape S, const typename M::
 template <typename W>
 __global__ __launch_bounds__(END_WAVES* WAVE) void end_kernel(Shape S, const int64_t* counts, const double* sums, int nsums, float* loss, const float* __restrict__ parts,
                                                               int nparts, W* __restrict__ d_weight) {
-    __shared__ double lds[END_WAVES][WAVE];
+    __shared__ float lds[END_WAVES][WAVE];
     const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
     if (loss && blockIdx.x == gridDim.x - 1) {
         if (wave) return;
@@ -552,12 +552,11 @@ __global__ __launch_bounds__(END_WAVES* WAVE) void end_kernel(Shape S, const int
 #pragma unroll 8
         for (int p = wave; p < nparts; p += END_WAVES) x += parts[p * size + e];
     }
-    float* part = reinterpret_cast<float*>(lds);
-    part[wave * WAVE + lane] = x;
+    lds[wave][lane] = x;
     __syncthreads();
     if (wave || e >= size) return;
 #pragma unroll
-    for (int w = 1; w < END_WAVES; w++) x += part[w * WAVE + lane];
+    for (int w = 1; w < END_WAVES; w++) x += lds[w][lane];
     const int64_t v = e / S.Dp, i = e % S.Dp;
     if (i < S.D) d_weight[v * S.D + i] = W(x);
 }
