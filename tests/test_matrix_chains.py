@@ -6,11 +6,16 @@ import subprocess
 
 import pytest
 
-from tests.test_wait_states import _regs, code_object
+from tests.test_wait_states import code_object
 
 MAGIC = b"__CLANG_OFFLOAD_BUNDLE__"
 
 NEAR = 16          # instructions that a result is followed for
+REG = re.compile(r"\b([av])(?:(\d+)\b|\[(\d+):(\d+)\])")
+
+
+def _regs(text):
+    return {f"{kind}{i}" for kind, one, lo, hi in REG.findall(text) for i in (range(int(lo), int(hi) + 1) if lo else (int(one),))}
 
 
 def mixed(lines):
@@ -56,6 +61,7 @@ def test_one_shape_a_sum(tmp_path):
 
 @pytest.mark.parametrize("code,n", [
     ("v_mfma_f32_16x16x16_bf16 v[18:21], v[122:123], v[110:111], 0\nv_mfma_f32_16x16x32_bf16 v[86:89], v[86:89], v[82:85], v[18:21]", 1),
+    ("v_mfma_f32_16x16x16_bf16 a[0:3], v[122:123], v[110:111], 0\nv_mfma_f32_16x16x32_bf16 v[86:89], v[86:89], v[82:85], a[0:3]", 1),
     ("v_mfma_f32_16x16x16_bf16 v[18:21], v[122:123], v[110:111], 0\nv_mfma_f32_16x16x16_bf16 v[86:89], v[86:87], v[82:83], v[18:21]", 0),
     ("v_mfma_f32_16x16x16_bf16 v[18:21], v[122:123], v[110:111], 0\nv_mfma_f32_16x16x32_bf16 v[86:89], v[86:89], v[82:85], v[22:25]", 0),
     ("v_mfma_f32_16x16x16_bf16 v[18:19], v[122:123], v[110:111], 0\nv_mov_b32_e32 v18, v2\nv_mov_b32_e32 v19, v2\nv_mfma_f32_16x16x32_bf16 v[86:89], v[86:89], v[82:85], v[18:19]", 0)])
