@@ -8,7 +8,7 @@
 // What bounds it: the bytes, read once for the norm and once more for the scaling where they are more than the caches hold.
 // Measured: 500 M bfloat16 elements in 300 tensors, squares 166 us (1.0 GB: 6.0 TB/s), scaling 328 us (2.0 GB: 6.1 TB/s; the last
 // tensors first, which the caches may still have). 2 M float32 elements in 150 tensors 17 us in three launches, where the host
-// needs 90 us for their addresses, sizes and types.
+// needs 95 us for their addresses, sizes, types and versions.
 #include "pv_ops.h"
 
 using namespace pvo;

@@ -18,12 +18,13 @@
 //       them, which is all of its 24 bits
 //   F3  weight in float32: values in 32 bits, 32-bit products
 //
-// What bounds it: the bytes where only losses are asked for (16 x 32,768 x 512 bfloat16 95-98 us, 537 MB: 5.5-5.7 TB/s). With
-// gradients each tile is a chain of three products, an exchange and a softmax, every wave doing the softmax again for itself; 16
-// waves a CU overlap it with the loads and stores: 8 x 8,192 x 1,024 bfloat16 65-67 us (268 MB: 4.0-4.1 TB/s) and 10 us for the
-// count before and the parts of d_weight after it. F3 is bound by its products' rate, an eighth of bfloat16's: the same in
-// float32 154 us (3.5 TB/s), float16 with weight in float32 132 us (2.0; all in float16 81 us with the launches beside it,
-// bfloat16 76). 5 x 2,049 x 500 float32, one or two tiles a workgroup, 20 us and 8: latency.
+// What bounds it: the bytes where only losses are asked for (16 x 32,768 x 512 bfloat16 95-97 us, 537 MB: 5.5-5.7 TB/s; float32
+// 195 us, 1.07 GB: 5.5; bfloat16 with weight in float32 191 us: 2.8, half of it the products). With gradients each tile is a chain
+// of three products, an exchange and a softmax, every wave doing the softmax again for itself; 16 waves a CU overlap it with the
+// loads and stores: 8 x 8,192 x 1,024 bfloat16 63-65 us (268 MB: 4.1-4.2 TB/s) and 10 us for the count before and the parts of
+// d_weight after it. F3 is the same chain with products at an eighth of bfloat16's rate, which by their count alone would be some
+// 58 us there: float32 152 us with the launches beside it (3.5 TB/s), bfloat16 with weight in float32 128 (2.1; all in float16 79,
+// bfloat16 73). 5 x 2,049 x 500 float32, one or two tiles a workgroup, 22 us and 8: latency.
 #include "pv_ops.h"
 
 #include <algorithm>
@@ -342,7 +343,8 @@ __device__ inline float mean_factor(const int64_t* counts, const float* scale) {
 
 
 // Logits (place c, ids 4 g + r) made the gradients of the place's loss times `w` (0 where it does not count); the loss itself
-// where it is wanted (wave-uniform)
+// where it is wanted (wave-uniform). The exponentials are off by some |l - top| 2^-24 of themselves, which is what the logits' own
+// rounding in 32 bits moves them by.
 __device__ inline float softmax(f32x4& l, int at, int V, float w, bool loss) {
     const int first = 4 * lane_g();
     const auto sum = [](float a, float b) { return a + b; };

@@ -10,10 +10,12 @@
 // pass, from the caches. Rows may begin at any element; a row's last pack may be a part of one. Sums in 32 bits.
 //
 // What bounds it: the bytes. x, residual, y and all of the backward pass's tensors are passed by the caches, so that the stream,
-// which the next layer and the backward pass read, stays in them (65,536 x 1,024 bfloat16 forwards and backwards 197 us with
-// this, 240 without; 3,487 x 4,127 float32, 58 MB a tensor, 49 and 70 us with it, 45 and 62 without). Measured: those forwards 80-84 us (537 MB: 6.4-6.7 TB/s), backwards 83-86 us (537 MB: 6.2-6.4) and 4 us
-// for the weight's parts; 32,768 x 4,096 to e4m3 167-175 us (939 MB: 5.4-5.6 TB/s); 65,536 x 513 67 and 84 us (4.0 and 3.2 TB/s;
-// rows off the lines); 16 x 1,024 3.6 us, a launch.
+// which the next layer and the backward pass read, stays in them (65,536 x 1,024 bfloat16 forwards 85 us with this, 98 without,
+// backwards 95 and 106; 13,826 x 4,839 float32 171 and 198, 218 and 227. It costs a little where a tensor is no larger than the
+// caches or rows are off the lines: 3,487 x 4,127 float32, 58 MB a tensor, 43.5 and 42 us forwards; 65,536 x 513 bfloat16 63 and 57,
+// 84 and 80). Measured: 65,536 x 1,024 forwards 80-84 us (537 MB: 6.4-6.7 TB/s), backwards 84-86 us (537 MB: 6.2-6.4) and 5 us for
+// the weight's parts; 32,768 x 4,096 to e4m3 168-170 us (939 MB: 5.5-5.6 TB/s), in single passes up to 197; to int8 178; 16 x 1,024
+// 3.7 us, a launch.
 #include "pv_ops.h"
 
 #include <algorithm>
@@ -146,9 +148,9 @@ __global__ __launch_bounds__(L::BLOCK) void norm_kernel(const E* __restrict__ x,
         }
     }
     sum = row_sum<L>(sum, lds);
-    // squares that leave 32 bits, or vanish in them where eps does not cover them: once more of m s, m s being between 2^-53 and 2^48 in
-    // either case, whatever finite number s is. (Every lane of a workgroup goes the same way where the sum has a barrier in it: such
-    // a workgroup has one row.)
+    // squares that leave 32 bits, or vanish in them where eps does not cover them: once more of m s, which has a square in 32 bits for
+    // the largest and for the smallest number of 32 bits alike. (Every lane of a workgroup goes the same way where the sum has a
+    // barrier in it: such a workgroup has one row.)
     float m = 1.0f;
     if (sum == INFINITY || (sum < 0x1p-96f && eps < 0x1p-66f)) {
         m = sum < 1.0f ? 0x1p96f : 0x1p-96f;

@@ -14,9 +14,9 @@
 // with a reset in it has A = CUT, which no product of (1 - z) can be.
 //
 // What bounds it: the bytes, three tensors forwards and five backwards. In bfloat16 the arithmetic is next (two transcendental
-// and some 25 other operations an element forwards, 40 backwards, at 24 and 16 waves a CU), and in long sequences the wait for
-// the maps of chunks that are still being loaded. Measured: 8 x 8,192 x 1,024 bfloat16 forwards 89-94 us (403 MB: 4.3-4.5 TB/s),
-// backwards 129-135 us (671 MB: 5.0-5.2); in float32 156 and 249 (5.2 and 5.4 TB/s); 1 x 2^20 x 512 bfloat16 forwards 621-632 us
+// and some 25 other operations an element forwards, 40 backwards, at 16 waves a CU), and in long sequences the wait for
+// the maps of chunks that are still being loaded. Measured: 8 x 8,192 x 1,024 bfloat16 forwards 88-91 us (403 MB: 4.4-4.6 TB/s),
+// backwards 128-133 us (671 MB: 5.0-5.2); in float32 152 and 250 (5.3 and 5.4 TB/s); 1 x 2^20 x 512 bfloat16 forwards 618-631 us
 // (5.1 TB/s); one step of 16 x 1,024 3.3 us, a launch.
 #include "pv_ops.h"
 

@@ -31,14 +31,11 @@ def test_narrow_rows(dtype):
     check(*make(3, 33_001, 24, 4, dtype, seed=2))
 
 
-@pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("T,D", [(30_011, 512), (14_007, 1024), (132_001, 1030), (131_501, 2051)])
+@pytest.mark.parametrize("T,D,dtype", [(t, d, k) for k in TYPES for t, d in ((30_011, 512), (14_007, 1024), (132_001, 1030) if k == torch.float32 else (131_501, 2051))])
 def test_scores(T, D, dtype):
     """Losses alone: 256 * (24 // waves) workgroups, or 2,048 of four tiles where the row has more than 16 slabs (1,030
     columns of 32 bits, 2,051 of 16). Compared at every 13th place and at the last ones."""
     from panvram_amd import ops
-    if T > 100_000 and (D < 2000) != (dtype == torch.float32):
-        pytest.skip("the other cut's size")
     hidden, weight, tokens = make(1, T, D, 5, dtype, seed=T)
     each = ops.next_base_loss(hidden, weight, tokens, reduction="none").cpu()
     at = torch.cat([torch.arange(0, T - 300, 13), torch.arange(T - 300, T - 1)])
