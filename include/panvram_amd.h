@@ -403,6 +403,28 @@ int32_t pv_add_rms_norm_backward_hip(const void* s, const float* rstd, const flo
                                      const void* d_stream, int32_t dtype, void* d, float* d_weight, void* work, uint64_t work_bytes, void* stream, char* err,
                                      size_t errcap);
 
+/* Dropout. Element i of a call is dropped where its 16 bits are below round(p 2^16), 0 <= p <= 1, and else multiplied by
+ * 2^16 / (2^16 - round(p 2^16)). The bits are word (i / 2) % 4, half i % 2 (the low one first) of the ten-round generator of four
+ * 32-bit words by Salmon, Moraes, Dror and Shaw (2011) with the seed as its key and counter (i / 8 in 64 bits, site, 0). The
+ * seed is *seed_at, read when the kernel runs, or with seed_at NULL the number `seed`. */
+/* y[i] = 0 or x[i] times that factor, n elements of `dtype`, neighbours each. The gradient is the same call on d_y. */
+int32_t pv_dropout_hip(const void* x, int64_t n, double p, const int64_t* seed_at, int64_t seed, uint32_t site, int32_t dtype, void* y, void* stream, char* err,
+                       size_t errcap);
+/* s = residual + dropout(x) (element n D + d; p 0: x itself), rounded to `dtype` (stream_out [N, D]; residual NULL: s = dropout(x),
+ * and with p 0 too s = x, stream_out is not written); y[n, :] = (s - mean) r weight + bias, r = 1 / sqrt(var + eps), mean and
+ * var over the row. x, residual: [N, D] of `dtype` with the given row strides; weight: f32[D]; bias: f32[D], or NULL: zero; y: [N, D]
+ * of `dtype`; stats: NULL, or f32[N, 3] that the backward pass takes. N, D < 2^31. */
+int32_t pv_add_layer_norm_hip(const void* x, const void* residual, const float* weight, const float* bias, int64_t N, int64_t D, int64_t x_row,
+                              int64_t residual_row, float eps, double p, const int64_t* seed_at, int64_t seed, uint32_t site, int32_t dtype, void* y, void* stream_out,
+                              float* stats, void* stream, char* err, size_t errcap);
+/* The gradients from d_y and d_stream (NULL: zero), both [N, D] of `dtype`, with s ([N, D], row stride s_row) and stats of the
+ * forward call, and its p, seed and site: d (of residual, [N, D] of `dtype`), d_x (likewise; with p 0 it is d, and not written),
+ * d_weight and d_bias (f32[D]). */
+uint64_t pv_add_layer_norm_work_bytes(int64_t N, int64_t D);
+int32_t pv_add_layer_norm_backward_hip(const void* s, const float* stats, const float* weight, int64_t N, int64_t D, int64_t s_row, const void* d_y,
+                                       const void* d_stream, double p, const int64_t* seed_at, int64_t seed, uint32_t site, int32_t dtype, void* d, void* d_x,
+                                       float* d_weight, float* d_bias, void* work, uint64_t work_bytes, void* stream, char* err, size_t errcap);
+
 /* Cross-entropy of the next token under softmax(hidden weight^T). hidden: [B, T, D] of `dtype`, strides (hidden_b, hidden_t);
  * D <= 2^23. weight: [V, D] of weight_dtype (`dtype` or PV_F32), V <= 16; tokens: [B, T], row stride tokens_b, u8 or i64 (token_bytes 1 or
  * 8). Place (b, t) counts if tokens[b, t+1] is in [0, V) and not `ignore` (t = T-1 never does). each: NULL, or f32[B, T], the

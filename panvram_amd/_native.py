@@ -24,7 +24,7 @@ E4M3, INT8 = 0, 1
 
 vp, i32, i64, u32, u64, cp, sz = (ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_uint32, ctypes.c_uint64,
                                   ctypes.c_char_p, ctypes.c_size_t)
-f32 = ctypes.c_float
+f32, f64 = ctypes.c_float, ctypes.c_double
 
 
 class FormatError(ValueError):
@@ -109,6 +109,10 @@ SIGNATURES = {
     "pv_add_rms_norm_8bit_hip": (i32, [vp, vp, vp, i64, i64, i64, i64, f32, i32, i32, vp, vp, vp, vp, cp, sz]),
     "pv_add_rms_norm_work_bytes": (u64, [i64, i64]),
     "pv_add_rms_norm_backward_hip": (i32, [vp, vp, vp, i64, i64, i64, vp, vp, i32, vp, vp, vp, u64, vp, cp, sz]),
+    "pv_dropout_hip": (i32, [vp, i64, f64, vp, i64, u32, i32, vp, vp, cp, sz]),
+    "pv_add_layer_norm_hip": (i32, [vp, vp, vp, vp, i64, i64, i64, i64, f32, f64, vp, i64, u32, i32, vp, vp, vp, vp, cp, sz]),
+    "pv_add_layer_norm_work_bytes": (u64, [i64, i64]),
+    "pv_add_layer_norm_backward_hip": (i32, [vp, vp, vp, i64, i64, i64, vp, vp, f64, vp, i64, u32, i32, vp, vp, vp, vp, vp, u64, vp, cp, sz]),
     "pv_next_base_loss_work_bytes": (u64, [i64, i64, i64, i32, i32]),
     "pv_next_base_loss_hip": (i32, [vp, vp, vp, i64, i64, i64, i32, i64, i64, i64, i64, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, u64, vp, cp, sz]),
     "pv_gradient_norm_work_bytes": (u64, [vp, vp, i32]),

@@ -16,15 +16,13 @@
 // 84 and 80). Measured: 65,536 x 1,024 forwards 80-84 us (537 MB: 6.4-6.7 TB/s), backwards 84-86 us (537 MB: 6.2-6.4) and 5 us for
 // the weight's parts; 32,768 x 4,096 to e4m3 168-170 us (939 MB: 5.5-5.6 TB/s), in single passes up to 197; to int8 178; 16 x 1,024
 // 3.7 us, a launch.
-#include "pv_ops.h"
+#include "pv_rows.h"
 
 #include <algorithm>
 
 using namespace pvo;
 
 namespace {
-
-constexpr int PARTS = 1024;                 // workgroups of the backward pass at most: rows of partial weight gradients
 
 // An 8-bit format: its largest value, and P values of it from floats that are at most that but for a rounding
 struct Fp8 {
@@ -53,43 +51,6 @@ struct Int8 {
         for (int j = 0; j < P; j++) o.v[j] = v[j] != v[j] ? 0 : type(fminf(fmaxf(rintf(v[j]), -MOST), MOST));
     }
 };
-
-// One row: D elements as packs of P, pack k * LANES + lane in register k of a lane; PACKS 0: not held, any number of packs.
-// ROWS: rows at a time of a workgroup
-template <int LANES_, int PACKS_, int ROWS_> struct Plan {
-    static constexpr int LANES = LANES_, PACKS = PACKS_, ROWS = ROWS_;
-    static constexpr int BLOCK = LANES * ROWS, WAVES = LANES > WAVE ? LANES / WAVE : 1;
-};
-
-// A sum, or a largest value, over the lanes of a row
-template <typename L, typename T, typename F> __device__ inline T over_row(T x, T* lds, F&& join) {
-#pragma unroll
-    for (int d = (L::LANES < WAVE ? L::LANES : WAVE) / 2; d; d >>= 1) x = join(x, T(__shfl_xor(x, d, WAVE)));
-    if constexpr (L::WAVES > 1) {
-        const int row = threadIdx.x / L::LANES, wave = threadIdx.x / WAVE;
-        __syncthreads();                                       // the last use of lds is over
-        if (threadIdx.x % WAVE == 0) lds[wave] = x;
-        __syncthreads();
-        x = lds[row * L::WAVES];
-#pragma unroll
-        for (int w = 1; w < L::WAVES; w++) x = join(x, lds[row * L::WAVES + w]);
-    }
-    return x;
-}
-template <typename L> __device__ inline float row_sum(float x, float* lds) {
-    return over_row<L>(x, lds, [](float a, float b) { return a + b; });
-}
-
-// A pack of a row at element i of D: whole, or a part of one at the row's end
-template <int P, bool ONCE, typename T> __device__ inline pack<T, P> take(const T* row, int64_t i, int64_t D) {
-    if (i + P <= D) return ONCE ? pack<T, P>::load_once(row + i) : pack<T, P>::load(row + i);
-    return pack<T, P>::load_part(row + i, D - i);
-}
-template <bool ONCE, typename T, int P> __device__ inline void leave(const pack<T, P>& v, T* row, int64_t i, int64_t D) {
-    if (i + P > D) v.store_part(row + i, D - i);
-    else if (ONCE) v.store_once(row + i);
-    else v.store(row + i);
-}
 
 template <typename E, typename Q, typename L>
 __global__ __launch_bounds__(L::BLOCK) void norm_kernel(const E* __restrict__ x, const E* __restrict__ residual, const float* __restrict__ weight, int64_t N,
@@ -317,25 +278,6 @@ __global__ __launch_bounds__(L::BLOCK) void norm_back_kernel(const E* __restrict
     }
 }
 
-// d_weight[i] = sum of the partial rows, from column `first` on: 64 columns a workgroup, its 16 waves a run of rows each
-constexpr int END_WAVES = 16;
-__global__ __launch_bounds__(END_WAVES* WAVE) void norm_weight_kernel(const float* __restrict__ parts, int64_t rows, int64_t D, int64_t first, float* __restrict__ d_weight) {
-    __shared__ float lds[END_WAVES][WAVE];
-    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
-    const int64_t i = first + int64_t(blockIdx.x) * WAVE + lane;
-    float sum = 0.0f;
-    if (i < D) {
-#pragma unroll 8
-        for (int64_t k = wave; k < rows; k += END_WAVES) sum += parts[k * D + i];
-    }
-    lds[wave][lane] = sum;
-    __syncthreads();
-    if (wave || i >= D) return;
-#pragma unroll
-    for (int w = 1; w < END_WAVES; w++) sum += lds[w][lane];
-    d_weight[i] = sum;
-}
-
 // f(Plan) for rows of D elements of type E: as few lanes as hold the row in one pack each, up to a wave, then more packs, then more
 // waves. Backwards, where three tensors, the weights and their gradients' sums are held, 16-bit elements have two packs a lane at
 // most; four packs elsewhere, in workgroups as large as the row fills (13,826 x 4,839 float32 by 512 lanes 172 us, by 1,024 195;
@@ -368,7 +310,6 @@ template <typename E> int rows_of(int64_t D) {
     with_plan<E, true>(D, [&](auto plan) { rows = decltype(plan)::ROWS; return 0; });
     return rows;
 }
-int64_t groups_of(int64_t N, int rows) { const int64_t g = (N + rows - 1) / rows; return g < PARTS ? g : PARTS; }
 
 int32_t check(int64_t N, int64_t D, int32_t dtype, char* err, size_t cap) {
     if (!element_bytes(dtype)) return fail(PV_EARG, err, cap, "dtype: one of PV_F32, PV_BF16, PV_F16");
