@@ -403,6 +403,22 @@ int32_t pv_add_rms_norm_backward_hip(const void* s, const float* rstd, const flo
                                      const void* d_stream, int32_t dtype, void* d, float* d_weight, void* work, uint64_t work_bytes, void* stream, char* err,
                                      size_t errcap);
 
+/* The gated delta rule. A state S [K, V] for each of B sequences and G value heads, over T steps: with a = 1 - sigmoid(gate),
+ * b = sigmoid(write), and query and key divided by sqrt(their squares' sum + eps),
+ *   u = b (value[t] - a S[t-1]^T key[t]),  S[t] = a S[t-1] + key[t] u^T,  out[t] = S[t]^T query[t].
+ * query, key: [B, T, H, K], value: [B, T, G, V], gate, write: [B, T, G], all of `dtype`; G is a multiple of H, and value head g
+ * goes with query and key head g / (G / H). strides: host array of 15, in elements: of a sequence, a step and a head of query, key,
+ * value, gate, write in turn; a step's at most 2^24. B, T, H >= 1, K <= 128, V <= 65,536; of 64 steps of a value head's sequence,
+ * and of 32 columns of a state, there are fewer than 2^24. Squares of a key's or query's length are within float32.
+ * state: f32[B, G, K, V] before step 0, or NULL: zero. reset: u8[B, T], or NULL; where not 0, S[t-1] is dropped. out: [B, T, G, V] of
+ * `dtype`; last: f32[B, G, K, V] = S[T-1], apart from state. For the backward pass: starts (pv_gated_delta_start_bytes, 16-byte
+ * aligned; NULL: none) and what the call leaves in `work`. work: pv_gated_delta_work_bytes with keep = 1 if there are starts, else 0. */
+uint64_t pv_gated_delta_work_bytes(int64_t B, int64_t T, int32_t G, int32_t dtype, int32_t keep);
+uint64_t pv_gated_delta_start_bytes(int64_t B, int64_t T, int32_t G, int32_t K, int32_t V, int32_t dtype);
+int32_t pv_gated_delta_hip(const void* query, const void* key, const void* value, const void* gate, const void* write, const float* state, const uint8_t* reset,
+                           int64_t B, int64_t T, int32_t H, int32_t G, int32_t K, int32_t V, const int64_t* strides, float eps, int32_t dtype, void* out, float* last,
+                           void* starts, void* work, uint64_t work_bytes, void* stream, char* err, size_t errcap);
+
 /* Dropout. Element i of a call is dropped where its 16 bits are below round(p 2^16), 0 <= p <= 1, and else multiplied by
  * 2^16 / (2^16 - round(p 2^16)). The bits are word (i / 2) % 4, half i % 2 (the low one first) of the ten-round generator of four
  * 32-bit words by Salmon, Moraes, Dror and Shaw (2011) with the seed as its key and counter (i / 8 in 64 bits, site, 0). The

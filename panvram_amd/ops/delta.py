@@ -1,0 +1,83 @@
+"""The gated delta rule over sequences (panvram_amd/csrc/pv_delta.hip)."""
+import ctypes
+
+import torch
+
+from .. import _native as N
+from ._call import DTYPES, call, on_gpu, once, ptr
+
+_Strides = ctypes.c_int64 * 15
+
+
+def _strided(t):
+    """`t` with neighbouring elements in a head, and steps at most 2^24 elements apart: itself, or a copy."""
+    if (t.dim() == 4 and t.stride(3) != 1 and t.shape[3] != 1) or t.stride(1) > 1 << 24:
+        t = t.contiguous()
+    return t
+
+
+def _strides(*tensors):
+    return _Strides(*(s for t in tensors for s in t.stride()[:3]))
+
+
+def _forward(index, query, key, value, gate, write, state, reset, eps, keep):
+    """out, last, and for the backward pass the states at chunks' starts and the chunks' records"""
+    B, T, H, K = query.shape
+    G, V = value.shape[2:]
+    dev, dtype = query.device, query.dtype
+    given = [_strided(t) for t in (query, key, value, gate, write)]
+    out = torch.empty((B, T, G, V), dtype=dtype, device=dev)
+    last = torch.empty((B, G, K, V), dtype=torch.float32, device=dev)
+    L, code = N.lib(), DTYPES[dtype]
+    starts = torch.empty(L.pv_gated_delta_start_bytes(B, T, G, K, V, code), dtype=torch.uint8, device=dev) if keep else None
+    size = L.pv_gated_delta_work_bytes(B, T, G, code, int(keep))
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    call(L.pv_gated_delta_hip, index, *(t.data_ptr() for t in given), ptr(state), ptr(reset), B, T, H, G, K, V, _strides(*given), eps, code, out.data_ptr(),
+         last.data_ptr(), ptr(starts), ptr(work), size)
+    return out, last, starts, work
+
+
+def gated_delta(query, key, value, gate, write, state=None, reset=None, eps=1e-6):
+    """The gated delta rule: each value head has a matrix S as its state, and with keep = 1 - sigmoid(gate),
+    rate = sigmoid(write), and query and key divided by sqrt(the sum of their squares + eps),
+
+        S[t] = keep[t] S[t-1] + key[t] u[t]^T,  u[t] = rate[t] (value[t] - keep[t] S[t-1]^T key[t]),  out[t] = S[t]^T query[t]:
+
+    what S holds for the direction of key[t] is replaced by value[t], in the share that rate says.
+
+    query, key: [B, T, H, K] with K up to 128; value: [B, T, G, V]; gate, write: [B, T, G]; float32, bfloat16 or float16, alike. G is
+    a multiple of H: value head g goes with query and key head g // (G // H). Parts of one projection are read where they are.
+    state: float32 [B, G, K, V], the S before the first step (None: zero). reset: bool or uint8 [B, T]; where it is set, the S of the
+    step before is dropped, as at the first base of a window packed behind another. Returns (out [B, T, G, V] in query's type,
+    last float32 [B, G, K, V]); `last` is the next call's state, so generation calls it with T = 1.
+
+    Sequences are worked on in chunks of 64 steps by matrix products: a NaN or an infinity in one step's inputs reaches the
+    outputs of all steps of its chunk, and through the state those of its head after it; a state that is not finite is dropped by a
+    reset all the same. Queries and keys have squares whose sum is a float32."""
+    index = on_gpu("gated_delta", query, key, value, gate, write, state, reset)
+    if query.dim() != 4 or query.shape != key.shape:
+        raise ValueError(f"gated_delta: query and key are [B, T, H, K] alike, got {list(query.shape)} and {list(key.shape)}")
+    dtype = query.dtype
+    if dtype not in DTYPES or any(t.dtype != dtype for t in (key, value, gate, write)):
+        raise ValueError(f"gated_delta: query, key, value, gate and write are float32, bfloat16 or float16 alike, got {[str(t.dtype) for t in (query, key, value, gate, write)]}")
+    B, T, H, K = query.shape
+    if value.dim() != 4 or value.shape[:2] != (B, T) or H < 1 or value.shape[2] < 1 or value.shape[2] % H:
+        raise ValueError(f"gated_delta: value is [{B}, {T}, G, V] with G a multiple of {H}, got {list(value.shape)}")
+    G, V = value.shape[2:]
+    if not 1 <= K <= 128 or not 1 <= V <= 1 << 16:
+        raise ValueError(f"gated_delta: keys have 1 to 128 elements and values 1 to 65,536, got {K} and {V}")
+    if gate.shape != (B, T, G) or write.shape != (B, T, G):
+        raise ValueError(f"gated_delta: gate and write are {[B, T, G]}, got {list(gate.shape)} and {list(write.shape)}")
+    if not eps >= 0:
+        raise ValueError(f"gated_delta: eps is not negative, got {eps}")
+    if state is not None:
+        if state.dtype != torch.float32 or state.shape != (B, G, K, V):
+            raise ValueError(f"gated_delta: state is float32 {[B, G, K, V]}, got {state.dtype} {list(state.shape)}")
+        state = state.contiguous()
+    if reset is not None:
+        if reset.dtype not in (torch.bool, torch.uint8) or reset.shape != (B, T):
+            raise ValueError(f"gated_delta: reset is bool or uint8 {[B, T]}, got {reset.dtype} {list(reset.shape)}")
+        reset = reset.contiguous()
+    if B == 0 or T == 0:
+        return value * 1, state.clone() if state is not None else torch.zeros(B, G, K, V, dtype=torch.float32, device=query.device)
+    return _forward(index, query, key, value, gate, write, state, reset, eps, False)[:2]
