@@ -113,6 +113,9 @@ template <typename S_, int ROWS, int COLS, int PARTS = 1> struct Tile {
         return f;
     }
     __device__ Frag<S, 1> cols_narrow(int c0, int kb) const { return Tile<S, ROWS, COLS, 1>{p}.cols(c0, kb); }
+    // eight neighbouring places of a row, in the first part
+    __device__ void put_places(int row, int at, const pack<S, 8>& v) const { v.store(p + row * ROW + at); }
+    __device__ S get(int row, int c) const { return p[row * ROW + place(c)]; }
     // eight neighbouring columns of a row, c a multiple of 8
     __device__ void put(int row, int c, const S (&v)[8]) const {
         S* at = p + row * ROW + place(c);
@@ -180,6 +183,15 @@ __device__ inline int since(uint64_t cut, int i) {         // the last step up t
     const uint64_t m = cut & (~0ull >> (63 - i));
     return m ? 63 - __builtin_clzll(m) : -1;
 }
+
+// What the forward pass keeps for the backward pass, and what the walk backwards leaves for the gradients: two arrays of the same
+// shapes, for a chunk of a value head. By columns of the state or of values, vp of them:
+//   states   [vp][DK]: S before the chunk, or the gradient of S after it; rows at their places
+//   steps    [vp][64]: U, or the gradient of b D; steps at their places
+template <typename S> struct Kept {
+    S *states, *steps;
+    Kept(void* p, const Shape& s, int dk) : states(static_cast<S*>(p)), steps(states + s.B * s.G * s.chunks * int64_t(s.vp) * dk) {}
+};
 
 // The value heads that share a query and key head are neighbours
 __device__ inline int shared(const Shape& S, int g) { return g / (S.G / S.H); }

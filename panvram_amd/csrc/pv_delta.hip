@@ -216,7 +216,7 @@ __global__ __launch_bounds__(BLOCK) void chunk_kernel(const E* __restrict__ quer
 template <typename E, int DK, int W>
 __global__ __launch_bounds__(W * WAVE) void state_kernel(const E* __restrict__ query, const E* __restrict__ key, const E* __restrict__ value,
                                                          const float* __restrict__ state, Shape S, const Chunk<typename Rep<E>::S>* __restrict__ records,
-                                                         E* __restrict__ out, float* __restrict__ last, typename Rep<E>::S* __restrict__ starts) {
+                                                         E* __restrict__ out, float* __restrict__ last, bool keep, Kept<typename Rep<E>::S> kept) {
     using St = typename Rep<E>::S;
     constexpr int WIDE = Rep<E>::WIDE, ND = DK / 16, KB = DK / 32, THREADS = W * WAVE;
     using In = Tile<St, C, DK>;
@@ -315,14 +315,15 @@ __global__ __launch_bounds__(W * WAVE) void state_kernel(const E* __restrict__ q
         Frag<St, WIDE> sf[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; kb++) sf[kb] = frag_of<St, WIDE>(s[2 * kb], s[2 * kb + 1]);
-        if (starts && col < S.vp) {        // the state before the chunk, by columns, rows at their places
-            St* to = starts + ((bg * S.chunks + n) * S.vp + col) * DK + 8 * grp;
+        const auto leave = [&](St* to, const auto& f) {    // eight places of an operand's first part
+            pack<St, 8> o;
+            __builtin_memcpy(&o, &f, sizeof o);
+            o.store(to);
+        };
+        const int64_t row = (bg * S.chunks + n) * S.vp + col;
+        if (keep && col < S.vp) {
 #pragma unroll
-            for (int kb = 0; kb < KB; kb++) {
-                pack<St, 8> o;
-                __builtin_memcpy(&o, &sf[kb], sizeof o);
-                o.store(to + 32 * kb);
-            }
+            for (int kb = 0; kb < KB; kb++) leave(kept.states + row * DK + 32 * kb + 8 * grp, sf[kb]);
         }
         // D = V - g K S, then b D as an operand; out's part g Q S
         f4 o[4];
@@ -366,6 +367,10 @@ __global__ __launch_bounds__(W * WAVE) void state_kernel(const E* __restrict__ q
         Frag<St, 1> uf[2];
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) uf[kb] = frag_of<St, 1>(u[2 * kb], u[2 * kb + 1]);
+        if (keep && col < S.vp) {
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++) leave(kept.steps + row * C + 32 * kb + 8 * grp, uf[kb]);
+        }
         const int64_t t0 = n * C;
         E* to = out + ((b * S.T + t0) * S.G + g) * S.V + col;
 #pragma unroll
@@ -481,7 +486,7 @@ constexpr int SHORT = 8;                   // steps that are walked one by one
 
 template <typename E, int DK>
 int32_t forward(const void* query, const void* key, const void* value, const void* gate, const void* write, const float* state, const uint8_t* reset, const Shape& S,
-                void* out, float* last, void* starts, void* work, hipStream_t stream, char* err, size_t errcap) {
+                void* out, float* last, void* kept, void* work, hipStream_t stream, char* err, size_t errcap) {
     using St = typename Rep<E>::S;
     constexpr int W = 4;
     const auto in = [](const void* p) { return static_cast<const E*>(p); };
@@ -489,7 +494,7 @@ int32_t forward(const void* query, const void* key, const void* value, const voi
     const int64_t heads = S.B * S.G;
     chunk_kernel<E, DK><<<dim3(heads * S.chunks), BLOCK, 0, stream>>>(in(query), in(key), in(gate), in(write), reset, S, records);
     state_kernel<E, DK, W><<<dim3(heads * ((S.vp / 16 + W - 1) / W)), W * WAVE, 0, stream>>>(in(query), in(key), in(value), state, S, records, static_cast<E*>(out), last,
-                                                                                            static_cast<St*>(starts));
+                                                                                            kept != nullptr, Kept<St>(kept, S, DK));
     return launched(err, errcap);
 }
 
@@ -503,19 +508,19 @@ uint64_t pv_gated_delta_work_bytes(int64_t B, int64_t T, int32_t G, int32_t dtyp
     return chunks * (dtype == PV_BF16 ? sizeof(Chunk<bf16>) : sizeof(Chunk<float>));
 }
 
-uint64_t pv_gated_delta_start_bytes(int64_t B, int64_t T, int32_t G, int32_t K, int32_t V, int32_t dtype) {
+uint64_t pv_gated_delta_kept_bytes(int64_t B, int64_t T, int32_t G, int32_t K, int32_t V, int32_t dtype) {
     if (B < 1 || G < 1 || T < 1 || K < 1 || V < 1) return 0;
-    return uint64_t(B) * uint64_t(G) * uint64_t((T + C - 1) / C) * uint64_t((V + 15) / 16 * 16) * (K <= 32 ? 32 : K <= 64 ? 64 : 128) * (dtype == PV_BF16 ? 2 : 4);
+    return uint64_t(B) * uint64_t(G) * uint64_t((T + C - 1) / C) * uint64_t((V + 15) / 16 * 16) * ((K <= 32 ? 32 : K <= 64 ? 64 : 128) + C) * (dtype == PV_BF16 ? 2 : 4);
 }
 
 int32_t pv_gated_delta_hip(const void* query, const void* key, const void* value, const void* gate, const void* write, const float* state, const uint8_t* reset,
                            int64_t B, int64_t T, int32_t H, int32_t G, int32_t K, int32_t V, const int64_t* strides, float eps, int32_t dtype, void* out, float* last,
-                           void* starts, void* work, uint64_t work_bytes, void* stream, char* err, size_t errcap) {
+                           void* kept, void* work, uint64_t work_bytes, void* stream, char* err, size_t errcap) {
     Shape S;
     if (int32_t e = shape_of(B, T, H, G, K, V, strides, eps, dtype, S, err, errcap)) return e;
     if (!query || !key || !value || !gate || !write || !out || !last) return fail(PV_EARG, err, errcap, "null argument");
-    if (starts && !aligned(starts, 16)) return fail(PV_EARG, err, errcap, "starts: not 16-byte aligned");
-    const uint64_t need = pv_gated_delta_work_bytes(B, T, G, dtype, starts != nullptr);
+    if (kept && !aligned(kept, 16)) return fail(PV_EARG, err, errcap, "kept: not 16-byte aligned");
+    const uint64_t need = pv_gated_delta_work_bytes(B, T, G, dtype, kept != nullptr);
     if (need && (!work || work_bytes < need || !aligned(work, 16))) return fail(PV_EARG, err, errcap, "work: too small, or not 16-byte aligned");
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
@@ -526,7 +531,7 @@ int32_t pv_gated_delta_hip(const void* query, const void* key, const void* value
             return launched(err, errcap);
         }
         return with_k(K, [&](auto k) {
-            return forward<E, decltype(k)::value>(query, key, value, gate, write, state, reset, S, out, last, starts, work, hipStream_t(stream), err, errcap);
+            return forward<E, decltype(k)::value>(query, key, value, gate, write, state, reset, S, out, last, kept, work, hipStream_t(stream), err, errcap);
         });
     });
 }

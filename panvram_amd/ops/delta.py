@@ -6,8 +6,6 @@ import torch
 from .. import _native as N
 from ._call import DTYPES, call, on_gpu, once, ptr
 
-_Strides = ctypes.c_int64 * 15
-
 
 def _strided(t):
     """`t` with neighbouring elements in a head, and steps at most 2^24 elements apart: itself, or a copy."""
@@ -17,11 +15,11 @@ def _strided(t):
 
 
 def _strides(*tensors):
-    return _Strides(*(s for t in tensors for s in t.stride()[:3]))
+    return (ctypes.c_int64 * (3 * len(tensors)))(*(s for t in tensors for s in t.stride()[:3]))
 
 
 def _forward(index, query, key, value, gate, write, state, reset, eps, keep):
-    """out, last, and for the backward pass the states at chunks' starts and the chunks' records"""
+    """out, last, and for the backward pass the states before the chunks and the chunks' records"""
     B, T, H, K = query.shape
     G, V = value.shape[2:]
     dev, dtype = query.device, query.dtype
@@ -29,12 +27,43 @@ def _forward(index, query, key, value, gate, write, state, reset, eps, keep):
     out = torch.empty((B, T, G, V), dtype=dtype, device=dev)
     last = torch.empty((B, G, K, V), dtype=torch.float32, device=dev)
     L, code = N.lib(), DTYPES[dtype]
-    starts = torch.empty(L.pv_gated_delta_start_bytes(B, T, G, K, V, code), dtype=torch.uint8, device=dev) if keep else None
+    kept = torch.empty(L.pv_gated_delta_kept_bytes(B, T, G, K, V, code), dtype=torch.uint8, device=dev) if keep else None
     size = L.pv_gated_delta_work_bytes(B, T, G, code, int(keep))
     work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     call(L.pv_gated_delta_hip, index, *(t.data_ptr() for t in given), ptr(state), ptr(reset), B, T, H, G, K, V, _strides(*given), eps, code, out.data_ptr(),
-         last.data_ptr(), ptr(starts), ptr(work), size)
-    return out, last, starts, work
+         last.data_ptr(), ptr(kept), ptr(work), size)
+    return out, last, kept, work
+
+
+class _GatedDelta(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, query, key, value, gate, write, state, reset, eps):
+        out, last, kept, records = _forward(query.get_device(), query, key, value, gate, write, state, reset, eps, True)
+        ctx.save_for_backward(query, key, gate, write, kept, records)
+        ctx.values, ctx.has_state, ctx.eps = value.shape[2:], state is not None, eps
+        ctx.set_materialize_grads(False)
+        return out, last
+
+    @staticmethod
+    @once
+    def backward(ctx, d_out, d_last):
+        query, key, gate, write, kept, records = ctx.saved_tensors
+        B, T, H, K = query.shape
+        G, V = ctx.values
+        dev, dtype = query.device, query.dtype
+        d_out = torch.zeros((B, T, G, V), dtype=dtype, device=dev) if d_out is None else _strided(d_out)
+        d_last = None if d_last is None else d_last.contiguous()
+        d_query, d_key, d_value, d_gate, d_write = (torch.empty(s, dtype=dtype, device=dev) for s in ((B, T, H, K), (B, T, H, K), (B, T, G, V), (B, T, G), (B, T, G)))
+        d_state = torch.empty((B, G, K, V), dtype=torch.float32, device=dev) if ctx.has_state else None
+        L, code = N.lib(), DTYPES[dtype]
+        size = L.pv_gated_delta_kept_bytes(B, T, G, K, V, code)
+        work = torch.empty(size, dtype=torch.uint8, device=dev)
+        query, key, gate, write = (_strided(t) for t in (query, key, gate, write))
+        # (values are not read backwards: any strides stand for theirs)
+        call(L.pv_gated_delta_backward_hip, query.get_device(), query.data_ptr(), key.data_ptr(), gate.data_ptr(), write.data_ptr(), d_out.data_ptr(), ptr(d_last), B, T,
+             H, G, K, V, _strides(query, key, d_value, gate, write, d_out), ctx.eps, code, kept.data_ptr(), records.data_ptr(), d_query.data_ptr(), d_key.data_ptr(),
+             d_value.data_ptr(), d_gate.data_ptr(), d_write.data_ptr(), ptr(d_state), work.data_ptr(), size)
+        return d_query, d_key, d_value, d_gate, d_write, d_state, None, None
 
 
 def gated_delta(query, key, value, gate, write, state=None, reset=None, eps=1e-6):
@@ -49,7 +78,8 @@ def gated_delta(query, key, value, gate, write, state=None, reset=None, eps=1e-6
     a multiple of H: value head g goes with query and key head g // (G // H). Parts of one projection are read where they are.
     state: float32 [B, G, K, V], the S before the first step (None: zero). reset: bool or uint8 [B, T]; where it is set, the S of the
     step before is dropped, as at the first base of a window packed behind another. Returns (out [B, T, G, V] in query's type,
-    last float32 [B, G, K, V]); `last` is the next call's state, so generation calls it with T = 1.
+    last float32 [B, G, K, V]); `last` is the next call's state, so generation calls it with T = 1. Gradients flow to query, key,
+    value, gate, write and state, from out and from last.
 
     Sequences are worked on in chunks of 64 steps by matrix products: a NaN or an infinity in one step's inputs reaches the
     outputs of all steps of its chunk, and through the state those of its head after it; a state that is not finite is dropped by a
@@ -80,4 +110,6 @@ def gated_delta(query, key, value, gate, write, state=None, reset=None, eps=1e-6
         reset = reset.contiguous()
     if B == 0 or T == 0:
         return value * 1, state.clone() if state is not None else torch.zeros(B, G, K, V, dtype=torch.float32, device=query.device)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (query, key, value, gate, write, state)):
+        return _GatedDelta.apply(query, key, value, gate, write, state, reset, eps)
     return _forward(index, query, key, value, gate, write, state, reset, eps, False)[:2]
