@@ -47,16 +47,16 @@ __device__ inline void leave16(float* to, int row, const f4& v, float sign) {
 }
 
 // A matrix of 64 x 64 in LDS into a record, in parts
-template <typename S, int WIDE> __device__ inline void record(const float* m, int row, S (*to)[C][C]) {
+template <typename S> __device__ inline void record(const float* m, int row, S (*to)[C][C]) {
     for (int k = threadIdx.x; k < C * C / 8; k += BLOCK) {
         const int i = k / 8, at = k % 8 * 8;                       // eight places: columns c .. c + 3 and c + 16 .. c + 19
         const int c = (at & ~31) | (at & 24) >> 1;
         float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = m[i * row + c + j % 4 + j / 4 * 16];
+        for (int j = 0; j < 8; j++) v[j] = SQUARE<S> * m[i * row + c + j % 4 + j / 4 * 16];
         pack<S, 8> o;
 #pragma unroll
-        for (int w = 0; w < WIDE; w++) {
+        for (int w = 0; w < wide_of<S>; w++) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 o.v[j] = S(v[j]);
@@ -83,23 +83,24 @@ __global__ __launch_bounds__(BLOCK) void chunk_kernel(const E* __restrict__ quer
     const int64_t b = bg / S.G, t0 = chunk * C;
     const int g = int(bg % S.G), h = shared(S, g), rows = int(S.T - t0 < C ? S.T - t0 : C);
     // queries and keys, and one over their lengths
-    constexpr int PER = DK / 8;            // packs of a row, one a lane
-    const E *q0 = query + b * S.qb + t0 * S.qt + h * S.qh, *k0 = key + b * S.kb + t0 * S.kt + h * S.kh;
+    using In8 = Rows<E, DK, BLOCK>;
+    In8 q, k;
+    q.load(query + b * S.qb + t0 * S.qt + h * S.qh, S.qt, rows, S.K);
+    k.load(key + b * S.kb + t0 * S.kt + h * S.kh, S.kt, rows, S.K);
+    In8::clear(Qt, S.K);
+    In8::clear(Kt, S.K);
 #pragma unroll
-    for (int p = tid; p < C * PER; p += BLOCK) {
-        const int i = p / PER, c = p % PER * 8;
-        Eight<E> q, k;
-        const int left = i < rows ? S.K - c : 0;
-        q.load(q0 + i * S.qt + c, left);
-        k.load(k0 + i * S.kt + c, left);
-        q.put(Qt, i, c);
-        k.put(Kt, i, c);
-        float sq = q.square(), sk = k.square();
+    for (int j = 0; j < In8::COUNT; j++) {
+        const int i = In8::row(j);
+        float sq = q.square(j, S.K), sk = k.square(j, S.K);
 #pragma unroll
-        for (int d = PER / 2; d; d >>= 1) { sq += __shfl_xor(sq, d, WAVE); sk += __shfl_xor(sk, d, WAVE); }
-        if (p % PER == 0) {
-            st.rq[i] = i < rows ? 1.0f / sqrtf(sq + S.eps) : 0.0f;
-            st.rk[i] = i < rows ? 1.0f / sqrtf(sk + S.eps) : 0.0f;
+        for (int d = In8::PER / 2; d; d >>= 1) { sq += __shfl_xor(sq, d, WAVE); sk += __shfl_xor(sk, d, WAVE); }
+        const float rq = i < rows ? 1.0f / sqrtf(sq + S.eps) : 0.0f, rk = i < rows ? 1.0f / sqrtf(sk + S.eps) : 0.0f;
+        q.put(Qt, j, length_up<St>(rq), S.K);
+        k.put(Kt, j, length_up<St>(rk), S.K);
+        if (tid % In8::PER == 0) {
+            st.rq[i] = rq;
+            st.rk[i] = rk;
         }
     }
     if (wave == 0) {                       // a lane for each step: gates, and their logarithms summed up
@@ -150,27 +151,26 @@ __global__ __launch_bounds__(BLOCK) void chunk_kernel(const E* __restrict__ quer
     const float shift = tid < C ? st.x[tid] : 0.0f;
     __syncthreads();
     if (tid < C) {
-        st.x[tid] = shift * st.rk[tid];
-        st.q[tid] = shift * st.rq[tid];
-        st.l[tid] *= st.rk[tid];
+        st.x[tid] = shift * length_rest<St>(st.rk[tid]);
+        st.q[tid] = shift * length_rest<St>(st.rq[tid]);
+        st.l[tid] *= length_rest<St>(st.rk[tid]);
     }
 #pragma unroll
     for (int j = 0; j < WAVES; j++) {
         const int col = 16 * j + m;
-        const float rk = st.rk[col], hi = st.hi[col], lo = st.lo[col];
+        const float rk = length_rest<St>(st.rk[col]), hi = st.hi[col], lo = st.lo[col];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int i = 16 * wave + 4 * grp + r;
             const bool on = col <= i && col >= since(cuts, i);
             const float M = on ? expf((st.hi[i] - hi) + (st.lo[i] - lo)) * rk : 0.0f;
-            P[i * ROW + col] = on ? M * st.rq[i] * qk[j][r] : 0.0f;
-            A[i * ROW + col] = on && col < i ? M * st.rk[i] * st.b[i] * kk[j][r] : 0.0f;
+            P[i * ROW + col] = on ? M * length_rest<St>(st.rq[i]) * qk[j][r] : 0.0f;
+            A[i * ROW + col] = on && col < i ? M * length_rest<St>(st.rk[i]) * st.b[i] * kk[j][r] : 0.0f;
             T[i * ROW + col] = 0.0f;
         }
     }
     __syncthreads();
     auto& out = records[blockIdx.x];
-    constexpr int WIDE = Rep<E>::WIDE;
     if (wave == 0) {                       // the inverses of the diagonal's blocks: a lane for a column of one
         float t[16];
         const float* a = A + 16 * grp * ROW + 16 * grp;
@@ -184,7 +184,7 @@ __global__ __launch_bounds__(BLOCK) void chunk_kernel(const E* __restrict__ quer
 #pragma unroll
         for (int i = 0; i < 16; i++) T[(16 * grp + i) * ROW + 16 * grp + m] = t[i];
     }
-    record<St, WIDE>(P, ROW, out.pair);
+    record<St>(P, ROW, out.pair);
     __syncthreads();
     const auto at = [&](float* p, int i, int j) { return p + 16 * i * ROW + 16 * j; };
     const f4 zero = {0, 0, 0, 0};
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(BLOCK) void chunk_kernel(const E* __restrict__ quer
         leave16(at(T, 3, wave), ROW, product16(at(T, 3, 3), ROW, y3, product16(at(T, 3, 2), ROW, y2, zero)), -1.0f);
     }
     __syncthreads();
-    record<St, WIDE>(T, ROW, out.inv);
+    record<St>(T, ROW, out.inv);
     const float* from = reinterpret_cast<const float*>(&st);
     float* to = reinterpret_cast<float*>(&out.steps);
     for (int k = tid; k < int(sizeof(Steps) / 4); k += BLOCK) to[k] = from[k];
@@ -218,10 +218,11 @@ __global__ __launch_bounds__(W * WAVE) void state_kernel(const E* __restrict__ q
                                                          const float* __restrict__ state, Shape S, const Chunk<typename Rep<E>::S>* __restrict__ records,
                                                          E* __restrict__ out, float* __restrict__ last, bool keep, Kept<typename Rep<E>::S> kept) {
     using St = typename Rep<E>::S;
-    constexpr int WIDE = Rep<E>::WIDE, ND = DK / 16, KB = DK / 32, THREADS = W * WAVE;
+    constexpr int WIDE = wide_of<St>, ND = DK / 16, KB = DK / 32, THREADS = W * WAVE;
     using In = Tile<St, C, DK>;
     using Square = Tile<St, C, C, WIDE>;
     using Part = Tile<St, C, C>;
+    using In8 = Rows<E, DK, THREADS>;
     __shared__ alignas(16) St lds[2 * In::SIZE + Square::SIZE + Part::SIZE];
     __shared__ alignas(16) Steps st;
     const In Kt{lds}, Qt{lds + In::SIZE};
@@ -233,8 +234,8 @@ __global__ __launch_bounds__(W * WAVE) void state_kernel(const E* __restrict__ q
     const int col = (int(blockIdx.x % groups) * W + wave) * 16 + m;
     const int64_t b = bg / S.G;
     const int g = int(bg % S.G), h = shared(S, g);
-    const bool on = col < S.V;
-    const E *q0 = query + b * S.qb + h * S.qh, *k0 = key + b * S.kb + h * S.kh, *v0 = value + b * S.vb + g * S.vh + col;
+    const bool on = col < S.V, held = keep && col < S.vp;
+    const E *q0 = query + b * S.qb + h * S.qh, *k0 = key + b * S.kb + h * S.kh, *v0 = value + b * S.vb + g * S.vh + (on ? col : S.V - 1);
     const Chunk<St>* rec = records + bg * S.chunks;
 
     f4 s[ND];
@@ -247,88 +248,57 @@ __global__ __launch_bounds__(W * WAVE) void state_kernel(const E* __restrict__ q
         }
 
     // a chunk on its way from memory to LDS
-    constexpr int PER = DK / 8, IN = C * PER / THREADS, SQ = C * C * int(sizeof(St)) / 16 / THREADS, ST = (int(sizeof(Steps) / 4) + THREADS - 1) / THREADS;
-    Eight<E> kp[IN], qp[IN];
-    pack<St, 16 / sizeof(St)> tp[WIDE][SQ], pp[SQ];
-    float sp[ST];
-    E vp[16];
+    In8 qp, kp;
+    float qr[In8::COUNT], kr[In8::COUNT];
+    SquareOnItsWay<St, WIDE, THREADS> tp;
+    SquareOnItsWay<St, 1, THREADS> pp;
+    StepsOnTheirWay<THREADS> sp;
+    Sixteen<E> vp;
     auto fetch = [&](int64_t n) {
         const int64_t t0 = n * C;
         const int rows = int(S.T - t0 < C ? S.T - t0 : C);
-        const E *q = q0 + t0 * S.qt, *k = k0 + t0 * S.kt, *v = v0 + t0 * S.vt;
+        kp.load(k0 + t0 * S.kt, S.kt, rows, S.K);
+        qp.load(q0 + t0 * S.qt, S.qt, rows, S.K);
 #pragma unroll
-        for (int j = 0; j < IN; j++) {
-            const int p = tid + j * THREADS, i = p / PER, c = p % PER * 8, left = i < rows ? S.K - c : 0;
-            kp[j].load(k + i * S.kt + c, left);
-            qp[j].load(q + i * S.qt + c, left);
+        for (int j = 0; j < In8::COUNT; j++) {
+            kr[j] = rec[n].steps.rk[In8::row(j)];
+            qr[j] = rec[n].steps.rq[In8::row(j)];
         }
-        constexpr int P = 16 / sizeof(St);
-        const St *inv = &rec[n].inv[0][0][0], *pair = &rec[n].pair[0][0][0];
-#pragma unroll
-        for (int j = 0; j < SQ; j++) {
-            const int at = (tid + j * THREADS) * P;
-#pragma unroll
-            for (int w = 0; w < WIDE; w++) tp[w][j] = pack<St, P>::load(inv + w * C * C + at);
-            pp[j] = pack<St, P>::load(pair + at);
-        }
-        const float* from = reinterpret_cast<const float*>(&rec[n].steps);
-#pragma unroll
-        for (int j = 0; j < ST; j++) if (tid + j * THREADS < int(sizeof(Steps) / 4)) sp[j] = from[tid + j * THREADS];
-#pragma unroll
-        for (int it = 0; it < 4; it++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int i = 16 * it + 4 * grp + r;
-                vp[4 * it + r] = on && i < rows ? v[i * S.vt] : E(0.0f);
-            }
-    };
-    auto stage = [&] {
-#pragma unroll
-        for (int j = 0; j < IN; j++) {
-            const int p = tid + j * THREADS, i = p / PER, c = p % PER * 8;
-            kp[j].put(Kt, i, c);
-            qp[j].put(Qt, i, c);
-        }
-        constexpr int P = 16 / sizeof(St);
-#pragma unroll
-        for (int j = 0; j < SQ; j++) {
-            const int at = (tid + j * THREADS) * P, i = at / C, c = at % C;
-#pragma unroll
-            for (int w = 0; w < WIDE; w++) tp[w][j].store(Tt.p + w * Square::PLANE + i * Square::ROW + c);
-            pp[j].store(Pt.p + i * Part::ROW + c);
-        }
-        float* to = reinterpret_cast<float*>(&st);
-#pragma unroll
-        for (int j = 0; j < ST; j++) if (tid + j * THREADS < int(sizeof(Steps) / 4)) to[tid + j * THREADS] = sp[j];
+        tp.load(rec[n].inv);
+        pp.load(rec[n].pair);
+        sp.load(rec[n].steps);
+        vp.load(v0 + t0 * S.vt, S.vt, rows);
     };
     const auto four = [&](const float* p, int it) { return *reinterpret_cast<const f4*>(p + 16 * it + 4 * grp); };
 
+    In8::clear(Kt, S.K);
+    In8::clear(Qt, S.K);
     fetch(0);
     for (int64_t n = 0; n < S.chunks; n++) {
         __syncthreads();                   // the chunk before has been used
-        stage();
-        float v[16];
 #pragma unroll
-        for (int j = 0; j < 16; j++) v[j] = float(vp[j]);
+        for (int j = 0; j < In8::COUNT; j++) {
+            kp.put(Kt, j, length_up<St>(kr[j]), S.K);
+            qp.put(Qt, j, length_up<St>(qr[j]), S.K);
+        }
+        tp.put(Tt);
+        pp.put(Pt);
+        sp.put(st);
+        f4 v[4];
+#pragma unroll
+        for (int it = 0; it < 4; it++) v[it] = vp.four(it, on);
         __syncthreads();
         if (n + 1 < S.chunks) fetch(n + 1);
+        const int64_t row = (bg * S.chunks + n) * S.vp + col;
+        const Scale ss = scale_of<St>(over_column(largest(s)));
         Frag<St, WIDE> sf[KB];
 #pragma unroll
-        for (int kb = 0; kb < KB; kb++) sf[kb] = frag_of<St, WIDE>(s[2 * kb], s[2 * kb + 1]);
-        const auto leave = [&](St* to, const auto& f) {    // eight places of an operand's first part
-            pack<St, 8> o;
-            __builtin_memcpy(&o, &f, sizeof o);
-            o.store(to);
-        };
-        const int64_t row = (bg * S.chunks + n) * S.vp + col;
-        if (keep && col < S.vp) {
-#pragma unroll
-            for (int kb = 0; kb < KB; kb++) leave(kept.states + row * DK + 32 * kb + 8 * grp, sf[kb]);
+        for (int kb = 0; kb < KB; kb++) {
+            sf[kb] = frag_of<St, WIDE>(s[2 * kb], s[2 * kb + 1], ss.up);
+            if (held) leave(kept.states + row * DK + 32 * kb + 8 * grp, sf[kb]);
         }
-        // D = V - g K S, then b D as an operand; out's part g Q S
-        f4 o[4];
-        Frag<St, WIDE> rf[2];
-        f4 pairs[2];
+        // D = V - g K S, then b D; out's part g Q S
+        f4 o[4], d[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) {
             f4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
@@ -339,48 +309,59 @@ __global__ __launch_bounds__(W * WAVE) void state_kernel(const E* __restrict__ q
             }
             const f4 xs = four(st.x, it), bs = four(st.b, it), qs = four(st.q, it);
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                pairs[it % 2][r] = bs[r] * (v[4 * it + r] - (xs[r] == 0.0f ? 0.0f : xs[r] * x[r]));      // (a dropped state may hold anything)
-                o[it][r] = qs[r] == 0.0f ? 0.0f : qs[r] * y[r];
+            for (int r = 0; r < 4; r++) {  // (a dropped state may hold anything)
+                d[it][r] = bs[r] * (v[it][r] - (xs[r] == 0.0f ? 0.0f : xs[r] * (ss.down * x[r])));
+                o[it][r] = qs[r] == 0.0f ? 0.0f : qs[r] * (ss.down * y[r]);
             }
-            if (it % 2) rf[it / 2] = frag_of<St, WIDE>(pairs[0], pairs[1]);
         }
-        // U = (I + A)^-1 b D; out's part (M Q K^T) U; what U adds to the state
+        // U = (I + A)^-1 b D
+        const Scale ds = scale_of<St>(over_column(largest(d)));
+        Frag<St, WIDE> df[2];
         f4 u[4];
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++) df[kb] = frag_of<St, WIDE>(d[2 * kb], d[2 * kb + 1], ds.up);
+        const float du = ds.down * (1.0f / SQUARE<St>);
 #pragma unroll
         for (int it = 0; it < 4; it++) {
             u[it] = f4{0, 0, 0, 0};
 #pragma unroll
-            for (int kb = 0; kb <= it / 2; kb++) mma(u[it], Tt.rows(16 * it, kb), rf[kb]);
+            for (int kb = 0; kb <= it / 2; kb++) mma(u[it], Tt.rows(16 * it, kb), df[kb]);
+            u[it] *= du;
         }
+        // what it adds to the state (l r is 2 / LONG at most); out's part (M Q K^T) U
+        const Scale us = scale_of<St>(over_column(largest(u)));
+        Frag<St, 1> uf[2];
         Frag<St, WIDE> lf[2];
 #pragma unroll
-        for (int kb = 0; kb < 2; kb++) lf[kb] = frag_of<St, WIDE>(u[2 * kb] * four(st.l, 2 * kb), u[2 * kb + 1] * four(st.l, 2 * kb + 1));
-        const float end = st.end;
+        for (int kb = 0; kb < 2; kb++) {
+            uf[kb] = frag_of<St, 1>(u[2 * kb], u[2 * kb + 1], us.up);
+            lf[kb] = frag_of<St, WIDE>(LONG<St> * u[2 * kb] * four(st.l, 2 * kb), LONG<St> * u[2 * kb + 1] * four(st.l, 2 * kb + 1), us.up);
+            if (held) leave(kept.steps + row * C + 32 * kb + 8 * grp, uf[kb]);
+        }
+        if (held && grp == 0) {
+            kept.scales[(bg * S.chunks + n) * 3 * S.vp + col] = ss.down;
+            kept.scales[((bg * S.chunks + n) * 3 + 1) * S.vp + col] = us.down;
+        }
+        const float end = st.end, dl = us.down * (1.0f / LONG<St>), dp = us.down * (1.0f / SQUARE<St>);
 #pragma unroll
         for (int k = 0; k < ND; k++) {
+            f4 x = {0, 0, 0, 0};
 #pragma unroll
-            for (int r = 0; r < 4; r++) s[k][r] = end == 0.0f ? 0.0f : end * s[k][r];
+            for (int kb = 0; kb < 2; kb++) mma(x, Kt.cols(16 * k, kb), lf[kb]);
 #pragma unroll
-            for (int kb = 0; kb < 2; kb++) mma(s[k], Kt.cols(16 * k, kb), lf[kb]);
-        }
-        Frag<St, 1> uf[2];
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++) uf[kb] = frag_of<St, 1>(u[2 * kb], u[2 * kb + 1]);
-        if (keep && col < S.vp) {
-#pragma unroll
-            for (int kb = 0; kb < 2; kb++) leave(kept.steps + row * C + 32 * kb + 8 * grp, uf[kb]);
+            for (int r = 0; r < 4; r++) s[k][r] = fmaf(dl, x[r], end == 0.0f ? 0.0f : end * s[k][r]);
         }
         const int64_t t0 = n * C;
         E* to = out + ((b * S.T + t0) * S.G + g) * S.V + col;
 #pragma unroll
         for (int it = 0; it < 4; it++) {
+            f4 x = {0, 0, 0, 0};
 #pragma unroll
-            for (int kb = 0; kb <= it / 2; kb++) mma(o[it], Pt.rows(16 * it, kb), uf[kb]);
+            for (int kb = 0; kb <= it / 2; kb++) mma(x, Pt.rows(16 * it, kb), uf[kb]);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int i = 16 * it + 4 * grp + r;
-                if (on && t0 + i < S.T) to[int64_t(i) * S.G * S.V] = E(o[it][r]);
+                if (on && t0 + i < S.T) to[int64_t(i) * S.G * S.V] = E(fmaf(dp, x[r], o[it][r]));
             }
         }
     }
@@ -505,12 +486,12 @@ extern "C" {
 uint64_t pv_gated_delta_work_bytes(int64_t B, int64_t T, int32_t G, int32_t dtype, int32_t keep) {
     if (B < 1 || G < 1 || T < 1 || (T <= SHORT && !keep)) return 0;
     const uint64_t chunks = uint64_t(B) * uint64_t(G) * uint64_t((T + C - 1) / C);
-    return chunks * (dtype == PV_BF16 ? sizeof(Chunk<bf16>) : sizeof(Chunk<float>));
+    return chunks * (dtype == PV_F32 ? sizeof(Chunk<float>) : sizeof(Chunk<f16>));
 }
 
 uint64_t pv_gated_delta_kept_bytes(int64_t B, int64_t T, int32_t G, int32_t K, int32_t V, int32_t dtype) {
     if (B < 1 || G < 1 || T < 1 || K < 1 || V < 1) return 0;
-    return uint64_t(B) * uint64_t(G) * uint64_t((T + C - 1) / C) * uint64_t((V + 15) / 16 * 16) * ((K <= 32 ? 32 : K <= 64 ? 64 : 128) + C) * (dtype == PV_BF16 ? 2 : 4);
+    return kept_bytes(uint64_t(B) * uint64_t(G) * uint64_t((T + C - 1) / C) * uint64_t((V + 15) / 16 * 16), K <= 32 ? 32 : K <= 64 ? 64 : 128, dtype);
 }
 
 int32_t pv_gated_delta_hip(const void* query, const void* key, const void* value, const void* gate, const void* write, const float* state, const uint8_t* reset,

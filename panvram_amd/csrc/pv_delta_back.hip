@@ -24,11 +24,12 @@ constexpr int WAVES = 4, BLOCK = WAVES * WAVE;
 template <typename E, int DK, int W>
 __global__ __launch_bounds__(W * WAVE) void walk_kernel(const E* __restrict__ query, const E* __restrict__ key, const E* __restrict__ d_out,
                                                         const float* __restrict__ d_last, Shape S, const Chunk<typename Rep<E>::S>* __restrict__ records,
-                                                        E* __restrict__ d_value, float* __restrict__ d_state, Kept<typename Rep<E>::S> left_over) {
+                                                        E* __restrict__ d_value, float* __restrict__ d_state, Kept<typename Rep<E>::S> walked) {
     using St = typename Rep<E>::S;
-    constexpr int WIDE = Rep<E>::WIDE, ND = DK / 16, KB = DK / 32, THREADS = W * WAVE;
+    constexpr int WIDE = wide_of<St>, ND = DK / 16, KB = DK / 32, THREADS = W * WAVE;
     using In = Tile<St, C, DK>;
     using Square = Tile<St, C, C, WIDE>;
+    using In8 = Rows<E, DK, THREADS>;
     __shared__ alignas(16) St lds[2 * In::SIZE + 2 * Square::SIZE];
     __shared__ alignas(16) Steps st;
     const In Kt{lds}, Qt{lds + In::SIZE};
@@ -39,8 +40,8 @@ __global__ __launch_bounds__(W * WAVE) void walk_kernel(const E* __restrict__ qu
     const int col = (int(blockIdx.x % groups) * W + wave) * 16 + m;
     const int64_t b = bg / S.G;
     const int g = int(bg % S.G), h = shared(S, g);
-    const bool on = col < S.V;
-    const E *q0 = query + b * S.qb + h * S.qh, *k0 = key + b * S.kb + h * S.kh, *o0 = d_out + b * S.ob + g * S.og + col;
+    const bool on = col < S.V, held = col < S.vp;
+    const E *q0 = query + b * S.qb + h * S.qh, *k0 = key + b * S.kb + h * S.kh, *o0 = d_out + b * S.ob + g * S.og + (on ? col : S.V - 1);
     const Chunk<St>* rec = records + bg * S.chunks;
 
     f4 s[ND];
@@ -52,148 +53,129 @@ __global__ __launch_bounds__(W * WAVE) void walk_kernel(const E* __restrict__ qu
             s[n][r] = d_last && on && d < S.K ? d_last[(bg * S.K + d) * S.V + col] : 0.0f;
         }
 
-    constexpr int PER = DK / 8, IN = C * PER / THREADS, SQ = C * C * int(sizeof(St)) / 16 / THREADS, ST = (int(sizeof(Steps) / 4) + THREADS - 1) / THREADS;
-    Eight<E> kp[IN], qp[IN];
-    pack<St, 16 / sizeof(St)> tp[WIDE][SQ], pp[WIDE][SQ];
-    float sp[ST];
-    E op[16];
+    In8 qp, kp;
+    float qr[In8::COUNT], kr[In8::COUNT];
+    SquareOnItsWay<St, WIDE, THREADS> tp, pp;
+    StepsOnTheirWay<THREADS> sp;
+    Sixteen<E> op;
     auto fetch = [&](int64_t n) {
         const int64_t t0 = n * C;
         const int rows = int(S.T - t0 < C ? S.T - t0 : C);
-        const E *q = q0 + t0 * S.qt, *k = k0 + t0 * S.kt, *o = o0 + t0 * S.ot;
+        kp.load(k0 + t0 * S.kt, S.kt, rows, S.K);
+        qp.load(q0 + t0 * S.qt, S.qt, rows, S.K);
 #pragma unroll
-        for (int j = 0; j < IN; j++) {
-            const int p = tid + j * THREADS, i = p / PER, c = p % PER * 8, left = i < rows ? S.K - c : 0;
-            kp[j].load(k + i * S.kt + c, left);
-            qp[j].load(q + i * S.qt + c, left);
+        for (int j = 0; j < In8::COUNT; j++) {
+            kr[j] = rec[n].steps.rk[In8::row(j)];
+            qr[j] = rec[n].steps.rq[In8::row(j)];
         }
-        constexpr int P = 16 / sizeof(St);
-        const St *inv = &rec[n].inv[0][0][0], *pair = &rec[n].pair[0][0][0];
-#pragma unroll
-        for (int j = 0; j < SQ; j++) {
-            const int at = (tid + j * THREADS) * P;
-#pragma unroll
-            for (int w = 0; w < WIDE; w++) {
-                tp[w][j] = pack<St, P>::load(inv + w * C * C + at);
-                pp[w][j] = pack<St, P>::load(pair + w * C * C + at);
-            }
-        }
-        const float* from = reinterpret_cast<const float*>(&rec[n].steps);
-#pragma unroll
-        for (int j = 0; j < ST; j++) if (tid + j * THREADS < int(sizeof(Steps) / 4)) sp[j] = from[tid + j * THREADS];
-#pragma unroll
-        for (int it = 0; it < 4; it++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int i = 16 * it + 4 * grp + r;
-                op[4 * it + r] = on && i < rows ? o[i * S.ot] : E(0.0f);
-            }
-    };
-    auto stage = [&] {
-#pragma unroll
-        for (int j = 0; j < IN; j++) {
-            const int p = tid + j * THREADS, i = p / PER, c = p % PER * 8;
-            kp[j].put(Kt, i, c);
-            qp[j].put(Qt, i, c);
-        }
-        constexpr int P = 16 / sizeof(St);
-#pragma unroll
-        for (int j = 0; j < SQ; j++) {
-            const int at = (tid + j * THREADS) * P, i = at / C, c = at % C;
-#pragma unroll
-            for (int w = 0; w < WIDE; w++) {
-                tp[w][j].store(Tt.p + w * Square::PLANE + i * Square::ROW + c);
-                pp[w][j].store(Pt.p + w * Square::PLANE + i * Square::ROW + c);
-            }
-        }
-        float* to = reinterpret_cast<float*>(&st);
-#pragma unroll
-        for (int j = 0; j < ST; j++) if (tid + j * THREADS < int(sizeof(Steps) / 4)) to[tid + j * THREADS] = sp[j];
+        tp.load(rec[n].inv);
+        pp.load(rec[n].pair);
+        sp.load(rec[n].steps);
+        op.load(o0 + t0 * S.ot, S.ot, rows);
     };
     const auto four = [&](const float* p, int it) { return *reinterpret_cast<const f4*>(p + 16 * it + 4 * grp); };
-    const auto leave = [&](St* to, const auto& f) {        // eight places of an operand's first part
-        pack<St, 8> o;
-        __builtin_memcpy(&o, &f, sizeof o);
-        o.store(to);
-    };
 
+    In8::clear(Kt, S.K);
+    In8::clear(Qt, S.K);
     fetch(S.chunks - 1);
     for (int64_t n = S.chunks - 1; n >= 0; n--) {
         __syncthreads();                   // the chunk after has been used
-        stage();
+#pragma unroll
+        for (int j = 0; j < In8::COUNT; j++) {
+            kp.put(Kt, j, length_up<St>(kr[j]), S.K);
+            qp.put(Qt, j, length_up<St>(qr[j]), S.K);
+        }
+        tp.put(Tt);
+        pp.put(Pt);
+        sp.put(st);
+        const int64_t t0 = n * C;
         f4 o[4];
 #pragma unroll
-        for (int j = 0; j < 16; j++) o[j / 4][j % 4] = float(op[j]);
+        for (int it = 0; it < 4; it++) {
+            o[it] = op.four(it, on);
+#pragma unroll
+            for (int r = 0; r < 4; r++) if (t0 + 16 * it + 4 * grp + r >= S.T) o[it][r] = 0.0f;
+        }
         __syncthreads();
         if (n) fetch(n - 1);
         const int64_t row = (bg * S.chunks + n) * S.vp + col;
+        const Scale ss = scale_of<St>(over_column(largest(s))), os = scale_of<St>(over_column(largest(o)));
         Frag<St, WIDE> sf[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; kb++) {
-            sf[kb] = frag_of<St, WIDE>(s[2 * kb], s[2 * kb + 1]);
-            if (col < S.vp) leave(left_over.states + row * DK + 32 * kb + 8 * grp, sf[kb]);
+            sf[kb] = frag_of<St, WIDE>(s[2 * kb], s[2 * kb + 1], ss.up);
+            if (held) leave(walked.states + row * DK + 32 * kb + 8 * grp, sf[kb]);
         }
         // dU = l K dS + P^T dO
-        Frag<St, WIDE> uf[2];
-        f4 u[4];
         Frag<St, 1> of[2];
 #pragma unroll
-        for (int kb = 0; kb < 2; kb++) of[kb] = frag_of<St, 1>(o[2 * kb], o[2 * kb + 1]);      // (exact: these are tensors' elements)
+        for (int kb = 0; kb < 2; kb++) of[kb] = frag_of<St, 1>(o[2 * kb], o[2 * kb + 1], os.up);       // (these are a tensor's elements: nothing is rounded off)
+        const float dp = os.down * (1.0f / SQUARE<St>);
+        f4 u[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) {
-            f4 x = {0, 0, 0, 0};
+            f4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) mma(x, Kt.rows(16 * it, kb), sf[kb]);
+#pragma unroll
+            for (int kb = it / 2; kb < 2; kb++) mma(y, Pt.cols(16 * it, kb), of[kb]);
             const f4 ls = four(st.l, it);
 #pragma unroll
-            for (int r = 0; r < 4; r++) u[it][r] = ls[r] == 0.0f ? 0.0f : ls[r] * x[r];
-#pragma unroll
-            for (int kb = it / 2; kb < 2; kb++) mma(u[it], Pt.cols(16 * it, kb), of[kb]);
-            if (it % 2) uf[it / 2] = frag_of<St, WIDE>(u[it - 1], u[it]);
+            for (int r = 0; r < 4; r++) u[it][r] = fmaf(dp, y[r], ls[r] == 0.0f ? 0.0f : ls[r] * (ss.down * x[r]));
         }
         // dR = T^T dU
-        Frag<St, WIDE> rf[2], qf[2];
+        const Scale us = scale_of<St>(over_column(largest(u)));
+        Frag<St, WIDE> uf[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++) uf[kb] = frag_of<St, WIDE>(u[2 * kb], u[2 * kb + 1], us.up);
+        const float du = us.down * (1.0f / SQUARE<St>);
         f4 d[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) {
             d[it] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int kb = it / 2; kb < 2; kb++) mma(d[it], Tt.cols(16 * it, kb), uf[kb]);
+            d[it] *= du;
         }
-        const int64_t t0 = n * C;
+        const Scale ds = scale_of<St>(over_column(largest(d)));
         E* to = d_value + ((b * S.T + t0) * S.G + g) * S.V + col;
+        f4 x[4], y[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) {
-            const f4 bs = four(st.b, it);
+            const f4 bs = four(st.b, it), bd = bs * d[it];
+            x[it] = four(st.q, it) * o[it];
+            y[it] = -four(st.x, it) * bd;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int i = 16 * it + 4 * grp + r;
-                if (on && t0 + i < S.T) to[int64_t(i) * S.G * S.V] = E(bs[r] * d[it][r]);
+                if (on && t0 + i < S.T) to[int64_t(i) * S.G * S.V] = E(bd[r]);
             }
         }
+        const Scale xs = scale_of<St>(over_column(fmaxf(largest(x), largest(y))));
+        Frag<St, WIDE> xf[2], yf[2];
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
-            f4 x[2], y[2];
-            const Frag<St, 1> df = frag_of<St, 1>(d[2 * kb], d[2 * kb + 1]);
-            if (col < S.vp) leave(left_over.steps + row * C + 32 * kb + 8 * grp, df);
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                x[j] = four(st.q, 2 * kb + j) * o[2 * kb + j];
-                y[j] = -(four(st.b, 2 * kb + j) * four(st.x, 2 * kb + j)) * d[2 * kb + j];
-            }
-            qf[kb] = frag_of<St, WIDE>(x[0], x[1]);
-            rf[kb] = frag_of<St, WIDE>(y[0], y[1]);
+            if (held) leave(walked.steps + row * C + 32 * kb + 8 * grp, frag_of<St, 1>(d[2 * kb], d[2 * kb + 1], ds.up));
+            xf[kb] = frag_of<St, WIDE>(x[2 * kb], x[2 * kb + 1], xs.up);
+            yf[kb] = frag_of<St, WIDE>(y[2 * kb], y[2 * kb + 1], xs.up);
+        }
+        if (held && grp == 0) {
+            float* scales = walked.scales + (bg * S.chunks + n) * 3 * S.vp + col;
+            scales[0] = ss.down;
+            scales[S.vp] = ds.down;
+            scales[2 * S.vp] = os.down;
         }
         const float end = st.end;
 #pragma unroll
         for (int k = 0; k < ND; k++) {
-#pragma unroll
-            for (int r = 0; r < 4; r++) s[k][r] = end == 0.0f ? 0.0f : end * s[k][r];
+            f4 z = {0, 0, 0, 0};
 #pragma unroll
             for (int kb = 0; kb < 2; kb++) {
-                mma(s[k], Qt.cols(16 * k, kb), qf[kb]);
-                mma(s[k], Kt.cols(16 * k, kb), rf[kb]);
+                mma(z, Qt.cols(16 * k, kb), xf[kb]);
+                mma(z, Kt.cols(16 * k, kb), yf[kb]);
             }
+#pragma unroll
+            for (int r = 0; r < 4; r++) s[k][r] = fmaf(xs.down, z[r], end == 0.0f ? 0.0f : end * s[k][r]);
         }
     }
     if (!d_state) return;
@@ -208,14 +190,18 @@ __global__ __launch_bounds__(W * WAVE) void walk_kernel(const E* __restrict__ qu
 
 // ---- gradient_kernel: a workgroup of four waves for each chunk of each query and key head. A wave has 16 steps' rows of every product;
 // columns of values are summed over in blocks of 32, staged while the block before is used.
+//
+// Five products are summed over columns of values, whose operands have a scale for each column. The two scales of a column go to the
+// left operand, over the largest of them: what they push below float16's numbers is that far below the sum's largest terms.
 
-constexpr int BLOCK_V = 32;
+constexpr int BLOCK_V = 32, PRODUCTS = 5;
 
 __device__ inline float row16(float x) {   // a sum over the 16 lanes that have a row's columns
 #pragma unroll
     for (int d = 1; d < 16; d <<= 1) x += __shfl_xor(x, d, WAVE);
     return x;
 }
+__device__ inline int exponent(float x) { return int(__float_as_uint(x) >> 23) - 127; }
 
 template <typename E, int DK>
 __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ query, const E* __restrict__ key, const E* __restrict__ gate, const E* __restrict__ write,
@@ -223,16 +209,20 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
                                                          const Kept<typename Rep<E>::S> kept, const Kept<typename Rep<E>::S> walked, E* __restrict__ d_query,
                                                          E* __restrict__ d_key, E* __restrict__ d_gate, E* __restrict__ d_write) {
     using St = typename Rep<E>::S;
+    constexpr bool HALF = sizeof(St) == 2;
     constexpr int ND = DK / 16, KB = DK / 32, PER = DK / 8;
     using In = Tile<St, C, DK>;
     using Ot = Tile<St, C, BLOCK_V>;
     using Sv = Tile<St, BLOCK_V, DK>;
     using Uv = Tile<St, BLOCK_V, C>;
     using Square = Tile<St, C, C>;
+    using In8 = Rows<E, DK, BLOCK>;
     constexpr int STAGED = Ot::SIZE + 2 * Sv::SIZE + 2 * Uv::SIZE, MORE = STAGED > 3 * Square::SIZE ? STAGED : 3 * Square::SIZE;
     __shared__ alignas(16) St lds[2 * In::SIZE + MORE];
     __shared__ alignas(16) Steps st;
+    __shared__ alignas(16) St factors[PRODUCTS][BLOCK_V];
     __shared__ float rows[C], columns[WAVES][C], left[C], whole[WAVES], writes[C];
+    __shared__ int tops[WAVES][PRODUCTS];
     const In Kt{lds}, Qt{lds + In::SIZE};
     St* const more = lds + 2 * In::SIZE;
     const Ot Od{more};
@@ -243,17 +233,30 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
     const int64_t chunk = blockIdx.x % S.chunks, bh = blockIdx.x / S.chunks;
     const int64_t b = bh / S.H, t0 = chunk * C;
     const int h = int(bh % S.H), share = S.G / S.H, steps = int(S.T - t0 < C ? S.T - t0 : C);
-    const E *q0 = query + b * S.qb + t0 * S.qt + h * S.qh, *k0 = key + b * S.kb + t0 * S.kt + h * S.kh;
-    for (int p = tid; p < C * PER; p += BLOCK) {
-        const int i = p / PER, c = p % PER * 8, n = i < steps ? S.K - c : 0;
-        Eight<E> q, k;
-        q.load(q0 + i * S.qt + c, n);
-        k.load(k0 + i * S.kt + c, n);
-        q.put(Qt, i, c);
-        k.put(Kt, i, c);
+    // products of E and F with keys and queries, over numbers of values each
+    const int many = HALF ? 32 - __builtin_clz(S.V) : 0;
+    const float few = __uint_as_float((127 - many) << 23);
+    {
+        In8 q, k;
+        float qr[In8::COUNT], kr[In8::COUNT];
+        const Steps& first = records[(b * S.G + h * share) * S.chunks + chunk].steps;
+        q.load(query + b * S.qb + t0 * S.qt + h * S.qh, S.qt, steps, S.K);
+        k.load(key + b * S.kb + t0 * S.kt + h * S.kh, S.kt, steps, S.K);
+#pragma unroll
+        for (int j = 0; j < In8::COUNT; j++) {
+            kr[j] = first.rk[In8::row(j)];
+            qr[j] = first.rq[In8::row(j)];
+        }
+        In8::clear(Qt, S.K);
+        In8::clear(Kt, S.K);
+#pragma unroll
+        for (int j = 0; j < In8::COUNT; j++) {
+            q.put(Qt, j, length_up<St>(qr[j]), S.K);
+            k.put(Kt, j, length_up<St>(kr[j]), S.K);
+        }
     }
     const f4 zero = {0, 0, 0, 0};
-    f4 tq[ND], tk[ND];                     // the gradients of the query and the key, over the value heads so far
+    f4 tq[ND], tk[ND];                     // the gradients of the query and the key of length 1, over the value heads so far
 #pragma unroll
     for (int n = 0; n < ND; n++) tq[n] = tk[n] = zero;
 
@@ -262,6 +265,28 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
         const int64_t at = (b * S.G + g) * S.chunks + chunk;
         const E* o0 = d_out + b * S.ob + t0 * S.ot + g * S.og;
         const St *s0 = kept.states + at * S.vp * DK, *s1 = walked.states + at * S.vp * DK, *u0 = kept.steps + at * S.vp * C, *r0 = walked.steps + at * S.vp * C;
+        const float *f0 = kept.scales + at * 3 * S.vp, *f1 = walked.scales + at * 3 * S.vp;    // of S, U and of dS, dR, dO
+        const auto left_scale = [&](int p, int c) { return p == 2 ? f0[S.vp + c] : p == 0 || p == 3 ? f1[2 * S.vp + c] : f1[S.vp + c]; };
+        const auto right_scale = [&](int p, int c) { return p < 2 ? f0[c] : p == 2 ? f1[c] : f0[S.vp + c]; };
+        if constexpr (HALF) {              // the largest of the columns' scales, by product: dO S, dR S, U dS, dO U, dR U
+            int top[PRODUCTS];
+#pragma unroll
+            for (int p = 0; p < PRODUCTS; p++) top[p] = -1000;
+            for (int c = tid; c < S.vp; c += BLOCK) {
+                const int es = exponent(f0[c]), eu = exponent(f0[S.vp + c]), ed = exponent(f1[c]), er = exponent(f1[S.vp + c]), eo = exponent(f1[2 * S.vp + c]);
+                top[0] = max(top[0], eo + es);
+                top[1] = max(top[1], er + es);
+                top[2] = max(top[2], eu + ed);
+                top[3] = max(top[3], eo + eu);
+                top[4] = max(top[4], er + eu);
+            }
+#pragma unroll
+            for (int p = 0; p < PRODUCTS; p++) {
+#pragma unroll
+                for (int d = WAVE / 2; d; d >>= 1) top[p] = max(top[p], __shfl_xor(top[p], d, WAVE));
+                if (l == 0) tops[wave][p] = top[p];
+            }
+        }
         f4 aq[ND], from[ND], to[ND], dp[WAVES], da[WAVES];
 #pragma unroll
         for (int n = 0; n < ND; n++) aq[n] = from[n] = to[n] = zero;
@@ -269,36 +294,69 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
         for (int n = 0; n < WAVES; n++) dp[n] = da[n] = zero;
         float both = 0.0f;                 // of state and gradient, summed over all elements
         constexpr int SP = BLOCK_V * PER / BLOCK ? BLOCK_V * PER / BLOCK : 1;
-        Eight<E> op;
+        pack<E, 8> op;
+        pack<float, 8> os;
         pack<St, 8> s0p[SP], s1p[SP], up, rp;
+        float sd[SP], lf, rf;
+        // (columns behind the last are read as the last one and put as 0; d_out's last eight one by one where V is no multiple of 8)
+        const int oc = tid % 4 * 8, orow = tid / 4, urow = tid / 8, ucol = tid % 8 * 8;
+        const E* orow0 = o0 + int64_t(orow < steps ? orow : steps - 1) * S.ot;
+        const auto last = [&](int c) { return c < S.vp ? c : S.vp - 1; };
         auto fetch = [&](int v0) {
-            op.load(o0 + (tid / 4) * S.ot + v0 + tid % 4 * 8, tid / 4 < steps ? S.V - v0 - tid % 4 * 8 : 0);
-            const int v = v0 + tid / 8;
-            const auto some = [](const St* p, bool on) { return on ? pack<St, 8>::load(p) : pack<St, 8>::load_part(p, 0); };
-            up = some(u0 + int64_t(v) * C + tid % 8 * 8, v < S.vp);
-            rp = some(r0 + int64_t(v) * C + tid % 8 * 8, v < S.vp);
+            if (S.V % 8 == 0) {
+                op = pack<E, 8>::load(orow0 + (v0 + oc < S.V ? v0 + oc : S.V - 8));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) op.v[e] = orow0[v0 + oc + e < S.V ? v0 + oc + e : S.V - 1];
+            }
+            if constexpr (HALF) {
+                os = pack<float, 8>::load(f1 + 2 * S.vp + (v0 + oc < S.vp ? v0 + oc : S.vp - 8));
+                lf = left_scale(tid / BLOCK_V < PRODUCTS ? tid / BLOCK_V : 0, last(v0 + tid % BLOCK_V));
+                rf = right_scale(tid / BLOCK_V < PRODUCTS ? tid / BLOCK_V : 0, last(v0 + tid % BLOCK_V));
+            }
+            up = pack<St, 8>::load(u0 + int64_t(last(v0 + urow)) * C + ucol);
+            rp = pack<St, 8>::load(r0 + int64_t(last(v0 + urow)) * C + ucol);
 #pragma unroll
             for (int k = 0; k < SP; k++) {
-                const int p = tid + k * BLOCK, c = v0 + p / PER;
-                const bool on = p < BLOCK_V * PER && c < S.vp;
-                s0p[k] = some(s0 + int64_t(c) * DK + p % PER * 8, on);
-                s1p[k] = some(s1 + int64_t(c) * DK + p % PER * 8, on);
+                const int p = tid + k * BLOCK, c = last(v0 + p / PER);
+                s0p[k] = pack<St, 8>::load(s0 + int64_t(c) * DK + p % PER * 8);
+                s1p[k] = pack<St, 8>::load(s1 + int64_t(c) * DK + p % PER * 8);
+                if constexpr (HALF) sd[k] = f0[c] * f1[c];
+                else sd[k] = 1.0f;
             }
         };
         fetch(0);
         for (int v0 = 0; v0 < S.vp; v0 += BLOCK_V) {
             __syncthreads();               // what lies there has been used
-            op.put(Od, tid / 4, tid % 4 * 8);
-            Us.put_places(tid / 8, tid % 8 * 8, up);
-            Rs.put_places(tid / 8, tid % 8 * 8, rp);
+            {
+                St x[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float d = v0 + oc + e < S.V ? float(op.v[e]) : 0.0f;
+                    x[e] = St(HALF ? d * __uint_as_float((254u << 23) - __float_as_uint(os.v[e])) : d);    // (over a power of two)
+                }
+                Od.put(orow, oc, x);
+            }
+            if constexpr (HALF) if (tid < PRODUCTS * BLOCK_V) {
+                const int p = tid / BLOCK_V, c = tid % BLOCK_V;
+                const int top = max(max(tops[0][p], tops[1][p]), max(tops[2][p], tops[3][p]));
+                const int e = exponent(lf) + exponent(rf) - top;   // 0 at most
+                factors[p][place(c)] = v0 + c < S.vp && e > -25 ? St(__uint_as_float((127 + e) << 23)) : St(0.0f);
+            }
+            const pack<St, 8> none = {};
+            Us.put_places(urow, ucol, v0 + urow < S.vp ? up : none);
+            Rs.put_places(urow, ucol, v0 + urow < S.vp ? rp : none);
 #pragma unroll
             for (int k = 0; k < SP; k++) {
                 const int p = tid + k * BLOCK;
                 if (p < BLOCK_V * PER) {
-                    S0.put_places(p / PER, p % PER * 8, s0p[k]);
-                    S1.put_places(p / PER, p % PER * 8, s1p[k]);
+                    const bool on = v0 + p / PER < S.vp;
+                    S0.put_places(p / PER, p % PER * 8, on ? s0p[k] : none);
+                    S1.put_places(p / PER, p % PER * 8, on ? s1p[k] : none);
+                    float x = 0.0f;
 #pragma unroll
-                    for (int c = 0; c < 8; c++) both = fmaf(float(s0p[k].v[c]), float(s1p[k].v[c]), both);
+                    for (int c = 0; c < 8; c++) x = fmaf(float(s0p[k].v[c]), float(s1p[k].v[c]), x);
+                    if (on) both = fmaf(x, sd[k], both);
                 }
             }
             if (v0 == 0) {                 // the steps' record with the first block
@@ -307,50 +365,57 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
             }
             __syncthreads();
             if (v0 + BLOCK_V < S.vp) fetch(v0 + BLOCK_V);
+            const auto scaled = [&](auto f, int p) {
+                if constexpr (HALF) f.p[0] *= *reinterpret_cast<const h8*>(&factors[p][8 * grp]);
+                return f;
+            };
             const auto of = Od.rows(band, 0);
             const auto rf = Rs.cols(band, 0), uf = Us.cols(band, 0);
+            const auto of0 = scaled(of, 0), rf1 = scaled(rf, 1), uf2 = scaled(uf, 2), of3 = scaled(of, 3), rf4 = scaled(rf, 4);
 #pragma unroll
             for (int n = 0; n < ND; n++) {
                 const auto sf = S0.cols(16 * n, 0);
-                mma(aq[n], of, sf);
-                mma(from[n], rf, sf);
-                mma(to[n], uf, S1.cols(16 * n, 0));
+                mma(aq[n], of0, sf);
+                mma(from[n], rf1, sf);
+                mma(to[n], uf2, S1.cols(16 * n, 0));
             }
 #pragma unroll
             for (int n = 0; n < WAVES; n++) if (n <= wave) {
                 const auto un = Us.cols(16 * n, 0);
-                mma(dp[n], of, un);
-                mma(da[n], rf, un);
+                mma(dp[n], of3, un);
+                mma(da[n], rf4, un);
             }
         }
+        int top[PRODUCTS];
+#pragma unroll
+        for (int p = 0; p < PRODUCTS; p++) top[p] = HALF ? max(max(tops[0][p], tops[1][p]), max(tops[2][p], tops[3][p])) : 0;
         const uint64_t cuts = uint64_t(st.cut[1]) << 32 | st.cut[0];
         // what a step has of the state before the chunk and leaves after it, and its row's sums
-        float gi[4], li[4], bi[4], rowsum[4], rki[4], rqi[4];
+        float bi[4], rowsum[4], rki[4], rqi[4];
         const float last_hi = st.hi[C - 1], last_lo = st.lo[C - 1];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int i = band + 4 * grp + r;
-            gi[r] = since(cuts, i) >= 0 ? 0.0f : expf(st.hi[i]);
-            li[r] = i < since(cuts, C - 1) ? 0.0f : expf((last_hi - st.hi[i]) + (last_lo - st.lo[i]));
+            const float gi = since(cuts, i) >= 0 ? 0.0f : expf(st.hi[i]);
+            const float li = i < since(cuts, C - 1) ? 0.0f : expf((last_hi - st.hi[i]) + (last_lo - st.lo[i]));
             bi[r] = st.b[i];
-            rki[r] = st.rk[i];
-            rqi[r] = st.rq[i];
+            rki[r] = length_rest<St>(st.rk[i]);
+            rqi[r] = length_rest<St>(st.rq[i]);
             float dq = 0.0f, df = 0.0f, dt = 0.0f;
 #pragma unroll
             for (int n = 0; n < ND; n++) {
+                const float x = gi == 0.0f ? 0.0f : gi * ldexpf(aq[n][r], top[0]), y = gi == 0.0f ? 0.0f : -bi[r] * gi * ldexpf(from[n][r], top[1]);
+                const float z = li == 0.0f ? 0.0f : li * ldexpf(to[n][r], top[2]);
                 const float q = float(Qt.get(i, 16 * n + m)), k = float(Kt.get(i, 16 * n + m));
-                dq = fmaf(q, aq[n][r], dq);
-                df = fmaf(k, from[n][r], df);
-                dt = fmaf(k, to[n][r], dt);
+                dq = fmaf(q, x, dq);
+                df = fmaf(k, y, df);
+                dt = fmaf(k, z, dt);
+                tq[n][r] += x;
+                tk[n][r] += y + z;
             }
-            rowsum[r] = (gi[r] == 0.0f ? 0.0f : gi[r] * (rqi[r] * dq - bi[r] * rki[r] * df));
+            rowsum[r] = rqi[r] * dq + rki[r] * df;
             dt = row16(dt);
-            if (m == 0) left[i] = li[r] == 0.0f ? 0.0f : li[r] * rki[r] * dt;
-#pragma unroll
-            for (int n = 0; n < ND; n++) {
-                tq[n][r] += gi[r] == 0.0f ? 0.0f : gi[r] * aq[n][r];
-                tk[n][r] += (li[r] == 0.0f ? 0.0f : li[r] * to[n][r]) - (gi[r] == 0.0f ? 0.0f : bi[r] * gi[r] * from[n][r]);
-            }
+            if (m == 0) left[i] = rki[r] * dt;
         }
         f4 kk[WAVES], qk[WAVES];
 #pragma unroll
@@ -372,7 +437,7 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
 #pragma unroll
         for (int n = 0; n < WAVES; n++) {
             const int c = 16 * n + m;
-            const float rk = st.rk[c], hi = st.hi[c], lo = st.lo[c];
+            const float rk = length_rest<St>(st.rk[c]), hi = st.hi[c], lo = st.lo[c];
             float column = 0.0f;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
@@ -384,13 +449,17 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
                     e = M * dp[n][r];
                     if (c < i) {
                         f = -M * bi[r] * da[n][r];
-                        const float pair = e * rqi[r] * rk * qk[n][r] + f * rki[r] * rk * kk[n][r];
+                        const float pair = ldexpf(e * rqi[r] * rk * qk[n][r], top[3]) + ldexpf(f * rki[r] * rk * kk[n][r], top[4]);
                         rowsum[r] += pair;
                         column += pair;
                     } else {
-                        writes[i] = da[n][r];
+                        writes[i] = ldexpf(da[n][r], top[4]);
                     }
                 }
+                // (numbers up to 2^28 V, of factors up to 2^14: V 2^14 of them, and lengths, are taken out)
+                constexpr float FIT = HALF ? 0x1p-15f * LONG<St> : 1.0f;
+                e *= few * FIT;
+                f *= few * FIT;
                 Ek.p[i * Square::ROW + place(c)] = St(e * rk);
                 Eq.p[i * Square::ROW + place(c)] = St(e * rqi[r]);
                 if (c <= i) {
@@ -408,15 +477,22 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
             if (m == 0) rows[band + 4 * grp + r] = x;
         }
         __syncthreads();
+        constexpr int OUT = HALF ? 15 - 6 : 0;             // (what FIT took out)
+        static_assert(!HALF || LONG<St> == 64.0f, "the exponent of LONG");
 #pragma unroll
-        for (int kb = 0; kb < 2; kb++) {
-            const auto ek = Ek.rows(band, kb), eq = Eq.cols(band, kb), ff = Ff.rows(band, kb);
+        for (int n = 0; n < ND; n++) {
+            f4 x = zero, y = zero, z = zero;
 #pragma unroll
-            for (int n = 0; n < ND; n++) {
+            for (int kb = 0; kb < 2; kb++) {
                 const auto kn = Kt.cols(16 * n, kb);
-                mma(tq[n], ek, kn);
-                mma(tk[n], ff, kn);
-                mma(tk[n], eq, Qt.cols(16 * n, kb));
+                mma(x, Ek.rows(band, kb), kn);
+                mma(y, Eq.cols(band, kb), Qt.cols(16 * n, kb));
+                mma(z, Ff.rows(band, kb), kn);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                tq[n][r] += ldexpf(x[r], top[3] + many + OUT);
+                tk[n][r] += ldexpf(y[r], top[3] + many + OUT) + ldexpf(z[r], top[4] + many + OUT);
             }
         }
         if (wave == 0) {                   // a lane for each step: gates
@@ -448,12 +524,12 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
 #pragma unroll
     for (int r = 0; r < 4; r++) {
         const int i = band + 4 * grp + r;
-        const float rk = st.rk[i], rq = st.rq[i];
+        const float rk = st.rk[i], rq = st.rq[i], rkr = length_rest<St>(rk), rqr = length_rest<St>(rq);
         float q[ND], k[ND], dq = 0.0f, dk = 0.0f;
 #pragma unroll
         for (int n = 0; n < ND; n++) {
-            q[n] = float(Qt.get(i, 16 * n + m)) * rq;
-            k[n] = float(Kt.get(i, 16 * n + m)) * rk;
+            q[n] = float(Qt.get(i, 16 * n + m)) * rqr;
+            k[n] = float(Kt.get(i, 16 * n + m)) * rkr;
             dq = fmaf(q[n], tq[n][r], dq);
             dk = fmaf(k[n], tk[n][r], dk);
         }
