@@ -408,24 +408,24 @@ int32_t pv_add_rms_norm_backward_hip(const void* s, const float* rstd, const flo
  *   u = b (value[t] - a S[t-1]^T key[t]),  S[t] = a S[t-1] + key[t] u^T,  out[t] = S[t]^T query[t].
  * query, key: [B, T, H, K], value: [B, T, G, V], gate, write: [B, T, G], all of `dtype`; G is a multiple of H, and value head g
  * goes with query and key head g / (G / H). strides: host array of 15, in elements: of a sequence, a step and a head of query, key,
- * value, gate, write in turn; a step's at most 2^24. B, T, H >= 1, K <= 128, V <= 65,536; of 64 steps of a value head's sequence,
+ * value, gate, write in turn; a step's at most 2^22. B, T, H >= 1, K <= 128, V <= 65,536, H K and G V at
+ * most 2^22; of 64 steps of a value head's sequence,
  * and of 32 columns of a state, there are fewer than 2^24. Squares of a key's or query's length are within float32.
  * state: f32[B, G, K, V] before step 0, or NULL: zero. reset: u8[B, T], or NULL; where not 0, S[t-1] is dropped. out: [B, T, G, V] of
  * `dtype`; last: f32[B, G, K, V] = S[T-1], apart from state. For the backward pass: kept (pv_gated_delta_kept_bytes, 16-byte
  * aligned; NULL: none) and what the call leaves in `work`. work: pv_gated_delta_work_bytes with keep = 1 if kept is given, else 0. */
-uint64_t pv_gated_delta_work_bytes(int64_t B, int64_t T, int32_t G, int32_t dtype, int32_t keep);
+uint64_t pv_gated_delta_work_bytes(int64_t B, int64_t T, int32_t H, int32_t G, int32_t K, int32_t dtype, int32_t keep);
 uint64_t pv_gated_delta_kept_bytes(int64_t B, int64_t T, int32_t G, int32_t K, int32_t V, int32_t dtype);
 int32_t pv_gated_delta_hip(const void* query, const void* key, const void* value, const void* gate, const void* write, const float* state, const uint8_t* reset,
                            int64_t B, int64_t T, int32_t H, int32_t G, int32_t K, int32_t V, const int64_t* strides, float eps, int32_t dtype, void* out, float* last,
                            void* kept, void* work, uint64_t work_bytes, void* stream, char* err, size_t errcap);
 
-/* Its gradients from d_out ([B, T, G, V] of `dtype`, its strides behind the others: 18) and d_last (f32[B, G, K, V], or NULL: zero), with
- * kept and records, the forward call's work, as that call left them: d_query, d_key, d_value, d_gate, d_write like the tensors, of
+/* Its gradients from d_out ([B, T, G, V] of `dtype`; strides: 9, of gate, write and d_out) and d_last (f32[B, G, K, V], or NULL: zero),
+ * with kept and records, the forward call's work, as that call left them: d_query, d_key, d_value, d_gate, d_write like the tensors, of
  * `dtype` and without gaps, and d_state (f32[B, G, K, V], or NULL). work: pv_gated_delta_kept_bytes. */
-int32_t pv_gated_delta_backward_hip(const void* query, const void* key, const void* gate, const void* write, const void* d_out, const float* d_last, int64_t B,
-                                    int64_t T, int32_t H, int32_t G, int32_t K, int32_t V, const int64_t* strides, float eps, int32_t dtype, const void* kept,
-                                    const void* records, void* d_query, void* d_key, void* d_value, void* d_gate, void* d_write, float* d_state, void* work,
-                                    uint64_t work_bytes, void* stream, char* err, size_t errcap);
+int32_t pv_gated_delta_backward_hip(const void* gate, const void* write, const void* d_out, const float* d_last, int64_t B, int64_t T, int32_t H, int32_t G, int32_t K,
+                                    int32_t V, const int64_t* strides, int32_t dtype, const void* kept, const void* records, void* d_query, void* d_key, void* d_value,
+                                    void* d_gate, void* d_write, float* d_state, void* work, uint64_t work_bytes, void* stream, char* err, size_t errcap);
 
 /* Dropout. Element i of a call is dropped where its 16 bits are below round(p 2^16), 0 <= p <= 1, and else multiplied by
  * 2^16 / (2^16 - round(p 2^16)). The bits are word (i / 2) % 4, half i % 2 (the low one first) of the ten-round generator of four

@@ -24,7 +24,7 @@ namespace pvd {
 using namespace pvo;
 
 constexpr int C = 64;                      // steps of a chunk
-constexpr int MAX_K = 128;
+constexpr int MAX_K = 128, MAX_STEP = 1 << 22;
 
 using f4 = __attribute__((ext_vector_type(4))) float;
 using h8 = __attribute__((ext_vector_type(8))) _Float16;
@@ -70,6 +70,10 @@ template <int N> __device__ inline float largest(const f4 (&v)[N]) {
         for (int r = 0; r < 4; r++) x = fmaxf(x, fabsf(v[n][r]));
     return x;
 }
+
+// Nothing is moved across: the loads before it are in flight while what comes after it runs. (Left to itself the compiler puts each
+// load of an operand right before its product, and a wave that is alone on its SIMD waits for every one.)
+__device__ inline void fence() { __builtin_amdgcn_sched_barrier(0); }
 
 template <typename S, int PARTS> struct Frag;
 template <int PARTS> struct Frag<f16, PARTS> { h8 p[PARTS]; };
@@ -153,8 +157,6 @@ template <typename S_, int ROWS, int COLS, int PARTS = 1> struct Tile {
         return f;
     }
     __device__ Frag<S, 1> cols_narrow(int c0, int kb) const { return Tile<S, ROWS, COLS, 1>{p}.cols(c0, kb); }
-    // eight neighbouring places of a row, in the first part
-    __device__ void put_places(int row, int at, const pack<S, 8>& v) const { v.store(p + row * ROW + at); }
     __device__ S get(int row, int c) const { return p[row * ROW + place(c)]; }
     // eight neighbouring columns of a row, c a multiple of 8
     __device__ void put(int row, int c, const S (&v)[8]) const {
@@ -168,27 +170,68 @@ template <typename S_, int ROWS, int COLS, int PARTS = 1> struct Tile {
     }
 };
 
-// Rows of queries or keys on their way from memory to a tile of 64 x DK, eight elements a lane. No load depends on a branch that
-// lanes take differently, as it would be waited for there: steps past the last are read as the last one (they have length 0, and
-// their elements come out as 0), elements past a row's end are not read, and its last eight are read as they lie, where K is no
-// multiple of 8, and put one by one.
+// A run of memory whose loads from behind its end are 0, and whose stores there are dropped: lanes that have nothing there take part
+// all the same, so that no wave branches on it (a branch around a store or a load makes the next wait one for everything in flight).
+constexpr uint32_t NOWHERE = 0x80000000u;
+struct Buffer {
+    __amdgpu_buffer_rsrc_t r;
+    __device__ Buffer(const void* base, int64_t bytes) : r(__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, int(bytes), 0x00027000)) {}
+    template <typename T> __device__ T load(uint32_t at, int more = 0) const {
+        T v;
+        if constexpr (sizeof(T) == 2) { const auto x = __builtin_amdgcn_raw_buffer_load_b16(r, at, more, 0); __builtin_memcpy(&v, &x, 2); }
+        if constexpr (sizeof(T) == 4) { const auto x = __builtin_amdgcn_raw_buffer_load_b32(r, at, more, 0); __builtin_memcpy(&v, &x, 4); }
+        if constexpr (sizeof(T) >= 16) {
+            char* to = reinterpret_cast<char*>(&v);
+#pragma unroll
+            for (int k = 0; k < int(sizeof(T)); k += 16) {
+                const auto x = __builtin_amdgcn_raw_buffer_load_b128(r, at + k, more, 0);
+                __builtin_memcpy(to + k, &x, 16);
+            }
+        }
+        return v;
+    }
+    template <typename T> __device__ void store(const T& v, uint32_t at, int more = 0) const {
+        if constexpr (sizeof(T) == 2) { uint16_t x; __builtin_memcpy(&x, &v, 2); __builtin_amdgcn_raw_buffer_store_b16(x, r, at, more, 0); }
+        if constexpr (sizeof(T) == 4) { uint32_t x; __builtin_memcpy(&x, &v, 4); __builtin_amdgcn_raw_buffer_store_b32(x, r, at, more, 0); }
+        if constexpr (sizeof(T) >= 16) {
+            const char* from = reinterpret_cast<const char*>(&v);
+#pragma unroll
+            for (int k = 0; k < int(sizeof(T)); k += 16) {
+                __attribute__((ext_vector_type(4))) uint32_t x;
+                __builtin_memcpy(&x, from + k, 16);
+                __builtin_amdgcn_raw_buffer_store_b128(x, r, at + k, more, 0);
+            }
+        }
+    }
+};
+// `rows` rows of `n` elements of E, `stride` apart
+template <typename E> __device__ inline Buffer rows_at(const E* at, int stride, int rows, int n) {
+    return Buffer(at, (int64_t(rows - 1) * stride + n) * int64_t(sizeof(E)));
+}
+
+// Rows of queries or keys on their way from memory to a tile of 64 x DK, eight elements a lane. Steps past the last come out as 0 (or,
+// where strides make steps overlap, as an earlier one's; their lengths are 0 in either case). A row's last eight are read as they
+// lie, where K is no multiple of 8, and put one by one.
 template <typename E, int DK, int THREADS> struct Rows {
     using S = typename Rep<E>::S;
-    static constexpr int PER = DK / 8, COUNT = C * PER / THREADS;
+    static constexpr int PER = DK / 8, COUNT = C * PER / THREADS, STEP = THREADS / PER;
     pack<E, 8> v[COUNT];
     static __device__ int column(int K) {                  // of the lane's first element
         const int c = threadIdx.x % PER * 8;
         return c + 8 <= K ? c : K >= 8 ? K - 8 : 0;
     }
-    static __device__ int row(int j) { return (threadIdx.x + j * THREADS) / PER; }
-    __device__ void load(const E* at, int64_t stride, int rows, int K) {
-        const int c = column(K);
+    static __device__ int row(int j) { return threadIdx.x / PER + j * STEP; }
+    __device__ void load(const E* at, int stride, int rows, int K) {
+        const Buffer from = rows_at(at, stride, rows, K);
+        const uint32_t off = (row(0) * stride + column(K)) * int(sizeof(E));
         if (K >= 8) {
 #pragma unroll
-            for (int j = 0; j < COUNT; j++) v[j] = pack<E, 8>::load(at + (row(j) < rows ? row(j) : rows - 1) * stride + c);
+            for (int j = 0; j < COUNT; j++) v[j] = from.load<pack<E, 8>>(off, j * STEP * stride * int(sizeof(E)));
         } else {
 #pragma unroll
-            for (int j = 0; j < COUNT; j++) v[j] = pack<E, 8>::load_part(at + (row(j) < rows ? row(j) : rows - 1) * stride, K);
+            for (int j = 0; j < COUNT; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[j].v[e] = from.load<E>(e < K ? off + e * uint32_t(sizeof(E)) : NOWHERE, j * STEP * stride * int(sizeof(E)));
         }
     }
     __device__ float square(int j, int K) const {          // of the lane's own elements, none of them a neighbour's too
@@ -226,15 +269,14 @@ template <typename E, int DK, int THREADS> struct Rows {
 struct Shape {
     int64_t B, T;
     int32_t H, G, K, V;
-    int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh;            // query, key, value: of a sequence, a step, a head
-    int64_t ab, at, ag, wb, wt, wg;                        // gate, write: of a sequence, a step, a head
-    int64_t ob, ot, og;                                    // d_out
+    int64_t qb, qh, kb, kh, vb, vh, ab, ag, wb, wg, ob, og;        // query, key, value, gate, write, d_out: of a sequence, a head
+    int32_t qt, kt, vt, at, wt, ot;                        // and of a step
     int64_t chunks;                                        // of T
-    int32_t vp;                                            // V up to a multiple of 16
+    int32_t vp;                                            // V up to a multiple of 32
     float eps;
 };
 
-// What is known of a chunk's steps before its state is: one record for each chunk of each value head.
+// What is known of a chunk's steps before its state is:
 //   x     g r: g what a step keeps of the state before the chunk (0 past a reset), r what is left of one over the key's length
 //   b     sigmoid(write)
 //   l     l r: l what is left of a step's addition at the chunk's end
@@ -245,10 +287,39 @@ struct Steps {
     float end;
     uint32_t cut[2], unused;
 };
-template <typename S> struct Chunk {
-    S inv[wide_of<S>][C][C], pair[wide_of<S>][C][C];       // (I + A)^-1 and M q k^T, times SQUARE, columns at their places
+
+// What one kernel leaves another lies in memory as it will lie in LDS, padding and all, and is copied there past the registers:
+//   a record for each chunk of each value head: its steps, (I + A)^-1 and M q k^T, times SQUARE;
+//   an image for each chunk of each key head: keys and queries.
+template <typename S> struct Record {
+    static constexpr int PAD = 16 / sizeof(S);
     Steps steps;
+    S inv[wide_of<S>][C][C + PAD], pair[wide_of<S>][C][C + PAD];
+    static constexpr int ALL = 2080 + 2 * wide_of<S> * C * (C + PAD) * int(sizeof(S));
+    static constexpr int NARROW = ALL - (wide_of<S> - 1) * C * (C + PAD) * int(sizeof(S));     // without the second part of M q k^T
+    static constexpr int STRIDE = (ALL + 1023) / 1024 * 1024;
 };
+template <typename S, int DK> constexpr int IMAGE = (2 * Tile<S, C, DK>::SIZE * int(sizeof(S)) + 1023) / 1024 * 1024;
+inline uint64_t image_bytes(int32_t dk, int32_t dtype) { return (2 * 64 * (dtype == PV_F32 ? (dk + 4) * 4 : (dk + 8) * 2) + 1023) / 1024 * 1024; }
+template <typename S> __device__ __host__ inline char* record_of(char* work, int64_t chunk) { return work + chunk * Record<S>::STRIDE; }
+
+// `bytes` of memory to LDS, by all W waves, 1,024 at a time (those behind the last whole kilobyte too, up to the next). Both begin at
+// 16 bytes' alignment. The lanes' data goes from the memory system to LDS by itself: bring() returns at once, and the memory is there
+// for a wave's own reads after arrived<N>(), N at most the number of its loads and stores since, and for the workgroup's after a barrier.
+template <int W> __device__ inline void bring(const void* from, void* to, int bytes) {
+    const uint64_t base = reinterpret_cast<uint64_t>(from);
+    const int last = (bytes + 1023) / 1024 - 1;
+    const __attribute__((ext_vector_type(4))) int r = {__builtin_amdgcn_readfirstlane(int(base)), __builtin_amdgcn_readfirstlane(int(base >> 32)), (last + 1) * 1024,
+                                                               0x00027000};
+    const uint32_t lds = __builtin_amdgcn_readfirstlane(int(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)to)));
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    for (int k = 0; k <= last; k += W) {   // (a wave without a kilobyte of its own copies the last one once more)
+        const int at = (k + wave < last ? k + wave : last) * 1024;
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds + at), "v"(threadIdx.x % WAVE * 16), "s"(r), "s"(at)
+                     : "memory", "m0");
+    }
+}
+template <int N> __device__ inline void arrived() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 // Steps that a record's cut lets through: whether step j's addition is still there at step i >= j
 __device__ inline int since(uint64_t cut, int i) {         // the last step up to i that drops the state, or -1
@@ -257,85 +328,68 @@ __device__ inline int since(uint64_t cut, int i) {         // the last step up t
 }
 
 // What the forward pass keeps for the backward pass, and what the walk backwards leaves for the gradients: arrays of the same
-// shapes, for a chunk of a value head. By columns of the state or of values, vp of them:
-//   states   [vp][DK]: S before the chunk, or the gradient of S after it; rows at their places
-//   steps    [vp][64]: U, or the gradient of b D; steps at their places
-//   scales   [3][vp]: what the columns of states, of steps, and (backwards) of the gradient of out are to be multiplied by
-template <typename S> struct Kept {
-    S *states, *steps;
+// shapes, for a chunk of a value head, in blocks of 32 columns of the state or of values. A block is, as it will lie in LDS,
+//   states   [32][DK + padding]: S before the chunk, or the gradient of S after it, by columns, rows at their places
+//   steps    [32][64 + padding]: U, or the gradient of b D; steps at their places
+// and beside the blocks scales [3][vp]: what the columns of states, of steps, and (backwards) of the gradient of out are to be multiplied by
+constexpr int COLS = 32;
+template <typename S, int DK> struct Kept {
+    static constexpr int PAD = 16 / sizeof(S), STATE = DK + PAD, STEP = C + PAD, BLOCK = COLS * (STATE + STEP);    // elements
+    static_assert(BLOCK * sizeof(S) % 1024 == 0, "whole kilobytes");
+    S* blocks;
     float* scales;
-    Kept(void* p, const Shape& s, int dk) : states(static_cast<S*>(p)), steps(states + s.B * s.G * s.chunks * int64_t(s.vp) * dk),
-                                            scales(reinterpret_cast<float*>(steps + s.B * s.G * s.chunks * int64_t(s.vp) * C)) {}
+    Kept(void* p, const Shape& s) : blocks(static_cast<S*>(p)), scales(reinterpret_cast<float*>(blocks + s.B * s.G * s.chunks * (s.vp / COLS) * int64_t(BLOCK))) {}
+    // of a column's first place, in bytes; nowhere behind the last column
+    static __device__ uint32_t state_at(int col, int vp) { return col < vp ? (col / COLS * BLOCK + col % COLS * STATE) * uint32_t(sizeof(S)) : NOWHERE; }
+    static __device__ uint32_t step_at(int col, int vp) { return col < vp ? (col / COLS * BLOCK + COLS * STATE + col % COLS * STEP) * uint32_t(sizeof(S)) : NOWHERE; }
 };
-// An operand's first part, eight places of a column, to memory
-template <typename S, int PARTS> __device__ inline void leave(S* to, const Frag<S, PARTS>& f) {
+// An operand's first part, eight places of a column, to `at`, in bytes
+template <typename S, int PARTS> __device__ inline void leave(const Buffer& to, uint32_t at, const Frag<S, PARTS>& f) {
     pack<S, 8> o;
     __builtin_memcpy(&o, &f, sizeof o);
-    o.store(to);
+    to.store(o, at);
 }
-inline uint64_t kept_bytes(uint64_t rows, int32_t dk, int32_t dtype) { return rows * (uint64_t(dk + C) * (dtype == PV_F32 ? 4 : 2) + 12); }
+inline uint64_t kept_bytes(uint64_t chunks, int32_t vp, int32_t dk, int32_t dtype) {
+    const uint64_t pad = dtype == PV_F32 ? 4 : 8, bytes = dtype == PV_F32 ? 4 : 2;
+    return chunks * vp * ((dk + pad + C + pad) * bytes + 12);
+}
 
-// A chunk's steps on their way from memory to LDS
-template <int THREADS> struct StepsOnTheirWay {
-    static constexpr int N = int(sizeof(Steps) / 4), COUNT = (N + THREADS - 1) / THREADS;
-    float v[COUNT];
-    __device__ void load(const Steps& s) {
-        const float* from = reinterpret_cast<const float*>(&s);
-#pragma unroll
-        for (int j = 0; j < COUNT; j++) {
-            const int at = threadIdx.x + j * THREADS;
-            v[j] = from[at < N ? at : N - 1];
-        }
-    }
-    __device__ void put(Steps& s) const {
-        float* to = reinterpret_cast<float*>(&s);
-#pragma unroll
-        for (int j = 0; j < COUNT; j++) if (int(threadIdx.x) + j * THREADS < N) to[threadIdx.x + j * THREADS] = v[j];
-    }
-};
-// A matrix of 64 x 64 from a record, in PARTS parts, on its way
-template <typename S, int PARTS, int THREADS> struct SquareOnItsWay {
-    static constexpr int P = 16 / sizeof(S), COUNT = C * C / P / THREADS;
-    pack<S, P> v[PARTS][COUNT];
-    __device__ void load(const S (*from)[C][C]) {
-#pragma unroll
-        for (int w = 0; w < PARTS; w++)
-#pragma unroll
-            for (int j = 0; j < COUNT; j++) v[w][j] = pack<S, P>::load(&from[w][0][0] + (threadIdx.x + j * THREADS) * P);
-    }
-    template <typename T> __device__ void put(const T& tile) const {
-#pragma unroll
-        for (int w = 0; w < PARTS; w++)
-#pragma unroll
-            for (int j = 0; j < COUNT; j++) {
-                const int at = (threadIdx.x + j * THREADS) * P;
-                v[w][j].store(tile.p + w * T::PLANE + at / C * T::ROW + at % C);
-            }
-    }
-};
-// A lane's sixteen elements of a column of values: rows 16 it + 4 g + r. Steps past the last are the last one's.
+// A lane's sixteen elements of a column of values: rows 16 it + 4 g + r. On their way each has a register of its own: two of 16 bits
+// would be joined in one, which waits for both.
 template <typename E> struct Sixteen {
-    E v[16];
-    __device__ void load(const E* at, int64_t stride, int rows) {
-        const int g = threadIdx.x % WAVE / 16;
+    uint32_t v[16];
+    static __device__ uint32_t first(int stride, int col, bool on) { return on ? (threadIdx.x % WAVE / 16 * 4 * stride + col) * uint32_t(sizeof(E)) : NOWHERE; }
+    __device__ void load(const Buffer& from, int stride, uint32_t off) {
 #pragma unroll
         for (int j = 0; j < 16; j++) {
-            const int i = 16 * (j / 4) + 4 * g + j % 4;
-            v[j] = at[(i < rows ? i : rows - 1) * stride];
+            const int more = (16 * (j / 4) + j % 4) * stride * int(sizeof(E));
+            if constexpr (sizeof(E) == 2) v[j] = __builtin_amdgcn_raw_buffer_load_b16(from.r, off, more, 0);
+            else v[j] = __builtin_amdgcn_raw_buffer_load_b32(from.r, off, more, 0);
         }
     }
-    __device__ f4 four(int it, bool on) const {
-        f4 x;
-#pragma unroll
-        for (int r = 0; r < 4; r++) x[r] = on ? float(v[4 * it + r]) : 0.0f;
-        return x;
+    static __device__ void store(const Buffer& to, int stride, uint32_t off, int j, float x) { to.store<E>(E(x), off, (16 * (j / 4) + j % 4) * stride * int(sizeof(E))); }
+    static __device__ float value(uint32_t bits) {
+        E e;
+        __builtin_memcpy(&e, &bits, sizeof e);
+        return float(e);
     }
+    __device__ f4 four(int it) const { return f4{value(v[4 * it]), value(v[4 * it + 1]), value(v[4 * it + 2]), value(v[4 * it + 3])}; }
 };
+
+// The head and the columns' group of a workgroup, of `groups` to a head. Workgroups go to the eight dies in turn: those of one head
+// are on one die, whose L2 then has the head's records once for all of them.
+struct Part { int64_t head; int group; };
+__device__ inline Part part_of(uint32_t block, int64_t heads, int groups) {
+    const int64_t even = heads / 8 * 8;
+    if (block >= even * groups) return {even + (block - even * groups) / groups, int((block - even * groups) % groups)};
+    return {block % 8 + int64_t(8) * (block / 8 / groups), int(block / 8 % groups)};
+}
 
 // The value heads that share a query and key head are neighbours
 __device__ inline int shared(const Shape& S, int g) { return g / (S.G / S.H); }
 
-// f of a number of key columns that kernels are made for, K or more
+// The number of key columns that kernels are made for, K or more, and f of it
+inline int32_t columns_of(int32_t K) { return K <= 32 ? 32 : K <= 64 ? 64 : 128; }
 template <typename F> int32_t with_k(int32_t K, F&& f) {
     if (K <= 32) return f(std::integral_constant<int, 32>{});
     if (K <= 64) return f(std::integral_constant<int, 64>{});
@@ -343,22 +397,38 @@ template <typename F> int32_t with_k(int32_t K, F&& f) {
 }
 
 
-// The call's sizes and strides: of query, key, value, gate and write in their order, each of a sequence, a step and a head
-inline int32_t shape_of(int64_t B, int64_t T, int32_t H, int32_t G, int32_t K, int32_t V, const int64_t* strides, float eps, int32_t dtype, Shape& S, char* err,
+// The call's sizes and `count` strides, each of a sequence, a step and a head: of query, key, value, gate and write, or backwards of gate,
+// write and d_out
+inline int32_t shape_of(int64_t B, int64_t T, int32_t H, int32_t G, int32_t K, int32_t V, const int64_t* strides, int count, float eps, int32_t dtype, Shape& S, char* err,
                         size_t cap) {
     if (!element_bytes(dtype)) return fail(PV_EARG, err, cap, "dtype: one of PV_F32, PV_BF16, PV_F16");
     if (B < 1 || T < 1 || H < 1 || G < H || G % H || V < 1 || V > 1 << 16)
         return fail(PV_EARG, err, cap, "shape: B, T, H >= 1, G a multiple of H, 1 <= V <= 65,536");
     if (K < 1 || K > MAX_K) return fail(PV_EARG, err, cap, "shape: 1 <= K <= 128");
     const int64_t chunks = (T + C - 1) / C, heads = B * G;
-    // a launch's work items: four waves for a chunk, or for 32 columns of a state
-    if (B >= int64_t(1) << 24 || G >= 1 << 24 || T >= int64_t(1) << 31 || heads >= int64_t(1) << 24 || heads * chunks >= int64_t(1) << 24 ||
-        heads * ((V + 31) / 32) >= int64_t(1) << 24)
-        return fail(PV_EARG, err, cap, "too many chunks of 64 steps, or columns of states: fewer than 2^24");
+    // a launch's work items: eight waves for a chunk, or four for 32 columns of a state
+    if (B >= int64_t(1) << 23 || G >= 1 << 23 || T >= int64_t(1) << 31 || heads >= int64_t(1) << 23 || heads * chunks >= int64_t(1) << 23 ||
+        heads * ((V + 31) / 32) >= int64_t(1) << 23)
+        return fail(PV_EARG, err, cap, "too many chunks of 64 steps, or columns of states: fewer than 2^23");
     if (!strides) return fail(PV_EARG, err, cap, "null argument");
-    for (int i = 1; i < 15; i += 3) if (strides[i] < -(1 << 24) || strides[i] > 1 << 24) return fail(PV_EARG, err, cap, "stride: a step's is 2^24 elements at most");
-    S = {B, T, H, G, K, V, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7], strides[8], strides[9], strides[10], strides[11],
-         strides[12], strides[13], strides[14], 0, 0, 0, chunks, (V + 15) / 16 * 16, eps};
+    // (64 steps are within reach of 32-bit offsets, in bytes)
+    for (int i = 1; i < count; i += 3) if (strides[i] < 0 || strides[i] > MAX_STEP) return fail(PV_EARG, err, cap, "stride: a step's is 2^22 elements at most");
+    if (int64_t(G) * V > MAX_STEP || int64_t(H) * K > MAX_STEP) return fail(PV_EARG, err, cap, "shape: G V and H K are 2^22 at most");
+    S = {};
+    S.B = B; S.T = T; S.H = H; S.G = G; S.K = K; S.V = V; S.chunks = chunks; S.vp = (V + 31) / 32 * 32; S.eps = eps;
+    const auto take = [&](int64_t& of_a_sequence, int32_t& step, int64_t& head) {
+        of_a_sequence = *strides++;
+        step = int32_t(*strides++);
+        head = *strides++;
+    };
+    if (count == 15) {
+        take(S.qb, S.qt, S.qh);
+        take(S.kb, S.kt, S.kh);
+        take(S.vb, S.vt, S.vh);
+    }
+    take(S.ab, S.at, S.ag);
+    take(S.wb, S.wt, S.wg);
+    if (count == 9) take(S.ob, S.ot, S.og);
     return PV_OK;
 }
 

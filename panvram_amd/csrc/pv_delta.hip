@@ -47,8 +47,8 @@ __device__ inline void leave16(float* to, int row, const f4& v, float sign) {
 }
 
 // A matrix of 64 x 64 in LDS into a record, in parts
-template <typename S> __device__ inline void record(const float* m, int row, S (*to)[C][C]) {
-    for (int k = threadIdx.x; k < C * C / 8; k += BLOCK) {
+template <typename S> __device__ inline void record(const float* m, int row, S (*to)[C][C + Record<S>::PAD], int first, int threads) {
+    for (int k = threadIdx.x - first; k < C * C / 8; k += threads) {
         const int i = k / 8, at = k % 8 * 8;                       // eight places: columns c .. c + 3 and c + 16 .. c + 19
         const int c = (at & ~31) | (at & 24) >> 1;
         float v[8];
@@ -69,24 +69,47 @@ template <typename S> __device__ inline void record(const float* m, int row, S (
 
 template <typename E, int DK>
 __global__ __launch_bounds__(BLOCK) void chunk_kernel(const E* __restrict__ query, const E* __restrict__ key, const E* __restrict__ gate, const E* __restrict__ write,
-                                                      const uint8_t* __restrict__ reset, Shape S, Chunk<typename Rep<E>::S>* __restrict__ records) {
+                                                      const uint8_t* __restrict__ reset, Shape S, char* __restrict__ records, char* __restrict__ images) {
     using St = typename Rep<E>::S;
     using In = Tile<St, C, DK>;
-    constexpr int ROW = C + 4, MATRIX = C * ROW * 4;
-    constexpr int BYTES = 2 * In::SIZE * int(sizeof(St)) > 3 * MATRIX ? 2 * In::SIZE * int(sizeof(St)) : 3 * MATRIX;
-    __shared__ alignas(16) char lds[BYTES];
-    __shared__ Steps st;
+    using In8 = Rows<E, DK, BLOCK>;
+    constexpr int ROW = C + 4, MATRIX = C * ROW * 4, KEYS = 2 * In::SIZE * int(sizeof(St));
+    __shared__ alignas(16) char lds[KEYS > 2 * MATRIX ? KEYS : 2 * MATRIX];
+    __shared__ alignas(16) Steps st;
     const In Kt{reinterpret_cast<St*>(lds)}, Qt{reinterpret_cast<St*>(lds) + In::SIZE};
-    float *A = reinterpret_cast<float*>(lds), *P = A + C * ROW, *T = P + C * ROW;       // (once K and Q have been used)
+    float *A = reinterpret_cast<float*>(lds), *T = A + C * ROW;      // (once K and Q have been used; T is M Q K^T first)
     const int tid = threadIdx.x, wave = tid / WAVE, l = tid % WAVE, grp = l / 16, m = l % 16;
     const int64_t chunk = blockIdx.x % S.chunks, bg = blockIdx.x / S.chunks;
     const int64_t b = bg / S.G, t0 = chunk * C;
     const int g = int(bg % S.G), h = shared(S, g), rows = int(S.T - t0 < C ? S.T - t0 : C);
     // queries and keys, and one over their lengths
-    using In8 = Rows<E, DK, BLOCK>;
     In8 q, k;
     q.load(query + b * S.qb + t0 * S.qt + h * S.qh, S.qt, rows, S.K);
     k.load(key + b * S.kb + t0 * S.kt + h * S.kh, S.kt, rows, S.K);
+    if (wave == 0) {                       // a lane for each step: gates, and their logarithms summed up
+        const int64_t t = t0 + (l < rows ? l : rows - 1);
+        const float x = float(gate[b * S.ab + t * S.at + g * S.ag]), w = float(write[b * S.wb + t * S.wt + g * S.wg]);
+        float la = -(fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))));
+        if (x != x) la = x;
+        const bool cut = l < rows && (la < -104.0f || (reset && reset[b * S.T + t]));      // (exp(-104) is 0 in 32 bits)
+        const uint64_t cuts = __ballot(cut);
+        double c = l < rows && !cut ? double(la) : 0.0;
+#pragma unroll
+        for (int d = 1; d < WAVE; d <<= 1) {
+            const double o = __shfl_up(c, d, WAVE);
+            if (l >= d) c += o;
+        }
+        const double last = __shfl(c, C - 1, WAVE);
+        const float hi = float(c);
+        st.b[l] = l < rows ? 1.0f / (1.0f + expf(-w)) : 0.0f;
+        st.hi[l] = hi;
+        st.lo[l] = float(c - double(hi));
+        st.x[l] = cuts & (~0ull >> (63 - l)) ? 0.0f : expf(hi);     // (times the lengths below)
+        st.l[l] = l < since(cuts, C - 1) ? 0.0f : expf(float(last - c));
+        if (l == C - 1) st.end = cuts ? 0.0f : expf(hi);
+        if (l < 2) st.cut[l] = uint32_t(cuts >> (32 * l));
+        if (l == 0) st.unused = 0;
+    }
     In8::clear(Qt, S.K);
     In8::clear(Kt, S.K);
 #pragma unroll
@@ -103,36 +126,11 @@ __global__ __launch_bounds__(BLOCK) void chunk_kernel(const E* __restrict__ quer
             st.rk[i] = rk;
         }
     }
-    if (wave == 0) {                       // a lane for each step: gates, and their logarithms summed up
-        const int64_t t = t0 + l;
-        float la = 0.0f, beta = 0.0f;
-        bool cut = false;
-        if (l < rows) {
-            const float x = float(gate[b * S.ab + t * S.at + g * S.ag]), w = float(write[b * S.wb + t * S.wt + g * S.wg]);
-            la = -(fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))));
-            if (x != x) la = x;
-            beta = 1.0f / (1.0f + expf(-w));
-            cut = la < -104.0f || (reset && reset[b * S.T + t]);    // (exp(-104) is 0 in 32 bits)
-        }
-        const uint64_t cuts = __ballot(cut);
-        double c = cut ? 0.0 : double(la);
-#pragma unroll
-        for (int d = 1; d < WAVE; d <<= 1) {
-            const double o = __shfl_up(c, d, WAVE);
-            if (l >= d) c += o;
-        }
-        const double last = __shfl(c, C - 1, WAVE);
-        const float hi = float(c);
-        st.b[l] = beta;
-        st.hi[l] = hi;
-        st.lo[l] = float(c - double(hi));
-        st.x[l] = cuts & (~0ull >> (63 - l)) ? 0.0f : expf(hi);     // (times the lengths below)
-        st.l[l] = l < since(cuts, C - 1) ? 0.0f : expf(float(last - c));
-        if (l == C - 1) st.end = cuts ? 0.0f : expf(hi);
-        if (l < 2) st.cut[l] = uint32_t(cuts >> (32 * l));
-        if (l == 0) st.unused = 0;
-    }
     __syncthreads();
+    if (g % (S.G / S.H) == 0) {            // the image of keys and queries, by the first of the value heads that share them
+        char* to = images + ((b * S.H + h) * S.chunks + chunk) * IMAGE<St, DK>;
+        for (int i = tid * 16; i < KEYS; i += BLOCK * 16) pack<char, 16>::load(lds + i).store(to + i);
+    }
     // rows 16 wave .. of K K^T and Q K^T, up to the diagonal
     f4 kk[WAVES], qk[WAVES];
 #pragma unroll
@@ -155,36 +153,60 @@ __global__ __launch_bounds__(BLOCK) void chunk_kernel(const E* __restrict__ quer
         st.q[tid] = shift * length_rest<St>(st.rq[tid]);
         st.l[tid] *= length_rest<St>(st.rk[tid]);
     }
+    float hi[4], lo[4], kf[4], qf[4];
+    int from[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int i = 16 * wave + 4 * grp + r;
+        hi[r] = st.hi[i];
+        lo[r] = st.lo[i];
+        kf[r] = length_rest<St>(st.rk[i]) * st.b[i];
+        qf[r] = length_rest<St>(st.rq[i]);
+        from[r] = since(cuts, i);
+    }
 #pragma unroll
     for (int j = 0; j < WAVES; j++) {
         const int col = 16 * j + m;
-        const float rk = length_rest<St>(st.rk[col]), hi = st.hi[col], lo = st.lo[col];
+        const float rk = length_rest<St>(st.rk[col]), hc = st.hi[col], lc = st.lo[col];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int i = 16 * wave + 4 * grp + r;
-            const bool on = col <= i && col >= since(cuts, i);
-            const float M = on ? expf((st.hi[i] - hi) + (st.lo[i] - lo)) * rk : 0.0f;
-            P[i * ROW + col] = on ? M * length_rest<St>(st.rq[i]) * qk[j][r] : 0.0f;
-            A[i * ROW + col] = on && col < i ? M * length_rest<St>(st.rk[i]) * st.b[i] * kk[j][r] : 0.0f;
-            T[i * ROW + col] = 0.0f;
+            const bool on = j <= wave && col <= i && col >= from[r];
+            const float M = on ? expf((hi[r] - hc) + (lo[r] - lc)) * rk : 0.0f;
+            T[i * ROW + col] = on ? M * qf[r] * qk[j][r] : 0.0f;
+            A[i * ROW + col] = on && col < i ? M * kf[r] * kk[j][r] : 0.0f;
         }
     }
     __syncthreads();
-    auto& out = records[blockIdx.x];
+    auto& out = *reinterpret_cast<Record<St>*>(record_of<St>(records, blockIdx.x));
+    float t[16];
     if (wave == 0) {                       // the inverses of the diagonal's blocks: a lane for a column of one
-        float t[16];
-        const float* a = A + 16 * grp * ROW + 16 * grp;
+        f4 a[16][4];
+        const float* from = A + 16 * grp * ROW + 16 * grp;
+#pragma unroll
+        for (int i = 1; i < 16; i++)
+#pragma unroll
+            for (int j = 0; j < (i + 3) / 4; j++) a[i][j] = *reinterpret_cast<const f4*>(from + i * ROW + 4 * j);
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             float v = i == m ? 1.0f : 0.0f;
 #pragma unroll
-            for (int j = 0; j < i; j++) v = fmaf(-a[i * ROW + j], t[j], v);
+            for (int j = 0; j < i; j++) v = fmaf(-a[i][j / 4][j % 4], t[j], v);
             t[i] = v;
         }
+    } else {
+        record<St>(T, ROW, out.pair, WAVE, BLOCK - WAVE);
+    }
+    __syncthreads();
+    if (wave == 0) {
 #pragma unroll
         for (int i = 0; i < 16; i++) T[(16 * grp + i) * ROW + 16 * grp + m] = t[i];
+    } else {                               // nothing above the diagonal's blocks
+        for (int k = tid - WAVE; k < C * C / 4; k += BLOCK - WAVE) {
+            const int i = k / 16, c = k % 16 * 4;
+            if (c / 16 > i / 16) *reinterpret_cast<f4*>(T + i * ROW + c) = f4{0, 0, 0, 0};
+        }
     }
-    record<St>(P, ROW, out.pair);
     __syncthreads();
     const auto at = [&](float* p, int i, int j) { return p + 16 * i * ROW + 16 * j; };
     const f4 zero = {0, 0, 0, 0};
@@ -203,40 +225,43 @@ __global__ __launch_bounds__(BLOCK) void chunk_kernel(const E* __restrict__ quer
         }
         leave16(at(T, 2, wave), ROW, product16(at(T, 2, 2), ROW, y2, zero), -1.0f);
         leave16(at(T, 3, wave), ROW, product16(at(T, 3, 3), ROW, y3, product16(at(T, 3, 2), ROW, y2, zero)), -1.0f);
+    } else {
+        const float* from = reinterpret_cast<const float*>(&st);
+        float* to = reinterpret_cast<float*>(&out.steps);
+        for (int k = tid - 2 * WAVE; k < int(sizeof(Steps) / 4); k += BLOCK - 2 * WAVE) to[k] = from[k];
     }
     __syncthreads();
-    record<St>(T, ROW, out.inv);
-    const float* from = reinterpret_cast<const float*>(&st);
-    float* to = reinterpret_cast<float*>(&out.steps);
-    for (int k = tid; k < int(sizeof(Steps) / 4); k += BLOCK) to[k] = from[k];
+    record<St>(T, ROW, out.inv, 0, BLOCK);
 }
 
-// ---- state_kernel: a workgroup of W waves for 16 W columns of a state
+// ---- state_kernel: a workgroup of W waves for 16 W columns of a state. Chunks come to LDS while the one before is worked on, where
+// two have room (tensors of 16 bits), else one after another.
 
-template <typename E, int DK, int W>
-__global__ __launch_bounds__(W * WAVE) void state_kernel(const E* __restrict__ query, const E* __restrict__ key, const E* __restrict__ value,
-                                                         const float* __restrict__ state, Shape S, const Chunk<typename Rep<E>::S>* __restrict__ records,
-                                                         E* __restrict__ out, float* __restrict__ last, bool keep, Kept<typename Rep<E>::S> kept) {
+template <typename E, int DK, int W, bool KEEP>
+__global__ __launch_bounds__(W * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))) void state_kernel(
+    const E* __restrict__ value, const float* __restrict__ state, Shape S, const char* __restrict__ records, const char* __restrict__ images, E* __restrict__ out,
+    float* __restrict__ last, Kept<typename Rep<E>::S, DK> kept) {
     using St = typename Rep<E>::S;
-    constexpr int WIDE = wide_of<St>, ND = DK / 16, KB = DK / 32, THREADS = W * WAVE;
+    using Ke = Kept<St, DK>;
+    constexpr int WIDE = wide_of<St>, ND = DK / 16, KB = DK / 32;
     using In = Tile<St, C, DK>;
     using Square = Tile<St, C, C, WIDE>;
-    using Part = Tile<St, C, C>;
-    using In8 = Rows<E, DK, THREADS>;
-    __shared__ alignas(16) St lds[2 * In::SIZE + Square::SIZE + Part::SIZE];
-    __shared__ alignas(16) Steps st;
-    const In Kt{lds}, Qt{lds + In::SIZE};
-    const Square Tt{lds + 2 * In::SIZE};
-    const Part Pt{lds + 2 * In::SIZE + Square::SIZE};
+    using Plain = Tile<St, C, C>;
+    using Re = Record<St>;
+    constexpr int BUFFERS = sizeof(St) == 2 ? 2 : 1, IN = IMAGE<St, DK>, BUFFER = IN + (Re::NARROW + 1023) / 1024 * 1024;
+    __shared__ alignas(1024) char lds[BUFFERS * BUFFER];
     const int tid = threadIdx.x, wave = tid / WAVE, l = tid % WAVE, grp = l / 16, m = l % 16;
     const int groups = (S.vp / 16 + W - 1) / W;
-    const int64_t bg = blockIdx.x / groups;
-    const int col = (int(blockIdx.x % groups) * W + wave) * 16 + m;
+    const auto [bg, group] = part_of(blockIdx.x, S.B * S.G, groups);
+    const int col = (group * W + wave) * 16 + m;
     const int64_t b = bg / S.G;
     const int g = int(bg % S.G), h = shared(S, g);
-    const bool on = col < S.V, held = keep && col < S.vp;
-    const E *q0 = query + b * S.qb + h * S.qh, *k0 = key + b * S.kb + h * S.kh, *v0 = value + b * S.vb + g * S.vh + (on ? col : S.V - 1);
-    const Chunk<St>* rec = records + bg * S.chunks;
+    const bool on = col < S.V;
+    const E* v0 = value + b * S.vb + g * S.vh;
+    const char *rec0 = records + bg * S.chunks * Re::STRIDE, *in0 = images + (b * S.H + h) * S.chunks * IN;
+    const int ot = S.G * S.V;              // steps of out
+    const uint32_t value_at = Sixteen<E>::first(S.vt, col, on), out_at = Sixteen<E>::first(ot, col, on);
+    const uint32_t state_at = Ke::state_at(col, S.vp) + 8 * grp * sizeof(St), step_at = Ke::step_at(col, S.vp) + 8 * grp * sizeof(St);
 
     f4 s[ND];
 #pragma unroll
@@ -246,89 +271,73 @@ __global__ __launch_bounds__(W * WAVE) void state_kernel(const E* __restrict__ q
             const int d = 16 * n + 4 * grp + r;
             s[n][r] = state && on && d < S.K ? state[(bg * S.K + d) * S.V + col] : 0.0f;
         }
-
-    // a chunk on its way from memory to LDS
-    In8 qp, kp;
-    float qr[In8::COUNT], kr[In8::COUNT];
-    SquareOnItsWay<St, WIDE, THREADS> tp;
-    SquareOnItsWay<St, 1, THREADS> pp;
-    StepsOnTheirWay<THREADS> sp;
     Sixteen<E> vp;
+    const auto rows_of = [&](int64_t n) { return int(S.T - n * C < C ? S.T - n * C : C); };
     auto fetch = [&](int64_t n) {
-        const int64_t t0 = n * C;
-        const int rows = int(S.T - t0 < C ? S.T - t0 : C);
-        kp.load(k0 + t0 * S.kt, S.kt, rows, S.K);
-        qp.load(q0 + t0 * S.qt, S.qt, rows, S.K);
-#pragma unroll
-        for (int j = 0; j < In8::COUNT; j++) {
-            kr[j] = rec[n].steps.rk[In8::row(j)];
-            qr[j] = rec[n].steps.rq[In8::row(j)];
-        }
-        tp.load(rec[n].inv);
-        pp.load(rec[n].pair);
-        sp.load(rec[n].steps);
-        vp.load(v0 + t0 * S.vt, S.vt, rows);
+        vp.load(rows_at(v0 + n * C * S.vt, S.vt, rows_of(n), S.V), S.vt, value_at);
+        char* to = lds + (BUFFERS == 2 ? int(n & 1) * BUFFER : 0);
+        bring<W>(in0 + n * IN, to, 2 * In::SIZE * int(sizeof(St)));
+        bring<W>(rec0 + n * Re::STRIDE, to + IN, Re::NARROW);
     };
-    const auto four = [&](const float* p, int it) { return *reinterpret_cast<const f4*>(p + 16 * it + 4 * grp); };
 
-    In8::clear(Kt, S.K);
-    In8::clear(Qt, S.K);
     fetch(0);
+    arrived<0>();
     for (int64_t n = 0; n < S.chunks; n++) {
-        __syncthreads();                   // the chunk before has been used
-#pragma unroll
-        for (int j = 0; j < In8::COUNT; j++) {
-            kp.put(Kt, j, length_up<St>(kr[j]), S.K);
-            qp.put(Qt, j, length_up<St>(qr[j]), S.K);
-        }
-        tp.put(Tt);
-        pp.put(Pt);
-        sp.put(st);
+        __syncthreads();                   // the chunk is there, and the one before has been used
+        char* here = lds + (BUFFERS == 2 ? int(n & 1) * BUFFER : 0);
+        const In Kt{reinterpret_cast<St*>(here)}, Qt{reinterpret_cast<St*>(here) + In::SIZE};
+        const Re& re = *reinterpret_cast<const Re*>(here + IN);
+        const Steps& st = re.steps;
+        const Square Tt{const_cast<St*>(&re.inv[0][0][0])};
+        const Plain Pt{const_cast<St*>(&re.pair[0][0][0])};
+        const auto four = [&](const float* p, int it) { return *reinterpret_cast<const f4*>(p + 16 * it + 4 * grp); };
         f4 v[4];
 #pragma unroll
-        for (int it = 0; it < 4; it++) v[it] = vp.four(it, on);
-        __syncthreads();
-        if (n + 1 < S.chunks) fetch(n + 1);
-        const int64_t row = (bg * S.chunks + n) * S.vp + col;
+        for (int it = 0; it < 4; it++) v[it] = vp.four(it);
+        if (BUFFERS == 2 && n + 1 < S.chunks) fetch(n + 1);
+        const int64_t at = (bg * S.chunks + n) * S.vp;     // of the chunk in what is kept
+        const Buffer blocks(kept.blocks + at / COLS * Ke::BLOCK, KEEP ? int64_t(S.vp / COLS) * Ke::BLOCK * int(sizeof(St)) : 0);
         const Scale ss = scale_of<St>(over_column(largest(s)));
         Frag<St, WIDE> sf[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; kb++) {
             sf[kb] = frag_of<St, WIDE>(s[2 * kb], s[2 * kb + 1], ss.up);
-            if (held) leave(kept.states + row * DK + 32 * kb + 8 * grp, sf[kb]);
+            if constexpr (KEEP) leave(blocks, state_at + 32 * kb * sizeof(St), sf[kb]);
         }
-        // D = V - g K S, then b D; out's part g Q S
-        f4 o[4], d[4];
+        // D = V - g K S, then b D; g Q S for out
+        f4 x[4], y[4], d[4];
+#pragma unroll
+        for (int it = 0; it < 4; it++) x[it] = y[it] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+            for (int it = 0; it < 4; it++) mma(x[it], Kt.rows(16 * it, kb), sf[kb]);
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+            for (int it = 0; it < 4; it++) mma(y[it], Qt.rows(16 * it, kb), narrow(sf[kb]));
 #pragma unroll
         for (int it = 0; it < 4; it++) {
-            f4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+            const f4 xs = four(st.x, it), bs = four(st.b, it);
 #pragma unroll
-            for (int kb = 0; kb < KB; kb++) {
-                mma(x, Kt.rows(16 * it, kb), sf[kb]);
-                mma(y, Qt.rows(16 * it, kb), narrow(sf[kb]));
-            }
-            const f4 xs = four(st.x, it), bs = four(st.b, it), qs = four(st.q, it);
-#pragma unroll
-            for (int r = 0; r < 4; r++) {  // (a dropped state may hold anything)
-                d[it][r] = bs[r] * (v[it][r] - (xs[r] == 0.0f ? 0.0f : xs[r] * (ss.down * x[r])));
-                o[it][r] = qs[r] == 0.0f ? 0.0f : qs[r] * (ss.down * y[r]);
-            }
+            for (int r = 0; r < 4; r++) d[it][r] = bs[r] * (v[it][r] - (xs[r] == 0.0f ? 0.0f : xs[r] * (ss.down * x[it][r])));      // (a dropped state may hold anything)
         }
         // U = (I + A)^-1 b D
         const Scale ds = scale_of<St>(over_column(largest(d)));
         Frag<St, WIDE> df[2];
-        f4 u[4];
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) df[kb] = frag_of<St, WIDE>(d[2 * kb], d[2 * kb + 1], ds.up);
+        f4 u[4];
+#pragma unroll
+        for (int it = 0; it < 4; it++) u[it] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int it = 2 * kb; it < 4; it++) mma(u[it], Tt.rows(16 * it, kb), df[kb]);
         const float du = ds.down * (1.0f / SQUARE<St>);
 #pragma unroll
-        for (int it = 0; it < 4; it++) {
-            u[it] = f4{0, 0, 0, 0};
-#pragma unroll
-            for (int kb = 0; kb <= it / 2; kb++) mma(u[it], Tt.rows(16 * it, kb), df[kb]);
-            u[it] *= du;
-        }
-        // what it adds to the state (l r is 2 / LONG at most); out's part (M Q K^T) U
+        for (int it = 0; it < 4; it++) u[it] *= du;
+        // what it adds to the state (l r is 2 / LONG at most)
         const Scale us = scale_of<St>(over_column(largest(u)));
         Frag<St, 1> uf[2];
         Frag<St, WIDE> lf[2];
@@ -336,32 +345,41 @@ __global__ __launch_bounds__(W * WAVE) void state_kernel(const E* __restrict__ q
         for (int kb = 0; kb < 2; kb++) {
             uf[kb] = frag_of<St, 1>(u[2 * kb], u[2 * kb + 1], us.up);
             lf[kb] = frag_of<St, WIDE>(LONG<St> * u[2 * kb] * four(st.l, 2 * kb), LONG<St> * u[2 * kb + 1] * four(st.l, 2 * kb + 1), us.up);
-            if (held) leave(kept.steps + row * C + 32 * kb + 8 * grp, uf[kb]);
+            if constexpr (KEEP) leave(blocks, step_at + 32 * kb * sizeof(St), uf[kb]);
         }
-        if (held && grp == 0) {
-            kept.scales[(bg * S.chunks + n) * 3 * S.vp + col] = ss.down;
-            kept.scales[((bg * S.chunks + n) * 3 + 1) * S.vp + col] = us.down;
+        if constexpr (KEEP) {
+            const Buffer scales(kept.scales + 3 * at, 3 * int64_t(S.vp) * 4);
+            const uint32_t to = grp == 0 && col < S.vp ? col * 4 : NOWHERE;
+            scales.store(ss.down, to);
+            scales.store(us.down, to, S.vp * 4);
         }
         const float end = st.end, dl = us.down * (1.0f / LONG<St>), dp = us.down * (1.0f / SQUARE<St>);
 #pragma unroll
         for (int k = 0; k < ND; k++) {
-            f4 x = {0, 0, 0, 0};
+            f4 z = {0, 0, 0, 0};
 #pragma unroll
-            for (int kb = 0; kb < 2; kb++) mma(x, Kt.cols(16 * k, kb), lf[kb]);
+            for (int kb = 0; kb < 2; kb++) mma(z, Kt.cols(16 * k, kb), lf[kb]);
 #pragma unroll
-            for (int r = 0; r < 4; r++) s[k][r] = fmaf(dl, x[r], end == 0.0f ? 0.0f : end * s[k][r]);
+            for (int r = 0; r < 4; r++) s[k][r] = fmaf(dl, z[r], end == 0.0f ? 0.0f : end * s[k][r]);
         }
-        const int64_t t0 = n * C;
-        E* to = out + ((b * S.T + t0) * S.G + g) * S.V + col;
+        // out = g Q S + (M Q K^T) U
+        const Buffer to = rows_at(out + ((b * S.T + n * C) * S.G + g) * S.V, ot, rows_of(n), S.V);
 #pragma unroll
         for (int it = 0; it < 4; it++) {
-            f4 x = {0, 0, 0, 0};
+            f4 w = {0, 0, 0, 0};
 #pragma unroll
-            for (int kb = 0; kb <= it / 2; kb++) mma(x, Pt.rows(16 * it, kb), uf[kb]);
+            for (int kb = 0; kb <= it / 2; kb++) mma(w, Pt.rows(16 * it, kb), uf[kb]);
+            const f4 qs = four(st.q, it);
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int i = 16 * it + 4 * grp + r;
-                if (on && t0 + i < S.T) to[int64_t(i) * S.G * S.V] = E(fmaf(dp, x[r], o[it][r]));
+            for (int r = 0; r < 4; r++) Sixteen<E>::store(to, ot, out_at, 4 * it + r, fmaf(dp, w[r], qs[r] == 0.0f ? 0.0f : qs[r] * (ss.down * y[it][r])));
+        }
+        if (n + 1 < S.chunks) {
+            if constexpr (BUFFERS == 2) {
+                arrived<16 + (KEEP ? KB + 4 : 0)>();       // (all but this chunk's stores)
+            } else {
+                __syncthreads();
+                fetch(n + 1);
+                arrived<0>();
             }
         }
     }
@@ -469,13 +487,15 @@ template <typename E, int DK>
 int32_t forward(const void* query, const void* key, const void* value, const void* gate, const void* write, const float* state, const uint8_t* reset, const Shape& S,
                 void* out, float* last, void* kept, void* work, hipStream_t stream, char* err, size_t errcap) {
     using St = typename Rep<E>::S;
-    constexpr int W = 4;
+    constexpr int W = 2;
     const auto in = [](const void* p) { return static_cast<const E*>(p); };
-    auto* records = static_cast<Chunk<St>*>(work);
     const int64_t heads = S.B * S.G;
-    chunk_kernel<E, DK><<<dim3(heads * S.chunks), BLOCK, 0, stream>>>(in(query), in(key), in(gate), in(write), reset, S, records);
-    state_kernel<E, DK, W><<<dim3(heads * ((S.vp / 16 + W - 1) / W)), W * WAVE, 0, stream>>>(in(query), in(key), in(value), state, S, records, static_cast<E*>(out), last,
-                                                                                            kept != nullptr, Kept<St>(kept, S, DK));
+    char *records = static_cast<char*>(work), *images = records + heads * S.chunks * Record<St>::STRIDE;
+    chunk_kernel<E, DK><<<dim3(heads * S.chunks), BLOCK, 0, stream>>>(in(query), in(key), in(gate), in(write), reset, S, records, images);
+    const dim3 grid(heads * ((S.vp / 16 + W - 1) / W));
+    const Kept<St, DK> to(kept, S);
+    if (kept) state_kernel<E, DK, W, true><<<grid, W * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to);
+    else state_kernel<E, DK, W, false><<<grid, W * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to);
     return launched(err, errcap);
 }
 
@@ -483,25 +503,25 @@ int32_t forward(const void* query, const void* key, const void* value, const voi
 
 extern "C" {
 
-uint64_t pv_gated_delta_work_bytes(int64_t B, int64_t T, int32_t G, int32_t dtype, int32_t keep) {
-    if (B < 1 || G < 1 || T < 1 || (T <= SHORT && !keep)) return 0;
-    const uint64_t chunks = uint64_t(B) * uint64_t(G) * uint64_t((T + C - 1) / C);
-    return chunks * (dtype == PV_F32 ? sizeof(Chunk<float>) : sizeof(Chunk<f16>));
+uint64_t pv_gated_delta_work_bytes(int64_t B, int64_t T, int32_t H, int32_t G, int32_t K, int32_t dtype, int32_t keep) {
+    if (B < 1 || H < 1 || G < 1 || T < 1 || (T <= SHORT && !keep)) return 0;
+    const uint64_t chunks = uint64_t(B) * uint64_t((T + C - 1) / C);
+    return chunks * (uint64_t(G) * (dtype == PV_F32 ? Record<float>::STRIDE : Record<f16>::STRIDE) + uint64_t(H) * image_bytes(columns_of(K), dtype));
 }
 
 uint64_t pv_gated_delta_kept_bytes(int64_t B, int64_t T, int32_t G, int32_t K, int32_t V, int32_t dtype) {
     if (B < 1 || G < 1 || T < 1 || K < 1 || V < 1) return 0;
-    return kept_bytes(uint64_t(B) * uint64_t(G) * uint64_t((T + C - 1) / C) * uint64_t((V + 15) / 16 * 16), K <= 32 ? 32 : K <= 64 ? 64 : 128, dtype);
+    return kept_bytes(uint64_t(B) * uint64_t(G) * uint64_t((T + C - 1) / C), (V + 31) / 32 * 32, columns_of(K), dtype);
 }
 
 int32_t pv_gated_delta_hip(const void* query, const void* key, const void* value, const void* gate, const void* write, const float* state, const uint8_t* reset,
                            int64_t B, int64_t T, int32_t H, int32_t G, int32_t K, int32_t V, const int64_t* strides, float eps, int32_t dtype, void* out, float* last,
                            void* kept, void* work, uint64_t work_bytes, void* stream, char* err, size_t errcap) {
     Shape S;
-    if (int32_t e = shape_of(B, T, H, G, K, V, strides, eps, dtype, S, err, errcap)) return e;
+    if (int32_t e = shape_of(B, T, H, G, K, V, strides, 15, eps, dtype, S, err, errcap)) return e;
     if (!query || !key || !value || !gate || !write || !out || !last) return fail(PV_EARG, err, errcap, "null argument");
     if (kept && !aligned(kept, 16)) return fail(PV_EARG, err, errcap, "kept: not 16-byte aligned");
-    const uint64_t need = pv_gated_delta_work_bytes(B, T, G, dtype, kept != nullptr);
+    const uint64_t need = pv_gated_delta_work_bytes(B, T, H, G, K, dtype, kept != nullptr);
     if (need && (!work || work_bytes < need || !aligned(work, 16))) return fail(PV_EARG, err, errcap, "work: too small, or not 16-byte aligned");
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);

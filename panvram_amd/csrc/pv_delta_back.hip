@@ -17,32 +17,32 @@ using namespace pvd;
 
 namespace {
 
-constexpr int WAVES = 4, BLOCK = WAVES * WAVE;
-
 // ---- walk_kernel: a workgroup of W waves for 16 W columns of a state's gradient
 
 template <typename E, int DK, int W>
-__global__ __launch_bounds__(W * WAVE) void walk_kernel(const E* __restrict__ query, const E* __restrict__ key, const E* __restrict__ d_out,
-                                                        const float* __restrict__ d_last, Shape S, const Chunk<typename Rep<E>::S>* __restrict__ records,
-                                                        E* __restrict__ d_value, float* __restrict__ d_state, Kept<typename Rep<E>::S> walked) {
+__global__ __launch_bounds__(W * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))) void walk_kernel(
+    const E* __restrict__ d_out, const float* __restrict__ d_last, Shape S, const char* __restrict__ records, const char* __restrict__ images, E* __restrict__ d_value,
+    float* __restrict__ d_state, Kept<typename Rep<E>::S, DK> walked) {
     using St = typename Rep<E>::S;
-    constexpr int WIDE = wide_of<St>, ND = DK / 16, KB = DK / 32, THREADS = W * WAVE;
+    using Ke = Kept<St, DK>;
+    constexpr int WIDE = wide_of<St>, ND = DK / 16, KB = DK / 32;
     using In = Tile<St, C, DK>;
     using Square = Tile<St, C, C, WIDE>;
-    using In8 = Rows<E, DK, THREADS>;
-    __shared__ alignas(16) St lds[2 * In::SIZE + 2 * Square::SIZE];
-    __shared__ alignas(16) Steps st;
-    const In Kt{lds}, Qt{lds + In::SIZE};
-    const Square Tt{lds + 2 * In::SIZE}, Pt{lds + 2 * In::SIZE + Square::SIZE};
+    using Re = Record<St>;
+    constexpr int BUFFERS = sizeof(St) == 2 ? 2 : 1, IN = IMAGE<St, DK>, BUFFER = IN + Re::STRIDE;
+    __shared__ alignas(1024) char lds[BUFFERS * BUFFER];
     const int tid = threadIdx.x, wave = tid / WAVE, l = tid % WAVE, grp = l / 16, m = l % 16;
     const int groups = (S.vp / 16 + W - 1) / W;
-    const int64_t bg = blockIdx.x / groups;
-    const int col = (int(blockIdx.x % groups) * W + wave) * 16 + m;
+    const auto [bg, group] = part_of(blockIdx.x, S.B * S.G, groups);
+    const int col = (group * W + wave) * 16 + m;
     const int64_t b = bg / S.G;
     const int g = int(bg % S.G), h = shared(S, g);
-    const bool on = col < S.V, held = col < S.vp;
-    const E *q0 = query + b * S.qb + h * S.qh, *k0 = key + b * S.kb + h * S.kh, *o0 = d_out + b * S.ob + g * S.og + (on ? col : S.V - 1);
-    const Chunk<St>* rec = records + bg * S.chunks;
+    const bool on = col < S.V;
+    const E* o0 = d_out + b * S.ob + g * S.og;
+    const char *rec0 = records + bg * S.chunks * Re::STRIDE, *in0 = images + (b * S.H + h) * S.chunks * IN;
+    const int vt = S.G * S.V;              // steps of d_value
+    const uint32_t out_at = Sixteen<E>::first(S.ot, col, on), value_at = Sixteen<E>::first(vt, col, on);
+    const uint32_t state_at = Ke::state_at(col, S.vp) + 8 * grp * sizeof(St), step_at = Ke::step_at(col, S.vp) + 8 * grp * sizeof(St);
 
     f4 s[ND];
 #pragma unroll
@@ -52,76 +52,64 @@ __global__ __launch_bounds__(W * WAVE) void walk_kernel(const E* __restrict__ qu
             const int d = 16 * n + 4 * grp + r;
             s[n][r] = d_last && on && d < S.K ? d_last[(bg * S.K + d) * S.V + col] : 0.0f;
         }
-
-    In8 qp, kp;
-    float qr[In8::COUNT], kr[In8::COUNT];
-    SquareOnItsWay<St, WIDE, THREADS> tp, pp;
-    StepsOnTheirWay<THREADS> sp;
     Sixteen<E> op;
+    const auto rows_of = [&](int64_t n) { return int(S.T - n * C < C ? S.T - n * C : C); };
     auto fetch = [&](int64_t n) {
-        const int64_t t0 = n * C;
-        const int rows = int(S.T - t0 < C ? S.T - t0 : C);
-        kp.load(k0 + t0 * S.kt, S.kt, rows, S.K);
-        qp.load(q0 + t0 * S.qt, S.qt, rows, S.K);
-#pragma unroll
-        for (int j = 0; j < In8::COUNT; j++) {
-            kr[j] = rec[n].steps.rk[In8::row(j)];
-            qr[j] = rec[n].steps.rq[In8::row(j)];
-        }
-        tp.load(rec[n].inv);
-        pp.load(rec[n].pair);
-        sp.load(rec[n].steps);
-        op.load(o0 + t0 * S.ot, S.ot, rows);
+        op.load(rows_at(o0 + n * C * S.ot, S.ot, rows_of(n), S.V), S.ot, out_at);
+        char* to = lds + (BUFFERS == 2 ? int(n & 1) * BUFFER : 0);
+        bring<W>(in0 + n * IN, to, 2 * In::SIZE * int(sizeof(St)));
+        bring<W>(rec0 + n * Re::STRIDE, to + IN, Re::ALL);
     };
-    const auto four = [&](const float* p, int it) { return *reinterpret_cast<const f4*>(p + 16 * it + 4 * grp); };
 
-    In8::clear(Kt, S.K);
-    In8::clear(Qt, S.K);
     fetch(S.chunks - 1);
+    arrived<0>();
     for (int64_t n = S.chunks - 1; n >= 0; n--) {
-        __syncthreads();                   // the chunk after has been used
-#pragma unroll
-        for (int j = 0; j < In8::COUNT; j++) {
-            kp.put(Kt, j, length_up<St>(kr[j]), S.K);
-            qp.put(Qt, j, length_up<St>(qr[j]), S.K);
-        }
-        tp.put(Tt);
-        pp.put(Pt);
-        sp.put(st);
-        const int64_t t0 = n * C;
+        __syncthreads();                   // the chunk is there, and the one after has been used
+        char* here = lds + (BUFFERS == 2 ? int(n & 1) * BUFFER : 0);
+        const In Kt{reinterpret_cast<St*>(here)}, Qt{reinterpret_cast<St*>(here) + In::SIZE};
+        const Re& re = *reinterpret_cast<const Re*>(here + IN);
+        const Steps& st = re.steps;
+        const Square Tt{const_cast<St*>(&re.inv[0][0][0])}, Pt{const_cast<St*>(&re.pair[0][0][0])};
+        const auto four = [&](const float* p, int it) { return *reinterpret_cast<const f4*>(p + 16 * it + 4 * grp); };
+        const int rows = rows_of(n);
         f4 o[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) {
-            o[it] = op.four(it, on);
+            o[it] = op.four(it);
 #pragma unroll
-            for (int r = 0; r < 4; r++) if (t0 + 16 * it + 4 * grp + r >= S.T) o[it][r] = 0.0f;
+            for (int r = 0; r < 4; r++) o[it][r] = 16 * it + 4 * grp + r < rows ? o[it][r] : 0.0f;
         }
-        __syncthreads();
-        if (n) fetch(n - 1);
-        const int64_t row = (bg * S.chunks + n) * S.vp + col;
+        if (BUFFERS == 2 && n) fetch(n - 1);
+        const int64_t at = (bg * S.chunks + n) * S.vp;     // of the chunk in what is left over
+        const Buffer blocks(walked.blocks + at / COLS * Ke::BLOCK, int64_t(S.vp / COLS) * Ke::BLOCK * int(sizeof(St)));
         const Scale ss = scale_of<St>(over_column(largest(s))), os = scale_of<St>(over_column(largest(o)));
         Frag<St, WIDE> sf[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; kb++) {
             sf[kb] = frag_of<St, WIDE>(s[2 * kb], s[2 * kb + 1], ss.up);
-            if (held) leave(walked.states + row * DK + 32 * kb + 8 * grp, sf[kb]);
+            leave(blocks, state_at + 32 * kb * sizeof(St), sf[kb]);
         }
         // dU = l K dS + P^T dO
         Frag<St, 1> of[2];
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) of[kb] = frag_of<St, 1>(o[2 * kb], o[2 * kb + 1], os.up);       // (these are a tensor's elements: nothing is rounded off)
         const float dp = os.down * (1.0f / SQUARE<St>);
-        f4 u[4];
+        f4 u[4], w[4];
+#pragma unroll
+        for (int it = 0; it < 4; it++) u[it] = w[it] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int it = 0; it < 2 * kb + 2; it++) mma(w[it], Pt.cols(16 * it, kb), of[kb]);
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+            for (int it = 0; it < 4; it++) mma(u[it], Kt.rows(16 * it, kb), sf[kb]);
 #pragma unroll
         for (int it = 0; it < 4; it++) {
-            f4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-#pragma unroll
-            for (int kb = 0; kb < KB; kb++) mma(x, Kt.rows(16 * it, kb), sf[kb]);
-#pragma unroll
-            for (int kb = it / 2; kb < 2; kb++) mma(y, Pt.cols(16 * it, kb), of[kb]);
             const f4 ls = four(st.l, it);
 #pragma unroll
-            for (int r = 0; r < 4; r++) u[it][r] = fmaf(dp, y[r], ls[r] == 0.0f ? 0.0f : ls[r] * (ss.down * x[r]));
+            for (int r = 0; r < 4; r++) u[it][r] = fmaf(dp, w[it][r], ls[r] == 0.0f ? 0.0f : ls[r] * (ss.down * u[it][r]));
         }
         // dR = T^T dU
         const Scale us = scale_of<St>(over_column(largest(u)));
@@ -131,40 +119,38 @@ __global__ __launch_bounds__(W * WAVE) void walk_kernel(const E* __restrict__ qu
         const float du = us.down * (1.0f / SQUARE<St>);
         f4 d[4];
 #pragma unroll
-        for (int it = 0; it < 4; it++) {
-            d[it] = f4{0, 0, 0, 0};
+        for (int it = 0; it < 4; it++) d[it] = f4{0, 0, 0, 0};
 #pragma unroll
-            for (int kb = it / 2; kb < 2; kb++) mma(d[it], Tt.cols(16 * it, kb), uf[kb]);
-            d[it] *= du;
-        }
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int it = 0; it < 2 * kb + 2; it++) mma(d[it], Tt.cols(16 * it, kb), uf[kb]);
+#pragma unroll
+        for (int it = 0; it < 4; it++) d[it] *= du;
         const Scale ds = scale_of<St>(over_column(largest(d)));
-        E* to = d_value + ((b * S.T + t0) * S.G + g) * S.V + col;
+        const Buffer to = rows_at(d_value + ((b * S.T + n * C) * S.G + g) * S.V, vt, rows, S.V);
         f4 x[4], y[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) {
-            const f4 bs = four(st.b, it), bd = bs * d[it];
+            const f4 bd = four(st.b, it) * d[it];
             x[it] = four(st.q, it) * o[it];
             y[it] = -four(st.x, it) * bd;
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int i = 16 * it + 4 * grp + r;
-                if (on && t0 + i < S.T) to[int64_t(i) * S.G * S.V] = E(bd[r]);
-            }
+            for (int r = 0; r < 4; r++) Sixteen<E>::store(to, vt, value_at, 4 * it + r, bd[r]);
         }
+        // (q and x are 2 / LONG at most)
         const Scale xs = scale_of<St>(over_column(fmaxf(largest(x), largest(y))));
         Frag<St, WIDE> xf[2], yf[2];
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
-            if (held) leave(walked.steps + row * C + 32 * kb + 8 * grp, frag_of<St, 1>(d[2 * kb], d[2 * kb + 1], ds.up));
+            leave(blocks, step_at + 32 * kb * sizeof(St), frag_of<St, 1>(d[2 * kb], d[2 * kb + 1], ds.up));
             xf[kb] = frag_of<St, WIDE>(x[2 * kb], x[2 * kb + 1], xs.up);
             yf[kb] = frag_of<St, WIDE>(y[2 * kb], y[2 * kb + 1], xs.up);
         }
-        if (held && grp == 0) {
-            float* scales = walked.scales + (bg * S.chunks + n) * 3 * S.vp + col;
-            scales[0] = ss.down;
-            scales[S.vp] = ds.down;
-            scales[2 * S.vp] = os.down;
-        }
+        const Buffer scales(walked.scales + 3 * at, 3 * int64_t(S.vp) * 4);
+        const uint32_t scale_at = grp == 0 && col < S.vp ? col * 4 : NOWHERE;
+        scales.store(ss.down, scale_at);
+        scales.store(ds.down, scale_at, S.vp * 4);
+        scales.store(os.down, scale_at, 2 * S.vp * 4);
         const float end = st.end;
 #pragma unroll
         for (int k = 0; k < ND; k++) {
@@ -177,6 +163,15 @@ __global__ __launch_bounds__(W * WAVE) void walk_kernel(const E* __restrict__ qu
 #pragma unroll
             for (int r = 0; r < 4; r++) s[k][r] = fmaf(xs.down, z[r], end == 0.0f ? 0.0f : end * s[k][r]);
         }
+        if (n) {
+            if constexpr (BUFFERS == 2) {
+                arrived<16 + KB + 5>();    // (all but this chunk's stores)
+            } else {
+                __syncthreads();
+                fetch(n - 1);
+                arrived<0>();
+            }
+        }
     }
     if (!d_state) return;
 #pragma unroll
@@ -188,13 +183,14 @@ __global__ __launch_bounds__(W * WAVE) void walk_kernel(const E* __restrict__ qu
         }
 }
 
-// ---- gradient_kernel: a workgroup of four waves for each chunk of each query and key head. A wave has 16 steps' rows of every product;
-// columns of values are summed over in blocks of 32, staged while the block before is used.
+// ---- gradient_kernel: a workgroup of eight waves for each chunk of each query and key head. A wave has 16 steps' rows of every product
+// and half of its columns; columns of values are summed over in blocks of 32, which come to LDS while the block before is used where
+// two have room.
 //
 // Five products are summed over columns of values, whose operands have a scale for each column. The two scales of a column go to the
 // left operand, over the largest of them: what they push below float16's numbers is that far below the sum's largest terms.
 
-constexpr int BLOCK_V = 32, PRODUCTS = 5;
+constexpr int BANDS = 4, HALVES = 2, MANY = BANDS * HALVES * WAVE, PRODUCTS = 5;
 
 __device__ inline float row16(float x) {   // a sum over the 16 lanes that have a row's columns
 #pragma unroll
@@ -204,57 +200,39 @@ __device__ inline float row16(float x) {   // a sum over the 16 lanes that have 
 __device__ inline int exponent(float x) { return int(__float_as_uint(x) >> 23) - 127; }
 
 template <typename E, int DK>
-__global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ query, const E* __restrict__ key, const E* __restrict__ gate, const E* __restrict__ write,
-                                                         const E* __restrict__ d_out, Shape S, const Chunk<typename Rep<E>::S>* __restrict__ records,
-                                                         const Kept<typename Rep<E>::S> kept, const Kept<typename Rep<E>::S> walked, E* __restrict__ d_query,
-                                                         E* __restrict__ d_key, E* __restrict__ d_gate, E* __restrict__ d_write) {
+__global__ __launch_bounds__(MANY) void gradient_kernel(const E* __restrict__ gate, const E* __restrict__ write, const E* __restrict__ d_out, Shape S,
+                                                        const char* __restrict__ records, const char* __restrict__ images, const Kept<typename Rep<E>::S, DK> kept,
+                                                        const Kept<typename Rep<E>::S, DK> walked, E* __restrict__ d_query, E* __restrict__ d_key,
+                                                        E* __restrict__ d_gate, E* __restrict__ d_write) {
     using St = typename Rep<E>::S;
+    using Ke = Kept<St, DK>;
+    using Re = Record<St>;
     constexpr bool HALF = sizeof(St) == 2;
-    constexpr int ND = DK / 16, KB = DK / 32, PER = DK / 8;
+    constexpr int ND = DK / 16 / HALVES, KB = DK / 32, WAVES = MANY / WAVE, UNIT = 16 / int(sizeof(St));
     using In = Tile<St, C, DK>;
-    using Ot = Tile<St, C, BLOCK_V>;
-    using Sv = Tile<St, BLOCK_V, DK>;
-    using Uv = Tile<St, BLOCK_V, C>;
+    using Ot = Tile<St, C, COLS>;
+    using Sv = Tile<St, COLS, DK>;
+    using Uv = Tile<St, COLS, C>;
     using Square = Tile<St, C, C>;
-    using In8 = Rows<E, DK, BLOCK>;
-    constexpr int STAGED = Ot::SIZE + 2 * Sv::SIZE + 2 * Uv::SIZE, MORE = STAGED > 3 * Square::SIZE ? STAGED : 3 * Square::SIZE;
-    __shared__ alignas(16) St lds[2 * In::SIZE + MORE];
+    static_assert(Sv::SIZE + Uv::SIZE == Ke::BLOCK, "blocks lie in LDS as they are kept");
+    constexpr int BUFFERS = HALF ? 2 : 1, IN = IMAGE<St, DK>, BLOCK = Ke::BLOCK * int(sizeof(St)), BUFFER = 2 * BLOCK + Ot::SIZE * int(sizeof(St));
+    constexpr int MORE = BUFFERS * BUFFER > 3 * Square::SIZE * int(sizeof(St)) ? BUFFERS * BUFFER : 3 * Square::SIZE * int(sizeof(St));
+    __shared__ alignas(1024) char lds[IN + MORE];
     __shared__ alignas(16) Steps st;
-    __shared__ alignas(16) St factors[PRODUCTS][BLOCK_V];
-    __shared__ float rows[C], columns[WAVES][C], left[C], whole[WAVES], writes[C];
+    __shared__ alignas(16) St factors[2][PRODUCTS][COLS];
+    __shared__ float rows[HALVES][C], columns[BANDS][C], left[HALVES][C], whole[WAVES], writes[C], dots[2][HALVES][C];
     __shared__ int tops[WAVES][PRODUCTS];
-    const In Kt{lds}, Qt{lds + In::SIZE};
-    St* const more = lds + 2 * In::SIZE;
-    const Ot Od{more};
-    const Sv S0{more + Ot::SIZE}, S1{more + Ot::SIZE + Sv::SIZE};
-    const Uv Us{more + Ot::SIZE + 2 * Sv::SIZE}, Rs{more + Ot::SIZE + 2 * Sv::SIZE + Uv::SIZE};
+    const In Kt{reinterpret_cast<St*>(lds)}, Qt{reinterpret_cast<St*>(lds) + In::SIZE};
+    St* const more = reinterpret_cast<St*>(lds + IN);
     const Square Ek{more}, Eq{more + Square::SIZE}, Ff{more + 2 * Square::SIZE};       // (once the blocks of values have been used)
-    const int tid = threadIdx.x, wave = tid / WAVE, l = tid % WAVE, grp = l / 16, m = l % 16, band = 16 * wave;
+    const int tid = threadIdx.x, wave = tid / WAVE, l = tid % WAVE, grp = l / 16, m = l % 16, half = wave / BANDS, own = wave % BANDS, band = 16 * own, d0 = half * DK / 2;
     const int64_t chunk = blockIdx.x % S.chunks, bh = blockIdx.x / S.chunks;
     const int64_t b = bh / S.H, t0 = chunk * C;
     const int h = int(bh % S.H), share = S.G / S.H, steps = int(S.T - t0 < C ? S.T - t0 : C);
     // products of E and F with keys and queries, over numbers of values each
     const int many = HALF ? 32 - __builtin_clz(S.V) : 0;
     const float few = __uint_as_float((127 - many) << 23);
-    {
-        In8 q, k;
-        float qr[In8::COUNT], kr[In8::COUNT];
-        const Steps& first = records[(b * S.G + h * share) * S.chunks + chunk].steps;
-        q.load(query + b * S.qb + t0 * S.qt + h * S.qh, S.qt, steps, S.K);
-        k.load(key + b * S.kb + t0 * S.kt + h * S.kh, S.kt, steps, S.K);
-#pragma unroll
-        for (int j = 0; j < In8::COUNT; j++) {
-            kr[j] = first.rk[In8::row(j)];
-            qr[j] = first.rq[In8::row(j)];
-        }
-        In8::clear(Qt, S.K);
-        In8::clear(Kt, S.K);
-#pragma unroll
-        for (int j = 0; j < In8::COUNT; j++) {
-            q.put(Qt, j, length_up<St>(qr[j]), S.K);
-            k.put(Kt, j, length_up<St>(kr[j]), S.K);
-        }
-    }
+    bring<WAVES>(images + (bh * S.chunks + chunk) * IN, lds, 2 * In::SIZE * int(sizeof(St)));
     const f4 zero = {0, 0, 0, 0};
     f4 tq[ND], tk[ND];                     // the gradients of the query and the key of length 1, over the value heads so far
 #pragma unroll
@@ -264,15 +242,67 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
         const int g = h * share + j;
         const int64_t at = (b * S.G + g) * S.chunks + chunk;
         const E* o0 = d_out + b * S.ob + t0 * S.ot + g * S.og;
-        const St *s0 = kept.states + at * S.vp * DK, *s1 = walked.states + at * S.vp * DK, *u0 = kept.steps + at * S.vp * C, *r0 = walked.steps + at * S.vp * C;
+        const St *b0 = kept.blocks + at * (S.vp / COLS) * Ke::BLOCK, *b1 = walked.blocks + at * (S.vp / COLS) * Ke::BLOCK;
         const float *f0 = kept.scales + at * 3 * S.vp, *f1 = walked.scales + at * 3 * S.vp;    // of S, U and of dS, dR, dO
-        const auto left_scale = [&](int p, int c) { return p == 2 ? f0[S.vp + c] : p == 0 || p == 3 ? f1[2 * S.vp + c] : f1[S.vp + c]; };
-        const auto right_scale = [&](int p, int c) { return p < 2 ? f0[c] : p == 2 ? f1[c] : f0[S.vp + c]; };
-        if constexpr (HALF) {              // the largest of the columns' scales, by product: dO S, dR S, U dS, dO U, dR U
+        const auto left_scale = [&](int p) { return p == 2 ? f0 + S.vp : p == 0 || p == 3 ? f1 + 2 * S.vp : f1 + S.vp; };
+        const auto right_scale = [&](int p) { return p < 2 ? f0 : p == 2 ? f1 : f0 + S.vp; };
+        f4 aq[ND], from[ND], to[ND], dp[2], da[2];     // (of 16 x 16 up to the diagonal a wave has those at columns half, half + 2)
+#pragma unroll
+        for (int n = 0; n < ND; n++) aq[n] = from[n] = to[n] = zero;
+        dp[0] = dp[1] = da[0] = da[1] = zero;
+        float both = 0.0f;                 // of state and gradient, summed over all elements
+        // d_out's 64 rows of 32 columns: four elements a lane; lanes 0 .. 159 the factors of a product's column
+        const int orow = tid / 8, ocol = tid % 8 * 4, product = tid / COLS < PRODUCTS ? tid / COLS : 0, column = tid % COLS;
+        const Buffer outs = rows_at(o0, S.ot, steps, S.V);
+        const uint32_t out_at = (orow * S.ot + ocol) * uint32_t(sizeof(E));
+        const float *fl = left_scale(product), *fr = right_scale(product);
+        uint32_t op[4];
+        f4 os = {1.0f, 1.0f, 1.0f, 1.0f};
+        float lf = 1.0f, rf = 1.0f;
+        auto fetch = [&](int v0, int to) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t off = v0 + ocol + e < S.V ? out_at + (v0 + e) * uint32_t(sizeof(E)) : NOWHERE;
+                if constexpr (sizeof(E) == 2) op[e] = __builtin_amdgcn_raw_buffer_load_b16(outs.r, off, 0, 0);
+                else op[e] = __builtin_amdgcn_raw_buffer_load_b32(outs.r, off, 0, 0);
+            }
+            if constexpr (HALF) {
+                os = *reinterpret_cast<const f4*>(f1 + 2 * S.vp + v0 + ocol);
+                lf = fl[v0 + column];
+                rf = fr[v0 + column];
+            }
+            char* buffer = lds + IN + to * BUFFER;
+            bring<WAVES>(b0 + v0 / COLS * Ke::BLOCK, buffer, BLOCK);
+            bring<WAVES>(b1 + v0 / COLS * Ke::BLOCK, buffer + BLOCK, BLOCK);
+        };
+        auto put = [&](int v0, int to) {   // what went by way of registers
+            const Ot Od{reinterpret_cast<St*>(lds + IN + to * BUFFER + 2 * BLOCK)};
+            pack<St, 4> x;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float d = Sixteen<E>::value(op[e]);
+                x.v[e] = St(HALF ? d * __uint_as_float((254u << 23) - __float_as_uint(os[e])) : d);    // (over a power of two)
+            }
+            x.store(Od.p + orow * Ot::ROW + place(ocol));
+            if constexpr (HALF) if (tid < PRODUCTS * COLS) {
+                int top = -1000;
+#pragma unroll
+                for (int w = 0; w < WAVES; w++) top = max(top, tops[w][product]);
+                const int e = exponent(lf) + exponent(rf) - top;       // 0 at most
+                factors[to][product][place(column)] = e > -25 ? St(__uint_as_float((127 + e) << 23)) : St(0.0f);
+            }
+        };
+        if (j) __syncthreads();            // the value head before has been dealt with
+        fetch(0, 0);
+        {                                  // the steps' record, and the largest of the columns' scales by product: dO S, dR S, U dS, dO U, dR U
+            const float* p = reinterpret_cast<const float*>(&reinterpret_cast<const Re*>(record_of<St>(const_cast<char*>(records), at))->steps);
+            for (int k = tid; k < int(sizeof(Steps) / 4); k += MANY) reinterpret_cast<float*>(&st)[k] = p[k];
+        }
+        if constexpr (HALF) {
             int top[PRODUCTS];
 #pragma unroll
             for (int p = 0; p < PRODUCTS; p++) top[p] = -1000;
-            for (int c = tid; c < S.vp; c += BLOCK) {
+            for (int c = tid; c < S.vp; c += MANY) {
                 const int es = exponent(f0[c]), eu = exponent(f0[S.vp + c]), ed = exponent(f1[c]), er = exponent(f1[S.vp + c]), eo = exponent(f1[2 * S.vp + c]);
                 top[0] = max(top[0], eo + es);
                 top[1] = max(top[1], er + es);
@@ -287,86 +317,20 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
                 if (l == 0) tops[wave][p] = top[p];
             }
         }
-        f4 aq[ND], from[ND], to[ND], dp[WAVES], da[WAVES];
-#pragma unroll
-        for (int n = 0; n < ND; n++) aq[n] = from[n] = to[n] = zero;
-#pragma unroll
-        for (int n = 0; n < WAVES; n++) dp[n] = da[n] = zero;
-        float both = 0.0f;                 // of state and gradient, summed over all elements
-        constexpr int SP = BLOCK_V * PER / BLOCK ? BLOCK_V * PER / BLOCK : 1;
-        pack<E, 8> op;
-        pack<float, 8> os;
-        pack<St, 8> s0p[SP], s1p[SP], up, rp;
-        float sd[SP], lf, rf;
-        // (columns behind the last are read as the last one and put as 0; d_out's last eight one by one where V is no multiple of 8)
-        const int oc = tid % 4 * 8, orow = tid / 4, urow = tid / 8, ucol = tid % 8 * 8;
-        const E* orow0 = o0 + int64_t(orow < steps ? orow : steps - 1) * S.ot;
-        const auto last = [&](int c) { return c < S.vp ? c : S.vp - 1; };
-        auto fetch = [&](int v0) {
-            if (S.V % 8 == 0) {
-                op = pack<E, 8>::load(orow0 + (v0 + oc < S.V ? v0 + oc : S.V - 8));
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; e++) op.v[e] = orow0[v0 + oc + e < S.V ? v0 + oc + e : S.V - 1];
-            }
-            if constexpr (HALF) {
-                os = pack<float, 8>::load(f1 + 2 * S.vp + (v0 + oc < S.vp ? v0 + oc : S.vp - 8));
-                lf = left_scale(tid / BLOCK_V < PRODUCTS ? tid / BLOCK_V : 0, last(v0 + tid % BLOCK_V));
-                rf = right_scale(tid / BLOCK_V < PRODUCTS ? tid / BLOCK_V : 0, last(v0 + tid % BLOCK_V));
-            }
-            up = pack<St, 8>::load(u0 + int64_t(last(v0 + urow)) * C + ucol);
-            rp = pack<St, 8>::load(r0 + int64_t(last(v0 + urow)) * C + ucol);
-#pragma unroll
-            for (int k = 0; k < SP; k++) {
-                const int p = tid + k * BLOCK, c = last(v0 + p / PER);
-                s0p[k] = pack<St, 8>::load(s0 + int64_t(c) * DK + p % PER * 8);
-                s1p[k] = pack<St, 8>::load(s1 + int64_t(c) * DK + p % PER * 8);
-                if constexpr (HALF) sd[k] = f0[c] * f1[c];
-                else sd[k] = 1.0f;
-            }
-        };
-        fetch(0);
-        for (int v0 = 0; v0 < S.vp; v0 += BLOCK_V) {
-            __syncthreads();               // what lies there has been used
-            {
-                St x[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float d = v0 + oc + e < S.V ? float(op.v[e]) : 0.0f;
-                    x[e] = St(HALF ? d * __uint_as_float((254u << 23) - __float_as_uint(os.v[e])) : d);    // (over a power of two)
-                }
-                Od.put(orow, oc, x);
-            }
-            if constexpr (HALF) if (tid < PRODUCTS * BLOCK_V) {
-                const int p = tid / BLOCK_V, c = tid % BLOCK_V;
-                const int top = max(max(tops[0][p], tops[1][p]), max(tops[2][p], tops[3][p]));
-                const int e = exponent(lf) + exponent(rf) - top;   // 0 at most
-                factors[p][place(c)] = v0 + c < S.vp && e > -25 ? St(__uint_as_float((127 + e) << 23)) : St(0.0f);
-            }
-            const pack<St, 8> none = {};
-            Us.put_places(urow, ucol, v0 + urow < S.vp ? up : none);
-            Rs.put_places(urow, ucol, v0 + urow < S.vp ? rp : none);
-#pragma unroll
-            for (int k = 0; k < SP; k++) {
-                const int p = tid + k * BLOCK;
-                if (p < BLOCK_V * PER) {
-                    const bool on = v0 + p / PER < S.vp;
-                    S0.put_places(p / PER, p % PER * 8, on ? s0p[k] : none);
-                    S1.put_places(p / PER, p % PER * 8, on ? s1p[k] : none);
-                    float x = 0.0f;
-#pragma unroll
-                    for (int c = 0; c < 8; c++) x = fmaf(float(s0p[k].v[c]), float(s1p[k].v[c]), x);
-                    if (on) both = fmaf(x, sd[k], both);
-                }
-            }
-            if (v0 == 0) {                 // the steps' record with the first block
-                const float* p = reinterpret_cast<const float*>(&records[at].steps);
-                for (int k = tid; k < int(sizeof(Steps) / 4); k += BLOCK) reinterpret_cast<float*>(&st)[k] = p[k];
-            }
-            __syncthreads();
-            if (v0 + BLOCK_V < S.vp) fetch(v0 + BLOCK_V);
+        __syncthreads();
+        put(0, 0);
+        arrived<0>();
+        int now = 0;
+        for (int v0 = 0; v0 < S.vp; v0 += COLS) {
+            __syncthreads();               // the block is there, and the one before has been used
+            const bool next = v0 + COLS < S.vp;
+            St* buffer = reinterpret_cast<St*>(lds + IN + now * BUFFER);
+            if (BUFFERS == 2 && next) fetch(v0 + COLS, now ^ 1);
+            const Sv S0{buffer}, S1{buffer + Ke::BLOCK};
+            const Uv Us{buffer + Sv::SIZE}, Rs{buffer + Ke::BLOCK + Sv::SIZE};
+            const Ot Od{buffer + 2 * Ke::BLOCK};
             const auto scaled = [&](auto f, int p) {
-                if constexpr (HALF) f.p[0] *= *reinterpret_cast<const h8*>(&factors[p][8 * grp]);
+                if constexpr (HALF) f.p[0] *= *reinterpret_cast<const h8*>(&factors[now][p][8 * grp]);
                 return f;
             };
             const auto of = Od.rows(band, 0);
@@ -374,30 +338,57 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
             const auto of0 = scaled(of, 0), rf1 = scaled(rf, 1), uf2 = scaled(uf, 2), of3 = scaled(of, 3), rf4 = scaled(rf, 4);
 #pragma unroll
             for (int n = 0; n < ND; n++) {
-                const auto sf = S0.cols(16 * n, 0);
+                const auto sf = S0.cols(d0 + 16 * n, 0);
                 mma(aq[n], of0, sf);
                 mma(from[n], rf1, sf);
-                mma(to[n], uf2, S1.cols(16 * n, 0));
+                mma(to[n], uf2, S1.cols(d0 + 16 * n, 0));
             }
 #pragma unroll
-            for (int n = 0; n < WAVES; n++) if (n <= wave) {
-                const auto un = Us.cols(16 * n, 0);
-                mma(dp[n], of3, un);
-                mma(da[n], rf4, un);
+            for (int k = 0; k < 2; k++) if (half + 2 * k <= own) {
+                const auto un = Us.cols(16 * (half + 2 * k), 0);
+                mma(dp[k], of3, un);
+                mma(da[k], rf4, un);
+            }
+            for (int p = tid; p < COLS * DK / UNIT; p += MANY) {
+                const int c = p / (DK / UNIT), at = c * Sv::ROW + p % (DK / UNIT) * UNIT;
+                const auto x = pack<St, UNIT>::load(S0.p + at), y = pack<St, UNIT>::load(S1.p + at);
+                float z = 0.0f;
+#pragma unroll
+                for (int e = 0; e < UNIT; e++) z = fmaf(float(x.v[e]), float(y.v[e]), z);
+                both = fmaf(z, HALF ? f0[v0 + c] * f1[v0 + c] : 1.0f, both);
+            }
+            if (next) {
+                if constexpr (BUFFERS == 1) {
+                    __syncthreads();
+                    fetch(v0 + COLS, 0);
+                }
+                put(v0 + COLS, BUFFERS == 2 ? now ^ 1 : 0);
+                arrived<0>();
+                if (BUFFERS == 2) now ^= 1;
             }
         }
         int top[PRODUCTS];
 #pragma unroll
-        for (int p = 0; p < PRODUCTS; p++) top[p] = HALF ? max(max(tops[0][p], tops[1][p]), max(tops[2][p], tops[3][p])) : 0;
+        for (int p = 0; p < PRODUCTS; p++) {
+            top[p] = HALF ? -1000 : 0;
+            if constexpr (HALF) {
+#pragma unroll
+                for (int w = 0; w < WAVES; w++) top[p] = max(top[p], tops[w][p]);
+            }
+        }
         const uint64_t cuts = uint64_t(st.cut[1]) << 32 | st.cut[0];
         // what a step has of the state before the chunk and leaves after it, and its row's sums
-        float bi[4], rowsum[4], rki[4], rqi[4];
+        float bi[4], rowsum[4], rki[4], rqi[4], hi[4], lo[4];
+        int since_i[4];
         const float last_hi = st.hi[C - 1], last_lo = st.lo[C - 1];
+        const int last_cut = since(cuts, C - 1);
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int i = band + 4 * grp + r;
-            const float gi = since(cuts, i) >= 0 ? 0.0f : expf(st.hi[i]);
-            const float li = i < since(cuts, C - 1) ? 0.0f : expf((last_hi - st.hi[i]) + (last_lo - st.lo[i]));
+            hi[r] = st.hi[i];
+            lo[r] = st.lo[i];
+            since_i[r] = since(cuts, i);
+            const float gi = since_i[r] >= 0 ? 0.0f : expf(hi[r]), li = i < last_cut ? 0.0f : expf((last_hi - hi[r]) + (last_lo - lo[r]));
             bi[r] = st.b[i];
             rki[r] = length_rest<St>(st.rk[i]);
             rqi[r] = length_rest<St>(st.rq[i]);
@@ -406,7 +397,7 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
             for (int n = 0; n < ND; n++) {
                 const float x = gi == 0.0f ? 0.0f : gi * ldexpf(aq[n][r], top[0]), y = gi == 0.0f ? 0.0f : -bi[r] * gi * ldexpf(from[n][r], top[1]);
                 const float z = li == 0.0f ? 0.0f : li * ldexpf(to[n][r], top[2]);
-                const float q = float(Qt.get(i, 16 * n + m)), k = float(Kt.get(i, 16 * n + m));
+                const float q = float(Qt.get(i, d0 + 16 * n + m)), k = float(Kt.get(i, d0 + 16 * n + m));
                 dq = fmaf(q, x, dq);
                 df = fmaf(k, y, df);
                 dt = fmaf(k, z, dt);
@@ -415,19 +406,17 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
             }
             rowsum[r] = rqi[r] * dq + rki[r] * df;
             dt = row16(dt);
-            if (m == 0) left[i] = rki[r] * dt;
+            if (m == 0) left[half][i] = rki[r] * dt;
         }
-        f4 kk[WAVES], qk[WAVES];
-#pragma unroll
-        for (int n = 0; n < WAVES; n++) kk[n] = qk[n] = zero;
+        f4 kk[2] = {zero, zero}, qk[2] = {zero, zero};
 #pragma unroll
         for (int kb = 0; kb < KB; kb++) {
             const auto ka = Kt.rows(band, kb), qa = Qt.rows(band, kb);
 #pragma unroll
-            for (int n = 0; n < WAVES; n++) if (n <= wave) {
-                const auto kn = Kt.rows(16 * n, kb);
-                mma(kk[n], ka, kn);
-                mma(qk[n], qa, kn);
+            for (int k = 0; k < 2; k++) if (half + 2 * k <= own) {
+                const auto kn = Kt.rows(16 * (half + 2 * k), kb);
+                mma(kk[k], ka, kn);
+                mma(qk[k], qa, kn);
             }
         }
         both = wave_sum(both);
@@ -435,28 +424,28 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
         __syncthreads();                   // the last block of values has been used
         // E and F with the lengths of what they are multiplied by, F on both sides of the diagonal
 #pragma unroll
-        for (int n = 0; n < WAVES; n++) {
-            const int c = 16 * n + m;
-            const float rk = length_rest<St>(st.rk[c]), hi = st.hi[c], lo = st.lo[c];
+        for (int k = 0; k < 2; k++) {
+            const int c = 16 * (half + 2 * k) + m;
+            const float rk = length_rest<St>(st.rk[c]), hc = st.hi[c], lc = st.lo[c];
             float column = 0.0f;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int i = band + 4 * grp + r;
-                const bool on = c <= i && c >= since(cuts, i);
+                const bool on = c <= i && c >= since_i[r];
                 float e = 0.0f, f = 0.0f;
                 if (on) {
-                    const float M = expf((st.hi[i] - hi) + (st.lo[i] - lo));
-                    e = M * dp[n][r];
+                    const float M = expf((hi[r] - hc) + (lo[r] - lc));
+                    e = M * dp[k][r];
                     if (c < i) {
-                        f = -M * bi[r] * da[n][r];
-                        const float pair = ldexpf(e * rqi[r] * rk * qk[n][r], top[3]) + ldexpf(f * rki[r] * rk * kk[n][r], top[4]);
+                        f = -M * bi[r] * da[k][r];
+                        const float pair = ldexpf(e * rqi[r] * rk * qk[k][r], top[3]) + ldexpf(f * rki[r] * rk * kk[k][r], top[4]);
                         rowsum[r] += pair;
                         column += pair;
                     } else {
-                        writes[i] = ldexpf(da[n][r], top[4]);
+                        writes[i] = ldexpf(da[k][r], top[4]);
                     }
                 }
-                // (numbers up to 2^28 V, of factors up to 2^14: V 2^14 of them, and lengths, are taken out)
+                // (dp and da are 2^28 V at most, a length's rest 2 / LONG: what is left is 2^14)
                 constexpr float FIT = HALF ? 0x1p-15f * LONG<St> : 1.0f;
                 e *= few * FIT;
                 f *= few * FIT;
@@ -469,25 +458,32 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
             }
             column += __shfl_xor(column, 16, WAVE);
             column += __shfl_xor(column, 32, WAVE);
-            if (grp == 0) columns[wave][c] = column;
+            if (grp == 0) columns[own][c] = column;
         }
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const float x = row16(rowsum[r]);
-            if (m == 0) rows[band + 4 * grp + r] = x;
+            if (m == 0) rows[half][band + 4 * grp + r] = x;
         }
         __syncthreads();
         constexpr int OUT = HALF ? 15 - 6 : 0;             // (what FIT took out)
         static_assert(!HALF || LONG<St> == 64.0f, "the exponent of LONG");
+        Frag<St, 1> ek[2], eq[2], ff[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++) {
+            ek[kb] = Ek.rows(band, kb);
+            eq[kb] = Eq.cols(band, kb);
+            ff[kb] = Ff.rows(band, kb);
+        }
 #pragma unroll
         for (int n = 0; n < ND; n++) {
             f4 x = zero, y = zero, z = zero;
 #pragma unroll
             for (int kb = 0; kb < 2; kb++) {
-                const auto kn = Kt.cols(16 * n, kb);
-                mma(x, Ek.rows(band, kb), kn);
-                mma(y, Eq.cols(band, kb), Qt.cols(16 * n, kb));
-                mma(z, Ff.rows(band, kb), kn);
+                const auto kn = Kt.cols(d0 + 16 * n, kb);
+                mma(x, ek[kb], kn);
+                mma(z, ff[kb], kn);
+                mma(y, eq[kb], Qt.cols(d0 + 16 * n, kb));
             }
 #pragma unroll
             for (int r = 0; r < 4; r++) {
@@ -497,8 +493,8 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
         }
         if (wave == 0) {                   // a lane for each step: gates
             const auto same = [&](int i) { return i < C && since(cuts, i) <= l; };     // no step up to i, from the next on, drops the state
-            double after = double(rows[l]) - (double(columns[0][l]) + columns[1][l] + columns[2][l] + columns[3][l]);
-            double before = left[l];
+            double after = double(rows[0][l]) + rows[1][l] - (double(columns[0][l]) + columns[1][l] + columns[2][l] + columns[3][l]);
+            double before = double(left[0][l]) + left[1][l];
 #pragma unroll
             for (int d = 1; d < WAVE; d <<= 1) {
                 const double x = __shfl_down(after, d, WAVE), y = __shfl_up(before, d, WAVE);
@@ -510,79 +506,90 @@ __global__ __launch_bounds__(BLOCK) void gradient_kernel(const E* __restrict__ q
             const int64_t t = t0 + l;
             if (l < steps) {
                 const float x = float(gate[b * S.ab + t * S.at + g * S.ag]), w = float(write[b * S.wb + t * S.wt + g * S.wg]);
-                const bool first = since(cuts, l) < 0;
                 double d = after + before;
-                if (first && st.end != 0.0f) d += double(st.end) * (double(whole[0]) + whole[1] + whole[2] + whole[3]);
-                const bool cut = cuts >> l & 1;
-                d_gate[(b * S.T + t) * S.G + g] = E(cut ? 0.0f : float(-d / (1.0 + exp(-double(x)))));
+                if (since(cuts, l) < 0 && st.end != 0.0f) {
+                    double sum = 0.0;
+#pragma unroll
+                    for (int w = 0; w < WAVES; w++) sum += whole[w];
+                    d += double(st.end) * sum;
+                }
+                d_gate[(b * S.T + t) * S.G + g] = E(cuts >> l & 1 ? 0.0f : float(-d / (1.0 + exp(-double(x)))));
                 d_write[(b * S.T + t) * S.G + g] = E(writes[l] / (1.0f + expf(w)));
             }
         }
     }
-    // of the query and the key themselves
-    E *dq0 = d_query + ((b * S.T + t0) * S.H + h) * S.K, *dk0 = d_key + ((b * S.T + t0) * S.H + h) * S.K;
+    // of the query and the key themselves: d - x^ (x^.d), over the length
+    const Buffer dq0 = rows_at(d_query + ((b * S.T + t0) * S.H + h) * S.K, S.H * S.K, steps, S.K), dk0 = rows_at(d_key + ((b * S.T + t0) * S.H + h) * S.K, S.H * S.K, steps, S.K);
+    float rk[4], rq[4], q[4][ND], k[4][ND];
 #pragma unroll
     for (int r = 0; r < 4; r++) {
         const int i = band + 4 * grp + r;
-        const float rk = st.rk[i], rq = st.rq[i], rkr = length_rest<St>(rk), rqr = length_rest<St>(rq);
-        float q[ND], k[ND], dq = 0.0f, dk = 0.0f;
+        rk[r] = st.rk[i];
+        rq[r] = st.rq[i];
+        const float rkr = length_rest<St>(rk[r]), rqr = length_rest<St>(rq[r]);
+        float dq = 0.0f, dk = 0.0f;
 #pragma unroll
         for (int n = 0; n < ND; n++) {
-            q[n] = float(Qt.get(i, 16 * n + m)) * rqr;
-            k[n] = float(Kt.get(i, 16 * n + m)) * rkr;
-            dq = fmaf(q[n], tq[n][r], dq);
-            dk = fmaf(k[n], tk[n][r], dk);
+            q[r][n] = float(Qt.get(i, d0 + 16 * n + m)) * rqr;
+            k[r][n] = float(Kt.get(i, d0 + 16 * n + m)) * rkr;
+            dq = fmaf(q[r][n], tq[n][r], dq);
+            dk = fmaf(k[r][n], tk[n][r], dk);
         }
         dq = row16(dq);
         dk = row16(dk);
+        if (m == 0) {
+            dots[0][half][i] = dq;
+            dots[1][half][i] = dk;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int i = band + 4 * grp + r;
+        const float dq = dots[0][0][i] + dots[0][1][i], dk = dots[1][0][i] + dots[1][1][i];
 #pragma unroll
         for (int n = 0; n < ND; n++) {
-            const int c = 16 * n + m;
-            if (i < steps && c < S.K) {
-                dq0[int64_t(i) * S.H * S.K + c] = E(rq * fmaf(-q[n], dq, tq[n][r]));
-                dk0[int64_t(i) * S.H * S.K + c] = E(rk * fmaf(-k[n], dk, tk[n][r]));
-            }
+            const int c = d0 + 16 * n + m;
+            const uint32_t to = c < S.K ? (i * S.H * S.K + c) * uint32_t(sizeof(E)) : NOWHERE;
+            dq0.store(E(rq[r] * fmaf(-q[r][n], dq, tq[n][r])), to);
+            dk0.store(E(rk[r] * fmaf(-k[r][n], dk, tk[n][r])), to);
         }
     }
 }
 
 template <typename E, int DK>
-int32_t backward(const void* query, const void* key, const void* gate, const void* write, const void* d_out, const float* d_last, const Shape& S, void* kept, void* records,
-                 void* d_query, void* d_key, void* d_value, void* d_gate, void* d_write, float* d_state, void* work, hipStream_t stream, char* err, size_t errcap) {
+int32_t backward(const void* gate, const void* write, const void* d_out, const float* d_last, const Shape& S, void* kept, const void* records, void* d_query, void* d_key,
+                 void* d_value, void* d_gate, void* d_write, float* d_state, void* work, hipStream_t stream, char* err, size_t errcap) {
     using St = typename Rep<E>::S;
-    constexpr int W = 4;
+    constexpr int W = 2;
     const auto in = [](const void* p) { return static_cast<const E*>(p); };
     const auto out = [](void* p) { return static_cast<E*>(p); };
-    const auto* rec = static_cast<const Chunk<St>*>(records);
-    const Kept<St> before(kept, S, DK), walked(work, S, DK);
-    walk_kernel<E, DK, W><<<dim3(S.B * S.G * ((S.vp / 16 + W - 1) / W)), W * WAVE, 0, stream>>>(in(query), in(key), in(d_out), d_last, S, rec, out(d_value), d_state, walked);
-    gradient_kernel<E, DK><<<dim3(S.B * S.H * S.chunks), BLOCK, 0, stream>>>(in(query), in(key), in(gate), in(write), in(d_out), S, rec, before, walked, out(d_query),
-                                                                            out(d_key), out(d_gate), out(d_write));
+    const int64_t heads = S.B * S.G;
+    const char *rec = static_cast<const char*>(records), *images = rec + heads * S.chunks * Record<St>::STRIDE;
+    const Kept<St, DK> before(kept, S), walked(work, S);
+    walk_kernel<E, DK, W><<<dim3(heads * ((S.vp / 16 + W - 1) / W)), W * WAVE, 0, stream>>>(in(d_out), d_last, S, rec, images, out(d_value), d_state, walked);
+    gradient_kernel<E, DK><<<dim3(S.B * S.H * S.chunks), MANY, 0, stream>>>(in(gate), in(write), in(d_out), S, rec, images, before, walked, out(d_query), out(d_key),
+                                                                           out(d_gate), out(d_write));
     return launched(err, errcap);
 }
 
 }  // namespace
 
-extern "C" int32_t pv_gated_delta_backward_hip(const void* query, const void* key, const void* gate, const void* write, const void* d_out, const float* d_last, int64_t B,
-                                               int64_t T, int32_t H, int32_t G, int32_t K, int32_t V, const int64_t* strides, float eps, int32_t dtype, const void* kept,
-                                               const void* records, void* d_query, void* d_key, void* d_value, void* d_gate, void* d_write, float* d_state, void* work,
-                                               uint64_t work_bytes, void* stream, char* err, size_t errcap) {
+extern "C" int32_t pv_gated_delta_backward_hip(const void* gate, const void* write, const void* d_out, const float* d_last, int64_t B, int64_t T, int32_t H, int32_t G,
+                                               int32_t K, int32_t V, const int64_t* strides, int32_t dtype, const void* kept, const void* records, void* d_query,
+                                               void* d_key, void* d_value, void* d_gate, void* d_write, float* d_state, void* work, uint64_t work_bytes, void* stream,
+                                               char* err, size_t errcap) {
     Shape S;
-    if (int32_t e = shape_of(B, T, H, G, K, V, strides, eps, dtype, S, err, errcap)) return e;
-    S.ob = strides[15];
-    S.ot = strides[16];
-    S.og = strides[17];
-    if (S.ot < -(1 << 24) || S.ot > 1 << 24) return fail(PV_EARG, err, errcap, "stride: a step's is 2^24 elements at most");
-    if (!query || !key || !gate || !write || !d_out || !kept || !records || !d_query || !d_key || !d_value || !d_gate || !d_write)
-        return fail(PV_EARG, err, errcap, "null argument");
+    if (int32_t e = shape_of(B, T, H, G, K, V, strides, 9, 0.0f, dtype, S, err, errcap)) return e;
+    if (!gate || !write || !d_out || !kept || !records || !d_query || !d_key || !d_value || !d_gate || !d_write) return fail(PV_EARG, err, errcap, "null argument");
     if (!aligned(kept, 16) || !aligned(records, 16)) return fail(PV_EARG, err, errcap, "kept, records: not 16-byte aligned");
     const uint64_t need = pv_gated_delta_kept_bytes(B, T, G, K, V, dtype);
     if (!work || work_bytes < need || !aligned(work, 16)) return fail(PV_EARG, err, errcap, "work: too small, or not 16-byte aligned");
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);
         return with_k(K, [&](auto k) {
-            return backward<E, decltype(k)::value>(query, key, gate, write, d_out, d_last, S, const_cast<void*>(kept), const_cast<void*>(records), d_query, d_key, d_value,
-                                                   d_gate, d_write, d_state, work, hipStream_t(stream), err, errcap);
+            return backward<E, decltype(k)::value>(gate, write, d_out, d_last, S, const_cast<void*>(kept), records, d_query, d_key, d_value, d_gate, d_write, d_state, work,
+                                                   hipStream_t(stream), err, errcap);
         });
     });
 }

@@ -8,8 +8,8 @@ from ._call import DTYPES, call, on_gpu, once, ptr
 
 
 def _strided(t):
-    """`t` with neighbouring elements in a head, and steps at most 2^24 elements apart: itself, or a copy."""
-    if (t.dim() == 4 and t.stride(3) != 1 and t.shape[3] != 1) or t.stride(1) > 1 << 24:
+    """`t` with neighbouring elements in a head, and steps at most 2^22 elements apart: itself, or a copy."""
+    if (t.dim() == 4 and t.stride(3) != 1 and t.shape[3] != 1) or t.stride(1) > 1 << 22:
         t = t.contiguous()
     return t
 
@@ -28,7 +28,7 @@ def _forward(index, query, key, value, gate, write, state, reset, eps, keep):
     last = torch.empty((B, G, K, V), dtype=torch.float32, device=dev)
     L, code = N.lib(), DTYPES[dtype]
     kept = torch.empty(L.pv_gated_delta_kept_bytes(B, T, G, K, V, code), dtype=torch.uint8, device=dev) if keep else None
-    size = L.pv_gated_delta_work_bytes(B, T, G, code, int(keep))
+    size = L.pv_gated_delta_work_bytes(B, T, H, G, K, code, int(keep))
     work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     call(L.pv_gated_delta_hip, index, *(t.data_ptr() for t in given), ptr(state), ptr(reset), B, T, H, G, K, V, _strides(*given), eps, code, out.data_ptr(),
          last.data_ptr(), ptr(kept), ptr(work), size)
@@ -39,18 +39,17 @@ class _GatedDelta(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, value, gate, write, state, reset, eps):
         out, last, kept, records = _forward(query.get_device(), query, key, value, gate, write, state, reset, eps, True)
-        ctx.save_for_backward(query, key, gate, write, kept, records)
-        ctx.values, ctx.has_state, ctx.eps = value.shape[2:], state is not None, eps
+        ctx.save_for_backward(gate, write, kept, records)          # (queries and keys are among the records)
+        ctx.shape, ctx.has_state = (*query.shape, *value.shape[2:]), state is not None
         ctx.set_materialize_grads(False)
         return out, last
 
     @staticmethod
     @once
     def backward(ctx, d_out, d_last):
-        query, key, gate, write, kept, records = ctx.saved_tensors
-        B, T, H, K = query.shape
-        G, V = ctx.values
-        dev, dtype = query.device, query.dtype
+        gate, write, kept, records = ctx.saved_tensors
+        B, T, H, K, G, V = ctx.shape
+        dev, dtype = gate.device, gate.dtype
         d_out = torch.zeros((B, T, G, V), dtype=dtype, device=dev) if d_out is None else _strided(d_out)
         d_last = None if d_last is None else d_last.contiguous()
         d_query, d_key, d_value, d_gate, d_write = (torch.empty(s, dtype=dtype, device=dev) for s in ((B, T, H, K), (B, T, H, K), (B, T, G, V), (B, T, G), (B, T, G)))
@@ -58,11 +57,10 @@ class _GatedDelta(torch.autograd.Function):
         L, code = N.lib(), DTYPES[dtype]
         size = L.pv_gated_delta_kept_bytes(B, T, G, K, V, code)
         work = torch.empty(size, dtype=torch.uint8, device=dev)
-        query, key, gate, write = (_strided(t) for t in (query, key, gate, write))
-        # (values are not read backwards: any strides stand for theirs)
-        call(L.pv_gated_delta_backward_hip, query.get_device(), query.data_ptr(), key.data_ptr(), gate.data_ptr(), write.data_ptr(), d_out.data_ptr(), ptr(d_last), B, T,
-             H, G, K, V, _strides(query, key, d_value, gate, write, d_out), ctx.eps, code, kept.data_ptr(), records.data_ptr(), d_query.data_ptr(), d_key.data_ptr(),
-             d_value.data_ptr(), d_gate.data_ptr(), d_write.data_ptr(), ptr(d_state), work.data_ptr(), size)
+        gate, write = _strided(gate), _strided(write)
+        call(L.pv_gated_delta_backward_hip, gate.get_device(), gate.data_ptr(), write.data_ptr(), d_out.data_ptr(), ptr(d_last), B, T, H, G, K, V,
+             _strides(gate, write, d_out), code, kept.data_ptr(), records.data_ptr(), d_query.data_ptr(), d_key.data_ptr(), d_value.data_ptr(), d_gate.data_ptr(),
+             d_write.data_ptr(), ptr(d_state), work.data_ptr(), size)
         return d_query, d_key, d_value, d_gate, d_write, d_state, None, None
 
 
