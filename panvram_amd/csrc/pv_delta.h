@@ -303,16 +303,15 @@ template <typename S, int DK> constexpr int IMAGE = (2 * Tile<S, C, DK>::SIZE * 
 inline uint64_t image_bytes(int32_t dk, int32_t dtype) { return (2 * 64 * (dtype == PV_F32 ? (dk + 4) * 4 : (dk + 8) * 2) + 1023) / 1024 * 1024; }
 template <typename S> __device__ __host__ inline char* record_of(char* work, int64_t chunk) { return work + chunk * Record<S>::STRIDE; }
 
-// `bytes` of memory to LDS, by all W waves, 1,024 at a time (those behind the last whole kilobyte too, up to the next). Both begin at
+// `bytes` of memory to LDS, by W waves of which this is number `wave`, 1,024 at a time (those behind the last whole kilobyte too, up to the next). Both begin at
 // 16 bytes' alignment. The lanes' data goes from the memory system to LDS by itself: bring() returns at once, and the memory is there
 // for a wave's own reads after arrived<N>(), N at most the number of its loads and stores since, and for the workgroup's after a barrier.
-template <int W> __device__ inline void bring(const void* from, void* to, int bytes) {
+template <int W> __device__ inline void bring(const void* from, void* to, int bytes, int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE)) {
     const uint64_t base = reinterpret_cast<uint64_t>(from);
     const int last = (bytes + 1023) / 1024 - 1;
     const __attribute__((ext_vector_type(4))) int r = {__builtin_amdgcn_readfirstlane(int(base)), __builtin_amdgcn_readfirstlane(int(base >> 32)), (last + 1) * 1024,
                                                                0x00027000};
     const uint32_t lds = __builtin_amdgcn_readfirstlane(int(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)to)));
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     for (int k = 0; k <= last; k += W) {   // (a wave without a kilobyte of its own copies the last one once more)
         const int at = (k + wave < last ? k + wave : last) * 1024;
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds + at), "v"(threadIdx.x % WAVE * 16), "s"(r), "s"(at)

@@ -234,11 +234,12 @@ __global__ __launch_bounds__(BLOCK) void chunk_kernel(const E* __restrict__ quer
     record<St>(T, ROW, out.inv, 0, BLOCK);
 }
 
-// ---- state_kernel: a workgroup of W waves for 16 W columns of a state. Chunks come to LDS while the one before is worked on, where
-// two have room (tensors of 16 bits), else one after another.
+// ---- state_kernel: a workgroup of W waves for 16 W columns of a state, and a wave more that brings chunks to LDS: while the one before is
+// worked on, where two have room (tensors of 16 bits), else one after another. (A wave that brings is held up until the memory system
+// has taken all it asks for, 3 us a chunk.)
 
 template <typename E, int DK, int W, bool KEEP>
-__global__ __launch_bounds__(W * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))) void state_kernel(
+__global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))) void state_kernel(
     const E* __restrict__ value, const float* __restrict__ state, Shape S, const char* __restrict__ records, const char* __restrict__ images, E* __restrict__ out,
     float* __restrict__ last, Kept<typename Rep<E>::S, DK> kept) {
     using St = typename Rep<E>::S;
@@ -271,19 +272,23 @@ __global__ __launch_bounds__(W * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))
             const int d = 16 * n + 4 * grp + r;
             s[n][r] = state && on && d < S.K ? state[(bg * S.K + d) * S.V + col] : 0.0f;
         }
-    Sixteen<E> vp;
     const auto rows_of = [&](int64_t n) { return int(S.T - n * C < C ? S.T - n * C : C); };
-    auto fetch = [&](int64_t n) {
-        vp.load(rows_at(v0 + n * C * S.vt, S.vt, rows_of(n), S.V), S.vt, value_at);
-        char* to = lds + (BUFFERS == 2 ? int(n & 1) * BUFFER : 0);
-        bring<W>(in0 + n * IN, to, 2 * In::SIZE * int(sizeof(St)));
-        bring<W>(rec0 + n * Re::STRIDE, to + IN, Re::NARROW);
-    };
-
-    fetch(0);
-    arrived<0>();
+    if (wave == W) {
+        for (int64_t n = 0; n < S.chunks; n++) {
+            if (n && BUFFERS == 1) __syncthreads();        // the chunk before has been used
+            char* to = lds + (BUFFERS == 2 ? int(n & 1) * BUFFER : 0);
+            bring<1>(in0 + n * IN, to, 2 * In::SIZE * int(sizeof(St)), 0);
+            bring<1>(rec0 + n * Re::STRIDE, to + IN, Re::NARROW, 0);
+            arrived<0>();
+            __syncthreads();               // the chunk is there (and of two, the one before has been used)
+        }
+        return;
+    }
+    Sixteen<E> vp;
+    vp.load(rows_at(v0, S.vt, rows_of(0), S.V), S.vt, value_at);
     for (int64_t n = 0; n < S.chunks; n++) {
-        __syncthreads();                   // the chunk is there, and the one before has been used
+        if (n && BUFFERS == 1) __syncthreads();
+        __syncthreads();
         char* here = lds + (BUFFERS == 2 ? int(n & 1) * BUFFER : 0);
         const In Kt{reinterpret_cast<St*>(here)}, Qt{reinterpret_cast<St*>(here) + In::SIZE};
         const Re& re = *reinterpret_cast<const Re*>(here + IN);
@@ -294,16 +299,28 @@ __global__ __launch_bounds__(W * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))
         f4 v[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) v[it] = vp.four(it);
-        if (BUFFERS == 2 && n + 1 < S.chunks) fetch(n + 1);
+        if (n + 1 < S.chunks) vp.load(rows_at(v0 + (n + 1) * C * S.vt, S.vt, rows_of(n + 1), S.V), S.vt, value_at);
         const int64_t at = (bg * S.chunks + n) * S.vp;     // of the chunk in what is kept
         const Buffer blocks(kept.blocks + at / COLS * Ke::BLOCK, KEEP ? int64_t(S.vp / COLS) * Ke::BLOCK * int(sizeof(St)) : 0);
+        // operands of a stage's products are loaded while the stage before runs
+        Frag<St, 1> ka[4][KB], qa[4][KB], kc[ND][2], pa[4][2];
+        Frag<St, WIDE> ta[4][2], sf[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+            for (int it = 0; it < 4; it++) ka[it][kb] = Kt.rows(16 * it, kb);
+        fence();
         const Scale ss = scale_of<St>(over_column(largest(s)));
-        Frag<St, WIDE> sf[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; kb++) {
             sf[kb] = frag_of<St, WIDE>(s[2 * kb], s[2 * kb + 1], ss.up);
             if constexpr (KEEP) leave(blocks, state_at + 32 * kb * sizeof(St), sf[kb]);
         }
+        fence();
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+            for (int it = 0; it < 4; it++) qa[it][kb] = Qt.rows(16 * it, kb);
         // D = V - g K S, then b D; g Q S for out
         f4 x[4], y[4], d[4];
 #pragma unroll
@@ -311,29 +328,39 @@ __global__ __launch_bounds__(W * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))
 #pragma unroll
         for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-            for (int it = 0; it < 4; it++) mma(x[it], Kt.rows(16 * it, kb), sf[kb]);
+            for (int it = 0; it < 4; it++) mma(x[it], ka[it][kb], sf[kb]);
+        fence();
+#pragma unroll
+        for (int it = 0; it < 4; it++)
+#pragma unroll
+            for (int kb = 0; kb <= it / 2; kb++) ta[it][kb] = Tt.rows(16 * it, kb);
 #pragma unroll
         for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-            for (int it = 0; it < 4; it++) mma(y[it], Qt.rows(16 * it, kb), narrow(sf[kb]));
+            for (int it = 0; it < 4; it++) mma(y[it], qa[it][kb], narrow(sf[kb]));
 #pragma unroll
         for (int it = 0; it < 4; it++) {
             const f4 xs = four(st.x, it), bs = four(st.b, it);
 #pragma unroll
             for (int r = 0; r < 4; r++) d[it][r] = bs[r] * (v[it][r] - (xs[r] == 0.0f ? 0.0f : xs[r] * (ss.down * x[it][r])));      // (a dropped state may hold anything)
         }
-        // U = (I + A)^-1 b D
         const Scale ds = scale_of<St>(over_column(largest(d)));
         Frag<St, WIDE> df[2];
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) df[kb] = frag_of<St, WIDE>(d[2 * kb], d[2 * kb + 1], ds.up);
+        fence();
+        // U = (I + A)^-1 b D
+#pragma unroll
+        for (int k = 0; k < ND; k++)
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++) kc[k][kb] = Kt.cols(16 * k, kb);
         f4 u[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) u[it] = f4{0, 0, 0, 0};
 #pragma unroll
         for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-            for (int it = 2 * kb; it < 4; it++) mma(u[it], Tt.rows(16 * it, kb), df[kb]);
+            for (int it = 2 * kb; it < 4; it++) mma(u[it], ta[it][kb], df[kb]);
         const float du = ds.down * (1.0f / SQUARE<St>);
 #pragma unroll
         for (int it = 0; it < 4; it++) u[it] *= du;
@@ -353,34 +380,37 @@ __global__ __launch_bounds__(W * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))
             scales.store(ss.down, to);
             scales.store(us.down, to, S.vp * 4);
         }
+        fence();
+#pragma unroll
+        for (int it = 0; it < 4; it++)
+#pragma unroll
+            for (int kb = 0; kb <= it / 2; kb++) pa[it][kb] = Pt.rows(16 * it, kb);
         const float end = st.end, dl = us.down * (1.0f / LONG<St>), dp = us.down * (1.0f / SQUARE<St>);
+        f4 z[ND], w[4];
 #pragma unroll
-        for (int k = 0; k < ND; k++) {
-            f4 z = {0, 0, 0, 0};
+        for (int k = 0; k < ND; k++) z[k] = f4{0, 0, 0, 0};
 #pragma unroll
-            for (int kb = 0; kb < 2; kb++) mma(z, Kt.cols(16 * k, kb), lf[kb]);
+        for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) s[k][r] = fmaf(dl, z[r], end == 0.0f ? 0.0f : end * s[k][r]);
-        }
+            for (int k = 0; k < ND; k++) mma(z[k], kc[k][kb], lf[kb]);
+        fence();
         // out = g Q S + (M Q K^T) U
+#pragma unroll
+        for (int it = 0; it < 4; it++) {
+            w[it] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int kb = 0; kb <= it / 2; kb++) mma(w[it], pa[it][kb], uf[kb]);
+        }
+#pragma unroll
+        for (int k = 0; k < ND; k++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) s[k][r] = fmaf(dl, z[k][r], end == 0.0f ? 0.0f : end * s[k][r]);
         const Buffer to = rows_at(out + ((b * S.T + n * C) * S.G + g) * S.V, ot, rows_of(n), S.V);
 #pragma unroll
         for (int it = 0; it < 4; it++) {
-            f4 w = {0, 0, 0, 0};
-#pragma unroll
-            for (int kb = 0; kb <= it / 2; kb++) mma(w, Pt.rows(16 * it, kb), uf[kb]);
             const f4 qs = four(st.q, it);
 #pragma unroll
-            for (int r = 0; r < 4; r++) Sixteen<E>::store(to, ot, out_at, 4 * it + r, fmaf(dp, w[r], qs[r] == 0.0f ? 0.0f : qs[r] * (ss.down * y[it][r])));
-        }
-        if (n + 1 < S.chunks) {
-            if constexpr (BUFFERS == 2) {
-                arrived<16 + (KEEP ? KB + 4 : 0)>();       // (all but this chunk's stores)
-            } else {
-                __syncthreads();
-                fetch(n + 1);
-                arrived<0>();
-            }
+            for (int r = 0; r < 4; r++) Sixteen<E>::store(to, ot, out_at, 4 * it + r, fmaf(dp, w[it][r], qs[r] == 0.0f ? 0.0f : qs[r] * (ss.down * y[it][r])));
         }
     }
 #pragma unroll
@@ -494,8 +524,8 @@ int32_t forward(const void* query, const void* key, const void* value, const voi
     chunk_kernel<E, DK><<<dim3(heads * S.chunks), BLOCK, 0, stream>>>(in(query), in(key), in(gate), in(write), reset, S, records, images);
     const dim3 grid(heads * ((S.vp / 16 + W - 1) / W));
     const Kept<St, DK> to(kept, S);
-    if (kept) state_kernel<E, DK, W, true><<<grid, W * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to);
-    else state_kernel<E, DK, W, false><<<grid, W * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to);
+    if (kept) state_kernel<E, DK, W, true><<<grid, (W + 1) * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to);
+    else state_kernel<E, DK, W, false><<<grid, (W + 1) * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to);
     return launched(err, errcap);
 }
 

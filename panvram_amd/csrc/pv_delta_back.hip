@@ -17,10 +17,10 @@ using namespace pvd;
 
 namespace {
 
-// ---- walk_kernel: a workgroup of W waves for 16 W columns of a state's gradient
+// ---- walk_kernel: a workgroup of W waves for 16 W columns of a state's gradient, and a wave more that brings chunks to LDS
 
 template <typename E, int DK, int W>
-__global__ __launch_bounds__(W * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))) void walk_kernel(
+__global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))) void walk_kernel(
     const E* __restrict__ d_out, const float* __restrict__ d_last, Shape S, const char* __restrict__ records, const char* __restrict__ images, E* __restrict__ d_value,
     float* __restrict__ d_state, Kept<typename Rep<E>::S, DK> walked) {
     using St = typename Rep<E>::S;
@@ -52,19 +52,23 @@ __global__ __launch_bounds__(W * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))
             const int d = 16 * n + 4 * grp + r;
             s[n][r] = d_last && on && d < S.K ? d_last[(bg * S.K + d) * S.V + col] : 0.0f;
         }
-    Sixteen<E> op;
     const auto rows_of = [&](int64_t n) { return int(S.T - n * C < C ? S.T - n * C : C); };
-    auto fetch = [&](int64_t n) {
-        op.load(rows_at(o0 + n * C * S.ot, S.ot, rows_of(n), S.V), S.ot, out_at);
-        char* to = lds + (BUFFERS == 2 ? int(n & 1) * BUFFER : 0);
-        bring<W>(in0 + n * IN, to, 2 * In::SIZE * int(sizeof(St)));
-        bring<W>(rec0 + n * Re::STRIDE, to + IN, Re::ALL);
-    };
-
-    fetch(S.chunks - 1);
-    arrived<0>();
+    if (wave == W) {
+        for (int64_t n = S.chunks - 1; n >= 0; n--) {
+            if (n < S.chunks - 1 && BUFFERS == 1) __syncthreads();     // the chunk after has been used
+            char* to = lds + (BUFFERS == 2 ? int(n & 1) * BUFFER : 0);
+            bring<1>(in0 + n * IN, to, 2 * In::SIZE * int(sizeof(St)), 0);
+            bring<1>(rec0 + n * Re::STRIDE, to + IN, Re::ALL, 0);
+            arrived<0>();
+            __syncthreads();               // the chunk is there (and of two, the one after has been used)
+        }
+        return;
+    }
+    Sixteen<E> op;
+    op.load(rows_at(o0 + (S.chunks - 1) * C * S.ot, S.ot, rows_of(S.chunks - 1), S.V), S.ot, out_at);
     for (int64_t n = S.chunks - 1; n >= 0; n--) {
-        __syncthreads();                   // the chunk is there, and the one after has been used
+        if (n < S.chunks - 1 && BUFFERS == 1) __syncthreads();
+        __syncthreads();
         char* here = lds + (BUFFERS == 2 ? int(n & 1) * BUFFER : 0);
         const In Kt{reinterpret_cast<St*>(here)}, Qt{reinterpret_cast<St*>(here) + In::SIZE};
         const Re& re = *reinterpret_cast<const Re*>(here + IN);
@@ -79,20 +83,30 @@ __global__ __launch_bounds__(W * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))
 #pragma unroll
             for (int r = 0; r < 4; r++) o[it][r] = 16 * it + 4 * grp + r < rows ? o[it][r] : 0.0f;
         }
-        if (BUFFERS == 2 && n) fetch(n - 1);
+        if (n) op.load(rows_at(o0 + (n - 1) * C * S.ot, S.ot, rows_of(n - 1), S.V), S.ot, out_at);
         const int64_t at = (bg * S.chunks + n) * S.vp;     // of the chunk in what is left over
         const Buffer blocks(walked.blocks + at / COLS * Ke::BLOCK, int64_t(S.vp / COLS) * Ke::BLOCK * int(sizeof(St)));
+        // operands of a stage's products are loaded while the stage before runs
+        Frag<St, 1> ka[4][KB], of[2];
+        Frag<St, WIDE> pa[4][2], ta[4][2], sf[KB];
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int it = 0; it < 2 * kb + 2; it++) pa[it][kb] = Pt.cols(16 * it, kb);
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+            for (int it = 0; it < 4; it++) ka[it][kb] = Kt.rows(16 * it, kb);
+        fence();
         const Scale ss = scale_of<St>(over_column(largest(s))), os = scale_of<St>(over_column(largest(o)));
-        Frag<St, WIDE> sf[KB];
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++) of[kb] = frag_of<St, 1>(o[2 * kb], o[2 * kb + 1], os.up);       // (these are a tensor's elements: nothing is rounded off)
 #pragma unroll
         for (int kb = 0; kb < KB; kb++) {
             sf[kb] = frag_of<St, WIDE>(s[2 * kb], s[2 * kb + 1], ss.up);
             leave(blocks, state_at + 32 * kb * sizeof(St), sf[kb]);
         }
         // dU = l K dS + P^T dO
-        Frag<St, 1> of[2];
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++) of[kb] = frag_of<St, 1>(o[2 * kb], o[2 * kb + 1], os.up);       // (these are a tensor's elements: nothing is rounded off)
         const float dp = os.down * (1.0f / SQUARE<St>);
         f4 u[4], w[4];
 #pragma unroll
@@ -100,11 +114,16 @@ __global__ __launch_bounds__(W * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))
 #pragma unroll
         for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-            for (int it = 0; it < 2 * kb + 2; it++) mma(w[it], Pt.cols(16 * it, kb), of[kb]);
+            for (int it = 0; it < 2 * kb + 2; it++) mma(w[it], pa[it][kb], of[kb]);
+        fence();
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int it = 0; it < 2 * kb + 2; it++) ta[it][kb] = Tt.cols(16 * it, kb);
 #pragma unroll
         for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-            for (int it = 0; it < 4; it++) mma(u[it], Kt.rows(16 * it, kb), sf[kb]);
+            for (int it = 0; it < 4; it++) mma(u[it], ka[it][kb], sf[kb]);
 #pragma unroll
         for (int it = 0; it < 4; it++) {
             const f4 ls = four(st.l, it);
@@ -117,13 +136,22 @@ __global__ __launch_bounds__(W * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) uf[kb] = frag_of<St, WIDE>(u[2 * kb], u[2 * kb + 1], us.up);
         const float du = us.down * (1.0f / SQUARE<St>);
+        fence();
+        Frag<St, 1> kc[ND][2], qc[ND][2];
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int k = 0; k < ND; k++) {
+                qc[k][kb] = Qt.cols(16 * k, kb);
+                kc[k][kb] = Kt.cols(16 * k, kb);
+            }
         f4 d[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) d[it] = f4{0, 0, 0, 0};
 #pragma unroll
         for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-            for (int it = 0; it < 2 * kb + 2; it++) mma(d[it], Tt.cols(16 * it, kb), uf[kb]);
+            for (int it = 0; it < 2 * kb + 2; it++) mma(d[it], ta[it][kb], uf[kb]);
 #pragma unroll
         for (int it = 0; it < 4; it++) d[it] *= du;
         const Scale ds = scale_of<St>(over_column(largest(d)));
@@ -151,27 +179,23 @@ __global__ __launch_bounds__(W * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))
         scales.store(ss.down, scale_at);
         scales.store(ds.down, scale_at, S.vp * 4);
         scales.store(os.down, scale_at, 2 * S.vp * 4);
+        fence();
         const float end = st.end;
+        f4 z[ND];
 #pragma unroll
-        for (int k = 0; k < ND; k++) {
-            f4 z = {0, 0, 0, 0};
+        for (int k = 0; k < ND; k++) z[k] = f4{0, 0, 0, 0};
 #pragma unroll
-            for (int kb = 0; kb < 2; kb++) {
-                mma(z, Qt.cols(16 * k, kb), xf[kb]);
-                mma(z, Kt.cols(16 * k, kb), yf[kb]);
-            }
+        for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) s[k][r] = fmaf(xs.down, z[r], end == 0.0f ? 0.0f : end * s[k][r]);
-        }
-        if (n) {
-            if constexpr (BUFFERS == 2) {
-                arrived<16 + KB + 5>();    // (all but this chunk's stores)
-            } else {
-                __syncthreads();
-                fetch(n - 1);
-                arrived<0>();
-            }
-        }
+            for (int k = 0; k < ND; k++) mma(z[k], qc[k][kb], xf[kb]);
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int k = 0; k < ND; k++) mma(z[k], kc[k][kb], yf[kb]);
+#pragma unroll
+        for (int k = 0; k < ND; k++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) s[k][r] = fmaf(xs.down, z[k][r], end == 0.0f ? 0.0f : end * s[k][r]);
     }
     if (!d_state) return;
 #pragma unroll
@@ -567,7 +591,7 @@ int32_t backward(const void* gate, const void* write, const void* d_out, const f
     const int64_t heads = S.B * S.G;
     const char *rec = static_cast<const char*>(records), *images = rec + heads * S.chunks * Record<St>::STRIDE;
     const Kept<St, DK> before(kept, S), walked(work, S);
-    walk_kernel<E, DK, W><<<dim3(heads * ((S.vp / 16 + W - 1) / W)), W * WAVE, 0, stream>>>(in(d_out), d_last, S, rec, images, out(d_value), d_state, walked);
+    walk_kernel<E, DK, W><<<dim3(heads * ((S.vp / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(in(d_out), d_last, S, rec, images, out(d_value), d_state, walked);
     gradient_kernel<E, DK><<<dim3(S.B * S.H * S.chunks), MANY, 0, stream>>>(in(gate), in(write), in(d_out), S, rec, images, before, walked, out(d_query), out(d_key),
                                                                            out(d_gate), out(d_write));
     return launched(err, errcap);
