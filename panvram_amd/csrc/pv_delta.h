@@ -71,6 +71,43 @@ template <int N> __device__ inline float largest(const f4 (&v)[N]) {
     return x;
 }
 
+// A sum over the 16 lanes of a row of columns, and over a wave; the largest over a wave
+template <int N> __device__ inline int turned(int x) { return __builtin_amdgcn_mov_dpp(x, 0x120 + N, 0xf, 0xf, true); }     // by N lanes of the 16
+__device__ inline float over_row(float x) {
+    x += __int_as_float(turned<8>(__float_as_int(x)));
+    x += __int_as_float(turned<4>(__float_as_int(x)));
+    x += __int_as_float(turned<2>(__float_as_int(x)));
+    return x + __int_as_float(turned<1>(__float_as_int(x)));
+}
+__device__ inline float sum_over_rows(float x) {           // of the four lanes that have a column
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+__device__ inline int largest_of_wave(int x) {
+    x = max(x, turned<8>(x));
+    x = max(x, turned<4>(x));
+    x = max(x, turned<2>(x));
+    x = max(x, turned<1>(x));
+    auto a = __builtin_amdgcn_permlane32_swap(uint32_t(x), uint32_t(x), false, false);
+    x = max(int(a[0]), int(a[1]));
+    a = __builtin_amdgcn_permlane16_swap(uint32_t(x), uint32_t(x), false, false);
+    return max(int(a[0]), int(a[1]));
+}
+// exp of a number that is not positive. Operands in 16 bits: off by |x| 2^-24 of itself, where what is left of it matters less.
+template <typename S> __device__ inline float decay(float x) {
+    if constexpr (sizeof(S) == 2) return __expf(x);
+    return expf(x);
+}
+// The thread's number, of which the compiler does not know that it is the same as before: what is made from it is made where it is used,
+// and no address is kept (and spilled) through a phase that has no use for it
+__device__ inline int thread() {
+    int id = threadIdx.x;
+    asm volatile("" : "+v"(id));
+    return id;
+}
+
 // Nothing is moved across: the loads before it are in flight while what comes after it runs. (Left to itself the compiler puts each
 // load of an operand right before its product, and a wave that is alone on its SIMD waits for every one.)
 __device__ inline void fence() { __builtin_amdgcn_sched_barrier(0); }

@@ -68,7 +68,7 @@ template <typename S> __device__ inline void record(const float* m, int row, S (
 }
 
 template <typename E, int DK>
-__global__ __launch_bounds__(BLOCK) void chunk_kernel(const E* __restrict__ query, const E* __restrict__ key, const E* __restrict__ gate, const E* __restrict__ write,
+__global__ __launch_bounds__(BLOCK, 4) void chunk_kernel(const E* __restrict__ query, const E* __restrict__ key, const E* __restrict__ gate, const E* __restrict__ write,
                                                       const uint8_t* __restrict__ reset, Shape S, char* __restrict__ records, char* __restrict__ images) {
     using St = typename Rep<E>::S;
     using In = Tile<St, C, DK>;
@@ -172,7 +172,7 @@ __global__ __launch_bounds__(BLOCK) void chunk_kernel(const E* __restrict__ quer
         for (int r = 0; r < 4; r++) {
             const int i = 16 * wave + 4 * grp + r;
             const bool on = j <= wave && col <= i && col >= from[r];
-            const float M = on ? expf((hi[r] - hc) + (lo[r] - lc)) * rk : 0.0f;
+            const float M = on ? decay<St>((hi[r] - hc) + (lo[r] - lc)) * rk : 0.0f;
             T[i * ROW + col] = on ? M * qf[r] * qk[j][r] : 0.0f;
             A[i * ROW + col] = on && col < i ? M * kf[r] * kk[j][r] : 0.0f;
         }

@@ -216,15 +216,10 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 
 constexpr int BANDS = 4, HALVES = 2, MANY = BANDS * HALVES * WAVE, PRODUCTS = 5;
 
-__device__ inline float row16(float x) {   // a sum over the 16 lanes that have a row's columns
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) x += __shfl_xor(x, d, WAVE);
-    return x;
-}
 __device__ inline int exponent(float x) { return int(__float_as_uint(x) >> 23) - 127; }
 
 template <typename E, int DK>
-__global__ __launch_bounds__(MANY) void gradient_kernel(const E* __restrict__ gate, const E* __restrict__ write, const E* __restrict__ d_out, Shape S,
+__global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) void gradient_kernel(const E* __restrict__ gate, const E* __restrict__ write, const E* __restrict__ d_out, Shape S,
                                                         const char* __restrict__ records, const char* __restrict__ images, const Kept<typename Rep<E>::S, DK> kept,
                                                         const Kept<typename Rep<E>::S, DK> walked, E* __restrict__ d_query, E* __restrict__ d_key,
                                                         E* __restrict__ d_gate, E* __restrict__ d_write) {
@@ -249,7 +244,7 @@ __global__ __launch_bounds__(MANY) void gradient_kernel(const E* __restrict__ ga
     const In Kt{reinterpret_cast<St*>(lds)}, Qt{reinterpret_cast<St*>(lds) + In::SIZE};
     St* const more = reinterpret_cast<St*>(lds + IN);
     const Square Ek{more}, Eq{more + Square::SIZE}, Ff{more + 2 * Square::SIZE};       // (once the blocks of values have been used)
-    const int tid = threadIdx.x, wave = tid / WAVE, l = tid % WAVE, grp = l / 16, m = l % 16, half = wave / BANDS, own = wave % BANDS, band = 16 * own, d0 = half * DK / 2;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), half = wave / BANDS, own = wave % BANDS, band = 16 * own, d0 = half * DK / 2;
     const int64_t chunk = blockIdx.x % S.chunks, bh = blockIdx.x / S.chunks;
     const int64_t b = bh / S.H, t0 = chunk * C;
     const int h = int(bh % S.H), share = S.G / S.H, steps = int(S.T - t0 < C ? S.T - t0 : C);
@@ -275,31 +270,30 @@ __global__ __launch_bounds__(MANY) void gradient_kernel(const E* __restrict__ ga
         for (int n = 0; n < ND; n++) aq[n] = from[n] = to[n] = zero;
         dp[0] = dp[1] = da[0] = da[1] = zero;
         float both = 0.0f;                 // of state and gradient, summed over all elements
-        // d_out's 64 rows of 32 columns: four elements a lane; lanes 0 .. 159 the factors of a product's column
-        const int orow = tid / 8, ocol = tid % 8 * 4, product = tid / COLS < PRODUCTS ? tid / COLS : 0, column = tid % COLS;
-        const Buffer outs = rows_at(o0, S.ot, steps, S.V);
-        const uint32_t out_at = (orow * S.ot + ocol) * uint32_t(sizeof(E));
-        const float *fl = left_scale(product), *fr = right_scale(product);
         uint32_t op[4];
         f4 os = {1.0f, 1.0f, 1.0f, 1.0f};
         float lf = 1.0f, rf = 1.0f;
+        // d_out's 64 rows of 32 columns: four elements a lane; lanes 0 .. 159 the factors of a product's column
         auto fetch = [&](int v0, int to) {
+            const int tid = thread(), row = tid / 8, col = tid % 8 * 4, product = tid / COLS < PRODUCTS ? tid / COLS : 0, column = tid % COLS;
+            const Buffer outs = rows_at(o0, S.ot, steps, S.V);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const uint32_t off = v0 + ocol + e < S.V ? out_at + (v0 + e) * uint32_t(sizeof(E)) : NOWHERE;
+                const uint32_t off = v0 + col + e < S.V ? (row * S.ot + v0 + col + e) * uint32_t(sizeof(E)) : NOWHERE;
                 if constexpr (sizeof(E) == 2) op[e] = __builtin_amdgcn_raw_buffer_load_b16(outs.r, off, 0, 0);
                 else op[e] = __builtin_amdgcn_raw_buffer_load_b32(outs.r, off, 0, 0);
             }
             if constexpr (HALF) {
-                os = *reinterpret_cast<const f4*>(f1 + 2 * S.vp + v0 + ocol);
-                lf = fl[v0 + column];
-                rf = fr[v0 + column];
+                os = *reinterpret_cast<const f4*>(f1 + 2 * S.vp + v0 + col);
+                lf = left_scale(product)[v0 + column];
+                rf = right_scale(product)[v0 + column];
             }
             char* buffer = lds + IN + to * BUFFER;
             bring<WAVES>(b0 + v0 / COLS * Ke::BLOCK, buffer, BLOCK);
             bring<WAVES>(b1 + v0 / COLS * Ke::BLOCK, buffer + BLOCK, BLOCK);
         };
-        auto put = [&](int v0, int to) {   // what went by way of registers
+        auto put = [&](int to) {           // what went by way of registers
+            const int tid = thread(), row = tid / 8, col = tid % 8 * 4;
             const Ot Od{reinterpret_cast<St*>(lds + IN + to * BUFFER + 2 * BLOCK)};
             pack<St, 4> x;
 #pragma unroll
@@ -307,86 +301,104 @@ __global__ __launch_bounds__(MANY) void gradient_kernel(const E* __restrict__ ga
                 const float d = Sixteen<E>::value(op[e]);
                 x.v[e] = St(HALF ? d * __uint_as_float((254u << 23) - __float_as_uint(os[e])) : d);    // (over a power of two)
             }
-            x.store(Od.p + orow * Ot::ROW + place(ocol));
+            x.store(Od.p + row * Ot::ROW + place(col));
             if constexpr (HALF) if (tid < PRODUCTS * COLS) {
                 int top = -1000;
 #pragma unroll
-                for (int w = 0; w < WAVES; w++) top = max(top, tops[w][product]);
+                for (int w = 0; w < WAVES; w++) top = max(top, tops[w][tid / COLS]);
                 const int e = exponent(lf) + exponent(rf) - top;       // 0 at most
-                factors[to][product][place(column)] = e > -25 ? St(__uint_as_float((127 + e) << 23)) : St(0.0f);
+                factors[to][tid / COLS][place(tid % COLS)] = e > -25 ? St(__uint_as_float((127 + e) << 23)) : St(0.0f);
             }
         };
         if (j) __syncthreads();            // the value head before has been dealt with
         fetch(0, 0);
         {                                  // the steps' record, and the largest of the columns' scales by product: dO S, dR S, U dS, dO U, dR U
+            const int tid = thread();
             const float* p = reinterpret_cast<const float*>(&reinterpret_cast<const Re*>(record_of<St>(const_cast<char*>(records), at))->steps);
-            for (int k = tid; k < int(sizeof(Steps) / 4); k += MANY) reinterpret_cast<float*>(&st)[k] = p[k];
-        }
-        if constexpr (HALF) {
-            int top[PRODUCTS];
+            constexpr int N = int(sizeof(Steps) / 4), EACH = (N + MANY - 1) / MANY;
+            float x[EACH];
 #pragma unroll
-            for (int p = 0; p < PRODUCTS; p++) top[p] = -1000;
-            for (int c = tid; c < S.vp; c += MANY) {
-                const int es = exponent(f0[c]), eu = exponent(f0[S.vp + c]), ed = exponent(f1[c]), er = exponent(f1[S.vp + c]), eo = exponent(f1[2 * S.vp + c]);
-                top[0] = max(top[0], eo + es);
-                top[1] = max(top[1], er + es);
-                top[2] = max(top[2], eu + ed);
-                top[3] = max(top[3], eo + eu);
-                top[4] = max(top[4], er + eu);
+            for (int k = 0; k < EACH; k++) x[k] = p[tid + k * MANY < N ? tid + k * MANY : N - 1];
+            if constexpr (HALF) {
+                int top[PRODUCTS];
+#pragma unroll
+                for (int p = 0; p < PRODUCTS; p++) top[p] = -1000;
+                for (int c = tid; c < S.vp; c += MANY) {
+                    const int es = exponent(f0[c]), eu = exponent(f0[S.vp + c]), ed = exponent(f1[c]), er = exponent(f1[S.vp + c]), eo = exponent(f1[2 * S.vp + c]);
+                    top[0] = max(top[0], eo + es);
+                    top[1] = max(top[1], er + es);
+                    top[2] = max(top[2], eu + ed);
+                    top[3] = max(top[3], eo + eu);
+                    top[4] = max(top[4], er + eu);
+                }
+#pragma unroll
+                for (int p = 0; p < PRODUCTS; p++) {
+                    top[p] = largest_of_wave(top[p]);
+                    if (tid % WAVE == 0) tops[wave][p] = top[p];
+                }
             }
 #pragma unroll
-            for (int p = 0; p < PRODUCTS; p++) {
-#pragma unroll
-                for (int d = WAVE / 2; d; d >>= 1) top[p] = max(top[p], __shfl_xor(top[p], d, WAVE));
-                if (l == 0) tops[wave][p] = top[p];
-            }
+            for (int k = 0; k < EACH; k++) if (tid + k * MANY < N) reinterpret_cast<float*>(&st)[tid + k * MANY] = x[k];
         }
         __syncthreads();
-        put(0, 0);
+        put(0);
         arrived<0>();
         int now = 0;
         for (int v0 = 0; v0 < S.vp; v0 += COLS) {
             __syncthreads();               // the block is there, and the one before has been used
             const bool next = v0 + COLS < S.vp;
+            const int tid = thread();
             St* buffer = reinterpret_cast<St*>(lds + IN + now * BUFFER);
-            if (BUFFERS == 2 && next) fetch(v0 + COLS, now ^ 1);
             const Sv S0{buffer}, S1{buffer + Ke::BLOCK};
             const Uv Us{buffer + Sv::SIZE}, Rs{buffer + Ke::BLOCK + Sv::SIZE};
             const Ot Od{buffer + 2 * Ke::BLOCK};
             const auto scaled = [&](auto f, int p) {
-                if constexpr (HALF) f.p[0] *= *reinterpret_cast<const h8*>(&factors[now][p][8 * grp]);
+                if constexpr (HALF) f.p[0] *= *reinterpret_cast<const h8*>(&factors[now][p][8 * (tid % WAVE / 16)]);
                 return f;
             };
             const auto of = Od.rows(band, 0);
             const auto rf = Rs.cols(band, 0), uf = Us.cols(band, 0);
-            const auto of0 = scaled(of, 0), rf1 = scaled(rf, 1), uf2 = scaled(uf, 2), of3 = scaled(of, 3), rf4 = scaled(rf, 4);
+            Frag<St, 1> sf[ND], gf[ND], un[2];
 #pragma unroll
             for (int n = 0; n < ND; n++) {
-                const auto sf = S0.cols(d0 + 16 * n, 0);
-                mma(aq[n], of0, sf);
-                mma(from[n], rf1, sf);
-                mma(to[n], uf2, S1.cols(d0 + 16 * n, 0));
+                sf[n] = S0.cols(d0 + 16 * n, 0);
+                gf[n] = S1.cols(d0 + 16 * n, 0);
             }
 #pragma unroll
-            for (int k = 0; k < 2; k++) if (half + 2 * k <= own) {
-                const auto un = Us.cols(16 * (half + 2 * k), 0);
-                mma(dp[k], of3, un);
-                mma(da[k], rf4, un);
-            }
-            for (int p = tid; p < COLS * DK / UNIT; p += MANY) {
-                const int c = p / (DK / UNIT), at = c * Sv::ROW + p % (DK / UNIT) * UNIT;
+            for (int k = 0; k < 2; k++) un[k] = Us.cols(16 * (half + 2 * k), 0);
+            float product[2] = {0.0f, 0.0f};
+            constexpr int UNITS = COLS * DK / UNIT, EACH = (UNITS + MANY - 1) / MANY;
+#pragma unroll
+            for (int k = 0; k < EACH; k++) {
+                const int p = tid + k * MANY < UNITS ? tid + k * MANY : 0, c = p / (DK / UNIT), at = c * Sv::ROW + p % (DK / UNIT) * UNIT;
                 const auto x = pack<St, UNIT>::load(S0.p + at), y = pack<St, UNIT>::load(S1.p + at);
                 float z = 0.0f;
 #pragma unroll
                 for (int e = 0; e < UNIT; e++) z = fmaf(float(x.v[e]), float(y.v[e]), z);
-                both = fmaf(z, HALF ? f0[v0 + c] * f1[v0 + c] : 1.0f, both);
+                if (HALF) z *= f0[v0 + c] * f1[v0 + c];
+                product[k % 2] += tid + k * MANY < UNITS ? z : 0.0f;
+            }
+            both += product[0] + product[1];
+            if (BUFFERS == 2 && next) fetch(v0 + COLS, now ^ 1);
+            fence();
+            const auto of0 = scaled(of, 0), rf1 = scaled(rf, 1), uf2 = scaled(uf, 2), of3 = scaled(of, 3), rf4 = scaled(rf, 4);
+#pragma unroll
+            for (int n = 0; n < ND; n++) {
+                mma(aq[n], of0, sf[n]);
+                mma(from[n], rf1, sf[n]);
+                mma(to[n], uf2, gf[n]);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; k++) {  // (those above the diagonal are not used)
+                mma(dp[k], of3, un[k]);
+                mma(da[k], rf4, un[k]);
             }
             if (next) {
                 if constexpr (BUFFERS == 1) {
                     __syncthreads();
                     fetch(v0 + COLS, 0);
                 }
-                put(v0 + COLS, BUFFERS == 2 ? now ^ 1 : 0);
+                put(BUFFERS == 2 ? now ^ 1 : 0);
                 arrived<0>();
                 if (BUFFERS == 2) now ^= 1;
             }
@@ -401,35 +413,39 @@ __global__ __launch_bounds__(MANY) void gradient_kernel(const E* __restrict__ ga
             }
         }
         const uint64_t cuts = uint64_t(st.cut[1]) << 32 | st.cut[0];
+        const int tid = thread(), l = tid % WAVE, grp = l / 16, m = l % 16;
         // what a step has of the state before the chunk and leaves after it, and its row's sums
-        float bi[4], rowsum[4], rki[4], rqi[4], hi[4], lo[4];
-        int since_i[4];
+        const f4 hi = *reinterpret_cast<const f4*>(st.hi + band + 4 * grp), lo = *reinterpret_cast<const f4*>(st.lo + band + 4 * grp);
+        const f4 bi = *reinterpret_cast<const f4*>(st.b + band + 4 * grp);
+        f4 rki = *reinterpret_cast<const f4*>(st.rk + band + 4 * grp), rqi = *reinterpret_cast<const f4*>(st.rq + band + 4 * grp), rowsum;
         const float last_hi = st.hi[C - 1], last_lo = st.lo[C - 1];
         const int last_cut = since(cuts, C - 1);
+        int since_i[4];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int i = band + 4 * grp + r;
-            hi[r] = st.hi[i];
-            lo[r] = st.lo[i];
             since_i[r] = since(cuts, i);
-            const float gi = since_i[r] >= 0 ? 0.0f : expf(hi[r]), li = i < last_cut ? 0.0f : expf((last_hi - hi[r]) + (last_lo - lo[r]));
-            bi[r] = st.b[i];
-            rki[r] = length_rest<St>(st.rk[i]);
-            rqi[r] = length_rest<St>(st.rq[i]);
-            float dq = 0.0f, df = 0.0f, dt = 0.0f;
+            const float gi = since_i[r] >= 0 ? 0.0f : decay<St>(hi[r]), li = i < last_cut ? 0.0f : decay<St>((last_hi - hi[r]) + (last_lo - lo[r]));
+            rki[r] = length_rest<St>(rki[r]);
+            rqi[r] = length_rest<St>(rqi[r]);
+            float q[ND], k[ND], dq = 0.0f, df = 0.0f, dt = 0.0f;
+#pragma unroll
+            for (int n = 0; n < ND; n++) {
+                q[n] = float(Qt.get(i, d0 + 16 * n + m));
+                k[n] = float(Kt.get(i, d0 + 16 * n + m));
+            }
 #pragma unroll
             for (int n = 0; n < ND; n++) {
                 const float x = gi == 0.0f ? 0.0f : gi * ldexpf(aq[n][r], top[0]), y = gi == 0.0f ? 0.0f : -bi[r] * gi * ldexpf(from[n][r], top[1]);
                 const float z = li == 0.0f ? 0.0f : li * ldexpf(to[n][r], top[2]);
-                const float q = float(Qt.get(i, d0 + 16 * n + m)), k = float(Kt.get(i, d0 + 16 * n + m));
-                dq = fmaf(q, x, dq);
-                df = fmaf(k, y, df);
-                dt = fmaf(k, z, dt);
+                dq = fmaf(q[n], x, dq);
+                df = fmaf(k[n], y, df);
+                dt = fmaf(k[n], z, dt);
                 tq[n][r] += x;
                 tk[n][r] += y + z;
             }
             rowsum[r] = rqi[r] * dq + rki[r] * df;
-            dt = row16(dt);
+            dt = over_row(dt);
             if (m == 0) left[half][i] = rki[r] * dt;
         }
         f4 kk[2] = {zero, zero}, qk[2] = {zero, zero};
@@ -437,56 +453,62 @@ __global__ __launch_bounds__(MANY) void gradient_kernel(const E* __restrict__ ga
         for (int kb = 0; kb < KB; kb++) {
             const auto ka = Kt.rows(band, kb), qa = Qt.rows(band, kb);
 #pragma unroll
-            for (int k = 0; k < 2; k++) if (half + 2 * k <= own) {
+            for (int k = 0; k < 2; k++) {
                 const auto kn = Kt.rows(16 * (half + 2 * k), kb);
                 mma(kk[k], ka, kn);
                 mma(qk[k], qa, kn);
             }
         }
-        both = wave_sum(both);
+        both = over_row(sum_over_rows(both));
         if (l == 0) whole[wave] = both;
         __syncthreads();                   // the last block of values has been used
         // E and F with the lengths of what they are multiplied by, F on both sides of the diagonal
+        // (dp and da are 2^28 V at most, a length's rest 2 / LONG: what is left is 2^14)
+        constexpr float FIT = HALF ? 0x1p-15f * LONG<St> : 1.0f;
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-            const int c = 16 * (half + 2 * k) + m;
-            const float rk = length_rest<St>(st.rk[c]), hc = st.hi[c], lc = st.lo[c];
+            const int n = half + 2 * k, c = 16 * n + m, at = place(c);
             float column = 0.0f;
+            if (n > own) {                 // above the diagonal
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int i = band + 4 * grp + r;
-                const bool on = c <= i && c >= since_i[r];
-                float e = 0.0f, f = 0.0f;
-                if (on) {
-                    const float M = expf((hi[r] - hc) + (lo[r] - lc));
-                    e = M * dp[k][r];
-                    if (c < i) {
-                        f = -M * bi[r] * da[k][r];
-                        const float pair = ldexpf(e * rqi[r] * rk * qk[k][r], top[3]) + ldexpf(f * rki[r] * rk * kk[k][r], top[4]);
-                        rowsum[r] += pair;
-                        column += pair;
-                    } else {
-                        writes[i] = ldexpf(da[k][r], top[4]);
+                for (int r = 0; r < 4; r++) Ek.p[(band + 4 * grp + r) * Square::ROW + at] = Eq.p[(band + 4 * grp + r) * Square::ROW + at] = St(0.0f);
+            } else {
+                const float rk = length_rest<St>(st.rk[c]), hc = st.hi[c], lc = st.lo[c];
+                f4 fk;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int i = band + 4 * grp + r;
+                    const bool on = c <= i && c >= since_i[r];
+                    const float M = decay<St>(on ? (hi[r] - hc) + (lo[r] - lc) : 0.0f);
+                    const float e = on ? M * dp[k][r] : 0.0f, f = on && c < i ? -M * bi[r] * da[k][r] : 0.0f;
+                    const float pair = c < i ? ldexpf(e * rqi[r] * rk * qk[k][r], top[3]) + ldexpf(f * rki[r] * rk * kk[k][r], top[4]) : 0.0f;
+                    rowsum[r] += pair;
+                    column += pair;
+                    Ek.p[i * Square::ROW + at] = St(e * (few * FIT) * rk);
+                    Eq.p[i * Square::ROW + at] = St(e * (few * FIT) * rqi[r]);
+                    if (n < own || c <= i) Ff.p[i * Square::ROW + at] = St(f * (few * FIT) * rk);
+                    fk[r] = f * (few * FIT) * rki[r];
+                }
+                if (n < own) {             // the four steps' places are neighbours
+                    pack<St, 4> x;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) x.v[r] = St(fk[r]);
+                    x.store(Ff.p + c * Square::ROW + place(band + 4 * grp));
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int i = band + 4 * grp + r;
+                        if (c < i) Ff.p[c * Square::ROW + place(i)] = St(fk[r]);
+                        if (c == i) writes[i] = ldexpf(da[k][r], top[4]);
                     }
                 }
-                // (dp and da are 2^28 V at most, a length's rest 2 / LONG: what is left is 2^14)
-                constexpr float FIT = HALF ? 0x1p-15f * LONG<St> : 1.0f;
-                e *= few * FIT;
-                f *= few * FIT;
-                Ek.p[i * Square::ROW + place(c)] = St(e * rk);
-                Eq.p[i * Square::ROW + place(c)] = St(e * rqi[r]);
-                if (c <= i) {
-                    Ff.p[i * Square::ROW + place(c)] = St(f * rk);
-                    if (c < i) Ff.p[c * Square::ROW + place(i)] = St(f * rki[r]);
-                }
+                column = sum_over_rows(column);
             }
-            column += __shfl_xor(column, 16, WAVE);
-            column += __shfl_xor(column, 32, WAVE);
             if (grp == 0) columns[own][c] = column;
         }
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            const float x = row16(rowsum[r]);
+            const float x = over_row(rowsum[r]);
             if (m == 0) rows[half][band + 4 * grp + r] = x;
         }
         __syncthreads();
@@ -517,6 +539,8 @@ __global__ __launch_bounds__(MANY) void gradient_kernel(const E* __restrict__ ga
         }
         if (wave == 0) {                   // a lane for each step: gates
             const auto same = [&](int i) { return i < C && since(cuts, i) <= l; };     // no step up to i, from the next on, drops the state
+            const int64_t t = t0 + (l < steps ? l : steps - 1);
+            const float x = float(gate[b * S.ab + t * S.at + g * S.ag]), w = float(write[b * S.wb + t * S.wt + g * S.wg]);
             double after = double(rows[0][l]) + rows[1][l] - (double(columns[0][l]) + columns[1][l] + columns[2][l] + columns[3][l]);
             double before = double(left[0][l]) + left[1][l];
 #pragma unroll
@@ -527,56 +551,51 @@ __global__ __launch_bounds__(MANY) void gradient_kernel(const E* __restrict__ ga
             }
             before = __shfl_up(before, 1, WAVE);
             if (l == 0) before = 0.0;
-            const int64_t t = t0 + l;
-            if (l < steps) {
-                const float x = float(gate[b * S.ab + t * S.at + g * S.ag]), w = float(write[b * S.wb + t * S.wt + g * S.wg]);
-                double d = after + before;
-                if (since(cuts, l) < 0 && st.end != 0.0f) {
-                    double sum = 0.0;
+            double d = after + before;
+            if (since(cuts, l) < 0 && st.end != 0.0f) {
+                double sum = 0.0;
 #pragma unroll
-                    for (int w = 0; w < WAVES; w++) sum += whole[w];
-                    d += double(st.end) * sum;
-                }
-                d_gate[(b * S.T + t) * S.G + g] = E(cuts >> l & 1 ? 0.0f : float(-d / (1.0 + exp(-double(x)))));
+                for (int w = 0; w < WAVES; w++) sum += whole[w];
+                d += double(st.end) * sum;
+            }
+            if (l < steps) {
+                d_gate[(b * S.T + t) * S.G + g] = E(cuts >> l & 1 ? 0.0f : -float(d) / (1.0f + expf(-x)));
                 d_write[(b * S.T + t) * S.G + g] = E(writes[l] / (1.0f + expf(w)));
             }
         }
     }
     // of the query and the key themselves: d - x^ (x^.d), over the length
-    const Buffer dq0 = rows_at(d_query + ((b * S.T + t0) * S.H + h) * S.K, S.H * S.K, steps, S.K), dk0 = rows_at(d_key + ((b * S.T + t0) * S.H + h) * S.K, S.H * S.K, steps, S.K);
-    float rk[4], rq[4], q[4][ND], k[4][ND];
+    const int l = thread() % WAVE, grp = l / 16, m = l % 16;
+    const f4 rk = *reinterpret_cast<const f4*>(st.rk + band + 4 * grp), rq = *reinterpret_cast<const f4*>(st.rq + band + 4 * grp);
 #pragma unroll
     for (int r = 0; r < 4; r++) {
         const int i = band + 4 * grp + r;
-        rk[r] = st.rk[i];
-        rq[r] = st.rq[i];
-        const float rkr = length_rest<St>(rk[r]), rqr = length_rest<St>(rq[r]);
         float dq = 0.0f, dk = 0.0f;
 #pragma unroll
         for (int n = 0; n < ND; n++) {
-            q[r][n] = float(Qt.get(i, d0 + 16 * n + m)) * rqr;
-            k[r][n] = float(Kt.get(i, d0 + 16 * n + m)) * rkr;
-            dq = fmaf(q[r][n], tq[n][r], dq);
-            dk = fmaf(k[r][n], tk[n][r], dk);
+            dq = fmaf(float(Qt.get(i, d0 + 16 * n + m)), tq[n][r], dq);
+            dk = fmaf(float(Kt.get(i, d0 + 16 * n + m)), tk[n][r], dk);
         }
-        dq = row16(dq);
-        dk = row16(dk);
+        dq = over_row(dq);
+        dk = over_row(dk);
         if (m == 0) {
             dots[0][half][i] = dq;
             dots[1][half][i] = dk;
         }
     }
     __syncthreads();
+    const Buffer dq0 = rows_at(d_query + ((b * S.T + t0) * S.H + h) * S.K, S.H * S.K, steps, S.K), dk0 = rows_at(d_key + ((b * S.T + t0) * S.H + h) * S.K, S.H * S.K, steps, S.K);
 #pragma unroll
     for (int r = 0; r < 4; r++) {
         const int i = band + 4 * grp + r;
-        const float dq = dots[0][0][i] + dots[0][1][i], dk = dots[1][0][i] + dots[1][1][i];
+        const float rkr = length_rest<St>(rk[r]), rqr = length_rest<St>(rq[r]);
+        const float dq = (dots[0][0][i] + dots[0][1][i]) * rqr * rqr, dk = (dots[1][0][i] + dots[1][1][i]) * rkr * rkr;
 #pragma unroll
         for (int n = 0; n < ND; n++) {
             const int c = d0 + 16 * n + m;
             const uint32_t to = c < S.K ? (i * S.H * S.K + c) * uint32_t(sizeof(E)) : NOWHERE;
-            dq0.store(E(rq[r] * fmaf(-q[r][n], dq, tq[n][r])), to);
-            dk0.store(E(rk[r] * fmaf(-k[r][n], dk, tk[n][r])), to);
+            dq0.store(E(rq[r] * fmaf(-dq, float(Qt.get(i, c)), tq[n][r])), to);
+            dk0.store(E(rk[r] * fmaf(-dk, float(Kt.get(i, c)), tk[n][r])), to);
         }
     }
 }
