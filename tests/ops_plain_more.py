@@ -60,3 +60,52 @@ def layer(stream, weight, bias, eps, d_y=None, d_stream=None):
     N = s.shape[0]
     return out | {"d": (d, e), "d_weight": ((d_y * u).sum(0), (N + 16) * U * (d_y * u).abs().sum(0) + (d_y.abs() * e_u).sum(0) + 1e-37),
                   "d_bias": (d_y.sum(0), (N + 16) * U * d_y.abs().sum(0))}
+
+
+def delta(query, key, value, gate, write, state=None, reset=None, eps=1e-6):
+    """(out, last) of the gated delta rule step by step, in the tensors' own precision; autograd gives its gradients."""
+    B, T, H, K = query.shape
+    G, V = value.shape[2:]
+    unit = lambda x: (x / torch.sqrt(x.square().sum(-1, keepdim=True) + eps)).repeat_interleave(G // H, 2)  # noqa: E731
+    q, k = unit(query), unit(key)
+    keep, rate = torch.sigmoid(-gate), torch.sigmoid(write)
+    S = state if state is not None else query.new_zeros(B, G, K, V)
+    outs = []
+    for t in range(T):
+        S = keep[:, t, :, None, None] * S
+        if reset is not None:
+            S = torch.where(reset[:, t, None, None, None].bool(), torch.zeros_like(S), S)
+        u = rate[:, t, :, None] * (value[:, t] - (k[:, t, :, None] @ S)[:, :, 0])
+        S = S + k[:, t, :, :, None] * u[:, :, None]
+        outs.append((q[:, t, :, None] @ S)[:, :, 0])
+    return torch.stack(outs, 1), S
+
+
+def delta_off(name, dtype):
+    """How far, in the 2-norm and relative to it, a result of the gated delta rule may be off, without its own rounding. What is
+    made in 32 bits is a chain of four sums of 256 terms at most (over a key, and over the steps of a chunk twice), each good to
+    as many last places, and four of them more backwards. For tensors of 16 bits its operands have 22 bits, or 11 where they
+    reach 16-bit outputs only: four such roundings each way, of half a unit of 2^-22 or 2^-11."""
+    sums = (8 if name.startswith("d_") else 4) * 256 * U
+    if dtype == torch.float32:
+        return sums
+    wide = 8 * 2.0 ** -23
+    return sums + wide + (0.0 if name in ("last", "d_state", "d_value") else 8 * 2.0 ** -12)
+
+
+def near(got, want, off, dtype):
+    """Asserts that `got` is within `off` and half a step of `dtype` of `want` in the 2-norm, and no element off by over 32 times that
+    of its own size or of the tensor's typical one (of terms that cancel to its size, about 1,000 as large)."""
+    got, want = got.detach().double().cpu(), want.detach().double().cpu()
+    assert got.shape == want.shape
+    assert torch.isfinite(got).all()
+    off = off + {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype]
+    norm, size = float(want.norm()), want.numel()
+    if not norm:
+        assert float(got.abs().max()) == 0.0 if size else True
+        return
+    d = (got - want).abs()
+    # (what lies below float32's smallest numbers, 2^-126, as after a step that keeps e^-120 = 2^-173, is 0 there)
+    assert float(d.norm()) <= off * norm + 2.0 ** -126 * size ** 0.5, f"{float(d.norm()) / norm} off, {off} allowed"
+    over = d - 2.0 ** -126 - 32 * off * torch.maximum(want.abs(), torch.full_like(want, norm / size ** 0.5))
+    assert float(over.max()) <= 0, f"{float(d.max())} off at {int(over.argmax())}, typical {norm / size ** 0.5}"
