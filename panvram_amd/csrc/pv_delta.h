@@ -128,6 +128,32 @@ template <int A, int B> __device__ inline void mma(f4& acc, const Frag<float, A>
     for (int j = 0; j < 8; j++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], acc, 0, 0, 0);
 }
 
+// The same of products FIRST .. N - 1 with one right operand, side by side: none waits for the one before it
+template <int FIRST = 0, int N, int A, int B> __device__ inline void mma_all(f4 (&acc)[N], const Frag<f16, A> (&a)[N], const Frag<f16, B>& b) {
+#pragma unroll
+    for (int i = A - 1; i >= 0; i--)
+#pragma unroll
+        for (int j = B - 1; j >= 0; j--)
+            if (i + j < (A > B ? A : B))
+#pragma unroll
+                for (int n = FIRST; n < N; n++) acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[n].p[i], b.p[j], acc[n], 0, 0, 0);
+}
+template <int FIRST = 0, int N, int A, int B> __device__ inline void mma_all(f4 (&acc)[N], const Frag<float, A> (&a)[N], const Frag<float, B>& b) {
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+#pragma unroll
+        for (int n = FIRST; n < N; n++) acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[n].v[j], b.v[j], acc[n], 0, 0, 0);
+}
+
+// of the first two alone
+template <int A, int B, typename S> __device__ inline void mma_first(f4 (&acc)[4], const Frag<S, A> (&a)[4], const Frag<S, B>& b) {
+    f4 two[2] = {acc[0], acc[1]};
+    const Frag<S, A> of_two[2] = {a[0], a[1]};
+    mma_all(two, of_two, b);
+    acc[0] = two[0];
+    acc[1] = two[1];
+}
+
 // Two results, rows 0..15 and 16..31, times `up` as an operand summed over their rows
 template <typename S, int PARTS> __device__ inline Frag<S, PARTS> frag_of(const f4& lo, const f4& hi, float up) {
     Frag<S, PARTS> f;
@@ -432,6 +458,13 @@ template <typename F> int32_t with_k(int32_t K, F&& f) {
     return f(std::integral_constant<int, 128>{});
 }
 
+
+// f of the waves of a workgroup that walks over chunks: four of them, 64 columns, where that makes workgroups for all CUs, else two (64
+// heads of 128 columns, 8,192 steps: 0.51 ms with two, 0.57 with four; a CU gets through a chunk of 64 columns in 4.5 us, of 32 in 3.9)
+template <typename F> int32_t with_waves(const Shape& S, F&& f) {
+    if (S.B * S.G * ((S.vp + 63) / 64) >= 256) return f(std::integral_constant<int, 4>{});
+    return f(std::integral_constant<int, 2>{});
+}
 
 // The call's sizes and `count` strides, each of a sequence, a step and a head: of query, key, value, gate and write, or backwards of gate,
 // write and d_out

@@ -303,12 +303,12 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         const int64_t at = (bg * S.chunks + n) * S.vp;     // of the chunk in what is kept
         const Buffer blocks(kept.blocks + at / COLS * Ke::BLOCK, KEEP ? int64_t(S.vp / COLS) * Ke::BLOCK * int(sizeof(St)) : 0);
         // operands of a stage's products are loaded while the stage before runs
-        Frag<St, 1> ka[4][KB], qa[4][KB], kc[ND][2], pa[4][2];
-        Frag<St, WIDE> ta[4][2], sf[KB];
+        Frag<St, 1> ka[KB][4], qa[KB][4], kc[2][ND], pa[2][4];
+        Frag<St, WIDE> ta[2][4], sf[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-            for (int it = 0; it < 4; it++) ka[it][kb] = Kt.rows(16 * it, kb);
+            for (int it = 0; it < 4; it++) ka[kb][it] = Kt.rows(16 * it, kb);
         fence();
         const Scale ss = scale_of<St>(over_column(largest(s)));
 #pragma unroll
@@ -320,24 +320,20 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
         for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-            for (int it = 0; it < 4; it++) qa[it][kb] = Qt.rows(16 * it, kb);
+            for (int it = 0; it < 4; it++) qa[kb][it] = Qt.rows(16 * it, kb);
         // D = V - g K S, then b D; g Q S for out
         f4 x[4], y[4], d[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) x[it] = y[it] = f4{0, 0, 0, 0};
 #pragma unroll
-        for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-            for (int it = 0; it < 4; it++) mma(x[it], ka[it][kb], sf[kb]);
+        for (int kb = 0; kb < KB; kb++) mma_all(x, ka[kb], sf[kb]);
         fence();
 #pragma unroll
         for (int it = 0; it < 4; it++)
 #pragma unroll
-            for (int kb = 0; kb <= it / 2; kb++) ta[it][kb] = Tt.rows(16 * it, kb);
+            for (int kb = 0; kb <= it / 2; kb++) ta[kb][it] = Tt.rows(16 * it, kb);
 #pragma unroll
-        for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-            for (int it = 0; it < 4; it++) mma(y[it], qa[it][kb], narrow(sf[kb]));
+        for (int kb = 0; kb < KB; kb++) mma_all(y, qa[kb], narrow(sf[kb]));
 #pragma unroll
         for (int it = 0; it < 4; it++) {
             const f4 xs = four(st.x, it), bs = four(st.b, it);
@@ -353,14 +349,12 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
         for (int k = 0; k < ND; k++)
 #pragma unroll
-            for (int kb = 0; kb < 2; kb++) kc[k][kb] = Kt.cols(16 * k, kb);
+            for (int kb = 0; kb < 2; kb++) kc[kb][k] = Kt.cols(16 * k, kb);
         f4 u[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) u[it] = f4{0, 0, 0, 0};
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-            for (int it = 2 * kb; it < 4; it++) mma(u[it], ta[it][kb], df[kb]);
+        mma_all(u, ta[0], df[0]);
+        mma_all<2>(u, ta[1], df[1]);
         const float du = ds.down * (1.0f / SQUARE<St>);
 #pragma unroll
         for (int it = 0; it < 4; it++) u[it] *= du;
@@ -384,23 +378,19 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
         for (int it = 0; it < 4; it++)
 #pragma unroll
-            for (int kb = 0; kb <= it / 2; kb++) pa[it][kb] = Pt.rows(16 * it, kb);
+            for (int kb = 0; kb <= it / 2; kb++) pa[kb][it] = Pt.rows(16 * it, kb);
         const float end = st.end, dl = us.down * (1.0f / LONG<St>), dp = us.down * (1.0f / SQUARE<St>);
         f4 z[ND], w[4];
 #pragma unroll
         for (int k = 0; k < ND; k++) z[k] = f4{0, 0, 0, 0};
 #pragma unroll
-        for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-            for (int k = 0; k < ND; k++) mma(z[k], kc[k][kb], lf[kb]);
+        for (int kb = 0; kb < 2; kb++) mma_all(z, kc[kb], lf[kb]);
         fence();
         // out = g Q S + (M Q K^T) U
 #pragma unroll
-        for (int it = 0; it < 4; it++) {
-            w[it] = f4{0, 0, 0, 0};
-#pragma unroll
-            for (int kb = 0; kb <= it / 2; kb++) mma(w[it], pa[it][kb], uf[kb]);
-        }
+        for (int it = 0; it < 4; it++) w[it] = f4{0, 0, 0, 0};
+        mma_all(w, pa[0], uf[0]);
+        mma_all<2>(w, pa[1], uf[1]);
 #pragma unroll
         for (int k = 0; k < ND; k++)
 #pragma unroll
@@ -517,16 +507,18 @@ template <typename E, int DK>
 int32_t forward(const void* query, const void* key, const void* value, const void* gate, const void* write, const float* state, const uint8_t* reset, const Shape& S,
                 void* out, float* last, void* kept, void* work, hipStream_t stream, char* err, size_t errcap) {
     using St = typename Rep<E>::S;
-    constexpr int W = 2;
     const auto in = [](const void* p) { return static_cast<const E*>(p); };
     const int64_t heads = S.B * S.G;
     char *records = static_cast<char*>(work), *images = records + heads * S.chunks * Record<St>::STRIDE;
     chunk_kernel<E, DK><<<dim3(heads * S.chunks), BLOCK, 0, stream>>>(in(query), in(key), in(gate), in(write), reset, S, records, images);
-    const dim3 grid(heads * ((S.vp / 16 + W - 1) / W));
     const Kept<St, DK> to(kept, S);
-    if (kept) state_kernel<E, DK, W, true><<<grid, (W + 1) * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to);
-    else state_kernel<E, DK, W, false><<<grid, (W + 1) * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to);
-    return launched(err, errcap);
+    return with_waves(S, [&](auto w) {
+        constexpr int W = decltype(w)::value;
+        const dim3 grid(heads * ((S.vp / 16 + W - 1) / W));
+        if (kept) state_kernel<E, DK, W, true><<<grid, (W + 1) * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to);
+        else state_kernel<E, DK, W, false><<<grid, (W + 1) * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to);
+        return launched(err, errcap);
+    });
 }
 
 }  // namespace

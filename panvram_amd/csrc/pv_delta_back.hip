@@ -87,16 +87,16 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         const int64_t at = (bg * S.chunks + n) * S.vp;     // of the chunk in what is left over
         const Buffer blocks(walked.blocks + at / COLS * Ke::BLOCK, int64_t(S.vp / COLS) * Ke::BLOCK * int(sizeof(St)));
         // operands of a stage's products are loaded while the stage before runs
-        Frag<St, 1> ka[4][KB], of[2];
-        Frag<St, WIDE> pa[4][2], ta[4][2], sf[KB];
+        Frag<St, 1> ka[KB][4], of[2];
+        Frag<St, WIDE> pa[2][4], ta[2][4], sf[KB];
 #pragma unroll
         for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-            for (int it = 0; it < 2 * kb + 2; it++) pa[it][kb] = Pt.cols(16 * it, kb);
+            for (int it = 0; it < 2 * kb + 2; it++) pa[kb][it] = Pt.cols(16 * it, kb);
 #pragma unroll
         for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-            for (int it = 0; it < 4; it++) ka[it][kb] = Kt.rows(16 * it, kb);
+            for (int it = 0; it < 4; it++) ka[kb][it] = Kt.rows(16 * it, kb);
         fence();
         const Scale ss = scale_of<St>(over_column(largest(s))), os = scale_of<St>(over_column(largest(o)));
 #pragma unroll
@@ -111,19 +111,15 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         f4 u[4], w[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) u[it] = w[it] = f4{0, 0, 0, 0};
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-            for (int it = 0; it < 2 * kb + 2; it++) mma(w[it], pa[it][kb], of[kb]);
+        mma_first(w, pa[0], of[0]);
+        mma_all(w, pa[1], of[1]);
         fence();
 #pragma unroll
         for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-            for (int it = 0; it < 2 * kb + 2; it++) ta[it][kb] = Tt.cols(16 * it, kb);
+            for (int it = 0; it < 2 * kb + 2; it++) ta[kb][it] = Tt.cols(16 * it, kb);
 #pragma unroll
-        for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-            for (int it = 0; it < 4; it++) mma(u[it], ka[it][kb], sf[kb]);
+        for (int kb = 0; kb < KB; kb++) mma_all(u, ka[kb], sf[kb]);
 #pragma unroll
         for (int it = 0; it < 4; it++) {
             const f4 ls = four(st.l, it);
@@ -137,21 +133,19 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         for (int kb = 0; kb < 2; kb++) uf[kb] = frag_of<St, WIDE>(u[2 * kb], u[2 * kb + 1], us.up);
         const float du = us.down * (1.0f / SQUARE<St>);
         fence();
-        Frag<St, 1> kc[ND][2], qc[ND][2];
+        Frag<St, 1> kc[2][ND], qc[2][ND];
 #pragma unroll
         for (int kb = 0; kb < 2; kb++)
 #pragma unroll
             for (int k = 0; k < ND; k++) {
-                qc[k][kb] = Qt.cols(16 * k, kb);
-                kc[k][kb] = Kt.cols(16 * k, kb);
+                qc[kb][k] = Qt.cols(16 * k, kb);
+                kc[kb][k] = Kt.cols(16 * k, kb);
             }
         f4 d[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) d[it] = f4{0, 0, 0, 0};
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-            for (int it = 0; it < 2 * kb + 2; it++) mma(d[it], ta[it][kb], uf[kb]);
+        mma_first(d, ta[0], uf[0]);
+        mma_all(d, ta[1], uf[1]);
 #pragma unroll
         for (int it = 0; it < 4; it++) d[it] *= du;
         const Scale ds = scale_of<St>(over_column(largest(d)));
@@ -185,13 +179,9 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
         for (int k = 0; k < ND; k++) z[k] = f4{0, 0, 0, 0};
 #pragma unroll
-        for (int kb = 0; kb < 2; kb++)
+        for (int kb = 0; kb < 2; kb++) mma_all(z, qc[kb], xf[kb]);
 #pragma unroll
-            for (int k = 0; k < ND; k++) mma(z[k], qc[k][kb], xf[kb]);
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-            for (int k = 0; k < ND; k++) mma(z[k], kc[k][kb], yf[kb]);
+        for (int kb = 0; kb < 2; kb++) mma_all(z, kc[kb], yf[kb]);
 #pragma unroll
         for (int k = 0; k < ND; k++)
 #pragma unroll
@@ -604,13 +594,16 @@ template <typename E, int DK>
 int32_t backward(const void* gate, const void* write, const void* d_out, const float* d_last, const Shape& S, void* kept, const void* records, void* d_query, void* d_key,
                  void* d_value, void* d_gate, void* d_write, float* d_state, void* work, hipStream_t stream, char* err, size_t errcap) {
     using St = typename Rep<E>::S;
-    constexpr int W = 2;
     const auto in = [](const void* p) { return static_cast<const E*>(p); };
     const auto out = [](void* p) { return static_cast<E*>(p); };
     const int64_t heads = S.B * S.G;
     const char *rec = static_cast<const char*>(records), *images = rec + heads * S.chunks * Record<St>::STRIDE;
     const Kept<St, DK> before(kept, S), walked(work, S);
-    walk_kernel<E, DK, W><<<dim3(heads * ((S.vp / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(in(d_out), d_last, S, rec, images, out(d_value), d_state, walked);
+    with_waves(S, [&](auto w) {
+        constexpr int W = decltype(w)::value;
+        walk_kernel<E, DK, W><<<dim3(heads * ((S.vp / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(in(d_out), d_last, S, rec, images, out(d_value), d_state, walked);
+        return 0;
+    });
     gradient_kernel<E, DK><<<dim3(S.B * S.H * S.chunks), MANY, 0, stream>>>(in(gate), in(write), in(d_out), S, rec, images, before, walked, out(d_query), out(d_key),
                                                                            out(d_gate), out(d_write));
     return launched(err, errcap);
