@@ -154,21 +154,39 @@ template <int A, int B, typename S> __device__ inline void mma_first(f4 (&acc)[4
     acc[1] = two[1];
 }
 
-// Two results, rows 0..15 and 16..31, times `up` as an operand summed over their rows
-template <typename S, int PARTS> __device__ inline Frag<S, PARTS> frag_of(const f4& lo, const f4& hi, float up) {
+// a x; in a chunk in which some step drops the state before it (CUT), 0 where a is 0 whatever x is: what is dropped may hold anything
+template <bool CUT> __device__ inline float part_of_it(float a, float x) { return CUT && a == 0.0f ? 0.0f : a * x; }
+template <bool CUT> __device__ inline f4 part_of_it(const f4& a, const f4& x) {
+    return f4{part_of_it<CUT>(a[0], x[0]), part_of_it<CUT>(a[1], x[1]), part_of_it<CUT>(a[2], x[2]), part_of_it<CUT>(a[3], x[3])};
+}
+// f(whether such a chunk it is) with that known to the compiler
+template <typename F> __device__ inline void by_cut(uint64_t cuts, F&& f) {
+    if (__builtin_amdgcn_readfirstlane(int(uint32_t(cuts >> 32) | uint32_t(cuts)))) f(std::true_type{});
+    else f(std::false_type{});
+}
+
+// Two results, rows 0..15 and 16..31, each times a factor, as an operand summed over their rows. (The product is a float32
+// before it is split: contracted into a conversion, which the compiler makes twice in two ways, its first part was now and then not the
+// one that the rest is of.)
+template <typename S, int PARTS> __device__ inline Frag<S, PARTS> frag_of(const f4& lo, const f4& hi, const f4& up_lo, const f4& up_hi) {
     Frag<S, PARTS> f;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        const float x = j < 4 ? lo[j] : hi[j - 4];
+        float x = j < 4 ? lo[j] * up_lo[j] : hi[j - 4] * up_hi[j - 4];
+        if constexpr (sizeof(S) == 2) asm("" : "+v"(x));
         if constexpr (sizeof(S) == 4) {
             f.v[j] = x;
         } else {
-            const f16 h = f16(x * up);
+            const f16 h = f16(x);
             f.p[0][j] = h;
-            if constexpr (PARTS == 2) f.p[1][j] = f16(fmaf(x, up, -float(h)));
+            if constexpr (PARTS == 2) f.p[1][j] = f16(x - float(h));
         }
     }
     return f;
+}
+template <typename S, int PARTS> __device__ inline Frag<S, PARTS> frag_of(const f4& lo, const f4& hi, float up) {
+    const f4 all = {up, up, up, up};
+    return frag_of<S, PARTS>(lo, hi, all, all);
 }
 template <int PARTS> __device__ inline const Frag<float, 1>& narrow(const Frag<float, PARTS>& f) { return f; }
 template <int PARTS> __device__ inline Frag<f16, 1> narrow(const Frag<f16, PARTS>& f) { return {{f.p[0]}}; }
@@ -340,7 +358,7 @@ struct Shape {
 };
 
 // What is known of a chunk's steps before its state is:
-//   x     g r: g what a step keeps of the state before the chunk (0 past a reset), r what is left of one over the key's length
+//   x     b g r: g what a step keeps of the state before the chunk (0 past a reset), r what is left of one over the key's length, b:
 //   b     sigmoid(write)
 //   l     l r: l what is left of a step's addition at the chunk's end
 //   q     g r of the query

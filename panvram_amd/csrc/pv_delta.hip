@@ -149,7 +149,7 @@ __global__ __launch_bounds__(BLOCK, 4) void chunk_kernel(const E* __restrict__ q
     const float shift = tid < C ? st.x[tid] : 0.0f;
     __syncthreads();
     if (tid < C) {
-        st.x[tid] = shift * length_rest<St>(st.rk[tid]);
+        st.x[tid] = st.b[tid] * (shift * length_rest<St>(st.rk[tid]));
         st.q[tid] = shift * length_rest<St>(st.rq[tid]);
         st.l[tid] *= length_rest<St>(st.rk[tid]);
     }
@@ -296,6 +296,7 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         const Square Tt{const_cast<St*>(&re.inv[0][0][0])};
         const Plain Pt{const_cast<St*>(&re.pair[0][0][0])};
         const auto four = [&](const float* p, int it) { return *reinterpret_cast<const f4*>(p + 16 * it + 4 * grp); };
+        const uint64_t cuts = uint64_t(st.cut[1]) << 32 | st.cut[0];
         f4 v[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) v[it] = vp.four(it);
@@ -334,12 +335,10 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
             for (int kb = 0; kb <= it / 2; kb++) ta[kb][it] = Tt.rows(16 * it, kb);
 #pragma unroll
         for (int kb = 0; kb < KB; kb++) mma_all(y, qa[kb], narrow(sf[kb]));
+        by_cut(cuts, [&](auto cut) {
 #pragma unroll
-        for (int it = 0; it < 4; it++) {
-            const f4 xs = four(st.x, it), bs = four(st.b, it);
-#pragma unroll
-            for (int r = 0; r < 4; r++) d[it][r] = bs[r] * (v[it][r] - (xs[r] == 0.0f ? 0.0f : xs[r] * (ss.down * x[it][r])));      // (a dropped state may hold anything)
-        }
+            for (int it = 0; it < 4; it++) d[it] = four(st.b, it) * v[it] - part_of_it<decltype(cut)::value>(four(st.x, it) * ss.down, x[it]);
+        });
         const Scale ds = scale_of<St>(over_column(largest(d)));
         Frag<St, WIDE> df[2];
 #pragma unroll
@@ -355,17 +354,16 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         for (int it = 0; it < 4; it++) u[it] = f4{0, 0, 0, 0};
         mma_all(u, ta[0], df[0]);
         mma_all<2>(u, ta[1], df[1]);
-        const float du = ds.down * (1.0f / SQUARE<St>);
-#pragma unroll
-        for (int it = 0; it < 4; it++) u[it] *= du;
+        const float du = ds.down * (1.0f / SQUARE<St>);        // of u
         // what it adds to the state (l r is 2 / LONG at most)
-        const Scale us = scale_of<St>(over_column(largest(u)));
+        const Scale us = scale_of<St>(over_column(largest(u)) * du);
         Frag<St, 1> uf[2];
         Frag<St, WIDE> lf[2];
+        const float up = sizeof(St) == 2 ? du * us.up : 1.0f;
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
-            uf[kb] = frag_of<St, 1>(u[2 * kb], u[2 * kb + 1], us.up);
-            lf[kb] = frag_of<St, WIDE>(LONG<St> * u[2 * kb] * four(st.l, 2 * kb), LONG<St> * u[2 * kb + 1] * four(st.l, 2 * kb + 1), us.up);
+            uf[kb] = frag_of<St, 1>(u[2 * kb], u[2 * kb + 1], up);
+            lf[kb] = frag_of<St, WIDE>(u[2 * kb], u[2 * kb + 1], four(st.l, 2 * kb) * (LONG<St> * up), four(st.l, 2 * kb + 1) * (LONG<St> * up));
             if constexpr (KEEP) leave(blocks, step_at + 32 * kb * sizeof(St), uf[kb]);
         }
         if constexpr (KEEP) {
@@ -391,16 +389,20 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         for (int it = 0; it < 4; it++) w[it] = f4{0, 0, 0, 0};
         mma_all(w, pa[0], uf[0]);
         mma_all<2>(w, pa[1], uf[1]);
+        by_cut(cuts, [&](auto cut) {
+            constexpr bool CUT = decltype(cut)::value;
 #pragma unroll
-        for (int k = 0; k < ND; k++)
+            for (int k = 0; k < ND; k++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) s[k][r] = fmaf(dl, z[k][r], end == 0.0f ? 0.0f : end * s[k][r]);
+                for (int r = 0; r < 4; r++) s[k][r] = fmaf(dl, z[k][r], part_of_it<CUT>(end, s[k][r]));
+#pragma unroll
+            for (int it = 0; it < 4; it++) y[it] = part_of_it<CUT>(four(st.q, it) * ss.down, y[it]);
+        });
         const Buffer to = rows_at(out + ((b * S.T + n * C) * S.G + g) * S.V, ot, rows_of(n), S.V);
 #pragma unroll
         for (int it = 0; it < 4; it++) {
-            const f4 qs = four(st.q, it);
 #pragma unroll
-            for (int r = 0; r < 4; r++) Sixteen<E>::store(to, ot, out_at, 4 * it + r, fmaf(dp, w[it][r], qs[r] == 0.0f ? 0.0f : qs[r] * (ss.down * y[it][r])));
+            for (int r = 0; r < 4; r++) Sixteen<E>::store(to, ot, out_at, 4 * it + r, fmaf(dp, w[it][r], y[it][r]));
         }
     }
 #pragma unroll

@@ -76,13 +76,10 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         const Square Tt{const_cast<St*>(&re.inv[0][0][0])}, Pt{const_cast<St*>(&re.pair[0][0][0])};
         const auto four = [&](const float* p, int it) { return *reinterpret_cast<const f4*>(p + 16 * it + 4 * grp); };
         const int rows = rows_of(n);
+        const uint64_t cuts = uint64_t(st.cut[1]) << 32 | st.cut[0];
         f4 o[4];
 #pragma unroll
-        for (int it = 0; it < 4; it++) {
-            o[it] = op.four(it);
-#pragma unroll
-            for (int r = 0; r < 4; r++) o[it][r] = 16 * it + 4 * grp + r < rows ? o[it][r] : 0.0f;
-        }
+        for (int it = 0; it < 4; it++) o[it] = op.four(it);
         if (n) op.load(rows_at(o0 + (n - 1) * C * S.ot, S.ot, rows_of(n - 1), S.V), S.ot, out_at);
         const int64_t at = (bg * S.chunks + n) * S.vp;     // of the chunk in what is left over
         const Buffer blocks(walked.blocks + at / COLS * Ke::BLOCK, int64_t(S.vp / COLS) * Ke::BLOCK * int(sizeof(St)));
@@ -120,12 +117,10 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
             for (int it = 0; it < 2 * kb + 2; it++) ta[kb][it] = Tt.cols(16 * it, kb);
 #pragma unroll
         for (int kb = 0; kb < KB; kb++) mma_all(u, ka[kb], sf[kb]);
+        by_cut(cuts, [&](auto cut) {
 #pragma unroll
-        for (int it = 0; it < 4; it++) {
-            const f4 ls = four(st.l, it);
-#pragma unroll
-            for (int r = 0; r < 4; r++) u[it][r] = fmaf(dp, w[it][r], ls[r] == 0.0f ? 0.0f : ls[r] * (ss.down * u[it][r]));
-        }
+            for (int it = 0; it < 4; it++) u[it] = part_of_it<decltype(cut)::value>(four(st.l, it) * ss.down, u[it]) + dp * w[it];
+        });
         // dR = T^T dU
         const Scale us = scale_of<St>(over_column(largest(u)));
         Frag<St, WIDE> uf[2];
@@ -146,25 +141,23 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         for (int it = 0; it < 4; it++) d[it] = f4{0, 0, 0, 0};
         mma_first(d, ta[0], uf[0]);
         mma_all(d, ta[1], uf[1]);
-#pragma unroll
-        for (int it = 0; it < 4; it++) d[it] *= du;
-        const Scale ds = scale_of<St>(over_column(largest(d)));
+        const Scale ds = scale_of<St>(over_column(largest(d)) * du);
         const Buffer to = rows_at(d_value + ((b * S.T + n * C) * S.G + g) * S.V, vt, rows, S.V);
         f4 x[4], y[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) {
-            const f4 bd = four(st.b, it) * d[it];
+            const f4 bs = four(st.b, it) * du;
             x[it] = four(st.q, it) * o[it];
-            y[it] = -four(st.x, it) * bd;
+            y[it] = four(st.x, it) * d[it] * -du;
 #pragma unroll
-            for (int r = 0; r < 4; r++) Sixteen<E>::store(to, vt, value_at, 4 * it + r, bd[r]);
+            for (int r = 0; r < 4; r++) Sixteen<E>::store(to, vt, value_at, 4 * it + r, bs[r] * d[it][r]);
         }
         // (q and x are 2 / LONG at most)
         const Scale xs = scale_of<St>(over_column(fmaxf(largest(x), largest(y))));
         Frag<St, WIDE> xf[2], yf[2];
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
-            leave(blocks, step_at + 32 * kb * sizeof(St), frag_of<St, 1>(d[2 * kb], d[2 * kb + 1], ds.up));
+            leave(blocks, step_at + 32 * kb * sizeof(St), frag_of<St, 1>(d[2 * kb], d[2 * kb + 1], sizeof(St) == 2 ? du * ds.up : 1.0f));
             xf[kb] = frag_of<St, WIDE>(x[2 * kb], x[2 * kb + 1], xs.up);
             yf[kb] = frag_of<St, WIDE>(y[2 * kb], y[2 * kb + 1], xs.up);
         }
@@ -182,10 +175,12 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         for (int kb = 0; kb < 2; kb++) mma_all(z, qc[kb], xf[kb]);
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) mma_all(z, kc[kb], yf[kb]);
+        by_cut(cuts, [&](auto cut) {
 #pragma unroll
-        for (int k = 0; k < ND; k++)
+            for (int k = 0; k < ND; k++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) s[k][r] = fmaf(xs.down, z[k][r], end == 0.0f ? 0.0f : end * s[k][r]);
+                for (int r = 0; r < 4; r++) s[k][r] = fmaf(xs.down, z[k][r], part_of_it<decltype(cut)::value>(end, s[k][r]));
+        });
     }
     if (!d_state) return;
 #pragma unroll
@@ -364,7 +359,12 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
                 const auto x = pack<St, UNIT>::load(S0.p + at), y = pack<St, UNIT>::load(S1.p + at);
                 float z = 0.0f;
 #pragma unroll
-                for (int e = 0; e < UNIT; e++) z = fmaf(float(x.v[e]), float(y.v[e]), z);
+                for (int e = 0; e < UNIT; e++) if constexpr (!HALF) z = fmaf(x.v[e], y.v[e], z);
+                if constexpr (HALF) {
+                    using h2 = __attribute__((ext_vector_type(2))) _Float16;
+#pragma unroll
+                    for (int e = 0; e < UNIT; e += 2) z = __builtin_amdgcn_fdot2(h2{x.v[e], x.v[e + 1]}, h2{y.v[e], y.v[e + 1]}, z, false);
+                }
                 if (HALF) z *= f0[v0 + c] * f1[v0 + c];
                 product[k % 2] += tid + k * MANY < UNITS ? z : 0.0f;
             }
@@ -426,8 +426,8 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
             }
 #pragma unroll
             for (int n = 0; n < ND; n++) {
-                const float x = gi == 0.0f ? 0.0f : gi * ldexpf(aq[n][r], top[0]), y = gi == 0.0f ? 0.0f : -bi[r] * gi * ldexpf(from[n][r], top[1]);
-                const float z = li == 0.0f ? 0.0f : li * ldexpf(to[n][r], top[2]);
+                const float x = part_of_it<true>(gi, ldexpf(aq[n][r], top[0])), y = part_of_it<true>(-bi[r] * gi, ldexpf(from[n][r], top[1]));
+                const float z = part_of_it<true>(li, ldexpf(to[n][r], top[2]));
                 dq = fmaf(q[n], x, dq);
                 df = fmaf(k[n], y, df);
                 dt = fmaf(k[n], z, dt);
