@@ -414,7 +414,7 @@ int32_t pv_add_rms_norm_backward_hip(const void* s, const float* rstd, const flo
  * state: f32[B, G, K, V] before step 0, or NULL: zero. reset: u8[B, T], or NULL; where not 0, S[t-1] is dropped. out: [B, T, G, V] of
  * `dtype`; last: f32[B, G, K, V] = S[T-1], apart from state. For the backward pass: kept (pv_gated_delta_kept_bytes, 16-byte
  * aligned; NULL: none) and what the call leaves in `work`. work: pv_gated_delta_work_bytes with keep = 1 if kept is given, else 0. */
-uint64_t pv_gated_delta_work_bytes(int64_t B, int64_t T, int32_t H, int32_t G, int32_t K, int32_t dtype, int32_t keep);
+uint64_t pv_gated_delta_work_bytes(int64_t B, int64_t T, int32_t H, int32_t G, int32_t K, int32_t V, int32_t dtype, int32_t keep);
 uint64_t pv_gated_delta_kept_bytes(int64_t B, int64_t T, int32_t G, int32_t K, int32_t V, int32_t dtype);
 int32_t pv_gated_delta_hip(const void* query, const void* key, const void* value, const void* gate, const void* write, const float* state, const uint8_t* reset,
                            int64_t B, int64_t T, int32_t H, int32_t G, int32_t K, int32_t V, const int64_t* strides, float eps, int32_t dtype, void* out, float* last,

@@ -378,6 +378,7 @@ template <typename S> struct Record {
     S inv[wide_of<S>][C][C + PAD], pair[wide_of<S>][C][C + PAD];
     static constexpr int ALL = 2080 + 2 * wide_of<S> * C * (C + PAD) * int(sizeof(S));
     static constexpr int NARROW = ALL - (wide_of<S> - 1) * C * (C + PAD) * int(sizeof(S));     // without the second part of M q k^T
+    static constexpr int INVERSE = 2080 + wide_of<S> * C * (C + PAD) * int(sizeof(S));          // without M q k^T
     static constexpr int STRIDE = (ALL + 1023) / 1024 * 1024;
 };
 template <typename S, int DK> constexpr int IMAGE = (2 * Tile<S, C, DK>::SIZE * int(sizeof(S)) + 1023) / 1024 * 1024;
@@ -477,10 +478,35 @@ template <typename F> int32_t with_k(int32_t K, F&& f) {
 }
 
 
+// Sequences of few heads are walked in pieces, all at once: each from a state of zero, and beside the columns of values those of a state of
+// one, which gives the map from the state before the piece to that after it; then the maps are joined from piece to piece; then each
+// piece is walked once more, from its true start. That is some three times the work, and a join costs what a few chunks do, so it takes
+// four pieces at least, of 8 chunks at least; there are as many as give all CUs a workgroup in the first walk.
+struct Pieces {
+    int32_t count;                         // 1: the walk is as it is
+    int64_t chunks;                        // of a piece; the last one's may be fewer
+};
+inline Pieces pieces_of(int64_t heads, int64_t chunks, int32_t vp, int32_t dk) {
+    int64_t n = 256 / (heads * ((vp + dk + 63) / 64));
+    n = n < chunks / 8 ? n : chunks / 8;
+    if (n < 4) return {1, chunks};
+    const int64_t each = (chunks + n - 1) / n;
+    return {int32_t((chunks + each - 1) / each), each};
+}
+// What lies in memory between them, in float32 and by columns: each piece's end from zero and, by the columns of one, its map; each
+// piece's start; whether some step of the piece drops the state before it (the map is zero then, whatever that state may hold)
+struct Joins {
+    float *ends, *starts;
+    uint32_t* cut;
+    __host__ __device__ Joins(void* p, int64_t heads, int32_t pieces, int32_t vp, int32_t dk)
+        : ends(static_cast<float*>(p)), starts(ends + heads * pieces * int64_t(vp + dk) * dk), cut(reinterpret_cast<uint32_t*>(starts + heads * pieces * int64_t(vp) * dk)) {}
+    static uint64_t bytes(uint64_t heads, uint64_t pieces, uint64_t vp, uint64_t dk) { return heads * pieces * ((vp + dk) * dk + vp * dk + 1) * 4; }
+};
+
 // f of the waves of a workgroup that walks over chunks: four of them, 64 columns, where that makes workgroups for all CUs, else two (64
 // heads of 128 columns, 8,192 steps: 0.51 ms with two, 0.57 with four; a CU gets through a chunk of 64 columns in 4.5 us, of 32 in 3.9)
-template <typename F> int32_t with_waves(const Shape& S, F&& f) {
-    if (S.B * S.G * ((S.vp + 63) / 64) >= 256) return f(std::integral_constant<int, 4>{});
+template <typename F> int32_t with_waves(const Shape& S, const Pieces& pieces, F&& f) {
+    if (pieces.count * S.B * S.G * ((S.vp + 63) / 64) >= 256) return f(std::integral_constant<int, 4>{});
     return f(std::integral_constant<int, 2>{});
 }
 

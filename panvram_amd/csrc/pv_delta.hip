@@ -238,10 +238,11 @@ __global__ __launch_bounds__(BLOCK, 4) void chunk_kernel(const E* __restrict__ q
 // worked on, where two have room (tensors of 16 bits), else one after another. (A wave that brings is held up until the memory system
 // has taken all it asks for, 3 us a chunk.)
 
-template <typename E, int DK, int W, bool KEEP>
+// MAP: the first walk of a sequence in pieces; there are no outputs, and DK columns more that begin as those of one.
+template <typename E, int DK, int W, bool KEEP, bool MAP>
 __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))) void state_kernel(
     const E* __restrict__ value, const float* __restrict__ state, Shape S, const char* __restrict__ records, const char* __restrict__ images, E* __restrict__ out,
-    float* __restrict__ last, Kept<typename Rep<E>::S, DK> kept) {
+    float* __restrict__ last, Kept<typename Rep<E>::S, DK> kept, Pieces pieces, Joins joins) {
     using St = typename Rep<E>::S;
     using Ke = Kept<St, DK>;
     constexpr int WIDE = wide_of<St>, ND = DK / 16, KB = DK / 32;
@@ -252,10 +253,11 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
     constexpr int BUFFERS = sizeof(St) == 2 ? 2 : 1, IN = IMAGE<St, DK>, BUFFER = IN + (Re::NARROW + 1023) / 1024 * 1024;
     __shared__ alignas(1024) char lds[BUFFERS * BUFFER];
     const int tid = threadIdx.x, wave = tid / WAVE, l = tid % WAVE, grp = l / 16, m = l % 16;
-    const int groups = (S.vp / 16 + W - 1) / W;
-    const auto [bg, group] = part_of(blockIdx.x, S.B * S.G, groups);
+    const int width = MAP ? S.vp + DK : S.vp, groups = (width / 16 + W - 1) / W;
+    const auto [piece, group] = part_of(blockIdx.x, S.B * S.G * pieces.count, groups);
     const int col = (group * W + wave) * 16 + m;
-    const int64_t b = bg / S.G;
+    const int64_t bg = piece / pieces.count, b = bg / S.G, first = piece % pieces.count * pieces.chunks;
+    const int64_t behind = first + pieces.chunks < S.chunks ? first + pieces.chunks : S.chunks;
     const int g = int(bg % S.G), h = shared(S, g);
     const bool on = col < S.V;
     const E* v0 = value + b * S.vb + g * S.vh;
@@ -270,24 +272,27 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int d = 16 * n + 4 * grp + r;
-            s[n][r] = state && on && d < S.K ? state[(bg * S.K + d) * S.V + col] : 0.0f;
+            if constexpr (MAP) s[n][r] = col - S.vp == d ? 1.0f : 0.0f;
+            else if (first) s[n][r] = col < S.vp ? joins.starts[(piece * S.vp + col) * DK + d] : 0.0f;
+            else s[n][r] = state && on && d < S.K ? state[(bg * S.K + d) * S.V + col] : 0.0f;
         }
     const auto rows_of = [&](int64_t n) { return int(S.T - n * C < C ? S.T - n * C : C); };
     if (wave == W) {
-        for (int64_t n = 0; n < S.chunks; n++) {
-            if (n && BUFFERS == 1) __syncthreads();        // the chunk before has been used
+        for (int64_t n = first; n < behind; n++) {
+            if (n != first && BUFFERS == 1) __syncthreads();   // the chunk before has been used
             char* to = lds + (BUFFERS == 2 ? int(n & 1) * BUFFER : 0);
-            bring<1>(in0 + n * IN, to, 2 * In::SIZE * int(sizeof(St)), 0);
-            bring<1>(rec0 + n * Re::STRIDE, to + IN, Re::NARROW, 0);
+            bring<1>(in0 + n * IN, to, (MAP ? 1 : 2) * In::SIZE * int(sizeof(St)), 0);
+            bring<1>(rec0 + n * Re::STRIDE, to + IN, MAP ? Re::INVERSE : Re::NARROW, 0);
             arrived<0>();
             __syncthreads();               // the chunk is there (and of two, the one before has been used)
         }
         return;
     }
     Sixteen<E> vp;
-    vp.load(rows_at(v0, S.vt, rows_of(0), S.V), S.vt, value_at);
-    for (int64_t n = 0; n < S.chunks; n++) {
-        if (n && BUFFERS == 1) __syncthreads();
+    vp.load(rows_at(v0 + first * C * S.vt, S.vt, rows_of(first), S.V), S.vt, value_at);
+    uint64_t any = 0;                      // step that drops the state before it
+    for (int64_t n = first; n < behind; n++) {
+        if (n != first && BUFFERS == 1) __syncthreads();
         __syncthreads();
         char* here = lds + (BUFFERS == 2 ? int(n & 1) * BUFFER : 0);
         const In Kt{reinterpret_cast<St*>(here)}, Qt{reinterpret_cast<St*>(here) + In::SIZE};
@@ -300,7 +305,8 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         f4 v[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) v[it] = vp.four(it);
-        if (n + 1 < S.chunks) vp.load(rows_at(v0 + (n + 1) * C * S.vt, S.vt, rows_of(n + 1), S.V), S.vt, value_at);
+        any |= cuts;
+        if (n + 1 < behind) vp.load(rows_at(v0 + (n + 1) * C * S.vt, S.vt, rows_of(n + 1), S.V), S.vt, value_at);
         const int64_t at = (bg * S.chunks + n) * S.vp;     // of the chunk in what is kept
         const Buffer blocks(kept.blocks + at / COLS * Ke::BLOCK, KEEP ? int64_t(S.vp / COLS) * Ke::BLOCK * int(sizeof(St)) : 0);
         // operands of a stage's products are loaded while the stage before runs
@@ -318,10 +324,12 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
             if constexpr (KEEP) leave(blocks, state_at + 32 * kb * sizeof(St), sf[kb]);
         }
         fence();
+        if constexpr (!MAP) {
 #pragma unroll
-        for (int kb = 0; kb < KB; kb++)
+            for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-            for (int it = 0; it < 4; it++) qa[kb][it] = Qt.rows(16 * it, kb);
+                for (int it = 0; it < 4; it++) qa[kb][it] = Qt.rows(16 * it, kb);
+        }
         // D = V - g K S, then b D; g Q S for out
         f4 x[4], y[4], d[4];
 #pragma unroll
@@ -334,7 +342,7 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
             for (int kb = 0; kb <= it / 2; kb++) ta[kb][it] = Tt.rows(16 * it, kb);
 #pragma unroll
-        for (int kb = 0; kb < KB; kb++) mma_all(y, qa[kb], narrow(sf[kb]));
+        for (int kb = 0; kb < KB; kb++) if constexpr (!MAP) mma_all(y, qa[kb], narrow(sf[kb]));
         by_cut(cuts, [&](auto cut) {
 #pragma unroll
             for (int it = 0; it < 4; it++) d[it] = four(st.b, it) * v[it] - part_of_it<decltype(cut)::value>(four(st.x, it) * ss.down, x[it]);
@@ -373,10 +381,12 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
             scales.store(us.down, to, S.vp * 4);
         }
         fence();
+        if constexpr (!MAP) {
 #pragma unroll
-        for (int it = 0; it < 4; it++)
+            for (int it = 0; it < 4; it++)
 #pragma unroll
-            for (int kb = 0; kb <= it / 2; kb++) pa[kb][it] = Pt.rows(16 * it, kb);
+                for (int kb = 0; kb <= it / 2; kb++) pa[kb][it] = Pt.rows(16 * it, kb);
+        }
         const float end = st.end, dl = us.down * (1.0f / LONG<St>), dp = us.down * (1.0f / SQUARE<St>);
         f4 z[ND], w[4];
 #pragma unroll
@@ -387,8 +397,10 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         // out = g Q S + (M Q K^T) U
 #pragma unroll
         for (int it = 0; it < 4; it++) w[it] = f4{0, 0, 0, 0};
-        mma_all(w, pa[0], uf[0]);
-        mma_all<2>(w, pa[1], uf[1]);
+        if constexpr (!MAP) {
+            mma_all(w, pa[0], uf[0]);
+            mma_all<2>(w, pa[1], uf[1]);
+        }
         by_cut(cuts, [&](auto cut) {
             constexpr bool CUT = decltype(cut)::value;
 #pragma unroll
@@ -396,8 +408,9 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
                 for (int r = 0; r < 4; r++) s[k][r] = fmaf(dl, z[k][r], part_of_it<CUT>(end, s[k][r]));
 #pragma unroll
-            for (int it = 0; it < 4; it++) y[it] = part_of_it<CUT>(four(st.q, it) * ss.down, y[it]);
+            for (int it = 0; it < 4; it++) if constexpr (!MAP) y[it] = part_of_it<CUT>(four(st.q, it) * ss.down, y[it]);
         });
+        if constexpr (MAP) continue;
         const Buffer to = rows_at(out + ((b * S.T + n * C) * S.G + g) * S.V, ot, rows_of(n), S.V);
 #pragma unroll
         for (int it = 0; it < 4; it++) {
@@ -410,8 +423,63 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int d = 16 * n + 4 * grp + r;
-            if (on && d < S.K) last[(bg * S.K + d) * S.V + col] = s[n][r];
+            if (!MAP && on && d < S.K && behind == S.chunks) last[(bg * S.K + d) * S.V + col] = s[n][r];
         }
+    if constexpr (MAP) {
+        if (col < width) {
+            float* to = joins.ends + (piece * width + col) * DK + 4 * grp;
+#pragma unroll
+            for (int n = 0; n < ND; n++) *reinterpret_cast<f4*>(to + 16 * n) = s[n];
+        }
+        if (group == 0 && tid == 0) joins.cut[piece] = any != 0;
+    }
+}
+
+// ---- join_kernel: each piece's start from the one before it, in 32 bits: a wave for 16 columns of a head's state
+
+template <int DK>
+__global__ __launch_bounds__(BLOCK) void join_kernel(const float* __restrict__ state, Shape S, int pieces, Joins joins) {
+    constexpr int ND = DK / 16, KB = DK / 32;
+    const int l = threadIdx.x % WAVE, grp = l / 16, m = l % 16, groups = (S.vp / 16 + WAVES - 1) / WAVES;
+    const int64_t bg = blockIdx.x / groups;
+    const int col = int(blockIdx.x % groups * WAVES + threadIdx.x / WAVE) * 16 + m;
+    if (col >= S.vp) return;               // (a whole wave)
+    f4 s[ND];
+#pragma unroll
+    for (int n = 0; n < ND; n++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int d = 16 * n + 4 * grp + r;
+            s[n][r] = state && col < S.V && d < S.K ? state[(bg * S.K + d) * S.V + col] : 0.0f;
+        }
+    for (int p = 0; p + 1 < pieces; p++) {
+        const int64_t piece = bg * pieces + p;
+        const float *end = joins.ends + piece * (S.vp + DK) * DK, *map = end + int64_t(S.vp) * DK;
+        const bool cut = joins.cut[piece];
+        f4 x[ND], z[ND];
+#pragma unroll
+        for (int n = 0; n < ND; n++) {
+            z[n] = f4{0, 0, 0, 0};
+            x[n] = *reinterpret_cast<const f4*>(end + int64_t(col) * DK + 16 * n + 4 * grp);
+        }
+        if (!cut) {
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) {
+                Frag<float, 1> a[ND];
+#pragma unroll
+                for (int n = 0; n < ND; n++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) a[n].v[j] = map[(32 * kb + 4 * grp + j % 4 + j / 4 * 16) * DK + 16 * n + m];
+                mma_all(z, a, frag_of<float, 1>(s[2 * kb], s[2 * kb + 1], 1.0f));
+            }
+        }
+        float* to = joins.starts + ((piece + 1) * S.vp + col) * DK + 4 * grp;
+#pragma unroll
+        for (int n = 0; n < ND; n++) {
+            s[n] = z[n] + x[n];
+            *reinterpret_cast<f4*>(to + 16 * n) = s[n];
+        }
+    }
 }
 
 // ---- step_kernel: few steps, one by one. A workgroup has 32 columns of a state, a lane four neighbouring ones of every 32nd row
@@ -514,11 +582,19 @@ int32_t forward(const void* query, const void* key, const void* value, const voi
     char *records = static_cast<char*>(work), *images = records + heads * S.chunks * Record<St>::STRIDE;
     chunk_kernel<E, DK><<<dim3(heads * S.chunks), BLOCK, 0, stream>>>(in(query), in(key), in(gate), in(write), reset, S, records, images);
     const Kept<St, DK> to(kept, S);
-    return with_waves(S, [&](auto w) {
+    const Pieces pieces = pieces_of(heads, S.chunks, S.vp, DK);
+    const Joins joins(images + S.B * S.H * S.chunks * IMAGE<St, DK>, heads, pieces.count, S.vp, DK);
+    if (pieces.count > 1) {
+        constexpr int W = 4;
+        state_kernel<E, DK, W, false, true><<<dim3(heads * pieces.count * (((S.vp + DK) / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(
+            in(value), nullptr, S, records, images, nullptr, nullptr, to, pieces, joins);
+        join_kernel<DK><<<dim3(heads * ((S.vp / 16 + WAVES - 1) / WAVES)), BLOCK, 0, stream>>>(state, S, pieces.count, joins);
+    }
+    return with_waves(S, pieces, [&](auto w) {
         constexpr int W = decltype(w)::value;
-        const dim3 grid(heads * ((S.vp / 16 + W - 1) / W));
-        if (kept) state_kernel<E, DK, W, true><<<grid, (W + 1) * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to);
-        else state_kernel<E, DK, W, false><<<grid, (W + 1) * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to);
+        const dim3 grid(heads * pieces.count * ((S.vp / 16 + W - 1) / W));
+        if (kept) state_kernel<E, DK, W, true, false><<<grid, (W + 1) * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to, pieces, joins);
+        else state_kernel<E, DK, W, false, false><<<grid, (W + 1) * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to, pieces, joins);
         return launched(err, errcap);
     });
 }
@@ -527,10 +603,13 @@ int32_t forward(const void* query, const void* key, const void* value, const voi
 
 extern "C" {
 
-uint64_t pv_gated_delta_work_bytes(int64_t B, int64_t T, int32_t H, int32_t G, int32_t K, int32_t dtype, int32_t keep) {
-    if (B < 1 || H < 1 || G < 1 || T < 1 || (T <= SHORT && !keep)) return 0;
-    const uint64_t chunks = uint64_t(B) * uint64_t((T + C - 1) / C);
-    return chunks * (uint64_t(G) * (dtype == PV_F32 ? Record<float>::STRIDE : Record<f16>::STRIDE) + uint64_t(H) * image_bytes(columns_of(K), dtype));
+uint64_t pv_gated_delta_work_bytes(int64_t B, int64_t T, int32_t H, int32_t G, int32_t K, int32_t V, int32_t dtype, int32_t keep) {
+    if (B < 1 || H < 1 || G < 1 || T < 1 || K < 1 || V < 1 || (T <= SHORT && !keep)) return 0;
+    const int64_t chunks = (T + C - 1) / C, heads = B * G;
+    const int32_t vp = (V + 31) / 32 * 32, dk = columns_of(K);
+    const Pieces pieces = pieces_of(heads, chunks, vp, dk);
+    return uint64_t(B) * chunks * (uint64_t(G) * (dtype == PV_F32 ? Record<float>::STRIDE : Record<f16>::STRIDE) + uint64_t(H) * image_bytes(dk, dtype)) +
+           (pieces.count > 1 ? Joins::bytes(heads, pieces.count, vp, dk) : 0);
 }
 
 uint64_t pv_gated_delta_kept_bytes(int64_t B, int64_t T, int32_t G, int32_t K, int32_t V, int32_t dtype) {
@@ -545,7 +624,7 @@ int32_t pv_gated_delta_hip(const void* query, const void* key, const void* value
     if (int32_t e = shape_of(B, T, H, G, K, V, strides, 15, eps, dtype, S, err, errcap)) return e;
     if (!query || !key || !value || !gate || !write || !out || !last) return fail(PV_EARG, err, errcap, "null argument");
     if (kept && !aligned(kept, 16)) return fail(PV_EARG, err, errcap, "kept: not 16-byte aligned");
-    const uint64_t need = pv_gated_delta_work_bytes(B, T, H, G, K, dtype, kept != nullptr);
+    const uint64_t need = pv_gated_delta_work_bytes(B, T, H, G, K, V, dtype, kept != nullptr);
     if (need && (!work || work_bytes < need || !aligned(work, 16))) return fail(PV_EARG, err, errcap, "work: too small, or not 16-byte aligned");
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);

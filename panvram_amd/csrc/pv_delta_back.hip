@@ -599,7 +599,7 @@ int32_t backward(const void* gate, const void* write, const void* d_out, const f
     const int64_t heads = S.B * S.G;
     const char *rec = static_cast<const char*>(records), *images = rec + heads * S.chunks * Record<St>::STRIDE;
     const Kept<St, DK> before(kept, S), walked(work, S);
-    with_waves(S, [&](auto w) {
+    with_waves(S, Pieces{1, S.chunks}, [&](auto w) {
         constexpr int W = decltype(w)::value;
         walk_kernel<E, DK, W><<<dim3(heads * ((S.vp / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(in(d_out), d_last, S, rec, images, out(d_value), d_state, walked);
         return 0;

@@ -28,7 +28,7 @@ def _forward(index, query, key, value, gate, write, state, reset, eps, keep):
     last = torch.empty((B, G, K, V), dtype=torch.float32, device=dev)
     L, code = N.lib(), DTYPES[dtype]
     kept = torch.empty(L.pv_gated_delta_kept_bytes(B, T, G, K, V, code), dtype=torch.uint8, device=dev) if keep else None
-    size = L.pv_gated_delta_work_bytes(B, T, H, G, K, code, int(keep))
+    size = L.pv_gated_delta_work_bytes(B, T, H, G, K, V, code, int(keep))
     work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     call(L.pv_gated_delta_hip, index, *(t.data_ptr() for t in given), ptr(state), ptr(reset), B, T, H, G, K, V, _strides(*given), eps, code, out.data_ptr(),
          last.data_ptr(), ptr(kept), ptr(work), size)
