@@ -435,16 +435,33 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
     }
 }
 
-// ---- join_kernel: each piece's start from the one before it, in 32 bits: a wave for 16 columns of a head's state
+// ---- join_kernel: each piece's start from the one before it, in 32 bits: a wave for 16 columns of a head's state, and a wave more that
+// brings the pieces' maps to LDS, the next one while one is used. (Read from memory by the waves that use it a map took 35 us.)
 
 template <int DK>
-__global__ __launch_bounds__(BLOCK) void join_kernel(const float* __restrict__ state, Shape S, int pieces, Joins joins) {
-    constexpr int ND = DK / 16, KB = DK / 32;
-    const int l = threadIdx.x % WAVE, grp = l / 16, m = l % 16, groups = (S.vp / 16 + WAVES - 1) / WAVES;
+__global__ __launch_bounds__((WAVES + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))) void join_kernel(const float* __restrict__ state, Shape S, int pieces, Joins joins) {
+    constexpr int ND = DK / 16, KB = DK / 32, MAP = DK * DK * 4;
+    __shared__ alignas(1024) char lds[2 * MAP];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), l = threadIdx.x % WAVE, grp = l / 16, m = l % 16, groups = (S.vp / 16 + WAVES - 1) / WAVES;
     const int64_t bg = blockIdx.x / groups;
-    const int col = int(blockIdx.x % groups * WAVES + threadIdx.x / WAVE) * 16 + m;
-    if (col >= S.vp) return;               // (a whole wave)
-    f4 s[ND];
+    const int col = int(blockIdx.x % groups * WAVES + wave) * 16 + m;
+    const auto end_of = [&](int p) { return joins.ends + (bg * pieces + p) * (S.vp + DK) * DK; };
+    if (wave == WAVES) {
+        for (int p = 0; p + 1 < pieces; p++) {
+            bring<1>(end_of(p) + int64_t(S.vp) * DK, lds + p % 2 * MAP, MAP, 0);
+            arrived<0>();
+            __syncthreads();               // the map is there, and the one before has been used
+        }
+        return;
+    }
+    const bool on = col < S.vp;            // (a whole wave)
+    f4 s[ND], x[ND];
+    bool cut = false;
+    const auto fetch = [&](int p) {
+#pragma unroll
+        for (int n = 0; n < ND; n++) x[n] = on ? *reinterpret_cast<const f4*>(end_of(p) + int64_t(col) * DK + 16 * n + 4 * grp) : f4{0, 0, 0, 0};
+        cut = joins.cut[bg * pieces + p];
+    };
 #pragma unroll
     for (int n = 0; n < ND; n++)
 #pragma unroll
@@ -452,16 +469,13 @@ __global__ __launch_bounds__(BLOCK) void join_kernel(const float* __restrict__ s
             const int d = 16 * n + 4 * grp + r;
             s[n][r] = state && col < S.V && d < S.K ? state[(bg * S.K + d) * S.V + col] : 0.0f;
         }
+    fetch(0);
     for (int p = 0; p + 1 < pieces; p++) {
-        const int64_t piece = bg * pieces + p;
-        const float *end = joins.ends + piece * (S.vp + DK) * DK, *map = end + int64_t(S.vp) * DK;
-        const bool cut = joins.cut[piece];
-        f4 x[ND], z[ND];
+        __syncthreads();
+        const float* map = reinterpret_cast<const float*>(lds + p % 2 * MAP);
+        f4 z[ND];
 #pragma unroll
-        for (int n = 0; n < ND; n++) {
-            z[n] = f4{0, 0, 0, 0};
-            x[n] = *reinterpret_cast<const f4*>(end + int64_t(col) * DK + 16 * n + 4 * grp);
-        }
+        for (int n = 0; n < ND; n++) z[n] = f4{0, 0, 0, 0};
         if (!cut) {
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) {
@@ -473,12 +487,13 @@ __global__ __launch_bounds__(BLOCK) void join_kernel(const float* __restrict__ s
                 mma_all(z, a, frag_of<float, 1>(s[2 * kb], s[2 * kb + 1], 1.0f));
             }
         }
-        float* to = joins.starts + ((piece + 1) * S.vp + col) * DK + 4 * grp;
+        float* to = joins.starts + ((bg * pieces + p + 1) * S.vp + col) * DK + 4 * grp;
 #pragma unroll
         for (int n = 0; n < ND; n++) {
             s[n] = z[n] + x[n];
-            *reinterpret_cast<f4*>(to + 16 * n) = s[n];
+            if (on) *reinterpret_cast<f4*>(to + 16 * n) = s[n];
         }
+        if (p + 2 < pieces) fetch(p + 1);
     }
 }
 
@@ -588,7 +603,7 @@ int32_t forward(const void* query, const void* key, const void* value, const voi
         constexpr int W = 4;
         state_kernel<E, DK, W, false, true><<<dim3(heads * pieces.count * (((S.vp + DK) / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(
             in(value), nullptr, S, records, images, nullptr, nullptr, to, pieces, joins);
-        join_kernel<DK><<<dim3(heads * ((S.vp / 16 + WAVES - 1) / WAVES)), BLOCK, 0, stream>>>(state, S, pieces.count, joins);
+        join_kernel<DK><<<dim3(heads * ((S.vp / 16 + WAVES - 1) / WAVES)), (WAVES + 1) * WAVE, 0, stream>>>(state, S, pieces.count, joins);
     }
     return with_waves(S, pieces, [&](auto w) {
         constexpr int W = decltype(w)::value;
