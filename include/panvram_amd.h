@@ -422,7 +422,8 @@ int32_t pv_gated_delta_hip(const void* query, const void* key, const void* value
 
 /* Its gradients from d_out ([B, T, G, V] of `dtype`; strides: 9, of gate, write and d_out) and d_last (f32[B, G, K, V], or NULL: zero),
  * with kept and records, the forward call's work, as that call left them: d_query, d_key, d_value, d_gate, d_write like the tensors, of
- * `dtype` and without gaps, and d_state (f32[B, G, K, V], or NULL). work: pv_gated_delta_kept_bytes. */
+ * `dtype` and without gaps, and d_state (f32[B, G, K, V], or NULL). */
+uint64_t pv_gated_delta_backward_work_bytes(int64_t B, int64_t T, int32_t G, int32_t K, int32_t V, int32_t dtype);
 int32_t pv_gated_delta_backward_hip(const void* gate, const void* write, const void* d_out, const float* d_last, int64_t B, int64_t T, int32_t H, int32_t G, int32_t K,
                                     int32_t V, const int64_t* strides, int32_t dtype, const void* kept, const void* records, void* d_query, void* d_key, void* d_value,
                                     void* d_gate, void* d_write, float* d_state, void* work, uint64_t work_bytes, void* stream, char* err, size_t errcap);

@@ -110,6 +110,7 @@ SIGNATURES = {
     "pv_add_rms_norm_work_bytes": (u64, [i64, i64]),
     "pv_add_rms_norm_backward_hip": (i32, [vp, vp, vp, i64, i64, i64, vp, vp, i32, vp, vp, vp, u64, vp, cp, sz]),
     "pv_gated_delta_work_bytes": (u64, [i64, i64, i32, i32, i32, i32, i32, i32]),
+    "pv_gated_delta_backward_work_bytes": (u64, [i64, i64, i32, i32, i32, i32]),
     "pv_gated_delta_kept_bytes": (u64, [i64, i64, i32, i32, i32, i32]),
     "pv_gated_delta_hip": (i32, [vp, vp, vp, vp, vp, vp, vp, i64, i64, i32, i32, i32, i32, vp, f32, i32, vp, vp, vp, vp, u64, vp, cp, sz]),
     "pv_gated_delta_backward_hip": (i32, [vp, vp, vp, vp, i64, i64, i32, i32, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, u64, vp, cp, sz]),

@@ -213,8 +213,6 @@ template <typename S_, int ROWS, int COLS, int PARTS = 1> struct Tile {
         }
         return f;
     }
-    // the same of its first part alone
-    __device__ Frag<S, 1> rows_narrow(int r0, int kb) const { return Tile<S, ROWS, COLS, 1>{p}.rows(r0, kb); }
     // columns c0 .. c0 + 15, summed over rows 32 kb ..
     __device__ Frag<S, PARTS> cols(int c0, int kb) const {
         const int l = threadIdx.x % WAVE, g = l / 16, m = l % 16;
@@ -237,7 +235,6 @@ template <typename S_, int ROWS, int COLS, int PARTS = 1> struct Tile {
         }
         return f;
     }
-    __device__ Frag<S, 1> cols_narrow(int c0, int kb) const { return Tile<S, ROWS, COLS, 1>{p}.cols(c0, kb); }
     __device__ S get(int row, int c) const { return p[row * ROW + place(c)]; }
     // eight neighbouring columns of a row, c a multiple of 8
     __device__ void put(int row, int c, const S (&v)[8]) const {
@@ -502,6 +499,74 @@ struct Joins {
         : ends(static_cast<float*>(p)), starts(ends + heads * pieces * int64_t(vp + dk) * dk), cut(reinterpret_cast<uint32_t*>(starts + heads * pieces * int64_t(vp) * dk)) {}
     static uint64_t bytes(uint64_t heads, uint64_t pieces, uint64_t vp, uint64_t dk) { return heads * pieces * ((vp + dk) * dk + vp * dk + 1) * 4; }
 };
+
+constexpr int JOIN_WAVES = 4;
+
+// ---- join_kernel: each piece's start from the one before it, in 32 bits: a wave for 16 columns of a head's state, and a wave more that
+// brings the pieces' maps to LDS, the next one while one is used. (Read from memory by the waves that use it a map took 35 us.)
+
+// TURNED: backwards, each piece's end from the one after it, by the maps transposed; `ends` are of the gradient, `maps` still those of the state.
+template <int DK, bool TURNED>
+static __global__ __launch_bounds__((JOIN_WAVES + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))) void join_kernel(const float* __restrict__ state, Shape S, int pieces, Joins joins, Joins maps) {
+    constexpr int ND = DK / 16, KB = DK / 32, MAP = DK * DK * 4;
+    __shared__ alignas(1024) char lds[2 * MAP];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), l = threadIdx.x % WAVE, grp = l / 16, m = l % 16, groups = (S.vp / 16 + JOIN_WAVES - 1) / JOIN_WAVES;
+    const int64_t bg = blockIdx.x / groups;
+    const int col = int(blockIdx.x % groups * JOIN_WAVES + wave) * 16 + m;
+    const auto piece_of = [&](int p) { return bg * pieces + (TURNED ? pieces - 1 - p : p); };
+    if (wave == JOIN_WAVES) {
+        for (int p = 0; p + 1 < pieces; p++) {
+            bring<1>(maps.ends + (piece_of(p) * (S.vp + DK) + S.vp) * DK, lds + p % 2 * MAP, MAP, 0);
+            arrived<0>();
+            __syncthreads();               // the map is there, and the one before has been used
+        }
+        return;
+    }
+    const bool on = col < S.vp;            // (a whole wave)
+    f4 s[ND], x[ND];
+    bool cut = false;
+    const auto fetch = [&](int p) {
+#pragma unroll
+        for (int n = 0; n < ND; n++) x[n] = on ? *reinterpret_cast<const f4*>(joins.ends + (piece_of(p) * (S.vp + DK) + col) * DK + 16 * n + 4 * grp) : f4{0, 0, 0, 0};
+        cut = maps.cut[piece_of(p)];
+    };
+#pragma unroll
+    for (int n = 0; n < ND; n++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int d = 16 * n + 4 * grp + r;
+            s[n][r] = state && col < S.V && d < S.K ? state[(bg * S.K + d) * S.V + col] : 0.0f;
+        }
+    fetch(0);
+    for (int p = 0; p + 1 < pieces; p++) {
+        __syncthreads();
+        const float* map = reinterpret_cast<const float*>(lds + p % 2 * MAP);
+        f4 z[ND];
+#pragma unroll
+        for (int n = 0; n < ND; n++) z[n] = f4{0, 0, 0, 0};
+        if (!cut) {
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) {
+                Frag<float, 1> a[ND];
+#pragma unroll
+                for (int n = 0; n < ND; n++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int d = 32 * kb + 4 * grp + j % 4 + j / 4 * 16;
+                        a[n].v[j] = TURNED ? map[(16 * n + m) * DK + d] : map[d * DK + 16 * n + m];
+                    }
+                mma_all(z, a, frag_of<float, 1>(s[2 * kb], s[2 * kb + 1], 1.0f));
+            }
+        }
+        float* to = joins.starts + (piece_of(p + 1) * S.vp + col) * DK + 4 * grp;
+#pragma unroll
+        for (int n = 0; n < ND; n++) {
+            s[n] = z[n] + x[n];
+            if (on) *reinterpret_cast<f4*>(to + 16 * n) = s[n];
+        }
+        if (p + 2 < pieces) fetch(p + 1);
+    }
+}
 
 // f of the waves of a workgroup that walks over chunks: four of them, 64 columns, where that makes workgroups for all CUs, else two (64
 // heads of 128 columns, 8,192 steps: 0.51 ms with two, 0.57 with four; a CU gets through a chunk of 64 columns in 4.5 us, of 32 in 3.9)

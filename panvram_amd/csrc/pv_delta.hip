@@ -306,6 +306,21 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
         for (int it = 0; it < 4; it++) v[it] = vp.four(it);
         any |= cuts;
+        bool lost = false;                 // the state before a chunk in which some step drops it is not finite
+        by_cut(cuts, [&](auto cut) {
+            if constexpr (decltype(cut)::value) {      // (zero times it would reach the steps that it is dropped at: it is zero, and the steps before are NaN)
+                float x = 0.0f;
+#pragma unroll
+                for (int k = 0; k < ND; k++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) x = fmaf(0.0f, s[k][r], x);
+                lost = over_column(x == 0.0f ? 0.0f : 1.0f) != 0.0f;
+#pragma unroll
+                for (int k = 0; k < ND; k++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) s[k][r] = lost ? 0.0f : s[k][r];
+            }
+        });
         if (n + 1 < behind) vp.load(rows_at(v0 + (n + 1) * C * S.vt, S.vt, rows_of(n + 1), S.V), S.vt, value_at);
         const int64_t at = (bg * S.chunks + n) * S.vp;     // of the chunk in what is kept
         const Buffer blocks(kept.blocks + at / COLS * Ke::BLOCK, KEEP ? int64_t(S.vp / COLS) * Ke::BLOCK * int(sizeof(St)) : 0);
@@ -408,7 +423,11 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
                 for (int r = 0; r < 4; r++) s[k][r] = fmaf(dl, z[k][r], part_of_it<CUT>(end, s[k][r]));
 #pragma unroll
-            for (int it = 0; it < 4; it++) if constexpr (!MAP) y[it] = part_of_it<CUT>(four(st.q, it) * ss.down, y[it]);
+            for (int it = 0; it < 4; it++) if constexpr (!MAP) {
+                y[it] = part_of_it<CUT>(four(st.q, it) * ss.down, y[it]);
+#pragma unroll
+                for (int r = 0; r < 4; r++) if (CUT && lost && 16 * it + 4 * grp + r < __builtin_ctzll(cuts)) y[it][r] = NAN;
+            }
         });
         if constexpr (MAP) continue;
         const Buffer to = rows_at(out + ((b * S.T + n * C) * S.G + g) * S.V, ot, rows_of(n), S.V);
@@ -432,68 +451,6 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
             for (int n = 0; n < ND; n++) *reinterpret_cast<f4*>(to + 16 * n) = s[n];
         }
         if (group == 0 && tid == 0) joins.cut[piece] = any != 0;
-    }
-}
-
-// ---- join_kernel: each piece's start from the one before it, in 32 bits: a wave for 16 columns of a head's state, and a wave more that
-// brings the pieces' maps to LDS, the next one while one is used. (Read from memory by the waves that use it a map took 35 us.)
-
-template <int DK>
-__global__ __launch_bounds__((WAVES + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))) void join_kernel(const float* __restrict__ state, Shape S, int pieces, Joins joins) {
-    constexpr int ND = DK / 16, KB = DK / 32, MAP = DK * DK * 4;
-    __shared__ alignas(1024) char lds[2 * MAP];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), l = threadIdx.x % WAVE, grp = l / 16, m = l % 16, groups = (S.vp / 16 + WAVES - 1) / WAVES;
-    const int64_t bg = blockIdx.x / groups;
-    const int col = int(blockIdx.x % groups * WAVES + wave) * 16 + m;
-    const auto end_of = [&](int p) { return joins.ends + (bg * pieces + p) * (S.vp + DK) * DK; };
-    if (wave == WAVES) {
-        for (int p = 0; p + 1 < pieces; p++) {
-            bring<1>(end_of(p) + int64_t(S.vp) * DK, lds + p % 2 * MAP, MAP, 0);
-            arrived<0>();
-            __syncthreads();               // the map is there, and the one before has been used
-        }
-        return;
-    }
-    const bool on = col < S.vp;            // (a whole wave)
-    f4 s[ND], x[ND];
-    bool cut = false;
-    const auto fetch = [&](int p) {
-#pragma unroll
-        for (int n = 0; n < ND; n++) x[n] = on ? *reinterpret_cast<const f4*>(end_of(p) + int64_t(col) * DK + 16 * n + 4 * grp) : f4{0, 0, 0, 0};
-        cut = joins.cut[bg * pieces + p];
-    };
-#pragma unroll
-    for (int n = 0; n < ND; n++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int d = 16 * n + 4 * grp + r;
-            s[n][r] = state && col < S.V && d < S.K ? state[(bg * S.K + d) * S.V + col] : 0.0f;
-        }
-    fetch(0);
-    for (int p = 0; p + 1 < pieces; p++) {
-        __syncthreads();
-        const float* map = reinterpret_cast<const float*>(lds + p % 2 * MAP);
-        f4 z[ND];
-#pragma unroll
-        for (int n = 0; n < ND; n++) z[n] = f4{0, 0, 0, 0};
-        if (!cut) {
-#pragma unroll
-            for (int kb = 0; kb < KB; kb++) {
-                Frag<float, 1> a[ND];
-#pragma unroll
-                for (int n = 0; n < ND; n++)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) a[n].v[j] = map[(32 * kb + 4 * grp + j % 4 + j / 4 * 16) * DK + 16 * n + m];
-                mma_all(z, a, frag_of<float, 1>(s[2 * kb], s[2 * kb + 1], 1.0f));
-            }
-        }
-        float* to = joins.starts + ((bg * pieces + p + 1) * S.vp + col) * DK + 4 * grp;
-#pragma unroll
-        for (int n = 0; n < ND; n++) {
-            s[n] = z[n] + x[n];
-            if (on) *reinterpret_cast<f4*>(to + 16 * n) = s[n];
-        }
-        if (p + 2 < pieces) fetch(p + 1);
     }
 }
 
@@ -603,7 +560,7 @@ int32_t forward(const void* query, const void* key, const void* value, const voi
         constexpr int W = 4;
         state_kernel<E, DK, W, false, true><<<dim3(heads * pieces.count * (((S.vp + DK) / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(
             in(value), nullptr, S, records, images, nullptr, nullptr, to, pieces, joins);
-        join_kernel<DK><<<dim3(heads * ((S.vp / 16 + WAVES - 1) / WAVES)), (WAVES + 1) * WAVE, 0, stream>>>(state, S, pieces.count, joins);
+        join_kernel<DK, false><<<dim3(heads * ((S.vp / 16 + JOIN_WAVES - 1) / JOIN_WAVES)), (JOIN_WAVES + 1) * WAVE, 0, stream>>>(state, S, pieces.count, joins, joins);
     }
     return with_waves(S, pieces, [&](auto w) {
         constexpr int W = decltype(w)::value;
@@ -630,6 +587,14 @@ uint64_t pv_gated_delta_work_bytes(int64_t B, int64_t T, int32_t H, int32_t G, i
 uint64_t pv_gated_delta_kept_bytes(int64_t B, int64_t T, int32_t G, int32_t K, int32_t V, int32_t dtype) {
     if (B < 1 || G < 1 || T < 1 || K < 1 || V < 1) return 0;
     return kept_bytes(uint64_t(B) * uint64_t(G) * uint64_t((T + C - 1) / C), (V + 31) / 32 * 32, columns_of(K), dtype);
+}
+
+uint64_t pv_gated_delta_backward_work_bytes(int64_t B, int64_t T, int32_t G, int32_t K, int32_t V, int32_t dtype) {
+    const uint64_t kept = pv_gated_delta_kept_bytes(B, T, G, K, V, dtype);
+    if (!kept) return 0;
+    const int32_t vp = (V + 31) / 32 * 32, dk = columns_of(K);
+    const Pieces pieces = pieces_of(B * G, (T + C - 1) / C, vp, dk);
+    return kept + (pieces.count > 1 ? Joins::bytes(B * G, pieces.count, vp, dk) : 0);
 }
 
 int32_t pv_gated_delta_hip(const void* query, const void* key, const void* value, const void* gate, const void* write, const float* state, const uint8_t* reset,

@@ -19,10 +19,11 @@ namespace {
 
 // ---- walk_kernel: a workgroup of W waves for 16 W columns of a state's gradient, and a wave more that brings chunks to LDS
 
-template <typename E, int DK, int W>
+// MAP: the first walk of a sequence in pieces, each from a gradient of zero behind it; nothing is left but the gradient before it.
+template <typename E, int DK, int W, bool MAP>
 __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))) void walk_kernel(
     const E* __restrict__ d_out, const float* __restrict__ d_last, Shape S, const char* __restrict__ records, const char* __restrict__ images, E* __restrict__ d_value,
-    float* __restrict__ d_state, Kept<typename Rep<E>::S, DK> walked) {
+    float* __restrict__ d_state, Kept<typename Rep<E>::S, DK> walked, Pieces pieces, Joins joins) {
     using St = typename Rep<E>::S;
     using Ke = Kept<St, DK>;
     constexpr int WIDE = wide_of<St>, ND = DK / 16, KB = DK / 32;
@@ -33,9 +34,10 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
     __shared__ alignas(1024) char lds[BUFFERS * BUFFER];
     const int tid = threadIdx.x, wave = tid / WAVE, l = tid % WAVE, grp = l / 16, m = l % 16;
     const int groups = (S.vp / 16 + W - 1) / W;
-    const auto [bg, group] = part_of(blockIdx.x, S.B * S.G, groups);
+    const auto [piece, group] = part_of(blockIdx.x, S.B * S.G * pieces.count, groups);
     const int col = (group * W + wave) * 16 + m;
-    const int64_t b = bg / S.G;
+    const int64_t bg = piece / pieces.count, b = bg / S.G, first = piece % pieces.count * pieces.chunks;
+    const int64_t behind = first + pieces.chunks < S.chunks ? first + pieces.chunks : S.chunks;
     const int g = int(bg % S.G), h = shared(S, g);
     const bool on = col < S.V;
     const E* o0 = d_out + b * S.ob + g * S.og;
@@ -50,12 +52,14 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int d = 16 * n + 4 * grp + r;
-            s[n][r] = d_last && on && d < S.K ? d_last[(bg * S.K + d) * S.V + col] : 0.0f;
+            if constexpr (MAP) s[n][r] = 0.0f;
+            else if (behind < S.chunks) s[n][r] = col < S.vp ? joins.starts[(piece * S.vp + col) * DK + d] : 0.0f;
+            else s[n][r] = d_last && on && d < S.K ? d_last[(bg * S.K + d) * S.V + col] : 0.0f;
         }
     const auto rows_of = [&](int64_t n) { return int(S.T - n * C < C ? S.T - n * C : C); };
     if (wave == W) {
-        for (int64_t n = S.chunks - 1; n >= 0; n--) {
-            if (n < S.chunks - 1 && BUFFERS == 1) __syncthreads();     // the chunk after has been used
+        for (int64_t n = behind - 1; n >= first; n--) {
+            if (n < behind - 1 && BUFFERS == 1) __syncthreads();       // the chunk after has been used
             char* to = lds + (BUFFERS == 2 ? int(n & 1) * BUFFER : 0);
             bring<1>(in0 + n * IN, to, 2 * In::SIZE * int(sizeof(St)), 0);
             bring<1>(rec0 + n * Re::STRIDE, to + IN, Re::ALL, 0);
@@ -65,9 +69,9 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         return;
     }
     Sixteen<E> op;
-    op.load(rows_at(o0 + (S.chunks - 1) * C * S.ot, S.ot, rows_of(S.chunks - 1), S.V), S.ot, out_at);
-    for (int64_t n = S.chunks - 1; n >= 0; n--) {
-        if (n < S.chunks - 1 && BUFFERS == 1) __syncthreads();
+    op.load(rows_at(o0 + (behind - 1) * C * S.ot, S.ot, rows_of(behind - 1), S.V), S.ot, out_at);
+    for (int64_t n = behind - 1; n >= first; n--) {
+        if (n < behind - 1 && BUFFERS == 1) __syncthreads();
         __syncthreads();
         char* here = lds + (BUFFERS == 2 ? int(n & 1) * BUFFER : 0);
         const In Kt{reinterpret_cast<St*>(here)}, Qt{reinterpret_cast<St*>(here) + In::SIZE};
@@ -80,7 +84,7 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         f4 o[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) o[it] = op.four(it);
-        if (n) op.load(rows_at(o0 + (n - 1) * C * S.ot, S.ot, rows_of(n - 1), S.V), S.ot, out_at);
+        if (n > first) op.load(rows_at(o0 + (n - 1) * C * S.ot, S.ot, rows_of(n - 1), S.V), S.ot, out_at);
         const int64_t at = (bg * S.chunks + n) * S.vp;     // of the chunk in what is left over
         const Buffer blocks(walked.blocks + at / COLS * Ke::BLOCK, int64_t(S.vp / COLS) * Ke::BLOCK * int(sizeof(St)));
         // operands of a stage's products are loaded while the stage before runs
@@ -101,7 +105,7 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
         for (int kb = 0; kb < KB; kb++) {
             sf[kb] = frag_of<St, WIDE>(s[2 * kb], s[2 * kb + 1], ss.up);
-            leave(blocks, state_at + 32 * kb * sizeof(St), sf[kb]);
+            if constexpr (!MAP) leave(blocks, state_at + 32 * kb * sizeof(St), sf[kb]);
         }
         // dU = l K dS + P^T dO
         const float dp = os.down * (1.0f / SQUARE<St>);
@@ -150,22 +154,24 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
             x[it] = four(st.q, it) * o[it];
             y[it] = four(st.x, it) * d[it] * -du;
 #pragma unroll
-            for (int r = 0; r < 4; r++) Sixteen<E>::store(to, vt, value_at, 4 * it + r, bs[r] * d[it][r]);
+            for (int r = 0; r < 4; r++) if constexpr (!MAP) Sixteen<E>::store(to, vt, value_at, 4 * it + r, bs[r] * d[it][r]);
         }
         // (q and x are 2 / LONG at most)
         const Scale xs = scale_of<St>(over_column(fmaxf(largest(x), largest(y))));
         Frag<St, WIDE> xf[2], yf[2];
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
-            leave(blocks, step_at + 32 * kb * sizeof(St), frag_of<St, 1>(d[2 * kb], d[2 * kb + 1], sizeof(St) == 2 ? du * ds.up : 1.0f));
+            if constexpr (!MAP) leave(blocks, step_at + 32 * kb * sizeof(St), frag_of<St, 1>(d[2 * kb], d[2 * kb + 1], sizeof(St) == 2 ? du * ds.up : 1.0f));
             xf[kb] = frag_of<St, WIDE>(x[2 * kb], x[2 * kb + 1], xs.up);
             yf[kb] = frag_of<St, WIDE>(y[2 * kb], y[2 * kb + 1], xs.up);
         }
         const Buffer scales(walked.scales + 3 * at, 3 * int64_t(S.vp) * 4);
         const uint32_t scale_at = grp == 0 && col < S.vp ? col * 4 : NOWHERE;
-        scales.store(ss.down, scale_at);
-        scales.store(ds.down, scale_at, S.vp * 4);
-        scales.store(os.down, scale_at, 2 * S.vp * 4);
+        if constexpr (!MAP) {
+            scales.store(ss.down, scale_at);
+            scales.store(ds.down, scale_at, S.vp * 4);
+            scales.store(os.down, scale_at, 2 * S.vp * 4);
+        }
         fence();
         const float end = st.end;
         f4 z[ND];
@@ -182,7 +188,15 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
                 for (int r = 0; r < 4; r++) s[k][r] = fmaf(xs.down, z[k][r], part_of_it<decltype(cut)::value>(end, s[k][r]));
         });
     }
-    if (!d_state) return;
+    if constexpr (MAP) {
+        if (col < S.vp) {
+            float* to = joins.ends + (piece * (S.vp + DK) + col) * DK + 4 * grp;
+#pragma unroll
+            for (int n = 0; n < ND; n++) *reinterpret_cast<f4*>(to + 16 * n) = s[n];
+        }
+        return;
+    }
+    if (!d_state || first) return;
 #pragma unroll
     for (int n = 0; n < ND; n++)
 #pragma unroll
@@ -599,9 +613,19 @@ int32_t backward(const void* gate, const void* write, const void* d_out, const f
     const int64_t heads = S.B * S.G;
     const char *rec = static_cast<const char*>(records), *images = rec + heads * S.chunks * Record<St>::STRIDE;
     const Kept<St, DK> before(kept, S), walked(work, S);
-    with_waves(S, Pieces{1, S.chunks}, [&](auto w) {
+    const Pieces pieces = pieces_of(heads, S.chunks, S.vp, DK);
+    const Joins maps(const_cast<char*>(images) + S.B * S.H * S.chunks * IMAGE<St, DK>, heads, pieces.count, S.vp, DK);
+    const Joins joins(walked.scales + heads * S.chunks * 3 * S.vp, heads, pieces.count, S.vp, DK);
+    if (pieces.count > 1) {
+        constexpr int W = 4;
+        walk_kernel<E, DK, W, true><<<dim3(heads * pieces.count * ((S.vp / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(in(d_out), nullptr, S, rec, images, nullptr,
+                                                                                                                      nullptr, walked, pieces, joins);
+        join_kernel<DK, true><<<dim3(heads * ((S.vp / 16 + JOIN_WAVES - 1) / JOIN_WAVES)), (JOIN_WAVES + 1) * WAVE, 0, stream>>>(d_last, S, pieces.count, joins, maps);
+    }
+    with_waves(S, pieces, [&](auto w) {
         constexpr int W = decltype(w)::value;
-        walk_kernel<E, DK, W><<<dim3(heads * ((S.vp / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(in(d_out), d_last, S, rec, images, out(d_value), d_state, walked);
+        walk_kernel<E, DK, W, false><<<dim3(heads * pieces.count * ((S.vp / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(in(d_out), d_last, S, rec, images, out(d_value),
+                                                                                                                       d_state, walked, pieces, joins);
         return 0;
     });
     gradient_kernel<E, DK><<<dim3(S.B * S.H * S.chunks), MANY, 0, stream>>>(in(gate), in(write), in(d_out), S, rec, images, before, walked, out(d_query), out(d_key),
@@ -619,7 +643,7 @@ extern "C" int32_t pv_gated_delta_backward_hip(const void* gate, const void* wri
     if (int32_t e = shape_of(B, T, H, G, K, V, strides, 9, 0.0f, dtype, S, err, errcap)) return e;
     if (!gate || !write || !d_out || !kept || !records || !d_query || !d_key || !d_value || !d_gate || !d_write) return fail(PV_EARG, err, errcap, "null argument");
     if (!aligned(kept, 16) || !aligned(records, 16)) return fail(PV_EARG, err, errcap, "kept, records: not 16-byte aligned");
-    const uint64_t need = pv_gated_delta_kept_bytes(B, T, G, K, V, dtype);
+    const uint64_t need = pv_gated_delta_backward_work_bytes(B, T, G, K, V, dtype);
     if (!work || work_bytes < need || !aligned(work, 16)) return fail(PV_EARG, err, errcap, "work: too small, or not 16-byte aligned");
     return with_type(dtype, [&](auto e) {
         using E = decltype(e);

@@ -55,7 +55,7 @@ class _GatedDelta(torch.autograd.Function):
         d_query, d_key, d_value, d_gate, d_write = (torch.empty(s, dtype=dtype, device=dev) for s in ((B, T, H, K), (B, T, H, K), (B, T, G, V), (B, T, G), (B, T, G)))
         d_state = torch.empty((B, G, K, V), dtype=torch.float32, device=dev) if ctx.has_state else None
         L, code = N.lib(), DTYPES[dtype]
-        size = L.pv_gated_delta_kept_bytes(B, T, G, K, V, code)
+        size = L.pv_gated_delta_backward_work_bytes(B, T, G, K, V, code)
         work = torch.empty(size, dtype=torch.uint8, device=dev)
         gate, write = _strided(gate), _strided(write)
         call(L.pv_gated_delta_backward_hip, gate.get_device(), gate.data_ptr(), write.data_ptr(), d_out.data_ptr(), ptr(d_last), B, T, H, G, K, V,
@@ -94,6 +94,8 @@ def gated_delta(query, key, value, gate, write, state=None, reset=None, eps=1e-6
     G, V = value.shape[2:]
     if not 1 <= K <= 128 or not 1 <= V <= 1 << 16:
         raise ValueError(f"gated_delta: keys have 1 to 128 elements and values 1 to 65,536, got {K} and {V}")
+    if G * V > 1 << 22 or H * K > 1 << 22:
+        raise ValueError(f"gated_delta: a step's values, and its keys, are 2^22 at most, got {G} x {V} and {H} x {K}")
     if gate.shape != (B, T, G) or write.shape != (B, T, G):
         raise ValueError(f"gated_delta: gate and write are {[B, T, G]}, got {list(gate.shape)} and {list(write.shape)}")
     if not eps >= 0:

@@ -88,16 +88,22 @@ def test_resets(dtype, share):
     compare(a | {"state": None}, d_out)
 
 
-@pytest.mark.parametrize("T", [1, 5, 70])
-def test_reset_drops_what_there_was(T):
-    """A state that is not finite, under a reset at the first step; and nothing before a reset matters behind it."""
+@pytest.mark.parametrize("T, at", [(1, 0), (5, 0), (5, 3), (70, 0), (70, 1), (70, 40), (70, 64), (200, 130)])
+def test_reset_drops_what_there_was(T, at):
+    """A state that is not finite, under a reset at the first step or later: nothing before a reset matters behind it."""
     a, _, _ = made(2, T, 1, 1, 16, 24, torch.bfloat16)
     a["reset"] = torch.zeros(2, T, dtype=torch.bool, device="cuda")
-    a["reset"][:, 0] = True
+    a["reset"][:, at] = True
     want = ops.gated_delta(**(a | {"state": None}))
-    for fill in (float("nan"), float("inf"), 3e38):
+    for fill in (float("nan"), float("inf"), -float("inf")):
         got = ops.gated_delta(**(a | {"state": torch.full_like(a["state"], fill)}))
-        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert torch.equal(got[0][:, at:], want[0][:, at:]) and torch.equal(got[1], want[1])
+        assert not torch.isfinite(got[0][:, :at]).any()
+    one = a["state"].clone()                                    # one column of it, and one element
+    one[0, 0, 3, 5] = float("nan")
+    got = ops.gated_delta(**(a | {"state": one}))
+    assert torch.equal(got[0][:, at:], want[0][:, at:]) and torch.equal(got[1], want[1])
+    assert torch.isnan(got[0][0, :at, 0, 5]).all() and torch.isfinite(got[0][:, :at, :, :5]).all()
 
 
 def test_packed_windows():
@@ -323,7 +329,72 @@ def test_past_32_bit_offsets():
     reset = torch.zeros(1, T, dtype=torch.bool, device="cuda")
     reset[:, T - 164] = True                    # the first step of a chunk
     assert (T - 164) % 64 == 0
+    # The window has its reset by itself too. Without one its sums of log(keep) begin with log(keep[0]), not with 0; the differences of
+    # two sums are those numbers again but rounded otherwise, 2^-24 of them, so that now and then an output is rounded the other way.
     with torch.no_grad():
         out, last = ops.gated_delta(**a, reset=reset)
-        o, s = ops.gated_delta(**{k: t[:, T - 164:] for k, t in a.items()})
+        o, s = ops.gated_delta(**{k: t[:, T - 164:] for k, t in a.items()}, reset=reset[:, T - 164:])
     assert torch.equal(out[:, T - 164:], o) and torch.equal(last, s)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T, H, G, K, V, reset", [(2048, 1, 1, 12, 10, None), (2113, 1, 2, 9, 40, 0.002), (3000, 1, 1, 33, 8, None)])
+def test_in_pieces(dtype, T, H, G, K, V, reset):
+    """Long sequences of few heads, which are walked in pieces: their starts, ends and gradients"""
+    a, d_out, d_last = made(1, T, H, G, K, V, dtype, seed=T, reset=reset, keep=-6.0)
+    compare(a, d_out, d_last)
+
+
+@pytest.mark.parametrize("at", [0, 1000, 2047])
+def test_reset_in_a_piece(at):
+    """A state that is not finite, dropped somewhere in a long sequence, reaches nothing from there on."""
+    a, _, _ = made(1, 2100, 1, 1, 16, 24, torch.bfloat16)
+    a["reset"] = torch.zeros(1, 2100, dtype=torch.bool, device="cuda")
+    a["reset"][:, at] = True
+    want = ops.gated_delta(**(a | {"state": None}))
+    got = ops.gated_delta(**(a | {"state": torch.full_like(a["state"], float("nan"))}))
+    assert torch.equal(got[0][:, at:], want[0][:, at:]) and torch.equal(got[1], want[1])
+    if at > 64:
+        assert torch.isnan(got[0][:, :at]).all()
+
+
+def test_pieces_captured():
+    a, d_out, _ = made(1, 2200, 1, 2, 16, 24, torch.bfloat16)
+    a = {k: t.detach().requires_grad_() if k in NAMES else t for k, t in a.items()}
+
+    def both():
+        out, last = ops.gated_delta(**a)
+        return (out.detach(), last.detach(), *torch.autograd.grad(out, [a[k] for k in NAMES], d_out))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both()
+    for k in range(3):
+        with torch.no_grad():
+            a["value"].copy_(torch.randn_like(a["value"]))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, both()))
+
+
+@pytest.mark.parametrize("T, H, G, K, V", [(1, 2, 2, 24, 40), (200, 1, 2, 24, 40), (2113, 1, 1, 17, 9)])
+def test_memory_that_held_something(T, H, G, K, V):
+    """Workspaces and records that lie where NaN lay: nothing is read before it is written."""
+    a, d_out, d_last = made(2, T, H, G, K, V, torch.bfloat16)
+    leaves = [a[k].requires_grad_() for k in NAMES]
+
+    def run():
+        got = ops.gated_delta(**a)
+        with torch.no_grad():
+            alone = ops.gated_delta(**a)
+        return [*(t.clone() for t in (*got, *alone)), *torch.autograd.grad(got, leaves, (d_out, d_last))]
+
+    first = run()
+    held = [torch.full((size,), float("nan"), device="cuda") for size in [1 << 22] * 8 + [1 << 16] * 64 + [1 << 10] * 64]
+    del held
+    for x, y in zip(first, run()):
+        assert torch.isfinite(x).all() and torch.equal(x, y)
