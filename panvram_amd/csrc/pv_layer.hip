@@ -398,11 +398,10 @@ int32_t pv_add_layer_norm_backward_hip(const void* s, const float* stats, const 
                                                                                                    weight, N, D, s_row, static_cast<const E*>(d_y),
                                                                                                    static_cast<const E*>(d_stream), drop, static_cast<E*>(d),
                                                                                                    static_cast<E*>(d_x), parts_w, parts_b);
-                constexpr int64_t MOST = MOST_ITEMS / END_WAVES / 2;               // columns of a launch
+                constexpr int64_t MOST = MOST_ITEMS / END_WAVES / 4;               // columns of a launch
                 for (int64_t i = 0; g != 1 && i < D; i += MOST) {
-                    const dim3 grid((std::min(D - i, MOST) + WAVE - 1) / WAVE);
-                    norm_weight_kernel<<<grid, END_WAVES * WAVE, 0, st>>>(parts_w, g, D, i, d_weight);
-                    norm_weight_kernel<<<grid, END_WAVES * WAVE, 0, st>>>(parts_b, g, D, i, d_bias);
+                    const dim3 grid((std::min(D - i, MOST) + WAVE - 1) / WAVE, 2);
+                    norm_weight_kernel<<<grid, END_WAVES * WAVE, 0, st>>>(parts_w, g, D, i, d_weight, d_bias);
                 }
                 return launched(err, errcap);
             });

@@ -383,7 +383,7 @@ int32_t pv_add_rms_norm_backward_hip(const void* s, const float* rstd, const flo
                                                                         static_cast<const E*>(d_stream), static_cast<E*>(d), parts);
             constexpr int64_t MOST = MOST_ITEMS / END_WAVES / 2;               // columns of a launch
             for (int64_t i = 0; g != 1 && i < D; i += MOST)
-                norm_weight_kernel<<<dim3((std::min(D - i, MOST) + WAVE - 1) / WAVE), END_WAVES * WAVE, 0, st>>>(parts, g, D, i, d_weight);
+                norm_weight_kernel<<<dim3((std::min(D - i, MOST) + WAVE - 1) / WAVE), END_WAVES * WAVE, 0, st>>>(parts, g, D, i, d_weight, nullptr);
             return launched(err, errcap);
         });
     });

@@ -44,13 +44,16 @@ template <bool ONCE, typename T, int P> __device__ inline void leave(const pack<
     else v.store(row + i);
 }
 
-// d_weight[i] = sum of the partial rows, from column `first` on: 64 columns a workgroup, its 16 waves a run of rows each
+// d_weight[i] = sum of the partial rows, from column `first` on: 64 columns a workgroup, its 16 waves a run of rows each. The grid's
+// second row does the same for d_second, whose partial rows lie behind.
 constexpr int END_WAVES = 16;
-static __global__ __launch_bounds__(END_WAVES* WAVE) void norm_weight_kernel(const float* __restrict__ parts, int64_t rows, int64_t D, int64_t first, float* __restrict__ d_weight) {
+static __global__ __launch_bounds__(END_WAVES* WAVE) void norm_weight_kernel(const float* __restrict__ parts, int64_t rows, int64_t D, int64_t first, float* __restrict__ d_weight,
+                                                                           float* __restrict__ d_second) {
     __shared__ float lds[END_WAVES][WAVE];
     const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
     const int64_t i = first + int64_t(blockIdx.x) * WAVE + lane;
     float sum = 0.0f;
+    parts += blockIdx.y * rows * D;
     if (i < D) {
 #pragma unroll 8
         for (int64_t k = wave; k < rows; k += END_WAVES) sum += parts[k * D + i];
@@ -60,7 +63,7 @@ static __global__ __launch_bounds__(END_WAVES* WAVE) void norm_weight_kernel(con
     if (wave || i >= D) return;
 #pragma unroll
     for (int w = 1; w < END_WAVES; w++) sum += lds[w][lane];
-    d_weight[i] = sum;
+    (blockIdx.y ? d_second : d_weight)[i] = sum;
 }
 
 inline int64_t groups_of(int64_t N, int rows) { const int64_t g = (N + rows - 1) / rows; return g < PARTS ? g : PARTS; }

@@ -51,12 +51,11 @@ class _AddLayerNorm(torch.autograd.Function):
         d_stream = d_stream.contiguous() if d_stream is not None else None
         d = torch.empty(s.shape, dtype=dtype, device=dev)
         d_x = torch.empty(s.shape, dtype=dtype, device=dev) if p else None
-        d_both = torch.empty((2, D), dtype=torch.float32, device=dev)
+        d_weight, d_bias = torch.empty(D, dtype=torch.float32, device=dev), torch.empty(D, dtype=torch.float32, device=dev)
         L = N.lib()
         size = L.pv_add_layer_norm_work_bytes(count, D)
         work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         flat, ss = _flat(s)
-        d_weight, d_bias = d_both.unbind()
         call(L.pv_add_layer_norm_backward_hip, s.get_device(), flat.data_ptr(), stats.data_ptr(), weight.data_ptr(), count, D, ss, d_y.data_ptr(), ptr(d_stream), p,
              ptr(at), seed, site, DTYPES[dtype], d.data_ptr(), ptr(d_x), d_weight.data_ptr(), d_bias.data_ptr(), ptr(work), size)
         return d if d_x is None else d_x, None if ctx.alone else d, d_weight, d_bias if ctx.biased else None, None, None, None, None, None
