@@ -105,6 +105,7 @@ template <typename S> __device__ inline float decay(float x) {
 __device__ inline int thread() {
     int id = threadIdx.x;
     asm volatile("" : "+v"(id));
+    __builtin_assume(id >= 0 && id < 1024);
     return id;
 }
 

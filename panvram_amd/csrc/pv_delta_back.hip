@@ -240,17 +240,19 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
     __shared__ alignas(16) St factors[2][PRODUCTS][COLS];
     __shared__ float rows[HALVES][C], columns[BANDS][C], left[HALVES][C], whole[WAVES], writes[C], dots[2][HALVES][C];
     __shared__ int tops[WAVES][PRODUCTS];
+    __shared__ double gates[2][C];
     const In Kt{reinterpret_cast<St*>(lds)}, Qt{reinterpret_cast<St*>(lds) + In::SIZE};
     St* const more = reinterpret_cast<St*>(lds + IN);
     const Square Ek{more}, Eq{more + Square::SIZE}, Ff{more + 2 * Square::SIZE};       // (once the blocks of values have been used)
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), half = wave / BANDS, own = wave % BANDS, band = 16 * own, d0 = half * DK / 2;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), half = wave / BANDS,
+              own = half ? BANDS - 1 - wave % BANDS : wave % BANDS,    // (the two of a SIMD have near as much up to the diagonal as any other two)
+              band = 16 * own, d0 = half * DK / 2;
     const int64_t chunk = blockIdx.x % S.chunks, bh = blockIdx.x / S.chunks;
     const int64_t b = bh / S.H, t0 = chunk * C;
     const int h = int(bh % S.H), share = S.G / S.H, steps = int(S.T - t0 < C ? S.T - t0 : C);
     // products of E and F with keys and queries, over numbers of values each
     const int many = HALF ? 32 - __builtin_clz(S.V) : 0;
     const float few = __uint_as_float((127 - many) << 23);
-    bring<WAVES>(images + (bh * S.chunks + chunk) * IN, lds, 2 * In::SIZE * int(sizeof(St)));
     const f4 zero = {0, 0, 0, 0};
     f4 tq[ND], tk[ND];                     // the gradients of the query and the key of length 1, over the value heads so far
 #pragma unroll
@@ -262,19 +264,25 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
         const E* o0 = d_out + b * S.ob + t0 * S.ot + g * S.og;
         const St *b0 = kept.blocks + at * (S.vp / COLS) * Ke::BLOCK, *b1 = walked.blocks + at * (S.vp / COLS) * Ke::BLOCK;
         const float *f0 = kept.scales + at * 3 * S.vp, *f1 = walked.scales + at * 3 * S.vp;    // of S, U and of dS, dR, dO
-        const auto left_scale = [&](int p) { return p == 2 ? f0 + S.vp : p == 0 || p == 3 ? f1 + 2 * S.vp : f1 + S.vp; };
-        const auto right_scale = [&](int p) { return p < 2 ? f0 : p == 2 ? f1 : f0 + S.vp; };
         f4 aq[ND], from[ND], to[ND], dp[2], da[2];     // (of 16 x 16 up to the diagonal a wave has those at columns half, half + 2)
 #pragma unroll
         for (int n = 0; n < ND; n++) aq[n] = from[n] = to[n] = zero;
         dp[0] = dp[1] = da[0] = da[1] = zero;
         float both = 0.0f;                 // of state and gradient, summed over all elements
-        uint32_t op[4];
+        // (kept as they come: 16 bits made 32 of are waited for at once where their loads are behind a branch)
+        std::conditional_t<sizeof(E) == 2, uint16_t, uint32_t> op[4];
         f4 os = {1.0f, 1.0f, 1.0f, 1.0f};
         float lf = 1.0f, rf = 1.0f;
+        const float *lp = f1, *rp = f0;    // of the lane's product and column
+        int most = 0;                      // the largest of that product's scales
+        if constexpr (HALF) {
+            const int tid = thread(), product = tid / COLS < PRODUCTS ? tid / COLS : 0, column = tid % COLS;
+            lp = (product == 2 ? f0 + S.vp : product == 0 || product == 3 ? f1 + 2 * S.vp : f1 + S.vp) + column;
+            rp = (product < 2 ? f0 : product == 2 ? f1 : f0 + S.vp) + column;
+        }
         // d_out's 64 rows of 32 columns: four elements a lane; lanes 0 .. 159 the factors of a product's column
         auto fetch = [&](int v0, int to) {
-            const int tid = thread(), row = tid / 8, col = tid % 8 * 4, product = tid / COLS < PRODUCTS ? tid / COLS : 0, column = tid % COLS;
+            const int tid = thread(), row = tid / 8, col = tid % 8 * 4;
             const Buffer outs = rows_at(o0, S.ot, steps, S.V);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
@@ -284,8 +292,8 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
             }
             if constexpr (HALF) {
                 os = *reinterpret_cast<const f4*>(f1 + 2 * S.vp + v0 + col);
-                lf = left_scale(product)[v0 + column];
-                rf = right_scale(product)[v0 + column];
+                lf = lp[v0];
+                rf = rp[v0];
             }
             char* buffer = lds + IN + to * BUFFER;
             bring<WAVES>(b0 + v0 / COLS * Ke::BLOCK, buffer, BLOCK);
@@ -302,15 +310,11 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
             }
             x.store(Od.p + row * Ot::ROW + place(col));
             if constexpr (HALF) if (tid < PRODUCTS * COLS) {
-                int top = -1000;
-#pragma unroll
-                for (int w = 0; w < WAVES; w++) top = max(top, tops[w][tid / COLS]);
-                const int e = exponent(lf) + exponent(rf) - top;       // 0 at most
+                const int e = exponent(lf) + exponent(rf) - most;      // 0 at most
                 factors[to][tid / COLS][place(tid % COLS)] = e > -25 ? St(__uint_as_float((127 + e) << 23)) : St(0.0f);
             }
         };
-        if (j) __syncthreads();            // the value head before has been dealt with
-        fetch(0, 0);
+        E gx, wx;                          // the gates of the lane's step
         {                                  // the steps' record, and the largest of the columns' scales by product: dO S, dR S, U dS, dO U, dR U
             const int tid = thread();
             const float* p = reinterpret_cast<const float*>(&reinterpret_cast<const Re*>(record_of<St>(const_cast<char*>(records), at))->steps);
@@ -318,17 +322,33 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
             float x[EACH];
 #pragma unroll
             for (int k = 0; k < EACH; k++) x[k] = p[tid + k * MANY < N ? tid + k * MANY : N - 1];
+            const int64_t t = t0 + (tid % WAVE < steps ? tid % WAVE : steps - 1);
+            gx = gate[b * S.ab + t * S.at + g * S.ag];
+            wx = write[b * S.wb + t * S.wt + g * S.wg];
+            const int c0 = tid < S.vp ? tid : S.vp - 1;
+            float scales[5];
+            const auto read = [&](int c) {
+                scales[0] = f0[c];
+                scales[1] = f0[S.vp + c];
+#pragma unroll
+                for (int k = 0; k < 3; k++) scales[2 + k] = f1[k * S.vp + c];
+            };
+            if constexpr (HALF) read(c0);
+            fetch(0, 0);
+            fence();                       // (all of it is on its way)
             if constexpr (HALF) {
                 int top[PRODUCTS];
 #pragma unroll
                 for (int p = 0; p < PRODUCTS; p++) top[p] = -1000;
-                for (int c = tid; c < S.vp; c += MANY) {
-                    const int es = exponent(f0[c]), eu = exponent(f0[S.vp + c]), ed = exponent(f1[c]), er = exponent(f1[S.vp + c]), eo = exponent(f1[2 * S.vp + c]);
+                for (int c = c0;;) {
+                    const int es = exponent(scales[0]), eu = exponent(scales[1]), ed = exponent(scales[2]), er = exponent(scales[3]), eo = exponent(scales[4]);
                     top[0] = max(top[0], eo + es);
                     top[1] = max(top[1], er + es);
                     top[2] = max(top[2], eu + ed);
                     top[3] = max(top[3], eo + eu);
                     top[4] = max(top[4], er + eu);
+                    if ((c += MANY) >= S.vp) break;
+                    read(c);
                 }
 #pragma unroll
                 for (int p = 0; p < PRODUCTS; p++) {
@@ -340,8 +360,20 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
             for (int k = 0; k < EACH; k++) if (tid + k * MANY < N) reinterpret_cast<float*>(&st)[tid + k * MANY] = x[k];
         }
         __syncthreads();
+        if constexpr (HALF) {
+            const int product = thread() / COLS < PRODUCTS ? thread() / COLS : 0;
+            most = -1000;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) most = max(most, tops[w][product]);
+        }
         put(0);
-        arrived<0>();
+        if (j == 0) {                      // keys and queries come while the first block is used
+            constexpr int BYTES = 2 * In::SIZE * int(sizeof(St));
+            bring<WAVES>(images + (bh * S.chunks + chunk) * IN, lds, BYTES);
+            arrived<(BYTES + 1024 * WAVES - 1) / (1024 * WAVES)>();
+        } else {
+            arrived<0>();
+        }
         int now = 0;
         for (int v0 = 0; v0 < S.vp; v0 += COLS) {
             __syncthreads();               // the block is there, and the one before has been used
@@ -355,6 +387,7 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
                 if constexpr (HALF) f.p[0] *= *reinterpret_cast<const h8*>(&factors[now][p][8 * (tid % WAVE / 16)]);
                 return f;
             };
+            if (BUFFERS == 2 && next) fetch(v0 + COLS, now ^ 1);
             const auto of = Od.rows(band, 0);
             const auto rf = Rs.cols(band, 0), uf = Us.cols(band, 0);
             Frag<St, 1> sf[ND], gf[ND], un[2];
@@ -383,7 +416,6 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
                 product[k % 2] += tid + k * MANY < UNITS ? z : 0.0f;
             }
             both += product[0] + product[1];
-            if (BUFFERS == 2 && next) fetch(v0 + COLS, now ^ 1);
             fence();
             const auto of0 = scaled(of, 0), rf1 = scaled(rf, 1), uf2 = scaled(uf, 2), of3 = scaled(of, 3), rf4 = scaled(rf, 4);
 #pragma unroll
@@ -406,6 +438,10 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
                 arrived<0>();
                 if (BUFFERS == 2) now ^= 1;
             }
+        }
+        if (j == 0) {
+            arrived<0>();                  // keys and queries, of all waves
+            __syncthreads();
         }
         int top[PRODUCTS];
 #pragma unroll
@@ -541,31 +577,38 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
                 tk[n][r] += ldexpf(y[r], top[3] + many + OUT) + ldexpf(z[r], top[4] + many + OUT);
             }
         }
-        if (wave == 0) {                   // a lane for each step: gates
+        // a lane for each step: what its gate gets from the pairs around it and from the states, by two waves
+        if (wave == 0) {
             const auto same = [&](int i) { return i < C && since(cuts, i) <= l; };     // no step up to i, from the next on, drops the state
-            const int64_t t = t0 + (l < steps ? l : steps - 1);
-            const float x = float(gate[b * S.ab + t * S.at + g * S.ag]), w = float(write[b * S.wb + t * S.wt + g * S.wg]);
             double after = double(rows[0][l]) + rows[1][l] - (double(columns[0][l]) + columns[1][l] + columns[2][l] + columns[3][l]);
+#pragma unroll
+            for (int d = 1; d < WAVE; d <<= 1) {
+                const double x = __shfl_down(after, d, WAVE);
+                if (same(l + d)) after += x;
+            }
+            gates[0][l] = after;
+        } else if (wave == 1) {
             double before = double(left[0][l]) + left[1][l];
 #pragma unroll
             for (int d = 1; d < WAVE; d <<= 1) {
-                const double x = __shfl_down(after, d, WAVE), y = __shfl_up(before, d, WAVE);
-                if (same(l + d)) after += x;
-                if (l >= d) before += y;
+                const double x = __shfl_up(before, d, WAVE);
+                if (l >= d) before += x;
             }
             before = __shfl_up(before, 1, WAVE);
             if (l == 0) before = 0.0;
-            double d = after + before;
             if (since(cuts, l) < 0 && st.end != 0.0f) {
                 double sum = 0.0;
 #pragma unroll
                 for (int w = 0; w < WAVES; w++) sum += whole[w];
-                d += double(st.end) * sum;
+                before += double(st.end) * sum;
             }
-            if (l < steps) {
-                d_gate[(b * S.T + t) * S.G + g] = E(cuts >> l & 1 ? 0.0f : -float(d) / (1.0f + expf(-x)));
-                d_write[(b * S.T + t) * S.G + g] = E(writes[l] / (1.0f + expf(w)));
-            }
+            gates[1][l] = before;
+        }
+        __syncthreads();
+        if (wave == 0 && l < steps) {
+            const int64_t to = (b * S.T + t0 + l) * S.G + g;
+            d_gate[to] = E(cuts >> l & 1 ? 0.0f : -float(gates[0][l] + gates[1][l]) / (1.0f + expf(-float(gx))));
+            d_write[to] = E(writes[l] / (1.0f + expf(float(wx))));
         }
     }
     // of the query and the key themselves: d - x^ (x^.d), over the length
