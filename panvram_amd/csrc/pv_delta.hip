@@ -543,7 +543,9 @@ __global__ __launch_bounds__(BLOCK) void step_kernel(const E* __restrict__ query
 
 namespace {
 
-constexpr int SHORT = 8;                   // steps that are walked one by one
+// Calls of so few steps walk them one by one, where nothing is kept for gradients. Heads of 128 x 128, us: 4 heads 5.7 for one step and
+// 20.6 for eight, in chunks 21.7 for nine and 22.1 for sixty-four; 512 heads 17.9, 62.7, 79 and 83.
+constexpr int SHORT = 8;
 
 template <typename E, int DK>
 int32_t forward(const void* query, const void* key, const void* value, const void* gate, const void* write, const float* state, const uint8_t* reset, const Shape& S,

@@ -338,7 +338,7 @@ def test_past_32_bit_offsets():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("T, H, G, K, V, reset", [(2048, 1, 1, 12, 10, None), (2113, 1, 2, 9, 40, 0.002), (3000, 1, 1, 33, 8, None)])
+@pytest.mark.parametrize("T, H, G, K, V, reset", [(2048, 1, 1, 12, 10, None), (2113, 1, 2, 9, 40, 0.002), (3000, 1, 1, 33, 8, None), (1600, 35, 70, 12, 10, 0.001)])
 def test_in_pieces(dtype, T, H, G, K, V, reset):
     """Long sequences of few heads, which are walked in pieces: their starts, ends and gradients"""
     a, d_out, d_last = made(1, T, H, G, K, V, dtype, seed=T, reset=reset, keep=-6.0)
