@@ -11,8 +11,10 @@
 // and what is computed in 32 bits column by column of the state, so that the column's largest value is 2^13 or a little more and what
 // falls below float16's numbers is 2^-37 of that. A product's scale is a number of the lane, as a lane has one column. `wide` operands
 // are two float16, a value and what its rounding left: 22 bits. `narrow` ones are the first alone, 11 bits, which only outputs in
-// 16 bits are made from. Wide are the states and all that they are made from: they are kept and returned in 32 bits. (Two bfloat16 in
-// their place, without any scale, left states off by 4e-6 and outputs in bfloat16 by 1.7 times their own rounding.) Of tensors in
+// bfloat16, of 8 bits, are made from; outputs in float16, as exact as a narrow operand, have wide ones, and gradients in float16 the
+// operands of float32 (two parts of all that they are made from have no room in LDS). Wide are the states and all that they are
+// made from: they are kept and returned in 32 bits. (Two bfloat16 in their place, without any scale, left states off by 4e-6 and
+// outputs in bfloat16 by 1.7 times their own rounding; narrow operands left outputs in float16 off by twice theirs.) Of tensors in
 // float32 the operands are float32, eight products of 16 x 16 x 4 in the place of one of 32, and scales are 1.
 #pragma once
 #include "pv_ops.h"
@@ -29,10 +31,10 @@ constexpr int MAX_K = 128, MAX_STEP = 1 << 22;
 using f4 = __attribute__((ext_vector_type(4))) float;
 using h8 = __attribute__((ext_vector_type(8))) _Float16;
 
-// What operands are held as for tensors of E: S, how many of them a wide one takes; lengths of keys and queries, and the scale
-// of the matrices of 64 x 64, whose elements are 1 at most
-template <typename E> struct Rep { using S = f16; };
-template <> struct Rep<float> { using S = float; };
+// What operands are held as for tensors of E (KEPT: where gradients are made from them); how many of those a wide one takes; lengths of
+// keys and queries, and the scale of the matrices of 64 x 64, whose elements are 1 at most
+template <typename E, bool KEPT> using Rep = std::conditional_t<std::is_same_v<E, bf16> || (std::is_same_v<E, f16> && !KEPT), f16, float>;
+inline bool in_16_bits(int32_t dtype, bool kept) { return dtype == PV_BF16 || (dtype == PV_F16 && !kept); }
 template <typename S> constexpr int wide_of = sizeof(S) == 2 ? 2 : 1;
 template <typename S> constexpr float LONG = sizeof(S) == 2 ? 64.0f : 1.0f;
 template <typename S> constexpr float SQUARE = sizeof(S) == 2 ? 4096.0f : 1.0f;
@@ -189,8 +191,11 @@ template <typename S, int PARTS> __device__ inline Frag<S, PARTS> frag_of(const 
     const f4 all = {up, up, up, up};
     return frag_of<S, PARTS>(lo, hi, all, all);
 }
-template <int PARTS> __device__ inline const Frag<float, 1>& narrow(const Frag<float, PARTS>& f) { return f; }
-template <int PARTS> __device__ inline Frag<f16, 1> narrow(const Frag<f16, PARTS>& f) { return {{f.p[0]}}; }
+// The first N parts of an operand
+template <int N, typename S, int PARTS> __device__ inline Frag<S, N> first_of(const Frag<S, PARTS>& f) {
+    if constexpr (N == PARTS) return f;
+    else return {{f.p[0]}};
+}
 
 // Where column c of a row lies in a tile: of each 32 the places of a lane are neighbours
 __host__ __device__ constexpr int place(int c) { return (c & ~31) | (c & 12) << 1 | (c & 16) >> 2 | (c & 3); }
@@ -291,8 +296,7 @@ template <typename E> __device__ inline Buffer rows_at(const E* at, int stride, 
 // Rows of queries or keys on their way from memory to a tile of 64 x DK, eight elements a lane. Steps past the last come out as 0 (or,
 // where strides make steps overlap, as an earlier one's; their lengths are 0 in either case). A row's last eight are read as they
 // lie, where K is no multiple of 8, and put one by one.
-template <typename E, int DK, int THREADS> struct Rows {
-    using S = typename Rep<E>::S;
+template <typename E, typename S, int DK, int THREADS> struct Rows {
     static constexpr int PER = DK / 8, COUNT = C * PER / THREADS, STEP = THREADS / PER;
     pack<E, 8> v[COUNT];
     static __device__ int column(int K) {                  // of the lane's first element
@@ -380,7 +384,7 @@ template <typename S> struct Record {
     static constexpr int STRIDE = (ALL + 1023) / 1024 * 1024;
 };
 template <typename S, int DK> constexpr int IMAGE = (2 * Tile<S, C, DK>::SIZE * int(sizeof(S)) + 1023) / 1024 * 1024;
-inline uint64_t image_bytes(int32_t dk, int32_t dtype) { return (2 * 64 * (dtype == PV_F32 ? (dk + 4) * 4 : (dk + 8) * 2) + 1023) / 1024 * 1024; }
+inline uint64_t image_bytes(int32_t dk, bool half) { return (2 * 64 * (half ? (dk + 8) * 2 : (dk + 4) * 4) + 1023) / 1024 * 1024; }
 template <typename S> __device__ __host__ inline char* record_of(char* work, int64_t chunk) { return work + chunk * Record<S>::STRIDE; }
 
 // `bytes` of memory to LDS, by W waves of which this is number `wave`, 1,024 at a time (those behind the last whole kilobyte too, up to the next). Both begin at
@@ -428,8 +432,8 @@ template <typename S, int PARTS> __device__ inline void leave(const Buffer& to, 
     __builtin_memcpy(&o, &f, sizeof o);
     to.store(o, at);
 }
-inline uint64_t kept_bytes(uint64_t chunks, int32_t vp, int32_t dk, int32_t dtype) {
-    const uint64_t pad = dtype == PV_F32 ? 4 : 8, bytes = dtype == PV_F32 ? 4 : 2;
+inline uint64_t kept_bytes(uint64_t chunks, int32_t vp, int32_t dk, bool half) {
+    const uint64_t pad = half ? 8 : 4, bytes = half ? 2 : 4;
     return chunks * vp * ((dk + pad + C + pad) * bytes + 12);
 }
 

@@ -67,12 +67,11 @@ template <typename S> __device__ inline void record(const float* m, int row, S (
     }
 }
 
-template <typename E, int DK>
+template <typename E, typename St, int DK>
 __global__ __launch_bounds__(BLOCK, 4) void chunk_kernel(const E* __restrict__ query, const E* __restrict__ key, const E* __restrict__ gate, const E* __restrict__ write,
                                                       const uint8_t* __restrict__ reset, Shape S, char* __restrict__ records, char* __restrict__ images) {
-    using St = typename Rep<E>::S;
     using In = Tile<St, C, DK>;
-    using In8 = Rows<E, DK, BLOCK>;
+    using In8 = Rows<E, St, DK, BLOCK>;
     constexpr int ROW = C + 4, MATRIX = C * ROW * 4, KEYS = 2 * In::SIZE * int(sizeof(St));
     __shared__ alignas(16) char lds[KEYS > 2 * MATRIX ? KEYS : 2 * MATRIX];
     __shared__ alignas(16) Steps st;
@@ -239,18 +238,18 @@ __global__ __launch_bounds__(BLOCK, 4) void chunk_kernel(const E* __restrict__ q
 // has taken all it asks for, 3 us a chunk.)
 
 // MAP: the first walk of a sequence in pieces; there are no outputs, and DK columns more that begin as those of one.
-template <typename E, int DK, int W, bool KEEP, bool MAP>
+template <typename E, typename St, int DK, int W, bool KEEP, bool MAP>
 __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))) void state_kernel(
     const E* __restrict__ value, const float* __restrict__ state, Shape S, const char* __restrict__ records, const char* __restrict__ images, E* __restrict__ out,
-    float* __restrict__ last, Kept<typename Rep<E>::S, DK> kept, Pieces pieces, Joins joins) {
-    using St = typename Rep<E>::S;
+    float* __restrict__ last, Kept<St, DK> kept, Pieces pieces, Joins joins) {
     using Ke = Kept<St, DK>;
-    constexpr int WIDE = wide_of<St>, ND = DK / 16, KB = DK / 32;
+    constexpr int WIDE = wide_of<St>, FINE = std::is_same_v<E, bf16> ? 1 : WIDE, ND = DK / 16, KB = DK / 32;       // (FINE: of what out is made from)
     using In = Tile<St, C, DK>;
     using Square = Tile<St, C, C, WIDE>;
-    using Plain = Tile<St, C, C>;
+    using Pairs = Tile<St, C, C, FINE>;
     using Re = Record<St>;
-    constexpr int BUFFERS = sizeof(St) == 2 ? 2 : 1, IN = IMAGE<St, DK>, BUFFER = IN + (Re::NARROW + 1023) / 1024 * 1024;
+    constexpr int RECORD = MAP ? Re::INVERSE : FINE == WIDE ? Re::ALL : Re::NARROW;
+    constexpr int BUFFERS = sizeof(St) == 2 ? 2 : 1, IN = IMAGE<St, DK>, BUFFER = IN + (RECORD + 1023) / 1024 * 1024;
     __shared__ alignas(1024) char lds[BUFFERS * BUFFER];
     const int tid = threadIdx.x, wave = tid / WAVE, l = tid % WAVE, grp = l / 16, m = l % 16;
     const int width = MAP ? S.vp + DK : S.vp, groups = (width / 16 + W - 1) / W;
@@ -282,7 +281,7 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
             if (n != first && BUFFERS == 1) __syncthreads();   // the chunk before has been used
             char* to = lds + (BUFFERS == 2 ? int(n & 1) * BUFFER : 0);
             bring<1>(in0 + n * IN, to, (MAP ? 1 : 2) * In::SIZE * int(sizeof(St)), 0);
-            bring<1>(rec0 + n * Re::STRIDE, to + IN, MAP ? Re::INVERSE : Re::NARROW, 0);
+            bring<1>(rec0 + n * Re::STRIDE, to + IN, RECORD, 0);
             arrived<0>();
             __syncthreads();               // the chunk is there (and of two, the one before has been used)
         }
@@ -299,7 +298,7 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         const Re& re = *reinterpret_cast<const Re*>(here + IN);
         const Steps& st = re.steps;
         const Square Tt{const_cast<St*>(&re.inv[0][0][0])};
-        const Plain Pt{const_cast<St*>(&re.pair[0][0][0])};
+        const Pairs Pt{const_cast<St*>(&re.pair[0][0][0])};
         const auto four = [&](const float* p, int it) { return *reinterpret_cast<const f4*>(p + 16 * it + 4 * grp); };
         const uint64_t cuts = uint64_t(st.cut[1]) << 32 | st.cut[0];
         f4 v[4];
@@ -325,7 +324,8 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         const int64_t at = (bg * S.chunks + n) * S.vp;     // of the chunk in what is kept
         const Buffer blocks(kept.blocks + at / COLS * Ke::BLOCK, KEEP ? int64_t(S.vp / COLS) * Ke::BLOCK * int(sizeof(St)) : 0);
         // operands of a stage's products are loaded while the stage before runs
-        Frag<St, 1> ka[KB][4], qa[KB][4], kc[2][ND], pa[2][4];
+        Frag<St, 1> ka[KB][4], qa[KB][4], kc[2][ND];
+        Frag<St, FINE> pa[2][4];
         Frag<St, WIDE> ta[2][4], sf[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; kb++)
@@ -357,7 +357,7 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
             for (int kb = 0; kb <= it / 2; kb++) ta[kb][it] = Tt.rows(16 * it, kb);
 #pragma unroll
-        for (int kb = 0; kb < KB; kb++) if constexpr (!MAP) mma_all(y, qa[kb], narrow(sf[kb]));
+        for (int kb = 0; kb < KB; kb++) if constexpr (!MAP) mma_all(y, qa[kb], first_of<FINE>(sf[kb]));
         by_cut(cuts, [&](auto cut) {
 #pragma unroll
             for (int it = 0; it < 4; it++) d[it] = four(st.b, it) * v[it] - part_of_it<decltype(cut)::value>(four(st.x, it) * ss.down, x[it]);
@@ -380,12 +380,12 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         const float du = ds.down * (1.0f / SQUARE<St>);        // of u
         // what it adds to the state (l r is 2 / LONG at most)
         const Scale us = scale_of<St>(over_column(largest(u)) * du);
-        Frag<St, 1> uf[2];
+        Frag<St, FINE> uf[2];
         Frag<St, WIDE> lf[2];
         const float up = sizeof(St) == 2 ? du * us.up : 1.0f;
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
-            uf[kb] = frag_of<St, 1>(u[2 * kb], u[2 * kb + 1], up);
+            uf[kb] = frag_of<St, FINE>(u[2 * kb], u[2 * kb + 1], up);
             lf[kb] = frag_of<St, WIDE>(u[2 * kb], u[2 * kb + 1], four(st.l, 2 * kb) * (LONG<St> * up), four(st.l, 2 * kb + 1) * (LONG<St> * up));
             if constexpr (KEEP) leave(blocks, step_at + 32 * kb * sizeof(St), uf[kb]);
         }
@@ -547,28 +547,31 @@ namespace {
 // 20.6 for eight, in chunks 21.7 for nine and 22.1 for sixty-four; 512 heads 17.9, 62.7, 79 and 83.
 constexpr int SHORT = 8;
 
-template <typename E, int DK>
+template <typename E, typename St, int DK>
 int32_t forward(const void* query, const void* key, const void* value, const void* gate, const void* write, const float* state, const uint8_t* reset, const Shape& S,
                 void* out, float* last, void* kept, void* work, hipStream_t stream, char* err, size_t errcap) {
-    using St = typename Rep<E>::S;
     const auto in = [](const void* p) { return static_cast<const E*>(p); };
     const int64_t heads = S.B * S.G;
     char *records = static_cast<char*>(work), *images = records + heads * S.chunks * Record<St>::STRIDE;
-    chunk_kernel<E, DK><<<dim3(heads * S.chunks), BLOCK, 0, stream>>>(in(query), in(key), in(gate), in(write), reset, S, records, images);
+    chunk_kernel<E, St, DK><<<dim3(heads * S.chunks), BLOCK, 0, stream>>>(in(query), in(key), in(gate), in(write), reset, S, records, images);
     const Kept<St, DK> to(kept, S);
     const Pieces pieces = pieces_of(heads, S.chunks, S.vp, DK);
     const Joins joins(images + S.B * S.H * S.chunks * IMAGE<St, DK>, heads, pieces.count, S.vp, DK);
     if (pieces.count > 1) {
         constexpr int W = 4;
-        state_kernel<E, DK, W, false, true><<<dim3(heads * pieces.count * (((S.vp + DK) / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(
+        state_kernel<E, St, DK, W, false, true><<<dim3(heads * pieces.count * (((S.vp + DK) / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(
             in(value), nullptr, S, records, images, nullptr, nullptr, to, pieces, joins);
         join_kernel<DK, false><<<dim3(heads * ((S.vp / 16 + JOIN_WAVES - 1) / JOIN_WAVES)), (JOIN_WAVES + 1) * WAVE, 0, stream>>>(state, S, pieces.count, joins, joins);
     }
     return with_waves(S, pieces, [&](auto w) {
         constexpr int W = decltype(w)::value;
         const dim3 grid(heads * pieces.count * ((S.vp / 16 + W - 1) / W));
-        if (kept) state_kernel<E, DK, W, true, false><<<grid, (W + 1) * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to, pieces, joins);
-        else state_kernel<E, DK, W, false, false><<<grid, (W + 1) * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to, pieces, joins);
+        const auto walk = [&](auto keep) {
+            state_kernel<E, St, DK, W, decltype(keep)::value, false><<<grid, (W + 1) * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to,
+                                                                                                      pieces, joins);
+        };
+        if constexpr (std::is_same_v<St, Rep<E, true>>) if (kept) walk(std::true_type{});
+        if constexpr (std::is_same_v<St, Rep<E, false>>) if (!kept) walk(std::false_type{});
         return launched(err, errcap);
     });
 }
@@ -582,13 +585,14 @@ uint64_t pv_gated_delta_work_bytes(int64_t B, int64_t T, int32_t H, int32_t G, i
     const int64_t chunks = (T + C - 1) / C, heads = B * G;
     const int32_t vp = (V + 31) / 32 * 32, dk = columns_of(K);
     const Pieces pieces = pieces_of(heads, chunks, vp, dk);
-    return uint64_t(B) * chunks * (uint64_t(G) * (dtype == PV_F32 ? Record<float>::STRIDE : Record<f16>::STRIDE) + uint64_t(H) * image_bytes(dk, dtype)) +
+    const bool half = in_16_bits(dtype, keep);
+    return uint64_t(B) * chunks * (uint64_t(G) * (half ? Record<f16>::STRIDE : Record<float>::STRIDE) + uint64_t(H) * image_bytes(dk, half)) +
            (pieces.count > 1 ? Joins::bytes(heads, pieces.count, vp, dk) : 0);
 }
 
 uint64_t pv_gated_delta_kept_bytes(int64_t B, int64_t T, int32_t G, int32_t K, int32_t V, int32_t dtype) {
     if (B < 1 || G < 1 || T < 1 || K < 1 || V < 1) return 0;
-    return kept_bytes(uint64_t(B) * uint64_t(G) * uint64_t((T + C - 1) / C), (V + 31) / 32 * 32, columns_of(K), dtype);
+    return kept_bytes(uint64_t(B) * uint64_t(G) * uint64_t((T + C - 1) / C), (V + 31) / 32 * 32, columns_of(K), in_16_bits(dtype, true));
 }
 
 uint64_t pv_gated_delta_backward_work_bytes(int64_t B, int64_t T, int32_t G, int32_t K, int32_t V, int32_t dtype) {
@@ -617,7 +621,10 @@ int32_t pv_gated_delta_hip(const void* query, const void* key, const void* value
             return launched(err, errcap);
         }
         return with_k(K, [&](auto k) {
-            return forward<E, decltype(k)::value>(query, key, value, gate, write, state, reset, S, out, last, kept, work, hipStream_t(stream), err, errcap);
+            const auto run = [&](auto st) {
+                return forward<E, decltype(st), decltype(k)::value>(query, key, value, gate, write, state, reset, S, out, last, kept, work, hipStream_t(stream), err, errcap);
+            };
+            return kept ? run(Rep<E, true>{}) : run(Rep<E, false>{});
         });
     });
 }

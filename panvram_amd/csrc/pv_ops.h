@@ -1,5 +1,5 @@
-// What the operators' kernels (pv_scan.hip, pv_norm.hip, pv_loss.hip, pv_clip.hip) share: element types, wide loads and
-// stores, wave sums, and the checks of a C entry.
+// What the operators' kernels (pv_scan.hip, pv_delta.hip, pv_delta_back.hip, pv_norm.hip, pv_layer.hip, pv_dropout.hip, pv_loss.hip,
+// pv_clip.hip) share: element types, wide loads and stores, wave sums, and the checks of a C entry.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

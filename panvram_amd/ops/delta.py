@@ -79,7 +79,8 @@ def gated_delta(query, key, value, gate, write, state=None, reset=None, eps=1e-6
     last float32 [B, G, K, V]); `last` is the next call's state, so generation calls it with T = 1. Gradients flow to query, key,
     value, gate, write and state, from out and from last.
 
-    Sequences are worked on in chunks of 64 steps by matrix products: a NaN or an infinity in one step's inputs reaches the
+    Calls of up to 8 steps without gradients go step by step, others in chunks of 64 by matrix products, long ones of few heads in
+    pieces: the same up to roundings, and equal from run to run, not from one of these ways to another. In chunks a NaN or an infinity in one step's inputs reaches the
     outputs of all steps of its chunk, and through the state those of its head after it; a state that is not finite is dropped by a
     reset all the same. Queries and keys have squares whose sum is a float32."""
     index = on_gpu("gated_delta", query, key, value, gate, write, state, reset)

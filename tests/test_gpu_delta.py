@@ -398,3 +398,28 @@ def test_memory_that_held_something(T, H, G, K, V):
     del held
     for x, y in zip(first, run()):
         assert torch.isfinite(x).all() and torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T, K, V", [(2, 38, 109), (300, 16, 25), (1300, 24, 64)])
+def test_only_outputs_are_rounded(dtype, T, K, V):
+    """Outputs and gradients in 16 bits are off by little more than what rounding them alone would be. That is spread evenly over
+    half a step to both sides, a root mean square of eps / sqrt(12) of the value where mantissas are all 1, the worst that they can
+    be. On top of it 5 % for the count of elements, and 0.3 of it, in squares, in bfloat16: one of narrow operands' 11 bits is off by
+    1 / 8 of bfloat16's step at most, and an output is made from four."""
+    a, d_out, d_last = made(2, T, 2, 4, K, V, dtype, seed=7)
+    ref = wide(a)
+    leaves = {k: ref[k].requires_grad_() for k in NAMES}
+    want = [*delta(**ref)]
+    want += torch.autograd.grad(want, list(leaves.values()), [d_out.double().cpu(), d_last.double().cpu()])
+    b = a | {k: a[k].detach().requires_grad_() for k in NAMES}
+    have = [*ops.gated_delta(**b)]
+    have += torch.autograd.grad(have, [b[k] for k in NAMES], [d_out, d_last])
+    with torch.no_grad():
+        have.append(ops.gated_delta(**a)[0])
+        want.append(want[0])
+    most = 1.05 * torch.finfo(dtype).eps / 12 ** 0.5 * (1.3 ** 0.5 if dtype == torch.bfloat16 else 1.0)
+    for name, h, w in zip(("out", "last", *(f"d_{k}" for k in NAMES), "alone"), have, want):
+        if h.dtype == dtype and h.numel() > 1000:
+            off = float((h.double().cpu() - w).norm() / w.norm())
+            assert off <= most, (name, off, most)
