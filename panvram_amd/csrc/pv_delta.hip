@@ -15,6 +15,11 @@
 // the inverse is, where a series of powers of A is not (keys that are alike make them grow as binomials do).
 //
 // Calls of few steps walk them one by one instead (`step_kernel`), the state in registers: one read and one write of it.
+//
+// What bounds it. bfloat16, 8 sequences of 8,192 steps, 8 heads of 128 x 128: chunk_kernel 222 us (8,192 chunks, 7 us each on a CU that has four
+// at once: chains of small products), state_kernel 492 (128 chunks in a row, 3.8 us each: one wave a SIMD, half of its time in vector
+// operations between products). In float32 a chunk takes it 7 us: eight products of a quarter of the rate, no second buffer. step_kernel
+// reads and writes 512 states of 128 x 128 in 17-18 us, 3.8 TB/s.
 #include "pv_delta.h"
 
 #include <algorithm>

