@@ -19,7 +19,7 @@
 // What bounds it. bfloat16, 8 sequences of 8,192 steps, 8 heads of 128 x 128: chunk_kernel 222 us (8,192 chunks, 7 us each on a CU that has four
 // at once: chains of small products), state_kernel 492 (128 chunks in a row, 3.8 us each: one wave a SIMD, half of its time in vector
 // operations between products). In float32 a chunk takes it 7 us: eight products of a quarter of the rate, no second buffer. step_kernel
-// reads and writes 512 states of 128 x 128 in 17-18 us, 3.8 TB/s.
+// reads and writes 512 states of 128 x 128 in 16 us, 4.2 TB/s (18 before a step's inputs were asked for ahead of the state).
 #include "pv_delta.h"
 
 #include <algorithm>
@@ -473,6 +473,18 @@ __global__ __launch_bounds__(BLOCK) void step_kernel(const E* __restrict__ query
     const int64_t bg = blockIdx.x / groups, b = bg / S.G;
     const int g = int(bg % S.G), h = shared(S, g), col = int(blockIdx.x % groups) * STEP_COLS + 4 * quad;
     const int left = S.V - col;            // columns up to the state's last
+    // what a step brings is asked for a step ahead, and the first before the state
+    E x0 = E(0.0f), v0[4], gate0, write0;  // (x0 of lanes 0 .. K-1: the key, of lanes 128 ..: the query)
+    const int d0 = tid % MAX_K;
+    const auto fetch = [&](int64_t t) {
+        if (d0 < S.K) x0 = tid < MAX_K ? key[b * S.kb + t * S.kt + h * S.kh + d0] : query[b * S.qb + t * S.qt + h * S.qh + d0];
+        gate0 = gate[b * S.ab + t * S.at + g * S.ag];
+        write0 = write[b * S.wb + t * S.wt + g * S.wg];
+        const int64_t at = b * S.vb + t * S.vt + g * S.vh + col;
+#pragma unroll
+        for (int c = 0; c < 4; c++) v0[c] = c < left ? value[at + c] : E(0.0f);
+    };
+    fetch(0);
     pack<float, 4> s[STEP_ROWS];
 #pragma unroll
     for (int j = 0; j < STEP_ROWS; j++) {
@@ -482,15 +494,16 @@ __global__ __launch_bounds__(BLOCK) void step_kernel(const E* __restrict__ query
         else s[j] = pack<float, 4>::load_part(from, state && d < S.K ? left : 0);
     }
     for (int64_t t = 0; t < S.T; t++) {
-        float x = 0.0f;                    // lanes 0 .. K-1: the key, lanes 128 ..: the query
-        const int d0 = tid % MAX_K;
-        if (d0 < S.K) x = tid < MAX_K ? float(key[b * S.kb + t * S.kt + h * S.kh + d0]) : float(query[b * S.qb + t * S.qt + h * S.qh + d0]);
+        const float x = float(x0), gt = float(gate0), wt = float(write0);
+        float v[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) v[c] = float(v0[c]);
+        if (t + 1 < S.T) fetch(t + 1);
         kq[tid / MAX_K][d0] = x;
         const float square = wave_sum(x * x);
         if (tid % WAVE == 0) dots[wave][0] = square;
         __syncthreads();
         const float rk = 1.0f / sqrtf(dots[0][0] + dots[1][0] + S.eps), rq = 1.0f / sqrtf(dots[2][0] + dots[3][0] + S.eps);
-        const float gt = float(gate[b * S.ab + t * S.at + g * S.ag]), wt = float(write[b * S.wb + t * S.wt + g * S.wg]);
         const float a = 1.0f / (1.0f + expf(gt)), beta = 1.0f / (1.0f + expf(-wt));
         const bool cut = a == 0.0f || (reset && reset[b * S.T + t]);
         float sk[4] = {0, 0, 0, 0}, sq[4] = {0, 0, 0, 0}, kd[STEP_ROWS], together = 0.0f;
@@ -520,13 +533,11 @@ __global__ __launch_bounds__(BLOCK) void step_kernel(const E* __restrict__ query
         }
         __syncthreads();
         const float kdq = (dots[0][1] + dots[1][1]) + (dots[2][1] + dots[3][1]);
-        const int64_t at = b * S.vb + t * S.vt + g * S.vh + col;
         E* to = out + ((b * S.T + t) * S.G + g) * S.V + col;
 #pragma unroll
         for (int c = 0; c < 4; c++) {
             const int n = 4 * quad + c;
-            const float v = c < left ? float(value[at + c]) : 0.0f;
-            const float u = beta * (v - ((sums[0][0][n] + sums[1][0][n]) + (sums[2][0][n] + sums[3][0][n])));
+            const float u = beta * (v[c] - ((sums[0][0][n] + sums[1][0][n]) + (sums[2][0][n] + sums[3][0][n])));
             const float o = fmaf(kdq, u, (sums[0][1][n] + sums[1][1][n]) + (sums[2][1][n] + sums[3][1][n]));
             if (row == 0 && c < left) to[c] = E(o);
 #pragma unroll
@@ -548,8 +559,8 @@ __global__ __launch_bounds__(BLOCK) void step_kernel(const E* __restrict__ query
 
 namespace {
 
-// Calls of so few steps walk them one by one, where nothing is kept for gradients. Heads of 128 x 128, us: 4 heads 5.7 for one step and
-// 20.6 for eight, in chunks 21.7 for nine and 22.1 for sixty-four; 512 heads 17.9, 62.7, 79 and 83.
+// Calls of so few steps walk them one by one, where nothing is kept for gradients. Heads of 128 x 128, us: 4 heads 5.3 for one step and
+// 17.5 for eight, in chunks 21.7 for nine and 22.1 for sixty-four; 512 heads 16.2, 53, 79 and 82.
 constexpr int SHORT = 8;
 
 template <typename E, typename St, int DK>

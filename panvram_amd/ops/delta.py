@@ -7,15 +7,16 @@ from .. import _native as N
 from ._call import DTYPES, call, on_gpu, once, ptr
 
 
+_FORWARD, _BACKWARD = ctypes.c_int64 * 15, ctypes.c_int64 * 9         # strides of a sequence, a step and a head of each tensor
+
+
 def _strided(t):
-    """`t` with neighbouring elements in a head, and steps at most 2^22 elements apart: itself, or a copy."""
-    if (t.dim() == 4 and t.stride(3) != 1 and t.shape[3] != 1) or t.stride(1) > 1 << 22:
+    """`t` with neighbouring elements in a head, and steps at most 2^22 elements apart: itself, or a copy; and its strides."""
+    s = t.stride()
+    if s[1] > 1 << 22 or (len(s) == 4 and s[3] != 1 and t.shape[3] != 1):
         t = t.contiguous()
-    return t
-
-
-def _strides(*tensors):
-    return (ctypes.c_int64 * (3 * len(tensors)))(*(s for t in tensors for s in t.stride()[:3]))
+        s = t.stride()
+    return t, *s[:3]
 
 
 def _forward(index, query, key, value, gate, write, state, reset, eps, keep):
@@ -23,15 +24,19 @@ def _forward(index, query, key, value, gate, write, state, reset, eps, keep):
     B, T, H, K = query.shape
     G, V = value.shape[2:]
     dev, dtype = query.device, query.dtype
-    given = [_strided(t) for t in (query, key, value, gate, write)]
+    query, *qs = _strided(query)
+    key, *ks = _strided(key)
+    value, *vs = _strided(value)
+    gate, *gs = _strided(gate)
+    write, *ws = _strided(write)
     out = torch.empty((B, T, G, V), dtype=dtype, device=dev)
     last = torch.empty((B, G, K, V), dtype=torch.float32, device=dev)
     L, code = N.lib(), DTYPES[dtype]
     kept = torch.empty(L.pv_gated_delta_kept_bytes(B, T, G, K, V, code), dtype=torch.uint8, device=dev) if keep else None
     size = L.pv_gated_delta_work_bytes(B, T, H, G, K, V, code, int(keep))
     work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    call(L.pv_gated_delta_hip, index, *(t.data_ptr() for t in given), ptr(state), ptr(reset), B, T, H, G, K, V, _strides(*given), eps, code, out.data_ptr(),
-         last.data_ptr(), ptr(kept), ptr(work), size)
+    call(L.pv_gated_delta_hip, index, query.data_ptr(), key.data_ptr(), value.data_ptr(), gate.data_ptr(), write.data_ptr(), ptr(state), ptr(reset), B, T, H, G, K, V,
+         _FORWARD(*qs, *ks, *vs, *gs, *ws), eps, code, out.data_ptr(), last.data_ptr(), ptr(kept), ptr(work), size)
     return out, last, kept, work
 
 
@@ -50,16 +55,17 @@ class _GatedDelta(torch.autograd.Function):
         gate, write, kept, records = ctx.saved_tensors
         B, T, H, K, G, V = ctx.shape
         dev, dtype = gate.device, gate.dtype
-        d_out = torch.zeros((B, T, G, V), dtype=dtype, device=dev) if d_out is None else _strided(d_out)
+        d_out, *os = _strided(torch.zeros((B, T, G, V), dtype=dtype, device=dev) if d_out is None else d_out)
         d_last = None if d_last is None else d_last.contiguous()
         d_query, d_key, d_value, d_gate, d_write = (torch.empty(s, dtype=dtype, device=dev) for s in ((B, T, H, K), (B, T, H, K), (B, T, G, V), (B, T, G), (B, T, G)))
         d_state = torch.empty((B, G, K, V), dtype=torch.float32, device=dev) if ctx.has_state else None
         L, code = N.lib(), DTYPES[dtype]
         size = L.pv_gated_delta_backward_work_bytes(B, T, G, K, V, code)
         work = torch.empty(size, dtype=torch.uint8, device=dev)
-        gate, write = _strided(gate), _strided(write)
+        gate, *gs = _strided(gate)
+        write, *ws = _strided(write)
         call(L.pv_gated_delta_backward_hip, gate.get_device(), gate.data_ptr(), write.data_ptr(), d_out.data_ptr(), ptr(d_last), B, T, H, G, K, V,
-             _strides(gate, write, d_out), code, kept.data_ptr(), records.data_ptr(), d_query.data_ptr(), d_key.data_ptr(), d_value.data_ptr(), d_gate.data_ptr(),
+             _BACKWARD(*gs, *ws, *os), code, kept.data_ptr(), records.data_ptr(), d_query.data_ptr(), d_key.data_ptr(), d_value.data_ptr(), d_gate.data_ptr(),
              d_write.data_ptr(), ptr(d_state), work.data_ptr(), size)
         return d_query, d_key, d_value, d_gate, d_write, d_state, None, None
 
@@ -79,6 +85,9 @@ def gated_delta(query, key, value, gate, write, state=None, reset=None, eps=1e-6
     last float32 [B, G, K, V]); `last` is the next call's state, so generation calls it with T = 1. Gradients flow to query, key,
     value, gate, write and state, from out and from last.
 
+    For its gradients a call keeps, beside gate and write, some 2 KB a step of each head of 128 x 128 in bfloat16 (3.3 in float16 and float32):
+    states and updates of each chunk, and what the chunks' steps do to each other. Queries, keys and values need not be kept.
+
     Calls of up to 8 steps without gradients go step by step, others in chunks of 64 by matrix products, long ones of few heads in
     pieces: the same up to roundings, and equal from run to run, not from one of these ways to another. In chunks a NaN or an infinity in one step's inputs reaches the
     outputs of all steps of its chunk, and through the state those of its head after it; a state that is not finite is dropped by a
@@ -87,7 +96,7 @@ def gated_delta(query, key, value, gate, write, state=None, reset=None, eps=1e-6
     if query.dim() != 4 or query.shape != key.shape:
         raise ValueError(f"gated_delta: query and key are [B, T, H, K] alike, got {list(query.shape)} and {list(key.shape)}")
     dtype = query.dtype
-    if dtype not in DTYPES or any(t.dtype != dtype for t in (key, value, gate, write)):
+    if dtype not in DTYPES or not (dtype == key.dtype == value.dtype == gate.dtype == write.dtype):
         raise ValueError(f"gated_delta: query, key, value, gate and write are float32, bfloat16 or float16 alike, got {[str(t.dtype) for t in (query, key, value, gate, write)]}")
     B, T, H, K = query.shape
     if value.dim() != 4 or value.shape[:2] != (B, T) or H < 1 or value.shape[2] < 1 or value.shape[2] % H:
