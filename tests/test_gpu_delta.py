@@ -423,3 +423,11 @@ def test_only_outputs_are_rounded(dtype, T, K, V):
         if h.dtype == dtype and h.numel() > 1000:
             off = float((h.double().cpu() - w).norm() / w.norm())
             assert off <= most, (name, off, most)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K, V", [(20, 700), (128, 517)])
+def test_wide_values(dtype, K, V):
+    """More columns of values than the gradients' lanes look at in one turn"""
+    a, d_out, d_last = made(1, 70, 1, 2, K, V, dtype, reset=0.02)
+    compare(a, d_out, d_last)
