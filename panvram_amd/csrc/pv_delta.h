@@ -485,7 +485,7 @@ template <typename F> int32_t with_k(int32_t K, F&& f) {
 // at least, as a join costs what a few chunks do; the two walks of three pieces take two thirds of the time of one over the whole.
 // One sequence, heads of 128 x 128, in pieces and as one, ms: 20 heads (three pieces) of 2,048 steps 0.12 and 0.13, of 32,768 steps 1.27 and
 // 1.78, in float32 3.5 and 5.8; 24 heads (two) of 2,048 steps 0.14 and 0.13, of 32,768 steps 1.79 and 1.87; 4 heads (sixteen) of 131,072
-// steps 1.0 and 5.9.
+// steps 0.98 and 5.9.
 struct Pieces {
     int32_t count;                         // 1: the walk is as it is
     int64_t chunks;                        // of a piece; the last one's may be fewer
@@ -509,17 +509,20 @@ struct Joins {
 
 constexpr int JOIN_WAVES = 4;
 
-// ---- join_kernel: each piece's start from the one before it, in 32 bits: a wave for 16 columns of a head's state, and a wave more that
-// brings the pieces' maps to LDS, the next one while one is used. (Read from memory by the waves that use it a map took 35 us.)
+// ---- join_kernel: each piece's start from the one before it, in 32 bits: a workgroup for 16 columns of a head's state, of which each wave
+// makes some rows of each piece, and a wave more that brings the pieces' maps to LDS, the next one while one is used. Products and
+// reads of a map bound it: 2.4 us a piece of 128 x 128, 3.2 backwards. (By one wave for all rows of 16 columns 7 us, with maps read from memory by the
+// waves that use them 35.)
 
 // TURNED: backwards, each piece's end from the one after it, by the maps transposed; `ends` are of the gradient, `maps` still those of the state.
 template <int DK, bool TURNED>
-static __global__ __launch_bounds__((JOIN_WAVES + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))) void join_kernel(const float* __restrict__ state, Shape S, int pieces, Joins joins, Joins maps) {
-    constexpr int ND = DK / 16, KB = DK / 32, MAP = DK * DK * 4;
+static __global__ __launch_bounds__((JOIN_WAVES + 1) * WAVE) void join_kernel(const float* __restrict__ state, Shape S, int pieces, Joins joins, Joins maps) {
+    constexpr int KB = DK / 32, MAP = DK * DK * 4, MINE = DK / 16 > JOIN_WAVES ? DK / 16 / JOIN_WAVES : 1, ROW = DK + 4;
     __shared__ alignas(1024) char lds[2 * MAP];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), l = threadIdx.x % WAVE, grp = l / 16, m = l % 16, groups = (S.vp / 16 + JOIN_WAVES - 1) / JOIN_WAVES;
+    __shared__ alignas(16) float states[2][16][ROW];       // this piece's and the next one's, by columns
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), l = threadIdx.x % WAVE, grp = l / 16, m = l % 16, groups = S.vp / 16;
     const int64_t bg = blockIdx.x / groups;
-    const int col = int(blockIdx.x % groups * JOIN_WAVES + wave) * 16 + m;
+    const int col = int(blockIdx.x % groups) * 16 + m, n0 = wave * MINE;
     const auto piece_of = [&](int p) { return bg * pieces + (TURNED ? pieces - 1 - p : p); };
     if (wave == JOIN_WAVES) {
         for (int p = 0; p + 1 < pieces; p++) {
@@ -529,47 +532,46 @@ static __global__ __launch_bounds__((JOIN_WAVES + 1) * WAVE) __attribute__((amdg
         }
         return;
     }
-    const bool on = col < S.vp;            // (a whole wave)
-    f4 s[ND], x[ND];
+    const bool on = n0 < DK / 16;          // (a whole wave)
+    f4 x[MINE];
     bool cut = false;
     const auto fetch = [&](int p) {
 #pragma unroll
-        for (int n = 0; n < ND; n++) x[n] = on ? *reinterpret_cast<const f4*>(joins.ends + (piece_of(p) * (S.vp + DK) + col) * DK + 16 * n + 4 * grp) : f4{0, 0, 0, 0};
+        for (int n = 0; n < MINE; n++) if (on) x[n] = *reinterpret_cast<const f4*>(joins.ends + (piece_of(p) * (S.vp + DK) + col) * DK + 16 * (n0 + n) + 4 * grp);
         cut = maps.cut[piece_of(p)];
     };
-#pragma unroll
-    for (int n = 0; n < ND; n++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int d = 16 * n + 4 * grp + r;
-            s[n][r] = state && col < S.V && d < S.K ? state[(bg * S.K + d) * S.V + col] : 0.0f;
-        }
+    for (int i = threadIdx.x; i < 16 * DK; i += JOIN_WAVES * WAVE) {
+        const int c = int(blockIdx.x % groups) * 16 + i % 16, d = i / 16;
+        states[0][i % 16][d] = state && c < S.V && d < S.K ? state[(bg * S.K + d) * S.V + c] : 0.0f;
+    }
     fetch(0);
     for (int p = 0; p + 1 < pieces; p++) {
-        __syncthreads();
-        const float* map = reinterpret_cast<const float*>(lds + p % 2 * MAP);
-        f4 z[ND];
+        __syncthreads();                   // the map and the state are there, and those before them have been used
+        if (!on) continue;
+        const float *map = reinterpret_cast<const float*>(lds + p % 2 * MAP), *from = &states[p % 2][m][4 * grp];
+        f4 z[MINE];
 #pragma unroll
-        for (int n = 0; n < ND; n++) z[n] = f4{0, 0, 0, 0};
+        for (int n = 0; n < MINE; n++) z[n] = f4{0, 0, 0, 0};
         if (!cut) {
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) {
-                Frag<float, 1> a[ND];
+                Frag<float, 1> a[MINE];
 #pragma unroll
-                for (int n = 0; n < ND; n++)
+                for (int n = 0; n < MINE; n++)
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
-                        const int d = 32 * kb + 4 * grp + j % 4 + j / 4 * 16;
-                        a[n].v[j] = TURNED ? map[(16 * n + m) * DK + d] : map[d * DK + 16 * n + m];
+                        const int d = 32 * kb + 4 * grp + j % 4 + j / 4 * 16, row = 16 * (n0 + n) + m;
+                        a[n].v[j] = TURNED ? map[row * DK + d] : map[d * DK + row];
                     }
-                mma_all(z, a, frag_of<float, 1>(s[2 * kb], s[2 * kb + 1], 1.0f));
+                mma_all(z, a, frag_of<float, 1>(*reinterpret_cast<const f4*>(from + 32 * kb), *reinterpret_cast<const f4*>(from + 32 * kb + 16), 1.0f));
             }
         }
-        float* to = joins.starts + (piece_of(p + 1) * S.vp + col) * DK + 4 * grp;
+        float *to = joins.starts + (piece_of(p + 1) * S.vp + col) * DK + 16 * n0 + 4 * grp, *next = &states[(p + 1) % 2][m][16 * n0 + 4 * grp];
 #pragma unroll
-        for (int n = 0; n < ND; n++) {
-            s[n] = z[n] + x[n];
-            if (on) *reinterpret_cast<f4*>(to + 16 * n) = s[n];
+        for (int n = 0; n < MINE; n++) {
+            const f4 s = z[n] + x[n];
+            *reinterpret_cast<f4*>(to + 16 * n) = s;
+            *reinterpret_cast<f4*>(next + 16 * n) = s;
         }
         if (p + 2 < pieces) fetch(p + 1);
     }

@@ -577,7 +577,7 @@ int32_t forward(const void* query, const void* key, const void* value, const voi
         constexpr int W = 4;
         state_kernel<E, St, DK, W, false, true><<<dim3(heads * pieces.count * (((S.vp + DK) / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(
             in(value), nullptr, S, records, images, nullptr, nullptr, to, pieces, joins);
-        join_kernel<DK, false><<<dim3(heads * ((S.vp / 16 + JOIN_WAVES - 1) / JOIN_WAVES)), (JOIN_WAVES + 1) * WAVE, 0, stream>>>(state, S, pieces.count, joins, joins);
+        join_kernel<DK, false><<<dim3(heads * (S.vp / 16)), (JOIN_WAVES + 1) * WAVE, 0, stream>>>(state, S, pieces.count, joins, joins);
     }
     return with_waves(S, pieces, [&](auto w) {
         constexpr int W = decltype(w)::value;

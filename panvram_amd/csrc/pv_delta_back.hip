@@ -667,7 +667,7 @@ int32_t backward(const void* gate, const void* write, const void* d_out, const f
         constexpr int W = 4;
         walk_kernel<E, DK, W, true><<<dim3(heads * pieces.count * ((S.vp / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(in(d_out), nullptr, S, rec, images, nullptr,
                                                                                                                       nullptr, walked, pieces, joins);
-        join_kernel<DK, true><<<dim3(heads * ((S.vp / 16 + JOIN_WAVES - 1) / JOIN_WAVES)), (JOIN_WAVES + 1) * WAVE, 0, stream>>>(d_last, S, pieces.count, joins, maps);
+        join_kernel<DK, true><<<dim3(heads * (S.vp / 16)), (JOIN_WAVES + 1) * WAVE, 0, stream>>>(d_last, S, pieces.count, joins, maps);
     }
     with_waves(S, pieces, [&](auto w) {
         constexpr int W = decltype(w)::value;
