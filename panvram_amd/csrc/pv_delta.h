@@ -10,11 +10,11 @@
 // Held as. Of tensors in 16 bits the operands are float16, scaled by powers of two: keys and queries step by step, to lengths near 64,
 // and what is computed in 32 bits column by column of the state, so that the column's largest value is 2^13 or a little more and what
 // falls below float16's numbers is 2^-37 of that. A product's scale is a number of the lane, as a lane has one column. `wide` operands
-// are two float16, a value and what its rounding left: 22 bits. `narrow` ones are the first alone, 11 bits, which only outputs in
-// bfloat16, of 8 bits, are made from; outputs in float16, as exact as a narrow operand, have wide ones, and gradients in float16 the
-// operands of float32 (two parts of all that they are made from have no room in LDS). Wide are the states and all that they are
-// made from: they are kept and returned in 32 bits. (Two bfloat16 in their place, without any scale, left states off by 4e-6 and
-// outputs in bfloat16 by 1.7 times their own rounding; narrow operands left outputs in float16 off by twice theirs.) Of tensors in
+// are two float16, a value and what its rounding left: 22 bits. `narrow` ones are the first alone, 11 bits, which only gradients in
+// bfloat16, of 8 bits, are made from; gradients in float16, as exact as a narrow operand, have the
+// operands of float32 (two parts of all that they are made from have no room in LDS). Wide are the states, outputs and all that they are
+// made from. (Two bfloat16 in their place, without any scale, left states off by 4e-6 and outputs in bfloat16 by 1.7 times their own
+// rounding; narrow operands left outputs in bfloat16 0.0011 off from the exact ones rounded, by flips to a neighbour, and wide ones 0.00001.) Of tensors in
 // float32 the operands are float32, eight products of 16 x 16 x 4 in the place of one of 32, and scales are 1.
 #pragma once
 #include "pv_ops.h"
@@ -190,11 +190,6 @@ template <typename S, int PARTS> __device__ inline Frag<S, PARTS> frag_of(const 
 template <typename S, int PARTS> __device__ inline Frag<S, PARTS> frag_of(const f4& lo, const f4& hi, float up) {
     const f4 all = {up, up, up, up};
     return frag_of<S, PARTS>(lo, hi, all, all);
-}
-// The first N parts of an operand
-template <int N, typename S, int PARTS> __device__ inline Frag<S, N> first_of(const Frag<S, PARTS>& f) {
-    if constexpr (N == PARTS) return f;
-    else return {{f.p[0]}};
 }
 
 // Where column c of a row lies in a tile: of each 32 the places of a lane are neighbours
@@ -379,7 +374,6 @@ template <typename S> struct Record {
     Steps steps;
     S inv[wide_of<S>][C][C + PAD], pair[wide_of<S>][C][C + PAD];
     static constexpr int ALL = 2080 + 2 * wide_of<S> * C * (C + PAD) * int(sizeof(S));
-    static constexpr int NARROW = ALL - (wide_of<S> - 1) * C * (C + PAD) * int(sizeof(S));     // without the second part of M q k^T
     static constexpr int INVERSE = 2080 + wide_of<S> * C * (C + PAD) * int(sizeof(S));          // without M q k^T
     static constexpr int STRIDE = (ALL + 1023) / 1024 * 1024;
 };

@@ -248,12 +248,11 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
     const E* __restrict__ value, const float* __restrict__ state, Shape S, const char* __restrict__ records, const char* __restrict__ images, E* __restrict__ out,
     float* __restrict__ last, Kept<St, DK> kept, Pieces pieces, Joins joins) {
     using Ke = Kept<St, DK>;
-    constexpr int WIDE = wide_of<St>, FINE = std::is_same_v<E, bf16> ? 1 : WIDE, ND = DK / 16, KB = DK / 32;       // (FINE: of what out is made from)
+    constexpr int WIDE = wide_of<St>, ND = DK / 16, KB = DK / 32;
     using In = Tile<St, C, DK>;
     using Square = Tile<St, C, C, WIDE>;
-    using Pairs = Tile<St, C, C, FINE>;
     using Re = Record<St>;
-    constexpr int RECORD = MAP ? Re::INVERSE : FINE == WIDE ? Re::ALL : Re::NARROW;
+    constexpr int RECORD = MAP ? Re::INVERSE : Re::ALL;
     constexpr int BUFFERS = sizeof(St) == 2 ? 2 : 1, IN = IMAGE<St, DK>, BUFFER = IN + (RECORD + 1023) / 1024 * 1024;
     __shared__ alignas(1024) char lds[BUFFERS * BUFFER];
     const int tid = threadIdx.x, wave = tid / WAVE, l = tid % WAVE, grp = l / 16, m = l % 16;
@@ -302,8 +301,7 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         const In Kt{reinterpret_cast<St*>(here)}, Qt{reinterpret_cast<St*>(here) + In::SIZE};
         const Re& re = *reinterpret_cast<const Re*>(here + IN);
         const Steps& st = re.steps;
-        const Square Tt{const_cast<St*>(&re.inv[0][0][0])};
-        const Pairs Pt{const_cast<St*>(&re.pair[0][0][0])};
+        const Square Tt{const_cast<St*>(&re.inv[0][0][0])}, Pt{const_cast<St*>(&re.pair[0][0][0])};
         const auto four = [&](const float* p, int it) { return *reinterpret_cast<const f4*>(p + 16 * it + 4 * grp); };
         const uint64_t cuts = uint64_t(st.cut[1]) << 32 | st.cut[0];
         f4 v[4];
@@ -330,8 +328,7 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         const Buffer blocks(kept.blocks + at / COLS * Ke::BLOCK, KEEP ? int64_t(S.vp / COLS) * Ke::BLOCK * int(sizeof(St)) : 0);
         // operands of a stage's products are loaded while the stage before runs
         Frag<St, 1> ka[KB][4], qa[KB][4], kc[2][ND];
-        Frag<St, FINE> pa[2][4];
-        Frag<St, WIDE> ta[2][4], sf[KB];
+        Frag<St, WIDE> ta[2][4], pa[2][4], sf[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; kb++)
 #pragma unroll
@@ -362,7 +359,7 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
             for (int kb = 0; kb <= it / 2; kb++) ta[kb][it] = Tt.rows(16 * it, kb);
 #pragma unroll
-        for (int kb = 0; kb < KB; kb++) if constexpr (!MAP) mma_all(y, qa[kb], first_of<FINE>(sf[kb]));
+        for (int kb = 0; kb < KB; kb++) if constexpr (!MAP) mma_all(y, qa[kb], sf[kb]);
         by_cut(cuts, [&](auto cut) {
 #pragma unroll
             for (int it = 0; it < 4; it++) d[it] = four(st.b, it) * v[it] - part_of_it<decltype(cut)::value>(four(st.x, it) * ss.down, x[it]);
@@ -385,12 +382,11 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         const float du = ds.down * (1.0f / SQUARE<St>);        // of u
         // what it adds to the state (l r is 2 / LONG at most)
         const Scale us = scale_of<St>(over_column(largest(u)) * du);
-        Frag<St, FINE> uf[2];
-        Frag<St, WIDE> lf[2];
+        Frag<St, WIDE> uf[2], lf[2];
         const float up = sizeof(St) == 2 ? du * us.up : 1.0f;
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
-            uf[kb] = frag_of<St, FINE>(u[2 * kb], u[2 * kb + 1], up);
+            uf[kb] = frag_of<St, WIDE>(u[2 * kb], u[2 * kb + 1], up);
             lf[kb] = frag_of<St, WIDE>(u[2 * kb], u[2 * kb + 1], four(st.l, 2 * kb) * (LONG<St> * up), four(st.l, 2 * kb + 1) * (LONG<St> * up));
             if constexpr (KEEP) leave(blocks, step_at + 32 * kb * sizeof(St), uf[kb]);
         }
