@@ -9,12 +9,10 @@
 //
 // Held as. Of tensors in 16 bits the operands are float16, scaled by powers of two: keys and queries step by step, to lengths near 64,
 // and what is computed in 32 bits column by column of the state, so that the column's largest value is 2^13 or a little more and what
-// falls below float16's numbers is 2^-37 of that. A product's scale is a number of the lane, as a lane has one column. `wide` operands
-// are two float16, a value and what its rounding left: 22 bits. `narrow` ones are the first alone, 11 bits, which only gradients in
-// bfloat16, of 8 bits, are made from; gradients in float16, as exact as a narrow operand, have the
-// operands of float32 (two parts of all that they are made from have no room in LDS). Wide are the states, outputs and all that they are
-// made from. (Two bfloat16 in their place, without any scale, left states off by 4e-6 and outputs in bfloat16 by 1.7 times their own
-// rounding; narrow operands left outputs in bfloat16 0.0011 off from the exact ones rounded, by flips to a neighbour, and wide ones 0.00001.) Of tensors in
+// falls below float16's numbers is 2^-37 of that. A product's scale is a number of the lane, as a lane has one column. What is computed
+// is `wide`: two float16, a value and what its rounding left, 22 bits. (Two bfloat16, without any scale, left states off by 4e-6
+// and outputs in bfloat16 by 1.7 times their own rounding; the first part alone, 11 bits, left outputs and gradients in bfloat16 0.0011 off from
+// the exact ones rounded, by flips to a neighbour, where both leave 0.00001 to 0.00005.) Gradients in float16 have the operands of float32. Of tensors in
 // float32 the operands are float32, eight products of 16 x 16 x 4 in the place of one of 32, and scales are 1.
 #pragma once
 #include "pv_ops.h"
@@ -406,29 +404,33 @@ __device__ inline int since(uint64_t cut, int i) {         // the last step up t
 
 // What the forward pass keeps for the backward pass, and what the walk backwards leaves for the gradients: arrays of the same
 // shapes, for a chunk of a value head, in blocks of 32 columns of the state or of values. A block is, as it will lie in LDS,
-//   states   [32][DK + padding]: S before the chunk, or the gradient of S after it, by columns, rows at their places
-//   steps    [32][64 + padding]: U, or the gradient of b D; steps at their places
+//   states   [parts][32][DK + padding]: S before the chunk, or the gradient of S after it, by columns, rows at their places
+//   steps    [parts][32][64 + padding]: U, or the gradient of b D; steps at their places
 // and beside the blocks scales [3][vp]: what the columns of states, of steps, and (backwards) of the gradient of out are to be multiplied by
 constexpr int COLS = 32;
 template <typename S, int DK> struct Kept {
-    static constexpr int PAD = 16 / sizeof(S), STATE = DK + PAD, STEP = C + PAD, BLOCK = COLS * (STATE + STEP);    // elements
+    static constexpr int PAD = 16 / sizeof(S), STATE = DK + PAD, STEP = C + PAD, BLOCK = wide_of<S> * COLS * (STATE + STEP);    // elements
+    static constexpr int STATES = COLS * STATE * int(sizeof(S)), STEPS = COLS * STEP * int(sizeof(S));     // of a part, in bytes
     static_assert(BLOCK * sizeof(S) % 1024 == 0, "whole kilobytes");
     S* blocks;
     float* scales;
     Kept(void* p, const Shape& s) : blocks(static_cast<S*>(p)), scales(reinterpret_cast<float*>(blocks + s.B * s.G * s.chunks * (s.vp / COLS) * int64_t(BLOCK))) {}
     // of a column's first place, in bytes; nowhere behind the last column
     static __device__ uint32_t state_at(int col, int vp) { return col < vp ? (col / COLS * BLOCK + col % COLS * STATE) * uint32_t(sizeof(S)) : NOWHERE; }
-    static __device__ uint32_t step_at(int col, int vp) { return col < vp ? (col / COLS * BLOCK + COLS * STATE + col % COLS * STEP) * uint32_t(sizeof(S)) : NOWHERE; }
+    static __device__ uint32_t step_at(int col, int vp) { return col < vp ? (col / COLS * BLOCK + col % COLS * STEP) * uint32_t(sizeof(S)) + wide_of<S> * STATES : NOWHERE; }
 };
-// An operand's first part, eight places of a column, to `at`, in bytes
-template <typename S, int PARTS> __device__ inline void leave(const Buffer& to, uint32_t at, const Frag<S, PARTS>& f) {
+// An operand's eight places of a column to `at`, in bytes, its second part `part` behind
+template <typename S, int PARTS> __device__ inline void leave(const Buffer& to, uint32_t at, const Frag<S, PARTS>& f, int part) {
     pack<S, 8> o;
-    __builtin_memcpy(&o, &f, sizeof o);
-    to.store(o, at);
+#pragma unroll
+    for (int k = 0; k < int(sizeof f / sizeof o); k++) {
+        __builtin_memcpy(&o, reinterpret_cast<const char*>(&f) + k * sizeof o, sizeof o);
+        to.store(o, at, k * part);
+    }
 }
 inline uint64_t kept_bytes(uint64_t chunks, int32_t vp, int32_t dk, bool half) {
-    const uint64_t pad = half ? 8 : 4, bytes = half ? 2 : 4;
-    return chunks * vp * ((dk + pad + C + pad) * bytes + 12);
+    const uint64_t pad = half ? 8 : 4;
+    return chunks * vp * ((dk + pad + C + pad) * 4 + 12);      // (two parts of two bytes, or one of four)
 }
 
 // A lane's sixteen elements of a column of values: rows 16 it + 4 g + r. On their way each has a register of its own: two of 16 bits

@@ -338,7 +338,7 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
         for (int kb = 0; kb < KB; kb++) {
             sf[kb] = frag_of<St, WIDE>(s[2 * kb], s[2 * kb + 1], ss.up);
-            if constexpr (KEEP) leave(blocks, state_at + 32 * kb * sizeof(St), sf[kb]);
+            if constexpr (KEEP) leave(blocks, state_at + 32 * kb * sizeof(St), sf[kb], Ke::STATES);
         }
         fence();
         if constexpr (!MAP) {
@@ -388,7 +388,7 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         for (int kb = 0; kb < 2; kb++) {
             uf[kb] = frag_of<St, WIDE>(u[2 * kb], u[2 * kb + 1], up);
             lf[kb] = frag_of<St, WIDE>(u[2 * kb], u[2 * kb + 1], four(st.l, 2 * kb) * (LONG<St> * up), four(st.l, 2 * kb + 1) * (LONG<St> * up));
-            if constexpr (KEEP) leave(blocks, step_at + 32 * kb * sizeof(St), uf[kb]);
+            if constexpr (KEEP) leave(blocks, step_at + 32 * kb * sizeof(St), uf[kb], Ke::STEPS);
         }
         if constexpr (KEEP) {
             const Buffer scales(kept.scales + 3 * at, 3 * int64_t(S.vp) * 4);

@@ -109,7 +109,7 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
         for (int kb = 0; kb < KB; kb++) {
             sf[kb] = frag_of<St, WIDE>(s[2 * kb], s[2 * kb + 1], ss.up);
-            if constexpr (!MAP) leave(blocks, state_at + 32 * kb * sizeof(St), sf[kb]);
+            if constexpr (!MAP) leave(blocks, state_at + 32 * kb * sizeof(St), sf[kb], Ke::STATES);
         }
         // dU = l K dS + P^T dO
         const float dp = os.down * (1.0f / SQUARE<St>);
@@ -165,7 +165,7 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         Frag<St, WIDE> xf[2], yf[2];
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
-            if constexpr (!MAP) leave(blocks, step_at + 32 * kb * sizeof(St), frag_of<St, 1>(d[2 * kb], d[2 * kb + 1], sizeof(St) == 2 ? du * ds.up : 1.0f));
+            if constexpr (!MAP) leave(blocks, step_at + 32 * kb * sizeof(St), frag_of<St, WIDE>(d[2 * kb], d[2 * kb + 1], sizeof(St) == 2 ? du * ds.up : 1.0f), Ke::STEPS);
             xf[kb] = frag_of<St, WIDE>(x[2 * kb], x[2 * kb + 1], xs.up);
             yf[kb] = frag_of<St, WIDE>(y[2 * kb], y[2 * kb + 1], xs.up);
         }
@@ -219,6 +219,18 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 
 constexpr int BANDS = 4, HALVES = 2, MANY = BANDS * HALVES * WAVE, PRODUCTS = 5;
 
+// x at place `at` of a tile's row, in parts
+template <typename T> __device__ inline void put_parts(const T& tile, int row, int at, float x) {
+    using S = typename T::S;
+    if constexpr (sizeof(S) == 2) asm("" : "+v"(x));       // (as in frag_of)
+    S* to = tile.p + row * T::ROW + at;
+#pragma unroll
+    for (int w = 0; w < T::SIZE / T::PLANE; w++) {
+        to[w * T::PLANE] = S(x);
+        x -= float(S(x));
+    }
+}
+
 __device__ inline int exponent(float x) { return int(__float_as_uint(x) >> 23) - 127; }
 
 template <typename E, int DK>
@@ -230,12 +242,12 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
     using Ke = Kept<St, DK>;
     using Re = Record<St>;
     constexpr bool HALF = sizeof(St) == 2;
-    constexpr int ND = DK / 16 / HALVES, KB = DK / 32, WAVES = MANY / WAVE, UNIT = 16 / int(sizeof(St));
+    constexpr int WIDE = wide_of<St>, ND = DK / 16 / HALVES, KB = DK / 32, WAVES = MANY / WAVE, UNIT = 16 / int(sizeof(St));
     using In = Tile<St, C, DK>;
     using Ot = Tile<St, C, COLS>;
-    using Sv = Tile<St, COLS, DK>;
-    using Uv = Tile<St, COLS, C>;
-    using Square = Tile<St, C, C>;
+    using Sv = Tile<St, COLS, DK, WIDE>;
+    using Uv = Tile<St, COLS, C, WIDE>;
+    using Square = Tile<St, C, C, WIDE>;
     static_assert(Sv::SIZE + Uv::SIZE == Ke::BLOCK, "blocks lie in LDS as they are kept");
     constexpr int BUFFERS = HALF ? 2 : 1, IN = IMAGE<St, DK>, BLOCK = Ke::BLOCK * int(sizeof(St)), BUFFER = 2 * BLOCK + Ot::SIZE * int(sizeof(St));
     constexpr int MORE = BUFFERS * BUFFER > 3 * Square::SIZE * int(sizeof(St)) ? BUFFERS * BUFFER : 3 * Square::SIZE * int(sizeof(St));
@@ -388,18 +400,20 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
             const Uv Us{buffer + Sv::SIZE}, Rs{buffer + Ke::BLOCK + Sv::SIZE};
             const Ot Od{buffer + 2 * Ke::BLOCK};
             const auto scaled = [&](auto f, int p) {
-                if constexpr (HALF) f.p[0] *= *reinterpret_cast<const h8*>(&factors[now][p][8 * (tid % WAVE / 16)]);
+                if constexpr (HALF) {
+                    const h8 by = *reinterpret_cast<const h8*>(&factors[now][p][8 * (tid % WAVE / 16)]);
+#pragma unroll
+                    for (auto& part : f.p) part *= by;
+                }
                 return f;
             };
             if (BUFFERS == 2 && next) fetch(v0 + COLS, now ^ 1);
+            // operands of two parts are loaded in two stages, where all at once have no room
             const auto of = Od.rows(band, 0);
-            const auto rf = Rs.cols(band, 0), uf = Us.cols(band, 0);
-            Frag<St, 1> sf[ND], gf[ND], un[2];
+            const auto rf = Rs.cols(band, 0);
+            Frag<St, WIDE> sf[ND], gf[ND], un[2];
 #pragma unroll
-            for (int n = 0; n < ND; n++) {
-                sf[n] = S0.cols(d0 + 16 * n, 0);
-                gf[n] = S1.cols(d0 + 16 * n, 0);
-            }
+            for (int n = 0; n < ND; n++) sf[n] = S0.cols(d0 + 16 * n, 0);
 #pragma unroll
             for (int k = 0; k < 2; k++) un[k] = Us.cols(16 * (half + 2 * k), 0);
             float product[2] = {0.0f, 0.0f};
@@ -407,32 +421,44 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
 #pragma unroll
             for (int k = 0; k < EACH; k++) {
                 const int p = tid + k * MANY < UNITS ? tid + k * MANY : 0, c = p / (DK / UNIT), at = c * Sv::ROW + p % (DK / UNIT) * UNIT;
-                const auto x = pack<St, UNIT>::load(S0.p + at), y = pack<St, UNIT>::load(S1.p + at);
                 float z = 0.0f;
 #pragma unroll
-                for (int e = 0; e < UNIT; e++) if constexpr (!HALF) z = fmaf(x.v[e], y.v[e], z);
-                if constexpr (HALF) {
-                    using h2 = __attribute__((ext_vector_type(2))) _Float16;
+                for (int i = WIDE - 1; i >= 0; i--)
 #pragma unroll
-                    for (int e = 0; e < UNIT; e += 2) z = __builtin_amdgcn_fdot2(h2{x.v[e], x.v[e + 1]}, h2{y.v[e], y.v[e + 1]}, z, false);
-                }
+                    for (int j = WIDE - 1; j >= 0; j--) if (i + j < WIDE) {
+                        const auto x = pack<St, UNIT>::load(S0.p + i * Sv::PLANE + at), y = pack<St, UNIT>::load(S1.p + j * Sv::PLANE + at);
+#pragma unroll
+                        for (int e = 0; e < UNIT; e++) if constexpr (!HALF) z = fmaf(x.v[e], y.v[e], z);
+                        if constexpr (HALF) {
+                            using h2 = __attribute__((ext_vector_type(2))) _Float16;
+#pragma unroll
+                            for (int e = 0; e < UNIT; e += 2) z = __builtin_amdgcn_fdot2(h2{x.v[e], x.v[e + 1]}, h2{y.v[e], y.v[e + 1]}, z, false);
+                        }
+                    }
                 if (HALF) z *= f0[v0 + c] * f1[v0 + c];
                 product[k % 2] += tid + k * MANY < UNITS ? z : 0.0f;
             }
             both += product[0] + product[1];
             fence();
-            const auto of0 = scaled(of, 0), rf1 = scaled(rf, 1), uf2 = scaled(uf, 2), of3 = scaled(of, 3), rf4 = scaled(rf, 4);
-#pragma unroll
-            for (int n = 0; n < ND; n++) {
-                mma(aq[n], of0, sf[n]);
-                mma(from[n], rf1, sf[n]);
-                mma(to[n], uf2, gf[n]);
-            }
+            const auto of0 = scaled(of, 0), of3 = scaled(of, 3);
+            const auto rf1 = scaled(rf, 1), rf4 = scaled(rf, 4);
 #pragma unroll
             for (int k = 0; k < 2; k++) {  // (those above the diagonal are not used)
                 mma(dp[k], of3, un[k]);
                 mma(da[k], rf4, un[k]);
             }
+            const auto uf = Us.cols(band, 0);
+#pragma unroll
+            for (int n = 0; n < ND; n++) gf[n] = S1.cols(d0 + 16 * n, 0);
+#pragma unroll
+            for (int n = 0; n < ND; n++) {
+                mma(aq[n], of0, sf[n]);
+                mma(from[n], rf1, sf[n]);
+            }
+            fence();
+            const auto uf2 = scaled(uf, 2);
+#pragma unroll
+            for (int n = 0; n < ND; n++) mma(to[n], uf2, gf[n]);
             if (next) {
                 if constexpr (BUFFERS == 1) {
                     __syncthreads();
@@ -515,7 +541,10 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
             float column = 0.0f;
             if (n > own) {                 // above the diagonal
 #pragma unroll
-                for (int r = 0; r < 4; r++) Ek.p[(band + 4 * grp + r) * Square::ROW + at] = Eq.p[(band + 4 * grp + r) * Square::ROW + at] = St(0.0f);
+                for (int r = 0; r < 4; r++) {
+                    put_parts(Ek, band + 4 * grp + r, at, 0.0f);
+                    put_parts(Eq, band + 4 * grp + r, at, 0.0f);
+                }
             } else {
                 const float rk = length_rest<St>(st.rk[c]), hc = st.hi[c], lc = st.lo[c];
                 f4 fk;
@@ -528,21 +557,27 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
                     const float pair = c < i ? ldexpf(e * rqi[r] * rk * qk[k][r], top[3]) + ldexpf(f * rki[r] * rk * kk[k][r], top[4]) : 0.0f;
                     rowsum[r] += pair;
                     column += pair;
-                    Ek.p[i * Square::ROW + at] = St(e * (few * FIT) * rk);
-                    Eq.p[i * Square::ROW + at] = St(e * (few * FIT) * rqi[r]);
-                    if (n < own || c <= i) Ff.p[i * Square::ROW + at] = St(f * (few * FIT) * rk);
+                    put_parts(Ek, i, at, e * (few * FIT) * rk);
+                    put_parts(Eq, i, at, e * (few * FIT) * rqi[r]);
+                    if (n < own || c <= i) put_parts(Ff, i, at, f * (few * FIT) * rk);
                     fk[r] = f * (few * FIT) * rki[r];
                 }
                 if (n < own) {             // the four steps' places are neighbours
                     pack<St, 4> x;
 #pragma unroll
-                    for (int r = 0; r < 4; r++) x.v[r] = St(fk[r]);
-                    x.store(Ff.p + c * Square::ROW + place(band + 4 * grp));
+                    for (int w = 0; w < WIDE; w++) {
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            x.v[r] = St(fk[r]);
+                            fk[r] -= float(x.v[r]);
+                        }
+                        x.store(Ff.p + w * Square::PLANE + c * Square::ROW + place(band + 4 * grp));
+                    }
                 } else {
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         const int i = band + 4 * grp + r;
-                        if (c < i) Ff.p[c * Square::ROW + place(i)] = St(fk[r]);
+                        if (c < i) put_parts(Ff, c, place(i), fk[r]);
                         if (c == i) writes[i] = ldexpf(da[k][r], top[4]);
                     }
                 }
@@ -558,7 +593,7 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
         __syncthreads();
         constexpr int OUT = HALF ? 15 - 6 : 0;             // (what FIT took out)
         static_assert(!HALF || LONG<St> == 64.0f, "the exponent of LONG");
-        Frag<St, 1> ek[2], eq[2], ff[2];
+        Frag<St, WIDE> ek[2], eq[2], ff[2];
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
             ek[kb] = Ek.rows(band, kb);

@@ -29,3 +29,18 @@ def test_outputs(dtype, B, T, H, G, K, V):
     a, _, _ = made(B, T, H, G, K, V, dtype, seed=T)
     with torch.no_grad():
         flips("out", ops.gated_delta(**a)[0], delta(**wide(a))[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B, T, H, G, K, V", SHAPES)
+def test_gradients(dtype, B, T, H, G, K, V):
+    """A gradient's chain of sums is twice an output's."""
+    a, d_out, d_last = made(B, T, H, G, K, V, dtype, seed=T)
+    ref = wide(a)
+    leaves = {k: ref[k].requires_grad_() for k in NAMES}
+    want = torch.autograd.grad(delta(**ref), list(leaves.values()), (d_out.double().cpu(), d_last.double().cpu()))
+    own = a | {k: a[k].detach().requires_grad_() for k in NAMES}
+    have = torch.autograd.grad(ops.gated_delta(**own), [own[k] for k in NAMES], (d_out, d_last))
+    for name, h, w in zip(NAMES, have, want):
+        if name != "state":
+            flips("d_" + name, h, w, 2.0)
