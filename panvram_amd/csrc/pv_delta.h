@@ -12,7 +12,7 @@
 // falls below float16's numbers is 2^-37 of that. A product's scale is a number of the lane, as a lane has one column. What is computed
 // is `wide`: two float16, a value and what its rounding left, 22 bits. (Two bfloat16, without any scale, left states off by 4e-6
 // and outputs in bfloat16 by 1.7 times their own rounding; the first part alone, 11 bits, left outputs and gradients in bfloat16 0.0011 off from
-// the exact ones rounded, by flips to a neighbour, where both leave 0.00001 to 0.00005.) Gradients in float16 have the operands of float32. Of tensors in
+// the exact ones rounded, by flips to a neighbour, where both leave 0.00001 to 0.00005.) Of tensors in
 // float32 the operands are float32, eight products of 16 x 16 x 4 in the place of one of 32, and scales are 1.
 #pragma once
 #include "pv_ops.h"
@@ -29,10 +29,10 @@ constexpr int MAX_K = 128, MAX_STEP = 1 << 22;
 using f4 = __attribute__((ext_vector_type(4))) float;
 using h8 = __attribute__((ext_vector_type(8))) _Float16;
 
-// What operands are held as for tensors of E (KEPT: where gradients are made from them); how many of those a wide one takes; lengths of
-// keys and queries, and the scale of the matrices of 64 x 64, whose elements are 1 at most
-template <typename E, bool KEPT> using Rep = std::conditional_t<std::is_same_v<E, bf16> || (std::is_same_v<E, f16> && !KEPT), f16, float>;
-inline bool in_16_bits(int32_t dtype, bool kept) { return dtype == PV_BF16 || (dtype == PV_F16 && !kept); }
+// What operands are held as for tensors of E; how many of those a wide one takes; lengths of keys and queries, and the scale of the
+// matrices of 64 x 64, whose elements are 1 at most
+template <typename E> using Rep = std::conditional_t<sizeof(E) == 2, f16, float>;
+inline bool in_16_bits(int32_t dtype) { return dtype != PV_F32; }
 template <typename S> constexpr int wide_of = sizeof(S) == 2 ? 2 : 1;
 template <typename S> constexpr float LONG = sizeof(S) == 2 ? 64.0f : 1.0f;
 template <typename S> constexpr float SQUARE = sizeof(S) == 2 ? 4096.0f : 1.0f;

@@ -72,9 +72,10 @@ template <typename S> __device__ inline void record(const float* m, int row, S (
     }
 }
 
-template <typename E, typename St, int DK>
+template <typename E, int DK>
 __global__ __launch_bounds__(BLOCK, 4) void chunk_kernel(const E* __restrict__ query, const E* __restrict__ key, const E* __restrict__ gate, const E* __restrict__ write,
                                                       const uint8_t* __restrict__ reset, Shape S, char* __restrict__ records, char* __restrict__ images) {
+    using St = Rep<E>;
     using In = Tile<St, C, DK>;
     using In8 = Rows<E, St, DK, BLOCK>;
     constexpr int ROW = C + 4, MATRIX = C * ROW * 4, KEYS = 2 * In::SIZE * int(sizeof(St));
@@ -243,10 +244,11 @@ __global__ __launch_bounds__(BLOCK, 4) void chunk_kernel(const E* __restrict__ q
 // has taken all it asks for, 3 us a chunk.)
 
 // MAP: the first walk of a sequence in pieces; there are no outputs, and DK columns more that begin as those of one.
-template <typename E, typename St, int DK, int W, bool KEEP, bool MAP>
+template <typename E, int DK, int W, bool KEEP, bool MAP>
 __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))) void state_kernel(
     const E* __restrict__ value, const float* __restrict__ state, Shape S, const char* __restrict__ records, const char* __restrict__ images, E* __restrict__ out,
-    float* __restrict__ last, Kept<St, DK> kept, Pieces pieces, Joins joins) {
+    float* __restrict__ last, Kept<Rep<E>, DK> kept, Pieces pieces, Joins joins) {
+    using St = Rep<E>;
     using Ke = Kept<St, DK>;
     constexpr int WIDE = wide_of<St>, ND = DK / 16, KB = DK / 32;
     using In = Tile<St, C, DK>;
@@ -559,19 +561,20 @@ namespace {
 // 17.5 for eight, in chunks 21.7 for nine and 22.1 for sixty-four; 512 heads 16.2, 53, 79 and 82.
 constexpr int SHORT = 8;
 
-template <typename E, typename St, int DK>
+template <typename E, int DK>
 int32_t forward(const void* query, const void* key, const void* value, const void* gate, const void* write, const float* state, const uint8_t* reset, const Shape& S,
                 void* out, float* last, void* kept, void* work, hipStream_t stream, char* err, size_t errcap) {
+    using St = Rep<E>;
     const auto in = [](const void* p) { return static_cast<const E*>(p); };
     const int64_t heads = S.B * S.G;
     char *records = static_cast<char*>(work), *images = records + heads * S.chunks * Record<St>::STRIDE;
-    chunk_kernel<E, St, DK><<<dim3(heads * S.chunks), BLOCK, 0, stream>>>(in(query), in(key), in(gate), in(write), reset, S, records, images);
+    chunk_kernel<E, DK><<<dim3(heads * S.chunks), BLOCK, 0, stream>>>(in(query), in(key), in(gate), in(write), reset, S, records, images);
     const Kept<St, DK> to(kept, S);
     const Pieces pieces = pieces_of(heads, S.chunks, S.vp, DK);
     const Joins joins(images + S.B * S.H * S.chunks * IMAGE<St, DK>, heads, pieces.count, S.vp, DK);
     if (pieces.count > 1) {
         constexpr int W = 4;
-        state_kernel<E, St, DK, W, false, true><<<dim3(heads * pieces.count * (((S.vp + DK) / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(
+        state_kernel<E, DK, W, false, true><<<dim3(heads * pieces.count * (((S.vp + DK) / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(
             in(value), nullptr, S, records, images, nullptr, nullptr, to, pieces, joins);
         join_kernel<DK, false><<<dim3(heads * (S.vp / 16)), (JOIN_WAVES + 1) * WAVE, 0, stream>>>(state, S, pieces.count, joins, joins);
     }
@@ -579,11 +582,11 @@ int32_t forward(const void* query, const void* key, const void* value, const voi
         constexpr int W = decltype(w)::value;
         const dim3 grid(heads * pieces.count * ((S.vp / 16 + W - 1) / W));
         const auto walk = [&](auto keep) {
-            state_kernel<E, St, DK, W, decltype(keep)::value, false><<<grid, (W + 1) * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to,
+            state_kernel<E, DK, W, decltype(keep)::value, false><<<grid, (W + 1) * WAVE, 0, stream>>>(in(value), state, S, records, images, static_cast<E*>(out), last, to,
                                                                                                       pieces, joins);
         };
-        if constexpr (std::is_same_v<St, Rep<E, true>>) if (kept) walk(std::true_type{});
-        if constexpr (std::is_same_v<St, Rep<E, false>>) if (!kept) walk(std::false_type{});
+        if (kept) walk(std::true_type{});
+        else walk(std::false_type{});
         return launched(err, errcap);
     });
 }
@@ -597,14 +600,14 @@ uint64_t pv_gated_delta_work_bytes(int64_t B, int64_t T, int32_t H, int32_t G, i
     const int64_t chunks = (T + C - 1) / C, heads = B * G;
     const int32_t vp = (V + 31) / 32 * 32, dk = columns_of(K);
     const Pieces pieces = pieces_of(heads, chunks, vp, dk);
-    const bool half = in_16_bits(dtype, keep);
+    const bool half = in_16_bits(dtype);
     return uint64_t(B) * chunks * (uint64_t(G) * (half ? Record<f16>::STRIDE : Record<float>::STRIDE) + uint64_t(H) * image_bytes(dk, half)) +
            (pieces.count > 1 ? Joins::bytes(heads, pieces.count, vp, dk) : 0);
 }
 
 uint64_t pv_gated_delta_kept_bytes(int64_t B, int64_t T, int32_t G, int32_t K, int32_t V, int32_t dtype) {
     if (B < 1 || G < 1 || T < 1 || K < 1 || V < 1) return 0;
-    return kept_bytes(uint64_t(B) * uint64_t(G) * uint64_t((T + C - 1) / C), (V + 31) / 32 * 32, columns_of(K), in_16_bits(dtype, true));
+    return kept_bytes(uint64_t(B) * uint64_t(G) * uint64_t((T + C - 1) / C), (V + 31) / 32 * 32, columns_of(K), in_16_bits(dtype));
 }
 
 uint64_t pv_gated_delta_backward_work_bytes(int64_t B, int64_t T, int32_t G, int32_t K, int32_t V, int32_t dtype) {
@@ -633,10 +636,7 @@ int32_t pv_gated_delta_hip(const void* query, const void* key, const void* value
             return launched(err, errcap);
         }
         return with_k(K, [&](auto k) {
-            const auto run = [&](auto st) {
-                return forward<E, decltype(st), decltype(k)::value>(query, key, value, gate, write, state, reset, S, out, last, kept, work, hipStream_t(stream), err, errcap);
-            };
-            return kept ? run(Rep<E, true>{}) : run(Rep<E, false>{});
+            return forward<E, decltype(k)::value>(query, key, value, gate, write, state, reset, S, out, last, kept, work, hipStream_t(stream), err, errcap);
         });
     });
 }

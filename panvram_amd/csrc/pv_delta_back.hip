@@ -27,8 +27,8 @@ namespace {
 template <typename E, int DK, int W, bool MAP>
 __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(1, 2))) void walk_kernel(
     const E* __restrict__ d_out, const float* __restrict__ d_last, Shape S, const char* __restrict__ records, const char* __restrict__ images, E* __restrict__ d_value,
-    float* __restrict__ d_state, Kept<Rep<E, true>, DK> walked, Pieces pieces, Joins joins) {
-    using St = Rep<E, true>;
+    float* __restrict__ d_state, Kept<Rep<E>, DK> walked, Pieces pieces, Joins joins) {
+    using St = Rep<E>;
     using Ke = Kept<St, DK>;
     constexpr int WIDE = wide_of<St>, ND = DK / 16, KB = DK / 32;
     using In = Tile<St, C, DK>;
@@ -235,10 +235,10 @@ __device__ inline int exponent(float x) { return int(__float_as_uint(x) >> 23) -
 
 template <typename E, int DK>
 __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) void gradient_kernel(const E* __restrict__ gate, const E* __restrict__ write, const E* __restrict__ d_out, Shape S,
-                                                        const char* __restrict__ records, const char* __restrict__ images, const Kept<Rep<E, true>, DK> kept,
-                                                        const Kept<Rep<E, true>, DK> walked, E* __restrict__ d_query, E* __restrict__ d_key,
+                                                        const char* __restrict__ records, const char* __restrict__ images, const Kept<Rep<E>, DK> kept,
+                                                        const Kept<Rep<E>, DK> walked, E* __restrict__ d_query, E* __restrict__ d_key,
                                                         E* __restrict__ d_gate, E* __restrict__ d_write) {
-    using St = Rep<E, true>;
+    using St = Rep<E>;
     using Ke = Kept<St, DK>;
     using Re = Record<St>;
     constexpr bool HALF = sizeof(St) == 2;
@@ -689,7 +689,7 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
 template <typename E, int DK>
 int32_t backward(const void* gate, const void* write, const void* d_out, const float* d_last, const Shape& S, void* kept, const void* records, void* d_query, void* d_key,
                  void* d_value, void* d_gate, void* d_write, float* d_state, void* work, hipStream_t stream, char* err, size_t errcap) {
-    using St = Rep<E, true>;
+    using St = Rep<E>;
     const auto in = [](const void* p) { return static_cast<const E*>(p); };
     const auto out = [](void* p) { return static_cast<E*>(p); };
     const int64_t heads = S.B * S.G;

@@ -85,7 +85,7 @@ def gated_delta(query, key, value, gate, write, state=None, reset=None, eps=1e-6
     last float32 [B, G, K, V]); `last` is the next call's state, so generation calls it with T = 1. Gradients flow to query, key,
     value, gate, write and state, from out and from last.
 
-    For its gradients a call keeps, beside gate and write, some 2.9 KB a step of each head of 128 x 128 in bfloat16 (3.3 in float16 and float32):
+    For its gradients a call keeps, beside gate and write, some 2.9 KB a step of each head of 128 x 128 in 16 bits, 3.3 in float32:
     states and updates of each chunk, and what the chunks' steps do to each other. Queries, keys and values need not be kept.
 
     Calls of up to 8 steps without gradients go step by step, others in chunks of 64 by matrix products, long ones of few heads in

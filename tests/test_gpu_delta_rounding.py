@@ -44,3 +44,15 @@ def test_gradients(dtype, B, T, H, G, K, V):
     for name, h, w in zip(NAMES, have, want):
         if name != "state":
             flips("d_" + name, h, w, 2.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B, T, H, G, K, V", SHAPES)
+def test_with_and_without_gradients(dtype, B, T, H, G, K, V):
+    """Whether gradients will be asked for does not change results."""
+    a, _, _ = made(B, T, H, G, K, V, dtype, seed=T)
+    with torch.no_grad():
+        want = ops.gated_delta(**a)
+    a["value"].requires_grad_()
+    got = ops.gated_delta(**a)
+    assert got[0].requires_grad and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
