@@ -409,8 +409,7 @@ int32_t pv_add_rms_norm_backward_hip(const void* s, const float* rstd, const flo
  * query, key: [B, T, H, K], value: [B, T, G, V], gate, write: [B, T, G], all of `dtype`; G is a multiple of H, and value head g
  * goes with query and key head g / (G / H). strides: host array of 15, in elements: of a sequence, a step and a head of query, key,
  * value, gate, write in turn; a step's at most 2^22. B, T, H >= 1, K <= 128, V <= 65,536, H K and G V at
- * most 2^22; of 64 steps of a value head's sequence,
- * and of 32 columns of a state, there are fewer than 2^24. Squares of a key's or query's length are within float32.
+ * most 2^22; B G ceil(T / 64) and B G ceil(V / 32) below 2^23, T below 2^31. Squares of a key's or query's length are within float32.
  * state: f32[B, G, K, V] before step 0, or NULL: zero. reset: u8[B, T], or NULL; where not 0, S[t-1] is dropped. out: [B, T, G, V] of
  * `dtype`; last: f32[B, G, K, V] = S[T-1], apart from state. For the backward pass: kept (pv_gated_delta_kept_bytes, 16-byte
  * aligned; NULL: none) and what the call leaves in `work`. work: pv_gated_delta_work_bytes with keep = 1 if kept is given, else 0. */

@@ -91,6 +91,8 @@ def gated_delta(query, key, value, gate, write, state=None, reset=None, eps=1e-6
     For its gradients a call keeps, beside gate and write, some 2.9 KB a step of each head of 128 x 128 in 16 bits, 3.3 in float32:
     states and updates of each chunk, and what the chunks' steps do to each other. Queries, keys and values need not be kept.
 
+    B G ceil(T / 64) and B G ceil(V / 32), the chunks and the columns' groups of a call, are below 2^23, H K and G V at most 2^22.
+
     Calls of up to 8 steps without gradients go step by step, others in chunks of 64 by matrix products, long ones of few heads in
     pieces: the same up to roundings, and equal from run to run, not from one of these ways to another. In chunks a NaN or an infinity in one step's inputs reaches the
     outputs of all steps of its chunk, and through the state those of its head after it; a state that is not finite is dropped by a
