@@ -310,6 +310,7 @@ template <typename E, typename S, int DK, int THREADS> struct Rows {
                 for (int e = 0; e < 8; e++) v[j].v[e] = from.load<E>(e < K ? off + e * uint32_t(sizeof(E)) : NOWHERE, j * STEP * stride * int(sizeof(E)));
         }
     }
+    __device__ void drop(int j, bool on) { if (on) v[j].bits = typename pack<E, 8>::raw{}; }
     __device__ float square(int j, int K) const {          // of the lane's own elements, none of them a neighbour's too
         const int own = K - int(threadIdx.x % PER * 8);
         float s = 0.0f;
@@ -358,10 +359,11 @@ struct Shape {
 //   l     l r: l what is left of a step's addition at the chunk's end
 //   q     g r of the query
 //   end   what the chunk keeps of the state;  cut: a bit for each step that drops the state before it
+//   odd   a bit for each step whose key, gate or write is not finite, odd_query: whose query is not
 struct Steps {
     float x[C], b[C], l[C], q[C], rk[C], rq[C], hi[C], lo[C];      // hi + lo: the logarithm of what is kept, summed up from the chunk's first step
     float end;
-    uint32_t cut[2], unused;
+    uint32_t cut[2], odd[2], odd_query[2], unused;
 };
 
 // What one kernel leaves another lies in memory as it will lie in LDS, padding and all, and is copied there past the registers:
@@ -400,6 +402,48 @@ template <int N> __device__ inline void arrived() { asm volatile("s_waitcnt vmcn
 __device__ inline int since(uint64_t cut, int i) {         // the last step up to i that drops the state, or -1
     const uint64_t m = cut & (~0ull >> (63 - i));
     return m ? 63 - __builtin_clzll(m) : -1;
+}
+
+// Steps that are not finite. The sums over a chunk's steps reach past them, where factors are 0, and 0 times NaN is NaN: so a key, query,
+// gate, value or gradient of out that is not finite counts as 0 in them, and as a NaN where the recurrence takes it: forwards in the
+// steps from it up to the next that drops the state, backwards in those before it down to one that drops the state.
+__device__ inline bool reached(uint64_t odd, uint64_t cut, int i) {
+    const int from = since(cut, i);
+    return odd & (~0ull >> (63 - i)) & (~0ull << (from < 0 ? 0 : from));
+}
+__device__ inline bool reached_back(uint64_t odd, uint64_t cut, int i) {
+    const uint64_t later = i < 63 ? cut >> (i + 1) << (i + 1) : 0;
+    return odd & (~0ull << i) & (later ? (later & -later) - 1 : ~0ull);
+}
+// A bit for each step whose element in the lane's column is not finite, which is 0 from here on. All lanes of the wave take part.
+__device__ inline uint64_t taken_out(f4 (&v)[4]) {
+    uint64_t odd = 0;
+#pragma unroll
+    for (int it = 0; it < 4; it++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const bool on = !(fabsf(v[it][r]) < INFINITY);
+            odd |= uint64_t(on) << (16 * it + r);
+            v[it][r] = on ? 0.0f : v[it][r];
+        }
+    odd <<= thread() % WAVE / 16 * 4;
+    odd |= __shfl_xor(odd, 16, WAVE);
+    return odd | __shfl_xor(odd, 32, WAVE);
+}
+// Whether any of a lane's numbers is not finite: 0 if none
+template <int N> __device__ inline float not_finite(const f4 (&v)[N]) {
+    float x = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) x = fmaf(0.0f, v[n][r], x);
+    return x == 0.0f ? 0.0f : 1.0f;
+}
+// NaN over what leave() has left at `at` (nearer below): over those of the operand's places, steps first .. first + 3 and first + 16 .. first + 19, that
+// f holds for. (A wave's stores to one address arrive in their order.)
+template <typename S, typename B, typename F> __device__ inline void spoil(const B& to, uint32_t at, int first, F&& f) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) to.template store<S>(S(NAN), f(first + j % 4 + j / 4 * 16) ? at + j * uint32_t(sizeof(S)) : 0x80000000u);
 }
 
 // What the forward pass keeps for the backward pass, and what the walk backwards leaves for the gradients: arrays of the same

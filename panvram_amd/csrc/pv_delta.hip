@@ -91,14 +91,15 @@ __global__ __launch_bounds__(BLOCK, 4) void chunk_kernel(const E* __restrict__ q
     In8 q, k;
     q.load(query + b * S.qb + t0 * S.qt + h * S.qh, S.qt, rows, S.K);
     k.load(key + b * S.kb + t0 * S.kt + h * S.kh, S.kt, rows, S.K);
+    bool odd = false;                      // gate or write is not a number
     if (wave == 0) {                       // a lane for each step: gates, and their logarithms summed up
         const int64_t t = t0 + (l < rows ? l : rows - 1);
         const float x = float(gate[b * S.ab + t * S.at + g * S.ag]), w = float(write[b * S.wb + t * S.wt + g * S.wg]);
         float la = -(fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))));
-        if (x != x) la = x;
         const bool cut = l < rows && (la < -104.0f || (reset && reset[b * S.T + t]));      // (exp(-104) is 0 in 32 bits)
         const uint64_t cuts = __ballot(cut);
-        double c = l < rows && !cut ? double(la) : 0.0;
+        odd = l < rows && ((x != x && !cut) || w != w);
+        double c = l < rows && !cut && !odd ? double(la) : 0.0;
 #pragma unroll
         for (int d = 1; d < WAVE; d <<= 1) {
             const double o = __shfl_up(c, d, WAVE);
@@ -106,7 +107,7 @@ __global__ __launch_bounds__(BLOCK, 4) void chunk_kernel(const E* __restrict__ q
         }
         const double last = __shfl(c, C - 1, WAVE);
         const float hi = float(c);
-        st.b[l] = l < rows ? 1.0f / (1.0f + expf(-w)) : 0.0f;
+        st.b[l] = l < rows && !odd ? 1.0f / (1.0f + expf(-w)) : 0.0f;
         st.hi[l] = hi;
         st.lo[l] = float(c - double(hi));
         st.x[l] = cuts & (~0ull >> (63 - l)) ? 0.0f : expf(hi);     // (times the lengths below)
@@ -124,11 +125,14 @@ __global__ __launch_bounds__(BLOCK, 4) void chunk_kernel(const E* __restrict__ q
 #pragma unroll
         for (int d = In8::PER / 2; d; d >>= 1) { sq += __shfl_xor(sq, d, WAVE); sk += __shfl_xor(sk, d, WAVE); }
         const float rq = i < rows ? 1.0f / sqrtf(sq + S.eps) : 0.0f, rk = i < rows ? 1.0f / sqrtf(sk + S.eps) : 0.0f;
-        q.put(Qt, j, length_up<St>(rq), S.K);
-        k.put(Kt, j, length_up<St>(rk), S.K);
+        const bool on_q = sq < INFINITY && rq < INFINITY, on_k = sk < INFINITY && rk < INFINITY;
+        q.drop(j, !on_q);
+        k.drop(j, !on_k);
+        q.put(Qt, j, on_q ? length_up<St>(rq) : 0.0f, S.K);
+        k.put(Kt, j, on_k ? length_up<St>(rk) : 0.0f, S.K);
         if (tid % In8::PER == 0) {
-            st.rq[i] = rq;
-            st.rk[i] = rk;
+            st.rq[i] = on_q || i >= rows ? rq : NAN;
+            st.rk[i] = on_k || i >= rows ? rk : NAN;
         }
     }
     __syncthreads();
@@ -152,6 +156,16 @@ __global__ __launch_bounds__(BLOCK, 4) void chunk_kernel(const E* __restrict__ q
     }
     const uint64_t cuts = uint64_t(st.cut[1]) << 32 | st.cut[0];
     const float shift = tid < C ? st.x[tid] : 0.0f;
+    if (wave == 0) {
+        const float rk = st.rk[l], rq = st.rq[l];
+        const uint64_t odds = __ballot(odd || rk != rk), queries = __ballot(rq != rq);
+        if (rk != rk) st.rk[l] = st.b[l] = 0.0f;
+        if (rq != rq) st.rq[l] = 0.0f;
+        if (l < 2) {
+            st.odd[l] = uint32_t(odds >> (32 * l));
+            st.odd_query[l] = uint32_t(queries >> (32 * l));
+        }
+    }
     __syncthreads();
     if (tid < C) {
         st.x[tid] = st.b[tid] * (shift * length_rest<St>(st.rk[tid]));
@@ -310,15 +324,13 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
         for (int it = 0; it < 4; it++) v[it] = vp.four(it);
         any |= cuts;
+        uint64_t odd = uint64_t(st.odd[1]) << 32 | st.odd[0];
+        const bool some = __builtin_amdgcn_readfirstlane(st.odd[0] | st.odd[1] | st.odd_query[0] | st.odd_query[1]) || __any(not_finite(v) != 0.0f);
+        if (some) odd |= taken_out(v);
         bool lost = false;                 // the state before a chunk in which some step drops it is not finite
         by_cut(cuts, [&](auto cut) {
             if constexpr (decltype(cut)::value) {      // (zero times it would reach the steps that it is dropped at: it is zero, and the steps before are NaN)
-                float x = 0.0f;
-#pragma unroll
-                for (int k = 0; k < ND; k++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) x = fmaf(0.0f, s[k][r], x);
-                lost = over_column(x == 0.0f ? 0.0f : 1.0f) != 0.0f;
+                lost = over_column(not_finite(s)) != 0.0f;
 #pragma unroll
                 for (int k = 0; k < ND; k++)
 #pragma unroll
@@ -432,6 +444,29 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
                 for (int r = 0; r < 4; r++) if (CUT && lost && 16 * it + 4 * grp + r < __builtin_ctzll(cuts)) y[it][r] = NAN;
             }
         });
+        if (some) {
+            const int first = thread() % WAVE / 16 * 4;
+            if (reached(odd, cuts, C - 1))
+#pragma unroll
+                for (int k = 0; k < ND; k++) s[k] = f4{NAN, NAN, NAN, NAN};
+            const uint64_t queries = uint64_t(st.odd_query[1]) << 32 | st.odd_query[0];
+#pragma unroll
+            for (int it = 0; it < 4; it++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int i = 16 * it + first + r;
+                    if (reached(odd, cuts, i) || queries >> i & 1) y[it][r] = NAN;
+                }
+        }
+        if constexpr (KEEP) if (some || __any(lost)) {     // (the gradients take from these what is NaN; their own products are by steps and heads)
+            const int first = thread() % WAVE / 16 * 4;
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+                spoil<St>(blocks, step_at + 32 * kb * sizeof(St), 32 * kb + first, [&](int i) { return reached(odd, cuts, i) || (lost && i < __builtin_ctzll(cuts)); });
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++)
+                spoil<St>(blocks, state_at + 32 * kb * sizeof(St), 0, [&](int) { return lost; });
+        }
         if constexpr (MAP) continue;
         const Buffer to = rows_at(out + ((b * S.T + n * C) * S.G + g) * S.V, ot, rows_of(n), S.V);
 #pragma unroll

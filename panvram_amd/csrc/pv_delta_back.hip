@@ -88,6 +88,19 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         f4 o[4];
 #pragma unroll
         for (int it = 0; it < 4; it++) o[it] = op.four(it);
+        uint64_t odd = uint64_t(st.odd[1] | st.odd_query[1]) << 32 | st.odd[0] | st.odd_query[0];
+        const bool some = __builtin_amdgcn_readfirstlane(uint32_t(odd >> 32) | uint32_t(odd)) || __any(not_finite(o) != 0.0f);
+        if (some) odd |= taken_out(o);
+        bool lost = false;                 // the gradient after a chunk in which some step drops the state is not finite
+        by_cut(cuts, [&](auto cut) {
+            if constexpr (decltype(cut)::value) {
+                lost = over_column(not_finite(s)) != 0.0f;
+#pragma unroll
+                for (int k = 0; k < ND; k++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) s[k][r] = lost ? 0.0f : s[k][r];
+            }
+        });
         if (n > first) op.load(rows_at(o0 + (n - 1) * C * S.ot, S.ot, rows_of(n - 1), S.V), S.ot, out_at);
         const int64_t at = (bg * S.chunks + n) * S.vp;     // of the chunk in what is left over
         const Buffer blocks(walked.blocks + at / COLS * Ke::BLOCK, int64_t(S.vp / COLS) * Ke::BLOCK * int(sizeof(St)));
@@ -191,6 +204,23 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
                 for (int r = 0; r < 4; r++) s[k][r] = fmaf(xs.down, z[k][r], part_of_it<decltype(cut)::value>(end, s[k][r]));
         });
+        if (some || __any(lost)) {         // (the gradients take from what is left which steps are NaN; their own products are by steps and heads)
+            const int first4 = thread() % WAVE / 16 * 4;
+            const auto spoils = [&](int i) { return reached_back(odd, cuts, i) || (lost && i >= since(cuts, C - 1)); };
+            if constexpr (!MAP) {
+#pragma unroll
+                for (int it = 0; it < 4; it++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) Sixteen<E>::store(to, vt, spoils(16 * it + first4 + r) ? value_at : NOWHERE, 4 * it + r, NAN);
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++) spoil<St>(blocks, step_at + 32 * kb * sizeof(St), 32 * kb + first4, spoils);
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++) spoil<St>(blocks, state_at + 32 * kb * sizeof(St), 0, [&](int) { return lost; });
+            }
+            if (odd & (cuts ? (cuts & -cuts) - 1 : ~0ull))
+#pragma unroll
+                for (int k = 0; k < ND; k++) s[k] = f4{NAN, NAN, NAN, NAN};
+        }
     }
     if constexpr (MAP) {
         if (col < S.vp) {
@@ -652,10 +682,13 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
     }
     // of the query and the key themselves: d - x^ (x^.d), over the length
     const int l = thread() % WAVE, grp = l / 16, m = l % 16;
-    const f4 rk = *reinterpret_cast<const f4*>(st.rk + band + 4 * grp), rq = *reinterpret_cast<const f4*>(st.rq + band + 4 * grp);
+    f4 rk = *reinterpret_cast<const f4*>(st.rk + band + 4 * grp), rq = *reinterpret_cast<const f4*>(st.rq + band + 4 * grp);
+    const uint64_t odd = uint64_t(st.odd[1]) << 32 | st.odd[0], queries = uint64_t(st.odd_query[1]) << 32 | st.odd_query[0];
 #pragma unroll
     for (int r = 0; r < 4; r++) {
         const int i = band + 4 * grp + r;
+        if ((odd | queries) >> i & 1) rk[r] = NAN;     // (a query that is not finite reaches its own step's key by way of the state)
+        if (queries >> i & 1) rq[r] = NAN;
         float dq = 0.0f, dk = 0.0f;
 #pragma unroll
         for (int n = 0; n < ND; n++) {

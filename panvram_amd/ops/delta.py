@@ -94,9 +94,10 @@ def gated_delta(query, key, value, gate, write, state=None, reset=None, eps=1e-6
     B G ceil(T / 64) and B G ceil(V / 32), the chunks and the columns' groups of a call, are below 2^23, H K and G V at most 2^22.
 
     Calls of up to 8 steps without gradients go step by step, others in chunks of 64 by matrix products, long ones of few heads in
-    pieces: the same up to roundings, and equal from run to run, not from one of these ways to another. In chunks a NaN or an infinity in one step's inputs reaches the
-    outputs of all steps of its chunk, and through the state those of its head after it; a state that is not finite is dropped by a
-    reset all the same. Queries and keys have squares whose sum is a float32."""
+    pieces: the same up to roundings, and equal from run to run, not from one of these ways to another. A NaN or an infinity among a
+    step's inputs reaches what it reaches in the formulas above, its own output and those after it up to the next reset, and is NaN there where
+    steps go in chunks; gradients that it reaches are NaN, and so may be those of gate at steps before it in its chunk, back to a reset. Queries
+    and keys have squares whose sum is a float32."""
     index = on_gpu("gated_delta", query, key, value, gate, write, state, reset)
     if query.dim() != 4 or query.shape != key.shape:
         raise ValueError(f"gated_delta: query and key are [B, T, H, K] alike, got {list(query.shape)} and {list(key.shape)}")
