@@ -719,6 +719,22 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
     }
 }
 
+// The same backwards. A workgroup of four waves and the one that brings has two on a SIMD, which are held to 256 registers each; with keys of
+// over 64 elements a wave backwards takes more, and spills cost more than two waves do. All of a backward pass, ms, with two and with four: 128 heads of 128 x 128,
+// 8,192 steps, bfloat16 2.85 and 2.93, float32 6.25 and 7.53; 192 heads 4.25 and 4.84; 256 heads of 64 x 64, 4,096 steps, bfloat16 1.51 and 1.48, float32 2.40
+// and 1.99.
+template <int DK, typename F> int32_t with_waves_back(const Shape& S, const Pieces& pieces, F&& f) {
+    if constexpr (DK > 64) return f(std::integral_constant<int, 2>{});
+    else return with_waves(S, pieces, f);
+}
+// And for the walk of pieces from zero, which has no columns beside those of values: two where the workgroups are no more than CUs. One
+// sequence of 32,768 steps, ms, with two and with four: 4 heads of 128 x 128 bfloat16 0.55 and 0.59, float32 1.22 and 1.59; past the CUs, 2 heads of 128 x 512
+// bfloat16 1.00 and 0.92, 8 heads of 64 x 128 float32 2.12 and 1.75.
+template <typename F> int32_t with_waves_from_zero(const Shape& S, const Pieces& pieces, F&& f) {
+    if (pieces.count * S.B * S.G * (S.vp / 32) <= 256) return f(std::integral_constant<int, 2>{});
+    return f(std::integral_constant<int, 4>{});
+}
+
 template <typename E, int DK>
 int32_t backward(const void* gate, const void* write, const void* d_out, const float* d_last, const Shape& S, void* kept, const void* records, void* d_query, void* d_key,
                  void* d_value, void* d_gate, void* d_write, float* d_state, void* work, hipStream_t stream, char* err, size_t errcap) {
@@ -732,12 +748,15 @@ int32_t backward(const void* gate, const void* write, const void* d_out, const f
     const Joins maps(const_cast<char*>(images) + S.B * S.H * S.chunks * IMAGE<St, DK>, heads, pieces.count, S.vp, DK);
     const Joins joins(walked.scales + heads * S.chunks * 3 * S.vp, heads, pieces.count, S.vp, DK);
     if (pieces.count > 1) {
-        constexpr int W = 4;
-        walk_kernel<E, DK, W, true><<<dim3(heads * pieces.count * ((S.vp / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(in(d_out), nullptr, S, rec, images, nullptr,
-                                                                                                                      nullptr, walked, pieces, joins);
+        with_waves_from_zero(S, pieces, [&](auto w) {
+            constexpr int W = decltype(w)::value;
+            walk_kernel<E, DK, W, true><<<dim3(heads * pieces.count * ((S.vp / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(in(d_out), nullptr, S, rec, images, nullptr,
+                                                                                                                          nullptr, walked, pieces, joins);
+            return 0;
+        });
         join_kernel<DK, true><<<dim3(heads * (S.vp / 16)), (JOIN_WAVES + 1) * WAVE, 0, stream>>>(d_last, S, pieces.count, joins, maps);
     }
-    with_waves(S, pieces, [&](auto w) {
+    with_waves_back<DK>(S, pieces, [&](auto w) {
         constexpr int W = decltype(w)::value;
         walk_kernel<E, DK, W, false><<<dim3(heads * pieces.count * ((S.vp / 16 + W - 1) / W)), (W + 1) * WAVE, 0, stream>>>(in(d_out), d_last, S, rec, images, out(d_value),
                                                                                                                        d_state, walked, pieces, joins);
