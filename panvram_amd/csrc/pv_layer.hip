@@ -141,7 +141,8 @@ __global__ __launch_bounds__(L::BLOCK) void layer_kernel(const E* __restrict__ x
         var = fmaxf(fmaf(sum.b, share, -off * off), 0.0f);
         if (sum.b != sum.b) var = sum.b;
     }
-    const float r = rsqrtf(var + m * (m * eps));
+    // (of elements that are all alike nothing but eps is left, which may have vanished with m)
+    const float more = m * (m * eps), r = var + more == 0.0f && eps != 0.0f ? rsqrtf(eps) / m : rsqrtf(var + more);
     if (stats && on && lane == 0) stats[n] = {0.5f * (mean / m), 0.5f * (off / m), 2.0f * (m * r)};
     each([&](const pk& h, int64_t i) {
         const auto w = take<P, false>(weight, i, D);
