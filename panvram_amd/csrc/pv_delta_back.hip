@@ -465,7 +465,7 @@ __global__ __launch_bounds__(MANY) __attribute__((amdgpu_waves_per_eu(2, 2))) vo
                             for (int e = 0; e < UNIT; e += 2) z = __builtin_amdgcn_fdot2(h2{x.v[e], x.v[e + 1]}, h2{y.v[e], y.v[e + 1]}, z, false);
                         }
                     }
-                if (HALF) z *= f0[v0 + c] * f1[v0 + c];
+                if constexpr (HALF) z = ldexpf(z, exponent(f0[v0 + c]) + exponent(f1[v0 + c]));        // (their product may be past float32 where z is 0)
                 product[k % 2] += tid + k * MANY < UNITS ? z : 0.0f;
             }
             both += product[0] + product[1];
