@@ -326,7 +326,7 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         any |= cuts;
         uint64_t odd = uint64_t(st.odd[1]) << 32 | st.odd[0];
         const bool some = __builtin_amdgcn_readfirstlane(st.odd[0] | st.odd[1] | st.odd_query[0] | st.odd_query[1]) || __any(not_finite(v) != 0.0f);
-        if (some) odd |= taken_out(v);
+        if (some) odd |= taken_out(v) & (~0ull >> (C - rows_of(n)));       // (where steps overlap, one behind the last reads an earlier one's)
         bool lost = false;                 // the state before a chunk in which some step drops it is not finite
         by_cut(cuts, [&](auto cut) {
             if constexpr (decltype(cut)::value) {      // (zero times it would reach the steps that it is dropped at: it is zero, and the steps before are NaN)

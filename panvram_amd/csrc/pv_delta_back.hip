@@ -90,7 +90,7 @@ __global__ __launch_bounds__((W + 1) * WAVE) __attribute__((amdgpu_waves_per_eu(
         for (int it = 0; it < 4; it++) o[it] = op.four(it);
         uint64_t odd = uint64_t(st.odd[1] | st.odd_query[1]) << 32 | st.odd[0] | st.odd_query[0];
         const bool some = __builtin_amdgcn_readfirstlane(uint32_t(odd >> 32) | uint32_t(odd)) || __any(not_finite(o) != 0.0f);
-        if (some) odd |= taken_out(o);
+        if (some) odd |= taken_out(o) & (~0ull >> (C - rows));
         bool lost = false;                 // the gradient after a chunk in which some step drops the state is not finite
         by_cut(cuts, [&](auto cut) {
             if constexpr (decltype(cut)::value) {

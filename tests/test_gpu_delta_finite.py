@@ -117,3 +117,23 @@ def test_gradients_of_windows(dtype, name, fill, T, at, lo, hi):
     if name in ("value", "gate", "write", "d_out"):
         for k in ("value", "gate", "write"):
             assert torch.equal(have[k][:, :, 1], want[k][:, :, 1]), k
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_steps_that_overlap(dtype):
+    """Values, and gradients of out, whose steps are windows of one run of numbers: what a step has in one column, another has in the next."""
+    T, V = 70, 24
+    a, d_out, _ = made(1, T, 1, 1, 16, V, dtype, state=False)
+    run, d_run = a["value"].flatten()[:T + V], d_out.flatten()[:T + V]
+    run[T] = d_run[T] = NAN                        # columns 1 .. V - 1 of steps T - 1 .. T - V + 1, and column 0 of none
+    a["value"], d_out = run.as_strided((1, T, 1, V), (0, 1, 0, 1)), d_run.as_strided((1, T, 1, V), (0, 1, 0, 1))
+    out, last = delta(**wide(a))
+    with torch.no_grad():
+        got = ops.gated_delta(**a)
+    same_places(got[0], out, delta_off("out", dtype), dtype)
+    same_places(got[1], last, delta_off("last", dtype), torch.float32)
+    assert torch.isfinite(got[1][..., 0]).all()
+    a["value"] = a["value"].nan_to_num()
+    leaves = {k: a[k].detach().requires_grad_() for k in NAMES[:5]}
+    (d_value,) = torch.autograd.grad(ops.gated_delta(**leaves)[0], (leaves["value"],), d_out)
+    assert torch.isfinite(d_value[..., 0]).all() and not torch.isfinite(d_value[:, :T - V + 1, :, 1:]).any()
