@@ -14,11 +14,11 @@ def _strided(t):
     """`t` with neighbouring elements in a head, and steps at most 2^22 elements apart: itself, or a copy; and its strides. (A single
     step has no stride, whatever the tensor says of it and keeps saying when it is made contiguous.)"""
     s = t.stride()
-    if t.shape[1] == 1:
-        s = (s[0], 0, *s[2:])
     if s[1] > 1 << 22 or (len(s) == 4 and s[3] != 1 and t.shape[3] != 1):
-        t = t.contiguous()
-        s = (t.stride(0), 0 if t.shape[1] == 1 else t.stride(1), t.stride(2))
+        if t.shape[1] != 1 or (len(s) == 4 and s[3] != 1):
+            t = t.contiguous()
+            s = t.stride()
+        s = (s[0], s[1] if t.shape[1] != 1 else 0, s[2])
     return t, *s[:3]
 
 
