@@ -51,13 +51,14 @@ def test_outputs(dtype, name, fill, T, at, reset):
         assert torch.equal(torch.nan_to_num(x.detach()), torch.nan_to_num(y))
 
 
-def test_several():
-    """Some of each, resets between them, in all columns and heads"""
-    a, _, _ = made(2, 300, 2, 4, 32, 40, torch.bfloat16, reset=0.04)
+@pytest.mark.parametrize("B, T, H, G, K, V", [(2, 300, 2, 4, 32, 40), (8, 130, 8, 16, 100, 70), (1, 2113, 1, 2, 128, 72)])
+def test_several(B, T, H, G, K, V):
+    """Some of each, resets between them, in all columns and heads; of few heads, many, and in pieces"""
+    a, _, _ = made(B, T, H, G, K, V, torch.bfloat16, reset=0.04)
     gen = torch.Generator(device="cuda").manual_seed(2)
     for name, fill in WHERE:
         t = a[name]
-        t[torch.rand(t.shape, generator=gen, device="cuda") < (0.004 if t.dim() == 3 else 0.0002)] = fill
+        t[torch.rand(t.shape, generator=gen, device="cuda") < (0.004 if t.dim() == 3 else 0.0064 / t.shape[3])] = fill
     out, last = delta(**wide(a))
     assert 0.1 < torch.isfinite(out).double().mean() < 0.9
     with torch.no_grad():
