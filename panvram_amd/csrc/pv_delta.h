@@ -523,9 +523,9 @@ template <typename F> int32_t with_k(int32_t K, F&& f) {
 // one, which gives the map from the state before the piece to that after it; then the maps are joined from piece to piece; then each
 // piece is walked once more, from its true start. There are as many pieces as give all CUs a workgroup in the first walk, of 8 chunks
 // at least, as a join costs what a few chunks do; the two walks of three pieces take two thirds of the time of one over the whole.
-// One sequence, heads of 128 x 128, in pieces and as one, ms: 20 heads (three pieces) of 2,048 steps 0.12 and 0.13, of 32,768 steps 1.27 and
-// 1.78, in float32 3.5 and 5.8; 24 heads (two) of 2,048 steps 0.14 and 0.13, of 32,768 steps 1.79 and 1.87; 4 heads (sixteen) of 131,072
-// steps 0.98 and 5.9.
+// One sequence, heads of 128 x 128, in pieces and as one, ms: 20 heads (three pieces) of 2,048 steps 0.11 and 0.13, of 32,768 steps 1.29 and
+// 1.92, in float32 3.5 and 5.8; 24 heads (two) of 2,048 steps 0.133 and 0.130, of 32,768 steps 1.84 and 2.00; 4 heads (sixteen) of 131,072
+// steps 1.00 and 6.7.
 struct Pieces {
     int32_t count;                         // 1: the walk is as it is
     int64_t chunks;                        // of a piece; the last one's may be fewer

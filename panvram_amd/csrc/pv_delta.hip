@@ -17,8 +17,8 @@
 // Calls of few steps walk them one by one instead (`step_kernel`), the state in registers: one read and one write of it.
 //
 // What bounds it. bfloat16, 8 sequences of 8,192 steps, 8 heads of 128 x 128: chunk_kernel 222 us (8,192 chunks, 7 us each on a CU that has four
-// at once: chains of small products), state_kernel 492 (128 chunks in a row, 3.8 us each: one wave a SIMD, half of its time in vector
-// operations between products). In float32 a chunk takes it 7 us: eight products of a quarter of the rate, no second buffer. step_kernel
+// at once: chains of small products), state_kernel 457 (128 chunks in a row, 3.6 us each: one wave a SIMD, half of its time in vector
+// operations between products), and 628 with the 104 KB a chunk that it keeps for gradients. In float32 a chunk takes it 7 us and more: eight products of a quarter of the rate, no second buffer. step_kernel
 // reads and writes 512 states of 128 x 128 in 16 us, 4.2 TB/s (18 before a step's inputs were asked for ahead of the state).
 #include "pv_delta.h"
 
@@ -593,7 +593,7 @@ __global__ __launch_bounds__(BLOCK) void step_kernel(const E* __restrict__ query
 namespace {
 
 // Calls of so few steps walk them one by one, where nothing is kept for gradients. Heads of 128 x 128, us: 4 heads 5.3 for one step and
-// 17.5 for eight, in chunks 21.7 for nine and 22.1 for sixty-four; 512 heads 16.2, 53, 79 and 82.
+// 18.4 for eight, in chunks 21.0 for nine and 21.3 for sixty-four; 512 heads 16.0, 53.6, 56.1 and 59.1.
 constexpr int SHORT = 8;
 
 template <typename E, int DK>

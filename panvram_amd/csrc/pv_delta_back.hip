@@ -12,9 +12,9 @@
 // their sums' rounding, and otherwise sums without a difference in them. The heads that share a query and key are taken one
 // after another by one workgroup, so that their gradients are summed up in a fixed order.
 //
-// What bounds it. bfloat16, 8 sequences of 8,192 steps, 8 heads of 128 x 128: walk_kernel 516 us, as state_kernel; gradient_kernel 645, 42,000 cycles
-// a chunk on a CU that has room for one (104 KB of LDS, 256 registers a lane): some 29,000 of them issue vector operations, the rest are waits
-// for the first block, LDS and barriers.
+// What bounds it. bfloat16, 8 sequences of 8,192 steps, 8 heads of 128 x 128: walk_kernel 653 us, as state_kernel; gradient_kernel 816, 57,000 cycles
+// a chunk on a CU that has room for one (155 KB of LDS, 256 registers a lane): 21,000 of them issue vector operations on each SIMD, 7,400 its matrix unit is
+// busy, the rest are waits for the first block, LDS and barriers.
 #include "pv_delta.h"
 
 using namespace pvd;
