@@ -377,6 +377,7 @@ template <typename S> struct Record {
     static constexpr int INVERSE = 2080 + wide_of<S> * C * (C + PAD) * int(sizeof(S));          // without M q k^T
     static constexpr int STRIDE = (ALL + 1023) / 1024 * 1024;
 };
+static_assert(sizeof(Record<f16>) == Record<f16>::ALL && sizeof(Record<float>) == Record<float>::ALL, "copied as they are");
 template <typename S, int DK> constexpr int IMAGE = (2 * Tile<S, C, DK>::SIZE * int(sizeof(S)) + 1023) / 1024 * 1024;
 inline uint64_t image_bytes(int32_t dk, bool half) { return (2 * 64 * (half ? (dk + 8) * 2 : (dk + 4) * 4) + 1023) / 1024 * 1024; }
 template <typename S> __device__ __host__ inline char* record_of(char* work, int64_t chunk) { return work + chunk * Record<S>::STRIDE; }
